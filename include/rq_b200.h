@@ -58,7 +58,7 @@ extern "C" {
 #define RQ_W_INT8_ROW 4     /* int8 per output row (per_channel=True) */
 
 /* ------------------------------------------------------------ utilities */
-RQ_API int rq_abi_version(void);                 /* bumps on any ABI change */
+RQ_API int rq_abi_version(void);                 /* bumps when an existing entry point changes */
 RQ_API const char* rq_status_string(int status);
 /* cudaError_t of the last RQ_ERR_CUDA in this thread, or 10000 + the CUresult
  * when a driver call (tensor-map encoding) failed */
@@ -307,6 +307,110 @@ RQ_API int rq_linear_forward_gather(int wfmt, const void* qweight, const void* s
                       const void* bias, int bias_dtype,
                       const void* lora_a, const void* lora_b, int r, float scaling,
                       const RqGather* gather, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------ adapters of many requests at once */
+
+/* A bank holds `count` adapters over one [N, K] projection as A [count, K, r]
+ * and B [count, N, r] (rank innermost, contiguous, RQ_BF16 or RQ_F16, r a
+ * multiple of 8 up to 128) and a fp32 factor per adapter.  Each of the M rows
+ * of a batch names its adapter; the plan, made once per batch and used by
+ * every layer, direction and gradient, orders the rows by adapter.
+ *
+ * rq_adapter_plan_words: int32 words of a plan of `rows` rows (-1: a bad
+ * argument; count is at most RQ_ADAPTERS_MAX).  rq_adapter_plan fills it from ids[rows] (int64 if wide != 0,
+ * else int32): 0..count-1 is the adapter, -1 is none, and a row with any
+ * other id gets NaN outputs.  tile_rows, 16, 32, 64 or 128, is how many rows
+ * of one adapter are computed together; choose about the mean number of rows
+ * per adapter. */
+#define RQ_ADAPTERS_MAX 4096
+RQ_API int64_t rq_adapter_plan_words(int64_t rows, int count, int tile_rows);
+RQ_API int rq_adapter_plan(const void* ids, int wide, int64_t rows, int count, int tile_rows,
+                    int32_t* plan, int64_t plan_words, void* stream);
+
+/* out[m, :] = base[m, :] + mid[m, :] . V_a^T,  mid[m, :] = scaling[a] * (in[m, :] . U_a)
+ * for in [M, D1], out and base [M, D2] (base may be NULL: zero, or out itself),
+ * U [count, D1, r], V [count, D2, r], mid [M, r] fp32 (written; the backward
+ * needs it).  Forward: U = A, V = B, in = x.  Input gradient: U = B, V = A,
+ * in = dy.  Everything is accumulated in fp32 and rounded once.  plan NULL:
+ * every row uses adapter 0.  Row strides (ld*) in elements, columns
+ * contiguous. */
+RQ_API int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const void* V,
+                      const float* scaling, const void* base, int64_t ld_base,
+                      int64_t M, int64_t D1, int64_t D2, int r, int count, int dtype,
+                      const int32_t* plan, int64_t plan_words, int tile_rows,
+                      float* mid, void* out, int64_t ld_out, void* stream);
+
+/* grad[a, d, j] = sum over the rows m of adapter a of z[m, d] * mid[m, j], for
+ * z [M, D] (row stride ld_z): the gradient of A with z = x and the backward's
+ * mid, of B with z = dy and the forward's mid.  With z_scales not NULL z is
+ * the 8-bit packed form (rq_act8_pack): int8 codes [M, ceil(D / 128) * 128]
+ * and z_scales [M, ceil(D / 128)].  grad [count, D, r] in dtype; an adapter
+ * without rows gets zeros. */
+RQ_API int rq_adapters_grad(const void* z, int64_t ld_z, const float* z_scales, const float* mid,
+                     int64_t M, int64_t D, int r, int count, int dtype,
+                     const int32_t* plan, int64_t plan_words, int tile_rows,
+                     void* grad, void* stream);
+
+/* ------------------------------------------- activations in 8 bits */
+
+/* Packed form of x [M, K]: blocks of RQ_ACT8_BLOCK columns of a row, codes
+ * int8 [M, nb * RQ_ACT8_BLOCK] and scales fp32 [M, nb], nb = ceil(K / block):
+ *   scale = max|x| / 127,  code = rint(x * (127 / max|x|))
+ * the last block filled with zero codes.  A block whose largest magnitude is
+ * below 2^-100 is stored as zeros; one with an infinity or NaN has scale NaN.
+ * codes must be 16-byte aligned.  unpack gives code * scale in dtype,
+ * [M, K] contiguous. */
+#define RQ_ACT8_BLOCK 128
+RQ_API int rq_act8_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K,
+                 int8_t* codes, float* scales, void* stream);
+RQ_API int rq_act8_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t K,
+                   void* out, int dtype, void* stream);
+
+/* h = silu(gate) * up for [M, K] (h contiguous), with `copies` packed forms
+ * written in the same pass one after the other (each [M, nb * block] codes
+ * and [M, nb] scales): gate, up and, with copies = 3, h as rounded.
+ * Backward from the packed gate and up:
+ *   p = 1 / (1 + exp(-gate)),  dgate = dh * up * p * (1 + gate * (1 - p)),
+ *   dup = dh * gate * p        ([M, K] contiguous). */
+RQ_API int rq_swiglu8_forward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype,
+                       int64_t M, int64_t K, void* h, int8_t* codes, float* scales, int copies, void* stream);
+RQ_API int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t M, int64_t K,
+                        const int8_t* codes, const float* scales, void* dgate, void* dup, void* stream);
+
+/* ------------------------------ token log-probabilities, preference loss */
+
+/* logits [B, L, V] (strides in elements, V contiguous), labels [B, L] int64
+ * contiguous: position l is scored on labels[b, l + 1]; a label equal to
+ * `ignore` (and the last position) does not count, and a label outside
+ * [0, V) gives NaN.  rq_token_logprobs writes stats [B, L, 4] fp32 (row
+ * maximum, sum of exp(x - maximum), the label's logit; rows that do not count
+ * are left as they are), 16-byte aligned, and, unless NULL, logps [B, L]:
+ * the log-probability of each label, 0 where it does not count. */
+RQ_API int rq_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_l,
+                      int64_t B, int64_t L, int64_t V, const int64_t* labels, int64_t ignore,
+                      float* stats, float* logps, void* stream);
+
+/* Sequences i (chosen) and i + B/2 (rejected) are a pair.  With ref [B, L] the
+ * reference model's log-probabilities, R_b = sum (log p - ref) over the
+ * labels that count, n_b their number (at least 1), z_i = beta (R_i - R_{i+B/2}):
+ *   RQ_PREF_SIGMOID: mean(-(1 - smooth) log sigma(z) - smooth log sigma(-z))
+ *   RQ_PREF_IPO:     mean((R_i / n_i - R_{i+B/2} / n_{i+B/2} - 1 / (2 beta))^2)
+ * Writes loss [1], logps [B] (sums of log p), rewards [B] (beta R) and
+ * slopes [B] (d loss / d R), all fp32. */
+#define RQ_PREF_SIGMOID 0
+#define RQ_PREF_IPO 1
+RQ_API int rq_preference_loss(int64_t B, int64_t L, const int64_t* labels, int64_t ignore,
+                       const float* stats, const float* ref, int form, float beta, float smooth,
+                       float* loss, float* logps, float* rewards, float* slopes, void* stream);
+
+/* dlogits [B, L, V] (contiguous) = upstream * slope * ([v = label] - softmax),
+ * zero where the position does not count; slope per sequence (slopes [B]) or,
+ * with per_token != 0, slopes [B, L] at the label's place.  upstream: one
+ * fp32 on the device, NULL for 1. */
+RQ_API int rq_token_logprobs_grad(const void* logits, int dtype, int64_t stride_b, int64_t stride_l,
+                           int64_t B, int64_t L, int64_t V, const int64_t* labels, int64_t ignore,
+                           const float* stats, const float* slopes, int per_token, const float* upstream,
+                           void* dlogits, void* stream);
 
 /* ------------------------------------- reference launcher drop-ins */
 

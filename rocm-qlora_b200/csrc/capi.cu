@@ -104,6 +104,29 @@ static int fill_args(LinearArgs* a, int wfmt, const void* q, const void* scales,
   return RQ_OK;
 }
 
+static bool half_ok(int dt) { return dt == RQ_BF16 || dt == RQ_F16; }
+
+// Sizes a kernel indexes with 32 bits.
+static bool fits(int64_t v) { return v >= 0 && v < (int64_t)1 << 31; }
+
+static int check_plan(int64_t rows, int count, int tile, const int32_t* plan, int64_t words) {
+  if (!fits(rows) || count < 1 || count > RQ_ADAPTERS_MAX) return RQ_ERR_INVALID;
+  if (!plan) return RQ_OK;
+  if (tile != 16 && tile != 32 && tile != 64 && tile != 128) return RQ_ERR_INVALID;
+  if (!fits(adapter_plan_words(rows, count, tile))) return RQ_ERR_INVALID;
+  if (words < adapter_plan_words(rows, count, tile)) return RQ_ERR_WORKSPACE;
+  return (uintptr_t)plan % 16 ? RQ_ERR_ALIGN : RQ_OK;
+}
+
+static int check_tokens(const void* logits, int dt, int64_t B, int64_t L, int64_t V, const int64_t* labels,
+                        const float* stats) {
+  if (!dtype_ok(dt)) return RQ_ERR_DTYPE;
+  if (B < 0 || L < 0 || V < 1 || !fits(V) || (L > 0 && !fits(B * L))) return RQ_ERR_INVALID;
+  if (B * L > 0 && (!logits || !labels || !stats)) return RQ_ERR_INVALID;
+  if ((uintptr_t)logits % dtype_size(dt) || (uintptr_t)labels % 8 || (uintptr_t)stats % 16) return RQ_ERR_ALIGN;
+  return RQ_OK;
+}
+
 }  // namespace rq
 
 using namespace rq;
@@ -301,6 +324,150 @@ int rq_weight_to_fp8(int wfmt, const void* qweight, const void* scales, int scal
   if (N * K > 0 && !fp8_out) return RQ_ERR_INVALID;
   const QWeight w{wfmt, qweight, scales, scale_dtype, c2, c2_scales, N, K, block_size};
   return weight_to_fp8(w, dtype, w_scale, fp8_out, (cudaStream_t)stream);
+}
+
+int64_t rq_adapter_plan_words(int64_t rows, int count, int tile_rows) {
+  if (!fits(rows) || count < 1 || count > RQ_ADAPTERS_MAX ||
+      (tile_rows != 16 && tile_rows != 32 && tile_rows != 64 && tile_rows != 128))
+    return -1;
+  return adapter_plan_words(rows, count, tile_rows);
+}
+
+int rq_adapter_plan(const void* ids, int wide, int64_t rows, int count, int tile_rows, int32_t* plan,
+                    int64_t plan_words, void* stream) {
+  RQ_PROLOGUE();
+  if (!plan || (rows > 0 && !ids)) return RQ_ERR_INVALID;
+  const int rc = check_plan(rows, count, tile_rows, plan, plan_words);
+  if (rc != RQ_OK) return rc;
+  if ((uintptr_t)ids % (wide ? 8 : 4)) return RQ_ERR_ALIGN;
+  return adapter_plan(ids, wide ? 1 : 0, rows, count, tile_rows, plan, (cudaStream_t)stream);
+}
+
+int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const void* V, const float* scaling,
+                      const void* base, int64_t ld_base, int64_t M, int64_t D1, int64_t D2, int r, int count,
+                      int dtype, const int32_t* plan, int64_t plan_words, int tile_rows, float* mid, void* out,
+                      int64_t ld_out, void* stream) {
+  RQ_PROLOGUE();
+  if (!half_ok(dtype)) return RQ_ERR_DTYPE;
+  const int rc = check_plan(M, count, tile_rows, plan, plan_words);
+  if (rc != RQ_OK) return rc;
+  if (!fits(D1) || !fits(D2) || r < 8 || r > 128 || r % 8) return RQ_ERR_INVALID;
+  if (M == 0) return RQ_OK;
+  if (!mid || !scaling || (D1 > 0 && (!in || !U)) || (D2 > 0 && (!V || !out))) return RQ_ERR_INVALID;
+  if ((M > 1) && (ld_in < D1 || ld_out < D2 || (base && ld_base < D2))) return RQ_ERR_INVALID;
+  if ((uintptr_t)in % 2 || (uintptr_t)base % 2 || (uintptr_t)out % 2 || (uintptr_t)U % 16 || (uintptr_t)V % 16 ||
+      (uintptr_t)mid % 16 || (uintptr_t)scaling % 4)
+    return RQ_ERR_ALIGN;
+  const AdapterRows a{M, D1, D2, r, count, dtype, tile_rows, plan};
+  return adapters_apply(a, in, ld_in, U, V, scaling, base, ld_base, mid, out, ld_out, (cudaStream_t)stream);
+}
+
+int rq_adapters_grad(const void* z, int64_t ld_z, const float* z_scales, const float* mid, int64_t M, int64_t D, int r,
+                     int count, int dtype, const int32_t* plan, int64_t plan_words, int tile_rows, void* grad,
+                     void* stream) {
+  RQ_PROLOGUE();
+  if (!half_ok(dtype)) return RQ_ERR_DTYPE;
+  const int rc = check_plan(M, count, tile_rows, plan, plan_words);
+  if (rc != RQ_OK) return rc;
+  if (!fits(D) || r < 8 || r > 128 || r % 8) return RQ_ERR_INVALID;
+  if (D == 0) return RQ_OK;
+  const int64_t nb = (D + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+  if (!grad || (M > 0 && (!z || !mid))) return RQ_ERR_INVALID;
+  if (M > 1 && ld_z < (z_scales ? nb * RQ_ACT8_BLOCK : D)) return RQ_ERR_INVALID;
+  if ((uintptr_t)z % (z_scales ? 16 : 2) || (z_scales && ld_z % 16) || (uintptr_t)mid % 16 || (uintptr_t)grad % 16)
+    return RQ_ERR_ALIGN;
+  const AdapterRows a{M, D, 0, r, count, dtype, tile_rows, plan};
+  return adapters_grad(a, z, ld_z, z_scales, nb, mid, grad, (cudaStream_t)stream);
+}
+
+int rq_act8_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, int8_t* codes, float* scales,
+                 void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!fits(M) || !fits(K) || (M > 1 && ld_x < K)) return RQ_ERR_INVALID;
+  if (M * K == 0) return RQ_OK;
+  if (!x || !codes || !scales) return RQ_ERR_INVALID;
+  if ((uintptr_t)x % dtype_size(dtype) || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return RQ_ERR_ALIGN;
+  return act8_pack(x, dtype, ld_x, M, K, codes, scales, (cudaStream_t)stream);
+}
+
+int rq_act8_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t K, void* out, int dtype,
+                   void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!fits(M) || !fits(K)) return RQ_ERR_INVALID;
+  if (M * K == 0) return RQ_OK;
+  if (!codes || !scales || !out) return RQ_ERR_INVALID;
+  if ((uintptr_t)out % dtype_size(dtype) || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return RQ_ERR_ALIGN;
+  return act8_unpack(codes, scales, M, K, out, dtype, (cudaStream_t)stream);
+}
+
+int rq_swiglu8_forward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, int64_t M,
+                       int64_t K, void* h, int8_t* codes, float* scales, int copies, void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!fits(M) || !fits(K) || (copies != 2 && copies != 3)) return RQ_ERR_INVALID;
+  if (M > 1 && (ld_gate < K || ld_up < K)) return RQ_ERR_INVALID;
+  if (M * K == 0) return RQ_OK;
+  if (!gate || !up || !h || !codes || !scales) return RQ_ERR_INVALID;
+  const int e = dtype_size(dtype);
+  if ((uintptr_t)gate % e || (uintptr_t)up % e || (uintptr_t)h % e || (uintptr_t)codes % 16 || (uintptr_t)scales % 4)
+    return RQ_ERR_ALIGN;
+  return swiglu8_forward(gate, ld_gate, up, ld_up, dtype, M, K, h, codes, scales, copies, (cudaStream_t)stream);
+}
+
+int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t M, int64_t K, const int8_t* codes,
+                        const float* scales, void* dgate, void* dup, void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!fits(M) || !fits(K) || (M > 1 && ld_dh < K)) return RQ_ERR_INVALID;
+  if (M * K == 0) return RQ_OK;
+  if (!dh || !codes || !scales || !dgate || !dup) return RQ_ERR_INVALID;
+  const int e = dtype_size(dtype);
+  if ((uintptr_t)dh % e || (uintptr_t)dgate % e || (uintptr_t)dup % e || (uintptr_t)codes % 16 ||
+      (uintptr_t)scales % 4)
+    return RQ_ERR_ALIGN;
+  return swiglu8_backward(dh, ld_dh, dtype, M, K, codes, scales, dgate, dup, (cudaStream_t)stream);
+}
+
+int rq_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_l, int64_t B, int64_t L,
+                      int64_t V, const int64_t* labels, int64_t ignore, float* stats, float* logps, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tokens(logits, dtype, B, L, V, labels, stats);
+  if (rc != RQ_OK) return rc;
+  if (B * L == 0) return RQ_OK;
+  if ((uintptr_t)logps % 4) return RQ_ERR_ALIGN;
+  const TokenRows t{logits, stride_b, stride_l, dtype, B, L, V, labels, ignore};
+  return token_logprobs(t, stats, logps, (cudaStream_t)stream);
+}
+
+int rq_preference_loss(int64_t B, int64_t L, const int64_t* labels, int64_t ignore, const float* stats,
+                       const float* ref, int form, float beta, float smooth, float* loss, float* logps, float* rewards,
+                       float* slopes, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tokens(stats, RQ_F32, B, L, 1, labels, stats);
+  if (rc != RQ_OK) return rc;
+  if (B < 2 || B % 2 || L < 1 || (form != RQ_PREF_SIGMOID && form != RQ_PREF_IPO)) return RQ_ERR_INVALID;
+  if (!(beta > 0.0f) || !(smooth >= 0.0f && smooth <= 0.5f)) return RQ_ERR_INVALID;
+  if (!ref || !loss || !logps || !rewards || !slopes) return RQ_ERR_INVALID;
+  if ((uintptr_t)ref % 4 || (uintptr_t)loss % 4 || (uintptr_t)logps % 4 || (uintptr_t)rewards % 4 ||
+      (uintptr_t)slopes % 4)
+    return RQ_ERR_ALIGN;
+  const TokenRows t{nullptr, 0, 0, RQ_F32, B, L, 1, labels, ignore};
+  return preference_loss(t, stats, ref, form, beta, smooth, loss, logps, rewards, slopes, (cudaStream_t)stream);
+}
+
+int rq_token_logprobs_grad(const void* logits, int dtype, int64_t stride_b, int64_t stride_l, int64_t B, int64_t L,
+                           int64_t V, const int64_t* labels, int64_t ignore, const float* stats, const float* slopes,
+                           int per_token, const float* upstream, void* dlogits, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tokens(logits, dtype, B, L, V, labels, stats);
+  if (rc != RQ_OK) return rc;
+  if (B * L == 0) return RQ_OK;
+  if (!slopes || !dlogits) return RQ_ERR_INVALID;
+  if ((uintptr_t)slopes % 4 || (uintptr_t)upstream % 4 || (uintptr_t)dlogits % dtype_size(dtype)) return RQ_ERR_ALIGN;
+  const TokenRows t{logits, stride_b, stride_l, dtype, B, L, V, labels, ignore};
+  return token_logprobs_grad(t, stats, slopes, per_token ? 1 : 0, upstream, dlogits, (cudaStream_t)stream);
 }
 
 void launch_int4_dequant_matmul(void* stream, void* x, void* w_packed, void* scales, void* c, int M, int N, int K,

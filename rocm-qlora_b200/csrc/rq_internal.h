@@ -102,4 +102,46 @@ int merge_weight(const QWeight& w, const float* A, const float* B, int r, float 
 int linear_dx(const LinearArgs& a, cudaStream_t st);
 int64_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int r);
 
+// Rows of a batch and the adapters they use (adapters.cu).
+struct AdapterRows {
+  int64_t M;        // rows
+  int64_t D1, D2;   // columns of the input and of the output (grad: D1 only)
+  int r;            // rank, a multiple of 8
+  int count;        // adapters of the bank
+  int dt;           // RQ_BF16 / RQ_F16
+  int tile;         // rows of a plan tile
+  const int* plan;  // nullptr: every row uses adapter 0
+};
+int64_t adapter_plan_words(int64_t rows, int count, int tile);
+int adapter_plan(const void* ids, int wide, int64_t rows, int count, int tile, int* plan, cudaStream_t st);
+int adapters_apply(const AdapterRows& a, const void* in, int64_t ldin, const void* U, const void* V,
+                   const float* scaling, const void* base, int64_t ldb, float* mid, void* out, int64_t ldo,
+                   cudaStream_t st);
+int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
+                  void* G, cudaStream_t st);
+
+// Activations in 8 bits (act8.cu).
+int act8_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, int8_t* codes, float* scales, cudaStream_t st);
+int act8_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st);
+int swiglu8_forward(const void* g, int64_t ldg, const void* u, int64_t ldu, int dt, int64_t M, int64_t K, void* h,
+                    int8_t* codes, float* scales, int copies, cudaStream_t st);
+int swiglu8_backward(const void* dh, int64_t ldh, int dt, int64_t M, int64_t K, const int8_t* codes,
+                     const float* scales, void* dg, void* du, cudaStream_t st);
+
+// Token log-probabilities and the preference loss on them (preference.cu).
+// Position l of sequence b is scored on label [b, l + 1].
+struct TokenRows {
+  const void* logits;      // [B, L, V], strides in elements, vocabulary innermost
+  int64_t sb, sl;
+  int dt;
+  int64_t B, L, V;
+  const int64_t* labels;   // [B, L] contiguous
+  int64_t ignore;          // label of a position that does not count
+};
+int token_logprobs(const TokenRows& t, float* stats, float* logps, cudaStream_t st);
+int preference_loss(const TokenRows& t, const float* stats, const float* ref, int form, float beta, float smooth,
+                    float* loss, float* logps, float* rewards, float* slopes, cudaStream_t st);
+int token_logprobs_grad(const TokenRows& t, const float* stats, const float* slopes, int per_token,
+                        const float* upstream, void* dlogits, cudaStream_t st);
+
 }  // namespace rq

@@ -10,33 +10,13 @@
 // computed here; the quantized weight arrives as its buffers plus the
 // format (wfmt, N, K, block_size), as the C ABI takes it.  The Meta
 // implementations give shapes to tracing (torch.compile, FakeTensor).
-#include <ATen/ATen.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/library.h>
-
-#include <optional>
-
-#include "../../include/rq_b200.h"
+#include "torch_ops.h"
 
 namespace {
 
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return RQ_F32;
-    case at::kBFloat16: return RQ_BF16;
-    case at::kHalf: return RQ_F16;
-    default: TORCH_CHECK(false, "rocm_qlora: unsupported dtype ", t);
-  }
-  return RQ_F32;
-}
-
-const void* ptr(const std::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
-
-void check(int rc, const char* what) {
-  TORCH_CHECK(rc == RQ_OK, "rocm_qlora: ", what, " failed: ", rq_status_string(rc), " (status ", rc,
-              rc == RQ_ERR_CUDA ? ", cuda error " + std::to_string(rq_last_cuda_error()) : std::string(), ")");
-}
+using rq_torch::check;
+using rq_torch::dtype_code;
+using rq_torch::ptr;
 
 at::Tensor linear_forward(const at::Tensor& x, int64_t wfmt, const at::Tensor& q, const std::optional<at::Tensor>& scales,
                           const std::optional<at::Tensor>& c2, const std::optional<at::Tensor>& c2s, int64_t N,

@@ -1,0 +1,303 @@
+// torch_ops_train.cpp -- torch operators of the adapters of many requests,
+// the 8-bit activations and the token log-probabilities with the preference
+// loss (include/rq_b200.h).  As in torch_ops.cpp, outputs are allocated here,
+// launches go to torch's current stream of the input's device, a status other
+// than RQ_OK raises, and nothing is computed.  On Meta tensors the operators
+// only give shapes.
+#include "torch_ops.h"
+
+#include <tuple>
+
+namespace {
+
+using at::Tensor;
+using rq_torch::check;
+using rq_torch::dtype_code;
+using rq_torch::ptr;
+using std::optional;
+
+cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+void check_rows(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), "rocm_qlora: ", name,
+              " must be a 2-D tensor with contiguous columns");
+}
+
+Tensor adapter_plan(const Tensor& ids, int64_t count, int64_t tile) {
+  TORCH_CHECK(ids.dim() == 1 && ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+              "rocm_qlora: ids must be a contiguous 1-D int64 or int32 tensor");
+  const int64_t words = rq_adapter_plan_words(ids.size(0), (int)count, (int)tile);
+  TORCH_CHECK(words >= 0, "rocm_qlora: no plan for ", ids.size(0), " rows and ", count, " adapters");
+  Tensor plan = at::empty({words}, ids.options().dtype(at::kInt));
+  if (ids.is_meta()) return plan;
+  const c10::cuda::CUDAGuard guard(ids.device());
+  check(rq_adapter_plan(ids.data_ptr(), ids.scalar_type() == at::kLong, ids.size(0), (int)count, (int)tile,
+                        plan.data_ptr<int>(), words, stream_of(ids)),
+        "rq_adapter_plan");
+  return plan;
+}
+
+// out (nullopt: mid only) = base + mid V^T, mid = scaling (in U)
+void apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling, const optional<Tensor>& base,
+           const optional<Tensor>& plan, int64_t tile, const Tensor& mid, const optional<Tensor>& out) {
+  const c10::cuda::CUDAGuard guard(in.device());
+  const bool has_base = base.has_value() && base->defined(), has_plan = plan.has_value() && plan->defined();
+  check(rq_adapters_apply(in.data_ptr(), in.stride(0), U.data_ptr(), V.data_ptr(), scaling.data_ptr<float>(), ptr(base),
+                          has_base ? base->stride(0) : 0, in.size(0), in.size(1), out ? out->size(1) : 0,
+                          (int)U.size(2), (int)U.size(0), dtype_code(in.scalar_type()),
+                          static_cast<const int32_t*>(ptr(plan)), has_plan ? plan->numel() : 0, (int)tile,
+                          mid.data_ptr<float>(), out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
+                          stream_of(in)),
+        "rq_adapters_apply");
+}
+
+void check_bank(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling) {
+  check_rows(in, "input");
+  TORCH_CHECK(U.dim() == 3 && V.dim() == 3 && U.is_contiguous() && V.is_contiguous() && U.size(0) == V.size(0) &&
+                  U.size(2) == V.size(2) && U.size(1) == in.size(1) && U.scalar_type() == in.scalar_type() &&
+                  V.scalar_type() == in.scalar_type(),
+              "rocm_qlora: adapters must be contiguous [count, columns, rank] tensors of the input's dtype and size");
+  TORCH_CHECK(scaling.is_contiguous() && scaling.scalar_type() == at::kFloat && scaling.numel() == U.size(0),
+              "rocm_qlora: scaling must be a contiguous float32 tensor of one value an adapter");
+}
+
+std::tuple<Tensor, Tensor> adapters_apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
+                                          const optional<Tensor>& base, const optional<Tensor>& plan, int64_t tile) {
+  check_bank(in, U, V, scaling);
+  if (base.has_value() && base->defined()) {
+    check_rows(*base, "base");
+    TORCH_CHECK(base->size(0) == in.size(0) && base->size(1) == V.size(1) && base->scalar_type() == in.scalar_type(),
+                "rocm_qlora: base must be [rows, ", V.size(1), "] of the input's dtype");
+  }
+  Tensor out = at::empty({in.size(0), V.size(1)}, in.options());
+  Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
+  if (!in.is_meta()) apply(in, U, V, scaling, base, plan, tile, mid, out);
+  return {out, mid};
+}
+
+Tensor adapters_apply_(Tensor out, const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
+                       const Tensor& base, const optional<Tensor>& plan, int64_t tile) {
+  check_bank(in, U, V, scaling);
+  check_rows(out, "out");
+  check_rows(base, "base");
+  TORCH_CHECK(out.size(0) == in.size(0) && out.size(1) == V.size(1) && out.scalar_type() == in.scalar_type() &&
+                  base.sizes() == out.sizes() && base.scalar_type() == in.scalar_type(),
+              "rocm_qlora: out and base must be [rows, ", V.size(1), "] of the input's dtype");
+  Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
+  if (!in.is_meta()) apply(in, U, V, scaling, base, plan, tile, mid, out);
+  return mid;
+}
+
+Tensor adapters_mid(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
+                    const optional<Tensor>& plan, int64_t tile) {
+  check_bank(in, U, V, scaling);
+  Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
+  if (!in.is_meta()) apply(in, U, V, scaling, std::nullopt, plan, tile, mid, std::nullopt);
+  return mid;
+}
+
+Tensor adapters_grad(const Tensor& z, const optional<Tensor>& scales, const Tensor& mid, int64_t D, int64_t count,
+                     at::ScalarType dtype, const optional<Tensor>& plan, int64_t tile) {
+  check_rows(z, "rows");
+  const bool packed = scales.has_value() && scales->defined(), has_plan = plan.has_value() && plan->defined();
+  const int64_t nb = (D + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+  TORCH_CHECK(mid.dim() == 2 && mid.is_contiguous() && mid.size(0) == z.size(0) && mid.scalar_type() == at::kFloat,
+              "rocm_qlora: mid must be a contiguous [rows, rank] float32 tensor");
+  TORCH_CHECK(packed ? z.scalar_type() == at::kChar && z.size(1) == nb * RQ_ACT8_BLOCK && scales->is_contiguous() &&
+                           scales->numel() == z.size(0) * nb && scales->scalar_type() == at::kFloat
+                     : z.scalar_type() == dtype && z.size(1) == D,
+              "rocm_qlora: rows must be [rows, ", D, "] of the adapters' dtype, or their packed form");
+  Tensor grad = at::empty({count, D, mid.size(1)}, z.options().dtype(dtype));
+  if (z.is_meta()) return grad;
+  const c10::cuda::CUDAGuard guard(z.device());
+  check(rq_adapters_grad(z.data_ptr(), z.stride(0), static_cast<const float*>(ptr(scales)), mid.data_ptr<float>(),
+                         z.size(0), D, (int)mid.size(1), (int)count, dtype_code(dtype),
+                         static_cast<const int32_t*>(ptr(plan)), has_plan ? plan->numel() : 0, (int)tile,
+                         grad.data_ptr(), stream_of(z)),
+        "rq_adapters_grad");
+  return grad;
+}
+
+std::tuple<Tensor, Tensor> packed_like(const Tensor& x, int64_t copies) {
+  const int64_t nb = (x.size(1) + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+  return {at::empty({copies, x.size(0), nb * RQ_ACT8_BLOCK}, x.options().dtype(at::kChar)),
+          at::empty({copies, x.size(0), nb}, x.options().dtype(at::kFloat))};
+}
+
+std::tuple<Tensor, Tensor> act8_pack(const Tensor& x) {
+  check_rows(x, "x");
+  auto [codes, scales] = packed_like(x, 1);
+  if (!x.is_meta()) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    check(rq_act8_pack(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), x.size(0), x.size(1),
+                       codes.data_ptr<int8_t>(), scales.data_ptr<float>(), stream_of(x)),
+          "rq_act8_pack");
+  }
+  return {codes[0], scales[0]};
+}
+
+void check_packed(const Tensor& codes, const Tensor& scales, int64_t K) {
+  const int64_t nb = (K + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous() && codes.scalar_type() == at::kChar &&
+                  scales.scalar_type() == at::kFloat && codes.dim() == scales.dim() &&
+                  codes.size(-1) == nb * RQ_ACT8_BLOCK && scales.size(-1) == nb &&
+                  codes.numel() == scales.numel() * RQ_ACT8_BLOCK,
+              "rocm_qlora: not the packed form of rows of ", K, " values");
+}
+
+Tensor act8_unpack(const Tensor& codes, const Tensor& scales, int64_t K, at::ScalarType dtype) {
+  TORCH_CHECK(codes.dim() == 2, "rocm_qlora: codes must be a 2-D tensor");
+  check_packed(codes, scales, K);
+  Tensor out = at::empty({codes.size(0), K}, codes.options().dtype(dtype));
+  if (codes.is_meta()) return out;
+  const c10::cuda::CUDAGuard guard(codes.device());
+  check(rq_act8_unpack(codes.data_ptr<int8_t>(), scales.data_ptr<float>(), codes.size(0), K, out.data_ptr(),
+                       dtype_code(dtype), stream_of(codes)),
+        "rq_act8_unpack");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor> swiglu8_forward(const Tensor& gate, const Tensor& up, int64_t copies) {
+  check_rows(gate, "gate");
+  check_rows(up, "up");
+  TORCH_CHECK(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type(),
+              "rocm_qlora: gate and up must have one shape and dtype");
+  auto [codes, scales] = packed_like(gate, copies);
+  Tensor h = at::empty({gate.size(0), gate.size(1)}, gate.options());
+  if (!gate.is_meta()) {
+    const c10::cuda::CUDAGuard guard(gate.device());
+    check(rq_swiglu8_forward(gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0),
+                             dtype_code(gate.scalar_type()), gate.size(0), gate.size(1), h.data_ptr(),
+                             codes.data_ptr<int8_t>(), scales.data_ptr<float>(), (int)copies, stream_of(gate)),
+          "rq_swiglu8_forward");
+  }
+  return {h, codes, scales};
+}
+
+std::tuple<Tensor, Tensor> swiglu8_backward(const Tensor& dh, const Tensor& codes, const Tensor& scales) {
+  check_rows(dh, "dh");
+  TORCH_CHECK(codes.dim() == 3 && codes.size(0) >= 2 && codes.size(1) == dh.size(0),
+              "rocm_qlora: codes must hold the packed gate and up of dh's rows");
+  check_packed(codes, scales, dh.size(1));
+  Tensor dgate = at::empty({dh.size(0), dh.size(1)}, dh.options()), dup = at::empty_like(dgate);
+  if (!dh.is_meta()) {
+    const c10::cuda::CUDAGuard guard(dh.device());
+    check(rq_swiglu8_backward(dh.data_ptr(), dh.stride(0), dtype_code(dh.scalar_type()), dh.size(0), dh.size(1),
+                              codes.data_ptr<int8_t>(), scales.data_ptr<float>(), dgate.data_ptr(), dup.data_ptr(),
+                              stream_of(dh)),
+          "rq_swiglu8_backward");
+  }
+  return {dgate, dup};
+}
+
+void check_logits(const Tensor& logits, const Tensor& labels) {
+  TORCH_CHECK(logits.dim() == 3 && (logits.size(2) <= 1 || logits.stride(2) == 1),
+              "rocm_qlora: logits must be [batch, length, vocabulary] with a contiguous vocabulary");
+  TORCH_CHECK(labels.dim() == 2 && labels.is_contiguous() && labels.scalar_type() == at::kLong &&
+                  labels.size(0) == logits.size(0) && labels.size(1) == logits.size(1),
+              "rocm_qlora: labels must be a contiguous [batch, length] int64 tensor");
+}
+
+void logprobs(const Tensor& logits, const Tensor& labels, int64_t ignore, const Tensor& stats, float* logps) {
+  check(rq_token_logprobs(logits.data_ptr(), dtype_code(logits.scalar_type()), logits.stride(0), logits.stride(1),
+                          logits.size(0), logits.size(1), logits.size(2), labels.data_ptr<int64_t>(), ignore,
+                          stats.data_ptr<float>(), logps, stream_of(logits)),
+        "rq_token_logprobs");
+}
+
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& labels, int64_t ignore) {
+  check_logits(logits, labels);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  Tensor logps = at::empty({logits.size(0), logits.size(1)}, f32);
+  Tensor stats = at::empty({logits.size(0), logits.size(1), 4}, f32);
+  if (!logits.is_meta()) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    logprobs(logits, labels, ignore, stats, logps.data_ptr<float>());
+  }
+  return {logps, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> preference_forward(const Tensor& logits, const Tensor& labels,
+                                                                      const Tensor& ref, int64_t ignore, int64_t form,
+                                                                      double beta, double smooth) {
+  check_logits(logits, labels);
+  TORCH_CHECK(ref.sizes() == labels.sizes() && ref.is_contiguous() && ref.scalar_type() == at::kFloat,
+              "rocm_qlora: ref must be a contiguous [batch, length] float32 tensor");
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const int64_t B = logits.size(0), L = logits.size(1);
+  Tensor loss = at::empty({}, f32), logps = at::empty({B}, f32), rewards = at::empty({B}, f32),
+         slopes = at::empty({B}, f32), stats = at::empty({B, L, 4}, f32);
+  if (!logits.is_meta()) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    logprobs(logits, labels, ignore, stats, nullptr);
+    check(rq_preference_loss(B, L, labels.data_ptr<int64_t>(), ignore, stats.data_ptr<float>(), ref.data_ptr<float>(),
+                             (int)form, (float)beta, (float)smooth, loss.data_ptr<float>(), logps.data_ptr<float>(),
+                             rewards.data_ptr<float>(), slopes.data_ptr<float>(), stream_of(logits)),
+          "rq_preference_loss");
+  }
+  return {loss, logps, rewards, slopes, stats};
+}
+
+Tensor token_logprobs_grad(const Tensor& logits, const Tensor& labels, int64_t ignore, const Tensor& stats,
+                           const Tensor& slopes, const optional<Tensor>& upstream) {
+  check_logits(logits, labels);
+  const bool per_token = slopes.dim() == 2;
+  TORCH_CHECK(slopes.is_contiguous() && slopes.scalar_type() == at::kFloat && slopes.size(0) == logits.size(0) &&
+                  (!per_token || slopes.size(1) == logits.size(1)) && stats.is_contiguous() &&
+                  stats.scalar_type() == at::kFloat && stats.numel() == logits.size(0) * logits.size(1) * 4,
+              "rocm_qlora: slopes must be contiguous [batch] or [batch, length] float32");
+  if (upstream) TORCH_CHECK(upstream->numel() == 1 && upstream->scalar_type() == at::kFloat, "rocm_qlora: upstream must be one float32");
+  Tensor d = at::empty({logits.size(0), logits.size(1), logits.size(2)}, logits.options());
+  if (logits.is_meta()) return d;
+  const c10::cuda::CUDAGuard guard(logits.device());
+  check(rq_token_logprobs_grad(logits.data_ptr(), dtype_code(logits.scalar_type()), logits.stride(0), logits.stride(1),
+                               logits.size(0), logits.size(1), logits.size(2), labels.data_ptr<int64_t>(), ignore,
+                               stats.data_ptr<float>(), slopes.data_ptr<float>(), per_token,
+                               static_cast<const float*>(ptr(upstream)), d.data_ptr(), stream_of(logits)),
+        "rq_token_logprobs_grad");
+  return d;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
+  m.def("adapter_plan(Tensor ids, int count, int tile) -> Tensor");
+  m.def(
+      "adapters_apply(Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor? base, Tensor? plan, int tile) "
+      "-> (Tensor, Tensor)");
+  m.def(
+      "adapters_apply_(Tensor(a!) out, Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor base, Tensor? plan, "
+      "int tile) -> Tensor");
+  m.def("adapters_mid(Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor? plan, int tile) -> Tensor");
+  m.def(
+      "adapters_grad(Tensor z, Tensor? scales, Tensor mid, int columns, int count, ScalarType dtype, Tensor? plan, "
+      "int tile) -> Tensor");
+  m.def("act8_pack(Tensor x) -> (Tensor, Tensor)");
+  m.def("act8_unpack(Tensor codes, Tensor scales, int columns, ScalarType dtype) -> Tensor");
+  m.def("swiglu8_forward(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor, Tensor)");
+  m.def("swiglu8_backward(Tensor dh, Tensor codes, Tensor scales) -> (Tensor, Tensor)");
+  m.def("token_logprobs(Tensor logits, Tensor labels, int ignore) -> (Tensor, Tensor)");
+  m.def(
+      "preference_forward(Tensor logits, Tensor labels, Tensor ref, int ignore, int form, float beta, float smooth) "
+      "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "token_logprobs_grad(Tensor logits, Tensor labels, int ignore, Tensor stats, Tensor slopes, Tensor? upstream) "
+      "-> Tensor");
+}
+
+#define RQ_IMPLS(m)                                          \
+  m.impl("adapter_plan", &adapter_plan);                     \
+  m.impl("adapters_apply", &adapters_apply);                 \
+  m.impl("adapters_apply_", &adapters_apply_);               \
+  m.impl("adapters_mid", &adapters_mid);                     \
+  m.impl("adapters_grad", &adapters_grad);                   \
+  m.impl("act8_pack", &act8_pack);                           \
+  m.impl("act8_unpack", &act8_unpack);                       \
+  m.impl("swiglu8_forward", &swiglu8_forward);               \
+  m.impl("swiglu8_backward", &swiglu8_backward);             \
+  m.impl("token_logprobs", &token_logprobs);                 \
+  m.impl("preference_forward", &preference_forward);         \
+  m.impl("token_logprobs_grad", &token_logprobs_grad)
+
+TORCH_LIBRARY_IMPL(rocm_qlora, CUDA, m) { RQ_IMPLS(m); }
+TORCH_LIBRARY_IMPL(rocm_qlora, Meta, m) { RQ_IMPLS(m); }

@@ -83,6 +83,17 @@ def _bind(L: ctypes.CDLL) -> None:
         "rq_peer_handle": ([P, P], I),
         "rq_peer_open": ([P, ctypes.POINTER(ctypes.c_void_p)], I),
         "rq_peer_close": ([P], I),
+        "rq_adapter_plan_words": ([I64, I, I], I64),
+        "rq_adapter_plan": ([P, I, I64, I, I, P, I64, P], I),
+        "rq_adapters_apply": ([P, I64, P, P, P, P, I64, I64, I64, I64, I, I, I, P, I64, I, P, P, I64, P], I),
+        "rq_adapters_grad": ([P, I64, P, P, I64, I64, I, I, I, P, I64, I, P, P], I),
+        "rq_act8_pack": ([P, I, I64, I64, I64, P, P, P], I),
+        "rq_act8_unpack": ([P, P, I64, I64, P, I, P], I),
+        "rq_swiglu8_forward": ([P, I64, P, I64, I, I64, I64, P, P, P, I, P], I),
+        "rq_swiglu8_backward": ([P, I64, I, I64, I64, P, P, P, P, P], I),
+        "rq_token_logprobs": ([P, I, I64, I64, I64, I64, I64, P, I64, P, P, P], I),
+        "rq_preference_loss": ([I64, I64, P, I64, P, P, I, F, F, P, P, P, P, P], I),
+        "rq_token_logprobs_grad": ([P, I, I64, I64, I64, I64, I64, P, I64, P, P, I, P, P, P], I),
         "launch_int4_dequant_matmul": ([P, P, P, P, P, I, I, I, I], None),
         "launch_int8_dequant_matmul": ([P, P, P, P, P, I, I, I, I], None),
     }
@@ -102,6 +113,9 @@ def exported_symbols() -> Tuple[str, ...]:
             "rq_linear_workspace_bytes", "rq_linear_forward", "rq_linear_dx", "rq_linear_forward_noalloc",
             "rq_linear_forward_gather", "rq_peer_alloc", "rq_peer_free", "rq_peer_handle", "rq_peer_open",
             "rq_peer_close",
+            "rq_adapter_plan_words", "rq_adapter_plan", "rq_adapters_apply", "rq_adapters_grad",
+            "rq_act8_pack", "rq_act8_unpack", "rq_swiglu8_forward", "rq_swiglu8_backward",
+            "rq_token_logprobs", "rq_preference_loss", "rq_token_logprobs_grad",
             "launch_int4_dequant_matmul", "launch_int8_dequant_matmul")
 
 
@@ -143,6 +157,22 @@ def ops() -> bool:
                         ok = False
                 _ops_state = ok
     return _ops_state
+
+
+def require_ops(*ts: torch.Tensor):
+    """torch.ops.rocm_qlora for operators that exist only there, after checking
+    that the tensors are on one sm_100 CUDA device."""
+    first = ts[0]
+    for t in ts:
+        if not t.is_cuda:
+            raise NativeUnavailable(
+                "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device")
+        if t.device != first.device:
+            raise RuntimeError(f"tensors are on different devices: {first.device} and {t.device}")
+    if not ops():
+        raise NativeUnavailable(f"the torch extension {OPS_PATH} is missing or does not load "
+                                "(run `make -C rocm-qlora_b200` or __graft_entry__.build())")
+    return torch.ops.rocm_qlora
 
 
 def device_supported(device: Optional[torch.device] = None) -> bool:

@@ -1,0 +1,44 @@
+"""silu(gate) * up that keeps gate and up in 8 bits for its backward."""
+from typing import Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from rocm_qlora import _native as nat
+from rocm_qlora.activation8.packed import PackedActivation, rows_of
+
+
+class _Swiglu8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up, copies):
+        h, codes, scales = nat.require_ops(gate, up).swiglu8_forward(rows_of(gate), rows_of(up), copies)
+        ctx.save_for_backward(codes[:2], scales[:2])
+        ctx.shape = gate.shape
+        ctx.mark_non_differentiable(codes, scales)
+        return h.view(gate.shape), codes, scales
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, _codes, _scales):
+        codes, scales = ctx.saved_tensors
+        dgate, dup = nat.require_ops(dh, codes).swiglu8_backward(rows_of(dh), codes, scales)
+        return dgate.view(ctx.shape), dup.view(ctx.shape), None
+
+
+def swiglu8(gate: torch.Tensor, up: torch.Tensor,
+            pack_output: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, PackedActivation]]:
+    """``silu(gate) * up`` for gate and up [..., K] of one dtype (float32,
+    bfloat16 or float16; row strides allowed, such as the two halves of one
+    projection's output).
+
+    The product is of the values as given; for the backward only their packed
+    forms are kept (2.06 bytes a column instead of 4).  ``pack_output=True``
+    also returns the packed form of the product, written in the same pass,
+    for the projection that reads it (``packed_x=``)."""
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ")
+    if gate.dim() < 1:
+        raise ValueError("swiglu8 needs at least one dimension")
+    nat.dtype_code(gate.dtype)
+    h, codes, scales = _Swiglu8.apply(gate, up, 3 if pack_output else 2)
+    return (h, PackedActivation(codes[2], scales[2], tuple(h.shape), h.dtype)) if pack_output else h

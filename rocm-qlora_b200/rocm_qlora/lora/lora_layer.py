@@ -11,6 +11,8 @@ import math
 import torch
 import torch.nn as nn
 
+from rocm_qlora.activation8 import pack_activation
+from rocm_qlora.lora import adapter_bank
 from rocm_qlora.quantization.quant_linear import QuantLinear
 from rocm_qlora.quantization import layer_ops
 
@@ -36,8 +38,28 @@ class LoRALinear(nn.Module):
         b = self.base_layer
         return isinstance(b, QuantLinear) and not (b.merged_mode and b.merged_fp16_weight is not None)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """base_output + (dropout(x) @ A.T @ B.T * scaling)."""
+    def _forward_packed(self, x: torch.Tensor, packed_x) -> torch.Tensor:
+        """forward with the input kept in 8 bits for lora_A's gradient."""
+        if not self._fusable():
+            raise RuntimeError("packed_x needs a QuantLinear base that is not merged")
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"packed_x takes bfloat16 or float16 activations, got {x.dtype}")
+        b = self.base_layer
+        A, B = adapter_bank.one_adapter(self.lora_A, self.lora_B, x.dtype)
+        scaling = torch.full((1,), self.scaling, dtype=torch.float32, device=x.device)
+        if isinstance(self.lora_dropout, nn.Dropout) and self.training and self.lora_dropout.p > 0:
+            # the adapter reads what dropout left of x, so that is what is packed
+            xd = self.lora_dropout(x)
+            return adapter_bank.adapters_add(b(x), xd, A, B, scaling, packed_x=pack_activation(xd.detach()))
+        return adapter_bank.bank_linear(x, b.weight_view(), b.bias, A, B, scaling, packed_x=packed_x)
+
+    def forward(self, x: torch.Tensor, packed_x=None) -> torch.Tensor:
+        """base_output + (dropout(x) @ A.T @ B.T * scaling).  With ``packed_x``
+        (``activation8.pack_activation`` of x, shared by the layers that read
+        x) training keeps that in x's place: the gradient of lora_A is of the
+        packed values, everything else is of x."""
+        if packed_x is not None and not self.merged:
+            return self._forward_packed(x, packed_x)
         if self.merged:
             return self.base_layer(x)
         if self._fusable():

@@ -1,0 +1,117 @@
+"""Log-probabilities of given tokens and the paired preference loss, straight
+from logits of any float dtype (csrc/preference.cu): one pass over the rows
+that count forward, one backward, no 32-bit copy of the logits.
+
+As in causal language models, position ``l`` is scored on ``labels[:, l + 1]``
+(the shift happens inside), and labels equal to ``ignore_index`` (prompts,
+padding) do not count; their rows are not read.
+"""
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from rocm_qlora import _native as nat
+
+_FORMS = {"sigmoid": 0, "ipo": 1}
+
+
+def _check(logits: torch.Tensor, labels: torch.Tensor):
+    if logits.dim() != 3 or labels.shape != logits.shape[:2]:
+        raise ValueError(f"logits must be [batch, length, vocabulary] and labels [batch, length]; got "
+                         f"{tuple(logits.shape)} and {tuple(labels.shape)}")
+    if labels.dtype != torch.int64:
+        raise TypeError(f"labels must be int64, got {labels.dtype}")
+    if logits.shape[2] < 1:
+        raise ValueError("the vocabulary is empty")
+    nat.dtype_code(logits.dtype)
+    if logits.stride(2) != 1 and logits.shape[2] > 1:
+        logits = logits.contiguous()
+    return logits, labels.contiguous()
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ignore):
+        logps, stats = nat.require_ops(logits, labels).token_logprobs(logits, labels, ignore)
+        ctx.save_for_backward(logits, labels, stats)
+        ctx.ignore = ignore
+        return logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, labels, stats = ctx.saved_tensors
+        d = nat.require_ops(logits, g).token_logprobs_grad(logits, labels, ctx.ignore, stats, g.contiguous(), None)
+        return d, None, None
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """[batch, length] float32: at each label's place its log-probability
+    under the position before it, 0 where the label does not count (and at
+    the first place).  A label outside the vocabulary gives NaN.
+    Differentiable in ``logits``."""
+    logits, labels = _check(logits, labels)
+    return _TokenLogprobs.apply(logits, labels, int(ignore_index))
+
+
+class PreferenceOutput(NamedTuple):
+    """``loss`` (differentiable), and without gradients: ``logps`` [batch] sums
+    of the log-probabilities that count, ``chosen_rewards`` and
+    ``rejected_rewards`` [batch / 2]: beta * (log-probability - reference's)."""
+    loss: torch.Tensor
+    logps: torch.Tensor
+    chosen_rewards: torch.Tensor
+    rejected_rewards: torch.Tensor
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ref, ignore, form, beta, smooth):
+        loss, logps, rewards, slopes, stats = nat.require_ops(logits, labels, ref).preference_forward(
+            logits, labels, ref, ignore, form, beta, smooth)
+        ctx.save_for_backward(logits, labels, stats, slopes)
+        ctx.ignore = ignore
+        ctx.mark_non_differentiable(logps, rewards)
+        return loss, logps, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _logps, _rewards):
+        logits, labels, stats, slopes = ctx.saved_tensors
+        d = nat.require_ops(logits, g).token_logprobs_grad(logits, labels, ctx.ignore, stats, slopes, g)
+        return d, None, None, None, None, None, None
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor, beta: float = 0.1,
+                    label_smoothing: float = 0.0, form: str = "sigmoid",
+                    ignore_index: int = -100) -> PreferenceOutput:
+    """The paired preference loss of a batch whose first half are the chosen
+    answers and whose second half the rejected ones of the same prompts.
+
+    ``ref_logps`` [batch, length] are the reference model's log-probabilities
+    as ``token_logprobs`` gives them: per token, since the loss takes a small
+    difference of two sums over the sequence.  With R the sum of
+    (log p - ref) over the tokens of an answer and n their number,
+
+        sigmoid: mean(-(1 - w) log sigma(z) - w log sigma(-z)),
+                 z = beta (R_chosen - R_rejected), w = label_smoothing
+        ipo:     mean((R_chosen / n - R_rejected / n - 1 / (2 beta))^2)
+    """
+    if form not in _FORMS:
+        raise ValueError(f"form must be one of {sorted(_FORMS)}, got {form!r}")
+    if not beta > 0.0:
+        raise ValueError(f"beta must be positive, got {beta}")
+    if not 0.0 <= label_smoothing <= 0.5:
+        raise ValueError(f"label_smoothing must be between 0 and 0.5, got {label_smoothing}")
+    if form == "ipo" and label_smoothing:
+        raise ValueError("label_smoothing belongs to the sigmoid form")
+    logits, labels = _check(logits, labels)
+    if logits.shape[0] < 2 or logits.shape[0] % 2 or logits.shape[1] < 1:
+        raise ValueError(f"a batch holds pairs (chosen, then rejected): got {logits.shape[0]} sequences")
+    if ref_logps.shape != labels.shape:
+        raise ValueError(f"ref_logps must be [batch, length] like labels, got {tuple(ref_logps.shape)}")
+    loss, logps, rewards = _PreferenceLoss.apply(logits, labels, ref_logps.detach().float().contiguous(),
+                                                 int(ignore_index), _FORMS[form], float(beta), float(label_smoothing))
+    half = logits.shape[0] // 2
+    return PreferenceOutput(loss, logps, rewards[:half], rewards[half:])
