@@ -12,9 +12,12 @@
 //
 // The plan orders the rows by adapter (stable: equal inputs give equal sums)
 // and cuts them into tiles of at most tile_rows rows of one adapter.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
-#include "linear_common.cuh"
+#include "gemv_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace rq {
 
@@ -134,77 +137,412 @@ int adapter_plan(const void* ids, int wide, int64_t rows, int count, int tile, i
 
 // ------------------------------------------------------------------ apply
 
-__device__ __forceinline__ int row_group(const AdapterRows& a, int place, int64_t* row) {
-  if (!a.plan) {
-    *row = place;
-    return 0;
-  }
-  *row = a.plan[plan_rows_at(a.M, a.count, a.tile) + place];
-  int lo = 0, hi = a.count + 2;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.plan[1 + mid] <= place) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+constexpr int kApThreads = 256, kApWarps = kApThreads / 32;
+constexpr int kApWin = 32;  // columns of a window: one 16-byte load of each lane of a quad
+
+// Bytes between rows of the staged U (conflict-free ldmatrix) and of the
+// intermediate's halves (a quarter warp's loads on distinct banks).
+__host__ __device__ constexpr int ap_pitch_u(int R) { return R * 2 + 16; }
+__host__ __device__ constexpr int ap_pitch_m(int R) { return R <= 32 ? R * 2 : R * 2 + 64; }
+
+struct ApplyArgs {
+  AdapterRows a;
+  const void* in;
+  int64_t ldin;
+  const void* U;
+  const void* V;
+  const float* scaling;
+  const void* base;
+  int64_t ldb;
+  float* mid;
+  void* out;
+  int64_t ldo;
+  bool vec_in, vec_out;  // 16-byte accesses to the rows of in, and of base and out
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool take) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
-// mid[m, j] = s_a sum_d in[m, d] U_a[d, j]; one CTA a row.
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&d)[4], const void* p) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a)
+               : "memory");
+}
+
+// 8 consecutive 16-bit values of a row from column c (zero past `cols`).
+__device__ __forceinline__ uint4 load_row8(const uint16_t* row, int64_t c, int64_t cols, bool vec) {
+  if (vec && c + 8 <= cols) return *reinterpret_cast<const uint4*>(row + c);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = c + 2 * i < cols ? row[c + 2 * i] : 0u, hi = c + 2 * i + 1 < cols ? row[c + 2 * i + 1] : 0u;
+    w[i] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int DT>
-__global__ void __launch_bounds__(128) adapter_down_k(AdapterRows a, const void* __restrict__ in, int64_t ld,
-                                                      const void* __restrict__ U, const float* __restrict__ scaling,
-                                                      float* __restrict__ mid) {
+__device__ __forceinline__ void split16(float v, uint16_t* hi, uint16_t* lo) {
   using T = typename DType<DT>::T;
-  int64_t m;
-  const int g = row_group(a, blockIdx.x, &m);
-  const int j = threadIdx.x;
-  if (j >= a.r) return;
-  float acc = 0.0f;
-  if (g < a.count) {
-    const T* x = static_cast<const T*>(in) + m * ld;
-    const T* u = static_cast<const T*>(U) + (int64_t)g * a.D1 * a.r + j;
-    for (int64_t d = 0; d < a.D1; ++d) acc = fmaf(DType<DT>::to_f32(x[d]), DType<DT>::to_f32(u[d * a.r]), acc);
-    acc *= scaling[g];
-  } else if (g > a.count) {
-    acc = __int_as_float(0x7fc00000);
-  }
-  mid[m * a.r + j] = acc;
+  const T h = DType<DT>::from_f32(v);
+  const T l = DType<DT>::from_f32(v - DType<DT>::to_f32(h));
+  *hi = *reinterpret_cast<const uint16_t*>(&h);
+  *lo = *reinterpret_cast<const uint16_t*>(&l);
 }
 
-// out[m, d] = base[m, d] + sum_j mid[m, j] V_a[d, j].
-template <int DT>
-__global__ void __launch_bounds__(256) adapter_up_k(AdapterRows a, const void* __restrict__ base, int64_t ldb,
-                                                    const float* __restrict__ mid, const void* __restrict__ V,
-                                                    void* __restrict__ out, int64_t ldo) {
+// One cluster computes one tile: `tile` rows (16 to 128) of one adapter.
+//
+// Mathematics.  mid = s (in U) and out = base + mid V^T, both on tensor cores
+// (mma m16n8k16, fp32 accumulation).  U and V enter as they are; mid is fp32
+// and is multiplied as the sum of two 16-bit halves, so it keeps 16 bits.
+// For fp16, whose exponent range a small gradient would leave, each row of
+// mid is first brought near 2^14 by a power of two that the output row takes
+// back.
+//
+// What bounds it: in and base are read and out written once (HBM), while U
+// and V are shared by the tile's rows (L2).  The sum over all input columns
+// has to be complete before the first output, so with one launch the split
+// is by columns inside a cluster: each CTA sums its share of the input
+// columns, the partial sums meet through distributed shared memory in rank
+// order (equal inputs give equal bits), and each CTA writes its share of the
+// output columns.  A decode row costs one launch, no workspace and no second
+// kernel.
+//
+// Loads.  A quad's four lanes hold 32 consecutive columns of a row, 8 each,
+// straight from global memory in one 16-byte load; the MMA's order of the
+// reduction index follows that, and U's rows are put into shared memory in
+// the order that ldmatrix then needs.  V's columns are permuted the same way
+// among the MMA's n index, so that a lane ends with 8 consecutive output
+// columns: one 16-byte load of base and one store.
+template <int DT, int R, int NW>
+__global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(const __grid_constant__ ApplyArgs p) {
   using T = typename DType<DT>::T;
-  int64_t m;
-  const int g = row_group(a, blockIdx.x, &m);
-  const int64_t d = (int64_t)blockIdx.y * 256 + threadIdx.x;
-  if (d >= a.D2) return;
-  float acc = base ? DType<DT>::to_f32(static_cast<const T*>(base)[m * ldb + d]) : 0.0f;
-  if (g < a.count) {
-    const T* v = static_cast<const T*>(V) + ((int64_t)g * a.D2 + d) * a.r;
-    float sum = 0.0f;
-    for (int j = 0; j < a.r; ++j) sum = fmaf(mid[m * a.r + j], DType<DT>::to_f32(v[j]), sum);
-    acc += sum;
-  } else if (g > a.count) {
-    acc = __int_as_float(0x7fc00000);
-  }
-  static_cast<T*>(out)[m * ldo + d] = DType<DT>::from_f32(acc);
-}
+  constexpr int NT = R / 8;               // n-tiles of the first product
+  constexpr int KS = R / 16;              // k-steps of the second
+  constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R);
+  extern __shared__ __align__(16) unsigned char smem[];
+  const AdapterRows& a = p.a;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-int adapters_apply(const AdapterRows& a, const void* in, int64_t ldin, const void* U, const void* V,
-                   const float* scaling, const void* base, int64_t ldb, float* mid, void* out, int64_t ldo,
-                   cudaStream_t st) {
-  const dim3 grid((unsigned)a.M, (unsigned)((a.D2 + 255) / 256));
-  if (a.dt == RQ_BF16) {
-    adapter_down_k<RQ_BF16><<<(unsigned)a.M, 128, 0, st>>>(a, in, ldin, U, scaling, mid);
-    adapter_up_k<RQ_BF16><<<grid, 256, 0, st>>>(a, base, ldb, mid, V, out, ldo);
+  // ---- the tile
+  const int tile_id = (int)(blockIdx.x / csize);
+  int group, first, rows;
+  const int* order = nullptr;
+  if (a.plan) {
+    if (tile_id >= a.plan[0]) return;
+    const int4 e = reinterpret_cast<const int4*>(a.plan + plan_tiles_at(a.count))[tile_id];
+    group = e.x, first = e.y, rows = e.z;
+    order = a.plan + plan_rows_at(a.M, a.count, a.tile);
   } else {
-    adapter_down_k<RQ_F16><<<(unsigned)a.M, 128, 0, st>>>(a, in, ldin, U, scaling, mid);
-    adapter_up_k<RQ_F16><<<grid, 256, 0, st>>>(a, base, ldb, mid, V, out, ldo);
+    group = 0, first = tile_id * a.tile;
+    rows = min(a.tile, (int)a.M - first);
+  }
+  const int WM = a.tile / 16, WK = kApWarps / WM;  // warps along rows, along columns
+  const bool none = group >= a.count;
+  const float fill = group > a.count ? __int_as_float(0x7fc00000) : 0.0f;
+
+  float* part = reinterpret_cast<float*>(smem);                       // [128][R], over the staged U
+  const int KC = NW * WK * kApWin;                                    // columns staged at once
+  unsigned char* mids = smem + 2 * KC * PU;                           // halves of mid: [2][tile][PM]
+  float* rowmul = reinterpret_cast<float*>(mids + 2 * a.tile * PM);   // [tile]
+  int* rowid = reinterpret_cast<int*>(rowmul + 128);                  // [tile]
+  for (int i = tid; i < a.tile; i += kApThreads) {
+    const int at = first + min(i, rows - 1);
+    rowid[i] = order ? order[at] : at;
+  }
+  __syncthreads();
+
+  if (!none) {
+    // ---- partial sums over this CTA's input columns
+    const uint16_t* U = static_cast<const uint16_t*>(p.U) + (int64_t)group * a.D1 * a.r;
+    const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
+    const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
+    const int step = NW * WK, chunks = (w_end - w_begin + step - 1) / step;
+    const int wm = warp % WM, wk = warp / WM;
+    const uint16_t* xa = static_cast<const uint16_t*>(p.in) + (int64_t)rowid[wm * 16 + g] * p.ldin;
+    const uint16_t* xb = static_cast<const uint16_t*>(p.in) + (int64_t)rowid[wm * 16 + g + 8] * p.ldin;
+
+    auto stage = [&](int c) {  // U's rows of chunk c, each at the place its window's order gives it
+      unsigned char* dst = smem + (c & 1) * KC * PU;
+      for (int i = tid; i < KC * NT; i += kApThreads) {
+        const int k = i / NT, q = i - k * NT;
+        const int64_t col = (int64_t)(w_begin + c * step) * kApWin + k;
+        const int in = k & 31, slot = (k & ~31) | ((in & 6) << 2) | ((in >> 3) << 1) | (in & 1);
+        const bool ok = col < a.D1 && q * 8 < a.r;
+        cp_async16(dst + slot * PU + q * 16, U + (ok ? col * a.r + q * 8 : 0), ok);
+      }
+      cp_async_commit();
+    };
+    auto fetch = [&](uint4 (&x)[NW][2], int c) {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const int win = w_begin + c * step + wk * NW + w;
+        const int64_t col = win < w_end ? (int64_t)win * kApWin + t * 8 : a.D1;
+        x[w][0] = load_row8(xa, col, a.D1, p.vec_in);
+        x[w][1] = load_row8(xb, col, a.D1, p.vec_in);
+      }
+    };
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+    uint4 x[NW][2], nx[NW][2];
+    if (chunks > 0) {
+      stage(0);
+      fetch(x, 0);
+    }
+    for (int c = 0; c < chunks; ++c) {
+      if (c + 1 < chunks) {
+        stage(c + 1);
+        fetch(nx, c + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncthreads();
+      const unsigned char* u = smem + (c & 1) * KC * PU + wk * NW * kApWin * PU;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t a0 = s ? x[w][0].z : x[w][0].x, a2 = s ? x[w][0].w : x[w][0].y;
+          const uint32_t a1 = s ? x[w][1].z : x[w][1].x, a3 = s ? x[w][1].w : x[w][1].y;
+          const unsigned char* row = u + (w * 32 + s * 16 + (lane & 15)) * PU + (lane >> 4) * 16;
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, row + j * 16);
+            Mma16816<DT>::run(acc[j], a0, a1, a2, a3, b[0], b[1]);
+            Mma16816<DT>::run(acc[j + 1], a0, a1, a2, a3, b[2], b[3]);
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) x[w][0] = nx[w][0], x[w][1] = nx[w][1];
+    }
+
+    // ---- the sums meet: warps of the CTA in order, then the cluster's CTAs in rank order
+    float* mine = part + (wk * a.tile + wm * 16) * R;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      *reinterpret_cast<float2*>(mine + g * R + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * R + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    if (WK > 1) {
+      for (int i = tid; i < a.tile * R; i += kApThreads) {
+        float v = part[i];
+        for (int w = 1; w < WK; ++w) v += part[w * a.tile * R + i];
+        part[i] = v;
+      }
+    }
+    cluster.sync();
+    // 16 lanes a row, this CTA's share of the rows; the result goes to every CTA
+    constexpr int E = R / 16;
+    const int share = (a.tile + csize - 1) / csize, l16 = tid & 15;
+    const float s = p.scaling[group];
+    for (int i0 = 0; i0 < share; i0 += kApThreads / 16) {
+      const int i = i0 + tid / 16, row = crank * share + i;
+      const bool on = i < share && row < a.tile;
+      float v[E];
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = 0.0f;
+      if (on) {
+        for (int c = 0; c < csize; ++c) {
+          const float* src = cluster.map_shared_rank(part, c) + row * R + l16 * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] += src[e];
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          v[e] *= s;
+          top = fmaxf(top, fabsf(v[e]));
+          if (p.mid && row < rows && l16 * E + e < a.r) p.mid[(int64_t)rowid[row] * a.r + l16 * E + e] = v[e];
+        }
+      }
+      float mul = 1.0f, back = 1.0f;
+      if constexpr (DT == RQ_F16) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = (int)(__float_as_uint(top) >> 23);  // biased exponent; 255: not finite, small: leave
+        if (ex > 30 && ex < 255) {
+          mul = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
+          back = __uint_as_float((uint32_t)(ex - 14) << 23);
+        }
+      }
+      if (on) {
+        __align__(16) uint16_t hi[E], lo[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) split16<DT>(v[e] * mul, &hi[e], &lo[e]);
+        for (int c = 0; c < csize; ++c) {
+          unsigned char* m = cluster.map_shared_rank(mids, c) + row * PM + l16 * E * 2;
+          uint16_t* h = reinterpret_cast<uint16_t*>(m);
+          uint16_t* l = reinterpret_cast<uint16_t*>(m + a.tile * PM);
+#pragma unroll
+          for (int e = 0; e < E; ++e) h[e] = hi[e], l[e] = lo[e];
+          if (l16 == 0) cluster.map_shared_rank(rowmul, c)[row] = back;
+        }
+      }
+    }
+    cluster.sync();
+  } else {
+    if (p.mid && crank == 0)
+      for (int i = tid; i < rows * a.r; i += kApThreads) p.mid[(int64_t)rowid[i / a.r] * a.r + i % a.r] = fill;
+    if (p.out == p.base && fill == 0.0f) return;
+  }
+
+  // ---- this warp's output columns, 32 at a time, all rows of the tile
+  const int n_tiles = (rows + 15) / 16;
+  const uint16_t* V = static_cast<const uint16_t*>(p.V) + (none ? 0 : (int64_t)group * a.D2 * a.r);
+  const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+  const int chunks2 = (int)((a.D2 + 31) / 32);
+  for (int ch = crank * kApWarps + warp; ch < chunks2; ch += csize * kApWarps) {
+    // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
+    uint32_t b[4][KS][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = (int64_t)ch * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
+      const uint16_t* v = V + n * a.r;
+      const bool in = !none && n < a.D2;
+      if constexpr (R == 16) {
+        const uint2 q = in && 4 * t < a.r ? *reinterpret_cast<const uint2*>(v + 4 * t) : make_uint2(0u, 0u);
+        b[j][0][0] = q.x, b[j][0][1] = q.y;
+      } else {
+#pragma unroll
+        for (int w = 0; w < KS / 2; ++w) {
+          const uint4 q = in && 32 * w + 8 * t < a.r ? *reinterpret_cast<const uint4*>(v + 32 * w + 8 * t)
+                                                     : make_uint4(0u, 0u, 0u, 0u);
+          b[j][2 * w][0] = q.x, b[j][2 * w][1] = q.y, b[j][2 * w + 1][0] = q.z, b[j][2 * w + 1][1] = q.w;
+        }
+      }
+    }
+    const int64_t col = (int64_t)ch * 32 + 8 * t;
+#pragma unroll 2
+    for (int mt = 0; mt < n_tiles; ++mt) {
+      const int ra = mt * 16 + g, rb = ra + 8;
+      const int64_t ma = rowid[ra], mb = rowid[rb];
+      uint4 old[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+      if (base) {
+        old[0] = load_row8(base + ma * p.ldb, col, ra < rows ? a.D2 : 0, p.vec_out);
+        old[1] = load_row8(base + mb * p.ldb, col, rb < rows ? a.D2 : 0, p.vec_out);
+      }
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = fill;
+      float mul_a = 1.0f, mul_b = 1.0f;
+      if (!none) {
+        if constexpr (DT == RQ_F16) mul_a = rowmul[ra], mul_b = rowmul[rb];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const unsigned char* ma_ = mids + (half * a.tile + ra) * PM;
+          const unsigned char* mb_ = mids + (half * a.tile + rb) * PM;
+          if constexpr (R == 16) {
+            const uint2 qa = *reinterpret_cast<const uint2*>(ma_ + 8 * t), qb = *reinterpret_cast<const uint2*>(mb_ + 8 * t);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][0][0], b[j][0][1]);
+          } else {
+#pragma unroll
+            for (int w = 0; w < KS / 2; ++w) {
+              const uint4 qa = *reinterpret_cast<const uint4*>(ma_ + 64 * w + 16 * t);
+              const uint4 qb = *reinterpret_cast<const uint4*>(mb_ + 64 * w + 16 * t);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][2 * w][0], b[j][2 * w][1]);
+                Mma16816<DT>::run(acc[j], qa.z, qb.z, qa.w, qb.w, b[j][2 * w + 1][0], b[j][2 * w + 1][1]);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if ((h ? rb : ra) >= rows) continue;
+        const float mul = h ? mul_b : mul_a;
+        const uint32_t w[4] = {old[h].x, old[h].y, old[h].z, old[h].w};
+        uint32_t res[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
+          res[j] = pack2<DT>(fmaf(acc[j][2 * h], mul, DType<DT>::to_f32(*reinterpret_cast<const T*>(&lo))),
+                             fmaf(acc[j][2 * h + 1], mul, DType<DT>::to_f32(*reinterpret_cast<const T*>(&hi))));
+        }
+        uint16_t* dst = out + (h ? mb : ma) * p.ldo + col;
+        if (p.vec_out && col + 8 <= a.D2) {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(res[0], res[1], res[2], res[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < a.D2) dst[i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
+        }
+      }
+    }
+  }
+}
+
+static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+
+template <int DT, int R, int NW>
+static int launch_apply(const ApplyArgs& p, int64_t tiles, int csize, cudaStream_t st) {
+  const int WK = kApWarps / (p.a.tile / 16);
+  const size_t stage = (size_t)2 * NW * WK * kApWin * ap_pitch_u(R);
+  const size_t smem = stage + (size_t)2 * p.a.tile * ap_pitch_m(R) + 128 * 8;
+  auto* kern = adapters_apply_k<DT, R, NW>;
+  const int rc = ensure_smem_limit((const void*)kern, smem);
+  if (rc != RQ_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * csize));
+  cfg.blockDim = dim3(kApThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = csize;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
   }
   return check_launch();
+}
+
+int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const void* U, const void* V,
+                   const float* scaling, const void* base, int64_t ldb, float* mid, void* out, int64_t ldo,
+                   cudaStream_t st) {
+  AdapterRows a = a0;
+  if (!a.plan) a.tile = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 1024 ? 64 : 128;
+  const int64_t tiles = a.plan ? plan_max_tiles(a.M, a.count, a.tile) : (a.M + a.tile - 1) / a.tile;
+  const ApplyArgs p{a,   in,  ldin, U,   V,  scaling, base, ldb, mid, out, ldo, rows16b(in, ldin) || a.D1 == 0,
+                    rows16b(out, ldo) && (!base || rows16b(base, ldb))};
+  const int csize = 8;
+#define RQ_APPLY(DT, R) \
+  return a.tile >= 64 ? launch_apply<DT, R, 4>(p, tiles, csize, st) : launch_apply<DT, R, 1>(p, tiles, csize, st)
+#define RQ_APPLY_R(DT)                 \
+  do {                                 \
+    if (a.r <= 16) RQ_APPLY(DT, 16);   \
+    if (a.r <= 32) RQ_APPLY(DT, 32);   \
+    if (a.r <= 64) RQ_APPLY(DT, 64);   \
+    RQ_APPLY(DT, 128);                 \
+  } while (0)
+  if (a.dt == RQ_BF16) RQ_APPLY_R(RQ_BF16);
+  RQ_APPLY_R(RQ_F16);
+#undef RQ_APPLY_R
+#undef RQ_APPLY
 }
 
 // ------------------------------------------------------------------- grad
