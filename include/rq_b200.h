@@ -329,8 +329,8 @@ RQ_API int rq_adapter_plan(const void* ids, int wide, int64_t rows, int count, i
 
 /* out[m, :] = base[m, :] + mid[m, :] . V_a^T,  mid[m, :] = scaling[a] * (in[m, :] . U_a)
  * for in [M, D1], out and base [M, D2] (base may be NULL: zero, or out itself),
- * U [count, D1, r], V [count, D2, r], mid [M, r] fp32 (written; the backward
- * needs it).  Forward: U = A, V = B, in = x.  Input gradient: U = B, V = A,
+ * U [count, D1, r], V [count, D2, r], mid [M, r] fp32 (written for
+ * the backward; may be NULL).  Forward: U = A, V = B, in = x.  Input gradient: U = B, V = A,
  * in = dy.  Everything is accumulated in fp32 and rounded once.  plan NULL:
  * every row uses adapter 0.  Row strides (ld*) in elements, columns
  * contiguous. */

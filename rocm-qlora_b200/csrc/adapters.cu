@@ -194,7 +194,8 @@ template <int DT>
 __device__ __forceinline__ void split16(float v, uint16_t* hi, uint16_t* lo) {
   using T = typename DType<DT>::T;
   const T h = DType<DT>::from_f32(v);
-  const T l = DType<DT>::from_f32(v - DType<DT>::to_f32(h));
+  const float d = v - DType<DT>::to_f32(h);
+  const T l = DType<DT>::from_f32(fabsf(v) < INFINITY ? d : 0.0f);  // an infinity stays one, NaN is in h
   *hi = *reinterpret_cast<const uint16_t*>(&h);
   *lo = *reinterpret_cast<const uint16_t*>(&l);
 }
@@ -547,35 +548,233 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
 
 // ------------------------------------------------------------------- grad
 
-// G_a[d, j] = sum over the rows of a of z[m, d] mid[m, j]; z either 16-bit
-// rows or 8-bit codes with one scale a 128 columns.
+constexpr int kGrThreads = 256, kGrWarps = kGrThreads / 32;
+constexpr int kGrCols = 128;                                 // columns of a CTA: one block of 8-bit codes
+constexpr int kGrSmem = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
+
+struct GradArgs {
+  AdapterRows a;
+  const void* z;
+  int64_t ldz;
+  const float* zscale;
+  int64_t lds;
+  const float* mid;
+  void* G;
+  int groups;  // warps along the rank, 16 of it each: 1, 2, 4 or 8
+  bool vec;
+};
+
+// Two packed 16-bit values of codes a (low) and b (high), exact.  bf16: 0x43qq
+// without the code's sign bit is 128 + (q mod 128), and 0x4300 with it alone
+// is 128 for q >= 0 and 256 for q < 0; their difference is q.  fp16: 0x64uu
+// with u = q + 128 is 1024 + u.
 template <int DT>
-__global__ void __launch_bounds__(128) adapter_grad_k(AdapterRows a, const void* __restrict__ z, int64_t ldz,
-                                                      const float* __restrict__ zscale, int64_t lds,
-                                                      const float* __restrict__ mid, void* __restrict__ G) {
-  using T = typename DType<DT>::T;
-  const int g = blockIdx.x, j = threadIdx.x;
-  const int64_t d = blockIdx.y;
-  if (j >= a.r) return;
-  const int first = a.plan ? a.plan[1 + g] : 0, last = a.plan ? a.plan[2 + g] : (int)a.M;
-  const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
-  float acc = 0.0f;
-  for (int p = first; p < last; ++p) {
-    const int64_t m = order ? order[p] : p;
-    const float v = zscale ? (float)static_cast<const int8_t*>(z)[m * ldz + d] * zscale[m * lds + d / 128]
-                           : DType<DT>::to_f32(static_cast<const T*>(z)[m * ldz + d]);
-    acc = fmaf(v, mid[m * a.r + j], acc);
+__device__ __forceinline__ uint32_t codes2(uint32_t two) {  // bytes: a, ?, b, ? -> halves
+  if constexpr (DT == RQ_BF16) {
+    const uint32_t w = (two & 0x00ff00ffu) | 0x43004300u, x = w & 0xff7fff7fu, y = w & 0xff80ff80u;
+    const __nv_bfloat162 d =
+        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  } else {
+    const uint32_t w = ((two & 0x00ff00ffu) ^ 0x00800080u) | 0x64006400u, y = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&d);
   }
-  static_cast<T*>(G)[((int64_t)g * a.D1 + d) * a.r + j] = DType<DT>::from_f32(acc);
+}
+
+// G_a[d, j] = sum over the rows m of a of z[m, d] mid[m, j].
+//
+// One CTA sums 128 columns of one adapter; its warps split the rows (and the
+// rank, 16 each), and the CTAs of a cluster split the rows again.  Sums meet
+// in shared and distributed shared memory in warp and rank order, so equal
+// inputs give equal bits, without atomics or a workspace.
+//
+// The reduction runs over rows, so the MMA's k index is the row: a lane holds
+// four rows (4t .. 4t+3 of 16) and, of each, 8 + 8 columns straight from
+// global memory; a pair of rows of one column is one byte permute, and the
+// columns are dealt to the MMA's m index so that this works out.  z is read
+// once (HBM bound up to rank 16; above, warps that share rows read them
+// through L1 and the tensor cores' rate takes over).  Codes become 16-bit
+// values exactly; their scale multiplies the other operand, mid, in fp32,
+// which then enters as two 16-bit halves as in the row products.
+template <int DT, bool CODES>
+__global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_constant__ GradArgs p) {
+  using T = typename DType<DT>::T;
+  extern __shared__ __align__(16) float sums[];
+  const AdapterRows& a = p.a;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
+  const int block = (int)(blockIdx.x / csize), adapter = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rg = warp % p.groups, mw = warp / p.groups, MW = kGrWarps / p.groups, R16 = p.groups * 16;
+
+  const int first = a.plan ? a.plan[1 + adapter] : 0, last = a.plan ? a.plan[2 + adapter] : (int)a.M;
+  const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
+  const int64_t c0 = (int64_t)block * kGrCols + 8 * g;
+  const int j0 = rg * 16 + 2 * g;  // this lane's pair of ranks: n index g of both n-tiles
+  float acc[8][2][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.0f;
+  int ex_now = 0;          // fp16: biased exponent that mid is scaled down by
+  float mul = 1.0f;
+
+  const int stride = csize * MW * 16;
+  for (int at = first + (crank * MW + mw) * 16; at < last; at += stride) {
+    uint4 z[4][2];
+    float2 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int place = at + 4 * t + i;
+      z[i][0] = z[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      v[i] = make_float2(0.0f, 0.0f);
+      if (place < last) {
+        const int64_t m = order ? order[place] : place;
+        if constexpr (CODES) {
+          const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0;
+          const uint2 q0 = *reinterpret_cast<const uint2*>(row), q1 = *reinterpret_cast<const uint2*>(row + 64);
+          z[i][0].x = q0.x, z[i][0].y = q0.y, z[i][1].x = q1.x, z[i][1].y = q1.y;
+        } else {
+          const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
+          z[i][0] = load_row8(row, c0, a.D1, p.vec);
+          z[i][1] = load_row8(row, c0 + 64, a.D1, p.vec);
+        }
+        if (j0 < a.r) {
+          v[i] = *reinterpret_cast<const float2*>(p.mid + m * a.r + j0);
+          if constexpr (CODES) {
+            const float s = p.zscale[m * p.lds + block];
+            v[i].x *= s, v[i].y *= s;
+          }
+        }
+      }
+    }
+    if constexpr (DT == RQ_F16) {
+      // keep mid near 2^14 as fp16: when a step's largest value passes the
+      // scale in use, the sums so far are scaled down to the new one
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top = max(top, max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu));
+      const int ex = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
+      if (ex > ex_now && ex > 30 && ex < 255) {
+        if (ex_now) {
+          const float down = ex - ex_now < 126 ? __uint_as_float((uint32_t)(127 - (ex - ex_now)) << 23) : 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][n][e] *= down;
+        }
+        ex_now = ex;
+        mul = __uint_as_float((uint32_t)(268 - ex) << 23);
+      }
+    }
+    // B fragments: halves of mid at (rows 4t, 4t+1 | 4t+2, 4t+3) and rank j0 + n-tile
+    uint32_t b[2][2][2];  // [half][n-tile][k pair]
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float e = n ? v[2 * k].y : v[2 * k].x, f = n ? v[2 * k + 1].y : v[2 * k + 1].x;
+        uint16_t h0, l0, h1, l1;
+        split16<DT>(e * mul, &h0, &l0);
+        split16<DT>(f * mul, &h1, &l1);
+        b[0][n][k] = h0 | ((uint32_t)h1 << 16);
+        b[1][n][k] = l0 | ((uint32_t)l1 << 16);
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t f[4];  // (columns, columns + 64) x (rows 4t, 4t+1 | 4t+2, 4t+3)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 &x = z[2 * k][h], &y = z[2 * k + 1][h];
+          if constexpr (CODES) {
+            const uint32_t w0 = i < 4 ? x.x : x.y, w1 = i < 4 ? y.x : y.y;
+            f[2 * k + h] = codes2<DT>(__byte_perm(w0, w1, (i & 3) | ((4 + (i & 3)) << 8)));
+          } else {
+            const uint32_t w0 = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;
+            const uint32_t w1 = i < 2 ? y.x : i < 4 ? y.y : i < 6 ? y.z : y.w;
+            f[2 * k + h] = __byte_perm(w0, w1, i & 1 ? 0x7632 : 0x5410);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          Mma16816<DT>::run(acc[i][n], f[0], f[1], f[2], f[3], b[half][n][0], b[half][n][1]);
+    }
+  }
+
+  // this warp's sums: column 8 g + i (+ 64) at row 8 i + g (+ 64), ranks 4t .. 4t+3
+  const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
+  float* mine = sums + mw * kGrCols * R16 + rg * 16 + 4 * t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<float4*>(mine + (8 * i + g + 64 * h) * R16) =
+          make_float4(acc[i][0][2 * h] * back, acc[i][1][2 * h] * back, acc[i][0][2 * h + 1] * back,
+                      acc[i][1][2 * h + 1] * back);
+  __syncthreads();
+  for (int i = tid; i < kGrCols * R16 / 4; i += kGrThreads) {
+    float4 s = reinterpret_cast<const float4*>(sums)[i];
+    for (int w = 1; w < MW; ++w) {
+      const float4 q = reinterpret_cast<const float4*>(sums + w * kGrCols * R16)[i];
+      s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+    }
+    reinterpret_cast<float4*>(sums)[i] = s;
+  }
+  cluster.sync();
+  // 8 ranks of a column are one 16-byte store; the cluster's CTAs take the columns in turn
+  const int units = R16 / 8;
+  for (int i = crank * kGrThreads + tid; i < kGrCols * units; i += csize * kGrThreads) {
+    const int at = i / units, j = (i - at * units) * 8;
+    const int64_t d = (int64_t)block * kGrCols + 8 * (at & 7) + ((at >> 3) & 7) + (at & 64);
+    if (d >= a.D1 || j >= a.r) continue;
+    float s[8] = {};
+    for (int c = 0; c < csize; ++c) {
+      const float* src = cluster.map_shared_rank(sums, c) + at * R16 + j;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += src[e];
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
+        make_uint4(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]), pack2<DT>(s[4], s[5]), pack2<DT>(s[6], s[7]));
+  }
+  cluster.sync();  // the others have read this CTA's sums
 }
 
 int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
                   void* G, cudaStream_t st) {
-  const dim3 grid((unsigned)a.count, (unsigned)a.D1);
-  if (a.dt == RQ_BF16)
-    adapter_grad_k<RQ_BF16><<<grid, 128, 0, st>>>(a, z, ldz, zscale, lds, mid, G);
-  else
-    adapter_grad_k<RQ_F16><<<grid, 128, 0, st>>>(a, z, ldz, zscale, lds, mid, G);
+  GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8, rows16b(z, ldz)};
+  // Rows are split over a cluster until the grid holds two CTAs an SM, as
+  // long as a warp keeps two steps of 16 rows of an adapter of mean size.
+  const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols, each = a.M / a.count * p.groups / (kGrWarps * 32);
+  int csize = 1;
+  while (csize < 8 && csize * 2 <= each && blocks * csize < 2 * num_sms()) csize *= 2;
+  auto* kern = a.dt == RQ_BF16 ? (zscale ? adapters_grad_k<RQ_BF16, true> : adapters_grad_k<RQ_BF16, false>)
+                               : (zscale ? adapters_grad_k<RQ_F16, true> : adapters_grad_k<RQ_F16, false>);
+  const int rc = ensure_smem_limit((const void*)kern, kGrSmem);
+  if (rc != RQ_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * csize), (unsigned)a.count);
+  cfg.blockDim = dim3(kGrThreads);
+  cfg.dynamicSmemBytes = kGrSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = csize;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
+  }
   return check_launch();
 }
 

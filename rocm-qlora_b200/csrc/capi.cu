@@ -353,7 +353,7 @@ int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const void* 
   if (rc != RQ_OK) return rc;
   if (!fits(D1) || !fits(D2) || r < 8 || r > 128 || r % 8) return RQ_ERR_INVALID;
   if (M == 0) return RQ_OK;
-  if (!mid || !scaling || (D1 > 0 && (!in || !U)) || (D2 > 0 && (!V || !out))) return RQ_ERR_INVALID;
+  if (!scaling || (D1 > 0 && (!in || !U)) || (D2 > 0 && (!V || !out))) return RQ_ERR_INVALID;
   if ((M > 1) && (ld_in < D1 || ld_out < D2 || (base && ld_base < D2))) return RQ_ERR_INVALID;
   if ((uintptr_t)in % 2 || (uintptr_t)base % 2 || (uintptr_t)out % 2 || (uintptr_t)U % 16 || (uintptr_t)V % 16 ||
       (uintptr_t)mid % 16 || (uintptr_t)scaling % 4)
