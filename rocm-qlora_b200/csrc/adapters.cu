@@ -157,12 +157,17 @@ struct ApplyArgs {
   float* mid;
   void* out;
   int64_t ldo;
-  bool vec_in, vec_out;  // 16-byte accesses to the rows of in, and of base and out
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool take) {
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+template <int BYTES>  // 4 or 8
+__device__ __forceinline__ void cp_async_small(void* dst, const void* src, bool take) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(d), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
@@ -178,9 +183,11 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&d)[4], const void* p)
                : "memory");
 }
 
-// 8 consecutive 16-bit values of a row from column c (zero past `cols`).
-__device__ __forceinline__ uint4 load_row8(const uint16_t* row, int64_t c, int64_t cols, bool vec) {
-  if (vec && c + 8 <= cols) return *reinterpret_cast<const uint4*>(row + c);
+// 8 consecutive 16-bit values of a row from column c, zero past `cols`.  VEC:
+// the row is 16-byte aligned and cols and c are multiples of 8.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_row8(const uint16_t* row, int64_t c, int64_t cols) {
+  if constexpr (VEC) return c < cols ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -190,14 +197,86 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int64_t c, int64
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two fp32 values rounded to 16 bits, packed (low, high): one conversion.
 template <int DT>
-__device__ __forceinline__ void split16(float v, uint16_t* hi, uint16_t* lo) {
-  using T = typename DType<DT>::T;
-  const T h = DType<DT>::from_f32(v);
-  const float d = v - DType<DT>::to_f32(h);
-  const T l = DType<DT>::from_f32(fabsf(v) < INFINITY ? d : 0.0f);  // an infinity stays one, NaN is in h
-  *hi = *reinterpret_cast<const uint16_t*>(&h);
-  *lo = *reinterpret_cast<const uint16_t*>(&l);
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {
+  if constexpr (DT == RQ_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float2 unpair16(uint32_t w) {
+  if constexpr (DT == RQ_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Two values as the sum of two 16-bit halves each.  An infinity keeps a zero
+// remainder, so that it stays an infinity; NaN is in the first half.
+template <int DT>
+__device__ __forceinline__ void split16x2(float x, float y, uint32_t* hi, uint32_t* lo) {
+  *hi = pair16<DT>(x, y);
+  const float2 h = unpair16<DT>(*hi);
+  *lo = pair16<DT>(fabsf(x) < INFINITY ? x - h.x : 0.0f, fabsf(y) < INFINITY ? y - h.y : 0.0f);
+}
+
+template <int N>
+__device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[N]) {
+  if constexpr (N == 1) *static_cast<uint32_t*>(p) = w[0];
+  if constexpr (N == 2) *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Columns [begin, end) of a 16-byte aligned row (both multiples of 8) into L2.
+__device__ __forceinline__ void prefetch_row(const uint16_t* row, int64_t begin, int64_t end) {
+  if (begin < end)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(row + begin), "r"((uint32_t)(end - begin) * 2)
+                 : "memory");
+}
+
+// The sum over the cluster's CTAs, in rank order, of what each has at p.  All
+// loads are issued before the first add.
+template <class V>
+__device__ __forceinline__ V cluster_sum(cg::cluster_group& cluster, float* p, int csize) {
+  constexpr int E = sizeof(V) / 4;
+  V q[8], s;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const V*>(cluster.map_shared_rank(p, c < csize ? c : 0));
+  float* f = reinterpret_cast<float*>(&s);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    f[e] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) f[e] += c < csize ? reinterpret_cast<const float*>(&q[c])[e] : 0.0f;
+  }
+  return s;
+}
+
+template <class P>
+static int launch_cluster(void (*kern)(P), const P& args, dim3 grid, int threads, size_t smem, int csize,
+                          cudaStream_t st) {
+  const int rc = ensure_smem_limit((const void*)kern, smem);
+  if (rc != RQ_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = csize;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
+  }
+  return check_launch();
 }
 
 // One cluster computes one tile: `tile` rows (16 to 128) of one adapter.
@@ -224,7 +303,7 @@ __device__ __forceinline__ void split16(float v, uint16_t* hi, uint16_t* lo) {
 // the order that ldmatrix then needs.  V's columns are permuted the same way
 // among the MMA's n index, so that a lane ends with 8 consecutive output
 // columns: one 16-byte load of base and one store.
-template <int DT, int R, int NW>
+template <int DT, int R, int NW, bool VEC>
 __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(const __grid_constant__ ApplyArgs p) {
   using T = typename DType<DT>::T;
   constexpr int NT = R / 8;               // n-tiles of the first product
@@ -243,7 +322,9 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   if (a.plan) {
     if (tile_id >= a.plan[0]) return;
     const int4 e = reinterpret_cast<const int4*>(a.plan + plan_tiles_at(a.count))[tile_id];
-    group = e.x, first = e.y, rows = e.z;
+    // held inside the batch, so that a plan that is not one cannot reach outside it
+    group = min(max(e.x, 0), a.count + 1), first = min(max(e.y, 0), (int)a.M - 1);
+    rows = min(max(e.z, 1), min(a.tile, (int)a.M - first));
     order = a.plan + plan_rows_at(a.M, a.count, a.tile);
   } else {
     group = 0, first = tile_id * a.tile;
@@ -260,19 +341,30 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   int* rowid = reinterpret_cast<int*>(rowmul + 128);                  // [tile]
   for (int i = tid; i < a.tile; i += kApThreads) {
     const int at = first + min(i, rows - 1);
-    rowid[i] = order ? order[at] : at;
+    rowid[i] = order ? min(max(order[at], 0), (int)a.M - 1) : at;
   }
   __syncthreads();
+  const int chunks2 = (int)((a.D2 + 31) / 32), per2 = (chunks2 + csize - 1) / csize;
+  const int ch_begin = min(chunks2, crank * per2), ch_end = min(chunks2, ch_begin + per2);
+  const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
+  const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
+  const uint16_t* in = static_cast<const uint16_t*>(p.in);
+  const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  if constexpr (VEC) {
+    // this CTA's share of the rows on its way into L2, ahead of the loads
+    if (tid < rows && !none)
+      prefetch_row(in + (int64_t)rowid[tid] * p.ldin, (int64_t)w_begin * kApWin, min((int64_t)w_end * kApWin, a.D1));
+    if (tid >= 128 && tid - 128 < rows && base)
+      prefetch_row(base + (int64_t)rowid[tid - 128] * p.ldb, (int64_t)ch_begin * 32, min((int64_t)ch_end * 32, a.D2));
+  }
 
   if (!none) {
     // ---- partial sums over this CTA's input columns
     const uint16_t* U = static_cast<const uint16_t*>(p.U) + (int64_t)group * a.D1 * a.r;
-    const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
-    const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
     const int step = NW * WK, chunks = (w_end - w_begin + step - 1) / step;
     const int wm = warp % WM, wk = warp / WM;
-    const uint16_t* xa = static_cast<const uint16_t*>(p.in) + (int64_t)rowid[wm * 16 + g] * p.ldin;
-    const uint16_t* xb = static_cast<const uint16_t*>(p.in) + (int64_t)rowid[wm * 16 + g + 8] * p.ldin;
+    const uint16_t* xa = in + (int64_t)rowid[wm * 16 + g] * p.ldin;
+    const uint16_t* xb = in + (int64_t)rowid[wm * 16 + g + 8] * p.ldin;
 
     auto stage = [&](int c) {  // U's rows of chunk c, each at the place its window's order gives it
       unsigned char* dst = smem + (c & 1) * KC * PU;
@@ -290,8 +382,8 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       for (int w = 0; w < NW; ++w) {
         const int win = w_begin + c * step + wk * NW + w;
         const int64_t col = win < w_end ? (int64_t)win * kApWin + t * 8 : a.D1;
-        x[w][0] = load_row8(xa, col, a.D1, p.vec_in);
-        x[w][1] = load_row8(xb, col, a.D1, p.vec_in);
+        x[w][0] = load_row8<VEC>(xa, col, a.D1);
+        x[w][1] = load_row8<VEC>(xb, col, a.D1);
       }
     };
     float acc[NT][4];
@@ -349,51 +441,45 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       }
     }
     cluster.sync();
-    // 16 lanes a row, this CTA's share of the rows; the result goes to every CTA
-    constexpr int E = R / 16;
-    const int share = (a.tile + csize - 1) / csize, l16 = tid & 15;
+    // LR lanes a row, this CTA's share of the rows; the result goes to every CTA
+    constexpr int LR = R == 16 ? 8 : 16, E = R / LR;
+    const int share = (a.tile + csize - 1) / csize, l = tid % LR;
     const float s = p.scaling[group];
-    for (int i0 = 0; i0 < share; i0 += kApThreads / 16) {
-      const int i = i0 + tid / 16, row = crank * share + i;
+    for (int i0 = 0; i0 < share; i0 += kApThreads / LR) {
+      const int i = i0 + tid / LR, row = crank * share + i;
       const bool on = i < share && row < a.tile;
-      float v[E];
+      __align__(16) float v[E];
+      float* src = part + (on ? row : 0) * R + l * E;
+      if constexpr (E == 2) *reinterpret_cast<float2*>(v) = cluster_sum<float2>(cluster, src, csize);
+#pragma unroll
+      for (int e = 0; e + 4 <= E; e += 4) *reinterpret_cast<float4*>(v + e) = cluster_sum<float4>(cluster, src + e, csize);
       float top = 0.0f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = 0.0f;
-      if (on) {
-        for (int c = 0; c < csize; ++c) {
-          const float* src = cluster.map_shared_rank(part, c) + row * R + l16 * E;
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[e] += src[e];
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          v[e] *= s;
-          top = fmaxf(top, fabsf(v[e]));
-          if (p.mid && row < rows && l16 * E + e < a.r) p.mid[(int64_t)rowid[row] * a.r + l16 * E + e] = v[e];
-        }
+      for (int e = 0; e < E; ++e) {
+        v[e] *= s;
+        top = fmaxf(top, fabsf(v[e]));
+        if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)rowid[row] * a.r + l * E + e] = v[e];
       }
       float mul = 1.0f, back = 1.0f;
       if constexpr (DT == RQ_F16) {
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int ex = (int)(__float_as_uint(top) >> 23);  // biased exponent; 255: not finite, small: leave
         if (ex > 30 && ex < 255) {
-          mul = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
+          mul = __uint_as_float((uint32_t)(268 - ex) << 23);
           back = __uint_as_float((uint32_t)(ex - 14) << 23);
         }
       }
       if (on) {
-        __align__(16) uint16_t hi[E], lo[E];
+        __align__(16) uint32_t hi[E / 2], lo[E / 2];
 #pragma unroll
-        for (int e = 0; e < E; ++e) split16<DT>(v[e] * mul, &hi[e], &lo[e]);
+        for (int e = 0; e < E; e += 2) split16x2<DT>(v[e] * mul, v[e + 1] * mul, &hi[e / 2], &lo[e / 2]);
+        unsigned char* at = mids + row * PM + l * E * 2;
         for (int c = 0; c < csize; ++c) {
-          unsigned char* m = cluster.map_shared_rank(mids, c) + row * PM + l16 * E * 2;
-          uint16_t* h = reinterpret_cast<uint16_t*>(m);
-          uint16_t* l = reinterpret_cast<uint16_t*>(m + a.tile * PM);
-#pragma unroll
-          for (int e = 0; e < E; ++e) h[e] = hi[e], l[e] = lo[e];
-          if (l16 == 0) cluster.map_shared_rank(rowmul, c)[row] = back;
+          unsigned char* m = cluster.map_shared_rank(at, c);
+          store_words<E / 2>(m, hi);
+          store_words<E / 2>(m + a.tile * PM, lo);
+          if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(rowmul, c)[row] = back;
         }
       }
     }
@@ -407,58 +493,59 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   // ---- this warp's output columns, 32 at a time, all rows of the tile
   const int n_tiles = (rows + 15) / 16;
   const uint16_t* V = static_cast<const uint16_t*>(p.V) + (none ? 0 : (int64_t)group * a.D2 * a.r);
-  const uint16_t* base = static_cast<const uint16_t*>(p.base);
   uint16_t* out = static_cast<uint16_t*>(p.out);
-  const int chunks2 = (int)((a.D2 + 31) / 32);
-  for (int ch = crank * kApWarps + warp; ch < chunks2; ch += csize * kApWarps) {
+  for (int ch = ch_begin + warp; ch < ch_end; ch += kApWarps) {
+    const int64_t col = (int64_t)ch * 32 + 8 * t;
+    auto fetch = [&](uint4 (&old)[2], int mt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        old[h] = base && mt < n_tiles ? load_row8<VEC>(base + (int64_t)rowid[mt * 16 + 8 * h + g] * p.ldb, col, a.D2)
+                                      : make_uint4(0u, 0u, 0u, 0u);
+    };
+    uint4 ahead[2][2];  // base of the next two m-tiles
+    fetch(ahead[0], 0);
+    fetch(ahead[1], 1);
     // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
     uint32_t b[4][KS][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t n = (int64_t)ch * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
       const uint16_t* v = V + n * a.r;
-      const bool in = !none && n < a.D2;
+      const bool ok = !none && n < a.D2;
       if constexpr (R == 16) {
-        const uint2 q = in && 4 * t < a.r ? *reinterpret_cast<const uint2*>(v + 4 * t) : make_uint2(0u, 0u);
+        const uint2 q = ok && 4 * t < a.r ? *reinterpret_cast<const uint2*>(v + 4 * t) : make_uint2(0u, 0u);
         b[j][0][0] = q.x, b[j][0][1] = q.y;
       } else {
 #pragma unroll
         for (int w = 0; w < KS / 2; ++w) {
-          const uint4 q = in && 32 * w + 8 * t < a.r ? *reinterpret_cast<const uint4*>(v + 32 * w + 8 * t)
+          const uint4 q = ok && 32 * w + 8 * t < a.r ? *reinterpret_cast<const uint4*>(v + 32 * w + 8 * t)
                                                      : make_uint4(0u, 0u, 0u, 0u);
           b[j][2 * w][0] = q.x, b[j][2 * w][1] = q.y, b[j][2 * w + 1][0] = q.z, b[j][2 * w + 1][1] = q.w;
         }
       }
     }
-    const int64_t col = (int64_t)ch * 32 + 8 * t;
-#pragma unroll 2
     for (int mt = 0; mt < n_tiles; ++mt) {
-      const int ra = mt * 16 + g, rb = ra + 8;
-      const int64_t ma = rowid[ra], mb = rowid[rb];
-      uint4 old[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (base) {
-        old[0] = load_row8(base + ma * p.ldb, col, ra < rows ? a.D2 : 0, p.vec_out);
-        old[1] = load_row8(base + mb * p.ldb, col, rb < rows ? a.D2 : 0, p.vec_out);
-      }
+      const int ra = mt * 16 + g;
+      uint4 old[2] = {ahead[0][0], ahead[0][1]};
+      ahead[0][0] = ahead[1][0], ahead[0][1] = ahead[1][1];
+      fetch(ahead[1], mt + 2);
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = fill;
-      float mul_a = 1.0f, mul_b = 1.0f;
       if (!none) {
-        if constexpr (DT == RQ_F16) mul_a = rowmul[ra], mul_b = rowmul[rb];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const unsigned char* ma_ = mids + (half * a.tile + ra) * PM;
-          const unsigned char* mb_ = mids + (half * a.tile + rb) * PM;
+          const unsigned char* ma = mids + (half * a.tile + ra) * PM;
+          const unsigned char* mb = ma + 8 * PM;
           if constexpr (R == 16) {
-            const uint2 qa = *reinterpret_cast<const uint2*>(ma_ + 8 * t), qb = *reinterpret_cast<const uint2*>(mb_ + 8 * t);
+            const uint2 qa = *reinterpret_cast<const uint2*>(ma + 8 * t), qb = *reinterpret_cast<const uint2*>(mb + 8 * t);
 #pragma unroll
             for (int j = 0; j < 4; ++j) Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][0][0], b[j][0][1]);
           } else {
 #pragma unroll
             for (int w = 0; w < KS / 2; ++w) {
-              const uint4 qa = *reinterpret_cast<const uint4*>(ma_ + 64 * w + 16 * t);
-              const uint4 qb = *reinterpret_cast<const uint4*>(mb_ + 64 * w + 16 * t);
+              const uint4 qa = *reinterpret_cast<const uint4*>(ma + 64 * w + 16 * t);
+              const uint4 qb = *reinterpret_cast<const uint4*>(mb + 64 * w + 16 * t);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][2 * w][0], b[j][2 * w][1]);
@@ -470,19 +557,20 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if ((h ? rb : ra) >= rows) continue;
-        const float mul = h ? mul_b : mul_a;
+        const int row = ra + 8 * h;
+        if (row >= rows) continue;
+        const float mul = DT == RQ_F16 && !none ? rowmul[row] : 1.0f;
         const uint32_t w[4] = {old[h].x, old[h].y, old[h].z, old[h].w};
         uint32_t res[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint16_t lo = (uint16_t)w[j], hi = (uint16_t)(w[j] >> 16);
-          res[j] = pack2<DT>(fmaf(acc[j][2 * h], mul, DType<DT>::to_f32(*reinterpret_cast<const T*>(&lo))),
-                             fmaf(acc[j][2 * h + 1], mul, DType<DT>::to_f32(*reinterpret_cast<const T*>(&hi))));
+          const float2 o = unpair16<DT>(w[j]);
+          res[j] = DT == RQ_F16 ? pair16<DT>(fmaf(acc[j][2 * h], mul, o.x), fmaf(acc[j][2 * h + 1], mul, o.y))
+                                : pair16<DT>(acc[j][2 * h] + o.x, acc[j][2 * h + 1] + o.y);
         }
-        uint16_t* dst = out + (h ? mb : ma) * p.ldo + col;
-        if (p.vec_out && col + 8 <= a.D2) {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(res[0], res[1], res[2], res[3]);
+        uint16_t* dst = out + (int64_t)rowid[row] * p.ldo + col;
+        if constexpr (VEC) {
+          if (col < a.D2) *reinterpret_cast<uint4*>(dst) = make_uint4(res[0], res[1], res[2], res[3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -496,30 +584,20 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
 static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
 
 template <int DT, int R, int NW>
-static int launch_apply(const ApplyArgs& p, int64_t tiles, int csize, cudaStream_t st) {
+static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, int csize, cudaStream_t st) {
   const int WK = kApWarps / (p.a.tile / 16);
   const size_t stage = (size_t)2 * NW * WK * kApWin * ap_pitch_u(R);
   const size_t smem = stage + (size_t)2 * p.a.tile * ap_pitch_m(R) + 128 * 8;
-  auto* kern = adapters_apply_k<DT, R, NW>;
-  const int rc = ensure_smem_limit((const void*)kern, smem);
-  if (rc != RQ_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * csize));
-  cfg.blockDim = dim3(kApThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return RQ_ERR_CUDA;
-  }
-  return check_launch();
+  return launch_cluster(vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>, p,
+                        dim3((unsigned)(tiles * csize)), kApThreads, smem, csize, st);
+}
+
+template <int DT, int NW>
+static int launch_apply_r(const ApplyArgs& p, bool vec, int64_t tiles, int csize, cudaStream_t st) {
+  if (p.a.r <= 16) return launch_apply<DT, 16, NW>(p, vec, tiles, csize, st);
+  if (p.a.r <= 32) return launch_apply<DT, 32, NW>(p, vec, tiles, csize, st);
+  if (p.a.r <= 64) return launch_apply<DT, 64, NW>(p, vec, tiles, csize, st);
+  return launch_apply<DT, 128, NW>(p, vec, tiles, csize, st);
 }
 
 int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const void* U, const void* V,
@@ -528,29 +606,27 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
   AdapterRows a = a0;
   if (!a.plan) a.tile = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 1024 ? 64 : 128;
   const int64_t tiles = a.plan ? plan_max_tiles(a.M, a.count, a.tile) : (a.M + a.tile - 1) / a.tile;
-  const ApplyArgs p{a,   in,  ldin, U,   V,  scaling, base, ldb, mid, out, ldo, rows16b(in, ldin) || a.D1 == 0,
-                    rows16b(out, ldo) && (!base || rows16b(base, ldb))};
-  const int csize = 8;
-#define RQ_APPLY(DT, R) \
-  return a.tile >= 64 ? launch_apply<DT, R, 4>(p, tiles, csize, st) : launch_apply<DT, R, 1>(p, tiles, csize, st)
-#define RQ_APPLY_R(DT)                 \
-  do {                                 \
-    if (a.r <= 16) RQ_APPLY(DT, 16);   \
-    if (a.r <= 32) RQ_APPLY(DT, 32);   \
-    if (a.r <= 64) RQ_APPLY(DT, 64);   \
-    RQ_APPLY(DT, 128);                 \
-  } while (0)
-  if (a.dt == RQ_BF16) RQ_APPLY_R(RQ_BF16);
-  RQ_APPLY_R(RQ_F16);
-#undef RQ_APPLY_R
-#undef RQ_APPLY
+  const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo};
+  const bool vec = a.D1 % 8 == 0 && a.D2 % 8 == 0 && rows16b(in, ldin) && rows16b(out, ldo) &&
+                   (!base || rows16b(base, ldb));
+  int csize = 8;
+  if (const char* e = getenv("RQ_CS")) csize = atoi(e);
+  if (a.dt == RQ_BF16)
+    return a.tile >= 64 ? launch_apply_r<RQ_BF16, 4>(p, vec, tiles, csize, st)
+                        : launch_apply_r<RQ_BF16, 1>(p, vec, tiles, csize, st);
+  return a.tile >= 64 ? launch_apply_r<RQ_F16, 4>(p, vec, tiles, csize, st)
+                      : launch_apply_r<RQ_F16, 1>(p, vec, tiles, csize, st);
 }
 
 // ------------------------------------------------------------------- grad
 
 constexpr int kGrThreads = 256, kGrWarps = kGrThreads / 32;
 constexpr int kGrCols = 128;                                 // columns of a CTA: one block of 8-bit codes
-constexpr int kGrSmem = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
+constexpr int kGrSums = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
+// A lane's part of one step in the ring: 4 rows of z (2 x 8 columns) and of mid
+// (2 ranks), and the rows' scales; [piece][lane], so that no lane shares a bank.
+__host__ __device__ constexpr int gr_step_bytes(bool codes) { return 32 * (codes ? 8 * 8 + 4 * 8 + 4 * 4 : 8 * 16 + 4 * 8); }
+__host__ __device__ constexpr int gr_stages(bool codes) { return codes ? 6 : 4; }
 
 struct GradArgs {
   AdapterRows a;
@@ -561,7 +637,6 @@ struct GradArgs {
   const float* mid;
   void* G;
   int groups;  // warps along the rank, 16 of it each: 1, 2, 4 or 8
-  bool vec;
 };
 
 // Two packed 16-bit values of codes a (low) and b (high), exact.  bf16: 0x43qq
@@ -590,17 +665,21 @@ __device__ __forceinline__ uint32_t codes2(uint32_t two) {  // bytes: a, ?, b, ?
 // inputs give equal bits, without atomics or a workspace.
 //
 // The reduction runs over rows, so the MMA's k index is the row: a lane holds
-// four rows (4t .. 4t+3 of 16) and, of each, 8 + 8 columns straight from
-// global memory; a pair of rows of one column is one byte permute, and the
-// columns are dealt to the MMA's m index so that this works out.  z is read
-// once (HBM bound up to rank 16; above, warps that share rows read them
-// through L1 and the tensor cores' rate takes over).  Codes become 16-bit
-// values exactly; their scale multiplies the other operand, mid, in fp32,
-// which then enters as two 16-bit halves as in the row products.
-template <int DT, bool CODES>
-__global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_constant__ GradArgs p) {
+// four rows (4t .. 4t+3 of 16) and, of each, 8 + 8 columns; a pair of rows of
+// one column is one byte permute, and the columns are dealt to the MMA's m
+// index so that this works out.  What a lane multiplies it also fetches, so
+// its loads go through a ring in shared memory by cp.async, several steps
+// ahead and without any barrier.  z is read once (HBM bound up to rank 32;
+// above, the warps that share rows read them through L1 and the tensor cores'
+// rate takes over).  Codes become 16-bit values exactly; their scale
+// multiplies the other operand, mid, in fp32, which then enters as two 16-bit
+// halves as in the row products.
+template <int DT, bool CODES, bool VEC>
+__global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_constant__ GradArgs p) {
   using T = typename DType<DT>::T;
-  extern __shared__ __align__(16) float sums[];
+  constexpr int STEP = gr_step_bytes(CODES), S = gr_stages(CODES), ZB = CODES ? 8 : 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* sums = reinterpret_cast<float*>(smem);
   const AdapterRows& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
   const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
@@ -608,10 +687,12 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % p.groups, mw = warp / p.groups, MW = kGrWarps / p.groups, R16 = p.groups * 16;
 
-  const int first = a.plan ? a.plan[1 + adapter] : 0, last = a.plan ? a.plan[2 + adapter] : (int)a.M;
+  const int first = a.plan ? max(a.plan[1 + adapter], 0) : 0;
+  const int last = a.plan ? min(a.plan[2 + adapter], (int)a.M) : (int)a.M;
   const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
   const int64_t c0 = (int64_t)block * kGrCols + 8 * g;
   const int j0 = rg * 16 + 2 * g;  // this lane's pair of ranks: n index g of both n-tiles
+  const bool ranks = j0 < a.r;
   float acc[8][2][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -620,35 +701,70 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   int ex_now = 0;          // fp16: biased exponent that mid is scaled down by
   float mul = 1.0f;
 
-  const int stride = csize * MW * 16;
-  for (int at = first + (crank * MW + mw) * 16; at < last; at += stride) {
+  const int begin = first + (crank * MW + mw) * 16, stride = csize * MW * 16;
+  const int steps = begin < last ? (last - begin + stride - 1) / stride : 0;
+  unsigned char* ring = smem + warp * S * STEP;
+  auto row_of = [&](int s, int i) {  // batch row of place i of this lane's four in step s; -1: none
+    const int place = begin + s * stride + 4 * t + i;
+    if (s >= steps || place >= last) return -1;
+    return order ? min(max(order[place], 0), (int)a.M - 1) : place;
+  };
+  int rows[4];  // of the next step to be fetched
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rows[i] = row_of(0, i);
+  auto fetch = [&](int s) {
+    unsigned char* dst = ring + (s % S) * STEP;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool on = rows[i] >= 0;
+      const int64_t m = on ? rows[i] : 0;
+      unsigned char* z0 = dst + (2 * i * 32 + lane) * ZB;
+      if constexpr (CODES) {
+        const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0;
+        cp_async_small<8>(z0, row, on);
+        cp_async_small<8>(z0 + 32 * ZB, row + 64, on);
+        cp_async_small<4>(dst + 32 * (8 * ZB + 32) + (i * 32 + lane) * 4, p.zscale + m * p.lds + block, on);
+      } else if constexpr (VEC) {
+        const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
+        cp_async16(z0, row + (c0 < a.D1 ? c0 : 0), on && c0 < a.D1);
+        cp_async16(z0 + 32 * ZB, row + (c0 + 64 < a.D1 ? c0 + 64 : 0), on && c0 + 64 < a.D1);
+      } else {
+        const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
+        *reinterpret_cast<uint4*>(z0) = load_row8<false>(row, c0, on ? a.D1 : 0);
+        *reinterpret_cast<uint4*>(z0 + 32 * ZB) = load_row8<false>(row, c0 + 64, on ? a.D1 : 0);
+      }
+      cp_async_small<8>(dst + 32 * 8 * ZB + (i * 32 + lane) * 8, p.mid + (ranks ? m * a.r + j0 : 0), on && ranks);
+    }
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = row_of(s + 1, i);
+  };
+  for (int s = 0; s < S - 1; ++s) fetch(s);
+
+  for (int s = 0; s < steps; ++s) {
+    cp_async_wait<S - 2>();
+    const unsigned char* src = ring + (s % S) * STEP;
     uint4 z[4][2];
     float2 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int place = at + 4 * t + i;
-      z[i][0] = z[i][1] = make_uint4(0u, 0u, 0u, 0u);
-      v[i] = make_float2(0.0f, 0.0f);
-      if (place < last) {
-        const int64_t m = order ? order[place] : place;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* q = src + ((2 * i + h) * 32 + lane) * ZB;
         if constexpr (CODES) {
-          const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0;
-          const uint2 q0 = *reinterpret_cast<const uint2*>(row), q1 = *reinterpret_cast<const uint2*>(row + 64);
-          z[i][0].x = q0.x, z[i][0].y = q0.y, z[i][1].x = q1.x, z[i][1].y = q1.y;
+          const uint2 w = *reinterpret_cast<const uint2*>(q);
+          z[i][h] = make_uint4(w.x, w.y, 0u, 0u);
         } else {
-          const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
-          z[i][0] = load_row8(row, c0, a.D1, p.vec);
-          z[i][1] = load_row8(row, c0 + 64, a.D1, p.vec);
-        }
-        if (j0 < a.r) {
-          v[i] = *reinterpret_cast<const float2*>(p.mid + m * a.r + j0);
-          if constexpr (CODES) {
-            const float s = p.zscale[m * p.lds + block];
-            v[i].x *= s, v[i].y *= s;
-          }
+          z[i][h] = *reinterpret_cast<const uint4*>(q);
         }
       }
+      v[i] = *reinterpret_cast<const float2*>(src + 32 * 8 * ZB + (i * 32 + lane) * 8);
+      if constexpr (CODES) {
+        const float f = *reinterpret_cast<const float*>(src + 32 * (8 * ZB + 32) + (i * 32 + lane) * 4);
+        v[i].x *= f, v[i].y *= f;
+      }
     }
+    fetch(s + S - 1);
     if constexpr (DT == RQ_F16) {
       // keep mid near 2^14 as fp16: when a step's largest value passes the
       // scale in use, the sums so far are scaled down to the new one
@@ -676,14 +792,9 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float e = n ? v[2 * k].y : v[2 * k].x, f = n ? v[2 * k + 1].y : v[2 * k + 1].x;
-        uint16_t h0, l0, h1, l1;
-        split16<DT>(e * mul, &h0, &l0);
-        split16<DT>(f * mul, &h1, &l1);
-        b[0][n][k] = h0 | ((uint32_t)h1 << 16);
-        b[1][n][k] = l0 | ((uint32_t)l1 << 16);
-      }
+      for (int k = 0; k < 2; ++k)
+        split16x2<DT>((n ? v[2 * k].y : v[2 * k].x) * mul, (n ? v[2 * k + 1].y : v[2 * k + 1].x) * mul, &b[0][n][k],
+                      &b[1][n][k]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t f[4];  // (columns, columns + 64) x (rows 4t, 4t+1 | 4t+2, 4t+3)
@@ -708,6 +819,8 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
           Mma16816<DT>::run(acc[i][n], f[0], f[1], f[2], f[3], b[half][n][0], b[half][n][1]);
     }
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the sums lie over the ring
 
   // this warp's sums: column 8 g + i (+ 64) at row 8 i + g (+ 64), ranks 4t .. 4t+3
   const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
@@ -729,53 +842,36 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     reinterpret_cast<float4*>(sums)[i] = s;
   }
   cluster.sync();
-  // 8 ranks of a column are one 16-byte store; the cluster's CTAs take the columns in turn
-  const int units = R16 / 8;
-  for (int i = crank * kGrThreads + tid; i < kGrCols * units; i += csize * kGrThreads) {
-    const int at = i / units, j = (i - at * units) * 8;
+  // 4 ranks of a column at a time, dealt to the cluster's CTAs
+  const int units = R16 / 4;
+  for (int i = tid * csize + crank; i < kGrCols * units; i += csize * kGrThreads) {
+    const int at = i / units, j = (i - at * units) * 4;
     const int64_t d = (int64_t)block * kGrCols + 8 * (at & 7) + ((at >> 3) & 7) + (at & 64);
     if (d >= a.D1 || j >= a.r) continue;
-    float s[8] = {};
-    for (int c = 0; c < csize; ++c) {
-      const float* src = cluster.map_shared_rank(sums, c) + at * R16 + j;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += src[e];
-    }
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
-        make_uint4(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]), pack2<DT>(s[4], s[5]), pack2<DT>(s[6], s[7]));
+    const float4 s = cluster_sum<float4>(cluster, sums + at * R16 + j, csize);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
+        make_uint2(pair16<DT>(s.x, s.y), pair16<DT>(s.z, s.w));
   }
   cluster.sync();  // the others have read this CTA's sums
 }
 
+template <int DT>
+static auto grad_kernel(bool codes, bool vec) {
+  return codes ? adapters_grad_k<DT, true, true> : vec ? adapters_grad_k<DT, false, true> : adapters_grad_k<DT, false, false>;
+}
+
 int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
                   void* G, cudaStream_t st) {
-  GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8, rows16b(z, ldz)};
-  // Rows are split over a cluster until the grid holds two CTAs an SM, as
-  // long as a warp keeps two steps of 16 rows of an adapter of mean size.
+  GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8};
+  // Rows are split over a cluster until the grid fills the GPU, as long as a
+  // warp keeps two steps of 16 rows of an adapter of mean size.
   const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols, each = a.M / a.count * p.groups / (kGrWarps * 32);
   int csize = 1;
-  while (csize < 8 && csize * 2 <= each && blocks * csize < 2 * num_sms()) csize *= 2;
-  auto* kern = a.dt == RQ_BF16 ? (zscale ? adapters_grad_k<RQ_BF16, true> : adapters_grad_k<RQ_BF16, false>)
-                               : (zscale ? adapters_grad_k<RQ_F16, true> : adapters_grad_k<RQ_F16, false>);
-  const int rc = ensure_smem_limit((const void*)kern, kGrSmem);
-  if (rc != RQ_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(blocks * csize), (unsigned)a.count);
-  cfg.blockDim = dim3(kGrThreads);
-  cfg.dynamicSmemBytes = kGrSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return RQ_ERR_CUDA;
-  }
-  return check_launch();
+  while (csize < 8 && csize * 2 <= each && blocks * csize < num_sms()) csize *= 2;
+  const bool codes = zscale != nullptr, vec = rows16b(z, ldz) && a.D1 % 8 == 0;
+  auto* kern = a.dt == RQ_BF16 ? grad_kernel<RQ_BF16>(codes, vec) : grad_kernel<RQ_F16>(codes, vec);
+  const int ring = kGrWarps * gr_stages(codes) * gr_step_bytes(codes), smem = ring > kGrSums ? ring : kGrSums;
+  return launch_cluster(kern, p, dim3((unsigned)(blocks * csize), (unsigned)a.count), kGrThreads, smem, csize, st);
 }
 
 }  // namespace rq
