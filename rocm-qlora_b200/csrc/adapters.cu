@@ -15,6 +15,8 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "gemv_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -145,6 +147,13 @@ constexpr int kApWin = 32;  // columns of a window: one 16-byte load of each lan
 __host__ __device__ constexpr int ap_pitch_u(int R) { return R * 2 + 16; }
 __host__ __device__ constexpr int ap_pitch_m(int R) { return R <= 32 ? R * 2 : R * 2 + 64; }
 
+// Steps of the first product under way at once, and their shared memory: a
+// step is NW windows of each warp, with U's rows for them.
+__host__ __device__ constexpr int ap_steps(int R, int NW) {
+  return NW == 1 ? (R <= 32 ? 3 : 2) : (R == 64 ? 3 : 4);
+}
+__host__ __device__ constexpr int ap_x_bytes(int NW) { return kApWarps * NW * 2 * 32 * 16; }
+
 struct ApplyArgs {
   AdapterRows a;
   const void* in;
@@ -157,6 +166,15 @@ struct ApplyArgs {
   float* mid;
   void* out;
   int64_t ldo;
+};
+
+// A tile's rows: batch row, where its base and output are and, for fp16, the
+// power of two that its intermediate was scaled down by.
+struct ApplyRows {
+  const uint16_t* base[128];
+  uint16_t* out[128];
+  int row[128];
+  float mul[128];
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool take) {
@@ -230,13 +248,6 @@ __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[N]) {
   if constexpr (N == 4) *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Columns [begin, end) of a 16-byte aligned row (both multiples of 8) into L2.
-__device__ __forceinline__ void prefetch_row(const uint16_t* row, int64_t begin, int64_t end) {
-  if (begin < end)
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(row + begin), "r"((uint32_t)(end - begin) * 2)
-                 : "memory");
-}
-
 // The sum over the cluster's CTAs, in rank order, of what each has at p.  All
 // loads are issued before the first add.
 template <class V>
@@ -253,6 +264,20 @@ __device__ __forceinline__ V cluster_sum(cg::cluster_group& cluster, float* p, i
     for (int c = 0; c < 8; ++c) f[e] += c < csize ? reinterpret_cast<const float*>(&q[c])[e] : 0.0f;
   }
   return s;
+}
+
+// CTAs a cluster (1 to `most`) so that `units` clusters fill whole rounds of
+// the GPU's `per_sm` CTAs an SM best; of equal fills the smaller number of rounds.
+static int fill_size(int64_t units, int per_sm, int most) {
+  const int64_t slots = (int64_t)per_sm * num_sms();
+  int best = 1;
+  double best_fill = 0.0;
+  for (int c = 1; c <= most; ++c) {
+    const int64_t ctas = units * c, rounds = (ctas + slots - 1) / slots;
+    const double fill = (double)ctas / (double)(rounds * slots);
+    if (fill > best_fill + 0.02) best = c, best_fill = fill;
+  }
+  return best;
 }
 
 template <class P>
@@ -297,10 +322,10 @@ static int launch_cluster(void (*kern)(P), const P& args, dim3 grid, int threads
 // output columns.  A decode row costs one launch, no workspace and no second
 // kernel.
 //
-// Loads.  A quad's four lanes hold 32 consecutive columns of a row, 8 each,
-// straight from global memory in one 16-byte load; the MMA's order of the
-// reduction index follows that, and U's rows are put into shared memory in
-// the order that ldmatrix then needs.  V's columns are permuted the same way
+// Loads.  A quad's four lanes hold 32 consecutive columns of a row, 8 each, in
+// one 16-byte piece that the lane fetches for itself by cp.async several steps
+// ahead; the MMA's order of the reduction index follows that, and U's rows are
+// put into shared memory in the order that ldmatrix then needs.  V's columns are permuted the same way
 // among the MMA's n index, so that a lane ends with 8 consecutive output
 // columns: one 16-byte load of base and one store.
 template <int DT, int R, int NW, bool VEC>
@@ -308,7 +333,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   using T = typename DType<DT>::T;
   constexpr int NT = R / 8;               // n-tiles of the first product
   constexpr int KS = R / 16;              // k-steps of the second
-  constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R);
+  constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R), S = ap_steps(R, NW);
   extern __shared__ __align__(16) unsigned char smem[];
   const AdapterRows& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
@@ -334,96 +359,91 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   const bool none = group >= a.count;
   const float fill = group > a.count ? __int_as_float(0x7fc00000) : 0.0f;
 
-  float* part = reinterpret_cast<float*>(smem);                       // [128][R], over the staged U
-  const int KC = NW * WK * kApWin;                                    // columns staged at once
-  unsigned char* mids = smem + 2 * KC * PU;                           // halves of mid: [2][tile][PM]
-  float* rowmul = reinterpret_cast<float*>(mids + 2 * a.tile * PM);   // [tile]
-  int* rowid = reinterpret_cast<int*>(rowmul + 128);                  // [tile]
-  for (int i = tid; i < a.tile; i += kApThreads) {
-    const int at = first + min(i, rows - 1);
-    rowid[i] = order ? min(max(order[at], 0), (int)a.M - 1) : at;
+  const int KC = NW * WK * kApWin, step_bytes = KC * PU + ap_x_bytes(NW);  // columns of a step
+  ApplyRows& at = *reinterpret_cast<ApplyRows*>(smem);
+  unsigned char* ring = smem + sizeof(ApplyRows);
+  float* part = reinterpret_cast<float*>(ring);  // [128][R], over the ring
+  unsigned char* mids = ring + 128 * R * 4;      // halves of mid: [2][tile][PM], over the ring
+  const uint16_t* in = static_cast<const uint16_t*>(p.in);
+  const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  if (tid < a.tile) {
+    const int place = first + min(tid, rows - 1);
+    const int m = order ? min(max(order[place], 0), (int)a.M - 1) : place;
+    at.row[tid] = m;
+    at.base[tid] = base + (int64_t)m * p.ldb;
+    at.out[tid] = static_cast<uint16_t*>(p.out) + (int64_t)m * p.ldo;
   }
   __syncthreads();
   const int chunks2 = (int)((a.D2 + 31) / 32), per2 = (chunks2 + csize - 1) / csize;
   const int ch_begin = min(chunks2, crank * per2), ch_end = min(chunks2, ch_begin + per2);
   const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
   const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
-  const uint16_t* in = static_cast<const uint16_t*>(p.in);
-  const uint16_t* base = static_cast<const uint16_t*>(p.base);
-  if constexpr (VEC) {
-    // this CTA's share of the rows on its way into L2, ahead of the loads
-    if (tid < rows && !none)
-      prefetch_row(in + (int64_t)rowid[tid] * p.ldin, (int64_t)w_begin * kApWin, min((int64_t)w_end * kApWin, a.D1));
-    if (tid >= 128 && tid - 128 < rows && base)
-      prefetch_row(base + (int64_t)rowid[tid - 128] * p.ldb, (int64_t)ch_begin * 32, min((int64_t)ch_end * 32, a.D2));
-  }
-
   if (!none) {
     // ---- partial sums over this CTA's input columns
     const uint16_t* U = static_cast<const uint16_t*>(p.U) + (int64_t)group * a.D1 * a.r;
     const int step = NW * WK, chunks = (w_end - w_begin + step - 1) / step;
     const int wm = warp % WM, wk = warp / WM;
-    const uint16_t* xa = in + (int64_t)rowid[wm * 16 + g] * p.ldin;
-    const uint16_t* xb = in + (int64_t)rowid[wm * 16 + g + 8] * p.ldin;
+    const uint16_t* xa = in + (int64_t)at.row[wm * 16 + g] * p.ldin;
+    const uint16_t* xb = in + (int64_t)at.row[wm * 16 + g + 8] * p.ldin;
 
-    auto stage = [&](int c) {  // U's rows of chunk c, each at the place its window's order gives it
-      unsigned char* dst = smem + (c & 1) * KC * PU;
-      for (int i = tid; i < KC * NT; i += kApThreads) {
-        const int k = i / NT, q = i - k * NT;
-        const int64_t col = (int64_t)(w_begin + c * step) * kApWin + k;
-        const int in = k & 31, slot = (k & ~31) | ((in & 6) << 2) | ((in >> 3) << 1) | (in & 1);
-        const bool ok = col < a.D1 && q * 8 < a.r;
-        cp_async16(dst + slot * PU + q * 16, U + (ok ? col * a.r + q * 8 : 0), ok);
+    auto stage = [&](int c) {
+      unsigned char* dst = ring + (c % S) * step_bytes;
+      const int64_t col0 = (int64_t)(w_begin + c * step) * kApWin;
+      if (c < chunks) {
+        // U's rows, each at the place that its window's order gives it
+        for (int i = tid; i < KC * NT; i += kApThreads) {
+          const int k = i / NT, q = i - k * NT;
+          const int in = k & 31, slot = (k & ~31) | ((in & 6) << 2) | ((in >> 3) << 1) | (in & 1);
+          const bool ok = col0 + k < a.D1 && q * 8 < a.r;
+          cp_async16(dst + slot * PU + q * 16, U + (ok ? (col0 + k) * a.r + q * 8 : 0), ok);
+        }
+        // this lane's part of the rows: what it multiplies it also fetches
+        unsigned char* x = dst + KC * PU + (warp * NW * 64 + lane) * 16;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const int win = w_begin + c * step + wk * NW + w;
+          const int64_t col = (int64_t)win * kApWin + t * 8;
+          if constexpr (VEC) {
+            const bool ok = win < w_end && col < a.D1;
+            cp_async16(x + w * 1024, xa + (ok ? col : 0), ok);
+            cp_async16(x + w * 1024 + 512, xb + (ok ? col : 0), ok);
+          } else {
+            *reinterpret_cast<uint4*>(x + w * 1024) = load_row8<false>(xa, win < w_end ? col : a.D1, a.D1);
+            *reinterpret_cast<uint4*>(x + w * 1024 + 512) = load_row8<false>(xb, win < w_end ? col : a.D1, a.D1);
+          }
+        }
       }
       cp_async_commit();
-    };
-    auto fetch = [&](uint4 (&x)[NW][2], int c) {
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const int win = w_begin + c * step + wk * NW + w;
-        const int64_t col = win < w_end ? (int64_t)win * kApWin + t * 8 : a.D1;
-        x[w][0] = load_row8<VEC>(xa, col, a.D1);
-        x[w][1] = load_row8<VEC>(xb, col, a.D1);
-      }
     };
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-    uint4 x[NW][2], nx[NW][2];
-    if (chunks > 0) {
-      stage(0);
-      fetch(x, 0);
-    }
+    for (int c = 0; c < S - 1; ++c) stage(c);
     for (int c = 0; c < chunks; ++c) {
-      if (c + 1 < chunks) {
-        stage(c + 1);
-        fetch(nx, c + 1);
-        cp_async_wait<1>();
-      } else {
-        cp_async_wait<0>();
-      }
-      __syncthreads();
-      const unsigned char* u = smem + (c & 1) * KC * PU + wk * NW * kApWin * PU;
+      cp_async_wait<S - 2>();
+      __syncthreads();  // step c is here, and step c - 1, whose place comes next, has been read
+      stage(c + S - 1);
+      const unsigned char* u = ring + (c % S) * step_bytes + wk * NW * kApWin * PU;
+      const unsigned char* mine = ring + (c % S) * step_bytes + KC * PU + (warp * NW * 64 + lane) * 16;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
+        const uint4 x = *reinterpret_cast<const uint4*>(mine + w * 1024);
+        const uint4 y = *reinterpret_cast<const uint4*>(mine + w * 1024 + 512);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t a0 = s ? x[w][0].z : x[w][0].x, a2 = s ? x[w][0].w : x[w][0].y;
-          const uint32_t a1 = s ? x[w][1].z : x[w][1].x, a3 = s ? x[w][1].w : x[w][1].y;
           const unsigned char* row = u + (w * 32 + s * 16 + (lane & 15)) * PU + (lane >> 4) * 16;
 #pragma unroll
           for (int j = 0; j < NT; j += 2) {
             uint32_t b[4];
             ldmatrix4_trans(b, row + j * 16);
-            Mma16816<DT>::run(acc[j], a0, a1, a2, a3, b[0], b[1]);
-            Mma16816<DT>::run(acc[j + 1], a0, a1, a2, a3, b[2], b[3]);
+            Mma16816<DT>::run(acc[j], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[0], b[1]);
+            Mma16816<DT>::run(acc[j + 1], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[2], b[3]);
           }
         }
       }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < NW; ++w) x[w][0] = nx[w][0], x[w][1] = nx[w][1];
     }
+    cp_async_wait<0>();
+    __syncthreads();  // the sums lie over the ring
 
     // ---- the sums meet: warps of the CTA in order, then the cluster's CTAs in rank order
     float* mine = part + (wk * a.tile + wm * 16) * R;
@@ -458,7 +478,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       for (int e = 0; e < E; ++e) {
         v[e] *= s;
         top = fmaxf(top, fabsf(v[e]));
-        if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)rowid[row] * a.r + l * E + e] = v[e];
+        if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)at.row[row] * a.r + l * E + e] = v[e];
       }
       float mul = 1.0f, back = 1.0f;
       if constexpr (DT == RQ_F16) {
@@ -474,64 +494,88 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
         __align__(16) uint32_t hi[E / 2], lo[E / 2];
 #pragma unroll
         for (int e = 0; e < E; e += 2) split16x2<DT>(v[e] * mul, v[e + 1] * mul, &hi[e / 2], &lo[e / 2]);
-        unsigned char* at = mids + row * PM + l * E * 2;
+        unsigned char* to = mids + row * PM + l * E * 2;
         for (int c = 0; c < csize; ++c) {
-          unsigned char* m = cluster.map_shared_rank(at, c);
+          unsigned char* m = cluster.map_shared_rank(to, c);
           store_words<E / 2>(m, hi);
           store_words<E / 2>(m + a.tile * PM, lo);
-          if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(rowmul, c)[row] = back;
+          if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(at.mul, c)[row] = back;
         }
       }
     }
     cluster.sync();
   } else {
     if (p.mid && crank == 0)
-      for (int i = tid; i < rows * a.r; i += kApThreads) p.mid[(int64_t)rowid[i / a.r] * a.r + i % a.r] = fill;
+      for (int i = tid; i < rows * a.r; i += kApThreads) p.mid[(int64_t)at.row[i / a.r] * a.r + i % a.r] = fill;
     if (p.out == p.base && fill == 0.0f) return;
   }
 
-  // ---- this warp's output columns, 32 at a time, all rows of the tile
+  // ---- this warp's output columns, CW x 32 at a time, all rows of the tile.
+  // base starts the accumulators, so the sum costs no instruction of its own.
+  constexpr int CW = R <= 32 ? 2 : 1, AHEAD = R <= 32 ? 2 : 4;  // m-tiles of base under way
   const int n_tiles = (rows + 15) / 16;
   const uint16_t* V = static_cast<const uint16_t*>(p.V) + (none ? 0 : (int64_t)group * a.D2 * a.r);
-  uint16_t* out = static_cast<uint16_t*>(p.out);
-  for (int ch = ch_begin + warp; ch < ch_end; ch += kApWarps) {
+  for (int ch = ch_begin + warp * CW; ch < ch_end; ch += kApWarps * CW) {
     const int64_t col = (int64_t)ch * 32 + 8 * t;
-    auto fetch = [&](uint4 (&old)[2], int mt) {
+    const int64_t end = min((int64_t)ch_end * 32, a.D2);  // columns this CTA writes
+    auto fetch = [&](uint4 (&old)[CW][2], int mt) {
+      const uint16_t* ra = at.base[mt * 16 + g];
+      const uint16_t* rb = at.base[mt * 16 + g + 8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        old[h] = base && mt < n_tiles ? load_row8<VEC>(base + (int64_t)rowid[mt * 16 + 8 * h + g] * p.ldb, col, a.D2)
-                                      : make_uint4(0u, 0u, 0u, 0u);
+      for (int w = 0; w < CW; ++w) {
+        old[w][0] = load_row8<VEC>(ra, col + 32 * w, end);
+        old[w][1] = load_row8<VEC>(rb, col + 32 * w, end);
+      }
     };
-    uint4 ahead[2][2];  // base of the next two m-tiles
-    fetch(ahead[0], 0);
-    fetch(ahead[1], 1);
-    // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
-    uint32_t b[4][KS][2];
+    uint4 ahead[AHEAD][CW][2] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = (int64_t)ch * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
+    for (int i = 0; i < AHEAD; ++i)
+      if (base && i < n_tiles) fetch(ahead[i], i);
+    // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
+    uint32_t b[CW][4][KS][2];
+#pragma unroll
+    for (int j = 0; j < 4 * CW; ++j) {
+      const int64_t n = (int64_t)ch * 32 + 32 * (j / 4) + 8 * (g >> 1) + 2 * (j % 4) + (g & 1);
       const uint16_t* v = V + n * a.r;
-      const bool ok = !none && n < a.D2;
+      const bool ok = !none && n < end;
       if constexpr (R == 16) {
         const uint2 q = ok && 4 * t < a.r ? *reinterpret_cast<const uint2*>(v + 4 * t) : make_uint2(0u, 0u);
-        b[j][0][0] = q.x, b[j][0][1] = q.y;
+        b[j / 4][j % 4][0][0] = q.x, b[j / 4][j % 4][0][1] = q.y;
       } else {
 #pragma unroll
         for (int w = 0; w < KS / 2; ++w) {
           const uint4 q = ok && 32 * w + 8 * t < a.r ? *reinterpret_cast<const uint4*>(v + 32 * w + 8 * t)
                                                      : make_uint4(0u, 0u, 0u, 0u);
-          b[j][2 * w][0] = q.x, b[j][2 * w][1] = q.y, b[j][2 * w + 1][0] = q.z, b[j][2 * w + 1][1] = q.w;
+          uint32_t(&f)[KS][2] = b[j / 4][j % 4];
+          f[2 * w][0] = q.x, f[2 * w][1] = q.y, f[2 * w + 1][0] = q.z, f[2 * w + 1][1] = q.w;
         }
       }
     }
-    for (int mt = 0; mt < n_tiles; ++mt) {
+    auto tile = [&](int mt, uint4 (&old)[CW][2]) {
       const int ra = mt * 16 + g;
-      uint4 old[2] = {ahead[0][0], ahead[0][1]};
-      ahead[0][0] = ahead[1][0], ahead[0][1] = ahead[1][1];
-      fetch(ahead[1], mt + 2);
-      float acc[4][4];
+      // fp16: the row's power of two, taken off base here and put back below
+      float off_a = 1.0f, off_b = 1.0f, mul_a = 1.0f, mul_b = 1.0f;
+      if (DT == RQ_F16 && !none) {
+        mul_a = at.mul[ra], mul_b = at.mul[ra + 8];
+        off_a = __uint_as_float((254u << 23) - __float_as_uint(mul_a));
+        off_b = __uint_as_float((254u << 23) - __float_as_uint(mul_b));
+      }
+      float acc[CW][4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = fill;
+      for (int w = 0; w < CW; ++w) {
+        const uint32_t qa[4] = {old[w][0].x, old[w][0].y, old[w][0].z, old[w][0].w};
+        const uint32_t qb[4] = {old[w][1].x, old[w][1].y, old[w][1].z, old[w][1].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = unpair16<DT>(qa[j]), y = unpair16<DT>(qb[j]);
+          if constexpr (DT == RQ_F16) {
+            acc[w][j][0] = x.x * off_a, acc[w][j][1] = x.y * off_a, acc[w][j][2] = y.x * off_b, acc[w][j][3] = y.y * off_b;
+          } else {
+            acc[w][j][0] = x.x, acc[w][j][1] = x.y, acc[w][j][2] = y.x, acc[w][j][3] = y.y;
+          }
+        }
+      }
+      if (base && mt + AHEAD < n_tiles) fetch(old, mt + AHEAD);
       if (!none) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -540,44 +584,55 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
           if constexpr (R == 16) {
             const uint2 qa = *reinterpret_cast<const uint2*>(ma + 8 * t), qb = *reinterpret_cast<const uint2*>(mb + 8 * t);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][0][0], b[j][0][1]);
+            for (int w = 0; w < CW; ++w)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][0][0], b[w][j][0][1]);
           } else {
 #pragma unroll
-            for (int w = 0; w < KS / 2; ++w) {
-              const uint4 qa = *reinterpret_cast<const uint4*>(ma + 64 * w + 16 * t);
-              const uint4 qb = *reinterpret_cast<const uint4*>(mb + 64 * w + 16 * t);
+            for (int k = 0; k < KS / 2; ++k) {
+              const uint4 qa = *reinterpret_cast<const uint4*>(ma + 64 * k + 16 * t);
+              const uint4 qb = *reinterpret_cast<const uint4*>(mb + 64 * k + 16 * t);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                Mma16816<DT>::run(acc[j], qa.x, qb.x, qa.y, qb.y, b[j][2 * w][0], b[j][2 * w][1]);
-                Mma16816<DT>::run(acc[j], qa.z, qb.z, qa.w, qb.w, b[j][2 * w + 1][0], b[j][2 * w + 1][1]);
-              }
+              for (int w = 0; w < CW; ++w)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][2 * k][0], b[w][j][2 * k][1]);
+                  Mma16816<DT>::run(acc[w][j], qa.z, qb.z, qa.w, qb.w, b[w][j][2 * k + 1][0], b[w][j][2 * k + 1][1]);
+                }
             }
           }
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int row = ra + 8 * h;
-        if (row >= rows) continue;
-        const float mul = DT == RQ_F16 && !none ? rowmul[row] : 1.0f;
-        const uint32_t w[4] = {old[h].x, old[h].y, old[h].z, old[h].w};
-        uint32_t res[4];
+        if (ra + 8 * h >= rows) continue;
+        uint16_t* dst = at.out[ra + 8 * h] + col;
+        const float mul = h ? mul_b : mul_a;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 o = unpair16<DT>(w[j]);
-          res[j] = DT == RQ_F16 ? pair16<DT>(fmaf(acc[j][2 * h], mul, o.x), fmaf(acc[j][2 * h + 1], mul, o.y))
-                                : pair16<DT>(acc[j][2 * h] + o.x, acc[j][2 * h + 1] + o.y);
-        }
-        uint16_t* dst = out + (int64_t)rowid[row] * p.ldo + col;
-        if constexpr (VEC) {
-          if (col < a.D2) *reinterpret_cast<uint4*>(dst) = make_uint4(res[0], res[1], res[2], res[3]);
-        } else {
+        for (int w = 0; w < CW; ++w) {
+          uint32_t res[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + i < a.D2) dst[i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
+          for (int j = 0; j < 4; ++j) {
+            float x = acc[w][j][2 * h], y = acc[w][j][2 * h + 1];
+            if constexpr (DT == RQ_F16) x *= mul, y *= mul;
+            res[j] = pair16<DT>(group > a.count ? fill : x, group > a.count ? fill : y);
+          }
+          if constexpr (VEC) {
+            if (col + 32 * w < end)
+              *reinterpret_cast<uint4*>(dst + 32 * w) = make_uint4(res[0], res[1], res[2], res[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (col + 32 * w + i < end) dst[32 * w + i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
+          }
         }
       }
-    }
+    };
+    for (int mt = 0; mt < n_tiles; mt += AHEAD)
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (mt + i < n_tiles) tile(mt + i, ahead[i]);
   }
 }
 
@@ -585,9 +640,9 @@ static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 &
 
 template <int DT, int R, int NW>
 static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, int csize, cudaStream_t st) {
-  const int WK = kApWarps / (p.a.tile / 16);
-  const size_t stage = (size_t)2 * NW * WK * kApWin * ap_pitch_u(R);
-  const size_t smem = stage + (size_t)2 * p.a.tile * ap_pitch_m(R) + 128 * 8;
+  const size_t ring = (size_t)ap_steps(R, NW) * (NW * (kApWarps / (p.a.tile / 16)) * kApWin * ap_pitch_u(R) + ap_x_bytes(NW));
+  const size_t after = (size_t)128 * R * 4 + (size_t)2 * p.a.tile * ap_pitch_m(R);
+  const size_t smem = sizeof(ApplyRows) + std::max(ring, after);
   return launch_cluster(vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>, p,
                         dim3((unsigned)(tiles * csize)), kApThreads, smem, csize, st);
 }
@@ -609,12 +664,11 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
   const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo};
   const bool vec = a.D1 % 8 == 0 && a.D2 % 8 == 0 && rows16b(in, ldin) && rows16b(out, ldo) &&
                    (!base || rows16b(base, ldb));
-  int csize = 8;
-  if (const char* e = getenv("RQ_CS")) csize = atoi(e);
+  const int csize = fill_size((a.M + a.tile - 1) / a.tile, a.r <= 64 ? 2 : 1, 8);
   if (a.dt == RQ_BF16)
-    return a.tile >= 64 ? launch_apply_r<RQ_BF16, 4>(p, vec, tiles, csize, st)
+    return a.tile >= 64 ? launch_apply_r<RQ_BF16, 2>(p, vec, tiles, csize, st)
                         : launch_apply_r<RQ_BF16, 1>(p, vec, tiles, csize, st);
-  return a.tile >= 64 ? launch_apply_r<RQ_F16, 4>(p, vec, tiles, csize, st)
+  return a.tile >= 64 ? launch_apply_r<RQ_F16, 2>(p, vec, tiles, csize, st)
                       : launch_apply_r<RQ_F16, 1>(p, vec, tiles, csize, st);
 }
 
@@ -623,10 +677,11 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
 constexpr int kGrThreads = 256, kGrWarps = kGrThreads / 32;
 constexpr int kGrCols = 128;                                 // columns of a CTA: one block of 8-bit codes
 constexpr int kGrSums = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
-// A lane's part of one step in the ring: 4 rows of z (2 x 8 columns) and of mid
-// (2 ranks), and the rows' scales; [piece][lane], so that no lane shares a bank.
-__host__ __device__ constexpr int gr_step_bytes(bool codes) { return 32 * (codes ? 8 * 8 + 4 * 8 + 4 * 4 : 8 * 16 + 4 * 8); }
-__host__ __device__ constexpr int gr_stages(bool codes) { return codes ? 6 : 4; }
+// One step of a warp in its ring: 16 rows of z (swizzled 16-byte pieces) and of
+// mid (16 ranks, padded so that fragment loads use distinct banks).
+constexpr int kGrMidPitch = 20 * 4;
+__host__ __device__ constexpr int gr_row_bytes(bool codes) { return codes ? kGrCols : kGrCols * 2; }
+__host__ __device__ constexpr int gr_step_bytes(bool codes) { return 16 * (gr_row_bytes(codes) + kGrMidPitch + (codes ? 4 : 0)); }
 
 struct GradArgs {
   AdapterRows a;
@@ -639,20 +694,20 @@ struct GradArgs {
   int groups;  // warps along the rank, 16 of it each: 1, 2, 4 or 8
 };
 
-// Two packed 16-bit values of codes a (low) and b (high), exact.  bf16: 0x43qq
-// without the code's sign bit is 128 + (q mod 128), and 0x4300 with it alone
-// is 128 for q >= 0 and 256 for q < 0; their difference is q.  fp16: 0x64uu
-// with u = q + 128 is 1024 + u.
+// Two codes in the low bytes of a word's halves as 16-bit values, exact.  bf16:
+// 0x4300 with the code's lower 7 bits is 128 + (q mod 128), and with its sign
+// bit alone 128 for q >= 0 and 256 for q < 0; their difference is q.  fp16:
+// 0x64uu with u = q + 128 is 1024 + u.
 template <int DT>
-__device__ __forceinline__ uint32_t codes2(uint32_t two) {  // bytes: a, ?, b, ? -> halves
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
   if constexpr (DT == RQ_BF16) {
-    const uint32_t w = (two & 0x00ff00ffu) | 0x43004300u, x = w & 0xff7fff7fu, y = w & 0xff80ff80u;
+    const uint32_t x = (w & 0x007f007fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
     const __nv_bfloat162 d =
         __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
     return *reinterpret_cast<const uint32_t*>(&d);
   } else {
-    const uint32_t w = ((two & 0x00ff00ffu) ^ 0x00800080u) | 0x64006400u, y = 0x64806480u;
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&y));
+    const uint32_t x = ((w & 0x00ff00ffu) ^ 0x64806480u), y = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
     return *reinterpret_cast<const uint32_t*>(&d);
   }
 }
@@ -664,20 +719,19 @@ __device__ __forceinline__ uint32_t codes2(uint32_t two) {  // bytes: a, ?, b, ?
 // in shared and distributed shared memory in warp and rank order, so equal
 // inputs give equal bits, without atomics or a workspace.
 //
-// The reduction runs over rows, so the MMA's k index is the row: a lane holds
-// four rows (4t .. 4t+3 of 16) and, of each, 8 + 8 columns; a pair of rows of
-// one column is one byte permute, and the columns are dealt to the MMA's m
-// index so that this works out.  What a lane multiplies it also fetches, so
-// its loads go through a ring in shared memory by cp.async, several steps
-// ahead and without any barrier.  z is read once (HBM bound up to rank 32;
-// above, the warps that share rows read them through L1 and the tensor cores'
-// rate takes over).  Codes become 16-bit values exactly; their scale
-// multiplies the other operand, mid, in fp32, which then enters as two 16-bit
-// halves as in the row products.
-template <int DT, bool CODES, bool VEC>
-__global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_constant__ GradArgs p) {
+// The reduction runs over rows, so the MMA's k index is the row and ldmatrix
+// transposes z's tile on its way to the registers.  Each warp fetches its own
+// 16-row steps by cp.async into its own ring (two lanes a row, so a lane needs
+// one row number a step) and nothing but its own lanes waits for them.  z is
+// read once (HBM bound up to rank 32; above, the warps that share rows read
+// them through L1 and the tensor cores' rate takes over).  Codes become 16-bit
+// values exactly; their scale multiplies the other operand, mid, in fp32,
+// which then enters as two 16-bit halves as in the row products.
+template <int DT, bool CODES, bool VEC, int S>
+__global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(const __grid_constant__ GradArgs p) {
   using T = typename DType<DT>::T;
-  constexpr int STEP = gr_step_bytes(CODES), S = gr_stages(CODES), ZB = CODES ? 8 : 16;
+  constexpr int ROW = gr_row_bytes(CODES), STEP = gr_step_bytes(CODES);
+  constexpr int PIECES = ROW / 32;  // 16-byte pieces a lane fetches: half a row
   extern __shared__ __align__(16) unsigned char smem[];
   float* sums = reinterpret_cast<float*>(smem);
   const AdapterRows& a = p.a;
@@ -690,9 +744,13 @@ __global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_co
   const int first = a.plan ? max(a.plan[1 + adapter], 0) : 0;
   const int last = a.plan ? min(a.plan[2 + adapter], (int)a.M) : (int)a.M;
   const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
-  const int64_t c0 = (int64_t)block * kGrCols + 8 * g;
-  const int j0 = rg * 16 + 2 * g;  // this lane's pair of ranks: n index g of both n-tiles
-  const bool ranks = j0 < a.r;
+  if (first >= last) {  // the whole cluster: no rows, zero gradient
+    const int64_t d0 = (int64_t)block * kGrCols, n = min((int64_t)kGrCols, a.D1 - d0) * a.r / 8;
+    uint4* G = reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d0) * a.r);
+    for (int64_t i = crank * kGrThreads + tid; i < n; i += csize * kGrThreads) G[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const int64_t c0 = (int64_t)block * kGrCols;
   float acc[8][2][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -701,70 +759,67 @@ __global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_co
   int ex_now = 0;          // fp16: biased exponent that mid is scaled down by
   float mul = 1.0f;
 
+  // fetching: lane's row of a step and half of its pieces (even or odd ones)
+  const int frow = lane >> 1, fhalf = lane & 1;
   const int begin = first + (crank * MW + mw) * 16, stride = csize * MW * 16;
   const int steps = begin < last ? (last - begin + stride - 1) / stride : 0;
   unsigned char* ring = smem + warp * S * STEP;
-  auto row_of = [&](int s, int i) {  // batch row of place i of this lane's four in step s; -1: none
-    const int place = begin + s * stride + 4 * t + i;
+  auto row_of = [&](int s) {  // batch row of this lane's row in step s; -1: none
+    const int place = begin + s * stride + frow;
     if (s >= steps || place >= last) return -1;
     return order ? min(max(order[place], 0), (int)a.M - 1) : place;
   };
-  int rows[4];  // of the next step to be fetched
-#pragma unroll
-  for (int i = 0; i < 4; ++i) rows[i] = row_of(0, i);
+  int next = row_of(0);
   auto fetch = [&](int s) {
     unsigned char* dst = ring + (s % S) * STEP;
+    const bool on = next >= 0;
+    const int64_t m = on ? next : 0;
+    const int j = rg * 16 + 8 * fhalf;
+    if constexpr (CODES) {
+      const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0 + 16 * fhalf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool on = rows[i] >= 0;
-      const int64_t m = on ? rows[i] : 0;
-      unsigned char* z0 = dst + (2 * i * 32 + lane) * ZB;
-      if constexpr (CODES) {
-        const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0;
-        cp_async_small<8>(z0, row, on);
-        cp_async_small<8>(z0 + 32 * ZB, row + 64, on);
-        cp_async_small<4>(dst + 32 * (8 * ZB + 32) + (i * 32 + lane) * 4, p.zscale + m * p.lds + block, on);
-      } else if constexpr (VEC) {
-        const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
-        cp_async16(z0, row + (c0 < a.D1 ? c0 : 0), on && c0 < a.D1);
-        cp_async16(z0 + 32 * ZB, row + (c0 + 64 < a.D1 ? c0 + 64 : 0), on && c0 + 64 < a.D1);
-      } else {
-        const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
-        *reinterpret_cast<uint4*>(z0) = load_row8<false>(row, c0, on ? a.D1 : 0);
-        *reinterpret_cast<uint4*>(z0 + 32 * ZB) = load_row8<false>(row, c0 + 64, on ? a.D1 : 0);
+      for (int i = 0; i < PIECES; ++i)
+        cp_async16(dst + frow * ROW + (((2 * i + fhalf) ^ (frow & 7)) << 4), row + 32 * i, on);
+    } else {
+      const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
+      const int64_t left = a.D1 - c0 - 8 * fhalf;  // columns from this lane's first piece
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        unsigned char* to = dst + frow * ROW + (((2 * i + fhalf) ^ (frow & 7)) << 4);
+        if constexpr (VEC)
+          cp_async16(to, row + (16 * i < left ? c0 + 8 * fhalf + 16 * i : 0), on && 16 * i < left);
+        else
+          *reinterpret_cast<uint4*>(to) = load_row8<false>(row, c0 + 8 * fhalf + 16 * i, on ? a.D1 : 0);
       }
-      cp_async_small<8>(dst + 32 * 8 * ZB + (i * 32 + lane) * 8, p.mid + (ranks ? m * a.r + j0 : 0), on && ranks);
     }
+    // 8 ranks of mid, and the row's scale
+    unsigned char* to = dst + 16 * ROW + frow * kGrMidPitch + 32 * fhalf;
+    const bool some = on && j < a.r;
+    const float* mid = p.mid + (some ? m * a.r + j : 0);
+    cp_async16(to, mid, some);
+    cp_async16(to + 16, mid + 4, some);
+    if (CODES && fhalf == 0)
+      cp_async_small<4>(dst + 16 * (ROW + kGrMidPitch) + frow * 4, p.zscale + m * p.lds + block, on);
     cp_async_commit();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = row_of(s + 1, i);
+    next = row_of(s + 1);
   };
   for (int s = 0; s < S - 1; ++s) fetch(s);
-
   for (int s = 0; s < steps; ++s) {
-    cp_async_wait<S - 2>();
+    fetch(s + S - 1);
+    cp_async_wait<S - 1>();
+    __syncwarp();
     const unsigned char* src = ring + (s % S) * STEP;
-    uint4 z[4][2];
+    // mid of rows 2t, 2t+1, 2t+8, 2t+9, ranks 2g and 2g+1 (n index g of the two n-tiles)
     float2 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned char* q = src + ((2 * i + h) * 32 + lane) * ZB;
-        if constexpr (CODES) {
-          const uint2 w = *reinterpret_cast<const uint2*>(q);
-          z[i][h] = make_uint4(w.x, w.y, 0u, 0u);
-        } else {
-          z[i][h] = *reinterpret_cast<const uint4*>(q);
-        }
-      }
-      v[i] = *reinterpret_cast<const float2*>(src + 32 * 8 * ZB + (i * 32 + lane) * 8);
+      const int row = 2 * t + (i & 1) + 4 * (i & 2);
+      v[i] = *reinterpret_cast<const float2*>(src + 16 * ROW + row * kGrMidPitch + 8 * g);
       if constexpr (CODES) {
-        const float f = *reinterpret_cast<const float*>(src + 32 * (8 * ZB + 32) + (i * 32 + lane) * 4);
+        const float f = *reinterpret_cast<const float*>(src + 16 * (ROW + kGrMidPitch) + row * 4);
         v[i].x *= f, v[i].y *= f;
       }
     }
-    fetch(s + S - 1);
     if constexpr (DT == RQ_F16) {
       // keep mid near 2^14 as fp16: when a step's largest value passes the
       // scale in use, the sums so far are scaled down to the new one
@@ -786,50 +841,50 @@ __global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_co
         ex_now = ex;
         mul = __uint_as_float((uint32_t)(268 - ex) << 23);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i].x *= mul, v[i].y *= mul;
     }
-    // B fragments: halves of mid at (rows 4t, 4t+1 | 4t+2, 4t+3) and rank j0 + n-tile
     uint32_t b[2][2][2];  // [half][n-tile][k pair]
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        split16x2<DT>((n ? v[2 * k].y : v[2 * k].x) * mul, (n ? v[2 * k + 1].y : v[2 * k + 1].x) * mul, &b[0][n][k],
-                      &b[1][n][k]);
+    for (int k = 0; k < 2; ++k) {
+      split16x2<DT>(v[2 * k].x, v[2 * k + 1].x, &b[0][0][k], &b[1][0][k]);
+      split16x2<DT>(v[2 * k].y, v[2 * k + 1].y, &b[0][1][k], &b[1][1][k]);
+    }
+    // A fragments: 8 x 8 pieces (rows 0-7 | 8-15) x (a piece | the next), transposed
+    const int lrow = (lane & 7) + 8 * (lane >> 4), lpiece = (lane >> 3) & 1;
+    const unsigned char* z = src + lrow * ROW;
+    uint32_t raw[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t f[4];  // (columns, columns + 64) x (rows 4t, 4t+1 | 4t+2, 4t+3)
+      uint32_t f[4];
+      if constexpr (CODES) {
+        // a piece holds 16 columns as 8 pairs: the even columns (i even) and the odd ones (i odd) of
+        // two pieces are an m-tile each
+        if (i % 2 == 0) ldmatrix4_trans(raw, z + (((i + lpiece) ^ (lrow & 7)) << 4));
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 &x = z[2 * k][h], &y = z[2 * k + 1][h];
-          if constexpr (CODES) {
-            const uint32_t w0 = i < 4 ? x.x : x.y, w1 = i < 4 ? y.x : y.y;
-            f[2 * k + h] = codes2<DT>(__byte_perm(w0, w1, (i & 3) | ((4 + (i & 3)) << 8)));
-          } else {
-            const uint32_t w0 = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;
-            const uint32_t w1 = i < 2 ? y.x : i < 4 ? y.y : i < 6 ? y.z : y.w;
-            f[2 * k + h] = __byte_perm(w0, w1, i & 1 ? 0x7632 : 0x5410);
-          }
-        }
+        for (int e = 0; e < 4; ++e) f[e] = codes2<DT>(i % 2 ? raw[e] >> 8 : raw[e]);
+      } else {
+        ldmatrix4_trans(f, z + (((2 * i + lpiece) ^ (lrow & 7)) << 4));
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
           Mma16816<DT>::run(acc[i][n], f[0], f[1], f[2], f[3], b[half][n][0], b[half][n][1]);
     }
+    __syncwarp();  // all lanes have read the step before its place is fetched into
   }
   cp_async_wait<0>();
   __syncthreads();  // the sums lie over the ring
 
-  // this warp's sums: column 8 g + i (+ 64) at row 8 i + g (+ 64), ranks 4t .. 4t+3
+  // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3
   const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
   float* mine = sums + mw * kGrCols * R16 + rg * 16 + 4 * t;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<float4*>(mine + (8 * i + g + 64 * h) * R16) =
+      *reinterpret_cast<float4*>(mine + (16 * i + g + 8 * h) * R16) =
           make_float4(acc[i][0][2 * h] * back, acc[i][1][2 * h] * back, acc[i][0][2 * h + 1] * back,
                       acc[i][1][2 * h + 1] * back);
   __syncthreads();
@@ -846,7 +901,8 @@ __global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_co
   const int units = R16 / 4;
   for (int i = tid * csize + crank; i < kGrCols * units; i += csize * kGrThreads) {
     const int at = i / units, j = (i - at * units) * 4;
-    const int64_t d = (int64_t)block * kGrCols + 8 * (at & 7) + ((at >> 3) & 7) + (at & 64);
+    // codes: m-tile i has the even (odd) columns of pieces i and i + 1, i even (odd)
+    const int64_t d = c0 + (CODES ? (at & ~31) + 2 * (at & 15) + ((at >> 4) & 1) : at);
     if (d >= a.D1 || j >= a.r) continue;
     const float4 s = cluster_sum<float4>(cluster, sums + at * R16 + j, csize);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
@@ -855,23 +911,43 @@ __global__ void __launch_bounds__(kGrThreads, 1) adapters_grad_k(const __grid_co
   cluster.sync();  // the others have read this CTA's sums
 }
 
+template <int DT, bool CODES, bool VEC, int S>
+static int launch_grad(const GradArgs& p, int64_t blocks, int csize, cudaStream_t st) {
+  const int ring = kGrWarps * S * gr_step_bytes(CODES), smem = ring > kGrSums ? ring : kGrSums;
+  return launch_cluster(adapters_grad_k<DT, CODES, VEC, S>, p, dim3((unsigned)(blocks * csize), (unsigned)p.a.count),
+                        kGrThreads, smem, csize, st);
+}
+
 template <int DT>
-static auto grad_kernel(bool codes, bool vec) {
-  return codes ? adapters_grad_k<DT, true, true> : vec ? adapters_grad_k<DT, false, true> : adapters_grad_k<DT, false, false>;
+static int launch_grad_dt(const GradArgs& p, bool vec, bool deep, int64_t blocks, int csize, cudaStream_t st) {
+  if (p.zscale) return deep ? launch_grad<DT, true, true, 7>(p, blocks, csize, st) : launch_grad<DT, true, true, 3>(p, blocks, csize, st);
+  if (!vec) return launch_grad<DT, false, false, 2>(p, blocks, csize, st);
+  return deep ? launch_grad<DT, false, true, 5>(p, blocks, csize, st) : launch_grad<DT, false, true, 2>(p, blocks, csize, st);
 }
 
 int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
                   void* G, cudaStream_t st) {
   GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8};
-  // Rows are split over a cluster until the grid fills the GPU, as long as a
-  // warp keeps two steps of 16 rows of an adapter of mean size.
-  const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols, each = a.M / a.count * p.groups / (kGrWarps * 32);
+  const bool vec = rows16b(z, ldz) && a.D1 % 8 == 0;
+  const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols;
+  // A CTA costs about as much as 5 steps besides its steps (its sums through
+  // shared memory, the cluster's meetings); the cluster size that takes the
+  // fewest steps over all rounds of the GPU, for adapters of mean size.
+  const int64_t per_step = kGrWarps / p.groups * 16, each = (a.M + a.count - 1) / a.count;
+  // Above rank 64 all warps read the same rows and the tensor cores wait for
+  // L1: one CTA an SM with a deeper ring takes 116 instead of 140 us at 8192
+  // rows, 4096 columns, rank 128.  At rank 16 and 11008 columns it is the two
+  // CTAs that win, 51 against 59 us.
+  const bool deep = p.groups == 8;
+  const int64_t slots = (deep ? 1 : 2) * num_sms();
   int csize = 1;
-  while (csize < 8 && csize * 2 <= each && blocks * csize < num_sms()) csize *= 2;
-  const bool codes = zscale != nullptr, vec = rows16b(z, ldz) && a.D1 % 8 == 0;
-  auto* kern = a.dt == RQ_BF16 ? grad_kernel<RQ_BF16>(codes, vec) : grad_kernel<RQ_F16>(codes, vec);
-  const int ring = kGrWarps * gr_stages(codes) * gr_step_bytes(codes), smem = ring > kGrSums ? ring : kGrSums;
-  return launch_cluster(kern, p, dim3((unsigned)(blocks * csize), (unsigned)a.count), kGrThreads, smem, csize, st);
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= 8; ++c) {
+    const int64_t rounds = (blocks * a.count * c + slots - 1) / slots, steps = (each + per_step * c - 1) / (per_step * c);
+    if (rounds * (5 + steps) < best) best = rounds * (5 + steps), csize = c;
+  }
+  return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, vec, deep, blocks, csize, st)
+                         : launch_grad_dt<RQ_F16>(p, vec, deep, blocks, csize, st);
 }
 
 }  // namespace rq
