@@ -382,10 +382,11 @@ RQ_API int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t
 /* logits [B, L, V] (strides in elements, V contiguous), labels [B, L] int64
  * contiguous: position l is scored on labels[b, l + 1]; a label equal to
  * `ignore` (and the last position) does not count, and a label outside
- * [0, V) gives NaN.  rq_token_logprobs writes stats [B, L, 4] fp32 (row
- * maximum, sum of exp(x - maximum), the label's logit; rows that do not count
- * are left as they are), 16-byte aligned, and, unless NULL, logps [B, L]:
- * the log-probability of each label, 0 where it does not count. */
+ * [0, V) gives NaN.  rq_token_logprobs writes stats [B, L, 4] fp32, 16-byte
+ * aligned (k, s, hi, lo: the sum of the row's exponentials is s 2^k, the
+ * label's log-probability hi + lo; rows that do not count are left as they
+ * are) and, unless NULL, logps [B, L]: the log-probability of each label, 0
+ * where it does not count. */
 RQ_API int rq_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_l,
                       int64_t B, int64_t L, int64_t V, const int64_t* labels, int64_t ignore,
                       float* stats, float* logps, void* stream);

@@ -17,7 +17,8 @@
 
 namespace rq {
 
-constexpr int kTokThreads = 256;
+constexpr int kTokThreads = 512, kTokBatch = 4;  // 16-byte loads of a thread at a time
+constexpr float kLog2e = 1.4426950408889634f;
 
 // The label that scores row `at` of B * L; false where the row does not count.
 __device__ __forceinline__ bool row_label(const TokenRows& t, int64_t at, int64_t* y) {
@@ -33,14 +34,98 @@ __device__ __forceinline__ const typename DType<DT>::T* row_of(const TokenRows& 
   return static_cast<const typename DType<DT>::T*>(t.logits) + b * t.sb + l * t.sl;
 }
 
-// stats[at] = (m, s, x_y, 0) of each row that counts; logps (optional), at the
-// label's own place [b, l + 1], is log p and 0 where nothing counts.
+// A row cut at 16-byte boundaries: `head` values, `vecs` loads, `tail` values.
+template <int DT>
+struct RowCut {
+  using T = typename DType<DT>::T;
+  static constexpr int E = 16 / (int)sizeof(T);
+  int head, vecs, tail;
+  __device__ RowCut(const T* x, int V) {
+    head = min(V, (int)((16u - ((uint32_t)(uintptr_t)x & 15u)) & 15u) / (int)sizeof(T));
+    vecs = (V - head) / E;
+    tail = V - head - vecs * E;
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void unpack16(const uint4& q, float* f) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == RQ_F32) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (DT == RQ_BF16) {
+      f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack16x2(float lo, float hi) {
+  if constexpr (DT == RQ_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A running sum of e^x as s * 2^k, k whole.  With a whole k the shift costs no
+// rounding: e^x = 2^(x log2(e) - k) is one fused multiply-add and one
+// exponential a value, and moving k scales s by a power of two.  k follows
+// the maximum only when a value would pass 2^64.
+struct ExpSum {
+  float k = 0.0f, s = 0.0f;
+  __device__ __forceinline__ void raise(float top) {  // top: the largest of the values to come
+    const float z = top * kLog2e;
+    if (z - k > 64.0f || s == 0.0f) {
+      if (fabsf(z) < INFINITY) {
+        const float to = rintf(z);
+        if (s != 0.0f) s *= exp2_fast(k - to);
+        k = to;
+      }
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N]) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+    raise(top);
+    float e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = exp2_fast(fmaf(x[i], kLog2e, -k));
+#pragma unroll
+    for (int w = N / 2; w > 0; w /= 2)
+#pragma unroll
+      for (int i = 0; i < w; ++i) e[i] += e[i + w];
+    s += e[0];
+  }
+};
+
+// stats[at] = (k, s, hi, lo) of each row that counts: the normaliser s 2^k and
+// the label's log-probability hi + lo; logps (optional) has it at the label's
+// own place [b, l + 1], and 0 where nothing counts.  One CTA a row, one pass:
+// HBM bound, with the exponentials at 72 % of the time a row takes to arrive.
 template <int DT>
 __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4* __restrict__ stats,
                                                              float* __restrict__ logps) {
+  using T = typename DType<DT>::T;
+  constexpr int E = RowCut<DT>::E;
   const int64_t at = blockIdx.x;
   const int tid = threadIdx.x;
-  __shared__ float red[kTokThreads / 32];
+  __shared__ float ks[kTokThreads / 32];
+  __shared__ double sums[kTokThreads / 32];
   int64_t y;
   const bool counts = row_label(t, at, &y);
   if (logps && tid == 0) {
@@ -48,114 +133,159 @@ __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4
     if (!counts && at % t.L + 1 < t.L) logps[at + 1] = 0.0f;
   }
   if (!counts) return;
-  const typename DType<DT>::T* x = row_of<DT>(t, at);
-  float m = -INFINITY;
-  bool bad = false;
-  for (int64_t v = tid; v < t.V; v += kTokThreads) {
-    const float f = DType<DT>::to_f32(x[v]);
-    bad |= isnan(f);
-    m = fmaxf(m, f);
-  }
-  if (bad) m = __uint_as_float(0x7fc00000u);
+  const T* x = row_of<DT>(t, at);
+  const RowCut<DT> cut(x, (int)t.V);
+  const uint4* body = reinterpret_cast<const uint4*>(x + cut.head);
+  ExpSum sum;
+  for (int i = tid; i < cut.vecs; i += kTokBatch * kTokThreads) {
+    uint4 q[kTokBatch];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float u = __shfl_xor_sync(0xffffffffu, m, o);
-    m = (isnan(u) || isnan(m)) ? __uint_as_float(0x7fc00000u) : fmaxf(m, u);
+    for (int j = 0; j < kTokBatch; ++j) {
+      const uint32_t low = DT == RQ_F32 ? 0xff800000u : DT == RQ_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+      q[j] = i + j * kTokThreads < cut.vecs ? body[i + j * kTokThreads] : make_uint4(low, low, low, low);
+    }
+    float f[kTokBatch * E];
+#pragma unroll
+    for (int j = 0; j < kTokBatch; ++j) unpack16<DT>(q[j], f + j * E);
+    sum.add(f);
   }
-  if ((tid & 31) == 0) red[tid >> 5] = m;
+  // the ends of a row that does not start or end on a 16-byte boundary
+  if (tid < cut.head + cut.tail) {
+    const float f[1] = {DType<DT>::to_f32(x[tid < cut.head ? tid : t.V - cut.tail + (tid - cut.head)])};
+    sum.add(f);
+  }
+  // the threads' sums meet at the largest k, in 64 bits
+  float k = sum.s == 0.0f ? -INFINITY : sum.k;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) k = fmaxf(k, __shfl_xor_sync(0xffffffffu, k, o));
+  if ((tid & 31) == 0) ks[tid >> 5] = k;
   __syncthreads();
-  for (int w = 0; w < kTokThreads / 32; ++w) m = (isnan(red[w]) || isnan(m)) ? __uint_as_float(0x7fc00000u) : fmaxf(m, red[w]);
-  __syncthreads();
-  float s = 0.0f;
-  for (int64_t v = tid; v < t.V; v += kTokThreads) s += expf(DType<DT>::to_f32(x[v]) - m);
+  k = ks[0];
+#pragma unroll
+  for (int w = 1; w < kTokThreads / 32; ++w) k = fmaxf(k, ks[w]);
+  double s = sum.s == 0.0f ? 0.0 : (double)sum.s * (double)exp2_fast(sum.k - k);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((tid & 31) == 0) red[tid >> 5] = s;
+  if ((tid & 31) == 0) sums[tid >> 5] = s;
   __syncthreads();
   if (tid == 0) {
-    s = 0.0f;
-    for (int w = 0; w < kTokThreads / 32; ++w) s += red[w];
+    s = sums[0];
+    for (int w = 1; w < kTokThreads / 32; ++w) s += sums[w];
+    // no finite logit at all, an infinity or a NaN among them: not a distribution
+    if (!(s > 0.0 && s < (double)INFINITY)) s = (double)__uint_as_float(0x7fc00000u);
     // a label outside the vocabulary has no probability: NaN, not a read past the row
     const float xy = y >= 0 && y < t.V ? DType<DT>::to_f32(x[y]) : __uint_as_float(0x7fc00000u);
-    stats[at] = make_float4(m, s, xy, 0.0f);
-    if (logps) logps[at + 1] = (float)((double)(xy - m) - log((double)s));
+    // in base 2 with the same fp32 log2(e) throughout, whose error then drops out
+    const double lp = ((double)xy * (double)kLog2e - (double)k - log2(s)) / (double)kLog2e;
+    const float hi = (float)lp;
+    stats[at] = make_float4(k, (float)s, hi, fabsf(hi) < INFINITY ? (float)(lp - (double)hi) : 0.0f);
+    if (logps) logps[at + 1] = hi;
   }
 }
 
 // One CTA: sums per sequence in 64 bits (thousands of tokens, of which the
 // loss takes a small difference), then the loss and each sequence's slope.
-__global__ void __launch_bounds__(1024) preference_loss_k(TokenRows t, const float4* __restrict__ stats,
-                                                          const float* __restrict__ ref, int form, float beta,
-                                                          float smooth, float* __restrict__ loss,
-                                                          float* __restrict__ logps, float* __restrict__ rewards,
-                                                          float* __restrict__ slopes) {
+// A sequence's rows are dealt to its warps, all 32 of them for one sequence.
+constexpr int kPrefWarps = 32;
+
+struct SequenceSum {
+  double lp, d;  // of log p, and of log p - ref
+  int n;
+};
+
+__global__ void __launch_bounds__(kPrefWarps * 32) preference_loss_k(TokenRows t, const float4* __restrict__ stats,
+                                                                     const float* __restrict__ ref, int form,
+                                                                     float beta, float smooth,
+                                                                     float* __restrict__ loss,
+                                                                     float* __restrict__ logps,
+                                                                     float* __restrict__ rewards,
+                                                                     float* __restrict__ slopes) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ double part[32];
-  const int64_t P = t.B / 2;
-  double mine = 0.0;  // warp's pairs, in order
-  for (int64_t i = warp; i < P; i += 32) {
-    double R[2], n[2];
-    for (int h = 0; h < 2; ++h) {
-      const int64_t b = i + h * P;
-      double lp = 0.0, rf = 0.0;
-      int cnt = 0;
-      for (int64_t l = lane; l + 1 < t.L; l += 32) {
+  __shared__ SequenceSum part[kPrefWarps];
+  __shared__ double total[kPrefWarps];
+  const int P = (int)(t.B / 2);
+  // warps of a sequence; pairs at a time
+  int ws = kPrefWarps / 2;
+  while (ws > 1 && 2 * P * ws > kPrefWarps) ws /= 2;
+  const int at_once = kPrefWarps / (2 * ws), slot = warp / ws;  // slot: pair and half
+  double mine = 0.0;  // of thread 0 of each pair's slot
+  for (int i0 = 0; i0 < P; i0 += at_once) {
+    const int i = i0 + slot / 2, b = i + (slot & 1) * P;
+    SequenceSum s{0.0, 0.0, 0};
+    if (i < P) {
+      for (int64_t l = (warp % ws) * 32 + lane; l + 1 < t.L; l += ws * 32) {
         int64_t y;
         if (!row_label(t, b * t.L + l, &y)) continue;
         const float4 q = stats[b * t.L + l];
-        lp += (double)(q.z - q.x) - log((double)q.y);
-        rf += (double)ref[b * t.L + l + 1];
-        ++cnt;
-      }
-      double d = lp - rf;
-      for (int o = 16; o > 0; o >>= 1) {
-        lp += __shfl_xor_sync(0xffffffffu, lp, o);
-        d += __shfl_xor_sync(0xffffffffu, d, o);
-        cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
-      }
-      R[h] = d;
-      n[h] = cnt > 0 ? cnt : 1;
-      if (lane == 0) {
-        logps[b] = (float)lp;
-        rewards[b] = (float)(beta * d);
+        const double lp = (double)q.z + (double)q.w;
+        s.lp += lp;
+        s.d += lp - (double)ref[b * t.L + l + 1];
+        ++s.n;
       }
     }
-    double slope, s0, s1;
-    if (form == RQ_PREF_IPO) {
-      const double off = R[0] / n[0] - R[1] / n[1] - 0.5 / beta;
-      mine += off * off;
-      slope = 2.0 * off / P;
-      s0 = slope / n[0], s1 = -slope / n[1];
-    } else {
-      const double z = beta * (R[0] - R[1]), soft = log1p(exp(-fabs(z)));
-      mine += (1.0 - smooth) * (soft + fmax(-z, 0.0)) + smooth * (soft + fmax(z, 0.0));
-      slope = beta * (1.0 / (1.0 + exp(-z)) - (1.0 - smooth)) / P;
-      s0 = slope, s1 = -slope;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s.lp += __shfl_xor_sync(0xffffffffu, s.lp, o);
+      s.d += __shfl_xor_sync(0xffffffffu, s.d, o);
+      s.n += __shfl_xor_sync(0xffffffffu, s.n, o);
     }
-    if (lane == 0) {
+    if (lane == 0) part[warp] = s;
+    __syncthreads();
+    if (lane == 0 && warp % (2 * ws) == 0 && i < P) {
+      SequenceSum h[2];
+      for (int k = 0; k < 2; ++k) {
+        h[k] = part[warp + k * ws];
+        for (int w = 1; w < ws; ++w) {
+          const SequenceSum& q = part[warp + k * ws + w];
+          h[k].lp += q.lp, h[k].d += q.d, h[k].n += q.n;
+        }
+        logps[i + k * P] = (float)h[k].lp;
+        rewards[i + k * P] = (float)(beta * h[k].d);
+      }
+      double s0, s1;
+      if (form == RQ_PREF_IPO) {
+        const double n0 = max(h[0].n, 1), n1 = max(h[1].n, 1);
+        const double off = h[0].d / n0 - h[1].d / n1 - 0.5 / beta;
+        mine += off * off;
+        s0 = 2.0 * off / P / n0, s1 = -2.0 * off / P / n1;
+      } else {
+        const double z = beta * (h[0].d - h[1].d), soft = log1p(exp(-fabs(z)));
+        mine += (1.0 - smooth) * (soft + fmax(-z, 0.0)) + smooth * (soft + fmax(z, 0.0));
+        s0 = beta * (1.0 / (1.0 + exp(-z)) - (1.0 - smooth)) / P;
+        s1 = -s0;
+      }
       slopes[i] = (float)s0;
       slopes[i + P] = (float)s1;
     }
+    __syncthreads();
   }
-  if (lane == 0) part[warp] = mine;
+  if (lane == 0) total[warp] = mine;
   __syncthreads();
   if (tid == 0) {
     double all = 0.0;
-    for (int w = 0; w < 32; ++w) all += part[w];
+    for (int w = 0; w < kPrefWarps; ++w) all += total[w];
     *loss = (float)(all / P);
   }
 }
 
+// dlogits = c ([v = y] - 2^(x log2(e) - k) / s), zero where the row does not
+// count.  One CTA a row, the rows in the reverse of the forward's order, so
+// that the last rows it read are still in L2.  HBM bound.
 template <int DT>
 __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const float4* __restrict__ stats,
                                                             const float* __restrict__ slopes, int per_token,
                                                             const float* __restrict__ upstream, void* __restrict__ out) {
   using T = typename DType<DT>::T;
-  const int64_t at = blockIdx.x;
+  constexpr int E = RowCut<DT>::E;
+  const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
+  const int tid = threadIdx.x;
   T* d = static_cast<T*>(out) + at * t.V;
   int64_t y;
   if (!row_label(t, at, &y)) {
-    for (int64_t v = threadIdx.x; v < t.V; v += kTokThreads) d[v] = DType<DT>::from_f32(0.0f);
+    const RowCut<DT> cut(d, (int)t.V);
+    uint4* body = reinterpret_cast<uint4*>(d + cut.head);
+    for (int i = tid; i < cut.vecs; i += kTokThreads) __stcs(body + i, make_uint4(0u, 0u, 0u, 0u));
+    if (tid < cut.head + cut.tail) d[tid < cut.head ? tid : t.V - cut.tail + (tid - cut.head)] = DType<DT>::from_f32(0.0f);
     return;
   }
   const T* x = row_of<DT>(t, at);
@@ -163,9 +293,47 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
   float c = per_token ? slopes[at + 1] : slopes[at / t.L];
   if (upstream) c *= *upstream;
   if (y < 0 || y >= t.V) c = __uint_as_float(0x7fc00000u);
-  const float k = -c / q.y;
-  for (int64_t v = threadIdx.x; v < t.V; v += kTokThreads)
-    d[v] = DType<DT>::from_f32(fmaf(k, expf(DType<DT>::to_f32(x[v]) - q.x), v == y ? c : 0.0f));
+  const float by = -c / q.y, k = -q.x;
+  auto value = [&](float f) { return by * exp2_fast(fmaf(f, kLog2e, k)); };
+  if ((((uintptr_t)x ^ (uintptr_t)d) & 15) == 0) {
+    const RowCut<DT> cut(x, (int)t.V);
+    const uint4* src = reinterpret_cast<const uint4*>(x + cut.head);
+    uint4* dst = reinterpret_cast<uint4*>(d + cut.head);
+    const int hit = y >= cut.head ? (int)(y - cut.head) / E : -1, which = (int)(y - cut.head) % E;  // the label's load
+    for (int i = tid; i < cut.vecs; i += kTokBatch * kTokThreads) {
+      uint4 v[kTokBatch];
+#pragma unroll
+      for (int j = 0; j < kTokBatch; ++j)
+        if (i + j * kTokThreads < cut.vecs) v[j] = __ldcs(src + i + j * kTokThreads);
+#pragma unroll
+      for (int j = 0; j < kTokBatch; ++j) {
+        const int at_vec = i + j * kTokThreads;
+        if (at_vec >= cut.vecs) continue;
+        float f[E];
+        unpack16<DT>(v[j], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = value(f[e]);
+        if (at_vec == hit) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] += e == which ? c : 0.0f;
+        }
+        uint4 r;
+        if constexpr (DT == RQ_F32)
+          r = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        else
+          r = make_uint4(pack16x2<DT>(f[0], f[1]), pack16x2<DT>(f[2], f[3]), pack16x2<DT>(f[E - 4], f[E - 3]),
+                         pack16x2<DT>(f[E - 2], f[E - 1]));
+        __stcs(dst + at_vec, r);
+      }
+    }
+    if (tid < cut.head + cut.tail) {
+      const int64_t v = tid < cut.head ? tid : t.V - cut.tail + (tid - cut.head);
+      d[v] = DType<DT>::from_f32(value(DType<DT>::to_f32(x[v])) + (v == y ? c : 0.0f));
+    }
+  } else {  // rows of different alignment: value by value
+    for (int64_t v = tid; v < t.V; v += kTokThreads)
+      d[v] = DType<DT>::from_f32(value(DType<DT>::to_f32(x[v])) + (v == y ? c : 0.0f));
+  }
 }
 
 #define RQ_TOK_LAUNCH(kern, ...)                                                                  \
@@ -183,7 +351,7 @@ int token_logprobs(const TokenRows& t, float* stats, float* logps, cudaStream_t 
 
 int preference_loss(const TokenRows& t, const float* stats, const float* ref, int form, float beta, float smooth,
                     float* loss, float* logps, float* rewards, float* slopes, cudaStream_t st) {
-  preference_loss_k<<<1, 1024, 0, st>>>(t, (const float4*)stats, ref, form, beta, smooth, loss, logps, rewards, slopes);
+  preference_loss_k<<<1, kPrefWarps * 32, 0, st>>>(t, (const float4*)stats, ref, form, beta, smooth, loss, logps, rewards, slopes);
   return check_launch();
 }
 
