@@ -11,13 +11,17 @@
 //   ipo:     loss = mean((R_i / n_i - R_{i+P} / n_{i+P} - 1 / (2 beta))^2)
 // and the gradient of every logit row of a sequence is one slope (dloss / dR)
 // times the row's derivative above.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
-#include "linear_common.cuh"
+#include "gemv_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace rq {
 
-constexpr int kTokThreads = 512, kTokBatch = 4;  // 16-byte loads of a thread at a time
+constexpr int kTokThreads = 512;  // of a row, in the gradient and where rows are few
+constexpr int kTokBatch = 4;      // 16-byte loads of a thread at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The label that scores row `at` of B * L; false where the row does not count.
@@ -115,18 +119,23 @@ struct ExpSum {
 
 // stats[at] = (k, s, hi, lo) of each row that counts: the normaliser s 2^k and
 // the label's log-probability hi + lo; logps (optional) has it at the label's
-// own place [b, l + 1], and 0 where nothing counts.  One CTA a row, one pass:
-// HBM bound, with the exponentials at 72 % of the time a row takes to arrive.
-template <int DT>
-__global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4* __restrict__ stats,
+// own place [b, l + 1], and 0 where nothing counts.  One CTA a row, one pass;
+// bound by HBM, with the exponentials (16 a clock of an SM) at 72 % of the
+// time a bf16 row takes to arrive.  The end of a row is a few serial steps, so
+// where rows are many, small CTAs of which eight share an SM hide it: 16384
+// rows of 32000 bf16 logits take 155 us with 128 threads (6.1 TB/s) and 244
+// with 512, but 128 rows 5.8 and 4.6 us.
+template <int DT, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, float4* __restrict__ stats,
                                                              float* __restrict__ logps) {
   using T = typename DType<DT>::T;
   constexpr int E = RowCut<DT>::E;
   const int64_t at = blockIdx.x;
   const int tid = threadIdx.x;
-  __shared__ float ks[kTokThreads / 32];
-  __shared__ double sums[kTokThreads / 32];
+  __shared__ float ks[TH / 32];
+  __shared__ double sums[TH / 32];
   int64_t y;
+  asm volatile("griddepcontrol.launch_dependents;");  // the loss kernel may come up; it waits for this grid
   const bool counts = row_label(t, at, &y);
   if (logps && tid == 0) {
     if (at % t.L == 0) logps[at] = 0.0f;
@@ -137,12 +146,12 @@ __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4
   const RowCut<DT> cut(x, (int)t.V);
   const uint4* body = reinterpret_cast<const uint4*>(x + cut.head);
   ExpSum sum;
-  for (int i = tid; i < cut.vecs; i += kTokBatch * kTokThreads) {
+  for (int i = tid; i < cut.vecs; i += kTokBatch * TH) {
     uint4 q[kTokBatch];
 #pragma unroll
     for (int j = 0; j < kTokBatch; ++j) {
       const uint32_t low = DT == RQ_F32 ? 0xff800000u : DT == RQ_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
-      q[j] = i + j * kTokThreads < cut.vecs ? body[i + j * kTokThreads] : make_uint4(low, low, low, low);
+      q[j] = i + j * TH < cut.vecs ? body[i + j * TH] : make_uint4(low, low, low, low);
     }
     float f[kTokBatch * E];
 #pragma unroll
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4
   __syncthreads();
   k = ks[0];
 #pragma unroll
-  for (int w = 1; w < kTokThreads / 32; ++w) k = fmaxf(k, ks[w]);
+  for (int w = 1; w < TH / 32; ++w) k = fmaxf(k, ks[w]);
   double s = sum.s == 0.0f ? 0.0 : (double)sum.s * (double)exp2_fast(sum.k - k);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4
   __syncthreads();
   if (tid == 0) {
     s = sums[0];
-    for (int w = 1; w < kTokThreads / 32; ++w) s += sums[w];
+    for (int w = 1; w < TH / 32; ++w) s += sums[w];
     // no finite logit at all, an infinity or a NaN among them: not a distribution
     if (!(s > 0.0 && s < (double)INFINITY)) s = (double)__uint_as_float(0x7fc00000u);
     // a label outside the vocabulary has no probability: NaN, not a read past the row
@@ -183,44 +192,57 @@ __global__ void __launch_bounds__(kTokThreads) token_stats_k(TokenRows t, float4
   }
 }
 
-// One CTA: sums per sequence in 64 bits (thousands of tokens, of which the
-// loss takes a small difference), then the loss and each sequence's slope.
-// A sequence's rows are dealt to its warps, all 32 of them for one sequence.
-constexpr int kPrefWarps = 32;
+// Sums per sequence in 64 bits (thousands of tokens, of which the loss takes a
+// small difference), then the loss and each sequence's slope.  One cluster:
+// pairs are dealt to its CTAs, a pair's two sequences to `ws` warps each, and
+// the loss's terms meet in rank order.
+constexpr int kPrefWarps = 32, kPrefCtas = 8;
 
 struct SequenceSum {
   double lp, d;  // of log p, and of log p - ref
   int n;
 };
 
-__global__ void __launch_bounds__(kPrefWarps * 32) preference_loss_k(TokenRows t, const float4* __restrict__ stats,
-                                                                     const float* __restrict__ ref, int form,
-                                                                     float beta, float smooth,
-                                                                     float* __restrict__ loss,
-                                                                     float* __restrict__ logps,
-                                                                     float* __restrict__ rewards,
-                                                                     float* __restrict__ slopes) {
+__global__ void __launch_bounds__(kPrefWarps * 32) __cluster_dims__(kPrefCtas, 1, 1)
+    preference_loss_k(TokenRows t, const float4* __restrict__ stats, const float* __restrict__ ref, int form,
+                      float beta, float smooth, float* __restrict__ loss, float* __restrict__ logps,
+                      float* __restrict__ rewards, float* __restrict__ slopes) {
+  constexpr int U = 4;  // rows of a lane under way
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cg::cluster_group cluster = cg::this_cluster();
   __shared__ SequenceSum part[kPrefWarps];
   __shared__ double total[kPrefWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' sums
   const int P = (int)(t.B / 2);
-  // warps of a sequence; pairs at a time
-  int ws = kPrefWarps / 2;
-  while (ws > 1 && 2 * P * ws > kPrefWarps) ws /= 2;
+  int ws = kPrefWarps / 2;  // warps of a sequence: fewer where that leaves lanes without a row
+  while (ws > 1 && ws * 32 >= 2 * t.L) ws /= 2;
   const int at_once = kPrefWarps / (2 * ws), slot = warp / ws;  // slot: pair and half
-  double mine = 0.0;  // of thread 0 of each pair's slot
-  for (int i0 = 0; i0 < P; i0 += at_once) {
+  double mine = 0.0;  // of the first lane of a pair's warps
+  for (int i0 = blockIdx.x * at_once; i0 < P; i0 += kPrefCtas * at_once) {
     const int i = i0 + slot / 2, b = i + (slot & 1) * P;
     SequenceSum s{0.0, 0.0, 0};
     if (i < P) {
-      for (int64_t l = (warp % ws) * 32 + lane; l + 1 < t.L; l += ws * 32) {
-        int64_t y;
-        if (!row_label(t, b * t.L + l, &y)) continue;
-        const float4 q = stats[b * t.L + l];
-        const double lp = (double)q.z + (double)q.w;
-        s.lp += lp;
-        s.d += lp - (double)ref[b * t.L + l + 1];
-        ++s.n;
+      const int64_t row0 = (int64_t)b * t.L;
+      for (int64_t l0 = (warp % ws) * 32 + lane; l0 + 1 < t.L; l0 += U * ws * 32) {
+        int64_t y[U];
+        float4 q[U];
+        float r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t l = l0 + u * ws * 32;
+          const bool in = l + 1 < t.L;
+          y[u] = in ? t.labels[row0 + l + 1] : t.ignore;
+          q[u] = in ? stats[row0 + l] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          r[u] = in ? ref[row0 + l + 1] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (y[u] == t.ignore) continue;
+          const double lp = (double)q[u].z + (double)q[u].w;
+          s.lp += lp;
+          s.d += lp - (double)r[u];
+          ++s.n;
+        }
       }
     }
 #pragma unroll
@@ -260,12 +282,15 @@ __global__ void __launch_bounds__(kPrefWarps * 32) preference_loss_k(TokenRows t
     __syncthreads();
   }
   if (lane == 0) total[warp] = mine;
-  __syncthreads();
-  if (tid == 0) {
+  cluster.sync();
+  if (blockIdx.x == 0 && warp == 0) {  // lane w: warp w of every CTA
     double all = 0.0;
-    for (int w = 0; w < kPrefWarps; ++w) all += total[w];
-    *loss = (float)(all / P);
+    for (int c = 0; c < kPrefCtas; ++c) all += *cluster.map_shared_rank(&total[lane], c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) *loss = (float)(all / P);
   }
+  cluster.sync();  // the others' terms have been read
 }
 
 // dlogits = c ([v = y] - 2^(x log2(e) - k) / s), zero where the row does not
@@ -336,28 +361,48 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
   }
 }
 
-#define RQ_TOK_LAUNCH(kern, ...)                                                                  \
-  do {                                                                                            \
-    const unsigned grid = (unsigned)(t.B * t.L);                                                  \
-    if (t.dt == RQ_F32) kern<RQ_F32><<<grid, kTokThreads, 0, st>>>(__VA_ARGS__);                  \
-    else if (t.dt == RQ_BF16) kern<RQ_BF16><<<grid, kTokThreads, 0, st>>>(__VA_ARGS__);           \
-    else kern<RQ_F16><<<grid, kTokThreads, 0, st>>>(__VA_ARGS__);                                 \
-    return check_launch();                                                                        \
-  } while (0)
+template <int DT>
+static void launch_stats(const TokenRows& t, float4* stats, float* logps, cudaStream_t st) {
+  const unsigned grid = (unsigned)(t.B * t.L);
+  if (grid >= 8u * num_sms()) token_stats_k<DT, 128><<<grid, 128, 0, st>>>(t, stats, logps);
+  else token_stats_k<DT, kTokThreads><<<grid, kTokThreads, 0, st>>>(t, stats, logps);
+}
 
 int token_logprobs(const TokenRows& t, float* stats, float* logps, cudaStream_t st) {
-  RQ_TOK_LAUNCH(token_stats_k, t, (float4*)stats, logps);
+  if (t.dt == RQ_F32) launch_stats<RQ_F32>(t, (float4*)stats, logps, st);
+  else if (t.dt == RQ_BF16) launch_stats<RQ_BF16>(t, (float4*)stats, logps, st);
+  else launch_stats<RQ_F16>(t, (float4*)stats, logps, st);
+  return check_launch();
 }
 
 int preference_loss(const TokenRows& t, const float* stats, const float* ref, int form, float beta, float smooth,
                     float* loss, float* logps, float* rewards, float* slopes, cudaStream_t st) {
-  preference_loss_k<<<1, kPrefWarps * 32, 0, st>>>(t, (const float4*)stats, ref, form, beta, smooth, loss, logps, rewards, slopes);
+  // the programmatic dependent of the kernel before it: it comes up while that
+  // one's last rows run, and waits for all of it before its first load
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kPrefCtas);
+  cfg.blockDim = dim3(kPrefWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, preference_loss_k, t, (const float4*)stats, ref, form, beta, smooth,
+                                           loss, logps, rewards, slopes);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
+  }
   return check_launch();
 }
 
 int token_logprobs_grad(const TokenRows& t, const float* stats, const float* slopes, int per_token,
                         const float* upstream, void* dlogits, cudaStream_t st) {
-  RQ_TOK_LAUNCH(token_grad_k, t, (const float4*)stats, slopes, per_token, upstream, dlogits);
+  const unsigned grid = (unsigned)(t.B * t.L);
+  auto* kern = t.dt == RQ_F32 ? token_grad_k<RQ_F32> : t.dt == RQ_BF16 ? token_grad_k<RQ_BF16> : token_grad_k<RQ_F16>;
+  kern<<<grid, kTokThreads, 0, st>>>(t, (const float4*)stats, slopes, per_token, upstream, dlogits);
+  return check_launch();
 }
 
 }  // namespace rq
