@@ -6,6 +6,8 @@
 // only give shapes.
 #include "torch_ops.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+
 #include <tuple>
 
 namespace {
@@ -258,6 +260,123 @@ Tensor token_logprobs_grad(const Tensor& logits, const Tensor& labels, int64_t i
   return d;
 }
 
+// ---- the differentiable entry points: one dispatcher call forward, and a
+// backward that never enters Python
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "rocm_qlora: ", what, " is differentiable once only");
+}
+
+Tensor rows_of(const Tensor& t) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
+
+struct AdaptersAdd : Function<AdaptersAdd> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B,
+                        const Tensor& scaling, const optional<Tensor>& plan, int64_t tile,
+                        const optional<Tensor>& codes, const optional<Tensor>& scales) {
+    auto [y, mid] = adapters_apply(x, A, B, scaling, base, plan, tile);
+    const bool packed = codes.has_value();
+    ctx->save_for_backward({packed ? *codes : x, packed ? *scales : Tensor(), A, B, scaling, mid, plan.value_or(Tensor())});
+    ctx->saved_data["tile"] = tile;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("adapters_add");
+    const auto v = ctx->get_saved_variables();
+    const Tensor &z = v[0], &A = v[2], &B = v[3], &scaling = v[4], &mid = v[5];
+    const optional<Tensor> scales = some(v[1]), plan = some(v[6]);
+    const int64_t tile = ctx->saved_data["tile"].toInt();
+    const Tensor dy = rows_of(grads[0]);
+    Tensor dx, dA, dB, gmid;
+    if (ctx->needs_input_grad(1)) std::tie(dx, gmid) = adapters_apply(dy, B, A, scaling, std::nullopt, plan, tile);
+    else if (ctx->needs_input_grad(2)) gmid = adapters_mid(dy, B, A, scaling, plan, tile);
+    if (ctx->needs_input_grad(2)) dA = adapters_grad(z, scales, gmid, A.size(1), A.size(0), A.scalar_type(), plan, tile);
+    if (ctx->needs_input_grad(3)) dB = adapters_grad(dy, std::nullopt, mid, B.size(1), B.size(0), B.scalar_type(), plan, tile);
+    return {ctx->needs_input_grad(0) ? grads[0] : Tensor(), dx, dA, dB, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& scaling,
+                    const optional<Tensor>& plan, int64_t tile, const optional<Tensor>& codes,
+                    const optional<Tensor>& scales) {
+  return AdaptersAdd::apply(base, x, A, B, scaling, plan, tile, codes, scales);
+}
+
+struct Swiglu8 : Function<Swiglu8> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up, int64_t copies) {
+    auto [h, codes, scales] = swiglu8_forward(rows_of(gate), rows_of(up), copies);
+    ctx->save_for_backward({codes.narrow(0, 0, 2), scales.narrow(0, 0, 2)});
+    ctx->saved_data["shape"] = gate.sizes().vec();
+    ctx->mark_non_differentiable({codes, scales});
+    return {h.view(gate.sizes()), codes, scales};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("swiglu8");
+    const auto v = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    auto [dgate, dup] = swiglu8_backward(rows_of(grads[0]), v[0], v[1]);
+    return {dgate.view(shape), dup.view(shape), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> swiglu8(const Tensor& gate, const Tensor& up, int64_t copies) {
+  auto v = Swiglu8::apply(gate, up, copies);
+  return {v[0], v[1], v[2]};
+}
+
+struct Preference : Function<Preference> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& ref,
+                               int64_t ignore, int64_t form, double beta, double smooth) {
+    auto [loss, logps, rewards, slopes, stats] = preference_forward(logits, labels, ref, ignore, form, beta, smooth);
+    ctx->save_for_backward({logits, labels, stats, slopes});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->mark_non_differentiable({logps, rewards});
+    return {loss, logps, rewards};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("preference_loss");
+    const auto v = ctx->get_saved_variables();
+    Tensor d;
+    if (grads[0].defined())
+      d = token_logprobs_grad(v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], v[3], grads[0]);
+    return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& labels, const Tensor& ref,
+                                                   int64_t ignore, int64_t form, double beta, double smooth) {
+  auto v = Preference::apply(logits, labels, ref, ignore, form, beta, smooth);
+  return {v[0], v[1], v[2]};
+}
+
+struct LabelLogprobs : Function<LabelLogprobs> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, int64_t ignore) {
+    auto [logps, stats] = token_logprobs(logits, labels, ignore);
+    ctx->save_for_backward({logits, labels, stats});
+    ctx->saved_data["ignore"] = ignore;
+    return logps;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("token_logprobs");
+    const auto v = ctx->get_saved_variables();
+    return {token_logprobs_grad(v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], grads[0].contiguous(), std::nullopt),
+            Tensor(), Tensor()};
+  }
+};
+
+Tensor label_logprobs(const Tensor& logits, const Tensor& labels, int64_t ignore) {
+  return LabelLogprobs::apply(logits, labels, ignore);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
@@ -283,6 +402,14 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
   m.def(
       "token_logprobs_grad(Tensor logits, Tensor labels, int ignore, Tensor stats, Tensor slopes, Tensor? upstream) "
       "-> Tensor");
+  m.def(
+      "adapters_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor scaling, Tensor? plan, int tile, "
+      "Tensor? codes, Tensor? scales) -> Tensor", &adapters_add);
+  m.def("swiglu8(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor, Tensor)", &swiglu8);
+  m.def(
+      "preference_loss(Tensor logits, Tensor labels, Tensor ref, int ignore, int form, float beta, float smooth) "
+      "-> (Tensor, Tensor, Tensor)", &preference_loss);
+  m.def("label_logprobs(Tensor logits, Tensor labels, int ignore) -> Tensor", &label_logprobs);
 }
 
 #define RQ_IMPLS(m)                                          \

@@ -2,27 +2,9 @@
 from typing import Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from rocm_qlora import _native as nat
-from rocm_qlora.activation8.packed import PackedActivation, rows_of
-
-
-class _Swiglu8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate, up, copies):
-        h, codes, scales = nat.require_ops(gate, up).swiglu8_forward(rows_of(gate), rows_of(up), copies)
-        ctx.save_for_backward(codes[:2], scales[:2])
-        ctx.shape = gate.shape
-        ctx.mark_non_differentiable(codes, scales)
-        return h.view(gate.shape), codes, scales
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, _codes, _scales):
-        codes, scales = ctx.saved_tensors
-        dgate, dup = nat.require_ops(dh, codes).swiglu8_backward(rows_of(dh), codes, scales)
-        return dgate.view(ctx.shape), dup.view(ctx.shape), None
+from rocm_qlora.activation8.packed import PackedActivation
 
 
 def swiglu8(gate: torch.Tensor, up: torch.Tensor,
@@ -40,5 +22,5 @@ def swiglu8(gate: torch.Tensor, up: torch.Tensor,
     if gate.dim() < 1:
         raise ValueError("swiglu8 needs at least one dimension")
     nat.dtype_code(gate.dtype)
-    h, codes, scales = _Swiglu8.apply(gate, up, 3 if pack_output else 2)
+    h, codes, scales = nat.require_ops(gate, up).swiglu8(gate, up, 3 if pack_output else 2)
     return (h, PackedActivation(codes[2], scales[2], tuple(h.shape), h.dtype)) if pack_output else h

@@ -64,33 +64,6 @@ def _plan_args(plan: Optional[AdapterPlan], rows: int, count: int):
     return plan.data, plan.tile
 
 
-class _AdaptersAdd(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, base, x, A, B, scaling, plan, codes, scales):
-        data, tile = plan
-        y, mid = nat.require_ops(base, x, A, B, scaling).adapters_apply(x, A, B, scaling, base, data, tile)
-        ctx.save_for_backward(*((x, None) if codes is None else (codes, scales)), A, B, scaling, mid, data)
-        ctx.tile = tile
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        z, scales, A, B, scaling, mid, data = ctx.saved_tensors
-        need_base, need_x, need_A, need_B = ctx.needs_input_grad[:4]
-        ops, rows = nat.require_ops(dy, A), rows_of(dy)
-        dx = dA = dB = None
-        if need_x:
-            dx, gmid = ops.adapters_apply(rows, B, A, scaling, None, data, ctx.tile)
-        elif need_A:
-            gmid = ops.adapters_mid(rows, B, A, scaling, data, ctx.tile)
-        if need_A:
-            dA = ops.adapters_grad(z, scales, gmid, A.shape[1], A.shape[0], A.dtype, data, ctx.tile)
-        if need_B:
-            dB = ops.adapters_grad(rows, None, mid, B.shape[1], B.shape[0], B.dtype, data, ctx.tile)
-        return dy if need_base else None, dx, dA, dB, None, None, None, None
-
-
 def _packed_args(packed_x: Optional[PackedActivation], x: torch.Tensor):
     if packed_x is None:
         return None, None
@@ -143,11 +116,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.
         nat.require_ops(base, x, A, B, scaling, out).adapters_apply_(out.view(base2.shape), x2, A, B, scaling, base2,
                                                                      *args)
         return out
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, A, B))):
-        # serving: the same call without the autograd bookkeeping
-        return nat.require_ops(base, x, A, B, scaling).adapters_apply(x2, A, B, scaling, base2, *args)[0].view(
-            base.shape)
-    return _AdaptersAdd.apply(base2, x2, A, B, scaling, args, codes, scales).view(base.shape)
+    y = nat.require_ops(base, x, A, B, scaling).adapters_add(base2, x2, A, B, scaling, *args, codes, scales)
+    return y if y.shape == base.shape else y.view(base.shape)
 
 
 class _BankLinear(torch.autograd.Function):

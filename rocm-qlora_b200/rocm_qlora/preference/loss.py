@@ -9,7 +9,6 @@ padding) do not count; their rows are not read.
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from rocm_qlora import _native as nat
 
@@ -30,29 +29,13 @@ def _check(logits: torch.Tensor, labels: torch.Tensor):
     return logits, labels.contiguous()
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ignore):
-        logps, stats = nat.require_ops(logits, labels).token_logprobs(logits, labels, ignore)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.ignore = ignore
-        return logps
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, labels, stats = ctx.saved_tensors
-        d = nat.require_ops(logits, g).token_logprobs_grad(logits, labels, ctx.ignore, stats, g.contiguous(), None)
-        return d, None, None
-
-
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """[batch, length] float32: at each label's place its log-probability
     under the position before it, 0 where the label does not count (and at
     the first place).  A label outside the vocabulary gives NaN.
     Differentiable in ``logits``."""
     logits, labels = _check(logits, labels)
-    return _TokenLogprobs.apply(logits, labels, int(ignore_index))
+    return nat.require_ops(logits, labels).label_logprobs(logits, labels, int(ignore_index))
 
 
 class PreferenceOutput(NamedTuple):
@@ -63,24 +46,6 @@ class PreferenceOutput(NamedTuple):
     logps: torch.Tensor
     chosen_rewards: torch.Tensor
     rejected_rewards: torch.Tensor
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ref, ignore, form, beta, smooth):
-        loss, logps, rewards, slopes, stats = nat.require_ops(logits, labels, ref).preference_forward(
-            logits, labels, ref, ignore, form, beta, smooth)
-        ctx.save_for_backward(logits, labels, stats, slopes)
-        ctx.ignore = ignore
-        ctx.mark_non_differentiable(logps, rewards)
-        return loss, logps, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _logps, _rewards):
-        logits, labels, stats, slopes = ctx.saved_tensors
-        d = nat.require_ops(logits, g).token_logprobs_grad(logits, labels, ctx.ignore, stats, slopes, g)
-        return d, None, None, None, None, None, None
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor, beta: float = 0.1,
@@ -111,7 +76,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"a batch holds pairs (chosen, then rejected): got {logits.shape[0]} sequences")
     if ref_logps.shape != labels.shape:
         raise ValueError(f"ref_logps must be [batch, length] like labels, got {tuple(ref_logps.shape)}")
-    loss, logps, rewards = _PreferenceLoss.apply(logits, labels, ref_logps.detach().float().contiguous(),
-                                                 int(ignore_index), _FORMS[form], float(beta), float(label_smoothing))
+    ref = ref_logps.detach().float().contiguous()
+    loss, logps, rewards = nat.require_ops(logits, labels, ref).preference_loss(
+        logits, labels, ref, int(ignore_index), _FORMS[form], float(beta), float(label_smoothing))
     half = logits.shape[0] // 2
     return PreferenceOutput(loss, logps, rewards[:half], rewards[half:])
