@@ -22,7 +22,10 @@ namespace rq {
 
 constexpr int kTokThreads = 512;  // of a row, in the gradient and where rows are few
 constexpr int kTokBatch = 4;      // 16-byte loads of a thread at a time
-constexpr float kLog2e = 1.4426950408889634f;
+// log2(e) as the sum of two floats: the first alone is 1.3e-8 of itself off,
+// which would shift every log-probability by that much of the row's entropy
+constexpr double kLog2eD = 1.4426950408889634;
+constexpr float kLog2e = (float)kLog2eD, kLog2eRest = (float)(kLog2eD - (double)(float)kLog2eD);
 
 // The label that scores row `at` of B * L; false where the row does not count.
 __device__ __forceinline__ bool row_label(const TokenRows& t, int64_t at, int64_t* y) {
@@ -84,10 +87,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// e^x / 2^k
+__device__ __forceinline__ float exp_over(float x, float k) {
+  return exp2_fast(fmaf(x, kLog2eRest, fmaf(x, kLog2e, -k)));
+}
+
 // A running sum of e^x as s * 2^k, k whole.  With a whole k the shift costs no
-// rounding: e^x = 2^(x log2(e) - k) is one fused multiply-add and one
-// exponential a value, and moving k scales s by a power of two.  k follows
-// the maximum only when a value would pass 2^64.
+// rounding: e^x / 2^k is two fused multiply-adds and one exponential a value,
+// and moving k scales s by a power of two.  k follows the maximum only when a
+// value would pass 2^64.
 struct ExpSum {
   float k = 0.0f, s = 0.0f;
   __device__ __forceinline__ void raise(float top) {  // top: the largest of the values to come
@@ -108,7 +116,7 @@ struct ExpSum {
     raise(top);
     float e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = exp2_fast(fmaf(x[i], kLog2e, -k));
+    for (int i = 0; i < N; ++i) e[i] = exp_over(x[i], k);
 #pragma unroll
     for (int w = N / 2; w > 0; w /= 2)
 #pragma unroll
@@ -184,8 +192,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, floa
     if (!(s > 0.0 && s < (double)INFINITY)) s = (double)__uint_as_float(0x7fc00000u);
     // a label outside the vocabulary has no probability: NaN, not a read past the row
     const float xy = y >= 0 && y < t.V ? DType<DT>::to_f32(x[y]) : __uint_as_float(0x7fc00000u);
-    // in base 2 with the same fp32 log2(e) throughout, whose error then drops out
-    const double lp = ((double)xy * (double)kLog2e - (double)k - log2(s)) / (double)kLog2e;
+    const double lp = (double)xy - ((double)k + log2(s)) / kLog2eD;
     const float hi = (float)lp;
     stats[at] = make_float4(k, (float)s, hi, fabsf(hi) < INFINITY ? (float)(lp - (double)hi) : 0.0f);
     if (logps) logps[at + 1] = hi;
@@ -318,8 +325,8 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
   float c = per_token ? slopes[at + 1] : slopes[at / t.L];
   if (upstream) c *= *upstream;
   if (y < 0 || y >= t.V) c = __uint_as_float(0x7fc00000u);
-  const float by = -c / q.y, k = -q.x;
-  auto value = [&](float f) { return by * exp2_fast(fmaf(f, kLog2e, k)); };
+  const float by = -c / q.y, k = q.x;
+  auto value = [&](float f) { return by * exp_over(f, k); };
   if ((((uintptr_t)x ^ (uintptr_t)d) & 15) == 0) {
     const RowCut<DT> cut(x, (int)t.V);
     const uint4* src = reinterpret_cast<const uint4*>(x + cut.head);
