@@ -109,6 +109,11 @@ static bool half_ok(int dt) { return dt == RQ_BF16 || dt == RQ_F16; }
 // Sizes a kernel indexes with 32 bits.
 static bool fits(int64_t v) { return v >= 0 && v < (int64_t)1 << 31; }
 
+// Rows whose 8-bit blocks are numbered with 32 bits.
+static bool fits_act8(int64_t M, int64_t K) {
+  return fits(M) && fits(K) && fits(M * ((K + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK));
+}
+
 static int check_plan(int64_t rows, int count, int tile, const int32_t* plan, int64_t words) {
   if (!fits(rows) || count < 1 || count > RQ_ADAPTERS_MAX) return RQ_ERR_INVALID;
   if (!plan) return RQ_OK;
@@ -384,7 +389,7 @@ int rq_act8_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, i
                  void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits(M) || !fits(K) || (M > 1 && ld_x < K)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K) || (M > 1 && ld_x < K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!x || !codes || !scales) return RQ_ERR_INVALID;
   if ((uintptr_t)x % dtype_size(dtype) || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return RQ_ERR_ALIGN;
@@ -395,7 +400,7 @@ int rq_act8_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t 
                    void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits(M) || !fits(K)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!codes || !scales || !out) return RQ_ERR_INVALID;
   if ((uintptr_t)out % dtype_size(dtype) || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return RQ_ERR_ALIGN;
@@ -406,7 +411,7 @@ int rq_swiglu8_forward(const void* gate, int64_t ld_gate, const void* up, int64_
                        int64_t K, void* h, int8_t* codes, float* scales, int copies, void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits(M) || !fits(K) || (copies != 2 && copies != 3)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K) || (copies != 2 && copies != 3)) return RQ_ERR_INVALID;
   if (M > 1 && (ld_gate < K || ld_up < K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!gate || !up || !h || !codes || !scales) return RQ_ERR_INVALID;
@@ -420,7 +425,7 @@ int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t M, int
                         const float* scales, void* dgate, void* dup, void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits(M) || !fits(K) || (M > 1 && ld_dh < K)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K) || (M > 1 && ld_dh < K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!dh || !codes || !scales || !dgate || !dup) return RQ_ERR_INVALID;
   const int e = dtype_size(dtype);
