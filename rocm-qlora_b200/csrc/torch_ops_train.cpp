@@ -41,14 +41,14 @@ Tensor adapter_plan(const Tensor& ids, int64_t count, int64_t tile) {
 
 // out (nullopt: mid only) = base + mid V^T, mid = scaling (in U)
 void apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling, const optional<Tensor>& base,
-           const optional<Tensor>& plan, int64_t tile, const Tensor& mid, const optional<Tensor>& out) {
+           const optional<Tensor>& plan, int64_t tile, const optional<Tensor>& mid, const optional<Tensor>& out) {
   const c10::cuda::CUDAGuard guard(in.device());
   const bool has_base = base.has_value() && base->defined(), has_plan = plan.has_value() && plan->defined();
   check(rq_adapters_apply(in.data_ptr(), in.stride(0), U.data_ptr(), V.data_ptr(), scaling.data_ptr<float>(), ptr(base),
                           has_base ? base->stride(0) : 0, in.size(0), in.size(1), out ? out->size(1) : 0,
                           (int)U.size(2), (int)U.size(0), dtype_code(in.scalar_type()),
                           static_cast<const int32_t*>(ptr(plan)), has_plan ? plan->numel() : 0, (int)tile,
-                          mid.data_ptr<float>(), out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
+                          mid ? mid->data_ptr<float>() : nullptr, out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
                           stream_of(in)),
         "rq_adapters_apply");
 }
@@ -304,10 +304,62 @@ struct AdaptersAdd : Function<AdaptersAdd> {
   }
 };
 
+std::string sizes_of(const Tensor& t) { return c10::str(t.sizes()); }
+
+// What a caller can get wrong, as Python's ValueError and TypeError; tensors
+// off the GPU as NotImplementedError.
+void check_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& scaling,
+               const optional<Tensor>& plan, int64_t plan_rows, int64_t plan_count, const optional<Tensor>& codes,
+               const optional<Tensor>& scales) {
+  const auto dt = x.scalar_type();
+  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, "adapters take bfloat16 or float16 activations, got ", dt);
+  TORCH_CHECK_VALUE(A.dim() == 3 && B.dim() == 3 && A.size(0) == B.size(0) && A.size(2) == B.size(2),
+                    "A must be [count, in, rank] and B [count, out, rank]; got ", sizes_of(A), ", ", sizes_of(B));
+  TORCH_CHECK_TYPE(A.scalar_type() == dt && B.scalar_type() == dt, "adapters are ", A.scalar_type(), " and ",
+                   B.scalar_type(), ", activations ", dt);
+  const int64_t count = A.size(0), r = A.size(2);
+  TORCH_CHECK_VALUE(r % 8 == 0 && r >= 8 && r <= 128, "rank must be a multiple of 8 up to 128, got ", r,
+                    " (AdapterBank pads)");
+  TORCH_CHECK_VALUE(count >= 1 && count <= RQ_ADAPTERS_MAX, "a bank holds 1 to ", RQ_ADAPTERS_MAX, " adapters, got ", count);
+  TORCH_CHECK_VALUE(scaling.dim() == 1 && scaling.size(0) == count && scaling.scalar_type() == at::kFloat,
+                    "scaling must be float32 [", count, "], got ", scaling.scalar_type(), " ", sizes_of(scaling));
+  TORCH_CHECK_VALUE(x.dim() >= 1 && base.dim() == x.dim() && x.size(-1) == A.size(1) && base.size(-1) == B.size(1),
+                    "base ", sizes_of(base), " and x ", sizes_of(x), " do not fit A ", sizes_of(A), " and B ", sizes_of(B));
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) {
+    TORCH_CHECK_VALUE(x.size(i) == base.size(i), "base is ", sizes_of(base), ", x ", sizes_of(x));
+    rows *= x.size(i);
+  }
+  TORCH_CHECK_TYPE(base.scalar_type() == dt, "base is ", base.scalar_type(), ", x ", dt);
+  TORCH_CHECK_VALUE(plan || count == 1, "a bank of several adapters needs a plan");
+  TORCH_CHECK_VALUE(!plan || (plan_rows == rows && plan_count == count), "the plan is for ", plan_rows, " rows and ",
+                    plan_count, " adapters, not ", rows, " and ", count);
+  if (codes) {
+    const int64_t nb = (A.size(1) + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+    TORCH_CHECK_VALUE(scales && codes->dim() == 2 && codes->size(0) == rows && codes->size(1) == nb * RQ_ACT8_BLOCK,
+                      "packed_x does not belong to x ", sizes_of(x));
+  }
+  for (const Tensor* t : {&base, &x, &A, &B, &scaling}) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->is_cpu(), "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device");
+    TORCH_CHECK(t->device() == x.device(), "tensors are on different devices: ", x.device(), " and ", t->device());
+  }
+}
+
 Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& scaling,
-                    const optional<Tensor>& plan, int64_t tile, const optional<Tensor>& codes,
-                    const optional<Tensor>& scales) {
-  return AdaptersAdd::apply(base, x, A, B, scaling, plan, tile, codes, scales);
+                    const optional<Tensor>& plan, int64_t plan_rows, int64_t plan_count, int64_t tile,
+                    const optional<Tensor>& codes, const optional<Tensor>& scales) {
+  check_add(base, x, A, B, scaling, plan, plan_rows, plan_count, codes, scales);
+  const Tensor b2 = rows_of(base), x2 = rows_of(x), a3 = A.contiguous(), b3 = B.contiguous(), s1 = scaling.contiguous();
+  const bool grad = at::GradMode::is_enabled() &&
+                    (base.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
+  Tensor y;
+  if (grad) {
+    y = AdaptersAdd::apply(b2, x2, a3, b3, s1, plan, tile, codes, scales);
+  } else {  // serving: nothing is kept
+    y = at::empty({x2.size(0), b3.size(1)}, x2.options());
+    if (!x2.is_meta()) apply(x2, a3, b3, s1, b2, plan, tile, std::nullopt, y);
+  }
+  return base.dim() == 2 ? y : y.view(base.sizes());
 }
 
 struct Swiglu8 : Function<Swiglu8> {
@@ -403,8 +455,8 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
       "token_logprobs_grad(Tensor logits, Tensor labels, int ignore, Tensor stats, Tensor slopes, Tensor? upstream) "
       "-> Tensor");
   m.def(
-      "adapters_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor scaling, Tensor? plan, int tile, "
-      "Tensor? codes, Tensor? scales) -> Tensor", &adapters_add);
+      "adapters_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor scaling, Tensor? plan, int plan_rows, "
+      "int plan_count, int tile, Tensor? codes, Tensor? scales) -> Tensor", &adapters_add);
   m.def("swiglu8(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor, Tensor)", &swiglu8);
   m.def(
       "preference_loss(Tensor logits, Tensor labels, Tensor ref, int ignore, int form, float beta, float smooth) "

@@ -169,7 +169,12 @@ def require_ops(*ts: torch.Tensor):
                 "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device")
         if t.device != first.device:
             raise RuntimeError(f"tensors are on different devices: {first.device} and {t.device}")
-    if not ops():
+    return loaded_ops()
+
+
+def loaded_ops():
+    """torch.ops.rocm_qlora, for operators that check their tensors themselves."""
+    if not (_ops_state or ops()):
         raise NativeUnavailable(f"the torch extension {OPS_PATH} is missing or does not load "
                                 "(run `make -C rocm-qlora_b200` or __graft_entry__.build())")
     return torch.ops.rocm_qlora

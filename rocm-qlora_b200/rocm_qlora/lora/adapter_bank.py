@@ -98,26 +98,32 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.
     in 32 bits and the sum is rounded once.  With ``packed_x`` (the packed
     form of x) the backward of A reads it and x is not kept.  ``out`` (no
     gradients then) takes the result and may be ``base`` itself."""
+    args = (plan.data, plan.rows, plan.count, plan.tile) if plan is not None else (None, 0, 0, 0)
+    if packed_x is not None:
+        _packed_args(packed_x, x)
+    if out is not None:
+        return _add_out(base, x, A, B, scaling, plan, out)
+    try:
+        return nat.loaded_ops().adapters_add(base, x, A, B, scaling, *args,
+                                             *((None, None) if packed_x is None else (packed_x.codes, packed_x.scales)))
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None
+
+
+def _add_out(base, x, A, B, scaling, plan, out) -> torch.Tensor:
     _check_bank(x, A, B, scaling)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, A, B, out)):
+        raise RuntimeError("adapters_add(out=...) does not support automatic differentiation")
+    if out.shape != base.shape or out.dtype != x.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of base's shape and dtype")
     if x.shape[:-1] != base.shape[:-1] or x.shape[-1] != A.shape[1] or base.shape[-1] != B.shape[1]:
         raise ValueError(f"base {tuple(base.shape)} and x {tuple(x.shape)} do not fit A {tuple(A.shape)} and "
                          f"B {tuple(B.shape)}")
-    if base.dtype != x.dtype:
-        raise TypeError(f"base is {base.dtype}, x {x.dtype}")
     x2, base2 = rows_of(x), rows_of(base)
-    args = _plan_args(plan, x2.shape[0], A.shape[0])
-    codes, scales = _packed_args(packed_x, x)
-    A, B, scaling = A.contiguous(), B.contiguous(), scaling.contiguous()
-    if out is not None:
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, A, B, out)):
-            raise RuntimeError("adapters_add(out=...) does not support automatic differentiation")
-        if out.shape != base.shape or out.dtype != x.dtype or not out.is_contiguous():
-            raise ValueError("out must be contiguous, of base's shape and dtype")
-        nat.require_ops(base, x, A, B, scaling, out).adapters_apply_(out.view(base2.shape), x2, A, B, scaling, base2,
-                                                                     *args)
-        return out
-    y = nat.require_ops(base, x, A, B, scaling).adapters_add(base2, x2, A, B, scaling, *args, codes, scales)
-    return y if y.shape == base.shape else y.view(base.shape)
+    nat.require_ops(base, x, A, B, scaling, out).adapters_apply_(
+        out.view(base2.shape), x2, A.contiguous(), B.contiguous(), scaling.contiguous(), base2,
+        *_plan_args(plan, x2.shape[0], A.shape[0]))
+    return out
 
 
 class _BankLinear(torch.autograd.Function):
