@@ -304,6 +304,19 @@ struct AdaptersAdd : Function<AdaptersAdd> {
   }
 };
 
+void check_float(at::ScalarType t) {
+  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "unsupported dtype ", t,
+                   "; rocm_qlora kernels take float32, bfloat16 or float16");
+}
+
+void check_gpu(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->is_cpu(), "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device");
+    TORCH_CHECK(t->device() == (*tensors.begin())->device(), "tensors are on different devices: ",
+                (*tensors.begin())->device(), " and ", t->device());
+  }
+}
+
 std::string sizes_of(const Tensor& t) { return c10::str(t.sizes()); }
 
 // What a caller can get wrong, as Python's ValueError and TypeError; tensors
@@ -339,10 +352,7 @@ void check_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tenso
     TORCH_CHECK_VALUE(scales && codes->dim() == 2 && codes->size(0) == rows && codes->size(1) == nb * RQ_ACT8_BLOCK,
                       "packed_x does not belong to x ", sizes_of(x));
   }
-  for (const Tensor* t : {&base, &x, &A, &B, &scaling}) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->is_cpu(), "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device");
-    TORCH_CHECK(t->device() == x.device(), "tensors are on different devices: ", x.device(), " and ", t->device());
-  }
+  check_gpu({&x, &base, &A, &B, &scaling});
 }
 
 Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& scaling,
@@ -381,6 +391,11 @@ struct Swiglu8 : Function<Swiglu8> {
 };
 
 std::tuple<Tensor, Tensor, Tensor> swiglu8(const Tensor& gate, const Tensor& up, int64_t copies) {
+  TORCH_CHECK_VALUE(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type(), "gate ", gate.sizes(), " ",
+                    gate.scalar_type(), " and up ", up.sizes(), " ", up.scalar_type(), " differ");
+  TORCH_CHECK_VALUE(gate.dim() >= 1, "swiglu8 needs at least one dimension");
+  check_float(gate.scalar_type());
+  check_gpu({&gate, &up});
   auto v = Swiglu8::apply(gate, up, copies);
   return {v[0], v[1], v[2]};
 }
@@ -404,10 +419,29 @@ struct Preference : Function<Preference> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& labels, const Tensor& ref,
-                                                   int64_t ignore, int64_t form, double beta, double smooth) {
-  auto v = Preference::apply(logits, labels, ref, ignore, form, beta, smooth);
-  return {v[0], v[1], v[2]};
+// logits with a contiguous vocabulary and contiguous labels
+std::pair<Tensor, Tensor> checked_logits(const Tensor& logits, const Tensor& labels) {
+  TORCH_CHECK_VALUE(logits.dim() == 3 && labels.dim() == 2 && labels.size(0) == logits.size(0) &&
+                        labels.size(1) == logits.size(1),
+                    "logits must be [batch, length, vocabulary] and labels [batch, length]; got ", logits.sizes(),
+                    " and ", labels.sizes());
+  TORCH_CHECK_TYPE(labels.scalar_type() == at::kLong, "labels must be int64, got ", labels.scalar_type());
+  TORCH_CHECK_VALUE(logits.size(2) >= 1, "the vocabulary is empty");
+  check_float(logits.scalar_type());
+  return {logits.stride(2) == 1 || logits.size(2) == 1 ? logits : logits.contiguous(), labels.contiguous()};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& labels,
+                                                           const Tensor& ref, int64_t ignore, int64_t form,
+                                                           double beta, double smooth) {
+  const auto [x, y] = checked_logits(logits, labels);
+  const int64_t B = x.size(0);
+  TORCH_CHECK_VALUE(B >= 2 && B % 2 == 0 && x.size(1) >= 1, "a batch holds pairs (chosen, then rejected): got ", B,
+                    " sequences");
+  TORCH_CHECK_VALUE(ref.sizes() == y.sizes(), "ref_logps must be [batch, length] like labels, got ", ref.sizes());
+  check_gpu({&logits, &labels, &ref});
+  auto v = Preference::apply(x, y, ref.detach().to(at::kFloat).contiguous(), ignore, form, beta, smooth);
+  return {v[0], v[1], v[2].narrow(0, 0, B / 2), v[2].narrow(0, B / 2, B / 2)};
 }
 
 struct LabelLogprobs : Function<LabelLogprobs> {
@@ -426,7 +460,9 @@ struct LabelLogprobs : Function<LabelLogprobs> {
 };
 
 Tensor label_logprobs(const Tensor& logits, const Tensor& labels, int64_t ignore) {
-  return LabelLogprobs::apply(logits, labels, ignore);
+  const auto [x, y] = checked_logits(logits, labels);
+  check_gpu({&logits, &labels});
+  return LabelLogprobs::apply(x, y, ignore);
 }
 
 }  // namespace
@@ -460,7 +496,7 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
   m.def("swiglu8(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor, Tensor)", &swiglu8);
   m.def(
       "preference_loss(Tensor logits, Tensor labels, Tensor ref, int ignore, int form, float beta, float smooth) "
-      "-> (Tensor, Tensor, Tensor)", &preference_loss);
+      "-> (Tensor, Tensor, Tensor, Tensor)", &preference_loss);
   m.def("label_logprobs(Tensor logits, Tensor labels, int ignore) -> Tensor", &label_logprobs);
 }
 

@@ -17,10 +17,8 @@ def swiglu8(gate: torch.Tensor, up: torch.Tensor,
     forms are kept (2.06 bytes a column instead of 4).  ``pack_output=True``
     also returns the packed form of the product, written in the same pass,
     for the projection that reads it (``packed_x=``)."""
-    if gate.shape != up.shape or gate.dtype != up.dtype:
-        raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ")
-    if gate.dim() < 1:
-        raise ValueError("swiglu8 needs at least one dimension")
-    nat.dtype_code(gate.dtype)
-    h, codes, scales = nat.require_ops(gate, up).swiglu8(gate, up, 3 if pack_output else 2)
+    try:
+        h, codes, scales = nat.loaded_ops().swiglu8(gate, up, 3 if pack_output else 2)
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None
     return (h, PackedActivation(codes[2], scales[2], tuple(h.shape), h.dtype)) if pack_output else h

@@ -15,27 +15,15 @@ from rocm_qlora import _native as nat
 _FORMS = {"sigmoid": 0, "ipo": 1}
 
 
-def _check(logits: torch.Tensor, labels: torch.Tensor):
-    if logits.dim() != 3 or labels.shape != logits.shape[:2]:
-        raise ValueError(f"logits must be [batch, length, vocabulary] and labels [batch, length]; got "
-                         f"{tuple(logits.shape)} and {tuple(labels.shape)}")
-    if labels.dtype != torch.int64:
-        raise TypeError(f"labels must be int64, got {labels.dtype}")
-    if logits.shape[2] < 1:
-        raise ValueError("the vocabulary is empty")
-    nat.dtype_code(logits.dtype)
-    if logits.stride(2) != 1 and logits.shape[2] > 1:
-        logits = logits.contiguous()
-    return logits, labels.contiguous()
-
-
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """[batch, length] float32: at each label's place its log-probability
     under the position before it, 0 where the label does not count (and at
     the first place).  A label outside the vocabulary gives NaN.
     Differentiable in ``logits``."""
-    logits, labels = _check(logits, labels)
-    return nat.require_ops(logits, labels).label_logprobs(logits, labels, int(ignore_index))
+    try:
+        return nat.loaded_ops().label_logprobs(logits, labels, int(ignore_index))
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None
 
 
 class PreferenceOutput(NamedTuple):
@@ -71,13 +59,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"label_smoothing must be between 0 and 0.5, got {label_smoothing}")
     if form == "ipo" and label_smoothing:
         raise ValueError("label_smoothing belongs to the sigmoid form")
-    logits, labels = _check(logits, labels)
-    if logits.shape[0] < 2 or logits.shape[0] % 2 or logits.shape[1] < 1:
-        raise ValueError(f"a batch holds pairs (chosen, then rejected): got {logits.shape[0]} sequences")
-    if ref_logps.shape != labels.shape:
-        raise ValueError(f"ref_logps must be [batch, length] like labels, got {tuple(ref_logps.shape)}")
-    ref = ref_logps.detach().float().contiguous()
-    loss, logps, rewards = nat.require_ops(logits, labels, ref).preference_loss(
-        logits, labels, ref, int(ignore_index), _FORMS[form], float(beta), float(label_smoothing))
-    half = logits.shape[0] // 2
-    return PreferenceOutput(loss, logps, rewards[:half], rewards[half:])
+    try:
+        return PreferenceOutput(*nat.loaded_ops().preference_loss(
+            logits, labels, ref_logps, int(ignore_index), _FORMS[form], float(beta), float(label_smoothing)))
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None
