@@ -16,6 +16,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <deque>
+#include <mutex>
 
 #include "gemv_common.cuh"
 
@@ -266,42 +269,93 @@ __device__ __forceinline__ V cluster_sum(cg::cluster_group& cluster, float* p, i
   return s;
 }
 
-// CTAs a cluster (1 to `most`) so that `units` clusters fill whole rounds of
-// the GPU's `per_sm` CTAs an SM best; of equal fills the smaller number of rounds.
-static int fill_size(int64_t units, int per_sm, int most) {
-  const int64_t slots = (int64_t)per_sm * num_sms();
-  int best = 1;
-  double best_fill = 0.0;
-  for (int c = 1; c <= most; ++c) {
-    const int64_t ctas = units * c, rounds = (ctas + slots - 1) / slots;
-    const double fill = (double)ctas / (double)(rounds * slots);
-    if (fill > best_fill + 0.02) best = c, best_fill = fill;
-  }
-  return best;
-}
-
 template <class P>
-static int launch_cluster(void (*kern)(P), const P& args, dim3 grid, int threads, size_t smem, int csize,
-                          cudaStream_t st) {
-  const int rc = ensure_smem_limit((const void*)kern, smem);
-  if (rc != RQ_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = csize;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return RQ_ERR_CUDA;
+struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at launch
+  void (*kern)(P);
+  int threads;
+  size_t smem;
+
+  cudaLaunchConfig_t config(dim3 grid, int csize, cudaLaunchAttribute* at, cudaStream_t st) const {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    at->id = cudaLaunchAttributeClusterDimension;
+    at->val.clusterDim.x = csize;
+    at->val.clusterDim.y = at->val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cfg;
   }
-  return check_launch();
+
+  // Clusters of each size 1..8 that the GPU holds at once (their CTAs have to
+  // share a GPC, so not simply its CTA slots over the size).
+  const int* resident() const {
+    struct Entry {
+      const void* k;
+      int dev;
+      size_t smem;
+      int n[9];
+    };
+    static std::mutex mu;
+    static std::deque<Entry> known;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Entry& e : known)
+      if (e.k == (const void*)kern && e.dev == dev && e.smem == smem) return e.n;
+    Entry e{(const void*)kern, dev, smem, {}};
+    for (int c = 1; c <= 8; ++c) {
+      cudaLaunchAttribute at;
+      const cudaLaunchConfig_t cfg = config(dim3(c), c, &at, nullptr);
+      if (cudaOccupancyMaxActiveClusters(&e.n[c], kern, &cfg) != cudaSuccess || e.n[c] < 1) {
+        cudaGetLastError();
+        e.n[c] = std::max(1, num_sms() / c);
+      }
+    }
+    known.push_back(e);
+    return known.back().n;
+  }
+
+  int prepare() const { return ensure_smem_limit((const void*)kern, smem); }
+
+  int launch(const P& args, dim3 grid, int csize, cudaStream_t st) const {
+    cudaLaunchAttribute at;
+    const cudaLaunchConfig_t cfg = config(grid, csize, &at, st);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return RQ_ERR_CUDA;
+    }
+    return check_launch();
+  }
+};
+
+// The rows of a tile without an adapter: out = base (or zero), mid = 0; NaN
+// for both where the id named no adapter.
+template <bool VEC>
+__device__ __noinline__ void rows_without(const ApplyArgs& p, const int* order, int first, int rows, bool bad,
+                                          int crank, int csize) {
+  const AdapterRows& a = p.a;
+  const float fill = bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+  const uint32_t bits = bad ? 0x7fff7fffu : 0u;  // NaN in both 16-bit types
+  const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  uint16_t* out = static_cast<uint16_t*>(p.out);
+  for (int i = crank; i < rows; i += csize) {
+    const int64_t m = order ? min(max(order[first + i], 0), (int)a.M - 1) : first + i;
+    if (p.mid)
+      for (int j = threadIdx.x; j < a.r; j += kApThreads) p.mid[m * a.r + j] = fill;
+    if (p.out == p.base && !bad) continue;
+    if constexpr (VEC) {
+      for (int64_t d = threadIdx.x * 8; d < a.D2; d += kApThreads * 8)
+        *reinterpret_cast<uint4*>(out + m * p.ldo + d) =
+            base && !bad ? *reinterpret_cast<const uint4*>(base + m * p.ldb + d) : make_uint4(bits, bits, bits, bits);
+    } else {
+      for (int64_t d = threadIdx.x; d < a.D2; d += kApThreads)
+        out[m * p.ldo + d] = base && !bad ? base[m * p.ldb + d] : (uint16_t)bits;
+    }
+  }
 }
 
 // One cluster computes one tile: `tile` rows (16 to 128) of one adapter.
@@ -334,6 +388,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   constexpr int NT = R / 8;               // n-tiles of the first product
   constexpr int KS = R / 16;              // k-steps of the second
   constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R), S = ap_steps(R, NW);
+  constexpr int CW = R <= 32 ? 2 : 1, AHEAD = R <= 32 ? 2 : 4;  // second product: 32-column chunks, m-tiles under way
   extern __shared__ __align__(16) unsigned char smem[];
   const AdapterRows& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
@@ -345,8 +400,9 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   int group, first, rows;
   const int* order = nullptr;
   if (a.plan) {
-    if (tile_id >= a.plan[0]) return;
+    const int tiles = a.plan[0];  // the table has room for every tile of the grid: both loads at once
     const int4 e = reinterpret_cast<const int4*>(a.plan + plan_tiles_at(a.count))[tile_id];
+    if (tile_id >= tiles) return;
     // held inside the batch, so that a plan that is not one cannot reach outside it
     group = min(max(e.x, 0), a.count + 1), first = min(max(e.y, 0), (int)a.M - 1);
     rows = min(max(e.z, 1), min(a.tile, (int)a.M - first));
@@ -356,8 +412,10 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     rows = min(a.tile, (int)a.M - first);
   }
   const int WM = a.tile / 16, WK = kApWarps / WM;  // warps along rows, along columns
-  const bool none = group >= a.count;
-  const float fill = group > a.count ? __int_as_float(0x7fc00000) : 0.0f;
+  if (group >= a.count) {  // no adapter: base as it is; an id that names none: NaN
+    rows_without<VEC>(p, order, first, rows, group > a.count, crank, csize);
+    return;
+  }
 
   const int KC = NW * WK * kApWin, step_bytes = KC * PU + ap_x_bytes(NW);  // columns of a step
   ApplyRows& at = *reinterpret_cast<ApplyRows*>(smem);
@@ -366,6 +424,41 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   unsigned char* mids = ring + 128 * R * 4;      // halves of mid: [2][tile][PM], over the ring
   const uint16_t* in = static_cast<const uint16_t*>(p.in);
   const uint16_t* base = static_cast<const uint16_t*>(p.base);
+  const int chunks2 = (int)((a.D2 + 31) / 32), per2 = (chunks2 + csize - 1) / csize;
+  const int ch_begin = min(chunks2, crank * per2), ch_end = min(chunks2, ch_begin + per2);
+  const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
+  const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
+  // ---- partial sums over this CTA's input columns
+  const uint16_t* U = static_cast<const uint16_t*>(p.U) + (int64_t)group * a.D1 * a.r;
+  const int step = NW * WK, chunks = (w_end - w_begin + step - 1) / step;
+  const int wm = warp % WM, wk = warp / WM;
+
+  // What a thread stages of U is an arithmetic sequence: piece q of every
+  // ROWS-th row from k0 on, each row at the place its window's order gives it.
+  constexpr int ROWS = kApThreads / NT;
+  const int q = tid % NT, k0 = tid / NT;
+  auto slot_of = [](int k) { return (k & ~31) | ((k & 6) << 2) | (((k & 31) >> 3) << 1) | (k & 1); };
+  const bool rank = q * 8 < a.r;
+  const uint16_t* u_src = U + ((int64_t)w_begin * kApWin + k0) * a.r + (rank ? q * 8 : 0);
+  int u_left = (int)(a.D1 - (int64_t)w_begin * kApWin) - k0;  // rows from u_src on
+  const uint32_t u_dst = slot_of(k0) * PU + q * 16;
+  auto stage_u = [&](int c) {
+    if (c >= chunks) return;
+    unsigned char* dst = ring + (c % S) * step_bytes + u_dst;
+#pragma unroll 4
+    for (int i = 0; i * ROWS + k0 < KC; ++i) {
+      // of 32 rows a window's order keeps multiples of 16 apart: 16 rows on are 4 places on
+      const uint32_t to = ROWS == 16 ? (i >> 1) * 32 * PU + (i & 1) * 4 * PU : i * ROWS * PU;
+      const bool ok = rank && i * ROWS < u_left;
+      cp_async16(dst + to, ok ? u_src + (int64_t)i * ROWS * a.r : U, ok);
+    }
+    u_src += (int64_t)KC * a.r;
+    u_left -= KC;
+  };
+  // The first steps of U need no row number: they are on their way while the
+  // plan's rows are looked up.
+  for (int c = 0; c < S - 1; ++c) stage_u(c);
+  const uint16_t* V = static_cast<const uint16_t*>(p.V) + (int64_t)group * a.D2 * a.r;
   if (tid < a.tile) {
     const int place = first + min(tid, rows - 1);
     const int m = order ? min(max(order[place], 0), (int)a.M - 1) : place;
@@ -374,170 +467,107 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     at.out[tid] = static_cast<uint16_t*>(p.out) + (int64_t)m * p.ldo;
   }
   __syncthreads();
-  const int chunks2 = (int)((a.D2 + 31) / 32), per2 = (chunks2 + csize - 1) / csize;
-  const int ch_begin = min(chunks2, crank * per2), ch_end = min(chunks2, ch_begin + per2);
-  const int wins = (int)((a.D1 + kApWin - 1) / kApWin), per = (wins + csize - 1) / csize;
-  const int w_begin = min(wins, crank * per), w_end = min(wins, w_begin + per);
-  if (!none) {
-    // ---- partial sums over this CTA's input columns
-    const uint16_t* U = static_cast<const uint16_t*>(p.U) + (int64_t)group * a.D1 * a.r;
-    const int step = NW * WK, chunks = (w_end - w_begin + step - 1) / step;
-    const int wm = warp % WM, wk = warp / WM;
-    const uint16_t* xa = in + (int64_t)at.row[wm * 16 + g] * p.ldin;
-    const uint16_t* xb = in + (int64_t)at.row[wm * 16 + g + 8] * p.ldin;
-
-    auto stage = [&](int c) {
-      unsigned char* dst = ring + (c % S) * step_bytes;
-      const int64_t col0 = (int64_t)(w_begin + c * step) * kApWin;
-      if (c < chunks) {
-        // U's rows, each at the place that its window's order gives it
-        for (int i = tid; i < KC * NT; i += kApThreads) {
-          const int k = i / NT, q = i - k * NT;
-          const int in = k & 31, slot = (k & ~31) | ((in & 6) << 2) | ((in >> 3) << 1) | (in & 1);
-          const bool ok = col0 + k < a.D1 && q * 8 < a.r;
-          cp_async16(dst + slot * PU + q * 16, U + (ok ? (col0 + k) * a.r + q * 8 : 0), ok);
-        }
-        // this lane's part of the rows: what it multiplies it also fetches
-        unsigned char* x = dst + KC * PU + (warp * NW * 64 + lane) * 16;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const int win = w_begin + c * step + wk * NW + w;
-          const int64_t col = (int64_t)win * kApWin + t * 8;
-          if constexpr (VEC) {
-            const bool ok = win < w_end && col < a.D1;
-            cp_async16(x + w * 1024, xa + (ok ? col : 0), ok);
-            cp_async16(x + w * 1024 + 512, xb + (ok ? col : 0), ok);
-          } else {
-            *reinterpret_cast<uint4*>(x + w * 1024) = load_row8<false>(xa, win < w_end ? col : a.D1, a.D1);
-            *reinterpret_cast<uint4*>(x + w * 1024 + 512) = load_row8<false>(xb, win < w_end ? col : a.D1, a.D1);
-          }
-        }
-      }
-      cp_async_commit();
-    };
-    float acc[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-    for (int c = 0; c < S - 1; ++c) stage(c);
-    for (int c = 0; c < chunks; ++c) {
-      cp_async_wait<S - 2>();
-      __syncthreads();  // step c is here, and step c - 1, whose place comes next, has been read
-      stage(c + S - 1);
-      const unsigned char* u = ring + (c % S) * step_bytes + wk * NW * kApWin * PU;
-      const unsigned char* mine = ring + (c % S) * step_bytes + KC * PU + (warp * NW * 64 + lane) * 16;
+  const uint16_t* xa = in + (int64_t)at.row[wm * 16 + g] * p.ldin;
+  const uint16_t* xb = in + (int64_t)at.row[wm * 16 + g + 8] * p.ldin;
+  // this lane's part of the rows: what it multiplies it also fetches
+  const uint32_t x_dst = KC * PU + (warp * NW * 64 + lane) * 16;
+  int64_t x_col = (int64_t)(w_begin + wk * NW) * kApWin + t * 8;
+  const int64_t x_end = min((int64_t)w_end * kApWin, a.D1);
+  auto stage_x = [&](int c) {
+    if (c < chunks) {
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const uint4 x = *reinterpret_cast<const uint4*>(mine + w * 1024);
-        const uint4 y = *reinterpret_cast<const uint4*>(mine + w * 1024 + 512);
+        const int64_t col = x_col + w * kApWin;
+        unsigned char* x = ring + (c % S) * step_bytes + x_dst + w * 1024;
+        if constexpr (VEC) {
+          const bool ok = col < x_end;
+          cp_async16(x, xa + (ok ? col : 0), ok);
+          cp_async16(x + 512, xb + (ok ? col : 0), ok);
+        } else {
+          *reinterpret_cast<uint4*>(x) = load_row8<false>(xa, col, x_end);
+          *reinterpret_cast<uint4*>(x + 512) = load_row8<false>(xb, col, x_end);
+        }
+      }
+      x_col += step * kApWin;
+    }
+    cp_async_commit();
+  };
+  float acc[NT][4];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const unsigned char* row = u + (w * 32 + s * 16 + (lane & 15)) * PU + (lane >> 4) * 16;
+  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+  for (int c = 0; c < S - 1; ++c) stage_x(c);
+  for (int c = 0; c < chunks; ++c) {
+    cp_async_wait<S - 2>();
+    __syncthreads();  // step c is here, and step c - 1, whose place comes next, has been read
+    stage_u(c + S - 1);
+    stage_x(c + S - 1);
+    const unsigned char* u = ring + (c % S) * step_bytes + wk * NW * kApWin * PU;
+    const unsigned char* mine = ring + (c % S) * step_bytes + KC * PU + (warp * NW * 64 + lane) * 16;
 #pragma unroll
-          for (int j = 0; j < NT; j += 2) {
-            uint32_t b[4];
-            ldmatrix4_trans(b, row + j * 16);
-            Mma16816<DT>::run(acc[j], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[0], b[1]);
-            Mma16816<DT>::run(acc[j + 1], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[2], b[3]);
-          }
+    for (int w = 0; w < NW; ++w) {
+      const uint4 x = *reinterpret_cast<const uint4*>(mine + w * 1024);
+      const uint4 y = *reinterpret_cast<const uint4*>(mine + w * 1024 + 512);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const unsigned char* row = u + (w * 32 + s * 16 + (lane & 15)) * PU + (lane >> 4) * 16;
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          uint32_t b[4];
+          ldmatrix4_trans(b, row + j * 16);
+          Mma16816<DT>::run(acc[j], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[0], b[1]);
+          Mma16816<DT>::run(acc[j + 1], s ? x.z : x.x, s ? y.z : y.x, s ? x.w : x.y, s ? y.w : y.y, b[2], b[3]);
         }
       }
     }
-    cp_async_wait<0>();
-    __syncthreads();  // the sums lie over the ring
-
-    // ---- the sums meet: warps of the CTA in order, then the cluster's CTAs in rank order
-    float* mine = part + (wk * a.tile + wm * 16) * R;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      *reinterpret_cast<float2*>(mine + g * R + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2*>(mine + (g + 8) * R + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
-    }
-    __syncthreads();
-    if (WK > 1) {
-      for (int i = tid; i < a.tile * R; i += kApThreads) {
-        float v = part[i];
-        for (int w = 1; w < WK; ++w) v += part[w * a.tile * R + i];
-        part[i] = v;
-      }
-    }
-    cluster.sync();
-    // LR lanes a row, this CTA's share of the rows; the result goes to every CTA
-    constexpr int LR = R == 16 ? 8 : 16, E = R / LR;
-    const int share = (a.tile + csize - 1) / csize, l = tid % LR;
-    const float s = p.scaling[group];
-    for (int i0 = 0; i0 < share; i0 += kApThreads / LR) {
-      const int i = i0 + tid / LR, row = crank * share + i;
-      const bool on = i < share && row < a.tile;
-      __align__(16) float v[E];
-      float* src = part + (on ? row : 0) * R + l * E;
-      if constexpr (E == 2) *reinterpret_cast<float2*>(v) = cluster_sum<float2>(cluster, src, csize);
-#pragma unroll
-      for (int e = 0; e + 4 <= E; e += 4) *reinterpret_cast<float4*>(v + e) = cluster_sum<float4>(cluster, src + e, csize);
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[e] *= s;
-        top = fmaxf(top, fabsf(v[e]));
-        if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)at.row[row] * a.r + l * E + e] = v[e];
-      }
-      float mul = 1.0f, back = 1.0f;
-      if constexpr (DT == RQ_F16) {
-#pragma unroll
-        for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int ex = (int)(__float_as_uint(top) >> 23);  // biased exponent; 255: not finite, small: leave
-        if (ex > 30 && ex < 255) {
-          mul = __uint_as_float((uint32_t)(268 - ex) << 23);
-          back = __uint_as_float((uint32_t)(ex - 14) << 23);
-        }
-      }
-      if (on) {
-        __align__(16) uint32_t hi[E / 2], lo[E / 2];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) split16x2<DT>(v[e] * mul, v[e + 1] * mul, &hi[e / 2], &lo[e / 2]);
-        unsigned char* to = mids + row * PM + l * E * 2;
-        for (int c = 0; c < csize; ++c) {
-          unsigned char* m = cluster.map_shared_rank(to, c);
-          store_words<E / 2>(m, hi);
-          store_words<E / 2>(m + a.tile * PM, lo);
-          if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(at.mul, c)[row] = back;
-        }
-      }
-    }
-    cluster.sync();
-  } else {
-    if (p.mid && crank == 0)
-      for (int i = tid; i < rows * a.r; i += kApThreads) p.mid[(int64_t)at.row[i / a.r] * a.r + i % a.r] = fill;
-    if (p.out == p.base && fill == 0.0f) return;
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the sums lie over the ring
 
-  // ---- this warp's output columns, CW x 32 at a time, all rows of the tile.
-  // base starts the accumulators, so the sum costs no instruction of its own.
-  constexpr int CW = R <= 32 ? 2 : 1, AHEAD = R <= 32 ? 2 : 4;  // m-tiles of base under way
-  const int n_tiles = (rows + 15) / 16;
-  const uint16_t* V = static_cast<const uint16_t*>(p.V) + (none ? 0 : (int64_t)group * a.D2 * a.r);
-  for (int ch = ch_begin + warp * CW; ch < ch_end; ch += kApWarps * CW) {
-    const int64_t col = (int64_t)ch * 32 + 8 * t;
-    const int64_t end = min((int64_t)ch_end * 32, a.D2);  // columns this CTA writes
-    auto fetch = [&](uint4 (&old)[CW][2], int mt) {
-      const uint16_t* ra = at.base[mt * 16 + g];
-      const uint16_t* rb = at.base[mt * 16 + g + 8];
+  // ---- the sums meet: warps of the CTA in order, then the cluster's CTAs in rank order
+  float* mine = part + (wk * a.tile + wm * 16) * R;
 #pragma unroll
-      for (int w = 0; w < CW; ++w) {
-        old[w][0] = load_row8<VEC>(ra, col + 32 * w, end);
-        old[w][1] = load_row8<VEC>(rb, col + 32 * w, end);
+  for (int j = 0; j < NT; ++j) {
+    *reinterpret_cast<float2*>(mine + g * R + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2*>(mine + (g + 8) * R + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+  }
+  __syncthreads();
+  if (WK > 1) {
+    for (int i = tid; i < a.tile * R; i += kApThreads) {
+      float v = part[i];
+      for (int w = 1; w < WK; ++w) v += part[w * a.tile * R + i];
+      part[i] = v;
+    }
+  }
+  // ---- this warp's output columns, CW x 32 at a time, all rows of the tile, as
+  // one sequence of (chunk, m-tile): base is fetched AHEAD of them in advance,
+  // the first before the sums meet.
+  const int n_tiles = (rows + 15) / 16, ch_step = kApWarps * CW;
+  const int64_t end = min((int64_t)ch_end * 32, a.D2);  // columns this CTA writes
+  int f_ch = ch_begin + warp * CW, f_mt = 0;            // next to be fetched
+  uint4 ahead[AHEAD][CW][2] = {};
+  auto fetch = [&](uint4 (&old)[CW][2]) {
+    if (f_ch < ch_end) {
+      if (base) {
+        const uint16_t* ra = at.base[f_mt * 16 + g];
+        const uint16_t* rb = at.base[f_mt * 16 + g + 8];
+        const int64_t col = (int64_t)f_ch * 32 + 8 * t;
+#pragma unroll
+        for (int w = 0; w < CW; ++w) {
+          old[w][0] = load_row8<VEC>(ra, col + 32 * w, end);
+          old[w][1] = load_row8<VEC>(rb, col + 32 * w, end);
+        }
       }
-    };
-    uint4 ahead[AHEAD][CW][2] = {};
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (base && i < n_tiles) fetch(ahead[i], i);
-    // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
-    uint32_t b[CW][4][KS][2];
+      if (++f_mt == n_tiles) f_mt = 0, f_ch += ch_step;
+    }
+  };
+  // B fragments: for n-tile j the lane's column is 8 (g / 2) + 2 j + g % 2
+  uint32_t b[CW][4][KS][2];
+  auto load_b = [&](int ch) {
 #pragma unroll
     for (int j = 0; j < 4 * CW; ++j) {
       const int64_t n = (int64_t)ch * 32 + 32 * (j / 4) + 8 * (g >> 1) + 2 * (j % 4) + (g & 1);
       const uint16_t* v = V + n * a.r;
-      const bool ok = !none && n < end;
+      const bool ok = n < end;
       if constexpr (R == 16) {
         const uint2 q = ok && 4 * t < a.r ? *reinterpret_cast<const uint2*>(v + 4 * t) : make_uint2(0u, 0u);
         b[j / 4][j % 4][0][0] = q.x, b[j / 4][j % 4][0][1] = q.y;
@@ -551,108 +581,179 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
         }
       }
     }
-    auto tile = [&](int mt, uint4 (&old)[CW][2]) {
-      const int ra = mt * 16 + g;
-      // fp16: the row's power of two, taken off base here and put back below
-      float off_a = 1.0f, off_b = 1.0f, mul_a = 1.0f, mul_b = 1.0f;
-      if (DT == RQ_F16 && !none) {
-        mul_a = at.mul[ra], mul_b = at.mul[ra + 8];
-        off_a = __uint_as_float((254u << 23) - __float_as_uint(mul_a));
-        off_b = __uint_as_float((254u << 23) - __float_as_uint(mul_b));
+  };
+  if (f_ch < ch_end) load_b(f_ch);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(ahead[i]);
+  cluster.sync();
+  // LR lanes a row, this CTA's share of the rows; the result goes to every CTA
+  constexpr int LR = R == 16 ? 8 : 16, E = R / LR;
+  const int share = (a.tile + csize - 1) / csize, l = tid % LR;
+  const float s = p.scaling[group];
+  for (int i0 = 0; i0 < share; i0 += kApThreads / LR) {
+    const int i = i0 + tid / LR, row = crank * share + i;
+    const bool on = i < share && row < a.tile;
+    __align__(16) float v[E];
+    float* src = part + (on ? row : 0) * R + l * E;
+    if constexpr (E == 2) *reinterpret_cast<float2*>(v) = cluster_sum<float2>(cluster, src, csize);
+#pragma unroll
+    for (int e = 0; e + 4 <= E; e += 4) *reinterpret_cast<float4*>(v + e) = cluster_sum<float4>(cluster, src + e, csize);
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      v[e] *= s;
+      top = fmaxf(top, fabsf(v[e]));
+      if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)at.row[row] * a.r + l * E + e] = v[e];
+    }
+    float mul = 1.0f, back = 1.0f;
+    if constexpr (DT == RQ_F16) {
+#pragma unroll
+      for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int ex = (int)(__float_as_uint(top) >> 23);  // biased exponent; 255: not finite, small: leave
+      if (ex > 30 && ex < 255) {
+        mul = __uint_as_float((uint32_t)(268 - ex) << 23);
+        back = __uint_as_float((uint32_t)(ex - 14) << 23);
       }
-      float acc[CW][4][4];
+    }
+    if (on) {
+      __align__(16) uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) split16x2<DT>(v[e] * mul, v[e + 1] * mul, &hi[e / 2], &lo[e / 2]);
+      unsigned char* to = mids + row * PM + l * E * 2;
+      for (int c = 0; c < csize; ++c) {
+        unsigned char* m = cluster.map_shared_rank(to, c);
+        store_words<E / 2>(m, hi);
+        store_words<E / 2>(m + a.tile * PM, lo);
+        if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(at.mul, c)[row] = back;
+      }
+    }
+  }
+  cluster.sync();
+
+  // base starts the accumulators, so the sum costs no instruction of its own
+  auto tile = [&](int64_t col, int mt, uint4 (&old)[CW][2]) {
+    const int ra = mt * 16 + g;
+    // fp16: the row's power of two, taken off base here and put back below
+    float off_a = 1.0f, off_b = 1.0f, mul_a = 1.0f, mul_b = 1.0f;
+    if constexpr (DT == RQ_F16) {
+      mul_a = at.mul[ra], mul_b = at.mul[ra + 8];
+      off_a = __uint_as_float((254u << 23) - __float_as_uint(mul_a));
+      off_b = __uint_as_float((254u << 23) - __float_as_uint(mul_b));
+    }
+    float acc[CW][4][4];
+#pragma unroll
+    for (int w = 0; w < CW; ++w) {
+      const uint32_t qa[4] = {old[w][0].x, old[w][0].y, old[w][0].z, old[w][0].w};
+      const uint32_t qb[4] = {old[w][1].x, old[w][1].y, old[w][1].z, old[w][1].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = unpair16<DT>(qa[j]), y = unpair16<DT>(qb[j]);
+        if constexpr (DT == RQ_F16) {
+          acc[w][j][0] = x.x * off_a, acc[w][j][1] = x.y * off_a, acc[w][j][2] = y.x * off_b, acc[w][j][3] = y.y * off_b;
+        } else {
+          acc[w][j][0] = x.x, acc[w][j][1] = x.y, acc[w][j][2] = y.x, acc[w][j][3] = y.y;
+        }
+      }
+    }
+    fetch(old);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned char* ma = mids + (half * a.tile + ra) * PM;
+      const unsigned char* mb = ma + 8 * PM;
+      if constexpr (R == 16) {
+        const uint2 qa = *reinterpret_cast<const uint2*>(ma + 8 * t), qb = *reinterpret_cast<const uint2*>(mb + 8 * t);
+#pragma unroll
+        for (int w = 0; w < CW; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][0][0], b[w][j][0][1]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS / 2; ++k) {
+          const uint4 qa = *reinterpret_cast<const uint4*>(ma + 64 * k + 16 * t);
+          const uint4 qb = *reinterpret_cast<const uint4*>(mb + 64 * k + 16 * t);
+#pragma unroll
+          for (int w = 0; w < CW; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][2 * k][0], b[w][j][2 * k][1]);
+              Mma16816<DT>::run(acc[w][j], qa.z, qb.z, qa.w, qb.w, b[w][j][2 * k + 1][0], b[w][j][2 * k + 1][1]);
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (ra + 8 * h >= rows) continue;
+      uint16_t* dst = at.out[ra + 8 * h] + col;
+      const float mul = h ? mul_b : mul_a;
 #pragma unroll
       for (int w = 0; w < CW; ++w) {
-        const uint32_t qa[4] = {old[w][0].x, old[w][0].y, old[w][0].z, old[w][0].w};
-        const uint32_t qb[4] = {old[w][1].x, old[w][1].y, old[w][1].z, old[w][1].w};
+        uint32_t res[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 x = unpair16<DT>(qa[j]), y = unpair16<DT>(qb[j]);
-          if constexpr (DT == RQ_F16) {
-            acc[w][j][0] = x.x * off_a, acc[w][j][1] = x.y * off_a, acc[w][j][2] = y.x * off_b, acc[w][j][3] = y.y * off_b;
-          } else {
-            acc[w][j][0] = x.x, acc[w][j][1] = x.y, acc[w][j][2] = y.x, acc[w][j][3] = y.y;
-          }
+          float x = acc[w][j][2 * h], y = acc[w][j][2 * h + 1];
+          if constexpr (DT == RQ_F16) x *= mul, y *= mul;
+          res[j] = pair16<DT>(x, y);
+        }
+        if constexpr (VEC) {
+          if (col + 32 * w < end)
+            *reinterpret_cast<uint4*>(dst + 32 * w) = make_uint4(res[0], res[1], res[2], res[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + 32 * w + i < end) dst[32 * w + i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
         }
       }
-      if (base && mt + AHEAD < n_tiles) fetch(old, mt + AHEAD);
-      if (!none) {
+    }
+  };
+  int ch = ch_begin + warp * CW, mt = 0;
+  while (ch < ch_end) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const unsigned char* ma = mids + (half * a.tile + ra) * PM;
-          const unsigned char* mb = ma + 8 * PM;
-          if constexpr (R == 16) {
-            const uint2 qa = *reinterpret_cast<const uint2*>(ma + 8 * t), qb = *reinterpret_cast<const uint2*>(mb + 8 * t);
-#pragma unroll
-            for (int w = 0; w < CW; ++w)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][0][0], b[w][j][0][1]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < KS / 2; ++k) {
-              const uint4 qa = *reinterpret_cast<const uint4*>(ma + 64 * k + 16 * t);
-              const uint4 qb = *reinterpret_cast<const uint4*>(mb + 64 * k + 16 * t);
-#pragma unroll
-              for (int w = 0; w < CW; ++w)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  Mma16816<DT>::run(acc[w][j], qa.x, qb.x, qa.y, qb.y, b[w][j][2 * k][0], b[w][j][2 * k][1]);
-                  Mma16816<DT>::run(acc[w][j], qa.z, qb.z, qa.w, qb.w, b[w][j][2 * k + 1][0], b[w][j][2 * k + 1][1]);
-                }
-            }
-          }
-        }
+    for (int i = 0; i < AHEAD; ++i) {
+      if (ch >= ch_end) break;
+      tile((int64_t)ch * 32 + 8 * t, mt, ahead[i]);
+      if (++mt == n_tiles) {
+        mt = 0, ch += ch_step;
+        if (ch < ch_end) load_b(ch);
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (ra + 8 * h >= rows) continue;
-        uint16_t* dst = at.out[ra + 8 * h] + col;
-        const float mul = h ? mul_b : mul_a;
-#pragma unroll
-        for (int w = 0; w < CW; ++w) {
-          uint32_t res[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float x = acc[w][j][2 * h], y = acc[w][j][2 * h + 1];
-            if constexpr (DT == RQ_F16) x *= mul, y *= mul;
-            res[j] = pair16<DT>(group > a.count ? fill : x, group > a.count ? fill : y);
-          }
-          if constexpr (VEC) {
-            if (col + 32 * w < end)
-              *reinterpret_cast<uint4*>(dst + 32 * w) = make_uint4(res[0], res[1], res[2], res[3]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (col + 32 * w + i < end) dst[32 * w + i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
-          }
-        }
-      }
-    };
-    for (int mt = 0; mt < n_tiles; mt += AHEAD)
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
-        if (mt + i < n_tiles) tile(mt + i, ahead[i]);
+    }
   }
 }
 
 static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
 
 template <int DT, int R, int NW>
-static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, int csize, cudaStream_t st) {
+static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_t st) {
   const size_t ring = (size_t)ap_steps(R, NW) * (NW * (kApWarps / (p.a.tile / 16)) * kApWin * ap_pitch_u(R) + ap_x_bytes(NW));
   const size_t after = (size_t)128 * R * 4 + (size_t)2 * p.a.tile * ap_pitch_m(R);
   const size_t smem = sizeof(ApplyRows) + std::max(ring, after);
-  return launch_cluster(vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>, p,
-                        dim3((unsigned)(tiles * csize)), kApThreads, smem, csize, st);
+  const ClusterLaunch<ApplyArgs> l{vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>,
+                                   kApThreads, smem};
+  const int rc = l.prepare();
+  if (rc != RQ_OK) return rc;
+  // The cluster size of the least time: rounds of the GPU, each about 6 us of
+  // fixed cost and 1e-4 us a value of a CTA's share of in, base and out (8192
+  // rows, 4096 x 4096, rank 16, tiles of 128: 47 us with 4, 50 with 8, 65
+  // with 2).
+  const int* resident = l.resident();
+  const double expected = (double)p.a.M / p.a.tile + (p.a.plan ? 0.5 * p.a.count : 0.0);
+  const double work = 1e-4 * p.a.tile * ((double)p.a.D1 + 2.0 * p.a.D2);
+  int csize = 8;
+  double best = 1e30;
+  for (int c = 8; c >= 1; --c) {
+    const double rounds = std::ceil(std::min(expected, (double)tiles) / resident[c]);
+    if (rounds * (6.0 + work / c) < best) best = rounds * (6.0 + work / c), csize = c;
+  }
+  return l.launch(p, dim3((unsigned)(tiles * csize)), csize, st);
 }
 
 template <int DT, int NW>
-static int launch_apply_r(const ApplyArgs& p, bool vec, int64_t tiles, int csize, cudaStream_t st) {
-  if (p.a.r <= 16) return launch_apply<DT, 16, NW>(p, vec, tiles, csize, st);
-  if (p.a.r <= 32) return launch_apply<DT, 32, NW>(p, vec, tiles, csize, st);
-  if (p.a.r <= 64) return launch_apply<DT, 64, NW>(p, vec, tiles, csize, st);
-  return launch_apply<DT, 128, NW>(p, vec, tiles, csize, st);
+static int launch_apply_r(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_t st) {
+  if (p.a.r <= 16) return launch_apply<DT, 16, NW>(p, vec, tiles, st);
+  if (p.a.r <= 32) return launch_apply<DT, 32, NW>(p, vec, tiles, st);
+  if (p.a.r <= 64) return launch_apply<DT, 64, NW>(p, vec, tiles, st);
+  return launch_apply<DT, 128, NW>(p, vec, tiles, st);
 }
 
 int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const void* U, const void* V,
@@ -664,12 +765,11 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
   const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo};
   const bool vec = a.D1 % 8 == 0 && a.D2 % 8 == 0 && rows16b(in, ldin) && rows16b(out, ldo) &&
                    (!base || rows16b(base, ldb));
-  const int csize = fill_size((a.M + a.tile - 1) / a.tile, a.r <= 64 ? 2 : 1, 8);
   if (a.dt == RQ_BF16)
-    return a.tile >= 64 ? launch_apply_r<RQ_BF16, 2>(p, vec, tiles, csize, st)
-                        : launch_apply_r<RQ_BF16, 1>(p, vec, tiles, csize, st);
-  return a.tile >= 64 ? launch_apply_r<RQ_F16, 2>(p, vec, tiles, csize, st)
-                      : launch_apply_r<RQ_F16, 1>(p, vec, tiles, csize, st);
+    return a.tile >= 64 ? launch_apply_r<RQ_BF16, 2>(p, vec, tiles, st)
+                        : launch_apply_r<RQ_BF16, 1>(p, vec, tiles, st);
+  return a.tile >= 64 ? launch_apply_r<RQ_F16, 2>(p, vec, tiles, st)
+                      : launch_apply_r<RQ_F16, 1>(p, vec, tiles, st);
 }
 
 // ------------------------------------------------------------------- grad
@@ -912,42 +1012,44 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
 }
 
 template <int DT, bool CODES, bool VEC, int S>
-static int launch_grad(const GradArgs& p, int64_t blocks, int csize, cudaStream_t st) {
-  const int ring = kGrWarps * S * gr_step_bytes(CODES), smem = ring > kGrSums ? ring : kGrSums;
-  return launch_cluster(adapters_grad_k<DT, CODES, VEC, S>, p, dim3((unsigned)(blocks * csize), (unsigned)p.a.count),
-                        kGrThreads, smem, csize, st);
-}
-
-template <int DT>
-static int launch_grad_dt(const GradArgs& p, bool vec, bool deep, int64_t blocks, int csize, cudaStream_t st) {
-  if (p.zscale) return deep ? launch_grad<DT, true, true, 7>(p, blocks, csize, st) : launch_grad<DT, true, true, 3>(p, blocks, csize, st);
-  if (!vec) return launch_grad<DT, false, false, 2>(p, blocks, csize, st);
-  return deep ? launch_grad<DT, false, true, 5>(p, blocks, csize, st) : launch_grad<DT, false, true, 2>(p, blocks, csize, st);
-}
-
-int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
-                  void* G, cudaStream_t st) {
-  GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8};
-  const bool vec = rows16b(z, ldz) && a.D1 % 8 == 0;
-  const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols;
+static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
+  const size_t ring = (size_t)kGrWarps * S * gr_step_bytes(CODES);
+  const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, S>, kGrThreads, std::max(ring, (size_t)kGrSums)};
+  const int rc = l.prepare();
+  if (rc != RQ_OK) return rc;
   // A CTA costs about as much as 5 steps besides its steps (its sums through
   // shared memory, the cluster's meetings); the cluster size that takes the
   // fewest steps over all rounds of the GPU, for adapters of mean size.
-  const int64_t per_step = kGrWarps / p.groups * 16, each = (a.M + a.count - 1) / a.count;
+  const int* resident = l.resident();
+  const int64_t per_step = kGrWarps / p.groups * 16, each = (p.a.M + p.a.count - 1) / p.a.count;
+  int csize = 1;
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= 8; ++c) {
+    const int64_t rounds = (blocks * p.a.count + resident[c] - 1) / resident[c];
+    const int64_t steps = (each + per_step * c - 1) / (per_step * c);
+    if (rounds * (5 + steps) < best) best = rounds * (5 + steps), csize = c;
+  }
+  return l.launch(p, dim3((unsigned)(blocks * csize), (unsigned)p.a.count), csize, st);
+}
+
+template <int DT>
+static int launch_grad_dt(const GradArgs& p, bool vec, int64_t blocks, cudaStream_t st) {
   // Above rank 64 all warps read the same rows and the tensor cores wait for
   // L1: one CTA an SM with a deeper ring takes 116 instead of 140 us at 8192
   // rows, 4096 columns, rank 128.  At rank 16 and 11008 columns it is the two
   // CTAs that win, 51 against 59 us.
   const bool deep = p.groups == 8;
-  const int64_t slots = (deep ? 1 : 2) * num_sms();
-  int csize = 1;
-  int64_t best = INT64_MAX;
-  for (int c = 1; c <= 8; ++c) {
-    const int64_t rounds = (blocks * a.count * c + slots - 1) / slots, steps = (each + per_step * c - 1) / (per_step * c);
-    if (rounds * (5 + steps) < best) best = rounds * (5 + steps), csize = c;
-  }
-  return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, vec, deep, blocks, csize, st)
-                         : launch_grad_dt<RQ_F16>(p, vec, deep, blocks, csize, st);
+  if (p.zscale) return deep ? launch_grad<DT, true, true, 7>(p, blocks, st) : launch_grad<DT, true, true, 3>(p, blocks, st);
+  if (!vec) return launch_grad<DT, false, false, 2>(p, blocks, st);
+  return deep ? launch_grad<DT, false, true, 5>(p, blocks, st) : launch_grad<DT, false, true, 2>(p, blocks, st);
+}
+
+int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
+                  void* G, cudaStream_t st) {
+  const GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8};
+  const bool vec = rows16b(z, ldz) && a.D1 % 8 == 0;
+  const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols;
+  return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, vec, blocks, st) : launch_grad_dt<RQ_F16>(p, vec, blocks, st);
 }
 
 }  // namespace rq

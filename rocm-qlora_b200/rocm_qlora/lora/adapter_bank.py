@@ -47,11 +47,12 @@ class AdapterPlan:
 
 
 def tile_rows(rows: int, count: int) -> int:
-    """Rows computed together: about as many as an adapter has."""
+    """Rows computed together: about as many as an adapter has, and 128 only
+    where there are enough of them to fill the GPU."""
     for tile in (16, 32, 64):
         if rows <= tile * count:
             return tile
-    return 128
+    return 128 if rows > 4096 else 64
 
 
 def _plan_args(plan: Optional[AdapterPlan], rows: int, count: int):
