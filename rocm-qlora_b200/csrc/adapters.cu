@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   constexpr int NT = R / 8;               // n-tiles of the first product
   constexpr int KS = R / 16;              // k-steps of the second
   constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R), S = ap_steps(R, NW);
-  constexpr int CW = R <= 32 ? 2 : 1, AHEAD = R <= 32 ? 2 : 4;  // second product: 32-column chunks, m-tiles under way
+  constexpr int CW = R <= 32 ? 2 : 1, AHEAD = 2;  // second product: 32-column chunks of a warp, m-tiles under way
   extern __shared__ __align__(16) unsigned char smem[];
   const AdapterRows& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
