@@ -777,11 +777,18 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
 constexpr int kGrThreads = 256, kGrWarps = kGrThreads / 32;
 constexpr int kGrCols = 128;                                 // columns of a CTA: one block of 8-bit codes
 constexpr int kGrSums = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
-// One step of a warp in its ring: 16 rows of z (swizzled 16-byte pieces) and of
-// mid (16 ranks, padded so that fragment loads use distinct banks).
-constexpr int kGrMidPitch = 20 * 4;
+// One step in a ring: 16 rows of z (swizzled 16-byte pieces) and of mid (16
+// ranks a warp, padded so that fragment loads use distinct banks), and the
+// scales of codes.  RG warps, 16 ranks each, share a ring and its rows.
 __host__ __device__ constexpr int gr_row_bytes(bool codes) { return codes ? kGrCols : kGrCols * 2; }
-__host__ __device__ constexpr int gr_step_bytes(bool codes) { return 16 * (gr_row_bytes(codes) + kGrMidPitch + (codes ? 4 : 0)); }
+__host__ __device__ constexpr int gr_mid_pitch(int RG) { return (16 * RG + 4) * 4; }
+__host__ __device__ constexpr int gr_step_bytes(bool codes, int RG) {
+  return 16 * (gr_row_bytes(codes) + gr_mid_pitch(RG) + (codes ? 4 : 0));
+}
+// steps of a ring: about 100 KB of rings a CTA, so that two share an SM
+__host__ __device__ constexpr int gr_steps(bool codes, bool vec, int RG) {
+  return !vec ? 2 : (codes ? 3 : 2) + (RG == 1 ? 0 : RG == 2 ? 2 : RG == 4 ? 4 : 6);
+}
 
 struct GradArgs {
   AdapterRows a;
@@ -791,7 +798,6 @@ struct GradArgs {
   int64_t lds;
   const float* mid;
   void* G;
-  int groups;  // warps along the rank, 16 of it each: 1, 2, 4 or 8
 };
 
 // Two codes in the low bytes of a word's halves as 16-bit values, exact.  bf16:
@@ -814,24 +820,27 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 
 // G_a[d, j] = sum over the rows m of a of z[m, d] mid[m, j].
 //
-// One CTA sums 128 columns of one adapter; its warps split the rows (and the
-// rank, 16 each), and the CTAs of a cluster split the rows again.  Sums meet
-// in shared and distributed shared memory in warp and rank order, so equal
-// inputs give equal bits, without atomics or a workspace.
+// One CTA sums 128 columns of one adapter.  RG warps hold 16 ranks each; the
+// 8 / RG groups of them split the rows, and the CTAs of a cluster split them
+// again.  Sums meet in shared and distributed shared memory in group and rank
+// order, so equal inputs give equal bits, without atomics or a workspace.
 //
 // The reduction runs over rows, so the MMA's k index is the row and ldmatrix
-// transposes z's tile on its way to the registers.  Each warp fetches its own
-// 16-row steps by cp.async into its own ring (two lanes a row, so a lane needs
-// one row number a step) and nothing but its own lanes waits for them.  z is
-// read once (HBM bound up to rank 32; above, the warps that share rows read
-// them through L1 and the tensor cores' rate takes over).  Codes become 16-bit
-// values exactly; their scale multiplies the other operand, mid, in fp32,
-// which then enters as two 16-bit halves as in the row products.
-template <int DT, bool CODES, bool VEC, int S>
-__global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(const __grid_constant__ GradArgs p) {
+// transposes z's tile on its way to the registers.  Each group fetches its own
+// 16-row steps by cp.async into its own ring, a thread one row a step, and
+// only the group waits for them.  z is read once.  Codes become 16-bit values
+// exactly; their scale multiplies the other operand, mid, in fp32, which then
+// enters as two 16-bit halves as in the row products.
+//
+// Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
+// meetings) is what is seen: 64 MB of z at rank 16 take 22 us.
+template <int DT, bool CODES, bool VEC, int RG>
+__global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_constant__ GradArgs p) {
   using T = typename DType<DT>::T;
-  constexpr int ROW = gr_row_bytes(CODES), STEP = gr_step_bytes(CODES);
-  constexpr int PIECES = ROW / 32;  // 16-byte pieces a lane fetches: half a row
+  constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
+  constexpr int S = gr_steps(CODES, VEC, RG), MW = kGrWarps / RG, R16 = RG * 16;
+  constexpr int TR = 2 * RG;                    // threads of a group that fetch one row
+  constexpr int PIECES = (ROW / 16 + TR - 1) / TR;  // 16-byte pieces of it each
   extern __shared__ __align__(16) unsigned char smem[];
   float* sums = reinterpret_cast<float*>(smem);
   const AdapterRows& a = p.a;
@@ -839,7 +848,7 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
   const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
   const int block = (int)(blockIdx.x / csize), adapter = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int rg = warp % p.groups, mw = warp / p.groups, MW = kGrWarps / p.groups, R16 = p.groups * 16;
+  const int rg = warp % RG, mw = warp / RG;
 
   const int first = a.plan ? max(a.plan[1 + adapter], 0) : 0;
   const int last = a.plan ? min(a.plan[2 + adapter], (int)a.M) : (int)a.M;
@@ -859,12 +868,12 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
   int ex_now = 0;          // fp16: biased exponent that mid is scaled down by
   float mul = 1.0f;
 
-  // fetching: lane's row of a step and half of its pieces (even or odd ones)
-  const int frow = lane >> 1, fhalf = lane & 1;
+  // fetching: a thread's row of a step and every TR-th of its pieces
+  const int gt = rg * 32 + lane, frow = gt / TR, fpart = gt % TR;
   const int begin = first + (crank * MW + mw) * 16, stride = csize * MW * 16;
   const int steps = begin < last ? (last - begin + stride - 1) / stride : 0;
-  unsigned char* ring = smem + warp * S * STEP;
-  auto row_of = [&](int s) {  // batch row of this lane's row in step s; -1: none
+  unsigned char* ring = smem + mw * S * STEP;
+  auto row_of = [&](int s) {  // batch row of this thread's row in step s; -1: none
     const int place = begin + s * stride + frow;
     if (s >= steps || place >= last) return -1;
     return order ? min(max(order[place], 0), (int)a.M - 1) : place;
@@ -874,49 +883,57 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
     unsigned char* dst = ring + (s % S) * STEP;
     const bool on = next >= 0;
     const int64_t m = on ? next : 0;
-    const int j = rg * 16 + 8 * fhalf;
     if constexpr (CODES) {
-      const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0 + 16 * fhalf;
+      const uint8_t* row = static_cast<const uint8_t*>(p.z) + m * p.ldz + c0 + 16 * fpart;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        cp_async16(dst + frow * ROW + (((2 * i + fhalf) ^ (frow & 7)) << 4), row + 32 * i, on);
+        if (TR * i + fpart < ROW / 16)
+          cp_async16(dst + frow * ROW + (((TR * i + fpart) ^ (frow & 7)) << 4), row + 16 * TR * i, on);
     } else {
       const uint16_t* row = static_cast<const uint16_t*>(p.z) + m * p.ldz;
-      const int64_t left = a.D1 - c0 - 8 * fhalf;  // columns from this lane's first piece
+      const int64_t left = a.D1 - c0 - 8 * fpart;  // columns from this thread's first piece
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        unsigned char* to = dst + frow * ROW + (((2 * i + fhalf) ^ (frow & 7)) << 4);
+        unsigned char* to = dst + frow * ROW + (((TR * i + fpart) ^ (frow & 7)) << 4);
         if constexpr (VEC)
-          cp_async16(to, row + (16 * i < left ? c0 + 8 * fhalf + 16 * i : 0), on && 16 * i < left);
+          cp_async16(to, row + (8 * TR * i < left ? c0 + 8 * fpart + 8 * TR * i : 0), on && 8 * TR * i < left);
         else
-          *reinterpret_cast<uint4*>(to) = load_row8<false>(row, c0 + 8 * fhalf + 16 * i, on ? a.D1 : 0);
+          *reinterpret_cast<uint4*>(to) = load_row8<false>(row, c0 + 8 * fpart + 8 * TR * i, on ? a.D1 : 0);
       }
     }
     // 8 ranks of mid, and the row's scale
-    unsigned char* to = dst + 16 * ROW + frow * kGrMidPitch + 32 * fhalf;
-    const bool some = on && j < a.r;
-    const float* mid = p.mid + (some ? m * a.r + j : 0);
+    unsigned char* to = dst + 16 * ROW + frow * PITCH + 32 * fpart;
+    const bool some = on && 8 * fpart < a.r;
+    const float* mid = p.mid + (some ? m * a.r + 8 * fpart : 0);
     cp_async16(to, mid, some);
     cp_async16(to + 16, mid + 4, some);
-    if (CODES && fhalf == 0)
-      cp_async_small<4>(dst + 16 * (ROW + kGrMidPitch) + frow * 4, p.zscale + m * p.lds + block, on);
+    if (CODES && fpart == 0)
+      cp_async_small<4>(dst + 16 * (ROW + PITCH) + frow * 4, p.zscale + m * p.lds + block, on);
     cp_async_commit();
     next = row_of(s + 1);
   };
+  auto meet = [&] {  // the group's warps
+    if constexpr (RG == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + mw), "n"(32 * RG) : "memory");
+  };
   for (int s = 0; s < S - 1; ++s) fetch(s);
   for (int s = 0; s < steps; ++s) {
-    fetch(s + S - 1);
-    cp_async_wait<S - 1>();
-    __syncwarp();
+    // one warp alone may fetch before it waits (its lanes have met after step
+    // s - 1); warps that share a ring meet once, when step s is here and step
+    // s - 1 has been read
+    if constexpr (RG == 1) fetch(s + S - 1), cp_async_wait<S - 1>();
+    else cp_async_wait<S - 2>();
+    meet();
+    if constexpr (RG != 1) fetch(s + S - 1);
     const unsigned char* src = ring + (s % S) * STEP;
     // mid of rows 2t, 2t+1, 2t+8, 2t+9, ranks 2g and 2g+1 (n index g of the two n-tiles)
     float2 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 2 * t + (i & 1) + 4 * (i & 2);
-      v[i] = *reinterpret_cast<const float2*>(src + 16 * ROW + row * kGrMidPitch + 8 * g);
+      v[i] = *reinterpret_cast<const float2*>(src + 16 * ROW + row * PITCH + 64 * rg + 8 * g);
       if constexpr (CODES) {
-        const float f = *reinterpret_cast<const float*>(src + 16 * (ROW + kGrMidPitch) + row * 4);
+        const float f = *reinterpret_cast<const float*>(src + 16 * (ROW + PITCH) + row * 4);
         v[i].x *= f, v[i].y *= f;
       }
     }
@@ -972,7 +989,7 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
         for (int half = 0; half < 2; ++half)
           Mma16816<DT>::run(acc[i][n], f[0], f[1], f[2], f[3], b[half][n][0], b[half][n][1]);
     }
-    __syncwarp();  // all lanes have read the step before its place is fetched into
+    if constexpr (RG == 1) meet();  // all lanes have read the step before its place is fetched into
   }
   cp_async_wait<0>();
   __syncthreads();  // the sums lie over the ring
@@ -1011,17 +1028,17 @@ __global__ void __launch_bounds__(kGrThreads, S <= 3 ? 2 : 1) adapters_grad_k(co
   cluster.sync();  // the others have read this CTA's sums
 }
 
-template <int DT, bool CODES, bool VEC, int S>
+template <int DT, bool CODES, bool VEC, int RG>
 static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
-  const size_t ring = (size_t)kGrWarps * S * gr_step_bytes(CODES);
-  const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, S>, kGrThreads, std::max(ring, (size_t)kGrSums)};
+  const size_t ring = (size_t)(kGrWarps / RG) * gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG);
+  const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, RG>, kGrThreads, std::max(ring, (size_t)kGrSums)};
   const int rc = l.prepare();
   if (rc != RQ_OK) return rc;
   // A CTA costs about as much as 5 steps besides its steps (its sums through
   // shared memory, the cluster's meetings); the cluster size that takes the
   // fewest steps over all rounds of the GPU, for adapters of mean size.
   const int* resident = l.resident();
-  const int64_t per_step = kGrWarps / p.groups * 16, each = (p.a.M + p.a.count - 1) / p.a.count;
+  const int64_t per_step = kGrWarps / RG * 16, each = (p.a.M + p.a.count - 1) / p.a.count;
   int csize = 1;
   int64_t best = INT64_MAX;
   for (int c = 1; c <= 8; ++c) {
@@ -1032,24 +1049,26 @@ static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
   return l.launch(p, dim3((unsigned)(blocks * csize), (unsigned)p.a.count), csize, st);
 }
 
+template <int DT, bool CODES, bool VEC>
+static int launch_grad_r(const GradArgs& p, int64_t blocks, cudaStream_t st) {
+  if (p.a.r <= 16) return launch_grad<DT, CODES, VEC, 1>(p, blocks, st);
+  if (p.a.r <= 32) return launch_grad<DT, CODES, VEC, 2>(p, blocks, st);
+  if (p.a.r <= 64) return launch_grad<DT, CODES, VEC, 4>(p, blocks, st);
+  return launch_grad<DT, CODES, VEC, 8>(p, blocks, st);
+}
+
 template <int DT>
-static int launch_grad_dt(const GradArgs& p, bool vec, int64_t blocks, cudaStream_t st) {
-  // Above rank 64 all warps read the same rows and the tensor cores wait for
-  // L1: one CTA an SM with a deeper ring takes 116 instead of 140 us at 8192
-  // rows, 4096 columns, rank 128.  At rank 16 and 11008 columns it is the two
-  // CTAs that win, 51 against 59 us.
-  const bool deep = p.groups == 8;
-  if (p.zscale) return deep ? launch_grad<DT, true, true, 7>(p, blocks, st) : launch_grad<DT, true, true, 3>(p, blocks, st);
-  if (!vec) return launch_grad<DT, false, false, 2>(p, blocks, st);
-  return deep ? launch_grad<DT, false, true, 5>(p, blocks, st) : launch_grad<DT, false, true, 2>(p, blocks, st);
+static int launch_grad_dt(const GradArgs& p, int64_t blocks, cudaStream_t st) {
+  if (p.zscale) return launch_grad_r<DT, true, true>(p, blocks, st);
+  return rows16b(p.z, p.ldz) && p.a.D1 % 8 == 0 ? launch_grad_r<DT, false, true>(p, blocks, st)
+                                                : launch_grad_r<DT, false, false>(p, blocks, st);
 }
 
 int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
                   void* G, cudaStream_t st) {
-  const GradArgs p{a, z, ldz, zscale, lds, mid, G, a.r <= 16 ? 1 : a.r <= 32 ? 2 : a.r <= 64 ? 4 : 8};
-  const bool vec = rows16b(z, ldz) && a.D1 % 8 == 0;
+  const GradArgs p{a, z, ldz, zscale, lds, mid, G};
   const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols;
-  return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, vec, blocks, st) : launch_grad_dt<RQ_F16>(p, vec, blocks, st);
+  return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, blocks, st) : launch_grad_dt<RQ_F16>(p, blocks, st);
 }
 
 }  // namespace rq
