@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <deque>
 #include <mutex>
 
 #include "gemv_common.cuh"
@@ -298,14 +297,18 @@ struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at 
       size_t smem;
       int n[9];
     };
+    // one entry a kernel, shared-memory size (by tile) and device; a full table
+    // (more devices than it is made for) only means asking again
     static std::mutex mu;
-    static std::deque<Entry> known;
+    static Entry known[512];
+    static int count = 0;
+    thread_local Entry e;
     int dev = 0;
     cudaGetDevice(&dev);
     std::lock_guard<std::mutex> lock(mu);
-    for (const Entry& e : known)
-      if (e.k == (const void*)kern && e.dev == dev && e.smem == smem) return e.n;
-    Entry e{(const void*)kern, dev, smem, {}};
+    for (int i = 0; i < count; ++i)
+      if (known[i].k == (const void*)kern && known[i].dev == dev && known[i].smem == smem) return known[i].n;
+    e = Entry{(const void*)kern, dev, smem, {}};
     for (int c = 1; c <= 8; ++c) {
       cudaLaunchAttribute at;
       const cudaLaunchConfig_t cfg = config(dim3(c), c, &at, nullptr);
@@ -314,8 +317,8 @@ struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at 
         e.n[c] = std::max(1, num_sms() / c);
       }
     }
-    known.push_back(e);
-    return known.back().n;
+    if (count < 512) known[count++] = e;
+    return e.n;
   }
 
   int prepare() const { return ensure_smem_limit((const void*)kern, smem); }
@@ -839,6 +842,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   using T = typename DType<DT>::T;
   constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
   constexpr int S = gr_steps(CODES, VEC, RG), MW = kGrWarps / RG, R16 = RG * 16;
+  constexpr bool CONV = CODES && RG > 1;        // codes become 16-bit once for all warps of a group
   constexpr int TR = 2 * RG;                    // threads of a group that fetch one row
   constexpr int PIECES = (ROW / 16 + TR - 1) / TR;  // 16-byte pieces of it each
   extern __shared__ __align__(16) unsigned char smem[];
@@ -873,6 +877,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   const int begin = first + (crank * MW + mw) * 16, stride = csize * MW * 16;
   const int steps = begin < last ? (last - begin + stride - 1) / stride : 0;
   unsigned char* ring = smem + mw * S * STEP;
+  unsigned char* wide = smem + MW * S * STEP + mw * 16 * 2 * kGrCols;
   auto row_of = [&](int s) {  // batch row of this thread's row in step s; -1: none
     const int place = begin + s * stride + frow;
     if (s >= steps || place >= last) return -1;
@@ -926,6 +931,27 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     meet();
     if constexpr (RG != 1) fetch(s + S - 1);
     const unsigned char* src = ring + (s % S) * STEP;
+    if constexpr (CONV) {
+      // the group's 16-bit copy of the step: this thread's part of its row
+      constexpr int W = ROW / TR / 4;  // words of codes
+      uint32_t q[W], w[2 * W];
+      const unsigned char* from = src + frow * ROW + (((fpart * W / 4) ^ (frow & 7)) << 4) + (fpart * W % 4) * 4;
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        // pieces of 4 words, at their swizzled places
+        const unsigned char* at_ = W > 4 && i >= 4 ? src + frow * ROW + (((fpart * W / 4 + 1) ^ (frow & 7)) << 4) + (i - 4) * 4 : from + i * 4;
+        const uint2 v = *reinterpret_cast<const uint2*>(at_);
+        q[i] = v.x, q[i + 1] = v.y;
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        w[2 * i] = codes2<DT>(__byte_perm(q[i], 0, 0x4140)), w[2 * i + 1] = codes2<DT>(__byte_perm(q[i], 0, 0x4342));
+#pragma unroll
+      for (int i = 0; i < 2 * W / 4; ++i)
+        *reinterpret_cast<uint4*>(wide + frow * 2 * kGrCols + (((fpart * (W / 2) + i) ^ (frow & 7)) << 4)) =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      meet();
+    }
     // mid of rows 2t, 2t+1, 2t+8, 2t+9, ranks 2g and 2g+1 (n index g of the two n-tiles)
     float2 v[4];
 #pragma unroll
@@ -969,25 +995,28 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     }
     // A fragments: 8 x 8 pieces (rows 0-7 | 8-15) x (a piece | the next), transposed
     const int lrow = (lane & 7) + 8 * (lane >> 4), lpiece = (lane >> 3) & 1;
-    const unsigned char* z = src + lrow * ROW;
-    uint32_t raw[4];
+    const unsigned char* z = (CONV ? wide : src) + lrow * (CONV ? 2 * kGrCols : ROW);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t f[4];
-      if constexpr (CODES) {
-        // a piece holds 16 columns as 8 pairs: the even columns (i even) and the odd ones (i odd) of
-        // two pieces are an m-tile each
-        if (i % 2 == 0) ldmatrix4_trans(raw, z + (((i + lpiece) ^ (lrow & 7)) << 4));
+    for (int i = 0; i < 8; i += 2) {  // two m-tiles at a time: four sums between two products of one
+      uint32_t f[2][4];
+      if constexpr (CODES && !CONV) {
+        // a piece holds 16 columns as 8 pairs: the even columns (tile i) and the odd ones (tile i + 1) of
+        // two pieces
+        uint32_t raw[4];
+        ldmatrix4_trans(raw, z + (((i + lpiece) ^ (lrow & 7)) << 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = codes2<DT>(i % 2 ? raw[e] >> 8 : raw[e]);
+        for (int e = 0; e < 4; ++e) f[0][e] = codes2<DT>(raw[e]), f[1][e] = codes2<DT>(raw[e] >> 8);
       } else {
-        ldmatrix4_trans(f, z + (((2 * i + lpiece) ^ (lrow & 7)) << 4));
+        ldmatrix4_trans(f[0], z + (((2 * i + lpiece) ^ (lrow & 7)) << 4));
+        ldmatrix4_trans(f[1], z + (((2 * i + 2 + lpiece) ^ (lrow & 7)) << 4));
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-          Mma16816<DT>::run(acc[i][n], f[0], f[1], f[2], f[3], b[half][n][0], b[half][n][1]);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            Mma16816<DT>::run(acc[i + k][n], f[k][0], f[k][1], f[k][2], f[k][3], b[half][n][0], b[half][n][1]);
     }
     if constexpr (RG == 1) meet();  // all lanes have read the step before its place is fetched into
   }
@@ -1018,8 +1047,8 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   const int units = R16 / 4;
   for (int i = tid * csize + crank; i < kGrCols * units; i += csize * kGrThreads) {
     const int at = i / units, j = (i - at * units) * 4;
-    // codes: m-tile i has the even (odd) columns of pieces i and i + 1, i even (odd)
-    const int64_t d = c0 + (CODES ? (at & ~31) + 2 * (at & 15) + ((at >> 4) & 1) : at);
+    // codes read as pairs: m-tile i has the even (odd) columns of pieces i and i + 1, i even (odd)
+    const int64_t d = c0 + (CODES && !CONV ? (at & ~31) + 2 * (at & 15) + ((at >> 4) & 1) : at);
     if (d >= a.D1 || j >= a.r) continue;
     const float4 s = cluster_sum<float4>(cluster, sums + at * R16 + j, csize);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
@@ -1030,7 +1059,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
 
 template <int DT, bool CODES, bool VEC, int RG>
 static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
-  const size_t ring = (size_t)(kGrWarps / RG) * gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG);
+  const size_t ring = (size_t)(kGrWarps / RG) * (gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG) + (CODES && RG > 1 ? 16 * 2 * kGrCols : 0));
   const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, RG>, kGrThreads, std::max(ring, (size_t)kGrSums)};
   const int rc = l.prepare();
   if (rc != RQ_OK) return rc;

@@ -379,7 +379,7 @@ int rq_adapters_grad(const void* z, int64_t ld_z, const float* z_scales, const f
   const int64_t nb = (D + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
   if (!grad || (M > 0 && (!z || !mid))) return RQ_ERR_INVALID;
   if (M > 1 && ld_z < (z_scales ? nb * RQ_ACT8_BLOCK : D)) return RQ_ERR_INVALID;
-  if ((uintptr_t)z % (z_scales ? 16 : 2) || (z_scales && ld_z % 16) || (uintptr_t)mid % 16 || (uintptr_t)grad % 16)
+  if ((uintptr_t)z % (z_scales ? 16 : 2) || (z_scales && (ld_z % 16 || (uintptr_t)z_scales % 4)) || (uintptr_t)mid % 16 || (uintptr_t)grad % 16)
     return RQ_ERR_ALIGN;
   const AdapterRows a{M, D, 0, r, count, dtype, tile_rows, plan};
   return adapters_grad(a, z, ld_z, z_scales, nb, mid, grad, (cudaStream_t)stream);

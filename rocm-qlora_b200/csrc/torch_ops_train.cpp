@@ -272,7 +272,7 @@ void once(const char* what) {
 }
 
 Tensor rows_of(const Tensor& t) {
-  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  Tensor r = t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), t.size(-1)});
   return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
 
@@ -360,6 +360,7 @@ Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const 
                     const optional<Tensor>& codes, const optional<Tensor>& scales) {
   check_add(base, x, A, B, scaling, plan, plan_rows, plan_count, codes, scales);
   const Tensor b2 = rows_of(base), x2 = rows_of(x), a3 = A.contiguous(), b3 = B.contiguous(), s1 = scaling.contiguous();
+  TORCH_CHECK_VALUE(!scaling.requires_grad(), "scaling has no gradient: fold a trainable factor into A or B");
   const bool grad = at::GradMode::is_enabled() &&
                     (base.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
   Tensor y;

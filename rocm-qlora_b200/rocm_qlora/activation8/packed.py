@@ -10,6 +10,7 @@ One packed input serves every projection that reads it (q, k and v; gate and
 up): ``packed_x=`` of ``LoRALinear``, ``MultiLoRALinear`` and
 ``adapters_add``, whose backward multiplies the codes themselves.
 """
+import math
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -38,7 +39,7 @@ class PackedActivation:
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t as [rows, columns] with contiguous columns: a view where its strides allow."""
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 

@@ -364,3 +364,75 @@ def test_c_entry_refuses_bad_arguments():
     assert L.rq_adapter_plan_words(10, 0, 16) == -1 and L.rq_adapter_plan_words(10, 2, 20) == -1
     assert L.rq_adapter_plan(None, 1, 4, 2, 16, plan.data_ptr(), 4096, None) == -1
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_row_offsets_past_32_bits():
+    """Rows of x, base and dy that lie over 2^31 elements apart."""
+    from rocm_qlora.lora import AdapterPlan, adapters_add
+    t = make(18, 136, 72, 16, 2, torch.bfloat16)
+    wide = torch.empty(18 << 27, dtype=torch.bfloat16, device="cuda")
+    far = {n: wide[at:].as_strided((18, t[n].shape[1]), (1 << 27, 1)) for n, at in (("x", 0), ("base", 256), ("dy", 512))}
+    for n, v in far.items():
+        v.copy_(t[n])
+    plan = AdapterPlan(t["ids"], 2)
+    out = []
+    for src in (t, far):
+        x, A, B = src["x"].detach().requires_grad_(), t["A"].clone().requires_grad_(), t["B"].clone().requires_grad_()
+        y = adapters_add(src["base"], x, A, B, t["scaling"], plan)
+        out.append((y, *torch.autograd.grad(y, (x, A, B), src["dy"])))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.gpu
+def test_graph_replay_follows_its_inputs():
+    from rocm_qlora.lora import AdapterPlan, adapters_add
+    t = make(40, 264, 136, 16, 3, torch.bfloat16)
+    ids, x = t["ids"].clone(), t["x"].clone()
+    call = lambda: adapters_add(t["base"], x, t["A"], t["B"], t["scaling"], AdapterPlan(ids, 3))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    for seed in (1, 2):
+        other = make(40, 264, 136, 16, 3, torch.bfloat16, seed=seed)
+        ids.copy_(other["ids"])
+        x.copy_(other["x"])
+        graph.replay()
+        assert torch.equal(y, call())
+
+
+@pytest.mark.gpu
+def test_small_float16_gradients_keep_their_precision():
+    """fp16 with gradients near 1e-6, as without loss scaling: the intermediate
+    is brought into fp16's range by a power of two, so A's gradient errs by
+    its own rounding (subnormal here) and no more."""
+    t = make(200, 264, 136, 16, 2, torch.float16)
+    t["dy"] = (t["dy"].float() * 1e-3).half()
+    t["x"] = (t["x"].float() * 30.0).half()
+    t["B"] = (t["B"].float() * 1e-2).half()
+    y, grads = run(t)
+    for got, w, name in zip((y, *grads[1:]), formula(t), ("y", "dx", "dA", "dB")):
+        check(got, w, name)
+
+
+@pytest.mark.gpu
+def test_create_graph_is_refused():
+    from rocm_qlora.lora import AdapterPlan, adapters_add
+    t = make(8, 64, 32, 8, 1, torch.bfloat16)
+    x = t["x"].requires_grad_()
+    y = adapters_add(t["base"], x, t["A"], t["B"], t["scaling"], AdapterPlan(t["ids"], 1))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y, x, t["dy"], create_graph=True)
+
+
+@pytest.mark.gpu
+def test_empty_dimensions():
+    from rocm_qlora.activation8 import pack_activation, swiglu8, unpack_activation
+    for shape in ((0, 5), (3, 0), (2, 0, 7), (2, 3, 0)):
+        x = torch.zeros(shape, device="cuda", dtype=torch.bfloat16)
+        assert unpack_activation(pack_activation(x)).shape == shape and swiglu8(x, x).shape == shape
