@@ -395,7 +395,7 @@ RQ_API int rq_token_logprobs(const void* logits, int dtype, int64_t stride_b, in
  * reference model's log-probabilities, R_b = sum (log p - ref) over the
  * labels that count, n_b their number (at least 1), z_i = beta (R_i - R_{i+B/2}):
  *   RQ_PREF_SIGMOID: mean(-(1 - smooth) log sigma(z) - smooth log sigma(-z))
- *   RQ_PREF_IPO:     mean((R_i / n_i - R_{i+B/2} / n_{i+B/2} - 1 / (2 beta))^2)
+ *   RQ_PREF_IPO:     mean((R_i / n_i - R_{i+B/2} / n_{i+B/2} - 1 / (2 beta))^2), smooth unused
  * Writes loss [1], logps [B] (sums of log p), rewards [B] (beta R) and
  * slopes [B] (d loss / d R), all fp32. */
 #define RQ_PREF_SIGMOID 0

@@ -49,7 +49,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
 
         sigmoid: mean(-(1 - w) log sigma(z) - w log sigma(-z)),
                  z = beta (R_chosen - R_rejected), w = label_smoothing
-        ipo:     mean((R_chosen / n - R_rejected / n - 1 / (2 beta))^2)
+        ipo:     mean((R_chosen / n - R_rejected / n - 1 / (2 beta))^2), which has no w
     """
     if form not in _FORMS:
         raise ValueError(f"form must be one of {sorted(_FORMS)}, got {form!r}")
@@ -57,8 +57,6 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError(f"beta must be positive, got {beta}")
     if not 0.0 <= label_smoothing <= 0.5:
         raise ValueError(f"label_smoothing must be between 0 and 0.5, got {label_smoothing}")
-    if form == "ipo" and label_smoothing:
-        raise ValueError("label_smoothing belongs to the sigmoid form")
     try:
         return PreferenceOutput(*nat.loaded_ops().preference_loss(
             logits, labels, ref_logps, int(ignore_index), _FORMS[form], float(beta), float(label_smoothing)))
