@@ -120,22 +120,20 @@ Tensor adapters_grad(const Tensor& z, const optional<Tensor>& scales, const Tens
   return grad;
 }
 
-std::tuple<Tensor, Tensor> packed_like(const Tensor& x, int64_t copies) {
-  const int64_t nb = (x.size(1) + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
-  return {at::empty({copies, x.size(0), nb * RQ_ACT8_BLOCK}, x.options().dtype(at::kChar)),
-          at::empty({copies, x.size(0), nb}, x.options().dtype(at::kFloat))};
-}
+int64_t blocks_of(int64_t K) { return (K + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK; }
 
 std::tuple<Tensor, Tensor> act8_pack(const Tensor& x) {
   check_rows(x, "x");
-  auto [codes, scales] = packed_like(x, 1);
+  const int64_t nb = blocks_of(x.size(1));
+  Tensor codes = at::empty({x.size(0), nb * RQ_ACT8_BLOCK}, x.options().dtype(at::kChar));
+  Tensor scales = at::empty({x.size(0), nb}, x.options().dtype(at::kFloat));
   if (!x.is_meta()) {
     const c10::cuda::CUDAGuard guard(x.device());
     check(rq_act8_pack(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), x.size(0), x.size(1),
                        codes.data_ptr<int8_t>(), scales.data_ptr<float>(), stream_of(x)),
           "rq_act8_pack");
   }
-  return {codes[0], scales[0]};
+  return {codes, scales};
 }
 
 void check_packed(const Tensor& codes, const Tensor& scales, int64_t K) {
@@ -164,7 +162,9 @@ std::tuple<Tensor, Tensor, Tensor> swiglu8_forward(const Tensor& gate, const Ten
   check_rows(up, "up");
   TORCH_CHECK(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type(),
               "rocm_qlora: gate and up must have one shape and dtype");
-  auto [codes, scales] = packed_like(gate, copies);
+  const int64_t nb = blocks_of(gate.size(1));
+  Tensor codes = at::empty({copies, gate.size(0), nb * RQ_ACT8_BLOCK}, gate.options().dtype(at::kChar));
+  Tensor scales = at::empty({copies, gate.size(0), nb}, gate.options().dtype(at::kFloat));
   Tensor h = at::empty({gate.size(0), gate.size(1)}, gate.options());
   if (!gate.is_meta()) {
     const c10::cuda::CUDAGuard guard(gate.device());
@@ -376,7 +376,7 @@ Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const 
 struct Swiglu8 : Function<Swiglu8> {
   static variable_list forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up, int64_t copies) {
     auto [h, codes, scales] = swiglu8_forward(rows_of(gate), rows_of(up), copies);
-    ctx->save_for_backward({codes.narrow(0, 0, 2), scales.narrow(0, 0, 2)});
+    ctx->save_for_backward({codes, scales});  // a third copy (of h) is in the same storage in any case
     ctx->saved_data["shape"] = gate.sizes().vec();
     ctx->mark_non_differentiable({codes, scales});
     return {h.view(gate.sizes()), codes, scales};
@@ -391,14 +391,32 @@ struct Swiglu8 : Function<Swiglu8> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor> swiglu8(const Tensor& gate, const Tensor& up, int64_t copies) {
+// h and, with copies = 3, the packed form of h
+std::tuple<Tensor, optional<Tensor>, optional<Tensor>> swiglu8(const Tensor& gate, const Tensor& up, int64_t copies) {
   TORCH_CHECK_VALUE(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type(), "gate ", gate.sizes(), " ",
                     gate.scalar_type(), " and up ", up.sizes(), " ", up.scalar_type(), " differ");
   TORCH_CHECK_VALUE(gate.dim() >= 1, "swiglu8 needs at least one dimension");
   check_float(gate.scalar_type());
   check_gpu({&gate, &up});
   auto v = Swiglu8::apply(gate, up, copies);
-  return {v[0], v[1], v[2]};
+  if (copies < 3) return {v[0], std::nullopt, std::nullopt};
+  return {v[0], v[1].select(0, 2), v[2].select(0, 2)};
+}
+
+// The public forms of pack and unpack: any shape [..., K].
+std::tuple<Tensor, Tensor> pack_activation(const Tensor& x) {
+  TORCH_CHECK_VALUE(x.dim() >= 1, "pack_activation needs at least one dimension");
+  check_float(x.scalar_type());
+  check_gpu({&x});
+  return act8_pack(rows_of(x.detach()));
+}
+
+Tensor unpack_activation(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, at::ScalarType dtype) {
+  check_float(dtype);
+  check_gpu({&codes, &scales});
+  TORCH_CHECK_VALUE(!shape.empty(), "unpack_activation needs at least one dimension");
+  Tensor out = act8_unpack(codes, scales, shape.back(), dtype);
+  return shape.size() == 2 ? out : out.view(shape);
 }
 
 struct Preference : Function<Preference> {
@@ -494,7 +512,9 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
   m.def(
       "adapters_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor scaling, Tensor? plan, int plan_rows, "
       "int plan_count, int tile, Tensor? codes, Tensor? scales) -> Tensor", &adapters_add);
-  m.def("swiglu8(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor, Tensor)", &swiglu8);
+  m.def("swiglu8(Tensor gate, Tensor up, int copies) -> (Tensor, Tensor?, Tensor?)", &swiglu8);
+  m.def("pack_activation(Tensor x) -> (Tensor, Tensor)", &pack_activation);
+  m.def("unpack_activation(Tensor codes, Tensor scales, int[] shape, ScalarType dtype) -> Tensor", &unpack_activation);
   m.def(
       "preference_loss(Tensor logits, Tensor labels, Tensor ref, int ignore, int form, float beta, float smooth) "
       "-> (Tensor, Tensor, Tensor, Tensor)", &preference_loss);

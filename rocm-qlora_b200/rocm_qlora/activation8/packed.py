@@ -47,17 +47,17 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     """Pack x [..., K] (float32, bfloat16 or float16).  A block whose largest
     magnitude is below 2^-100 is stored as zeros; one that holds an infinity
     or NaN unpacks to NaN."""
-    if x.dim() < 1:
-        raise ValueError("pack_activation needs at least one dimension")
-    nat.dtype_code(x.dtype)
-    with torch.no_grad():
-        codes, scales = nat.require_ops(x).act8_pack(rows_of(x))
+    try:
+        codes, scales = nat.loaded_ops().pack_activation(x)
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None
     return PackedActivation(codes, scales, tuple(x.shape), x.dtype)
 
 
 def unpack_activation(packed: PackedActivation, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """code * scale, rounded to ``dtype`` (default: the dtype that was packed)."""
-    dtype = packed.dtype if dtype is None else dtype
-    nat.dtype_code(dtype)
-    out = nat.require_ops(packed.codes, packed.scales).act8_unpack(packed.codes, packed.scales, packed.shape[-1], dtype)
-    return out.view(packed.shape)
+    try:
+        return nat.loaded_ops().unpack_activation(packed.codes, packed.scales, packed.shape,
+                                                  packed.dtype if dtype is None else dtype)
+    except NotImplementedError as e:
+        raise nat.NativeUnavailable(str(e)) from None

@@ -21,4 +21,4 @@ def swiglu8(gate: torch.Tensor, up: torch.Tensor,
         h, codes, scales = nat.loaded_ops().swiglu8(gate, up, 3 if pack_output else 2)
     except NotImplementedError as e:
         raise nat.NativeUnavailable(str(e)) from None
-    return (h, PackedActivation(codes[2], scales[2], tuple(h.shape), h.dtype)) if pack_output else h
+    return (h, PackedActivation(codes, scales, tuple(h.shape), h.dtype)) if pack_output else h
