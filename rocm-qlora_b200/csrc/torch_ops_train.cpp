@@ -379,6 +379,7 @@ struct Swiglu8 : Function<Swiglu8> {
     ctx->save_for_backward({codes, scales});  // a third copy (of h) is in the same storage in any case
     ctx->saved_data["shape"] = gate.sizes().vec();
     ctx->mark_non_differentiable({codes, scales});
+    ctx->set_materialize_grads(false);  // no zeros in the place of the codes' gradient
     return {h.view(gate.sizes()), codes, scales};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -426,6 +427,7 @@ struct Preference : Function<Preference> {
     ctx->save_for_backward({logits, labels, stats, slopes});
     ctx->saved_data["ignore"] = ignore;
     ctx->mark_non_differentiable({logps, rewards});
+    ctx->set_materialize_grads(false);
     return {loss, logps, rewards};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
