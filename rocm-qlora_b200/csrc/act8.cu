@@ -255,13 +255,18 @@ __global__ void __launch_bounds__(kA8Threads) act8_unpack_k(const int8_t* __rest
   store8<DT, VEC>(static_cast<T*>(out) + p.row * K + p.col, p.left, from_floats<DT>(v));
 }
 
-// 1 / (1 + e^-g).  The fast exponential and reciprocal err by a few units in
-// the last place of 32 bits, far below a 16-bit result's rounding; 32-bit
-// tensors take the accurate ones.
+// 1 / (1 + e^-g).  For 16-bit tensors the approximate exponential and
+// reciprocal, which err by 2^-22 of their value, and by the rounding of
+// g log2(e) in the exponent's argument (|g| 2^-24): far below a 16-bit
+// result's rounding.  Denormal results (g below -87) are zero.  32-bit tensors
+// take the accurate functions.
 template <int DT>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (DT == RQ_F32) return ieee_div(1.0f, 1.0f + expf(-g));
-  return __fdividef(1.0f, 1.0f + __expf(-g));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
 }
 
 // h = silu(g) u, with g and u (and h as it was rounded) packed in the same pass.
