@@ -843,6 +843,10 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
   constexpr int S = gr_steps(CODES, VEC, RG), MW = kGrWarps / RG, R16 = RG * 16;
   constexpr bool CONV = CODES && RG > 1;        // codes become 16-bit once for all warps of a group
+  // m-tiles at a time: two put four sums between two products of one sum; with
+  // one warp a ring the registers for that are not there (22 against 25 us at
+  // 8192 rows, 4096 columns, rank 16)
+  constexpr int PAIR = RG == 1 && !CODES ? 1 : 2;
   constexpr int TR = 2 * RG;                    // threads of a group that fetch one row
   constexpr int PIECES = (ROW / 16 + TR - 1) / TR;  // 16-byte pieces of it each
   extern __shared__ __align__(16) unsigned char smem[];
@@ -997,23 +1001,23 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     const int lrow = (lane & 7) + 8 * (lane >> 4), lpiece = (lane >> 3) & 1;
     const unsigned char* z = (CONV ? wide : src) + lrow * (CONV ? 2 * kGrCols : ROW);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {  // two m-tiles at a time: four sums between two products of one
-      uint32_t f[2][4];
+    for (int i = 0; i < 8; i += PAIR) {
+      uint32_t f[PAIR][4];
       if constexpr (CODES && !CONV) {
         // a piece holds 16 columns as 8 pairs: the even columns (tile i) and the odd ones (tile i + 1) of
         // two pieces
         uint32_t raw[4];
         ldmatrix4_trans(raw, z + (((i + lpiece) ^ (lrow & 7)) << 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[0][e] = codes2<DT>(raw[e]), f[1][e] = codes2<DT>(raw[e] >> 8);
+        for (int e = 0; e < 4; ++e) f[0][e] = codes2<DT>(raw[e]), f[PAIR - 1][e] = codes2<DT>(raw[e] >> 8);
       } else {
-        ldmatrix4_trans(f[0], z + (((2 * i + lpiece) ^ (lrow & 7)) << 4));
-        ldmatrix4_trans(f[1], z + (((2 * i + 2 + lpiece) ^ (lrow & 7)) << 4));
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) ldmatrix4_trans(f[k], z + (((2 * (i + k) + lpiece) ^ (lrow & 7)) << 4));
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < PAIR; ++k)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
             Mma16816<DT>::run(acc[i + k][n], f[k][0], f[k][1], f[k][2], f[k][3], b[half][n][0], b[half][n][1]);
