@@ -257,7 +257,8 @@ __device__ __forceinline__ V cluster_sum(cg::cluster_group& cluster, float* p, i
   constexpr int E = sizeof(V) / 4;
   V q[8], s;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) q[c] = *reinterpret_cast<const V*>(cluster.map_shared_rank(p, c < csize ? c : 0));
+  for (int c = 0; c < 8; ++c)
+    if (c < csize) q[c] = *reinterpret_cast<const V*>(cluster.map_shared_rank(p, c));
   float* f = reinterpret_cast<float*>(&s);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -1027,20 +1028,24 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   cp_async_wait<0>();
   __syncthreads();  // the sums lie over the ring
 
-  // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3
+  // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3; groups
+  // without a row have nothing to add
+  const int active = min(MW, max(1, (last - first - crank * MW * 16 + 15) / 16));
   const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
   float* mine = sums + mw * kGrCols * R16 + rg * 16 + 4 * t;
+  if (mw < active) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<float4*>(mine + (16 * i + g + 8 * h) * R16) =
-          make_float4(acc[i][0][2 * h] * back, acc[i][1][2 * h] * back, acc[i][0][2 * h + 1] * back,
-                      acc[i][1][2 * h + 1] * back);
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float4*>(mine + (16 * i + g + 8 * h) * R16) =
+            make_float4(acc[i][0][2 * h] * back, acc[i][1][2 * h] * back, acc[i][0][2 * h + 1] * back,
+                        acc[i][1][2 * h + 1] * back);
+  }
   __syncthreads();
-  for (int i = tid; i < kGrCols * R16 / 4; i += kGrThreads) {
+  for (int i = tid; active > 1 && i < kGrCols * R16 / 4; i += kGrThreads) {
     float4 s = reinterpret_cast<const float4*>(sums)[i];
-    for (int w = 1; w < MW; ++w) {
+    for (int w = 1; w < active; ++w) {
       const float4 q = reinterpret_cast<const float4*>(sums + w * kGrCols * R16)[i];
       s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
     }
