@@ -154,7 +154,9 @@ __host__ __device__ constexpr int ap_pitch_m(int R) { return R <= 32 ? R * 2 : R
 __host__ __device__ constexpr int ap_steps(int R, int NW) {
   return NW == 1 ? (R <= 32 ? 3 : 2) : (R == 64 ? 3 : 4);
 }
-__host__ __device__ constexpr int ap_x_bytes(int NW) { return kApWarps * NW * 2 * 32 * 16; }
+// A lane's piece of a row is 16 bytes, or 5 words where rows are not 16-byte
+// aligned (its 8 values and what shares their first or last word).
+__host__ __device__ constexpr int ap_x_bytes(int NW, bool words) { return kApWarps * NW * 2 * 32 * (words ? 20 : 16); }
 
 struct ApplyArgs {
   AdapterRows a;
@@ -168,6 +170,7 @@ struct ApplyArgs {
   float* mid;
   void* out;
   int64_t ldo;
+  bool vec_in;  // rows of `in` are whole aligned 16-byte pieces
 };
 
 // A tile's rows: batch row, where its base and output are and, for fp16, the
@@ -189,6 +192,16 @@ __device__ __forceinline__ void cp_async_small(void* dst, const void* src, bool 
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(d), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0)
                : "memory");
 }
+// The 4-byte word of values e and e + 1 of a row (e may be -1: the row's first
+// value sits in the word's upper half), as far as they lie before `end`.
+__device__ __forceinline__ void cp_async_word(void* dst, const uint16_t* row, int64_t e, int64_t end) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  const int64_t left = end - e;
+  const uint32_t bytes = left >= 2 ? 4u : left == 1 ? 2u : 0u;
+  // no bytes: any address will do, as long as it is aligned
+  const uint16_t* src = bytes ? row + e : reinterpret_cast<const uint16_t*>((uintptr_t)row & ~(uintptr_t)3);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -203,18 +216,44 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&d)[4], const void* p)
                : "memory");
 }
 
-// 8 consecutive 16-bit values of a row from column c, zero past `cols`.  VEC:
-// the row is 16-byte aligned and cols and c are multiples of 8.
+// 8 consecutive 16-bit values of a row from column c (a multiple of 8), zero
+// past `cols`.  VEC: the row is 16-byte aligned and cols a multiple of 8.
+// Other rows are read in aligned 4-byte words and shifted into place; a row at
+// an odd 2-byte address then reads the two bytes before its first value, which
+// share that value's word.
 template <bool VEC>
 __device__ __forceinline__ uint4 load_row8(const uint16_t* row, int64_t c, int64_t cols) {
   if constexpr (VEC) return c < cols ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
-  uint32_t w[4];
+  const uint32_t odd = ((uintptr_t)row >> 1) & 1;
+  uint32_t w[5];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = c + 2 * i < cols ? row[c + 2 * i] : 0u, hi = c + 2 * i + 1 < cols ? row[c + 2 * i + 1] : 0u;
-    w[i] = lo | (hi << 16);
+  for (int j = 0; j < 5; ++j) {
+    const int64_t e = c - odd + 2 * j;  // the word's first value
+    w[j] = 0;
+    if (j < 4 || odd) {
+      if (e + 1 < cols) w[j] = *reinterpret_cast<const uint32_t*>(row + e);
+      else if (e < cols) w[j] = row[e];
+    }
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(__funnelshift_r(w[0], w[1], 16 * odd), __funnelshift_r(w[1], w[2], 16 * odd),
+                    __funnelshift_r(w[2], w[3], 16 * odd), __funnelshift_r(w[3], w[4], 16 * odd));
+}
+
+// The first `n` of 8 packed values to a row that is only 2-byte aligned.
+__device__ __forceinline__ void store_row8(uint16_t* p, const uint32_t (&w)[4], int64_t n) {
+  if (n >= 8 && ((uintptr_t)p & 2) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+  } else if (n >= 8) {
+    p[0] = (uint16_t)w[0];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(p + 1 + 2 * i) = __funnelshift_r(w[i], w[i + 1], 16);
+    p[7] = (uint16_t)(w[3] >> 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
 }
 
 // Two fp32 values rounded to 16 bits, packed (low, high): one conversion.
@@ -421,7 +460,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     return;
   }
 
-  const int KC = NW * WK * kApWin, step_bytes = KC * PU + ap_x_bytes(NW);  // columns of a step
+  const int KC = NW * WK * kApWin, step_bytes = KC * PU + ap_x_bytes(NW, !p.vec_in);  // columns of a step
   ApplyRows& at = *reinterpret_cast<ApplyRows*>(smem);
   unsigned char* ring = smem + sizeof(ApplyRows);
   float* part = reinterpret_cast<float*>(ring);  // [128][R], over the ring
@@ -474,7 +513,8 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   const uint16_t* xa = in + (int64_t)at.row[wm * 16 + g] * p.ldin;
   const uint16_t* xb = in + (int64_t)at.row[wm * 16 + g + 8] * p.ldin;
   // this lane's part of the rows: what it multiplies it also fetches
-  const uint32_t x_dst = KC * PU + (warp * NW * 64 + lane) * 16;
+  const uint32_t x_dst = KC * PU + warp * NW * 64 * (p.vec_in ? 16 : 20) + lane * (p.vec_in ? 16 : 4);
+  const uint32_t odd_a = ((uintptr_t)xa >> 1) & 1, odd_b = ((uintptr_t)xb >> 1) & 1;
   int64_t x_col = (int64_t)(w_begin + wk * NW) * kApWin + t * 8;
   const int64_t x_end = min((int64_t)w_end * kApWin, a.D1);
   auto stage_x = [&](int c) {
@@ -482,19 +522,31 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const int64_t col = x_col + w * kApWin;
-        unsigned char* x = ring + (c % S) * step_bytes + x_dst + w * 1024;
-        if constexpr (VEC) {
+        unsigned char* x = ring + (c % S) * step_bytes + x_dst;
+        if (p.vec_in) {
           const bool ok = col < x_end;
-          cp_async16(x, xa + (ok ? col : 0), ok);
-          cp_async16(x + 512, xb + (ok ? col : 0), ok);
+          cp_async16(x + w * 1024, xa + (ok ? col : 0), ok);
+          cp_async16(x + w * 1024 + 512, xb + (ok ? col : 0), ok);
         } else {
-          *reinterpret_cast<uint4*>(x) = load_row8<false>(xa, col, x_end);
-          *reinterpret_cast<uint4*>(x + 512) = load_row8<false>(xb, col, x_end);
+#pragma unroll
+          for (int j = 0; j < 5; ++j) {
+            cp_async_word(x + w * 1280 + j * 128, xa, col - odd_a + 2 * j, col < x_end ? x_end : 0);
+            cp_async_word(x + w * 1280 + 640 + j * 128, xb, col - odd_b + 2 * j, col < x_end ? x_end : 0);
+          }
         }
       }
       x_col += step * kApWin;
     }
     cp_async_commit();
+  };
+  auto piece = [&](const unsigned char* x, int w, int h) {
+    if (p.vec_in) return *reinterpret_cast<const uint4*>(x + w * 1024 + h * 512);
+    uint32_t q[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) q[j] = *reinterpret_cast<const uint32_t*>(x + w * 1280 + h * 640 + j * 128);
+    const uint32_t by = 16 * (h ? odd_b : odd_a);
+    return make_uint4(__funnelshift_r(q[0], q[1], by), __funnelshift_r(q[1], q[2], by), __funnelshift_r(q[2], q[3], by),
+                      __funnelshift_r(q[3], q[4], by));
   };
   float acc[NT][4];
 #pragma unroll
@@ -506,11 +558,10 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     stage_u(c + S - 1);
     stage_x(c + S - 1);
     const unsigned char* u = ring + (c % S) * step_bytes + wk * NW * kApWin * PU;
-    const unsigned char* mine = ring + (c % S) * step_bytes + KC * PU + (warp * NW * 64 + lane) * 16;
+    const unsigned char* mine = ring + (c % S) * step_bytes + x_dst;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const uint4 x = *reinterpret_cast<const uint4*>(mine + w * 1024);
-      const uint4 y = *reinterpret_cast<const uint4*>(mine + w * 1024 + 512);
+      const uint4 x = piece(mine, w, 0), y = piece(mine, w, 1);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const unsigned char* row = u + (w * 32 + s * 16 + (lane & 15)) * PU + (lane >> 4) * 16;
@@ -704,9 +755,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
           if (col + 32 * w < end)
             *reinterpret_cast<uint4*>(dst + 32 * w) = make_uint4(res[0], res[1], res[2], res[3]);
         } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col + 32 * w + i < end) dst[32 * w + i] = (uint16_t)(res[i / 2] >> (16 * (i & 1)));
+          store_row8(dst + 32 * w, res, end - col - 32 * w);
         }
       }
     }
@@ -729,7 +778,7 @@ static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 &
 
 template <int DT, int R, int NW>
 static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_t st) {
-  const size_t ring = (size_t)ap_steps(R, NW) * (NW * (kApWarps / (p.a.tile / 16)) * kApWin * ap_pitch_u(R) + ap_x_bytes(NW));
+  const size_t ring = (size_t)ap_steps(R, NW) * (NW * (kApWarps / (p.a.tile / 16)) * kApWin * ap_pitch_u(R) + ap_x_bytes(NW, !p.vec_in));
   const size_t after = (size_t)128 * R * 4 + (size_t)2 * p.a.tile * ap_pitch_m(R);
   const size_t smem = sizeof(ApplyRows) + std::max(ring, after);
   const ClusterLaunch<ApplyArgs> l{vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>,
@@ -766,9 +815,8 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
   AdapterRows a = a0;
   if (!a.plan) a.tile = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 1024 ? 64 : 128;
   const int64_t tiles = a.plan ? plan_max_tiles(a.M, a.count, a.tile) : (a.M + a.tile - 1) / a.tile;
-  const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo};
-  const bool vec = a.D1 % 8 == 0 && a.D2 % 8 == 0 && rows16b(in, ldin) && rows16b(out, ldo) &&
-                   (!base || rows16b(base, ldb));
+  const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo, a.D1 % 8 == 0 && rows16b(in, ldin)};
+  const bool vec = a.D2 % 8 == 0 && rows16b(out, ldo) && (!base || rows16b(base, ldb));  // base and out
   if (a.dt == RQ_BF16)
     return a.tile >= 64 ? launch_apply_r<RQ_BF16, 2>(p, vec, tiles, st)
                         : launch_apply_r<RQ_BF16, 1>(p, vec, tiles, st);
