@@ -321,7 +321,7 @@ RQ_API int rq_linear_forward_gather(int wfmt, const void* qweight, const void* s
  * else int32): 0..count-1 is the adapter, -1 is none, and a row with any
  * other id gets NaN outputs.  tile_rows, 16, 32, 64 or 128, is how many rows
  * of one adapter are computed together; choose about the mean number of rows
- * per adapter. */
+ * per adapter, 128 only from some thousands of rows on. */
 #define RQ_ADAPTERS_MAX 4096
 RQ_API int64_t rq_adapter_plan_words(int64_t rows, int count, int tile_rows);
 RQ_API int rq_adapter_plan(const void* ids, int wide, int64_t rows, int count, int tile_rows,

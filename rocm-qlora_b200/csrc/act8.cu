@@ -7,9 +7,12 @@
 // 2^-100 (where 127 / max|x| could overflow) is stored as zeros; one that
 // holds an infinity or a NaN keeps scale NaN, so it stays visible.
 //
-// Everything here is one pass over the data, bound by HBM.  16 lanes hold a
-// block (8 values a lane: one 16-byte load of a 16-bit type), so the block's
-// maximum is four shuffles.
+// Everything here is one pass over the data.  16 lanes hold a block (8 values
+// a lane: one 16-byte load of a 16-bit type), so the block's maximum is four
+// shuffles.  Measured (bf16, 8192 x 11008): swiglu8 forward with three copies
+// 147 us, 5.5 TB/s (issue bound, 76 % of the slots: the encoding), backward
+// 115 us, 6.3 TB/s, and unpack 49 us, 5.5 TB/s (HBM); pack of 8192 x 4096 22
+// us, 4.6 TB/s.
 #include <cuda_runtime.h>
 
 #include "linear_common.cuh"

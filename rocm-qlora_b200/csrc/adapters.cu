@@ -186,11 +186,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool take
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-template <int BYTES>  // 4 or 8
-__device__ __forceinline__ void cp_async_small(void* dst, const void* src, bool take) {
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool take) {
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(d), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0)
-               : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(d), "l"(src), "r"(take ? 4 : 0) : "memory");
 }
 // The 4-byte word of values e and e + 1 of a row (e may be -1: the row's first
 // value sits in the word's upper half), as far as they lie before `end`.
@@ -422,12 +420,17 @@ __device__ __noinline__ void rows_without(const ApplyArgs& p, const int* order, 
 // Loads.  A quad's four lanes hold 32 consecutive columns of a row, 8 each, in
 // one 16-byte piece that the lane fetches for itself by cp.async several steps
 // ahead; the MMA's order of the reduction index follows that, and U's rows are
-// put into shared memory in the order that ldmatrix then needs.  V's columns are permuted the same way
-// among the MMA's n index, so that a lane ends with 8 consecutive output
-// columns: one 16-byte load of base and one store.
+// put into shared memory in the order that ldmatrix then needs.  V's columns
+// are permuted the same way among the MMA's n index, so that a lane ends with
+// 8 consecutive output columns: one 16-byte load of base and one store.
+//
+// Measured (bf16): one row of 4096 to 4096, rank 16, 5.9 us (a launch and a
+// chain of five dependent loads); 8192 rows, 45 us, 4.4 TB/s of the 201 MB
+// (31 us at the copy bandwidth; launch, plan, meeting and sums are the rest);
+// rank 64, 67 us, with the tensor pipe a third active: the two halves of mid
+// on mma.sync.  fp16 rows of 1093 to 1088, rank 64, 1111 of them: 14 us.
 template <int DT, int R, int NW, bool VEC>
 __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(const __grid_constant__ ApplyArgs p) {
-  using T = typename DType<DT>::T;
   constexpr int NT = R / 8;               // n-tiles of the first product
   constexpr int KS = R / 16;              // k-steps of the second
   constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R), S = ap_steps(R, NW);
@@ -778,7 +781,8 @@ static bool rows16b(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 &
 
 template <int DT, int R, int NW>
 static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_t st) {
-  const size_t ring = (size_t)ap_steps(R, NW) * (NW * (kApWarps / (p.a.tile / 16)) * kApWin * ap_pitch_u(R) + ap_x_bytes(NW, !p.vec_in));
+  const int columns = NW * (kApWarps / (p.a.tile / 16)) * kApWin;  // of a step
+  const size_t ring = (size_t)ap_steps(R, NW) * (columns * ap_pitch_u(R) + ap_x_bytes(NW, !p.vec_in));
   const size_t after = (size_t)128 * R * 4 + (size_t)2 * p.a.tile * ap_pitch_m(R);
   const size_t smem = sizeof(ApplyRows) + std::max(ring, after);
   const ClusterLaunch<ApplyArgs> l{vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>,
@@ -813,7 +817,7 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
                    const float* scaling, const void* base, int64_t ldb, float* mid, void* out, int64_t ldo,
                    cudaStream_t st) {
   AdapterRows a = a0;
-  if (!a.plan) a.tile = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 1024 ? 64 : 128;
+  if (!a.plan) a.tile = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 4096 ? 64 : 128;  // as plans are made
   const int64_t tiles = a.plan ? plan_max_tiles(a.M, a.count, a.tile) : (a.M + a.tile - 1) / a.tile;
   const ApplyArgs p{a, in, ldin, U, V, scaling, base, ldb, mid, out, ldo, a.D1 % 8 == 0 && rows16b(in, ldin)};
   const bool vec = a.D2 % 8 == 0 && rows16b(out, ldo) && (!base || rows16b(base, ldb));  // base and out
@@ -885,7 +889,9 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 // enters as two 16-bit halves as in the row products.
 //
 // Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
-// meetings) is what is seen: 64 MB of z at rank 16 take 22 us.
+// meetings) is what is seen: 64 MB of z at rank 16 take 21 us, 32 MB of codes
+// 20; rank 64 49 and 54 us, where four warps a group share the rows and the
+// two halves of mid are mma.sync's work.
 template <int DT, bool CODES, bool VEC, int RG>
 __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_constant__ GradArgs p) {
   using T = typename DType<DT>::T;
@@ -966,7 +972,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     cp_async16(to, mid, some);
     cp_async16(to + 16, mid + 4, some);
     if (CODES && fpart == 0)
-      cp_async_small<4>(dst + 16 * (ROW + PITCH) + frow * 4, p.zscale + m * p.lds + block, on);
+      cp_async4(dst + 16 * (ROW + PITCH) + frow * 4, p.zscale + m * p.lds + block, on);
     cp_async_commit();
     next = row_of(s + 1);
   };
@@ -988,12 +994,10 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
       // the group's 16-bit copy of the step: this thread's part of its row
       constexpr int W = ROW / TR / 4;  // words of codes
       uint32_t q[W], w[2 * W];
-      const unsigned char* from = src + frow * ROW + (((fpart * W / 4) ^ (frow & 7)) << 4) + (fpart * W % 4) * 4;
 #pragma unroll
       for (int i = 0; i < W; i += 2) {
-        // pieces of 4 words, at their swizzled places
-        const unsigned char* at_ = W > 4 && i >= 4 ? src + frow * ROW + (((fpart * W / 4 + 1) ^ (frow & 7)) << 4) + (i - 4) * 4 : from + i * 4;
-        const uint2 v = *reinterpret_cast<const uint2*>(at_);
+        const int k = fpart * W + i;  // word of the row, in piece k / 4
+        const uint2 v = *reinterpret_cast<const uint2*>(src + frow * ROW + (((k / 4) ^ (frow & 7)) << 4) + k % 4 * 4);
         q[i] = v.x, q[i + 1] = v.y;
       }
 #pragma unroll
@@ -1116,7 +1120,8 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
 
 template <int DT, bool CODES, bool VEC, int RG>
 static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
-  const size_t ring = (size_t)(kGrWarps / RG) * (gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG) + (CODES && RG > 1 ? 16 * 2 * kGrCols : 0));
+  const size_t wide = CODES && RG > 1 ? 16 * 2 * kGrCols : 0;  // the 16-bit copy of a step
+  const size_t ring = (size_t)(kGrWarps / RG) * (gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG) + wide);
   const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, RG>, kGrThreads, std::max(ring, (size_t)kGrSums)};
   const int rc = l.prepare();
   if (rc != RQ_OK) return rc;

@@ -139,8 +139,8 @@ struct ExpSum {
 // bound by HBM, with the exponentials (16 a clock of an SM) at 72 % of the
 // time a bf16 row takes to arrive.  The end of a row is a few serial steps, so
 // where rows are many, small CTAs of which eight share an SM hide it: 16384
-// rows of 32000 bf16 logits take 155 us with 128 threads (6.1 TB/s) and 244
-// with 512, but 128 rows 5.8 and 4.6 us.
+// rows of 32000 bf16 logits (14792 count) take 155 us with 128 threads (6.1
+// TB/s) and 244 with 512, but 128 rows 5.8 and 4.6 us.
 template <int DT, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, float4* __restrict__ stats,
                                                              float* __restrict__ logps) {
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(kPrefWarps * 32) __cluster_dims__(kPrefCtas, 1
 
 // dlogits = c ([v = y] - 2^(x log2(e) - k) / s), zero where the row does not
 // count.  One CTA a row, the rows in the reverse of the forward's order, so
-// that the last rows it read are still in L2.  HBM bound.
+// that the last rows it read are still in L2.  HBM bound: 300 us for 16384
+// rows of 32000 bf16 logits of which 14792 count, 6.7 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const float4* __restrict__ stats,
                                                             const float* __restrict__ slopes, int per_token,
