@@ -239,6 +239,7 @@ template <int DT, bool VEC>
 __global__ void __launch_bounds__(kA8Threads) act8_pack_k(const void* __restrict__ x, int64_t ld, uint32_t blocks,
                                                           int K, Divide nb, int8_t* __restrict__ codes,
                                                           float* __restrict__ scales) {
+  grid_begin();
   using T = typename DType<DT>::T;
   Place8 p;
   const bool any = place8<VEC>(p, blocks, K, nb);
@@ -250,6 +251,7 @@ template <int DT, bool VEC>
 __global__ void __launch_bounds__(kA8Threads) act8_unpack_k(const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales, uint32_t blocks, int K,
                                                             Divide nb, void* __restrict__ out) {
+  grid_begin();
   using T = typename DType<DT>::T;
   Place8 p;
   if (!place8<VEC>(p, blocks, K, nb)) return;
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(kA8Threads) swiglu8_forward_k(const void* __re
                                                                 uint32_t blocks, int K, Divide nb,
                                                                 void* __restrict__ h, int8_t* __restrict__ codes,
                                                                 float* __restrict__ scales) {
+  grid_begin();
   using T = typename DType<DT>::T;
   Place8 p;
   const bool any = place8<VEC>(p, blocks, K, nb);
@@ -303,6 +306,7 @@ __global__ void __launch_bounds__(kA8Threads) swiglu8_backward_k(const void* __r
                                                                  const float* __restrict__ scales, uint32_t blocks,
                                                                  int K, Divide nb, void* __restrict__ dg,
                                                                  void* __restrict__ du) {
+  grid_begin();
   using T = typename DType<DT>::T;
   Place8 p;
   if (!place8<VEC>(p, blocks, K, nb)) return;
@@ -329,19 +333,13 @@ static bool rows16(const void* p, int64_t ld, int64_t K, int dt) {
 
 static uint32_t a8_row_blocks(int64_t K) { return (uint32_t)((K + kA8Block - 1) / kA8Block); }
 
-#define RQ_A8_LAUNCH(kern, vec, ...)                                                              \
-  do {                                                                                            \
-    const unsigned grid = (blocks + kA8PerCta - 1) / kA8PerCta;                                   \
-    if (vec) {                                                                                    \
-      if (dt == RQ_F32) kern<RQ_F32, true><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);             \
-      else if (dt == RQ_BF16) kern<RQ_BF16, true><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);      \
-      else kern<RQ_F16, true><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);                          \
-    } else {                                                                                      \
-      if (dt == RQ_F32) kern<RQ_F32, false><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);            \
-      else if (dt == RQ_BF16) kern<RQ_BF16, false><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);     \
-      else kern<RQ_F16, false><<<grid, kA8Threads, 0, st>>>(__VA_ARGS__);                         \
-    }                                                                                             \
-    return check_launch();                                                                        \
+#define RQ_A8_LAUNCH(kern, vec, ...)                                                                         \
+  do {                                                                                                       \
+    const unsigned grid = (blocks + kA8PerCta - 1) / kA8PerCta;                                              \
+    auto* k = dt == RQ_F32 ? ((vec) ? kern<RQ_F32, true> : kern<RQ_F32, false>)                              \
+              : dt == RQ_BF16 ? ((vec) ? kern<RQ_BF16, true> : kern<RQ_BF16, false>)                         \
+                              : ((vec) ? kern<RQ_F16, true> : kern<RQ_F16, false>);                          \
+    return launch_dependent(k, grid, kA8Threads, st, __VA_ARGS__);                                           \
   } while (0)
 
 int act8_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, int8_t* codes, float* scales, cudaStream_t st) {
@@ -357,10 +355,11 @@ int act8_unpack(const int8_t* codes, const float* scales, int64_t M, int64_t K, 
 }
 
 template <int DT, bool VEC>
-static void launch_swiglu8(const void* g, int64_t ldg, const void* u, int64_t ldu, uint32_t blocks, int K,
+static int launch_swiglu8(const void* g, int64_t ldg, const void* u, int64_t ldu, uint32_t blocks, int K,
                            const Divide& nb, void* h, int8_t* codes, float* scales, int copies, cudaStream_t st) {
   auto* kern = copies == 3 ? swiglu8_forward_k<DT, VEC, 3> : swiglu8_forward_k<DT, VEC, 2>;
-  kern<<<(blocks + kA8PerCta - 1) / kA8PerCta, kA8Threads, 0, st>>>(g, ldg, u, ldu, blocks, K, nb, h, codes, scales);
+  return launch_dependent(kern, (blocks + kA8PerCta - 1) / kA8PerCta, kA8Threads, st, g, ldg, u, ldu, blocks, K, nb, h,
+                          codes, scales);
 }
 
 int swiglu8_forward(const void* g, int64_t ldg, const void* u, int64_t ldu, int dt, int64_t M, int64_t K, void* h,
@@ -371,8 +370,7 @@ int swiglu8_forward(const void* g, int64_t ldg, const void* u, int64_t ldu, int 
   auto* launch = dt == RQ_F32 ? (vec ? launch_swiglu8<RQ_F32, true> : launch_swiglu8<RQ_F32, false>)
                  : dt == RQ_BF16 ? (vec ? launch_swiglu8<RQ_BF16, true> : launch_swiglu8<RQ_BF16, false>)
                                  : (vec ? launch_swiglu8<RQ_F16, true> : launch_swiglu8<RQ_F16, false>);
-  launch(g, ldg, u, ldu, blocks, (int)K, nb, h, codes, scales, copies, st);
-  return check_launch();
+  return launch(g, ldg, u, ldu, blocks, (int)K, nb, h, codes, scales, copies, st);
 }
 
 int swiglu8_backward(const void* dh, int64_t ldh, int dt, int64_t M, int64_t K, const int8_t* codes,

@@ -312,17 +312,19 @@ struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at 
   int threads;
   size_t smem;
 
-  cudaLaunchConfig_t config(dim3 grid, int csize, cudaLaunchAttribute* at, cudaStream_t st) const {
+  cudaLaunchConfig_t config(dim3 grid, int csize, cudaLaunchAttribute (&at)[2], cudaStream_t st) const {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    at->id = cudaLaunchAttributeClusterDimension;
-    at->val.clusterDim.x = csize;
-    at->val.clusterDim.y = at->val.clusterDim.z = 1;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = csize;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernels begin with grid_begin()
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cfg;
   }
 
@@ -348,8 +350,9 @@ struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at 
       if (known[i].k == (const void*)kern && known[i].dev == dev && known[i].smem == smem) return known[i].n;
     e = Entry{(const void*)kern, dev, smem, {}};
     for (int c = 1; c <= 8; ++c) {
-      cudaLaunchAttribute at;
-      const cudaLaunchConfig_t cfg = config(dim3(c), c, &at, nullptr);
+      cudaLaunchAttribute at[2];
+      cudaLaunchConfig_t cfg = config(dim3(c), c, at, nullptr);
+      cfg.numAttrs = 1;
       if (cudaOccupancyMaxActiveClusters(&e.n[c], kern, &cfg) != cudaSuccess || e.n[c] < 1) {
         cudaGetLastError();
         e.n[c] = std::max(1, num_sms() / c);
@@ -362,8 +365,8 @@ struct ClusterLaunch {  // a kernel of one argument, its cluster size chosen at 
   int prepare() const { return ensure_smem_limit((const void*)kern, smem); }
 
   int launch(const P& args, dim3 grid, int csize, cudaStream_t st) const {
-    cudaLaunchAttribute at;
-    const cudaLaunchConfig_t cfg = config(grid, csize, &at, st);
+    cudaLaunchAttribute at[2];
+    const cudaLaunchConfig_t cfg = config(grid, csize, at, st);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);
     if (e != cudaSuccess) {
       set_cuda_error(e);
@@ -440,6 +443,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   cg::cluster_group cluster = cg::this_cluster();
   const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  grid_begin();
 
   // ---- the tile
   const int tile_id = (int)(blockIdx.x / csize);
@@ -912,6 +916,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   const int block = (int)(blockIdx.x / csize), adapter = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, mw = warp / RG;
+  grid_begin();
 
   const int first = a.plan ? max(a.plan[1 + adapter], 0) : 0;
   const int last = a.plan ? min(a.plan[2 + adapter], (int)a.M) : (int)a.M;

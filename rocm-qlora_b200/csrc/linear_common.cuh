@@ -9,6 +9,16 @@ namespace rq {
 
 constexpr int kDQBlock2 = 256;  // second-level block of QuantLinear.enable_double_quant
 
+// First statement of a kernel that is launched as the programmatic dependent
+// of the one before it: it reads and writes nothing before every grid before
+// it has finished, and lets its own dependent come up only then, so that a
+// dependent that reads ahead of its own wait (the decode GEMV its weights)
+// sees all that was written before this kernel.
+__device__ __forceinline__ void grid_begin() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ float load_scalar(const void* p, int dt, int64_t i) {
   switch (dt) {
     case RQ_BF16: return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);

@@ -144,6 +144,7 @@ struct ExpSum {
 template <int DT, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, float4* __restrict__ stats,
                                                              float* __restrict__ logps) {
+  grid_begin();
   using T = typename DType<DT>::T;
   constexpr int E = RowCut<DT>::E;
   const int64_t at = blockIdx.x;
@@ -151,7 +152,6 @@ __global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, floa
   __shared__ float ks[TH / 32];
   __shared__ double sums[TH / 32];
   int64_t y;
-  asm volatile("griddepcontrol.launch_dependents;");  // the loss kernel may come up; it waits for this grid
   const bool counts = row_label(t, at, &y);
   if (logps && tid == 0) {
     if (at % t.L == 0) logps[at] = 0.0f;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kPrefWarps * 32) __cluster_dims__(kPrefCtas, 1
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ SequenceSum part[kPrefWarps];
   __shared__ double total[kPrefWarps];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' sums
+  grid_begin();
   const int P = (int)(t.B / 2);
   int ws = kPrefWarps / 2;  // warps of a sequence: fewer where that leaves lanes without a row
   while (ws > 1 && ws * 32 >= 2 * t.L) ws /= 2;
@@ -317,6 +317,7 @@ template <int DT>
 __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const float4* __restrict__ stats,
                                                             const float* __restrict__ slopes, int per_token,
                                                             const float* __restrict__ upstream, void* __restrict__ out) {
+  grid_begin();
   using T = typename DType<DT>::T;
   constexpr int E = RowCut<DT>::E;
   const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x;
@@ -379,47 +380,28 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
 }
 
 template <int DT>
-static void launch_stats(const TokenRows& t, float4* stats, float* logps, cudaStream_t st) {
+static int launch_stats(const TokenRows& t, float4* stats, float* logps, cudaStream_t st) {
   const unsigned grid = (unsigned)(t.B * t.L);
-  if (grid >= 8u * num_sms()) token_stats_k<DT, 128><<<grid, 128, 0, st>>>(t, stats, logps);
-  else token_stats_k<DT, kTokThreads><<<grid, kTokThreads, 0, st>>>(t, stats, logps);
+  if (grid >= 8u * num_sms()) return launch_dependent(token_stats_k<DT, 128>, grid, 128, st, t, stats, logps);
+  return launch_dependent(token_stats_k<DT, kTokThreads>, grid, kTokThreads, st, t, stats, logps);
 }
 
 int token_logprobs(const TokenRows& t, float* stats, float* logps, cudaStream_t st) {
-  if (t.dt == RQ_F32) launch_stats<RQ_F32>(t, (float4*)stats, logps, st);
-  else if (t.dt == RQ_BF16) launch_stats<RQ_BF16>(t, (float4*)stats, logps, st);
-  else launch_stats<RQ_F16>(t, (float4*)stats, logps, st);
-  return check_launch();
+  auto* launch = t.dt == RQ_F32 ? launch_stats<RQ_F32> : t.dt == RQ_BF16 ? launch_stats<RQ_BF16> : launch_stats<RQ_F16>;
+  return launch(t, (float4*)stats, logps, st);
 }
 
 int preference_loss(const TokenRows& t, const float* stats, const float* ref, int form, float beta, float smooth,
                     float* loss, float* logps, float* rewards, float* slopes, cudaStream_t st) {
-  // the programmatic dependent of the kernel before it: it comes up while that
-  // one's last rows run, and waits for all of it before its first load
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kPrefCtas);
-  cfg.blockDim = dim3(kPrefWarps * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, preference_loss_k, t, (const float4*)stats, ref, form, beta, smooth,
-                                           loss, logps, rewards, slopes);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return RQ_ERR_CUDA;
-  }
-  return check_launch();
+  return launch_dependent(preference_loss_k, kPrefCtas, kPrefWarps * 32, st, t, (const float4*)stats, ref, form, beta,
+                          smooth, loss, logps, rewards, slopes);
 }
 
 int token_logprobs_grad(const TokenRows& t, const float* stats, const float* slopes, int per_token,
                         const float* upstream, void* dlogits, cudaStream_t st) {
-  const unsigned grid = (unsigned)(t.B * t.L);
   auto* kern = t.dt == RQ_F32 ? token_grad_k<RQ_F32> : t.dt == RQ_BF16 ? token_grad_k<RQ_BF16> : token_grad_k<RQ_F16>;
-  kern<<<grid, kTokThreads, 0, st>>>(t, (const float4*)stats, slopes, per_token, upstream, dlogits);
-  return check_launch();
+  return launch_dependent(kern, (unsigned)(t.B * t.L), kTokThreads, st, t, (const float4*)stats, slopes, per_token,
+                          upstream, dlogits);
 }
 
 }  // namespace rq
