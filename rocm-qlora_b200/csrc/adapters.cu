@@ -834,9 +834,9 @@ int adapters_apply(const AdapterRows& a0, const void* in, int64_t ldin, const vo
 
 // ------------------------------------------------------------------- grad
 
-constexpr int kGrThreads = 256, kGrWarps = kGrThreads / 32;
+constexpr int kGrWarps = 8;                                  // of a CTA whose groups split the rows
 constexpr int kGrCols = 128;                                 // columns of a CTA: one block of 8-bit codes
-constexpr int kGrSums = kGrWarps * kGrCols * 16 * 4;         // every warp's 128 x 16 sums
+constexpr int kGrSums = kGrCols * 16 * 4;                    // a warp's 128 x 16 sums
 // One step in a ring: 16 rows of z (swizzled 16-byte pieces) and of mid (16
 // ranks a warp, padded so that fragment loads use distinct banks), and the
 // scales of codes.  RG warps, 16 ranks each, share a ring and its rows.
@@ -858,7 +858,40 @@ struct GradArgs {
   int64_t lds;
   const float* mid;
   void* G;
+  int beside;  // the adapters of more than `most` rows are summed by the launch before
+  int most;
 };
+
+// Rows of an adapter: places [first, last) of the plan's order, or the batch.
+__device__ __forceinline__ int2 grad_rows(const AdapterRows& a, int adapter) {
+  if (!a.plan) return make_int2(0, (int)a.M);
+  const int first = max(a.plan[1 + adapter], 0);
+  return make_int2(first, max(first, min(a.plan[2 + adapter], (int)a.M)));
+}
+
+// The nth adapter of more than `most` rows; -1: there are not so many.
+template <int THREADS>
+__device__ int nth_large(const GradArgs& p, int nth) {
+  __shared__ uint32_t votes[THREADS / 32];
+  for (int i0 = 0; i0 < p.a.count; i0 += THREADS) {
+    const int i = i0 + (int)threadIdx.x;
+    const int2 rows = i < p.a.count ? grad_rows(p.a, i) : make_int2(0, 0);
+    const uint32_t vote = __ballot_sync(0xffffffffu, rows.y - rows.x > p.most);
+    if (threadIdx.x % 32 == 0) votes[threadIdx.x / 32] = vote;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w) {
+      uint32_t v = votes[w];
+      const int n = __popc(v);
+      if (nth < n) {
+        for (; nth > 0; --nth) v &= v - 1;
+        return i0 + 32 * w + __ffs(v) - 1;
+      }
+      nth -= n;
+    }
+    __syncthreads();  // all have read the votes
+  }
+  return -1;
+}
 
 // Two codes in the low bytes of a word's halves as 16-bit values, exact.  bf16:
 // 0x4300 with the code's lower 7 bits is 128 + (q mod 128), and with its sign
@@ -881,8 +914,8 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 // G_a[d, j] = sum over the rows m of a of z[m, d] mid[m, j].
 //
 // One CTA sums 128 columns of one adapter.  RG warps hold 16 ranks each; the
-// 8 / RG groups of them split the rows, and the CTAs of a cluster split them
-// again.  Sums meet in shared and distributed shared memory in group and rank
+// MW groups of them (8 / RG, or 1) split the rows, and the CTAs of a cluster
+// split them again.  Sums meet in shared and distributed shared memory in group and rank
 // order, so equal inputs give equal bits, without atomics or a workspace.
 //
 // The reduction runs over rows, so the MMA's k index is the row and ldmatrix
@@ -896,11 +929,11 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 // meetings) is what is seen: 64 MB of z at rank 16 take 21 us, 32 MB of codes
 // 20; rank 64 49 and 54 us, where four warps a group share the rows and the
 // two halves of mid are mma.sync's work.
-template <int DT, bool CODES, bool VEC, int RG>
-__global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_constant__ GradArgs p) {
+template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
+__device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
   using T = typename DType<DT>::T;
   constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
-  constexpr int S = gr_steps(CODES, VEC, RG), MW = kGrWarps / RG, R16 = RG * 16;
+  constexpr int S = gr_steps(CODES, VEC, RG), R16 = RG * 16, THREADS = 32 * RG * MW;
   constexpr bool CONV = CODES && RG > 1;        // codes become 16-bit once for all warps of a group
   // m-tiles at a time: two put four sums between two products of one sum; with
   // one warp a ring the registers for that are not there (22 against 25 us at
@@ -913,18 +946,23 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   const AdapterRows& a = p.a;
   cg::cluster_group cluster = cg::this_cluster();
   const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
-  const int block = (int)(blockIdx.x / csize), adapter = blockIdx.y;
+  const int block = (int)(blockIdx.x / csize);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, mw = warp / RG;
-  grid_begin();
 
-  const int first = a.plan ? max(a.plan[1 + adapter], 0) : 0;
-  const int last = a.plan ? min(a.plan[2 + adapter], (int)a.M) : (int)a.M;
+  int adapter = blockIdx.y;
+  if constexpr (LARGE) {
+    adapter = nth_large<THREADS>(p, adapter);
+    if (adapter < 0) return;
+  }
+  const int2 places = grad_rows(a, adapter);
+  const int first = places.x, last = places.y;
+  if (MW == 1 && p.beside && last - first > p.most) return;
   const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
   if (first >= last) {  // the whole cluster: no rows, zero gradient
     const int64_t d0 = (int64_t)block * kGrCols, n = min((int64_t)kGrCols, a.D1 - d0) * a.r / 8;
     uint4* G = reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d0) * a.r);
-    for (int64_t i = crank * kGrThreads + tid; i < n; i += csize * kGrThreads) G[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t i = crank * THREADS + tid; i < n; i += csize * THREADS) G[i] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
   const int64_t c0 = (int64_t)block * kGrCols;
@@ -983,6 +1021,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   };
   auto meet = [&] {  // the group's warps
     if constexpr (RG == 1) __syncwarp();
+    else if constexpr (MW == 1) __syncthreads();  // a barrier by number counts as all 16: 4 CTAs an SM
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + mw), "n"(32 * RG) : "memory");
   };
   for (int s = 0; s < S - 1; ++s) fetch(s);
@@ -1083,12 +1122,29 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
     if constexpr (RG == 1) meet();  // all lanes have read the step before its place is fetched into
   }
   cp_async_wait<0>();
-  __syncthreads();  // the sums lie over the ring
 
-  // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3; groups
-  // without a row have nothing to add
-  const int active = min(MW, max(1, (last - first - crank * MW * 16 + 15) / 16));
+  // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3
   const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
+  // codes read as pairs: m-tile i has the even (odd) columns of pieces i and i + 1, i even (odd)
+  auto column = [&](int at) { return c0 + (CODES && !CONV ? (at & ~31) + 2 * (at & 15) + ((at >> 4) & 1) : at); };
+  auto write = [&](int64_t d, int j, float4 s) {
+    if (d < a.D1 && j < a.r)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
+          make_uint2(pair16<DT>(s.x, s.y), pair16<DT>(s.z, s.w));
+  };
+  if (MW == 1 && csize == 1) {  // nobody to meet
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        write(column(16 * i + g + 8 * h), rg * 16 + 4 * t,
+              make_float4(acc[i][0][2 * h] * back, acc[i][1][2 * h] * back, acc[i][0][2 * h + 1] * back,
+                          acc[i][1][2 * h + 1] * back));
+    return;
+  }
+  __syncthreads();  // the sums lie over the ring
+  // groups without a row have nothing to add
+  const int active = min(MW, max(1, (last - first - crank * MW * 16 + 15) / 16));
   float* mine = sums + mw * kGrCols * R16 + rg * 16 + 4 * t;
   if (mw < active) {
 #pragma unroll
@@ -1100,7 +1156,7 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
                         acc[i][1][2 * h + 1] * back);
   }
   __syncthreads();
-  for (int i = tid; active > 1 && i < kGrCols * R16 / 4; i += kGrThreads) {
+  for (int i = tid; active > 1 && i < kGrCols * R16 / 4; i += THREADS) {
     float4 s = reinterpret_cast<const float4*>(sums)[i];
     for (int w = 1; w < active; ++w) {
       const float4 q = reinterpret_cast<const float4*>(sums + w * kGrCols * R16)[i];
@@ -1111,38 +1167,86 @@ __global__ void __launch_bounds__(kGrThreads, 2) adapters_grad_k(const __grid_co
   cluster.sync();
   // 4 ranks of a column at a time, dealt to the cluster's CTAs
   const int units = R16 / 4;
-  for (int i = tid * csize + crank; i < kGrCols * units; i += csize * kGrThreads) {
+  for (int i = tid * csize + crank; i < kGrCols * units; i += csize * THREADS) {
     const int at = i / units, j = (i - at * units) * 4;
-    // codes read as pairs: m-tile i has the even (odd) columns of pieces i and i + 1, i even (odd)
-    const int64_t d = c0 + (CODES && !CONV ? (at & ~31) + 2 * (at & 15) + ((at >> 4) & 1) : at);
-    if (d >= a.D1 || j >= a.r) continue;
-    const float4 s = cluster_sum<float4>(cluster, sums + at * R16 + j, csize);
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d) * a.r + j) =
-        make_uint2(pair16<DT>(s.x, s.y), pair16<DT>(s.z, s.w));
+    if (column(at) >= a.D1 || j >= a.r) continue;
+    write(column(at), j, cluster_sum<float4>(cluster, sums + at * R16 + j, csize));
   }
   cluster.sync();  // the others have read this CTA's sums
 }
 
+// The two launches of a call with LARGE ones run beside one another: the first
+// lets its dependent start once everything before it is complete, and the
+// second, which reads and writes nothing of the first's, waits for it only at
+// its end, so that whatever follows finds both complete.
+template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
+__global__ void __launch_bounds__(32 * RG * MW, 16 / (RG * MW)) adapters_grad_k(const __grid_constant__ GradArgs p) {
+  if (MW > 1 || !p.beside) grid_begin();
+  adapter_gradient<DT, CODES, VEC, RG, MW, LARGE>(p);
+  if (MW == 1 && p.beside) grid_begin();
+}
+
+template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE = false>
+static ClusterLaunch<GradArgs> grad_kernel() {
+  const size_t wide = CODES && RG > 1 ? 16 * 2 * kGrCols : 0;  // the 16-bit copy of a step
+  const size_t ring = (size_t)MW * (gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG) + wide);
+  return {adapters_grad_k<DT, CODES, VEC, RG, MW, LARGE>, 32 * RG * MW, std::max(ring, (size_t)RG * MW * kGrSums)};
+}
+
+// A CTA costs about as much as 5 steps besides its steps (its sums through
+// shared memory, the cluster's meetings): the cluster size that takes the
+// fewest steps over all rounds of the GPU for `count` adapters of `each` rows,
+// of which a CTA takes per_step a step.  That number of steps is left in best.
+static int grad_cluster(const int* resident, int64_t blocks, int64_t count, int64_t each, int64_t per_step,
+                        int64_t* best) {
+  int csize = 1;
+  *best = INT64_MAX;
+  for (int c = 1; c <= 8; ++c) {
+    const int64_t rounds = (blocks * count + resident[c] - 1) / resident[c];
+    const int64_t steps = (each + per_step * c - 1) / (per_step * c);
+    if (rounds * (5 + steps) < *best) *best = rounds * (5 + steps), csize = c;
+  }
+  return csize;
+}
+
+// For many adapters of few rows most groups of a CTA of 8 warps have none: they
+// take CTAs of one group, of which up to 16 share an SM: 64 rows of 32 adapters,
+// 11008 columns, rank 16, 10 us against 38; 8192 rows of 64, 4096
+// columns, rank 16 27 against 52, rank 64 47 against 82.  The host does not
+// know how the rows are spread, and an adapter of most of them would keep its
+// one group for long (all 8192 rows, rank 16: 457 us): those of more than 4
+// times the mean and 64 rows, no more than M / most of them, go to CTAs of 8
+// warps in a launch beside (74 us; 69 where all adapters have such CTAs).
 template <int DT, bool CODES, bool VEC, int RG>
 static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
-  const size_t wide = CODES && RG > 1 ? 16 * 2 * kGrCols : 0;  // the 16-bit copy of a step
-  const size_t ring = (size_t)(kGrWarps / RG) * (gr_steps(CODES, VEC, RG) * gr_step_bytes(CODES, RG) + wide);
-  const ClusterLaunch<GradArgs> l{adapters_grad_k<DT, CODES, VEC, RG>, kGrThreads, std::max(ring, (size_t)kGrSums)};
-  const int rc = l.prepare();
+  const int64_t M = p.a.M, count = p.a.count, each = (M + count - 1) / count;
+  const auto many = grad_kernel<DT, CODES, VEC, RG, kGrWarps / RG>();
+  int rc = many.prepare();
   if (rc != RQ_OK) return rc;
-  // A CTA costs about as much as 5 steps besides its steps (its sums through
-  // shared memory, the cluster's meetings); the cluster size that takes the
-  // fewest steps over all rounds of the GPU, for adapters of mean size.
-  const int* resident = l.resident();
-  const int64_t per_step = kGrWarps / RG * 16, each = (p.a.M + p.a.count - 1) / p.a.count;
-  int csize = 1;
-  int64_t best = INT64_MAX;
-  for (int c = 1; c <= 8; ++c) {
-    const int64_t rounds = (blocks * p.a.count + resident[c] - 1) / resident[c];
-    const int64_t steps = (each + per_step * c - 1) / (per_step * c);
-    if (rounds * (5 + steps) < best) best = rounds * (5 + steps), csize = c;
+  int64_t steps;
+  int csize = grad_cluster(many.resident(), blocks, count, each, kGrWarps / RG * 16, &steps);
+  if constexpr (RG < kGrWarps) {
+    const auto one = grad_kernel<DT, CODES, VEC, RG, 1>();
+    if ((rc = one.prepare()) != RQ_OK) return rc;
+    GradArgs q = p;
+    q.most = (int)std::min<int64_t>(std::max<int64_t>(64, 4 * each), INT32_MAX - 1);
+    const int64_t large = std::min(count, M / (q.most + 1));  // no more adapters than that have so many rows
+    int64_t one_steps, rest = 0;
+    const int one_csize = grad_cluster(one.resident(), blocks, count, each, 16, &one_steps);
+    if (large) rest = 3 + (blocks * large + many.resident()[1] - 1) / many.resident()[1];  // a launch, CTAs that find none
+    if (one_steps + rest < steps) {
+      if (large) {
+        const auto first = grad_kernel<DT, CODES, VEC, RG, kGrWarps / RG, true>();
+        if ((rc = first.prepare()) != RQ_OK) return rc;
+        csize = grad_cluster(first.resident(), blocks, large, M / large, kGrWarps / RG * 16, &steps);
+        rc = first.launch(q, dim3((unsigned)(blocks * csize), (unsigned)large), csize, st);
+        if (rc != RQ_OK) return rc;
+        q.beside = 1;
+      }
+      return one.launch(q, dim3((unsigned)(blocks * one_csize), (unsigned)count), one_csize, st);
+    }
   }
-  return l.launch(p, dim3((unsigned)(blocks * csize), (unsigned)p.a.count), csize, st);
+  return many.launch(p, dim3((unsigned)(blocks * csize), (unsigned)count), csize, st);
 }
 
 template <int DT, bool CODES, bool VEC>
@@ -1162,7 +1266,7 @@ static int launch_grad_dt(const GradArgs& p, int64_t blocks, cudaStream_t st) {
 
 int adapters_grad(const AdapterRows& a, const void* z, int64_t ldz, const float* zscale, int64_t lds, const float* mid,
                   void* G, cudaStream_t st) {
-  const GradArgs p{a, z, ldz, zscale, lds, mid, G};
+  const GradArgs p{a, z, ldz, zscale, lds, mid, G, 0, 0};
   const int64_t blocks = (a.D1 + kGrCols - 1) / kGrCols;
   return a.dt == RQ_BF16 ? launch_grad_dt<RQ_BF16>(p, blocks, st) : launch_grad_dt<RQ_F16>(p, blocks, st);
 }

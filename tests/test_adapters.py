@@ -99,6 +99,34 @@ def test_long_rows_of_large_layers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("spread", ["even", "half", "one", "two"])
+@pytest.mark.parametrize("rows,k,n,rank,count,dtype", [
+    (90, 2048, 4099, 16, 40, torch.bfloat16), (1500, 2048, 1027, 16, 40, torch.bfloat16),
+    (1500, 2048, 1032, 32, 40, torch.float16), (1200, 2056, 1027, 64, 70, torch.bfloat16),
+    (2500, 512, 264, 16, 300, torch.float16)])
+def test_many_adapters(rows, k, n, rank, count, dtype, spread):
+    """Banks of many adapters, their rows spread evenly or most of them on one or two."""
+    from rocm_qlora.activation8 import pack_activation
+    t = make(rows, k, n, rank, count, dtype, seed=rows)
+    g = torch.Generator().manual_seed(1)
+    some = torch.rand(rows, generator=g).to(t["ids"].device)
+    if spread == "half":
+        t["ids"][some < 0.5] = count - 1
+    elif spread == "one":
+        t["ids"][:] = count // 2
+    elif spread == "two":
+        t["ids"][:] = torch.where(some < 0.6, 0, count - 2)
+    packed = pack_activation(t["x"])
+    y, grads = run(t)
+    for got, w, name in zip((y, *grads[1:]), formula(t), ("y", "dx", "dA", "dB")):
+        check(got, w, f"{name} {spread}")
+    again = run(t)[1]
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    codes = packed.codes[:, :k].to(F8) * packed.scales.to(F8).repeat_interleave(128, 1)[:, :k]
+    check(run(t, packed_x=packed)[1][2], formula(t, z=codes)[2], f"dA of codes {spread}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [7, 200])
 def test_rows_without_an_adapter(rows):
     t = make(rows, 264, 136, 16, 3, torch.bfloat16, none=1.1)
