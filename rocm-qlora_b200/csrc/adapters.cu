@@ -145,7 +145,7 @@ constexpr int kApThreads = 256, kApWarps = kApThreads / 32;
 constexpr int kApWin = 32;  // columns of a window: one 16-byte load of each lane of a quad
 
 // Bytes between rows of the staged U (conflict-free ldmatrix) and of the
-// intermediate's halves (a quarter warp's loads on distinct banks).
+// intermediate's pieces (a quarter warp's loads on distinct banks).
 __host__ __device__ constexpr int ap_pitch_u(int R) { return R * 2 + 16; }
 __host__ __device__ constexpr int ap_pitch_m(int R) { return R <= 32 ? R * 2 : R * 2 + 64; }
 
@@ -271,13 +271,24 @@ __device__ __forceinline__ float2 unpair16(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// Two values as the sum of two 16-bit halves each.  An infinity keeps a zero
-// remainder, so that it stays an infinity; NaN is in the first half.
+// Two values as sums of 16-bit pieces: three for bf16, the upper halves of the
+// value and of what is left twice, which are its 24 bits; two for fp16, rounded,
+// which are 22 bits.  An infinity keeps zero remainders, so that it stays an
+// infinity; NaN is in one of the first two pieces.
+template <int DT> constexpr int kPieces = DT == RQ_BF16 ? 3 : 2;
 template <int DT>
-__device__ __forceinline__ void split16x2(float x, float y, uint32_t* hi, uint32_t* lo) {
-  *hi = pair16<DT>(x, y);
-  const float2 h = unpair16<DT>(*hi);
-  *lo = pair16<DT>(fabsf(x) < INFINITY ? x - h.x : 0.0f, fabsf(y) < INFINITY ? y - h.y : 0.0f);
+__device__ __forceinline__ void split16(float x, float y, uint32_t (&p)[kPieces<DT>]) {
+  if constexpr (DT == RQ_BF16) {
+    auto upper = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+    p[0] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    x = fabsf(x) == INFINITY ? 0.0f : x - upper(x), y = fabsf(y) == INFINITY ? 0.0f : y - upper(y);
+    p[1] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    p[2] = __byte_perm(__float_as_uint(x - upper(x)), __float_as_uint(y - upper(y)), 0x7632);
+  } else {
+    p[0] = pair16<DT>(x, y);
+    const float2 h = unpair16<DT>(p[0]);
+    p[1] = pair16<DT>(fabsf(x) < INFINITY ? x - h.x : 0.0f, fabsf(y) < INFINITY ? y - h.y : 0.0f);
+  }
 }
 
 template <int N>
@@ -406,10 +417,11 @@ __device__ __noinline__ void rows_without(const ApplyArgs& p, const int* order, 
 //
 // Mathematics.  mid = s (in U) and out = base + mid V^T, both on tensor cores
 // (mma m16n8k16, fp32 accumulation).  U and V enter as they are; mid is fp32
-// and is multiplied as the sum of two 16-bit halves, so it keeps 16 bits.
-// For fp16, whose exponent range a small gradient would leave, each row of
-// mid is first brought near 2^14 by a power of two that the output row takes
-// back.
+// and is multiplied as the sum of 16-bit pieces, so that it keeps its 24 bits
+// (bf16, three pieces; with two, 16 bits, one result in a thousand rounds the
+// other way) or 22 (fp16, two pieces).  For fp16, whose exponent range a small
+// gradient would leave, each row of mid is first brought near 2^14 by a power
+// of two that the output row takes back.
 //
 // What bounds it: in and base are read and out written once (HBM), while U
 // and V are shared by the tile's rows (L2).  The sum over all input columns
@@ -430,13 +442,14 @@ __device__ __noinline__ void rows_without(const ApplyArgs& p, const int* order, 
 // Measured (bf16): one row of 4096 to 4096, rank 16, 5.9 us (a launch and a
 // chain of five dependent loads); 8192 rows, 45 us, 4.4 TB/s of the 201 MB
 // (31 us at the copy bandwidth; launch, plan, meeting and sums are the rest);
-// rank 64, 67 us, with the tensor pipe a third active: the two halves of mid
-// on mma.sync.  fp16 rows of 1093 to 1088, rank 64, 1111 of them: 14 us.
+// rank 64, 76 us: the three pieces of mid on mma.sync.  fp16 rows of 1093 to
+// 1088, rank 64, 1111 of them: 14 us.
 template <int DT, int R, int NW, bool VEC>
 __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(const __grid_constant__ ApplyArgs p) {
   constexpr int NT = R / 8;               // n-tiles of the first product
   constexpr int KS = R / 16;              // k-steps of the second
   constexpr int PU = ap_pitch_u(R), PM = ap_pitch_m(R), S = ap_steps(R, NW);
+  constexpr int P = kPieces<DT>;
   constexpr int CW = R <= 32 ? 2 : 1, AHEAD = 2;  // second product: 32-column chunks of a warp, m-tiles under way
   extern __shared__ __align__(16) unsigned char smem[];
   const AdapterRows& a = p.a;
@@ -471,7 +484,7 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   ApplyRows& at = *reinterpret_cast<ApplyRows*>(smem);
   unsigned char* ring = smem + sizeof(ApplyRows);
   float* part = reinterpret_cast<float*>(ring);  // [128][R], over the ring
-  unsigned char* mids = ring + 128 * R * 4;      // halves of mid: [2][tile][PM], over the ring
+  unsigned char* mids = ring + 128 * R * 4;      // pieces of mid: [P][tile][PM], over the ring
   const uint16_t* in = static_cast<const uint16_t*>(p.in);
   const uint16_t* base = static_cast<const uint16_t*>(p.base);
   const int chunks2 = (int)((a.D2 + 31) / 32), per2 = (chunks2 + csize - 1) / csize;
@@ -678,14 +691,19 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       }
     }
     if (on) {
-      __align__(16) uint32_t hi[E / 2], lo[E / 2];
+      __align__(16) uint32_t w[P][E / 2];
 #pragma unroll
-      for (int e = 0; e < E; e += 2) split16x2<DT>(v[e] * mul, v[e + 1] * mul, &hi[e / 2], &lo[e / 2]);
+      for (int e = 0; e < E; e += 2) {
+        uint32_t q[P];
+        split16<DT>(v[e] * mul, v[e + 1] * mul, q);
+#pragma unroll
+        for (int k = 0; k < P; ++k) w[k][e / 2] = q[k];
+      }
       unsigned char* to = mids + row * PM + l * E * 2;
       for (int c = 0; c < csize; ++c) {
         unsigned char* m = cluster.map_shared_rank(to, c);
-        store_words<E / 2>(m, hi);
-        store_words<E / 2>(m + a.tile * PM, lo);
+#pragma unroll
+        for (int k = 0; k < P; ++k) store_words<E / 2>(m + k * a.tile * PM, w[k]);
         if (DT == RQ_F16 && l == 0) cluster.map_shared_rank(at.mul, c)[row] = back;
       }
     }
@@ -719,8 +737,8 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     }
     fetch(old);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const unsigned char* ma = mids + (half * a.tile + ra) * PM;
+    for (int piece = 0; piece < P; ++piece) {
+      const unsigned char* ma = mids + (piece * a.tile + ra) * PM;
       const unsigned char* mb = ma + 8 * PM;
       if constexpr (R == 16) {
         const uint2 qa = *reinterpret_cast<const uint2*>(ma + 8 * t), qb = *reinterpret_cast<const uint2*>(mb + 8 * t);
@@ -787,7 +805,7 @@ template <int DT, int R, int NW>
 static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_t st) {
   const int columns = NW * (kApWarps / (p.a.tile / 16)) * kApWin;  // of a step
   const size_t ring = (size_t)ap_steps(R, NW) * (columns * ap_pitch_u(R) + ap_x_bytes(NW, !p.vec_in));
-  const size_t after = (size_t)128 * R * 4 + (size_t)2 * p.a.tile * ap_pitch_m(R);
+  const size_t after = (size_t)128 * R * 4 + (size_t)kPieces<DT> * p.a.tile * ap_pitch_m(R);
   const size_t smem = sizeof(ApplyRows) + std::max(ring, after);
   const ClusterLaunch<ApplyArgs> l{vec ? adapters_apply_k<DT, R, NW, true> : adapters_apply_k<DT, R, NW, false>,
                                    kApThreads, smem};
@@ -923,12 +941,12 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 // 16-row steps by cp.async into its own ring, a thread one row a step, and
 // only the group waits for them.  z is read once.  Codes become 16-bit values
 // exactly; their scale multiplies the other operand, mid, in fp32, which then
-// enters as two 16-bit halves as in the row products.
+// enters as 16-bit pieces as in the row products.
 //
 // Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
-// meetings) is what is seen: 64 MB of z at rank 16 take 21 us, 32 MB of codes
-// 20; rank 64 49 and 54 us, where four warps a group share the rows and the
-// two halves of mid are mma.sync's work.
+// meetings) is what is seen: 64 MB of z at rank 16 take 22 us, 32 MB of codes
+// 22; rank 64 59 and 66 us, where four warps a group share the rows and the
+// three pieces of mid are mma.sync's work.
 template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
 __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
   using T = typename DType<DT>::T;
@@ -1088,11 +1106,15 @@ __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i].x *= mul, v[i].y *= mul;
     }
-    uint32_t b[2][2][2];  // [half][n-tile][k pair]
+    constexpr int P = kPieces<DT>;
+    uint32_t b[P][2][2];  // [piece][n-tile][k pair]
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      split16x2<DT>(v[2 * k].x, v[2 * k + 1].x, &b[0][0][k], &b[1][0][k]);
-      split16x2<DT>(v[2 * k].y, v[2 * k + 1].y, &b[0][1][k], &b[1][1][k]);
+      uint32_t q[2][P];
+      split16<DT>(v[2 * k].x, v[2 * k + 1].x, q[0]);
+      split16<DT>(v[2 * k].y, v[2 * k + 1].y, q[1]);
+#pragma unroll
+      for (int e = 0; e < P; ++e) b[e][0][k] = q[0][e], b[e][1][k] = q[1][e];
     }
     // A fragments: 8 x 8 pieces (rows 0-7 | 8-15) x (a piece | the next), transposed
     const int lrow = (lane & 7) + 8 * (lane >> 4), lpiece = (lane >> 3) & 1;
@@ -1112,12 +1134,12 @@ __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
         for (int k = 0; k < PAIR; ++k) ldmatrix4_trans(f[k], z + (((2 * (i + k) + lpiece) ^ (lrow & 7)) << 4));
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int e = 0; e < P; ++e)
 #pragma unroll
         for (int k = 0; k < PAIR; ++k)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
-            Mma16816<DT>::run(acc[i + k][n], f[k][0], f[k][1], f[k][2], f[k][3], b[half][n][0], b[half][n][1]);
+            Mma16816<DT>::run(acc[i + k][n], f[k][0], f[k][1], f[k][2], f[k][3], b[e][n][0], b[e][n][1]);
     }
     if constexpr (RG == 1) meet();  // all lanes have read the step before its place is fetched into
   }
