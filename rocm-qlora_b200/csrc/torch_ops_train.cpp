@@ -25,6 +25,26 @@ void check_rows(const Tensor& t, const char* name) {
               " must be a 2-D tensor with contiguous columns");
 }
 
+// The kernels take pointers: every tensor of a call is on the first one's device.
+void check_device(const Tensor& first, const Tensor& t) {
+  TORCH_CHECK(t.device() == first.device(), "rocm_qlora: tensors are on different devices: ", first.device(), " and ",
+              t.device());
+}
+void check_device(const Tensor& first, const optional<Tensor>& t) {
+  if (t.has_value() && t->defined()) check_device(first, *t);
+}
+template <class... Rest>
+void one_device(const Tensor& first, const Rest&... rest) {
+  (check_device(first, rest), ...);
+}
+
+bool plan_ok(const Tensor& plan) { return plan.dim() == 1 && plan.is_contiguous() && plan.scalar_type() == at::kInt; }
+
+void check_plan(const optional<Tensor>& plan) {
+  TORCH_CHECK(!plan.has_value() || !plan->defined() || plan_ok(*plan),
+              "rocm_qlora: plan must be a contiguous 1-D int32 tensor, as adapter_plan makes it");
+}
+
 Tensor adapter_plan(const Tensor& ids, int64_t count, int64_t tile) {
   TORCH_CHECK(ids.dim() == 1 && ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
               "rocm_qlora: ids must be a contiguous 1-D int64 or int32 tensor");
@@ -53,8 +73,11 @@ void apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& sca
         "rq_adapters_apply");
 }
 
-void check_bank(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling) {
+void check_bank(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
+                const optional<Tensor>& plan) {
   check_rows(in, "input");
+  one_device(in, U, V, scaling, plan);
+  check_plan(plan);
   TORCH_CHECK(U.dim() == 3 && V.dim() == 3 && U.is_contiguous() && V.is_contiguous() && U.size(0) == V.size(0) &&
                   U.size(2) == V.size(2) && U.size(1) == in.size(1) && U.scalar_type() == in.scalar_type() &&
                   V.scalar_type() == in.scalar_type(),
@@ -65,7 +88,8 @@ void check_bank(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor
 
 std::tuple<Tensor, Tensor> adapters_apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
                                           const optional<Tensor>& base, const optional<Tensor>& plan, int64_t tile) {
-  check_bank(in, U, V, scaling);
+  check_bank(in, U, V, scaling, plan);
+  one_device(in, base);
   if (base.has_value() && base->defined()) {
     check_rows(*base, "base");
     TORCH_CHECK(base->size(0) == in.size(0) && base->size(1) == V.size(1) && base->scalar_type() == in.scalar_type(),
@@ -79,7 +103,8 @@ std::tuple<Tensor, Tensor> adapters_apply(const Tensor& in, const Tensor& U, con
 
 Tensor adapters_apply_(Tensor out, const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
                        const Tensor& base, const optional<Tensor>& plan, int64_t tile) {
-  check_bank(in, U, V, scaling);
+  check_bank(in, U, V, scaling, plan);
+  one_device(in, out, base);
   check_rows(out, "out");
   check_rows(base, "base");
   TORCH_CHECK(out.size(0) == in.size(0) && out.size(1) == V.size(1) && out.scalar_type() == in.scalar_type() &&
@@ -92,7 +117,7 @@ Tensor adapters_apply_(Tensor out, const Tensor& in, const Tensor& U, const Tens
 
 Tensor adapters_mid(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
                     const optional<Tensor>& plan, int64_t tile) {
-  check_bank(in, U, V, scaling);
+  check_bank(in, U, V, scaling, plan);
   Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
   if (!in.is_meta()) apply(in, U, V, scaling, std::nullopt, plan, tile, mid, std::nullopt);
   return mid;
@@ -101,6 +126,8 @@ Tensor adapters_mid(const Tensor& in, const Tensor& U, const Tensor& V, const Te
 Tensor adapters_grad(const Tensor& z, const optional<Tensor>& scales, const Tensor& mid, int64_t D, int64_t count,
                      at::ScalarType dtype, const optional<Tensor>& plan, int64_t tile) {
   check_rows(z, "rows");
+  one_device(z, scales, mid, plan);
+  check_plan(plan);
   const bool packed = scales.has_value() && scales->defined(), has_plan = plan.has_value() && plan->defined();
   const int64_t nb = (D + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
   TORCH_CHECK(mid.dim() == 2 && mid.is_contiguous() && mid.size(0) == z.size(0) && mid.scalar_type() == at::kFloat,
@@ -138,6 +165,7 @@ std::tuple<Tensor, Tensor> act8_pack(const Tensor& x) {
 
 void check_packed(const Tensor& codes, const Tensor& scales, int64_t K) {
   const int64_t nb = (K + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
+  one_device(codes, scales);
   TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous() && codes.scalar_type() == at::kChar &&
                   scales.scalar_type() == at::kFloat && codes.dim() == scales.dim() &&
                   codes.size(-1) == nb * RQ_ACT8_BLOCK && scales.size(-1) == nb &&
@@ -160,6 +188,7 @@ Tensor act8_unpack(const Tensor& codes, const Tensor& scales, int64_t K, at::Sca
 std::tuple<Tensor, Tensor, Tensor> swiglu8_forward(const Tensor& gate, const Tensor& up, int64_t copies) {
   check_rows(gate, "gate");
   check_rows(up, "up");
+  one_device(gate, up);
   TORCH_CHECK(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type(),
               "rocm_qlora: gate and up must have one shape and dtype");
   const int64_t nb = blocks_of(gate.size(1));
@@ -178,6 +207,7 @@ std::tuple<Tensor, Tensor, Tensor> swiglu8_forward(const Tensor& gate, const Ten
 
 std::tuple<Tensor, Tensor> swiglu8_backward(const Tensor& dh, const Tensor& codes, const Tensor& scales) {
   check_rows(dh, "dh");
+  one_device(dh, codes);
   TORCH_CHECK(codes.dim() == 3 && codes.size(0) >= 2 && codes.size(1) == dh.size(0),
               "rocm_qlora: codes must hold the packed gate and up of dh's rows");
   check_packed(codes, scales, dh.size(1));
@@ -193,6 +223,7 @@ std::tuple<Tensor, Tensor> swiglu8_backward(const Tensor& dh, const Tensor& code
 }
 
 void check_logits(const Tensor& logits, const Tensor& labels) {
+  one_device(logits, labels);
   TORCH_CHECK(logits.dim() == 3 && (logits.size(2) <= 1 || logits.stride(2) == 1),
               "rocm_qlora: logits must be [batch, length, vocabulary] with a contiguous vocabulary");
   TORCH_CHECK(labels.dim() == 2 && labels.is_contiguous() && labels.scalar_type() == at::kLong &&
@@ -223,6 +254,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> preference_forward(const Tens
                                                                       const Tensor& ref, int64_t ignore, int64_t form,
                                                                       double beta, double smooth) {
   check_logits(logits, labels);
+  one_device(logits, ref);
   TORCH_CHECK(ref.sizes() == labels.sizes() && ref.is_contiguous() && ref.scalar_type() == at::kFloat,
               "rocm_qlora: ref must be a contiguous [batch, length] float32 tensor");
   const auto f32 = logits.options().dtype(at::kFloat);
@@ -243,6 +275,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> preference_forward(const Tens
 Tensor token_logprobs_grad(const Tensor& logits, const Tensor& labels, int64_t ignore, const Tensor& stats,
                            const Tensor& slopes, const optional<Tensor>& upstream) {
   check_logits(logits, labels);
+  one_device(logits, stats, slopes, upstream);
   const bool per_token = slopes.dim() == 2;
   TORCH_CHECK(slopes.is_contiguous() && slopes.scalar_type() == at::kFloat && slopes.size(0) == logits.size(0) &&
                   (!per_token || slopes.size(1) == logits.size(1)) && stats.is_contiguous() &&
@@ -345,14 +378,20 @@ void check_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tenso
   }
   TORCH_CHECK_TYPE(base.scalar_type() == dt, "base is ", base.scalar_type(), ", x ", dt);
   TORCH_CHECK_VALUE(plan || count == 1, "a bank of several adapters needs a plan");
+  TORCH_CHECK_VALUE(!plan || plan_ok(*plan), "plan must be a contiguous 1-D int32 tensor: the data of an AdapterPlan");
   TORCH_CHECK_VALUE(!plan || (plan_rows == rows && plan_count == count), "the plan is for ", plan_rows, " rows and ",
                     plan_count, " adapters, not ", rows, " and ", count);
   if (codes) {
     const int64_t nb = (A.size(1) + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
-    TORCH_CHECK_VALUE(scales && codes->dim() == 2 && codes->size(0) == rows && codes->size(1) == nb * RQ_ACT8_BLOCK,
+    TORCH_CHECK_VALUE(scales && codes->dim() == 2 && codes->size(0) == rows && codes->size(1) == nb * RQ_ACT8_BLOCK &&
+                          scales->dim() == 2 && scales->size(0) == rows && scales->size(1) == nb,
                       "packed_x does not belong to x ", sizes_of(x));
+    TORCH_CHECK_VALUE(codes->scalar_type() == at::kChar && scales->scalar_type() == at::kFloat &&
+                          codes->is_contiguous() && scales->is_contiguous(),
+                      "packed_x holds contiguous int8 codes and float32 scales, got ", codes->scalar_type(), " and ",
+                      scales->scalar_type());
   }
-  check_gpu({&x, &base, &A, &B, &scaling});
+  check_gpu({&x, &base, &A, &B, &scaling, plan ? &*plan : &x, codes ? &*codes : &x, codes ? &*scales : &x});
 }
 
 Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B, const Tensor& scaling,

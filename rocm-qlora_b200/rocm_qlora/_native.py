@@ -159,11 +159,13 @@ def ops() -> bool:
     return _ops_state
 
 
-def require_ops(*ts: torch.Tensor):
+def require_ops(*ts: Optional[torch.Tensor]):
     """torch.ops.rocm_qlora for operators that exist only there, after checking
-    that the tensors are on one sm_100 CUDA device."""
+    that the tensors (None: not given) are on one sm_100 CUDA device."""
     first = ts[0]
     for t in ts:
+        if t is None:
+            continue
         if not t.is_cuda:
             raise NativeUnavailable(
                 "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device")

@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from rocm_qlora import _native as nat
-from rocm_qlora.activation8.packed import PackedActivation, rows_of
+from rocm_qlora.activation8.packed import BLOCK, PackedActivation, rows_of
 from rocm_qlora.quantization import layer_ops
 
 MAX_RANK = 128
@@ -68,9 +68,13 @@ def _plan_args(plan: Optional[AdapterPlan], rows: int, count: int):
 def _packed_args(packed_x: Optional[PackedActivation], x: torch.Tensor):
     if packed_x is None:
         return None, None
-    if packed_x.shape[-1] != x.shape[-1] or packed_x.codes.shape[0] != x.numel() // max(1, x.shape[-1]):
+    codes, scales = packed_x.codes, packed_x.scales
+    if packed_x.shape[-1] != x.shape[-1] or codes.shape[0] != x.numel() // max(1, x.shape[-1]):
         raise ValueError(f"packed_x is of {packed_x.shape}, x of {tuple(x.shape)}")
-    return packed_x.codes, packed_x.scales
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32 or codes.numel() != scales.numel() * BLOCK:
+        raise ValueError(f"packed_x holds int8 codes and a float32 scale for each {BLOCK} of them, got {codes.dtype} "
+                         f"{tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+    return codes, scales
 
 
 def _check_bank(x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, scaling: torch.Tensor) -> None:
@@ -121,9 +125,9 @@ def _add_out(base, x, A, B, scaling, plan, out) -> torch.Tensor:
         raise ValueError(f"base {tuple(base.shape)} and x {tuple(x.shape)} do not fit A {tuple(A.shape)} and "
                          f"B {tuple(B.shape)}")
     x2, base2 = rows_of(x), rows_of(base)
-    nat.require_ops(base, x, A, B, scaling, out).adapters_apply_(
-        out.view(base2.shape), x2, A.contiguous(), B.contiguous(), scaling.contiguous(), base2,
-        *_plan_args(plan, x2.shape[0], A.shape[0]))
+    data, tile = _plan_args(plan, x2.shape[0], A.shape[0])
+    nat.require_ops(base, x, A, B, scaling, out, data).adapters_apply_(
+        out.view(base2.shape), x2, A.contiguous(), B.contiguous(), scaling.contiguous(), base2, data, tile)
     return out
 
 
@@ -134,7 +138,7 @@ class _BankLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, A, B, w, bias, scaling, plan, codes, scales):
         data, tile = plan
-        ops = nat.require_ops(x, A, B, scaling)
+        ops = nat.require_ops(x, A, B, scaling, data, codes, scales)
         rows = x.reshape(-1, w.K).contiguous()
         y = layer_ops.forward(w, rows, bias.to(x.dtype).contiguous() if bias is not None else None, None, None, 1.0)
         mid = ops.adapters_apply_(y, rows, A, B, scaling, y, data, tile)
