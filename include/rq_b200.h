@@ -345,7 +345,7 @@ RQ_API int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const
  * mid, of B with z = dy and the forward's mid.  With z_scales not NULL z is
  * the 8-bit packed form (rq_act8_pack): int8 codes [M, ceil(D / 128) * 128]
  * and z_scales [M, ceil(D / 128)].  grad [count, D, r] in dtype; an adapter
- * without rows gets zeros. */
+ * without rows gets zeros.  plan NULL: every row is adapter 0's. */
 RQ_API int rq_adapters_grad(const void* z, int64_t ld_z, const float* z_scales, const float* mid,
                      int64_t M, int64_t D, int r, int count, int dtype,
                      const int32_t* plan, int64_t plan_words, int tile_rows,

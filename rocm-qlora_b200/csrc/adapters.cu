@@ -880,9 +880,10 @@ struct GradArgs {
   int most;
 };
 
-// Rows of an adapter: places [first, last) of the plan's order, or the batch.
+// Rows of an adapter: places [first, last) of the plan's order; without a plan
+// the whole batch is adapter 0's.
 __device__ __forceinline__ int2 grad_rows(const AdapterRows& a, int adapter) {
-  if (!a.plan) return make_int2(0, (int)a.M);
+  if (!a.plan) return make_int2(0, adapter == 0 ? (int)a.M : 0);
   const int first = max(a.plan[1 + adapter], 0);
   return make_int2(first, max(first, min(a.plan[2 + adapter], (int)a.M)));
 }
