@@ -333,7 +333,8 @@ RQ_API int rq_adapter_plan(const void* ids, int wide, int64_t rows, int count, i
  * the backward; may be NULL).  Forward: U = A, V = B, in = x.  Input gradient: U = B, V = A,
  * in = dy.  Everything is accumulated in fp32 and rounded once.  plan NULL:
  * every row uses adapter 0.  Row strides (ld*) in elements, columns
- * contiguous. */
+ * contiguous; a stride of 0, here and in the functions below, is one input row
+ * for all (not for out). */
 RQ_API int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const void* V,
                       const float* scaling, const void* base, int64_t ld_base,
                       int64_t M, int64_t D1, int64_t D2, int r, int count, int dtype,

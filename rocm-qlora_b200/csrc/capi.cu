@@ -109,6 +109,10 @@ static bool half_ok(int dt) { return dt == RQ_BF16 || dt == RQ_F16; }
 // Sizes a kernel indexes with 32 bits.
 static bool fits(int64_t v) { return v >= 0 && v < (int64_t)1 << 31; }
 
+// Distances between the rows of an input, which is only read: 0 is one row
+// broadcast to all.
+static bool row_stride(int64_t M, int64_t ld, int64_t columns) { return M <= 1 || ld == 0 || ld >= columns; }
+
 // Rows whose 8-bit blocks are numbered with 32 bits.
 static bool fits_act8(int64_t M, int64_t K) {
   return fits(M) && fits(K) && fits(M * ((K + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK));
@@ -359,7 +363,7 @@ int rq_adapters_apply(const void* in, int64_t ld_in, const void* U, const void* 
   if (!fits(D1) || !fits(D2) || r < 8 || r > 128 || r % 8) return RQ_ERR_INVALID;
   if (M == 0) return RQ_OK;
   if (!scaling || (D1 > 0 && (!in || !U)) || (D2 > 0 && (!V || !out))) return RQ_ERR_INVALID;
-  if ((M > 1) && (ld_in < D1 || ld_out < D2 || (base && ld_base < D2))) return RQ_ERR_INVALID;
+  if (!row_stride(M, ld_in, D1) || (base && !row_stride(M, ld_base, D2)) || (M > 1 && ld_out < D2)) return RQ_ERR_INVALID;
   if ((uintptr_t)in % 2 || (uintptr_t)base % 2 || (uintptr_t)out % 2 || (uintptr_t)U % 16 || (uintptr_t)V % 16 ||
       (uintptr_t)mid % 16 || (uintptr_t)scaling % 4)
     return RQ_ERR_ALIGN;
@@ -378,7 +382,7 @@ int rq_adapters_grad(const void* z, int64_t ld_z, const float* z_scales, const f
   if (D == 0) return RQ_OK;
   const int64_t nb = (D + RQ_ACT8_BLOCK - 1) / RQ_ACT8_BLOCK;
   if (!grad || (M > 0 && (!z || !mid))) return RQ_ERR_INVALID;
-  if (M > 1 && ld_z < (z_scales ? nb * RQ_ACT8_BLOCK : D)) return RQ_ERR_INVALID;
+  if (!row_stride(M, ld_z, z_scales ? nb * RQ_ACT8_BLOCK : D)) return RQ_ERR_INVALID;
   if ((uintptr_t)z % (z_scales ? 16 : 2) || (z_scales && (ld_z % 16 || (uintptr_t)z_scales % 4)) || (uintptr_t)mid % 16 || (uintptr_t)grad % 16)
     return RQ_ERR_ALIGN;
   const AdapterRows a{M, D, 0, r, count, dtype, tile_rows, plan};
@@ -389,7 +393,7 @@ int rq_act8_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, i
                  void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits_act8(M, K) || (M > 1 && ld_x < K)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K) || !row_stride(M, ld_x, K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!x || !codes || !scales) return RQ_ERR_INVALID;
   if ((uintptr_t)x % dtype_size(dtype) || (uintptr_t)codes % 16 || (uintptr_t)scales % 4) return RQ_ERR_ALIGN;
@@ -412,7 +416,7 @@ int rq_swiglu8_forward(const void* gate, int64_t ld_gate, const void* up, int64_
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
   if (!fits_act8(M, K) || (copies != 2 && copies != 3)) return RQ_ERR_INVALID;
-  if (M > 1 && (ld_gate < K || ld_up < K)) return RQ_ERR_INVALID;
+  if (!row_stride(M, ld_gate, K) || !row_stride(M, ld_up, K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!gate || !up || !h || !codes || !scales) return RQ_ERR_INVALID;
   const int e = dtype_size(dtype);
@@ -425,7 +429,7 @@ int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t M, int
                         const float* scales, void* dgate, void* dup, void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
-  if (!fits_act8(M, K) || (M > 1 && ld_dh < K)) return RQ_ERR_INVALID;
+  if (!fits_act8(M, K) || !row_stride(M, ld_dh, K)) return RQ_ERR_INVALID;
   if (M * K == 0) return RQ_OK;
   if (!dh || !codes || !scales || !dgate || !dup) return RQ_ERR_INVALID;
   const int e = dtype_size(dtype);

@@ -304,9 +304,13 @@ void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "rocm_qlora: ", what, " is differentiable once only");
 }
 
+// t as [rows, columns]: contiguous columns, rows apart or one row for all; a
+// copy where its strides are others (rows that overlap among them).
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), t.size(-1)});
-  return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
+  const bool columns = r.size(1) <= 1 || r.stride(1) == 1;
+  const bool rows = r.size(0) <= 1 || r.stride(0) == 0 || r.stride(0) >= r.size(1);
+  return columns && rows ? r : r.contiguous();
 }
 
 optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }

@@ -37,10 +37,13 @@ class PackedActivation:
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
-    """t as [rows, columns] with contiguous columns: a view where its strides allow."""
+    """t as [rows, columns] with contiguous columns, its rows apart or one row
+    for all (stride 0): a view where its strides allow."""
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    columns = t.shape[1] <= 1 or t.stride(1) == 1
+    rows = t.shape[0] <= 1 or t.stride(0) == 0 or t.stride(0) >= t.shape[1]
+    return t if columns and rows else t.contiguous()
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:
