@@ -404,8 +404,10 @@ Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const 
   check_add(base, x, A, B, scaling, plan, plan_rows, plan_count, codes, scales);
   const Tensor b2 = rows_of(base), x2 = rows_of(x), a3 = A.contiguous(), b3 = B.contiguous(), s1 = scaling.contiguous();
   TORCH_CHECK_VALUE(!scaling.requires_grad(), "scaling has no gradient: fold a trainable factor into A or B");
-  const bool grad = at::GradMode::is_enabled() &&
-                    (base.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
+  bool grad = at::GradMode::is_enabled() &&
+              (base.requires_grad() || x.requires_grad() || A.requires_grad() || B.requires_grad());
+  // a tangent of forward-mode differentiation goes to the autograd node too, which refuses it
+  for (const Tensor* t : {&base, &x, &A, &B, &scaling}) grad |= t->_fw_grad(/*level=*/0).defined();
   Tensor y;
   if (grad) {
     y = AdaptersAdd::apply(b2, x2, a3, b3, s1, plan, tile, codes, scales);

@@ -14,6 +14,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from rocm_qlora import _native as nat
@@ -117,7 +118,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.
 
 def _add_out(base, x, A, B, scaling, plan, out) -> torch.Tensor:
     _check_bank(x, A, B, scaling)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, A, B, out)):
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, A, B, out))
+            or any(unpack_dual(t).tangent is not None for t in (base, x, A, B, scaling, out))):
         raise RuntimeError("adapters_add(out=...) does not support automatic differentiation")
     if out.shape != base.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of base's shape and dtype")
