@@ -6,6 +6,7 @@
 // only give shapes.
 #include "torch_ops.h"
 
+#include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <tuple>
@@ -112,6 +113,23 @@ Tensor adapters_apply_(Tensor out, const Tensor& in, const Tensor& U, const Tens
               "rocm_qlora: out and base must be [rows, ", V.size(1), "] of the input's dtype");
   Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
   if (!in.is_meta()) apply(in, U, V, scaling, base, plan, tile, mid, out);
+  return mid;
+}
+
+// Above the backends: autograd's version counter of `out` counts the write, so
+// that a node which saved it refuses its backward.
+Tensor adapters_apply_versioned(c10::DispatchKeySet keys, Tensor out, const Tensor& in, const Tensor& U, const Tensor& V,
+                                const Tensor& scaling, const Tensor& base, const optional<Tensor>& plan, int64_t tile) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("rocm_qlora::adapters_apply_", "")
+                             .typed<Tensor(Tensor, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                           const Tensor&, const optional<Tensor>&, int64_t)>();
+  Tensor mid;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    mid = op.redispatch(keys & c10::after_ADInplaceOrView_keyset, out, in, U, V, scaling, base, plan, tile);
+  }
+  torch::autograd::increment_version(out);
   return mid;
 }
 
@@ -584,3 +602,4 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
 
 TORCH_LIBRARY_IMPL(rocm_qlora, CUDA, m) { RQ_IMPLS(m); }
 TORCH_LIBRARY_IMPL(rocm_qlora, Meta, m) { RQ_IMPLS(m); }
+TORCH_LIBRARY_IMPL(rocm_qlora, ADInplaceOrView, m) { m.impl("adapters_apply_", &adapters_apply_versioned); }
