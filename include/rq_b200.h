@@ -384,9 +384,9 @@ RQ_API int rq_swiglu8_backward(const void* dh, int64_t ld_dh, int dtype, int64_t
  * contiguous: position l is scored on labels[b, l + 1]; a label equal to
  * `ignore` (and the last position) does not count, and a label outside
  * [0, V) gives NaN.  rq_token_logprobs writes stats [B, L, 4] fp32, 16-byte
- * aligned (k, s, hi, lo: the sum of the row's exponentials is s 2^k, the
- * label's log-probability hi + lo; rows that do not count are left as they
- * are) and, unless NULL, logps [B, L]: the log-probability of each label, 0
+ * aligned (k, s, hi, lo: the sum of the row's exponentials is s 2^k or, where
+ * s < 0, in rows whose logits leave +-2^19, -s e^k; the label's log-probability
+ * is hi + lo; rows that do not count are left as they are) and, unless NULL, logps [B, L]: the log-probability of each label, 0
  * where it does not count. */
 RQ_API int rq_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_l,
                       int64_t B, int64_t L, int64_t V, const int64_t* labels, int64_t ignore,

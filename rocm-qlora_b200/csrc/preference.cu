@@ -106,11 +106,17 @@ __device__ __forceinline__ float whole_exp2(float n) {
 // thousands of tokens it would add up.
 constexpr double kExp2Low = 4.97e-8;
 
+// The range of k.  Beyond it fp32 no longer holds x log2(e) to a fraction, and
+// at the type's ends not at all.  Values further down count as none beside a
+// largest one that is not down there itself; values further up make the sum
+// infinite.  Rows of either kind are summed again, by wide_row.
+constexpr float kWhole = 0x1p20f;
+
 struct ExpSum {
   float k = 0.0f, s = 0.0f;
   __device__ __forceinline__ void raise(float top) {  // top: the largest of the values to come
     const float z = top * kLog2e;
-    if ((z > k || s == 0.0f) && fabsf(z) < INFINITY) {
+    if ((z > k || s == 0.0f) && fabsf(z) < kWhole) {
       const float to = ceilf(z);
       if (s != 0.0f) s *= whole_exp2(k - to);
       k = to;
@@ -133,7 +139,36 @@ struct ExpSum {
   }
 };
 
-// stats[at] = (k, s, hi, lo) of each row that counts: the normaliser s 2^k and
+// A row of logits of any magnitude (masked whole with the type's lowest value,
+// say), by its definition: the largest value first, then the sum of e^(x - m)
+// in 64 bits.  NaN where that is no distribution: an infinity above, a NaN, or
+// nothing finite.  Leaves the warps' largest values and sums for their threads to join.
+template <int DT, int TH>
+__device__ __noinline__ void wide_row(const typename DType<DT>::T* x, int V, float* tops, double* sums) {
+  const int tid = threadIdx.x;
+  float top = -INFINITY;
+  bool none = false;
+  for (int v = tid; v < V; v += TH) {
+    const float f = DType<DT>::to_f32(x[v]);
+    none |= !(f < INFINITY);
+    top = fmaxf(top, f);
+  }
+  none = __syncthreads_or(none);  // and all have read what tops held
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+  for (int w = 0; w < TH / 32; ++w) top = fmaxf(top, tops[w]);
+  double s = 0.0;
+  for (int v = tid; v < V; v += TH) s += (double)expf(DType<DT>::to_f32(x[v]) - top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((tid & 31) == 0) sums[tid >> 5] = none ? (double)__uint_as_float(0x7fc00000u) : s;
+  __syncthreads();
+}
+
+// stats[at] = (k, s, hi, lo) of each row that counts: the normaliser s 2^k (of
+// a wide row (m, -s): -s below zero marks it, and the normaliser is s e^m) and
 // the label's log-probability hi + lo; logps (optional) has it at the label's
 // own place [b, l + 1], and 0 where nothing counts.  One CTA a row, one pass;
 // bound by HBM, with the exponentials (16 a clock of an SM) at 72 % of the
@@ -184,26 +219,31 @@ __global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, floa
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) k = fmaxf(k, __shfl_xor_sync(0xffffffffu, k, o));
   if ((tid & 31) == 0) ks[tid >> 5] = k;
-  __syncthreads();
+  bool wide = __syncthreads_or(!(sum.s < INFINITY));
   k = ks[0];
 #pragma unroll
   for (int w = 1; w < TH / 32; ++w) k = fmaxf(k, ks[w]);
-  double s = sum.s == 0.0f ? 0.0 : (double)sum.s * (double)whole_exp2(sum.k - k);
+  wide |= k < -0.5f * kWhole;
+  if (wide) {
+    wide_row<DT, TH>(x, (int)t.V, ks, sums);
+    k = ks[0];
+    for (int w = 1; w < TH / 32; ++w) k = fmaxf(k, ks[w]);
+  } else {
+    double s = sum.s == 0.0f ? 0.0 : (double)sum.s * (double)whole_exp2(sum.k - k);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((tid & 31) == 0) sums[tid >> 5] = s;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((tid & 31) == 0) sums[tid >> 5] = s;
+    __syncthreads();
+  }
   if (tid == 0) {
-    s = sums[0];
+    double s = sums[0];
     for (int w = 1; w < TH / 32; ++w) s += sums[w];
-    s *= 1.0 + kExp2Low;
-    // no finite logit at all, an infinity or a NaN among them: not a distribution
-    if (!(s > 0.0 && s < (double)INFINITY)) s = (double)__uint_as_float(0x7fc00000u);
+    if (!wide) s *= 1.0 + kExp2Low;
     // a label outside the vocabulary has no probability: NaN, not a read past the row
     const float xy = y >= 0 && y < t.V ? DType<DT>::to_f32(x[y]) : __uint_as_float(0x7fc00000u);
-    const double lp = (double)xy - ((double)k + log2(s)) / kLog2eD;
+    const double lp = (double)xy - (wide ? (double)k : (double)k / kLog2eD) - log2(s) / kLog2eD;
     const float hi = (float)lp;
-    stats[at] = make_float4(k, (float)s, hi, fabsf(hi) < INFINITY ? (float)(lp - (double)hi) : 0.0f);
+    stats[at] = make_float4(k, wide ? (float)-s : (float)s, hi, fabsf(hi) < INFINITY ? (float)(lp - (double)hi) : 0.0f);
     if (logps) logps[at + 1] = hi;
   }
 }
@@ -310,7 +350,7 @@ __global__ void __launch_bounds__(kPrefWarps * 32) __cluster_dims__(kPrefCtas, 1
 }
 
 // dlogits = c ([v = y] - 2^(x log2(e) - k) / s), zero where the row does not
-// count.  One CTA a row, the rows in the reverse of the forward's order, so
+// count; of a wide row e^(x - m) / s.  One CTA a row, the rows in the reverse of the forward's order, so
 // that the last rows it read are still in L2.  HBM bound: 300 us for 16384
 // rows of 32000 bf16 logits of which 14792 count, 6.7 TB/s.
 template <int DT>
@@ -336,9 +376,10 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
   float c = per_token ? slopes[at + 1] : slopes[at / t.L];
   if (upstream) c *= *upstream;
   if (y < 0 || y >= t.V) c = __uint_as_float(0x7fc00000u);
-  const float by = -c / q.y, k = q.x;
+  const bool wide = q.y < 0.0f;
+  const float by = -c / fabsf(q.y), k = wide ? 0.0f : q.x, m = wide ? q.x : 0.0f;
   auto value = [&](float f) { return by * exp_over(f, k); };
-  if ((((uintptr_t)x ^ (uintptr_t)d) & 15) == 0) {
+  if (!wide && (((uintptr_t)x ^ (uintptr_t)d) & 15) == 0) {
     const RowCut<DT> cut(x, (int)t.V);
     const uint4* src = reinterpret_cast<const uint4*>(x + cut.head);
     uint4* dst = reinterpret_cast<uint4*>(d + cut.head);
@@ -373,9 +414,9 @@ __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const f
       const int64_t v = tid < cut.head ? tid : t.V - cut.tail + (tid - cut.head);
       d[v] = DType<DT>::from_f32(value(DType<DT>::to_f32(x[v])) + (v == y ? c : 0.0f));
     }
-  } else {  // rows of different alignment: value by value
+  } else {  // rows of different alignment, wide rows: value by value
     for (int64_t v = tid; v < t.V; v += kTokThreads)
-      d[v] = DType<DT>::from_f32(value(DType<DT>::to_f32(x[v])) + (v == y ? c : 0.0f));
+      d[v] = DType<DT>::from_f32(value(DType<DT>::to_f32(x[v]) - m) + (v == y ? c : 0.0f));
   }
 }
 
