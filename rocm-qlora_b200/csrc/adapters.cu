@@ -291,6 +291,29 @@ __device__ __forceinline__ void split16(float x, float y, uint32_t (&p)[kPieces<
   }
 }
 
+__device__ __forceinline__ bool any_nan(float x, float y) { return !(x == x && y == y); }
+
+// sum + 0 w, for both 16-bit values of a word.
+template <int DT>
+__device__ __forceinline__ uint32_t add_zeros(uint32_t w, uint32_t sum) {
+  if constexpr (DT == RQ_BF16) {
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(0.0f),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(0.0f),
+                              *reinterpret_cast<const __half2*>(&sum));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// The values that are not finite as zeros.
+template <int DT>
+__device__ __forceinline__ uint32_t finite16(uint32_t w) {
+  constexpr uint32_t top = DT == RQ_BF16 ? 0x7f807f80u : 0x7c007c00u;
+  return w & ~__vcmpeq2(w & top, top);
+}
+
 template <int N>
 __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[N]) {
   if constexpr (N == 1) *static_cast<uint32_t*>(p) = w[0];
@@ -413,6 +436,34 @@ __device__ __noinline__ void rows_without(const ApplyArgs& p, const int* order, 
   }
 }
 
+// A lane's outputs of an m-tile and 32-column chunks, value by value: for
+// chunks of V that hold an infinity (times a piece of mid that is zero it would
+// be NaN; times their sum it is not, unless that is zero) or a NaN.
+template <int DT, int R, int CW>
+__device__ __noinline__ void tile_by_value(const ApplyRows& at, const unsigned char* mids, int piece_bytes,
+                                           const uint16_t* V, int r, bool has_base, int row0, int rows, int64_t col,
+                                           int64_t end) {
+  using T = typename DType<DT>::T;
+  for (int h = 0; h < 2; ++h) {
+    const int row = row0 + 8 * h;
+    if (row >= rows) continue;
+    const float mul = DT == RQ_F16 ? at.mul[row] : 1.0f;
+    for (int w = 0; w < CW * 32; w += w % 32 == 7 ? 25 : 1) {
+      const int64_t n = col + w;
+      if (n >= end) break;
+      float s = 0.0f;
+      for (int j = 0; j < r; ++j) {
+        float t = 0.0f;
+        for (int k = 0; k < kPieces<DT>; ++k)
+          t += DType<DT>::to_f32(reinterpret_cast<const T*>(mids + k * piece_bytes + row * ap_pitch_m(R))[j]);
+        s = fmaf(t, DType<DT>::to_f32(reinterpret_cast<const T*>(V + n * r)[j]), s);
+      }
+      const float old = has_base ? DType<DT>::to_f32(reinterpret_cast<const T*>(at.base[row])[n]) : 0.0f;
+      reinterpret_cast<T*>(at.out[row])[n] = DType<DT>::from_f32(fmaf(s, mul, old));
+    }
+  }
+}
+
 // One cluster computes one tile: `tile` rows (16 to 128) of one adapter.
 //
 // Mathematics.  mid = s (in U) and out = base + mid V^T, both on tensor cores
@@ -503,7 +554,8 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
   auto slot_of = [](int k) { return (k & ~31) | ((k & 6) << 2) | (((k & 31) >> 3) << 1) | (k & 1); };
   const bool rank = q * 8 < a.r;
   const uint16_t* u_src = U + ((int64_t)w_begin * kApWin + k0) * a.r + (rank ? q * 8 : 0);
-  int u_left = (int)(a.D1 - (int64_t)w_begin * kApWin) - k0;  // rows from u_src on
+  // rows from u_src on that are this CTA's: x is zero past them, which an infinity of U would make a NaN
+  int u_left = (int)(min((int64_t)w_end * kApWin, a.D1) - (int64_t)w_begin * kApWin) - k0;
   const uint32_t u_dst = slot_of(k0) * PU + q * 16;
   auto stage_u = [&](int c) {
     if (c >= chunks) return;
@@ -657,6 +709,18 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
       }
     }
   };
+  // Whether all of the chunk's V is finite: a sum of zeros times it is NaN else.
+  // Of the first chunk it is asked after the sums have met, so that V is on its
+  // way until then.
+  auto finite_b = [&] {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4 * CW; ++j)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) sum = add_zeros<DT>(b[j / 4][j % 4][k][1], add_zeros<DT>(b[j / 4][j % 4][k][0], sum));
+    const float2 zero = unpair16<DT>(sum);
+    return !__any_sync(0xffffffffu, any_nan(zero.x, zero.y));
+  };
   if (f_ch < ch_end) load_b(f_ch);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(ahead[i]);
@@ -676,8 +740,8 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     float top = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      v[e] *= s;
-      top = fmaxf(top, fabsf(v[e]));
+      v[e] = l * E + e < a.r ? v[e] * s : 0.0f;  // an infinity of x times the padding is NaN
+      top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
       if (p.mid && on && row < rows && l * E + e < a.r) p.mid[(int64_t)at.row[row] * a.r + l * E + e] = v[e];
     }
     float mul = 1.0f, back = 1.0f;
@@ -786,14 +850,24 @@ __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(
     }
   };
   int ch = ch_begin + warp * CW, mt = 0;
+  bool by_value = ch < ch_end && !finite_b();
   while (ch < ch_end) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       if (ch >= ch_end) break;
-      tile((int64_t)ch * 32 + 8 * t, mt, ahead[i]);
+      if (by_value) {
+        tile_by_value<DT, R, CW>(at, mids, a.tile * PM, V, a.r, base != nullptr, mt * 16 + g, rows,
+                                 (int64_t)ch * 32 + 8 * t, end);
+        fetch(ahead[i]);
+      } else {
+        tile((int64_t)ch * 32 + 8 * t, mt, ahead[i]);
+      }
       if (++mt == n_tiles) {
         mt = 0, ch += ch_step;
-        if (ch < ch_end) load_b(ch);
+        if (ch < ch_end) {
+          load_b(ch);
+          by_value = !finite_b();
+        }
       }
     }
   }
@@ -930,29 +1004,16 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   }
 }
 
-// G_a[d, j] = sum over the rows m of a of z[m, d] mid[m, j].
-//
-// One CTA sums 128 columns of one adapter.  RG warps hold 16 ranks each; the
-// MW groups of them (8 / RG, or 1) split the rows, and the CTAs of a cluster
-// split them again.  Sums meet in shared and distributed shared memory in group and rank
-// order, so equal inputs give equal bits, without atomics or a workspace.
-//
-// The reduction runs over rows, so the MMA's k index is the row and ldmatrix
-// transposes z's tile on its way to the registers.  Each group fetches its own
-// 16-row steps by cp.async into its own ring, a thread one row a step, and
-// only the group waits for them.  z is read once.  Codes become 16-bit values
-// exactly; their scale multiplies the other operand, mid, in fp32, which then
-// enters as 16-bit pieces as in the row products.
-//
-// Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
-// meetings) is what is seen: 64 MB of z at rank 16 take 22 us, 32 MB of codes
-// 22; rank 64 59 and 66 us, where four warps a group share the rows and the
-// three pieces of mid are mma.sync's work.
-template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
-__device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
-  using T = typename DType<DT>::T;
+// The sums of one warp: 128 columns from block * 128 on, 16 ranks, over the
+// rows of its group; acc[m-tile][rank of a pair][].  Gives, for fp16, the
+// biased exponent that they are scaled down by.  AGAIN: what is not finite in z
+// meets only the first piece of mid (a piece that is zero would make an
+// infinity NaN).
+template <int DT, bool CODES, bool VEC, int RG, int MW, bool AGAIN>
+__device__ __forceinline__ int sum_rows(const GradArgs& p, int2 places, int block, int crank, int csize,
+                                        float (&acc)[8][2][4]) {
   constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
-  constexpr int S = gr_steps(CODES, VEC, RG), R16 = RG * 16, THREADS = 32 * RG * MW;
+  constexpr int S = gr_steps(CODES, VEC, RG);
   constexpr bool CONV = CODES && RG > 1;        // codes become 16-bit once for all warps of a group
   // m-tiles at a time: two put four sums between two products of one sum; with
   // one warp a ring the registers for that are not there (22 against 25 us at
@@ -961,31 +1022,12 @@ __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
   constexpr int TR = 2 * RG;                    // threads of a group that fetch one row
   constexpr int PIECES = (ROW / 16 + TR - 1) / TR;  // 16-byte pieces of it each
   extern __shared__ __align__(16) unsigned char smem[];
-  float* sums = reinterpret_cast<float*>(smem);
   const AdapterRows& a = p.a;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
-  const int block = (int)(blockIdx.x / csize);
+  const int first = places.x, last = places.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, mw = warp / RG;
-
-  int adapter = blockIdx.y;
-  if constexpr (LARGE) {
-    adapter = nth_large<THREADS>(p, adapter);
-    if (adapter < 0) return;
-  }
-  const int2 places = grad_rows(a, adapter);
-  const int first = places.x, last = places.y;
-  if (MW == 1 && p.beside && last - first > p.most) return;
   const int* order = a.plan ? a.plan + plan_rows_at(a.M, a.count, a.tile) : nullptr;
-  if (first >= last) {  // the whole cluster: no rows, zero gradient
-    const int64_t d0 = (int64_t)block * kGrCols, n = min((int64_t)kGrCols, a.D1 - d0) * a.r / 8;
-    uint4* G = reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d0) * a.r);
-    for (int64_t i = crank * THREADS + tid; i < n; i += csize * THREADS) G[i] = make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
   const int64_t c0 = (int64_t)block * kGrCols;
-  float acc[8][2][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -1090,10 +1132,18 @@ __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         top = max(top, max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu));
-      const int ex = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
+      int ex = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
+      if (ex == 255) {  // the largest finite one
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          for (const float x : {fabsf(v[i].x), fabsf(v[i].y)})
+            if (x < INFINITY) top = max(top, __float_as_uint(x));
+        ex = (int)(__reduce_max_sync(0xffffffffu, top) >> 23);
+      }
       if (ex > ex_now && ex > 30 && ex < 255) {
         if (ex_now) {
-          const float down = ex - ex_now < 126 ? __uint_as_float((uint32_t)(127 - (ex - ex_now)) << 23) : 0.0f;
+          const float down = ex - ex_now < 126 ? __uint_as_float((uint32_t)(127 - (ex - ex_now)) << 23) : 0x1p-126f;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -1135,16 +1185,115 @@ __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
         for (int k = 0; k < PAIR; ++k) ldmatrix4_trans(f[k], z + (((2 * (i + k) + lpiece) ^ (lrow & 7)) << 4));
       }
 #pragma unroll
-      for (int e = 0; e < P; ++e)
+      for (int e = 0; e < P; ++e) {
+        if constexpr (AGAIN) {
+          if (e == 1)
+#pragma unroll
+            for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) f[k][q] = finite16<DT>(f[k][q]);
+        }
 #pragma unroll
         for (int k = 0; k < PAIR; ++k)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
             Mma16816<DT>::run(acc[i + k][n], f[k][0], f[k][1], f[k][2], f[k][3], b[e][n][0], b[e][n][1]);
+      }
     }
     if constexpr (RG == 1) meet();  // all lanes have read the step before its place is fetched into
   }
   cp_async_wait<0>();
+  return ex_now;
+}
+
+template <int DT, bool VEC, int RG, int MW>
+__device__ __noinline__ int sum_rows_again(const GradArgs& p, int2 places, int block, int crank, int csize, float* sums) {
+  float acc[8][2][4];
+  const int ex = sum_rows<DT, false, VEC, RG, MW, true>(p, places, block, crank, csize, acc);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) sums[i] = acc[i / 8][i / 4 % 2][i % 4];
+  return ex;
+}
+
+// Whether one of a group's threads says so; its threads meet.
+template <int RG, int MW>
+__device__ __forceinline__ bool group_any(int mw, bool v) {
+  if constexpr (RG == 1) {
+    return __any_sync(0xffffffffu, v);
+  } else if constexpr (MW == 1) {
+    return __syncthreads_or(v);
+  } else {
+    int any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.s32 %0, 1, 0, q;\n}"
+                 : "=r"(any)
+                 : "r"((int)v), "r"(1 + mw), "n"(32 * RG)
+                 : "memory");
+    return any;
+  }
+}
+
+// G_a[d, j] = sum over the rows m of a of z[m, d] mid[m, j].
+//
+// One CTA sums 128 columns of one adapter.  RG warps hold 16 ranks each; the
+// MW groups of them (8 / RG, or 1) split the rows, and the CTAs of a cluster
+// split them again.  Sums meet in shared and distributed shared memory in group and rank
+// order, so equal inputs give equal bits, without atomics or a workspace.
+//
+// The reduction runs over rows, so the MMA's k index is the row and ldmatrix
+// transposes z's tile on its way to the registers.  Each group fetches its own
+// 16-row steps by cp.async into its own ring, a thread one row a step, and
+// only the group waits for them.  z is read once.  Codes become 16-bit values
+// exactly; their scale multiplies the other operand, mid, in fp32, which then
+// enters as 16-bit pieces as in the row products.
+//
+// Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
+// meetings) is what is seen: 64 MB of z at rank 16 take 22 us, 32 MB of codes
+// 22; rank 64 59 and 66 us, where four warps a group share the rows and the
+// three pieces of mid are mma.sync's work.
+template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
+__device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
+  using T = typename DType<DT>::T;
+  constexpr int R16 = RG * 16, THREADS = 32 * RG * MW;
+  constexpr bool CONV = CODES && RG > 1;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* sums = reinterpret_cast<float*>(smem);
+  const AdapterRows& a = p.a;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int crank = (int)cluster.block_rank(), csize = (int)cluster.num_blocks();
+  const int block = (int)(blockIdx.x / csize);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rg = warp % RG, mw = warp / RG;
+
+  int adapter = blockIdx.y;
+  if constexpr (LARGE) {
+    adapter = nth_large<THREADS>(p, adapter);
+    if (adapter < 0) return;
+  }
+  const int2 places = grad_rows(a, adapter);
+  const int first = places.x, last = places.y;
+  if (MW == 1 && p.beside && last - first > p.most) return;
+  if (first >= last) {  // the whole cluster: no rows, zero gradient
+    const int64_t d0 = (int64_t)block * kGrCols, n = min((int64_t)kGrCols, a.D1 - d0) * a.r / 8;
+    uint4* G = reinterpret_cast<uint4*>(static_cast<T*>(p.G) + ((int64_t)adapter * a.D1 + d0) * a.r);
+    for (int64_t i = crank * THREADS + tid; i < n; i += csize * THREADS) G[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const int64_t c0 = (int64_t)block * kGrCols;
+  float acc[8][2][4];
+  int ex_now = sum_rows<DT, CODES, VEC, RG, MW, false>(p, places, block, crank, csize, acc);
+  if constexpr (!CODES) {  // codes are finite, but for a scale that is NaN
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) nan |= any_nan(acc[i][n][0], acc[i][n][1]) || any_nan(acc[i][n][2], acc[i][n][3]);
+    if (group_any<RG, MW>(mw, nan)) {
+      float again[64];
+      ex_now = sum_rows_again<DT, VEC, RG, MW>(p, places, block, crank, csize, again);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i / 8][i / 4 % 2][i % 4] = again[i];
+    }
+  }
 
   // this warp's sums: m-tile i's rows g and g + 8, ranks 4t .. 4t+3
   const float back = DT == RQ_F16 && ex_now ? __uint_as_float((uint32_t)(ex_now - 14) << 23) : 1.0f;
