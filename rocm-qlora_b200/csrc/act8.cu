@@ -263,15 +263,18 @@ __global__ void __launch_bounds__(kA8Threads) act8_unpack_k(const int8_t* __rest
 // 1 / (1 + e^-g).  For 16-bit tensors the approximate exponential and
 // reciprocal, which err by 2^-22 of their value, and by the rounding of
 // g log2(e) in the exponent's argument (|g| 2^-24): far below a 16-bit
-// result's rounding.  Denormal results (g below -87) are zero.  32-bit tensors
-// take the accurate functions.
+// result's rounding.  They have no denormal results, but a bf16 product of a
+// gate down to -96 and such a sigmoid can be a normal number: both work 2^24
+// times up, in 2^-24 + e^-g 2^-24, and one multiplication takes that back.
+// 32-bit tensors take the accurate functions.
 template <int DT>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (DT == RQ_F32) return ieee_div(1.0f, 1.0f + expf(-g));
+  constexpr float up = DT == RQ_BF16 ? 24.0f : 0.0f, down = DT == RQ_BF16 ? 0x1p-24f : 1.0f;
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -1.4426950408889634f, -up)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(down + e));
+  return r * down;
 }
 
 // h = silu(g) u, with g and u (and h as it was rounded) packed in the same pass.
