@@ -3,7 +3,8 @@
 // loss (include/rq_b200.h).  As in torch_ops.cpp, outputs are allocated here,
 // launches go to torch's current stream of the input's device, a status other
 // than RQ_OK raises, and nothing is computed.  On Meta tensors the operators
-// only give shapes.
+// only give shapes; the public ones, at the end, call the others through the
+// dispatcher, so that tracing (FakeTensor, make_fx) sees those.
 #include "torch_ops.h"
 
 #include <torch/csrc/autograd/VariableTypeUtils.h>
@@ -87,15 +88,17 @@ void check_bank(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor
               "rocm_qlora: scaling must be a contiguous float32 tensor of one value an adapter");
 }
 
+void check_base(const Tensor& in, const Tensor& V, const Tensor& base) {
+  one_device(in, base);
+  check_rows(base, "base");
+  TORCH_CHECK(base.size(0) == in.size(0) && base.size(1) == V.size(1) && base.scalar_type() == in.scalar_type(),
+              "rocm_qlora: base must be [rows, ", V.size(1), "] of the input's dtype");
+}
+
 std::tuple<Tensor, Tensor> adapters_apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
                                           const optional<Tensor>& base, const optional<Tensor>& plan, int64_t tile) {
   check_bank(in, U, V, scaling, plan);
-  one_device(in, base);
-  if (base.has_value() && base->defined()) {
-    check_rows(*base, "base");
-    TORCH_CHECK(base->size(0) == in.size(0) && base->size(1) == V.size(1) && base->scalar_type() == in.scalar_type(),
-                "rocm_qlora: base must be [rows, ", V.size(1), "] of the input's dtype");
-  }
+  if (base.has_value() && base->defined()) check_base(in, V, *base);
   Tensor out = at::empty({in.size(0), V.size(1)}, in.options());
   Tensor mid = at::empty({in.size(0), U.size(2)}, in.options().dtype(at::kFloat));
   if (!in.is_meta()) apply(in, U, V, scaling, base, plan, tile, mid, out);
@@ -131,6 +134,16 @@ Tensor adapters_apply_versioned(c10::DispatchKeySet keys, Tensor out, const Tens
   }
   torch::autograd::increment_version(out);
   return mid;
+}
+
+// The output alone, for calls without a backward.
+Tensor adapters_product(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling, const Tensor& base,
+                        const optional<Tensor>& plan, int64_t tile) {
+  check_bank(in, U, V, scaling, plan);
+  check_base(in, V, base);
+  Tensor out = at::empty({in.size(0), V.size(1)}, in.options());
+  if (!in.is_meta()) apply(in, U, V, scaling, base, plan, tile, std::nullopt, out);
+  return out;
 }
 
 Tensor adapters_mid(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& scaling,
@@ -314,6 +327,17 @@ Tensor token_logprobs_grad(const Tensor& logits, const Tensor& labels, int64_t i
 // ---- the differentiable entry points: one dispatcher call forward, and a
 // backward that never enters Python
 
+// One of the operators above, through the dispatcher but for its autograd keys:
+// the nodes here are the gradients.
+template <auto F, class... A>
+auto via(const char* name, A&&... args) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<std::remove_pointer_t<decltype(F)>>();
+  const at::AutoDispatchBelowAutograd below;
+  return op.call(std::forward<A>(args)...);
+}
+#define RQ_VIA(op, ...) via<&op>("rocm_qlora::" #op, __VA_ARGS__)
+
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
@@ -337,7 +361,7 @@ struct AdaptersAdd : Function<AdaptersAdd> {
   static Tensor forward(AutogradContext* ctx, const Tensor& base, const Tensor& x, const Tensor& A, const Tensor& B,
                         const Tensor& scaling, const optional<Tensor>& plan, int64_t tile,
                         const optional<Tensor>& codes, const optional<Tensor>& scales) {
-    auto [y, mid] = adapters_apply(x, A, B, scaling, base, plan, tile);
+    auto [y, mid] = RQ_VIA(adapters_apply, x, A, B, scaling, base, plan, tile);
     const bool packed = codes.has_value();
     ctx->save_for_backward({packed ? *codes : x, packed ? *scales : Tensor(), A, B, scaling, mid, plan.value_or(Tensor())});
     ctx->saved_data["tile"] = tile;
@@ -351,10 +375,10 @@ struct AdaptersAdd : Function<AdaptersAdd> {
     const int64_t tile = ctx->saved_data["tile"].toInt();
     const Tensor dy = rows_of(grads[0]);
     Tensor dx, dA, dB, gmid;
-    if (ctx->needs_input_grad(1)) std::tie(dx, gmid) = adapters_apply(dy, B, A, scaling, std::nullopt, plan, tile);
-    else if (ctx->needs_input_grad(2)) gmid = adapters_mid(dy, B, A, scaling, plan, tile);
-    if (ctx->needs_input_grad(2)) dA = adapters_grad(z, scales, gmid, A.size(1), A.size(0), A.scalar_type(), plan, tile);
-    if (ctx->needs_input_grad(3)) dB = adapters_grad(dy, std::nullopt, mid, B.size(1), B.size(0), B.scalar_type(), plan, tile);
+    if (ctx->needs_input_grad(1)) std::tie(dx, gmid) = RQ_VIA(adapters_apply, dy, B, A, scaling, std::nullopt, plan, tile);
+    else if (ctx->needs_input_grad(2)) gmid = RQ_VIA(adapters_mid, dy, B, A, scaling, plan, tile);
+    if (ctx->needs_input_grad(2)) dA = RQ_VIA(adapters_grad, z, scales, gmid, A.size(1), A.size(0), A.scalar_type(), plan, tile);
+    if (ctx->needs_input_grad(3)) dB = RQ_VIA(adapters_grad, dy, std::nullopt, mid, B.size(1), B.size(0), B.scalar_type(), plan, tile);
     return {ctx->needs_input_grad(0) ? grads[0] : Tensor(), dx, dA, dB, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -430,15 +454,14 @@ Tensor adapters_add(const Tensor& base, const Tensor& x, const Tensor& A, const 
   if (grad) {
     y = AdaptersAdd::apply(b2, x2, a3, b3, s1, plan, tile, codes, scales);
   } else {  // serving: nothing is kept
-    y = at::empty({x2.size(0), b3.size(1)}, x2.options());
-    if (!x2.is_meta()) apply(x2, a3, b3, s1, b2, plan, tile, std::nullopt, y);
+    y = RQ_VIA(adapters_product, x2, a3, b3, s1, b2, plan, tile);
   }
   return base.dim() == 2 ? y : y.view(base.sizes());
 }
 
 struct Swiglu8 : Function<Swiglu8> {
   static variable_list forward(AutogradContext* ctx, const Tensor& gate, const Tensor& up, int64_t copies) {
-    auto [h, codes, scales] = swiglu8_forward(rows_of(gate), rows_of(up), copies);
+    auto [h, codes, scales] = RQ_VIA(swiglu8_forward, rows_of(gate), rows_of(up), copies);
     ctx->save_for_backward({codes, scales});  // a third copy (of h) is in the same storage in any case
     ctx->saved_data["shape"] = gate.sizes().vec();
     ctx->mark_non_differentiable({codes, scales});
@@ -450,7 +473,7 @@ struct Swiglu8 : Function<Swiglu8> {
     const auto v = ctx->get_saved_variables();
     const auto shape = ctx->saved_data["shape"].toIntVector();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    auto [dgate, dup] = swiglu8_backward(rows_of(grads[0]), v[0], v[1]);
+    auto [dgate, dup] = RQ_VIA(swiglu8_backward, rows_of(grads[0]), v[0], v[1]);
     return {dgate.view(shape), dup.view(shape), Tensor()};
   }
 };
@@ -472,21 +495,21 @@ std::tuple<Tensor, Tensor> pack_activation(const Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() >= 1, "pack_activation needs at least one dimension");
   check_float(x.scalar_type());
   check_gpu({&x});
-  return act8_pack(rows_of(x.detach()));
+  return RQ_VIA(act8_pack, rows_of(x.detach()));
 }
 
 Tensor unpack_activation(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, at::ScalarType dtype) {
   check_float(dtype);
   check_gpu({&codes, &scales});
   TORCH_CHECK_VALUE(!shape.empty(), "unpack_activation needs at least one dimension");
-  Tensor out = act8_unpack(codes, scales, shape.back(), dtype);
+  Tensor out = RQ_VIA(act8_unpack, codes, scales, shape.back(), dtype);
   return shape.size() == 2 ? out : out.view(shape);
 }
 
 struct Preference : Function<Preference> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& ref,
                                int64_t ignore, int64_t form, double beta, double smooth) {
-    auto [loss, logps, rewards, slopes, stats] = preference_forward(logits, labels, ref, ignore, form, beta, smooth);
+    auto [loss, logps, rewards, slopes, stats] = RQ_VIA(preference_forward, logits, labels, ref, ignore, form, beta, smooth);
     ctx->save_for_backward({logits, labels, stats, slopes});
     ctx->saved_data["ignore"] = ignore;
     ctx->mark_non_differentiable({logps, rewards});
@@ -498,7 +521,7 @@ struct Preference : Function<Preference> {
     const auto v = ctx->get_saved_variables();
     Tensor d;
     if (grads[0].defined())
-      d = token_logprobs_grad(v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], v[3], grads[0]);
+      d = RQ_VIA(token_logprobs_grad, v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], v[3], grads[0]);
     return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -530,7 +553,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits,
 
 struct LabelLogprobs : Function<LabelLogprobs> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, int64_t ignore) {
-    auto [logps, stats] = token_logprobs(logits, labels, ignore);
+    auto [logps, stats] = RQ_VIA(token_logprobs, logits, labels, ignore);
     ctx->save_for_backward({logits, labels, stats});
     ctx->saved_data["ignore"] = ignore;
     return logps;
@@ -538,7 +561,7 @@ struct LabelLogprobs : Function<LabelLogprobs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("token_logprobs");
     const auto v = ctx->get_saved_variables();
-    return {token_logprobs_grad(v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], grads[0].contiguous(), std::nullopt),
+    return {RQ_VIA(token_logprobs_grad, v[0], v[1], ctx->saved_data["ignore"].toInt(), v[2], grads[0].contiguous(), std::nullopt),
             Tensor(), Tensor()};
   }
 };
@@ -559,6 +582,7 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
   m.def(
       "adapters_apply_(Tensor(a!) out, Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor base, Tensor? plan, "
       "int tile) -> Tensor");
+  m.def("adapters_product(Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor base, Tensor? plan, int tile) -> Tensor");
   m.def("adapters_mid(Tensor inp, Tensor u, Tensor v, Tensor scaling, Tensor? plan, int tile) -> Tensor");
   m.def(
       "adapters_grad(Tensor z, Tensor? scales, Tensor mid, int columns, int count, ScalarType dtype, Tensor? plan, "
@@ -590,6 +614,7 @@ TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
   m.impl("adapter_plan", &adapter_plan);                     \
   m.impl("adapters_apply", &adapters_apply);                 \
   m.impl("adapters_apply_", &adapters_apply_);               \
+  m.impl("adapters_product", &adapters_product);             \
   m.impl("adapters_mid", &adapters_mid);                     \
   m.impl("adapters_grad", &adapters_grad);                   \
   m.impl("act8_pack", &act8_pack);                           \
