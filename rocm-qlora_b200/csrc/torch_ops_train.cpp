@@ -362,8 +362,10 @@ struct AdaptersAdd : Function<AdaptersAdd> {
                         const Tensor& scaling, const optional<Tensor>& plan, int64_t tile,
                         const optional<Tensor>& codes, const optional<Tensor>& scales) {
     auto [y, mid] = RQ_VIA(adapters_apply, x, A, B, scaling, base, plan, tile);
-    const bool packed = codes.has_value();
-    ctx->save_for_backward({packed ? *codes : x, packed ? *scales : Tensor(), A, B, scaling, mid, plan.value_or(Tensor())});
+    // x, or its packed form, is for A's gradient alone
+    const bool keep = A.requires_grad(), packed = codes.has_value();
+    ctx->save_for_backward({!keep ? Tensor() : packed ? *codes : x, keep && packed ? *scales : Tensor(), A, B, scaling,
+                            mid, plan.value_or(Tensor())});
     ctx->saved_data["tile"] = tile;
     return y;
   }

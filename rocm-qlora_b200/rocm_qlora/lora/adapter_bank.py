@@ -144,7 +144,8 @@ class _BankLinear(torch.autograd.Function):
         rows = x.reshape(-1, w.K).contiguous()
         y = layer_ops.forward(w, rows, bias.to(x.dtype).contiguous() if bias is not None else None, None, None, 1.0)
         mid = ops.adapters_apply_(y, rows, A, B, scaling, y, data, tile)
-        ctx.save_for_backward(*((rows, None) if codes is None else (codes, scales)), A, B, scaling, mid, data)
+        z = (None, None) if not ctx.needs_input_grad[1] else (rows, None) if codes is None else (codes, scales)
+        ctx.save_for_backward(*z, A, B, scaling, mid, data)
         ctx.w, ctx.tile, ctx.shape = w, tile, x.shape
         return y.view(*x.shape[:-1], w.N)
 
@@ -155,7 +156,7 @@ class _BankLinear(torch.autograd.Function):
         w, tile = ctx.w, ctx.tile
         need_x, need_A, need_B = ctx.needs_input_grad[:3]
         rows = dy.reshape(-1, w.N).contiguous()
-        ops = nat.require_ops(dy, A)
+        ops = nat.require_ops(rows, A)
         dx = dA = dB = None
         if need_x:
             dx = layer_ops.dx(w, rows, None, None, 1.0)
