@@ -130,7 +130,7 @@ static int check_plan(int64_t rows, int count, int tile, const int32_t* plan, in
 static int check_tokens(const void* logits, int dt, int64_t B, int64_t L, int64_t V, const int64_t* labels,
                         const float* stats) {
   if (!dtype_ok(dt)) return RQ_ERR_DTYPE;
-  if (B < 0 || L < 0 || V < 1 || !fits(V) || (L > 0 && !fits(B * L))) return RQ_ERR_INVALID;
+  if (V < 1 || !fits(V) || !fits(B) || !fits(L) || !fits(B * L)) return RQ_ERR_INVALID;
   if (B * L > 0 && (!logits || !labels || !stats)) return RQ_ERR_INVALID;
   if ((uintptr_t)logits % dtype_size(dt) || (uintptr_t)labels % 8 || (uintptr_t)stats % 16) return RQ_ERR_ALIGN;
   return RQ_OK;
