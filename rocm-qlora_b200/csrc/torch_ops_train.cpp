@@ -47,6 +47,12 @@ void check_plan(const optional<Tensor>& plan) {
               "rocm_qlora: plan must be a contiguous 1-D int32 tensor, as adapter_plan makes it");
 }
 
+// The kernels read banks and codes in 16-byte pieces: a view that starts
+// between two of them is copied.
+Tensor aligned(const Tensor& t) {
+  return t.is_meta() || (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 Tensor adapter_plan(const Tensor& ids, int64_t count, int64_t tile) {
   TORCH_CHECK(ids.dim() == 1 && ids.is_contiguous() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
               "rocm_qlora: ids must be a contiguous 1-D int64 or int32 tensor");
@@ -66,7 +72,8 @@ void apply(const Tensor& in, const Tensor& U, const Tensor& V, const Tensor& sca
            const optional<Tensor>& plan, int64_t tile, const optional<Tensor>& mid, const optional<Tensor>& out) {
   const c10::cuda::CUDAGuard guard(in.device());
   const bool has_base = base.has_value() && base->defined(), has_plan = plan.has_value() && plan->defined();
-  check(rq_adapters_apply(in.data_ptr(), in.stride(0), U.data_ptr(), V.data_ptr(), scaling.data_ptr<float>(), ptr(base),
+  const Tensor u = aligned(U), v = aligned(V);
+  check(rq_adapters_apply(in.data_ptr(), in.stride(0), u.data_ptr(), v.data_ptr(), scaling.data_ptr<float>(), ptr(base),
                           has_base ? base->stride(0) : 0, in.size(0), in.size(1), out ? out->size(1) : 0,
                           (int)U.size(2), (int)U.size(0), dtype_code(in.scalar_type()),
                           static_cast<const int32_t*>(ptr(plan)), has_plan ? plan->numel() : 0, (int)tile,
@@ -170,7 +177,8 @@ Tensor adapters_grad(const Tensor& z, const optional<Tensor>& scales, const Tens
   Tensor grad = at::empty({count, D, mid.size(1)}, z.options().dtype(dtype));
   if (z.is_meta()) return grad;
   const c10::cuda::CUDAGuard guard(z.device());
-  check(rq_adapters_grad(z.data_ptr(), z.stride(0), static_cast<const float*>(ptr(scales)), mid.data_ptr<float>(),
+  const Tensor rows = packed ? aligned(z) : z;
+  check(rq_adapters_grad(rows.data_ptr(), rows.stride(0), static_cast<const float*>(ptr(scales)), mid.data_ptr<float>(),
                          z.size(0), D, (int)mid.size(1), (int)count, dtype_code(dtype),
                          static_cast<const int32_t*>(ptr(plan)), has_plan ? plan->numel() : 0, (int)tile,
                          grad.data_ptr(), stream_of(z)),
@@ -210,7 +218,7 @@ Tensor act8_unpack(const Tensor& codes, const Tensor& scales, int64_t K, at::Sca
   Tensor out = at::empty({codes.size(0), K}, codes.options().dtype(dtype));
   if (codes.is_meta()) return out;
   const c10::cuda::CUDAGuard guard(codes.device());
-  check(rq_act8_unpack(codes.data_ptr<int8_t>(), scales.data_ptr<float>(), codes.size(0), K, out.data_ptr(),
+  check(rq_act8_unpack(aligned(codes).data_ptr<int8_t>(), scales.data_ptr<float>(), codes.size(0), K, out.data_ptr(),
                        dtype_code(dtype), stream_of(codes)),
         "rq_act8_unpack");
   return out;
