@@ -174,10 +174,11 @@ __device__ __noinline__ void wide_row(const typename DType<DT>::T* x, int V, flo
 // bound by HBM, with the exponentials (16 a clock of an SM) at 72 % of the
 // time a bf16 row takes to arrive.  The end of a row is a few serial steps, so
 // where rows are many, small CTAs of which eight share an SM hide it: 16384
-// rows of 32000 bf16 logits (14792 count) take 155 us with 128 threads (6.1
-// TB/s) and 244 with 512, but 128 rows 5.8 and 4.6 us.
+// rows of 32000 bf16 logits (14792 count) take 159 us with 128 threads (6.0
+// TB/s; nine CTAs an SM, with eight 166) and 256 with 512, but 128 rows 6.3
+// and 4.9 us.
 template <int DT, int TH>
-__global__ void __launch_bounds__(TH, 1024 / TH) token_stats_k(TokenRows t, float4* __restrict__ stats,
+__global__ void __launch_bounds__(TH, TH == 128 ? 9 : 2) token_stats_k(TokenRows t, float4* __restrict__ stats,
                                                              float* __restrict__ logps) {
   grid_begin();
   using T = typename DType<DT>::T;
