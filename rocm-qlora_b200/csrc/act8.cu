@@ -278,14 +278,13 @@ __device__ __forceinline__ float sigmoid(float g) {
 }
 
 // h = silu(g) u, with g and u (and h as it was rounded) packed in the same pass.
-// 16-bit: six CTAs an SM, 40 registers (149 us; 155 with the 44 that it would
-// take).
+// Six CTAs an SM, 40 registers (16-bit 149 us; 155 with the 44 that it would
+// take), fewer where fp32 values need more.
 template <int DT, bool VEC, int COPIES>
-__global__ void __launch_bounds__(kA8Threads, DT == RQ_F32 ? 1 : 6) swiglu8_forward_k(const void* __restrict__ g, int64_t ldg,
-                                                                const void* __restrict__ u, int64_t ldu,
-                                                                uint32_t blocks, int K, Divide nb,
-                                                                void* __restrict__ h, int8_t* __restrict__ codes,
-                                                                float* __restrict__ scales) {
+__global__ void __launch_bounds__(kA8Threads, DT != RQ_F32 || (VEC && COPIES == 2) ? 6 : VEC ? 5 : 4)
+    swiglu8_forward_k(const void* __restrict__ g, int64_t ldg, const void* __restrict__ u, int64_t ldu,
+                      uint32_t blocks, int K, Divide nb, void* __restrict__ h, int8_t* __restrict__ codes,
+                      float* __restrict__ scales) {
   grid_begin();
   using T = typename DType<DT>::T;
   Place8 p;
