@@ -887,8 +887,8 @@ static int launch_apply(const ApplyArgs& p, bool vec, int64_t tiles, cudaStream_
   if (rc != RQ_OK) return rc;
   // The cluster size of the least time: rounds of the GPU, each about 6 us of
   // fixed cost and 1e-4 us a value of a CTA's share of in, base and out (8192
-  // rows, 4096 x 4096, rank 16, tiles of 128: 47 us with 4, 50 with 8, 65
-  // with 2).
+  // rows, 4096 x 4096, rank 16, tiles of 128: 46 us with 4, 53 with 8, 58
+  // with 2; rank 64 74, 85 and 91).
   const int* resident = l.resident();
   const double expected = (double)p.a.M / p.a.tile + (p.a.plan ? 0.5 * p.a.count : 0.0);
   const double work = 1e-4 * p.a.tile * ((double)p.a.D1 + 2.0 * p.a.D2);
@@ -1015,10 +1015,7 @@ __device__ __forceinline__ int sum_rows(const GradArgs& p, int2 places, int bloc
   constexpr int ROW = gr_row_bytes(CODES), PITCH = gr_mid_pitch(RG), STEP = gr_step_bytes(CODES, RG);
   constexpr int S = gr_steps(CODES, VEC, RG);
   constexpr bool CONV = CODES && RG > 1;        // codes become 16-bit once for all warps of a group
-  // m-tiles at a time: two put four sums between two products of one sum; with
-  // one warp a ring the registers for that are not there (22 against 25 us at
-  // 8192 rows, 4096 columns, rank 16)
-  constexpr int PAIR = RG == 1 && !CODES ? 1 : 2;
+  constexpr int PAIR = 2;                       // m-tiles at a time: four sums between two products of one sum
   constexpr int TR = 2 * RG;                    // threads of a group that fetch one row
   constexpr int PIECES = (ROW / 16 + TR - 1) / TR;  // 16-byte pieces of it each
   extern __shared__ __align__(16) unsigned char smem[];
