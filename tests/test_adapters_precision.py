@@ -61,3 +61,23 @@ def test_bank_gradients(rows, k, count, rank, dtype):
     got = ops.adapters_grad(p.codes, p.scales, mid, k, count, dtype, plan.data, plan.tile)
     # each row's 127 * (mid / 127) rounds twice: the scale, the product
     assert bool(((got[0].double() - SMALL).abs() <= 2.0 ** -21).all()), float(got[0].max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [8, 32, 64, 128])
+@pytest.mark.parametrize("rows,k", [(4200, 22016), (4200, 22015), (1000, 22016)])
+def test_sums_of_long_rows_are_not_shifted(rows, k, rank, dtype):
+    """Positive products: a tensor core cuts its sum off at each step, half of 2^-23 of it on average at most, and
+    a run of 16 steps between two rounded additions therefore shifts it by 2^-20 at most."""
+    from rocm_qlora import _native as nat
+    ops = nat.loaded_ops()
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    x = torch.rand(rows, k, generator=g, device="cuda").to(dtype)
+    U = torch.rand(1, k, rank, generator=g, device="cuda").div(64).to(dtype)
+    mid = ops.adapters_mid(x, U, torch.zeros(1, 8, rank, device="cuda", dtype=dtype), torch.ones(1, device="cuda"), None, 0)
+    shift = []
+    for at in range(0, rows, 700):
+        want = x[at:at + 700].double() @ U[0].double()
+        shift.append(((mid[at:at + 700].double() - want) / want).mean())
+    assert abs(float(torch.stack(shift).mean())) <= 2.0 ** -20
