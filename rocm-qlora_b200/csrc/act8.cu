@@ -10,9 +10,9 @@
 // Everything here is one pass over the data.  16 lanes hold a block (8 values
 // a lane: one 16-byte load of a 16-bit type), so the block's maximum is four
 // shuffles.  Measured (bf16, 8192 x 11008): swiglu8 forward with three copies
-// 147 us, 5.5 TB/s (issue bound, 76 % of the slots: the encoding), backward
-// 115 us, 6.3 TB/s, and unpack 49 us, 5.5 TB/s (HBM); pack of 8192 x 4096 22
-// us, 4.6 TB/s.
+// 149 us, 5.4 TB/s (issue bound, 76 % of the slots: the encoding), backward
+// 115 us, 6.3 TB/s, and unpack 49 us, 5.5 TB/s (HBM); pack of 8192 x 4096 21
+// us, 4.7 TB/s; fp32, 4096 x 11008, forward 108 us, 6.3 TB/s, backward 94, 6.7.
 #include <cuda_runtime.h>
 
 #include "linear_common.cuh"

@@ -490,10 +490,10 @@ __device__ __noinline__ void tile_by_value(const ApplyRows& at, const unsigned c
 // are permuted the same way among the MMA's n index, so that a lane ends with
 // 8 consecutive output columns: one 16-byte load of base and one store.
 //
-// Measured (bf16): one row of 4096 to 4096, rank 16, 5.9 us (a launch and a
-// chain of five dependent loads); 8192 rows, 45 us, 4.4 TB/s of the 201 MB
+// Measured (bf16): one row of 4096 to 4096, rank 16, 6.1 us (a launch and a
+// chain of five dependent loads); 8192 rows, 46 us, 4.3 TB/s of the 201 MB
 // (31 us at the copy bandwidth; launch, plan, meeting and sums are the rest);
-// rank 64, 76 us: the three pieces of mid on mma.sync.  fp16 rows of 1093 to
+// rank 64, 74 us, the tensor pipe 40 % active: the three pieces of mid.  fp16 rows of 1093 to
 // 1088, rank 64, 1111 of them: 14 us.
 template <int DT, int R, int NW, bool VEC>
 __global__ void __launch_bounds__(kApThreads, R <= 64 ? 2 : 1) adapters_apply_k(const __grid_constant__ ApplyArgs p) {
@@ -1255,8 +1255,8 @@ __device__ __forceinline__ bool group_any(int mw, bool v) {
 // enters as 16-bit pieces as in the row products.
 //
 // Bound by HBM in the limit; what a CTA costs besides its rows (sums, the
-// meetings) is what is seen: 64 MB of z at rank 16 take 22 us, 32 MB of codes
-// 22; rank 64 59 and 66 us, where four warps a group share the rows and the
+// meetings) is what is seen: 64 MB of z at rank 16 take 24 us, 32 MB of codes
+// 22; rank 64 61 and 64 us, where four warps a group share the rows and the
 // three pieces of mid are mma.sync's work.
 template <int DT, bool CODES, bool VEC, int RG, int MW, bool LARGE>
 __device__ __forceinline__ void adapter_gradient(const GradArgs& p) {
@@ -1391,12 +1391,14 @@ static int grad_cluster(const int* resident, int64_t blocks, int64_t count, int6
 
 // For many adapters of few rows most groups of a CTA of 8 warps have none: they
 // take CTAs of one group, of which up to 16 share an SM: 64 rows of 32 adapters,
-// 11008 columns, rank 16, 10 us against 38; 8192 rows of 64, 4096
-// columns, rank 16 27 against 52, rank 64 47 against 82.  The host does not
+// 11008 columns, rank 16, 10 us against 43; 8192 rows of 64, 4096
+// columns, rank 16 31 against 57, rank 64 55 against 90.  The host does not
 // know how the rows are spread, and an adapter of most of them would keep its
-// one group for long (all 8192 rows, rank 16: 457 us): those of more than 4
+// one group for long (all 8192 rows, rank 16: 509 us): those of more than 4
 // times the mean and 64 rows, no more than M / most of them, go to CTAs of 8
-// warps in a launch beside (74 us; 69 where all adapters have such CTAs).
+// warps in a launch beside.  Half of the rows on one adapter, and all: rank 16
+// 62 and 90 us (66 and 85 where all adapters have such CTAs), rank 64 142 and
+// 218 (164 and 286).
 template <int DT, bool CODES, bool VEC, int RG>
 static int launch_grad(const GradArgs& p, int64_t blocks, cudaStream_t st) {
   const int64_t M = p.a.M, count = p.a.count, each = (M + count - 1) / count;

@@ -98,12 +98,13 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``base + scaling * (x @ A) @ B.T`` per row with the row's own adapter.
 
-    base [..., N] and x [..., K] (bfloat16 or float16, rows may be strided),
-    A [count, K, rank], B [count, N, rank] (contiguous), scaling [count]
-    float32; ``plan`` may be None for a bank of one.  Products are accumulated
-    in 32 bits and the sum is rounded once.  With ``packed_x`` (the packed
-    form of x) the backward of A reads it and x is not kept.  ``out`` (no
-    gradients then) takes the result and may be ``base`` itself."""
+    base [..., N] and x [..., K] (bfloat16 or float16, rows may be strided or
+    expanded), A [count, K, rank], B [count, N, rank] (contiguous), scaling
+    [count] float32; ``plan`` may be None for a bank of one.  All on one
+    device.  Products are accumulated in 32 bits and the sum is rounded once.
+    With ``packed_x`` (the packed form of x) the backward of A reads it and x
+    is not kept.  Differentiable once, in reverse mode.  ``out`` (no gradients
+    then) takes the result and may be ``base`` itself."""
     args = (plan.data, plan.rows, plan.count, plan.tile) if plan is not None else (None, 0, 0, 0)
     if packed_x is not None:
         _packed_args(packed_x, x)
@@ -174,7 +175,7 @@ class _BankLinear(torch.autograd.Function):
 def bank_linear(x: torch.Tensor, w: layer_ops.WeightView, bias: Optional[torch.Tensor], A: torch.Tensor,
                 B: torch.Tensor, scaling: torch.Tensor, plan: Optional[AdapterPlan] = None,
                 packed_x: Optional[PackedActivation] = None) -> torch.Tensor:
-    """``adapters_add`` onto ``x @ deq(w).T + bias``."""
+    """``adapters_add`` onto ``x @ deq(w).T + bias``, which is rounded to x's dtype first."""
     _check_bank(x, A, B, scaling)
     if x.shape[-1] != w.K or A.shape[1] != w.K or B.shape[1] != w.N:
         raise ValueError(f"x {tuple(x.shape)}, A {tuple(A.shape)} and B {tuple(B.shape)} do not fit a "

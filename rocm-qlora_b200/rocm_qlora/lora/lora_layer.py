@@ -57,7 +57,9 @@ class LoRALinear(nn.Module):
         """base_output + (dropout(x) @ A.T @ B.T * scaling).  With ``packed_x``
         (``activation8.pack_activation`` of x, shared by the layers that read
         x) training keeps that in x's place: the gradient of lora_A is of the
-        packed values, everything else is of x."""
+        packed values, everything else is of x.  The adapter's product is then
+        accumulated in 32 bits and rounded once with the base's rounded output,
+        instead of the reference's rounding of each intermediate."""
         if packed_x is not None and not self.merged:
             return self._forward_packed(x, packed_x)
         if self.merged:
