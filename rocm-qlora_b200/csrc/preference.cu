@@ -351,9 +351,11 @@ __global__ void __launch_bounds__(kPrefWarps * 32) __cluster_dims__(kPrefCtas, 1
 }
 
 // dlogits = c ([v = y] - 2^(x log2(e) - k) / s), zero where the row does not
-// count; of a wide row e^(x - m) / s.  One CTA a row, the rows in the reverse of the forward's order, so
-// that the last rows it read are still in L2.  HBM bound: 301 us for 16384
-// rows of 32000 bf16 logits of which 14792 count, 6.6 TB/s.
+// count; of a wide row e^(x - m) / s.  The approximate exponential errs by
+// 2^-22 of a probability: fp32 gradients are 3.8e-7 of their norm off, 3.7e-7
+// with torch's 32-bit operations.  One CTA a row, the rows in the reverse of the
+// forward's order, so that the last rows it read are still in L2.  HBM bound:
+// 301 us for 16384 rows of 32000 bf16 logits of which 14792 count, 6.6 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(kTokThreads) token_grad_k(TokenRows t, const float4* __restrict__ stats,
                                                             const float* __restrict__ slopes, int per_token,
