@@ -1,0 +1,514 @@
+// adamw.cu -- an AdamW step over many tensors in one launch, with the gradient
+// norm that clips it, and moments held in 32 or in 8 bits.
+//
+//   g = c grad                       c = min(1, max_norm / (norm + 1e-6)), or 1
+//   m = b1 m + (1 - b1) g            v = b2 v + (1 - b2) g g
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// A tensor's values are cut into blocks of 256 (the last one short); the
+// moments of all tensors lie in one arena of whole blocks.  A warp takes a
+// block, 8 values a lane.  Three launches, each the programmatic dependent of
+// the one before: the norm's partial sums (where it clips), one CTA that ends
+// the norm, counts the steps and forms each tensor's factors, and the update.
+//
+// Moments in 8 bits, per block:
+//   m          e4m3 codes of m (448 / max|m|), scale max|m| / 448
+//   sqrt(v)    codes of 4 exponent and 4 mantissa bits (the whole numbers up to
+//              31, then 16 steps to a power of two, up to 31 2^14) of
+//              r (507904 / max r), scale max r / 507904; r > 0 never becomes 0,
+//              which would make the next quotient unbounded.
+// The root has half of v's range, and no sign bit is spent on it.  Maxima
+// below 2^-100 are stored as zeros, an infinity or NaN makes the scale NaN.
+// The parameters are updated with the moments as they were before rounding.
+// Products and sums of the moments are rounded one by one (no fused
+// multiply-add), so that a code is what the formula in 32 bits gives.
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "gemv_common.cuh"
+#include "linear_common.cuh"
+
+namespace rq {
+
+constexpr int kAdBlock = RQ_ADAM_BLOCK, kAdThreads = 256, kAdWarps = kAdThreads / 32;
+constexpr float kMTop = 448.0f, kRTop = 507904.0f;
+
+// The tensors of a launch, as kernel parameters (32 KB at most): nothing is
+// copied to the device beforehand, and a captured launch keeps them.
+template <int MAX>
+struct AdTensors {
+  void* p[MAX];
+  const void* g[MAX];
+  uint32_t first[MAX + 1];  // launch-wide number of a tensor's first block; [count]: blocks in all
+  uint32_t block[MAX];      // its first block in the arena
+  uint16_t slot[MAX];       // its place among the steps and factors
+  uint16_t tail[MAX];       // values of its last block
+  int count;
+};
+constexpr int kAdSmall = 64, kAdLarge = RQ_ADAM_TENSORS;
+static_assert(sizeof(AdTensors<kAdLarge>) <= 31 * 1024, "kernel parameters end at 32764 bytes");
+
+// The tensor that holds launch-wide block b.
+template <int MAX>
+__device__ __forceinline__ int tensor_of(const AdTensors<MAX>& t, uint32_t b) {
+  int lo = 0, hi = t.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (t.first[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A CTA's share of the blocks: side by side, so that one search finds the
+// first tensor and the next ones follow.
+__device__ __forceinline__ void share(uint32_t blocks, uint32_t& b, uint32_t& end) {
+  b = (uint32_t)((uint64_t)blocks * blockIdx.x / gridDim.x);
+  end = (uint32_t)((uint64_t)blocks * (blockIdx.x + 1) / gridDim.x);
+}
+
+// 8 values at `at`, of which the first `n` exist (the others 0); VEC: all, and aligned.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8f(const void* p, int64_t at, int n, float (&v)[8]) {
+  using T = typename DType<DT>::T;
+  const T* from = static_cast<const T*>(p) + at;
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? DType<DT>::to_f32(from[i]) : 0.0f;
+  } else if constexpr (DT == RQ_F32) {
+    *reinterpret_cast<float4*>(v) = reinterpret_cast<const float4*>(from)[0];
+    *reinterpret_cast<float4*>(v + 4) = reinterpret_cast<const float4*>(from)[1];
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(from);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == RQ_BF16) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8f(void* p, int64_t at, int n, const float (&v)[8]) {
+  using T = typename DType<DT>::T;
+  T* to = static_cast<T*>(p) + at;
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) to[i] = DType<DT>::from_f32(v[i]);
+  } else if constexpr (DT == RQ_F32) {
+    reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
+    reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
+  } else {
+    *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
+                                               pack2<DT>(v[6], v[7]));
+  }
+}
+
+// ------------------------------------------------------------------ norm
+
+// Sums of squares in 64 bits: any order of the sums gives the same 32-bit
+// norm but for ties of the last rounding, and no square leaves the range.
+template <int DT, bool VEC>
+__device__ __forceinline__ double squares8(const void* g, int64_t at, int n) {
+  float v[8];
+  load8f<DT, VEC>(g, at, n, v);
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fma((double)v[i], (double)v[i], s);
+  return s;
+}
+
+template <int DT, int MAX>
+__global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_constant__ AdTensors<MAX> t,
+                                                             double* __restrict__ partials) {
+  grid_begin();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  uint32_t b, end;
+  share(t.first[t.count], b, end);
+  b += warp;
+  double sum = 0.0;
+  int i = b < end ? tensor_of(t, b) : 0;
+  for (; b < end; b += kAdWarps) {
+    while (b >= t.first[i + 1]) ++i;
+    const uint32_t in = b - t.first[i];
+    const bool last = b + 1 == t.first[i + 1];
+    const int n = (last ? t.tail[i] : kAdBlock) - lane * 8;
+    const int64_t at = (int64_t)in * kAdBlock + lane * 8;
+    const bool vec = (uintptr_t)t.g[i] % 16 == 0 && (!last || t.tail[i] == kAdBlock);
+    sum += vec ? squares8<DT, true>(t.g[i], at, n) : squares8<DT, false>(t.g[i], at, n);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __shared__ double part[kAdWarps];
+  if (lane == 0) part[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int w = 0; w < kAdWarps; ++w) s += part[w];
+    partials[blockIdx.x] = s;
+  }
+  // what the caller sums has RQ_NORM_PARTIALS values whatever the grid
+  if (blockIdx.x == 0)
+    for (int j = gridDim.x + threadIdx.x; j < RQ_NORM_PARTIALS; j += kAdThreads) partials[j] = 0.0;
+}
+
+// Sum of the partial sums, by one CTA in a fixed order; every thread gets it.
+__device__ __forceinline__ double sum_partials(const double* partials, int n) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kAdThreads) s += partials[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __shared__ double part[kAdWarps];
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int w = 0; w < kAdWarps; ++w) s += part[w];
+  return s;
+}
+
+__global__ void __launch_bounds__(kAdThreads) norm_end_k(const double* __restrict__ partials, int n,
+                                                         float* __restrict__ norm) {
+  grid_begin();
+  const double s = sum_partials(partials, n);
+  if (threadIdx.x == 0) *norm = (float)sqrt(s);
+}
+
+// ---------------------------------------------------------------- factors
+
+struct AdSlots {
+  uint16_t slot[kAdLarge];
+  int count;
+};
+struct AdFactors {
+  double lr, decay, log_beta1, log_beta2;  // log 0 = -inf: the first moment is the gradient itself
+  const float* lr_at;                      // learning rate on the device, or null
+  float max_norm;
+};
+
+// One CTA: ends the norm, counts each tensor's step t and writes its factors
+//   x = lr / (1 - b1^t), y = 1 / sqrt(1 - b2^t), z = 1 - lr wd, w = c.
+// 1 - b^t is -expm1(t log b), in 64 bits.
+__global__ void __launch_bounds__(kAdThreads) adam_begin_k(const __grid_constant__ AdSlots s, AdFactors f,
+                                                           const double* __restrict__ partials, int n_partials,
+                                                           float* __restrict__ norm, int32_t* __restrict__ steps,
+                                                           float4* __restrict__ factors) {
+  grid_begin();
+  float c = 1.0f;
+  if (n_partials > 0) {
+    const float total = (float)sqrt(sum_partials(partials, n_partials));
+    if (threadIdx.x == 0) *norm = total;
+    const float quotient = __fmul_rn(ieee_div(1.0f, __fadd_rn(total, 1e-6f)), f.max_norm);
+    c = quotient > 1.0f ? 1.0f : quotient;  // a NaN stays one
+  }
+  const double lr = f.lr_at ? (double)*f.lr_at : f.lr;
+  for (int i = threadIdx.x; i < s.count; i += kAdThreads) {
+    const int t = steps[s.slot[i]] + 1;
+    steps[s.slot[i]] = t;
+    const double c1 = -expm1(t * f.log_beta1), c2 = -expm1(t * f.log_beta2);
+    factors[s.slot[i]] = make_float4((float)(lr / c1), (float)(1.0 / sqrt(c2)), (float)(1.0 - lr * f.decay), c);
+  }
+}
+
+// ------------------------------------------------------- moments in 8 bits
+
+// The root's code of a value t in [0, kRTop]: a float of 4 exponent and 4
+// mantissa bits, whose first 16 codes are the numbers 0 to 15.  Ties to even.
+__device__ __forceinline__ uint32_t root_code(float t) {
+  const uint32_t bits = __float_as_uint(t);
+  const uint32_t high = ((bits + 0x3ffffu + ((bits >> 19) & 1u)) >> 19) - (130u << 4);
+  const uint32_t low = __float_as_uint(__fadd_rn(t, 12582912.0f)) & 0xffu;  // 1.5 2^23: rounds to a whole number
+  return t < 16.0f ? low : high;
+}
+__device__ __forceinline__ float root_value(uint32_t c) {
+  const bool low = c < 16u;
+  const float v = __uint_as_float(((low ? c + 16u : c) << 19) + (130u << 23));
+  return low ? v - 16.0f : v;
+}
+
+// A block's scales: what its values are multiplied by on the way to codes
+// (0: all codes are 0) and on the way back.
+struct Scale8 {
+  float to, from;
+};
+__device__ __forceinline__ Scale8 scale8(uint32_t top_bits, float most) {
+  const float top = __uint_as_float(top_bits);
+  Scale8 s;
+  const bool live = top >= 0x1p-100f, bad = top_bits >= 0x7f800000u;
+  s.to = live && !bad ? ieee_div(most, top) : 0.0f;
+  s.from = bad ? __uint_as_float(0x7fc00000u) : live ? ieee_div(top, most) : 0.0f;
+  return s;
+}
+
+// Largest magnitude of the warp's values as a bit pattern, in which an
+// infinity or NaN is the largest.
+__device__ __forceinline__ uint32_t warp_top(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+__device__ __forceinline__ void decode_moments(const uint8_t* codes_m, const uint8_t* codes_r, float2 scale,
+                                               int64_t at, float (&m)[8], float (&v)[8]) {
+  const uint2 cm = *reinterpret_cast<const uint2*>(codes_m + at), cr = *reinterpret_cast<const uint2*>(codes_r + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1));
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    m[2 * i] = __fmul_rn(f.x, scale.x);
+    m[2 * i + 1] = __fmul_rn(f.y, scale.x);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = __fmul_rn(root_value(((i < 4 ? cr.x : cr.y) >> (8 * (i & 3))) & 0xffu), scale.y);
+    v[i] = __fmul_rn(r, r);
+  }
+}
+
+// m and r = sqrt(v) of a whole warp's block to codes and scales.
+__device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&r)[8], int64_t block, int lane,
+                                               uint8_t* codes_m, uint8_t* codes_r, float2* scales) {
+  uint32_t tm = 0, tr = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    tm = max(tm, __float_as_uint(m[i]) & 0x7fffffffu);
+    tr = max(tr, __float_as_uint(r[i]) & 0x7fffffffu);
+  }
+  const Scale8 sm = scale8(warp_top(tm), kMTop), sr = scale8(warp_top(tr), kRTop);
+  if (lane == 0) scales[block] = make_float2(sm.from, sr.from);
+  uint32_t cm[4], cr[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    cm[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[2 * i], sm.to), __fmul_rn(m[2 * i + 1], sm.to)),
+                                     __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t c = root_code(__fmul_rn(r[i], sr.to));
+    cr[i / 4] |= (r[i] > 0.0f && sr.to > 0.0f ? max(c, 1u) : 0u) << (8 * (i & 3));
+  }
+  const int64_t at = block * kAdBlock + lane * 8;
+  *reinterpret_cast<uint2*>(codes_m + at) = make_uint2(cm[0] | cm[1] << 16, cm[2] | cm[3] << 16);
+  *reinterpret_cast<uint2*>(codes_r + at) = make_uint2(cr[0], cr[1]);
+}
+
+// ------------------------------------------------------------------ update
+
+struct AdState {
+  void* m;           // fp32 [blocks * 256], or codes
+  void* v;
+  float2* scales;    // 8 bits: [blocks] (m, root)
+  int16_t* low;      // what bf16 parameters leave of a 32-bit value, or null
+  const float4* factors;
+  float beta1, rest1, beta2, rest2, eps;
+};
+
+template <int DT, bool VEC, bool EIGHT, bool LOW>
+__device__ __forceinline__ void update8(void* p, const void* g, int64_t at, int n, int64_t block, int lane,
+                                        const float4& f, const AdState& a) {
+  const int64_t sat = block * kAdBlock + lane * 8;
+  float gv[8], pv[8], m[8], v[8];
+  load8f<DT, VEC>(g, at, n, gv);
+  load8f<DT, VEC>(p, at, n, pv);
+  uint32_t low[4] = {};
+  if constexpr (LOW) {
+    const uint4 w = *reinterpret_cast<const uint4*>(a.low + sat);
+    low[0] = w.x, low[1] = w.y, low[2] = w.z, low[3] = w.w;
+  }
+  if constexpr (EIGHT) {
+    decode_moments(static_cast<const uint8_t*>(a.m), static_cast<const uint8_t*>(a.v), a.scales[block], sat, m, v);
+  } else {
+    load8f<RQ_F32, true>(a.m, sat, 8, m);
+    load8f<RQ_F32, true>(a.v, sat, 8, v);
+  }
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = __fmul_rn(gv[i], f.w);
+    m[i] = __fadd_rn(__fmul_rn(m[i], a.beta1), __fmul_rn(x, a.rest1));
+    v[i] = __fadd_rn(__fmul_rn(v[i], a.beta2), __fmul_rn(__fmul_rn(x, x), a.rest2));
+    r[i] = __fsqrt_rn(v[i]);
+    if constexpr (LOW) {
+      const int16_t l = (int16_t)(low[i / 2] >> (16 * (i & 1)));
+      pv[i] = __uint_as_float(__float_as_uint(pv[i]) + (uint32_t)(int32_t)l);
+    }
+    pv[i] = pv[i] * f.z - f.x * __fdividef(m[i], r[i] * f.y + a.eps);
+  }
+  if constexpr (LOW) {
+    // The 32-bit value's upper half as bf16, rounded half away from zero so
+    // that what is left fits 16 bits with its sign.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t bits = __float_as_uint(pv[2 * i + h]);
+        const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+        const uint32_t top = finite ? (bits + 0x8000u) & 0xffff0000u : (bits & 0x7fffffu) ? 0x7fc00000u : bits;
+        w |= ((finite ? bits - top : 0u) & 0xffffu) << (16 * h);
+        pv[2 * i + h] = __uint_as_float(top);
+      }
+      low[i] = w;
+    }
+    *reinterpret_cast<uint4*>(a.low + sat) = make_uint4(low[0], low[1], low[2], low[3]);
+  }
+  store8f<DT, VEC>(p, at, n, pv);
+  if constexpr (EIGHT) {
+    encode_moments(m, r, block, lane, static_cast<uint8_t*>(a.m), static_cast<uint8_t*>(a.v), a.scales);
+  } else {
+    store8f<RQ_F32, true>(a.m, sat, 8, m);
+    store8f<RQ_F32, true>(a.v, sat, 8, v);
+  }
+}
+
+template <int DT, bool EIGHT, bool LOW, int MAX>
+__global__ void __launch_bounds__(kAdThreads) adam_update_k(const __grid_constant__ AdTensors<MAX> t, const AdState a) {
+  grid_begin();
+  const int lane = threadIdx.x % 32;
+  uint32_t b, end;
+  share(t.first[t.count], b, end);
+  b += threadIdx.x / 32;
+  int i = b < end ? tensor_of(t, b) : 0;
+  for (; b < end; b += kAdWarps) {
+    while (b >= t.first[i + 1]) ++i;
+    const uint32_t in = b - t.first[i];
+    const bool last = b + 1 == t.first[i + 1];
+    const int n = (last ? t.tail[i] : kAdBlock) - lane * 8;
+    const int64_t at = (int64_t)in * kAdBlock + lane * 8, block = (int64_t)t.block[i] + in;
+    const float4 f = a.factors[t.slot[i]];
+    const bool vec = ((uintptr_t)t.g[i] | (uintptr_t)t.p[i]) % 16 == 0 && (!last || t.tail[i] == kAdBlock);
+    if (vec) update8<DT, true, EIGHT, LOW>(t.p[i], t.g[i], at, n, block, lane, f, a);
+    else update8<DT, false, EIGHT, LOW>(t.p[i], t.g[i], at, n, block, lane, f, a);
+  }
+}
+
+// Values of 8-bit moments, and codes of values (v is squared, not the root).
+__global__ void __launch_bounds__(kAdThreads) adam_unpack_k(const uint8_t* codes_m, const uint8_t* codes_r,
+                                                            const float2* scales, uint32_t blocks, float* m, float* v) {
+  grid_begin();
+  const uint32_t b = blockIdx.x * kAdWarps + threadIdx.x / 32;
+  if (b >= blocks) return;
+  const int64_t at = (int64_t)b * kAdBlock + threadIdx.x % 32 * 8;
+  float x[8], y[8];
+  decode_moments(codes_m, codes_r, scales[b], at, x, y);
+  store8f<RQ_F32, true>(m, at, 8, x);
+  store8f<RQ_F32, true>(v, at, 8, y);
+}
+
+__global__ void __launch_bounds__(kAdThreads) adam_pack_k(const float* m, const float* v, uint32_t blocks,
+                                                          uint8_t* codes_m, uint8_t* codes_r, float2* scales) {
+  grid_begin();
+  const uint32_t b = blockIdx.x * kAdWarps + threadIdx.x / 32;
+  if (b >= blocks) return;
+  const int64_t at = (int64_t)b * kAdBlock + threadIdx.x % 32 * 8;
+  float x[8], y[8];
+  load8f<RQ_F32, true>(m, at, 8, x);
+  load8f<RQ_F32, true>(v, at, 8, y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __fsqrt_rn(y[i]);
+  encode_moments(x, y, b, threadIdx.x % 32, codes_m, codes_r, scales);
+}
+
+// -------------------------------------------------------------- host side
+
+template <int MAX>
+static void fill(AdTensors<MAX>& t, const RqAdamTensor* list, int count) {
+  uint32_t at = 0;
+  t.count = count;
+  for (int i = 0; i < count; ++i) {
+    const int64_t blocks = (list[i].n + kAdBlock - 1) / kAdBlock;
+    t.p[i] = list[i].param;
+    t.g[i] = list[i].grad;
+    t.first[i] = at;
+    t.block[i] = (uint32_t)list[i].block;
+    t.slot[i] = (uint16_t)list[i].slot;
+    t.tail[i] = (uint16_t)(list[i].n - (blocks - 1) * kAdBlock);
+    at += (uint32_t)blocks;
+  }
+  t.first[count] = at;
+}
+
+static unsigned grid_for(uint32_t blocks, int ctas_per_sm) {
+  const unsigned want = (blocks + kAdWarps - 1) / kAdWarps, most = (unsigned)(num_sms() * ctas_per_sm);
+  return want < 1 ? 1 : want < most ? want : most;
+}
+
+template <int DT>
+static int norm_t(const RqAdamTensor* list, int count, double* partials, cudaStream_t st) {
+  if (count <= kAdSmall) {
+    AdTensors<kAdSmall> t;
+    fill(t, list, count);
+    unsigned grid = grid_for(t.first[count], 4);
+    if (grid > RQ_NORM_PARTIALS) grid = RQ_NORM_PARTIALS;
+    return launch_dependent(norm_partial_k<DT, kAdSmall>, grid, kAdThreads, st, t, partials);
+  }
+  AdTensors<kAdLarge> t;
+  fill(t, list, count);
+  unsigned grid = grid_for(t.first[count], 4);
+  if (grid > RQ_NORM_PARTIALS) grid = RQ_NORM_PARTIALS;
+  return launch_dependent(norm_partial_k<DT, kAdLarge>, grid, kAdThreads, st, t, partials);
+}
+
+int grad_norm_partial(const RqAdamTensor* list, int count, int dt, double* partials, cudaStream_t st) {
+  return dt == RQ_F32 ? norm_t<RQ_F32>(list, count, partials, st)
+         : dt == RQ_BF16 ? norm_t<RQ_BF16>(list, count, partials, st)
+                         : norm_t<RQ_F16>(list, count, partials, st);
+}
+
+int grad_norm_end(const double* partials, int n, float* norm, cudaStream_t st) {
+  return launch_dependent(norm_end_k, 1, kAdThreads, st, partials, n, norm);
+}
+
+int adam_begin(const RqAdamTensor* list, int count, double lr, const float* lr_at, double beta1, double beta2,
+               double decay, const double* partials, int n_partials, float max_norm, float* norm, int32_t* steps,
+               float* factors, cudaStream_t st) {
+  AdSlots s;
+  s.count = count;
+  for (int i = 0; i < count; ++i) s.slot[i] = (uint16_t)list[i].slot;
+  const AdFactors f{lr, decay, log(beta1), log(beta2), lr_at, max_norm};
+  return launch_dependent(adam_begin_k, 1, kAdThreads, st, s, f, partials, n_partials, norm, steps,
+                          reinterpret_cast<float4*>(factors));
+}
+
+template <int DT, bool EIGHT, bool LOW, int MAX>
+static int update_t(const RqAdamTensor* list, int count, const AdState& a, cudaStream_t st) {
+  AdTensors<MAX> t;
+  fill(t, list, count);
+  return launch_dependent(adam_update_k<DT, EIGHT, LOW, MAX>, grid_for(t.first[count], 8), kAdThreads, st, t, a);
+}
+
+template <bool EIGHT, int MAX>
+static int update_d(const RqAdamTensor* list, int count, int dt, const AdState& a, cudaStream_t st) {
+  if (a.low) return update_t<RQ_BF16, EIGHT, true, MAX>(list, count, a, st);
+  return dt == RQ_F32 ? update_t<RQ_F32, EIGHT, false, MAX>(list, count, a, st)
+         : dt == RQ_BF16 ? update_t<RQ_BF16, EIGHT, false, MAX>(list, count, a, st)
+                         : update_t<RQ_F16, EIGHT, false, MAX>(list, count, a, st);
+}
+
+int adam_update(const RqAdamTensor* list, int count, int dt, int bits, void* m, void* v, float* scales, int16_t* low,
+                const float* factors, double beta1, double beta2, double eps, cudaStream_t st) {
+  const AdState a{m, v, reinterpret_cast<float2*>(scales), low, reinterpret_cast<const float4*>(factors), (float)beta1,
+                  (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
+  if (bits == 8)
+    return count <= kAdSmall ? update_d<true, kAdSmall>(list, count, dt, a, st)
+                             : update_d<true, kAdLarge>(list, count, dt, a, st);
+  return count <= kAdSmall ? update_d<false, kAdSmall>(list, count, dt, a, st)
+                           : update_d<false, kAdLarge>(list, count, dt, a, st);
+}
+
+int adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks, float* m, float* v,
+                cudaStream_t st) {
+  return launch_dependent(adam_unpack_k, (unsigned)((blocks + kAdWarps - 1) / kAdWarps), kAdThreads, st, m8, r8,
+                          reinterpret_cast<const float2*>(scales), (uint32_t)blocks, m, v);
+}
+
+int adam_pack(const float* m, const float* v, int64_t blocks, uint8_t* m8, uint8_t* r8, float* scales,
+              cudaStream_t st) {
+  return launch_dependent(adam_pack_k, (unsigned)((blocks + kAdWarps - 1) / kAdWarps), kAdThreads, st, m, v,
+                          (uint32_t)blocks, m8, r8, reinterpret_cast<float2*>(scales));
+}
+
+}  // namespace rq

@@ -136,6 +136,36 @@ static int check_tokens(const void* logits, int dt, int64_t B, int64_t L, int64_
   return RQ_OK;
 }
 
+static int check_mx4(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t K) {
+  // pieces of 128 columns, of rows padded to 128, are numbered with 32 bits
+  if (!fits(rows) || !fits(K) || !fits((rows + 127) / 128 * 128 * (mx4_pitch(K) / 128))) return RQ_ERR_INVALID;
+  if (rows * K == 0) return RQ_OK;
+  if (!codes || !scales) return RQ_ERR_INVALID;
+  return (uintptr_t)codes % 16 || (uintptr_t)scales % 16 ? RQ_ERR_ALIGN : RQ_OK;
+}
+
+// The operands of a product [M, K] . [N, K]^T, and grid sizes it can have.
+static int check_product(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (!half_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!fits(M) || !fits(N) || !fits(K) || M > 65535LL * 128 || N > 65535LL * 128) return RQ_ERR_INVALID;
+  return RQ_OK;
+}
+
+static int check_tensors(const RqAdamTensor* t, int count, int dtype, bool params, bool state) {
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (count < 0 || count > RQ_ADAM_TENSORS || (count > 0 && !t)) return RQ_ERR_INVALID;
+  int64_t blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].n < 0 || (t[i].n > 0 && (!t[i].grad || (params && !t[i].param)))) return RQ_ERR_INVALID;
+    const int64_t own = (t[i].n + RQ_ADAM_BLOCK - 1) / RQ_ADAM_BLOCK;
+    blocks += own;
+    if (!fits(blocks) || (state && (t[i].slot < 0 || t[i].slot > 65535 || t[i].block < 0 || !fits(t[i].block + own))))
+      return RQ_ERR_INVALID;
+    if ((uintptr_t)t[i].grad % dtype_size(dtype) || (uintptr_t)t[i].param % dtype_size(dtype)) return RQ_ERR_ALIGN;
+  }
+  return RQ_OK;
+}
+
 }  // namespace rq
 
 using namespace rq;
@@ -477,6 +507,151 @@ int rq_token_logprobs_grad(const void* logits, int dtype, int64_t stride_b, int6
   if ((uintptr_t)slopes % 4 || (uintptr_t)upstream % 4 || (uintptr_t)dlogits % dtype_size(dtype)) return RQ_ERR_ALIGN;
   const TokenRows t{logits, stride_b, stride_l, dtype, B, L, V, labels, ignore};
   return token_logprobs_grad(t, stats, slopes, per_token ? 1 : 0, upstream, dlogits, (cudaStream_t)stream);
+}
+
+int64_t rq_mx4_scale_bytes(int64_t M, int64_t K) {
+  return !fits(M) || !fits(K) ? -1 : (M + 127) / 128 * (mx4_pitch(K) / 128) * 512;
+}
+
+int rq_mx4_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
+                int32_t* top, void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  if (!row_stride(M, ld_x, K)) return RQ_ERR_INVALID;
+  const int rc = check_mx4(codes, scales, M, K);
+  if (rc != RQ_OK) return rc;
+  if (M * K == 0) return RQ_OK;
+  if (!x) return RQ_ERR_INVALID;
+  if ((uintptr_t)x % dtype_size(dtype) || (uintptr_t)top % 4) return RQ_ERR_ALIGN;
+  return mx4_pack(x, dtype, ld_x, M, K, codes, scales, top, (cudaStream_t)stream);
+}
+
+int rq_mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dtype,
+                  void* stream) {
+  RQ_PROLOGUE();
+  if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
+  const int rc = check_mx4(codes, scales, M, K);
+  if (rc != RQ_OK) return rc;
+  if (M * K == 0) return RQ_OK;
+  if (!out) return RQ_ERR_INVALID;
+  if ((uintptr_t)out % dtype_size(dtype)) return RQ_ERR_ALIGN;
+  return mx4_unpack(codes, scales, M, K, out, dtype, (cudaStream_t)stream);
+}
+
+int rq_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
+                  const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, void* out, int dtype,
+                  void* stream) {
+  RQ_PROLOGUE();
+  int rc = check_product(dtype, M, N, K);
+  if (rc == RQ_OK) rc = check_mx4(a_codes, a_scales, M, K);
+  if (rc == RQ_OK) rc = check_mx4(b_codes, b_scales, N, K);
+  if (rc != RQ_OK) return rc;
+  if (M * N == 0) return RQ_OK;
+  if (K < 1 || !out) return RQ_ERR_INVALID;
+  if ((uintptr_t)out % 2 || (uintptr_t)bias % 2) return RQ_ERR_ALIGN;
+  return mx4_matmul(Mx4{a_codes, a_scales, M}, Mx4{b_codes, b_scales, N}, K, bias, out, dtype, (cudaStream_t)stream);
+}
+
+int64_t rq_mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  return !fits(M) || !fits(N) || !fits(K) ? -1 : mx4_linear_workspace_bytes(M, N, K);
+}
+
+int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M, const uint8_t* w_codes, const uint8_t* w_scales,
+                  int64_t N, int64_t K, const void* bias, void* out, void* workspace, int64_t workspace_bytes,
+                  void* stream) {
+  RQ_PROLOGUE();
+  int rc = check_product(dtype, M, N, K);
+  if (rc == RQ_OK) rc = check_mx4(w_codes, w_scales, N, K);
+  if (rc != RQ_OK) return rc;
+  if (!row_stride(M, ld_x, K) || !fits((M + 127) / 128 * 128 * (mx4_pitch(K) / 128))) return RQ_ERR_INVALID;
+  if (M * N == 0) return RQ_OK;
+  if (K < 1 || !x || !out) return RQ_ERR_INVALID;
+  if (!workspace || workspace_bytes < mx4_linear_workspace_bytes(M, N, K)) return RQ_ERR_WORKSPACE;
+  if ((uintptr_t)x % 2 || (uintptr_t)out % 2 || (uintptr_t)bias % 2 || (uintptr_t)workspace % 256) return RQ_ERR_ALIGN;
+  return mx4_linear(x, dtype, ld_x, M, Mx4{w_codes, w_scales, N}, K, bias, out, workspace, (cudaStream_t)stream);
+}
+
+int rq_mx4_dx(const void* dy, int dtype, int64_t ld_dy, int64_t M, const uint8_t* w_codes, const uint8_t* w_scales,
+              const int32_t* top, int64_t N, int64_t K, void* dx, void* stream) {
+  RQ_PROLOGUE();
+  int rc = check_product(dtype, M, N, K);
+  if (rc == RQ_OK) rc = check_mx4(w_codes, w_scales, N, K);
+  if (rc != RQ_OK) return rc;
+  if (M * K == 0) return RQ_OK;
+  if (N < 1 || !dy || !dx || !top || ld_dy < N || ld_dy % 8) return RQ_ERR_INVALID;
+  if ((uintptr_t)dy % 16 || (uintptr_t)dx % 2 || (uintptr_t)top % 4) return RQ_ERR_ALIGN;
+  return mx4_dx(dy, dtype, ld_dy, M, Mx4{w_codes, w_scales, N}, top, K, dx, (cudaStream_t)stream);
+}
+
+int rq_grad_norm_partial(const RqAdamTensor* tensors, int count, int dtype, double* partials, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tensors(tensors, count, dtype, false, false);
+  if (rc != RQ_OK) return rc;
+  if (count < 1 || !partials) return RQ_ERR_INVALID;
+  if ((uintptr_t)partials % 8) return RQ_ERR_ALIGN;
+  return grad_norm_partial(tensors, count, dtype, partials, (cudaStream_t)stream);
+}
+
+int rq_grad_norm_end(const double* partials, int n, float* norm, void* stream) {
+  RQ_PROLOGUE();
+  if (n < 0 || (n > 0 && !partials) || !norm) return RQ_ERR_INVALID;
+  if ((uintptr_t)partials % 8 || (uintptr_t)norm % 4) return RQ_ERR_ALIGN;
+  return grad_norm_end(partials, n, norm, (cudaStream_t)stream);
+}
+
+static bool beta_ok(double b) { return b >= 0.0 && b < 1.0; }
+
+int rq_adam_begin(const RqAdamTensor* tensors, int count, double lr, const float* lr_at, double beta1, double beta2,
+                  double decay, const double* partials, int n_partials, float max_norm, float* norm, int32_t* steps,
+                  float* factors, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tensors(tensors, count, RQ_F32, false, true);
+  if (rc != RQ_OK && rc != RQ_ERR_ALIGN) return rc;  // the values' type is the update's to check
+  if (!beta_ok(beta1) || !beta_ok(beta2) || n_partials < 0 || (n_partials > 0 && (!partials || !norm)))
+    return RQ_ERR_INVALID;
+  if (count == 0) return RQ_OK;
+  if (!steps || !factors) return RQ_ERR_INVALID;
+  if ((uintptr_t)partials % 8 || (uintptr_t)norm % 4 || (uintptr_t)steps % 4 || (uintptr_t)factors % 16 ||
+      (uintptr_t)lr_at % 4)
+    return RQ_ERR_ALIGN;
+  return adam_begin(tensors, count, lr, lr_at, beta1, beta2, decay, partials, n_partials, max_norm, norm, steps,
+                    factors, (cudaStream_t)stream);
+}
+
+int rq_adam_update(const RqAdamTensor* tensors, int count, int dtype, int bits, void* m, void* v, float* scales,
+                   int16_t* low, const float* factors, double beta1, double beta2, double eps, void* stream) {
+  RQ_PROLOGUE();
+  const int rc = check_tensors(tensors, count, dtype, true, true);
+  if (rc != RQ_OK) return rc;
+  if ((bits != 8 && bits != 32) || !beta_ok(beta1) || !beta_ok(beta2) || !(eps >= 0.0)) return RQ_ERR_INVALID;
+  if (low && dtype != RQ_BF16) return RQ_ERR_DTYPE;
+  if (count == 0) return RQ_OK;
+  if (!m || !v || !factors || (bits == 8 && !scales)) return RQ_ERR_INVALID;
+  if ((uintptr_t)m % 16 || (uintptr_t)v % 16 || (uintptr_t)scales % 8 || (uintptr_t)low % 16 || (uintptr_t)factors % 16)
+    return RQ_ERR_ALIGN;
+  return adam_update(tensors, count, dtype, bits, m, v, scales, low, factors, beta1, beta2, eps, (cudaStream_t)stream);
+}
+
+int rq_adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks, float* m, float* v,
+                   void* stream) {
+  RQ_PROLOGUE();
+  if (!fits(blocks)) return RQ_ERR_INVALID;
+  if (blocks == 0) return RQ_OK;
+  if (!m8 || !r8 || !scales || !m || !v) return RQ_ERR_INVALID;
+  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 16 || (uintptr_t)v % 16)
+    return RQ_ERR_ALIGN;
+  return adam_unpack(m8, r8, scales, blocks, m, v, (cudaStream_t)stream);
+}
+
+int rq_adam_pack(const float* m, const float* v, int64_t blocks, uint8_t* m8, uint8_t* r8, float* scales,
+                 void* stream) {
+  RQ_PROLOGUE();
+  if (!fits(blocks)) return RQ_ERR_INVALID;
+  if (blocks == 0) return RQ_OK;
+  if (!m8 || !r8 || !scales || !m || !v) return RQ_ERR_INVALID;
+  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 16 || (uintptr_t)v % 16)
+    return RQ_ERR_ALIGN;
+  return adam_pack(m, v, blocks, m8, r8, scales, (cudaStream_t)stream);
 }
 
 void launch_int4_dequant_matmul(void* stream, void* x, void* w_packed, void* scales, void* c, int M, int N, int K,

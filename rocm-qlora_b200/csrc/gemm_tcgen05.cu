@@ -61,17 +61,15 @@
 #include <vector>
 
 #include "gemv_common.cuh"
+#include "mx4_common.cuh"
 #include "rq_internal.h"
+#include "tcgen05_common.cuh"
 
 namespace rq {
 
 // Bounded waits of this file's kernels that ran out (read and cleared with
 // the GEMV's counter by rq_take_kernel_timeouts).
 __device__ unsigned int g_gemm_timeouts;
-
-// 2-D/3-D tensor map, cached (gemv_nf4.cu)
-int tensor_map_encode(int type, int swz, int rank, const void* ptr, const uint64_t* dims, const uint64_t* strides,
-                      const uint32_t* box, CUtensorMap* out);
 
 int gemm_take_timeouts(unsigned int* v) {
   unsigned int zero = 0;
@@ -139,68 +137,11 @@ struct GemmArgs {
   void* y;            // Y [M][N] (dX: dX [M][K])
   int M, N, K, r;
   float s;            // LoRA scaling (dX: 1, gt already carries it)
+  // microscaled weights (dX): scale pieces, largest scale byte, padded columns
+  const uint8_t* mx_scales;
+  const int32_t* mx_top;
+  int pitch;
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// shared::cluster address of the variable at shared::cta address `a` in CTA `rank`
-__device__ __forceinline__ uint32_t mapa(uint32_t a, uint32_t rank) {
-  uint32_t d;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(rank));
-  return d;
-}
-__device__ __forceinline__ void st_cluster(uint32_t caddr, int v) {
-  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(caddr), "r"(v) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Signal a barrier of the peer CTA without a fence in this thread: a 16-byte
-// shared-to-peer-shared bulk copy whose completion adds 16 transaction bytes
-// to the peer's barrier `cbar` (dst and cbar are shared::cluster addresses).
-// The receiving CTA posts the matching expect_tx.  A release-arrive at
-// cluster scope would wait for this thread's previous remote operations to
-// be acknowledged (about a microsecond a stage).
-__device__ __forceinline__ void bulk_signal(uint32_t cdst, uint32_t src, uint32_t cbar) {
-  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(cdst),
-               "r"(src), "r"(cbar)
-               : "memory");
-}
-// Non-blocking test of a phase (test_wait: the thread is never suspended,
-// so it sees the completion as soon as it happens).
-template <bool kCluster>
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  if constexpr (kCluster)
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  else
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  return ok != 0;
-}
 
 // The abort state of a CTA pair: this CTA's flag and the peer's (remote).
 struct Abort {
@@ -213,33 +154,6 @@ struct Abort {
   }
 };
 
-// Potentially blocking test of a phase (try_wait: a thread whose phase is
-// not complete is suspended in the barrier until it completes or a
-// system-dependent time limit passes, so it neither polls the barrier word
-// nor oversleeps the completion).
-template <bool kCluster>
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  if constexpr (kCluster)
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  else
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ uint64_t gtimer_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 constexpr uint64_t kWaitNs = 2000000000ull;  // a bounded wait gives up after about 2 s
 
 // Bounded wait for the phase of parity `parity`; false if either CTA of the
@@ -260,26 +174,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const A
 }
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < kWaitLimit && !mbar_test<false>(bar, parity); ++i) __nanosleep(kPollNs);
-}
-
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-          "r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-
-// Shared-memory descriptor of a K-major operand tile with 128-byte swizzle:
-// rows of 128 bytes (64 16-bit elements), 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);        // start address
-  d |= (uint64_t)1 << 16;                         // leading byte offset (unused for swizzled K-major)
-  d |= (uint64_t)(1024 >> 4) << 32;               // stride byte offset: next 8-row group
-  d |= (uint64_t)1 << 46;                         // descriptor version (sm_100)
-  d |= (uint64_t)2 << 61;                         // layout: 128-byte swizzle
-  return d;
 }
 
 // Shared-memory descriptor of an MN-major operand with 128-byte swizzle:
@@ -320,22 +214,6 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t mask) {
       : "memory");
 }
 
-// 32 consecutive fp32 columns of this thread's accumulator row
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 // Two 32-column loads (base and LoRA accumulators of the same rows) under
 // one wait: one tensor-memory round trip instead of two.
 __device__ __forceinline__ void tmem_ld32x2(uint32_t ta, uint32_t tb, float (&a)[32], float (&b)[32]) {
@@ -368,19 +246,11 @@ __device__ __forceinline__ float ldg_pin_f32(const void* p) {
   return v;
 }
 
-// two fp32 values rounded to the 16-bit type DT (one packed convert)
-template <int DT>
-__device__ __forceinline__ uint32_t pack_rn(float lo, float hi) {
-  if constexpr (DT == RQ_BF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
-template <int DT, bool DX, int BN, bool I8>
+// MX (dX only): codes are e2m1, with a power of two as the scale of 32 columns,
+// and N, which the reduction runs over, is any number (rows past it are zeros
+// by the TMA bounds).  In bf16 the weights are exact; in f16 they are taken
+// relative to the weight's largest scale, which the epilogue multiplies back.
+template <int DT, bool DX, int BN, bool I8, bool MX = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(const __grid_constant__ GemmArgs g) {
   using TL = Tile<BN, I8>;
   using T = typename DType<DT>::T;
@@ -406,7 +276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
 
   const int M = g.M, N = g.N, K = g.K;
   const int W_out = DX ? K : N;       // output columns
-  const int nkb = (DX ? N : K) / BK;  // reduction steps
+  const int nkb = MX ? (N + BK - 1) / BK : (DX ? N : K) / BK;  // reduction steps
   const int n0 = blockIdx.y * BN;     // the pair's first output column
   const int nh0 = n0 + (int)rank * BNH;  // this CTA's half: weight rows (forward) / output columns (dX)
   const int m0 = (blockIdx.z * 2 + (int)rank) * BM;  // this CTA's token rows
@@ -443,9 +313,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
   float* sclut = reinterpret_cast<float*>(sm + TL::kSmScl);
   for (int i = tid; i < 256 * kLutReps; i += kThreads) {
     const int v = i / kLutReps;
-    lutp[i] = make_float2(kNF4[v & 15], kNF4[v >> 4]);
+    if constexpr (MX) lutp[i] = make_float2(e2m1_to_f32(v), e2m1_to_f32(v >> 4));
+    else lutp[i] = make_float2(kNF4[v & 15], kNF4[v >> 4]);
   }
-  if (g.w.fmt != RQ_W_NF4)
+  if (!MX && g.w.fmt != RQ_W_NF4)
     for (int v = tid; v < 256; v += kThreads)
       sclut[v] = g.w.fmt == RQ_W_NF4_DQ_FP8 ? e4m3fnuz_to_f32(v) : ieee_div((float)(int8_t)v, 127.0f);
   // both CTAs' barriers initialised and the tensor memory allocated before
@@ -649,7 +520,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
       if (lane == 0) mbar_arrive(fullB0 + 8 * slot);
       return true;
     };
-    if constexpr (DX) {
+    if constexpr (MX) {
+      // as below, with one scale byte for the thread's 32 or 16 columns
+      const int kt = g.pitch / 128, blk = (nh0 + dcol) / 32;
+      const int base = DT == RQ_F16 ? *g.mx_top : 127;
+      auto mfetch = [&](int kb) -> uint32_t {
+        const int n = kb * 64 + frow;
+        if (kb >= nkb || blk >= 4 * kt) return 0u;
+        return ldg_pin_u8(g.mx_scales + ((int64_t)(n / 128) * kt + blk / 4) * 512 + (n % 32) * 16 + (n % 128) / 32 * 4 +
+                          blk % 4);
+      };
+      uint32_t ring[kPrefetch];
+#pragma unroll
+      for (int i = 0; i < kPrefetch; ++i) ring[i] = mfetch(i);
+      bool go = true;
+      for (int kb = 0; kb < nkb && go; kb += kPrefetch) {
+#pragma unroll
+        for (int i = 0; i < kPrefetch; ++i) {
+          if (go && kb + i < nkb) {
+            go = convert(kb + i, pow2_scale((int)ring[i], base));
+            ring[i] = mfetch(kb + i + kPrefetch);
+          }
+        }
+      }
+    } else if constexpr (DX) {
       // dX: the thread's block scale changes with the weight row, 64 rows a
       // stage; a register ring holds kPrefetch stages of raw scales (static
       // indices: fully unrolled)
@@ -742,6 +636,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
       const int c_lo = ((warp - 2) >> 2) * (BN / 2);  // warps w and w+4 split the columns
       const bool has_bias = !DX && g.bias != nullptr;
       T* y = static_cast<T*>(g.y);
+      const float back = MX && DT == RQ_F16 ? pow2_scale(*g.mx_top, 127) : 1.0f;
       for (int cb = c_lo; cb < c_lo + BN / 2; cb += 32) {
         float acc[32], u[32];
         if (has_lora)
@@ -757,7 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
           for (int e = 0; e < 2; ++e) {
             const int n = n0 + cb + j + e;
             const float bv = (has_bias && n < W_out) ? load_scalar(g.bias, g.bdt, n) : 0.0f;
-            o[e] = lora_epilogue<DT>(acc[j + e], has_bias, bv, has_lora ? u[j + e] : 0.0f, has_lora, g.s);
+            o[e] = lora_epilogue<DT>(MX && DT == RQ_F16 ? acc[j + e] * back : acc[j + e], has_bias, bv, has_lora ? u[j + e] : 0.0f, has_lora, g.s);
           }
           pk[j / 2] = pack_rn<DT>(o[0], o[1]);
         }
@@ -1007,10 +902,10 @@ bool gemm_supported(const LinearArgs& a, bool dx) {
   return a.w.N <= 0x7fffffff && a.w.K <= 0x7fffffff && a.M <= 0x7fffffff;
 }
 
-template <int DT, bool DX, int BN, bool I8>
+template <int DT, bool DX, int BN, bool I8, bool MX = false>
 static int gemm_run(const GemmArgs& g, uint64_t wout, uint64_t M, cudaStream_t st) {
   constexpr uint32_t smem = Tile<BN, I8>::kSmBytes;
-  const void* kern = (const void*)gemm_k<DT, DX, BN, I8>;
+  const void* kern = (const void*)gemm_k<DT, DX, BN, I8, MX>;
   const int rc = ensure_smem_limit(kern, smem);
   if (rc != RQ_OK) return rc;
   // CTA pairs along x, output tiles along y, 256-row token pairs along z
@@ -1028,7 +923,7 @@ static int gemm_run(const GemmArgs& g, uint64_t wout, uint64_t M, cudaStream_t s
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_k<DT, DX, BN, I8>, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_k<DT, DX, BN, I8, MX>, g);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return RQ_ERR_CUDA;
@@ -1194,6 +1089,40 @@ int lora_down_tc(int dt, bool wt, const void* X, int64_t M, int64_t Kr, const vo
 int gemm_dx(const LinearArgs& a, const void* gt, cudaStream_t st) {
   if (a.r > 0 && ((uintptr_t)a.lora_a % 16 || (a.w.K * 2) % 16)) return RQ_ERR_ALIGN;
   return gemm_launch(a, true, a.x, gt, st);
+}
+
+// dX of a microscaled weight: dy [M][N] (row stride ld), w [N][pitch].
+int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
+           cudaStream_t st) {
+  GemmArgs g = {};
+  const uint64_t N = (uint64_t)w.rows, pitch = (uint64_t)mx4_pitch(K);
+  const int bn = pick_bn((uint64_t)K, (uint64_t)M);
+  {
+    const uint64_t d[3] = {N, (uint64_t)M, 1}, s[2] = {(uint64_t)ld * 2, 0};
+    const uint32_t b[3] = {BK, BM, 1};
+    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, 2, dy, d, s, b, &g.xmap);
+    if (rc != RQ_OK) return rc;
+  }
+  {
+    const uint64_t d[3] = {pitch / 2, N, 1}, s[2] = {pitch / 2, 0};
+    const uint32_t b[3] = {(uint32_t)bn / 4, 64, 1};
+    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, 2, w.codes, d, s, b, &g.cmap);
+    if (rc != RQ_OK) return rc;
+  }
+  g.tmap = g.bmap = g.xmap;
+  g.y = dx;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = (int)K;
+  g.s = 1.0f;
+  g.mx_scales = w.scales;
+  g.mx_top = top;
+  g.pitch = (int)pitch;
+  if (dt == RQ_BF16)
+    return bn == 256 ? gemm_run<RQ_BF16, true, 256, false, true>(g, (uint64_t)K, (uint64_t)M, st)
+                     : gemm_run<RQ_BF16, true, 128, false, true>(g, (uint64_t)K, (uint64_t)M, st);
+  return bn == 256 ? gemm_run<RQ_F16, true, 256, false, true>(g, (uint64_t)K, (uint64_t)M, st)
+                   : gemm_run<RQ_F16, true, 128, false, true>(g, (uint64_t)K, (uint64_t)M, st);
 }
 
 }  // namespace rq

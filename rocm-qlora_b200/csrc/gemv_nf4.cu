@@ -1479,18 +1479,20 @@ int gemv_nf4_forward(const GemvArgs& g, bool beside, cudaStream_t st) {
 
 namespace rq {
 int gemm_take_timeouts(unsigned int* v);  // gemm_tcgen05.cu
+int mx4_take_timeouts(unsigned int* v);   // mx4_gemm.cu
 }
 
 extern "C" int rq_take_kernel_timeouts(unsigned int* count) {
-  unsigned int v = 0, w = 0, zero = 0;
+  unsigned int v = 0, w = 0, u = 0, zero = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, rq::g_kernel_timeouts, sizeof(v));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(rq::g_kernel_timeouts, &zero, sizeof(zero));
   if (e != cudaSuccess) {
     rq::set_cuda_error(e);
     return RQ_ERR_CUDA;
   }
-  const int rc = rq::gemm_take_timeouts(&w);
+  int rc = rq::gemm_take_timeouts(&w);
+  if (rc == RQ_OK) rc = rq::mx4_take_timeouts(&u);
   if (rc != RQ_OK) return rc;
-  if (count) *count = v + w;
+  if (count) *count = v + w + u;
   return RQ_OK;
 }

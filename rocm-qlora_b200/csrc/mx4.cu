@@ -1,0 +1,184 @@
+// mx4.cu -- rows to and from microscaled 4-bit values: blocks of 32 columns
+// with e = max(floor(log2 max|x|) - 2, -127), codes e2m1(x 2^-e), scale byte
+// e + 127.  e is read off the maximum's exponent bits and 2^-e is exact, so the
+// codes are those of the definition bit for bit.
+//
+// One pass over the data.  4 lanes hold a block and 16 a piece of 128 columns
+// (8 values a lane: one 16-byte load of a 16-bit type); the piece's four scale
+// bytes are written as one word.  Rows past M up to whole pieces of 128 are
+// warps of their own that write zero scales.
+#include <cuda_runtime.h>
+
+#include "mx4_common.cuh"
+
+namespace rq {
+
+constexpr int kM4Threads = 256, kM4Lanes = 16, kM4PerCta = kM4Threads / kM4Lanes;
+
+// Division of n < 2^31 by a number known at launch: (n * mul) >> shift.
+struct M4Divide {
+  uint32_t mul;
+  int shift;
+  uint32_t by;
+};
+static M4Divide m4_divide(uint32_t d) {
+  int s = 0;
+  while ((1ull << s) < d) ++s;
+  return M4Divide{(uint32_t)((1ull << (31 + s)) / d + 1), 31 + s, d};
+}
+
+// A lane's 8 values at columns col .. col + 7, 0 past K.  VEC: whole 16-byte
+// pieces, so all 8 exist or none does.
+template <int DT, bool VEC>
+__device__ __forceinline__ void m4_load(const typename DType<DT>::T* row, int col, int K, float (&v)[8]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < K ? DType<DT>::to_f32(row[col + i]) : 0.0f;
+  } else if constexpr (DT == RQ_F32) {
+    const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    *reinterpret_cast<float4*>(v) = col < K ? *reinterpret_cast<const float4*>(row + col) : z;
+    *reinterpret_cast<float4*>(v + 4) = col < K ? *reinterpret_cast<const float4*>(row + col + 4) : z;
+  } else {
+    const uint4 w = col < K ? *reinterpret_cast<const uint4*>(row + col) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == RQ_BF16) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+
+// Eight e2m1 codes (nearest, ties to even, saturating), the first in the low bits.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float by) {
+  uint32_t w;
+  asm("{\n .reg .b8 a, b, c, d;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      " mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(w)
+      : "f"(v[0] * by), "f"(v[1] * by), "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by),
+        "f"(v[7] * by));
+  return w;
+}
+
+// The scale byte of a block of which each of 4 neighbouring lanes has 8 values.
+__device__ __forceinline__ uint32_t m4_scale(const float (&v)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const uint32_t e = top >> 23;  // 127 + floor(log2 top), 0 below 2^-126
+  return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+}
+
+// 2^(127 - byte), the factor that takes values to codes.
+__device__ __forceinline__ float m4_factor(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict__ x, int64_t ld, int64_t M, int K,
+                                                         uint32_t pieces, M4Divide nt, uint8_t* __restrict__ codes,
+                                                         uint8_t* __restrict__ scales, int32_t* __restrict__ top) {
+  grid_begin();
+  using T = typename DType<DT>::T;
+  const uint32_t p = blockIdx.x * kM4PerCta + threadIdx.x / kM4Lanes;
+  const int l = threadIdx.x % kM4Lanes;
+  const bool in = p < pieces;
+  const uint32_t row = in ? (uint32_t)(((uint64_t)p * nt.mul) >> nt.shift) : 0u, tile = in ? p - row * nt.by : 0u;
+  const bool any = in && row < M;
+  float v[8];
+  m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), (int)tile * 128 + l * 8, any ? K : 0, v);
+  const uint32_t byte = m4_scale(v);
+  const uint32_t w = e2m1x8(v, m4_factor(byte));
+  if (any) *reinterpret_cast<uint32_t*>(codes + ((int64_t)row * nt.by + tile) * 64 + l * 4) = w;
+  const uint32_t b0 = __shfl_sync(0xffffffffu, byte, 0, kM4Lanes), b1 = __shfl_sync(0xffffffffu, byte, 4, kM4Lanes),
+                 b2 = __shfl_sync(0xffffffffu, byte, 8, kM4Lanes), b3 = __shfl_sync(0xffffffffu, byte, 12, kM4Lanes);
+  if (in && l == 0)
+    *reinterpret_cast<uint32_t*>(scales + ((int64_t)(row / 128) * nt.by + tile) * 512 + row % 32 * 16 + row % 128 / 32 * 4) =
+        b0 | b1 << 8 | b2 << 16 | b3 << 24;
+  if (top) {
+    const int most = (int)__reduce_max_sync(0xffffffffu, any && byte != 255u ? byte : 0u);
+    if (threadIdx.x % 32 == 0 && most > *reinterpret_cast<volatile int32_t*>(top)) atomicMax(top, most);
+  }
+}
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kM4Threads) mx4_unpack_k(const uint8_t* __restrict__ codes,
+                                                           const uint8_t* __restrict__ scales, uint32_t pieces, int K,
+                                                           M4Divide nt, void* __restrict__ out) {
+  grid_begin();
+  using T = typename DType<DT>::T;
+  const uint32_t p = blockIdx.x * kM4PerCta + threadIdx.x / kM4Lanes;
+  if (p >= pieces) return;
+  const int l = threadIdx.x % kM4Lanes;
+  const uint32_t row = (uint32_t)(((uint64_t)p * nt.mul) >> nt.shift), tile = p - row * nt.by;
+  const float s = pow2_scale(scales[mx4_scale_at(row, (int)tile * 4 + l / 4, (int)nt.by)], 127);
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + ((int64_t)row * nt.by + tile) * 64 + l * 4);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h;
+    asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"((w >> (8 * i)) & 0xffu));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * i] = f.x * s;
+    v[2 * i + 1] = f.y * s;
+  }
+  const int col = (int)tile * 128 + l * 8;
+  T* to = static_cast<T*>(out) + (int64_t)row * K + col;
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < K) to[i] = DType<DT>::from_f32(v[i]);
+  } else if (col < K) {
+    if constexpr (DT == RQ_F32) {
+      reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
+      reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
+    } else {
+      *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
+                                                 pack2<DT>(v[6], v[7]));
+    }
+  }
+}
+
+// Rows of K columns in whole aligned pieces of a lane.
+static bool m4_rows(const void* p, int64_t ld, int64_t K, int dt) {
+  return (uintptr_t)p % 16 == 0 && ld * (dt == RQ_F32 ? 4 : 2) % 16 == 0 && K % 8 == 0;
+}
+
+int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
+             cudaStream_t st) {
+  const M4Divide nt = m4_divide((uint32_t)(mx4_pitch(K) / 128));
+  const uint32_t pieces = (uint32_t)((M + 127) / 128 * 128) * nt.by;
+  if (top) {
+    const cudaError_t e = cudaMemsetAsync(top, 0, 4, st);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return RQ_ERR_CUDA;
+    }
+  }
+  const bool vec = m4_rows(x, ld, K, dt);
+  auto* k = dt == RQ_F32 ? (vec ? mx4_pack_k<RQ_F32, true> : mx4_pack_k<RQ_F32, false>)
+            : dt == RQ_BF16 ? (vec ? mx4_pack_k<RQ_BF16, true> : mx4_pack_k<RQ_BF16, false>)
+                            : (vec ? mx4_pack_k<RQ_F16, true> : mx4_pack_k<RQ_F16, false>);
+  return launch_dependent(k, (pieces + kM4PerCta - 1) / kM4PerCta, kM4Threads, st, x, ld, M, (int)K, pieces, nt, codes,
+                          scales, top);
+}
+
+int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st) {
+  const M4Divide nt = m4_divide((uint32_t)(mx4_pitch(K) / 128));
+  const uint32_t pieces = (uint32_t)M * nt.by;
+  const bool vec = m4_rows(out, K, K, dt);
+  auto* k = dt == RQ_F32 ? (vec ? mx4_unpack_k<RQ_F32, true> : mx4_unpack_k<RQ_F32, false>)
+            : dt == RQ_BF16 ? (vec ? mx4_unpack_k<RQ_BF16, true> : mx4_unpack_k<RQ_BF16, false>)
+                            : (vec ? mx4_unpack_k<RQ_F16, true> : mx4_unpack_k<RQ_F16, false>);
+  return launch_dependent(k, (pieces + kM4PerCta - 1) / kM4PerCta, kM4Threads, st, codes, scales, pieces, (int)K, nt, out);
+}
+
+}  // namespace rq

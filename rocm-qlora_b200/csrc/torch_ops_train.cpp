@@ -14,30 +14,11 @@
 
 namespace {
 
-using at::Tensor;
-using rq_torch::check;
-using rq_torch::dtype_code;
-using rq_torch::ptr;
-using std::optional;
-
-cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+using namespace rq_torch;
 
 void check_rows(const Tensor& t, const char* name) {
   TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), "rocm_qlora: ", name,
               " must be a 2-D tensor with contiguous columns");
-}
-
-// The kernels take pointers: every tensor of a call is on the first one's device.
-void check_device(const Tensor& first, const Tensor& t) {
-  TORCH_CHECK(t.device() == first.device(), "rocm_qlora: tensors are on different devices: ", first.device(), " and ",
-              t.device());
-}
-void check_device(const Tensor& first, const optional<Tensor>& t) {
-  if (t.has_value() && t->defined()) check_device(first, *t);
-}
-template <class... Rest>
-void one_device(const Tensor& first, const Rest&... rest) {
-  (check_device(first, rest), ...);
 }
 
 bool plan_ok(const Tensor& plan) { return plan.dim() == 1 && plan.is_contiguous() && plan.scalar_type() == at::kInt; }
@@ -45,12 +26,6 @@ bool plan_ok(const Tensor& plan) { return plan.dim() == 1 && plan.is_contiguous(
 void check_plan(const optional<Tensor>& plan) {
   TORCH_CHECK(!plan.has_value() || !plan->defined() || plan_ok(*plan),
               "rocm_qlora: plan must be a contiguous 1-D int32 tensor, as adapter_plan makes it");
-}
-
-// The kernels read banks and codes in 16-byte pieces: a view that starts
-// between two of them is copied.
-Tensor aligned(const Tensor& t) {
-  return t.is_meta() || (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 Tensor adapter_plan(const Tensor& ids, int64_t count, int64_t tile) {
@@ -335,33 +310,9 @@ Tensor token_logprobs_grad(const Tensor& logits, const Tensor& labels, int64_t i
 // ---- the differentiable entry points: one dispatcher call forward, and a
 // backward that never enters Python
 
-// One of the operators above, through the dispatcher but for its autograd keys:
-// the nodes here are the gradients.
-template <auto F, class... A>
-auto via(const char* name, A&&... args) {
-  static const auto op =
-      c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<std::remove_pointer_t<decltype(F)>>();
-  const at::AutoDispatchBelowAutograd below;
-  return op.call(std::forward<A>(args)...);
-}
-#define RQ_VIA(op, ...) via<&op>("rocm_qlora::" #op, __VA_ARGS__)
-
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
-
-void once(const char* what) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), "rocm_qlora: ", what, " is differentiable once only");
-}
-
-// t as [rows, columns]: contiguous columns, rows apart or one row for all; a
-// copy where its strides are others (rows that overlap among them).
-Tensor rows_of(const Tensor& t) {
-  Tensor r = t.dim() == 2 ? t : t.reshape({c10::multiply_integers(t.sizes().slice(0, t.dim() - 1)), t.size(-1)});
-  const bool columns = r.size(1) <= 1 || r.stride(1) == 1;
-  const bool rows = r.size(0) <= 1 || r.stride(0) == 0 || r.stride(0) >= r.size(1);
-  return columns && rows ? r : r.contiguous();
-}
 
 optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
@@ -392,19 +343,6 @@ struct AdaptersAdd : Function<AdaptersAdd> {
     return {ctx->needs_input_grad(0) ? grads[0] : Tensor(), dx, dA, dB, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
-
-void check_float(at::ScalarType t) {
-  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "unsupported dtype ", t,
-                   "; rocm_qlora kernels take float32, bfloat16 or float16");
-}
-
-void check_gpu(std::initializer_list<const Tensor*> tensors) {
-  for (const Tensor* t : tensors) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->is_cpu(), "rocm_qlora (B200 build) computes on the GPU only: move the tensors to a CUDA device");
-    TORCH_CHECK(t->device() == (*tensors.begin())->device(), "tensors are on different devices: ",
-                (*tensors.begin())->device(), " and ", t->device());
-  }
-}
 
 std::string sizes_of(const Tensor& t) { return c10::str(t.sizes()); }
 
