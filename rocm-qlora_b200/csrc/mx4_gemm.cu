@@ -6,21 +6,27 @@
 // memory, and sums in fp32 in tensor memory: 4 times the rate of 16-bit
 // operands, and no value is ever unpacked.
 //
-// A CTA computes 128 rows of operand P times BN rows of operand Q.  A stage of
-// its ring holds 256 columns: P's codes [128 x 128 bytes] and Q's [BN x 128
-// bytes] by TMA (128-byte swizzle), and both scales' pieces of 512 bytes (128
-// rows x 128 columns, stored in the order that tensor memory takes) by bulk
-// copies.  tcgen05.cp spreads a piece over 4 columns of tensor memory; every
-// slot has columns of its own, so a copy never overwrites scales in use.
+// A stage of a CTA's ring holds 256 columns: the codes of 128 rows of operand P
+// and of some of operand Q (128 bytes a row, by TMA with 128-byte swizzle), and
+// both scales' pieces of 512 bytes (128 rows x 128 columns, stored in the order
+// that tensor memory takes).  tcgen05.cp spreads a piece over 4 columns of
+// tensor memory; every slot has columns of its own, so a copy never overwrites
+// scales in use.
 //   warp 0     producer (one thread)
 //   warp 1     tensor memory; one thread copies scales and issues the MMAs
 //   warps 2-9  epilogue: warps w and w + 4 share the 32 rows of lane quarter w % 4
-// P are rows of a (tokens) and Q rows of b (outputs), or, with SWAP, the other
-// way round: few tokens then fill the narrow side.  With few tiles a cluster
-// splits the columns: each CTA parks its sums in shared memory, and all add up
-// a share in rank order (fixed order: deterministic).
-// Waits are bounded: one that runs out counts a kernel timeout, the CTA drains
-// its copies and stores nothing.
+// Two kernels:
+//   mx4_pair_k   many tiles.  CTA pairs stay and take tiles of 256 tokens x 256
+//                outputs in turn (2-SM MMAs; a CTA loads its 128 tokens and half
+//                of the outputs, so a stage's 35 KB feed 512 cycles of MMA, where
+//                a CTA alone needs 51 KB: the L2 gave 45 bytes a cycle and SM);
+//                the epilogue empties the accumulator into shared memory, and
+//                the next tile's MMAs run while it stores.
+//   mx4_split_k  few tiles.  P are outputs, Q up to 256 tokens, and a cluster
+//                splits the columns: each CTA parks its sums in shared memory,
+//                and all add up a share in rank order (fixed order: deterministic).
+// Waits are bounded: one that runs out counts a kernel timeout, the CTAs drain
+// their copies and store nothing.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -53,6 +59,8 @@ constexpr uint32_t kPBytes = kP * 128;        // codes of a stage: 256 columns
 constexpr uint32_t kPiece = 512;
 constexpr uint64_t kWaitNs = 2000000000ull;   // a bounded wait gives up after about 2 s
 
+constexpr int kPark = 132;                    // floats of a token's parked sums
+
 template <int BN>
 struct Plan {
   static constexpr int NB = (BN + 127) / 128;                       // scale pieces of Q a 128 columns
@@ -60,8 +68,8 @@ struct Plan {
   static constexpr uint32_t kSP = kPBytes + kQBytes;                // P's scale pieces in a stage
   static constexpr uint32_t kSQ = kSP + 2 * kPiece;                 // Q's: [piece][128 columns]
   static constexpr uint32_t kStage = kSQ + 2 * NB * kPiece;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6;
-  static constexpr uint32_t kRed = BN * 129 * 4;                    // parked sums, in the ring's place
+  static constexpr int kStages = BN == 128 ? 5 : 6;
+  static constexpr uint32_t kRed = BN * kPark * 4;                  // parked sums, in the ring's place
   static constexpr uint32_t kRing = kStages * kStage;
   static constexpr uint32_t kSmem = (kRing > kRed ? kRing : kRed) + 1024;
   static constexpr uint32_t kAcc = BN < 32 ? 32 : BN;               // accumulator columns
@@ -88,25 +96,32 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // 32 rows of 16 bytes (8-row groups 128 bytes apart, no swizzle) to 4 columns
-// of all four lane quarters.
+// of all four lane quarters (of a pair: each CTA's from its own shared memory).
+template <int CTAS>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
   const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-// e2m1 operands, power-of-two scales, M = 128; `half`: which two of a word's
+// e2m1 operands, power-of-two scales; `half`: which two of a word's
 // four scale bytes the 64 columns take.
-template <int BN>
+template <int M, int N>
 __device__ __forceinline__ uint32_t idesc_mx4(uint32_t half) {
-  return (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (1u << 23) | (1u << 27) | (2 * half) << 4 | (2 * half) << 29;
+  return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | (2 * half) << 4 |
+         (2 * half) << 29;
 }
+#define RQ_MMA_MX4(group)                                                                                          \
+  asm volatile(                                                                                                    \
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"                                                               \
+      " tcgen05.mma.cta_group::" group ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" \
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum)                                           \
+      : "memory")
+template <int CTAS>
 __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                         uint32_t accum) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum)
-      : "memory");
+  if constexpr (CTAS == 1) RQ_MMA_MX4("1");
+  else RQ_MMA_MX4("2");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -130,8 +145,9 @@ __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   while (!mbar_test<false>(bar, parity) && gtimer_ns() - t0 < kWaitNs) __nanosleep(100);
 }
 
-template <int DT, int BN, bool SWAP>
-__global__ void __launch_bounds__(kThreads, 1) mx4_gemm_k(const __grid_constant__ Args g) {
+// out[q, p] (tokens Q, outputs P): sums of its share of the columns.
+template <int DT, int BN>
+__global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant__ Args g) {
   using PL = Plan<BN>;
   using T = typename DType<DT>::T;
   constexpr int S = PL::kStages, NB = PL::NB;
@@ -199,13 +215,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_k(const __grid_constant_
         const int nt = min(2, g.tiles - 2 * st);
         for (int t = 0; t < nt; ++t) {
           const uint32_t tp = tsc + t * (PL::kSlotCols / 2), tq = tp + 4;
-          copy_scales(tp, at + PL::kSP + t * kPiece);
+          copy_scales<1>(tp, at + PL::kSP + t * kPiece);
 #pragma unroll
-          for (int j = 0; j < NB; ++j) copy_scales(tq + 4 * j, at + PL::kSQ + (2 * j + t) * kPiece);
+          for (int j = 0; j < NB; ++j) copy_scales<1>(tq + 4 * j, at + PL::kSQ + (2 * j + t) * kPiece);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            mma_mx4(tmem, sw128_desc(at + (2 * t + h) * 32), sw128_desc(at + kPBytes + (2 * t + h) * 32),
-                    idesc_mx4<BN>(h), tp, tq, (i > 0 || t > 0 || h > 0) ? 1u : 0u);
+            mma_mx4<1>(tmem, sw128_desc(at + (2 * t + h) * 32), sw128_desc(at + kPBytes + (2 * t + h) * 32),
+                       idesc_mx4<128, BN>(h), tp, tq, (i > 0 || t > 0 || h > 0) ? 1u : 0u);
         }
         mma_commit(empty0 + 8 * slot);
         *reinterpret_cast<volatile int*>(&consumed) = i + 1;
@@ -227,43 +243,20 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_k(const __grid_constant_
   }
   if (warp >= 2 && (BN >= 64 || warp < 6)) {
     float* red = reinterpret_cast<float*>(sm);
+    const int n = p0 + row;
+    const float bv = has_bias && n < g.prows ? DType<DT>::to_f32(static_cast<const T*>(g.bias)[n]) : 0.0f;
     for (int c = c_lo; c < c_hi; c += 32) {
       float acc[32];
       tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + c, acc);
       if (sk > 1) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (c + j < BN) red[(c + j) * 129 + row] = ok && s1 > s0 ? acc[j] : 0.0f;
-      } else if (!ok) {
-        continue;
-      } else if constexpr (SWAP) {
-        // rows of P are outputs, one a lane; columns are tokens
-        const int n = p0 + row;
-        const float bv = has_bias && n < g.prows ? DType<DT>::to_f32(static_cast<const T*>(g.bias)[n]) : 0.0f;
+          if (c + j < BN) red[(c + j) * kPark + row] = ok && s1 > s0 ? acc[j] : 0.0f;
+      } else if (ok) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (c + j < BN && q0 + c + j < g.qrows && n < g.prows)
             out[(int64_t)(q0 + c + j) * g.ld + n] = DType<DT>::from_f32(acc[j] + bv);
-      } else {
-        const int m = p0 + row;
-        if (m >= g.prows) continue;
-        T* to = out + (int64_t)m * g.ld + q0 + c;
-        if (has_bias) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            acc[j] += q0 + c + j < g.qrows ? DType<DT>::to_f32(static_cast<const T*>(g.bias)[q0 + c + j]) : 0.0f;
-        }
-        if (q0 + c + 32 <= g.qrows && (uintptr_t)to % 16 == 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            reinterpret_cast<uint4*>(to)[j] =
-                make_uint4(pack_rn<DT>(acc[8 * j], acc[8 * j + 1]), pack_rn<DT>(acc[8 * j + 2], acc[8 * j + 3]),
-                           pack_rn<DT>(acc[8 * j + 4], acc[8 * j + 5]), pack_rn<DT>(acc[8 * j + 6], acc[8 * j + 7]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (q0 + c + j < g.qrows) to[j] = DType<DT>::from_f32(acc[j]);
-        }
       }
     }
   }
@@ -282,25 +275,35 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_k(const __grid_constant_
   if (sk > 1) {
     __syncwarp();
     cluster_sync();  // all sums are parked
+    // this CTA's share: groups of 4 outputs of a token, the loads of all ranks at once
     const uint32_t red = smem_u32(sm);
-    // this CTA's share of the Q rows (SWAP: tokens) or of the P rows (tokens): a warp a token
-    constexpr int kTokens = SWAP ? BN : (int)kP, kOut = SWAP ? (int)kP : BN;
-    const int t0 = kTokens * rank / sk, t1 = kTokens * (rank + 1) / sk;
-    for (int t = t0 + warp; t < t1; t += kThreads / 32) {
-      const int m = (SWAP ? q0 : p0) + t, rows = SWAP ? g.qrows : g.prows;
-      if (m >= rows) continue;
-      for (int o = lane; o < kOut; o += 32) {
-        const int n = (SWAP ? p0 : q0) + o;
-        if (n >= (SWAP ? g.prows : g.qrows)) continue;
-        const uint32_t at = red + (SWAP ? t * 129 + o : o * 129 + t) * 4;
-        float sum = 0.0f;
-        for (int r = 0; r < sk; ++r) {
-          float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa(at, (uint32_t)r)));
-          sum += v;
-        }
-        if (has_bias) sum += DType<DT>::to_f32(static_cast<const T*>(g.bias)[n]);
-        out[(int64_t)m * g.ld + n] = DType<DT>::from_f32(sum);
+    const int groups = min(BN, g.qrows - q0) * 32;
+    for (int e = groups * rank / sk + tid; e < groups * (rank + 1) / sk; e += kThreads) {
+      const int t = e / 32, o = e % 32 * 4, n = p0 + o;
+      if (n >= g.prows) continue;
+      float4 v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < sk)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                       : "r"(mapa(red + (t * kPark + o) * 4, (uint32_t)r)));
+      float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int r = 1; r < 8; ++r)
+        if (r < sk) sum[0] += v[r].x, sum[1] += v[r].y, sum[2] += v[r].z, sum[3] += v[r].w;
+      if (has_bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < g.prows) sum[j] += DType<DT>::to_f32(static_cast<const T*>(g.bias)[n + j]);
+      }
+      T* to = out + (int64_t)(q0 + t) * g.ld + n;
+      if (n + 4 <= g.prows && (uintptr_t)to % 8 == 0) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_rn<DT>(sum[0], sum[1]), pack_rn<DT>(sum[2], sum[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < g.prows) to[j] = DType<DT>::from_f32(sum[j]);
       }
     }
     __syncwarp();
@@ -308,26 +311,265 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_gemm_k(const __grid_constant_
   }
 }
 
-template <int DT, int BN, bool SWAP>
-int run(const Args& g, int sk, cudaStream_t st) {
-  const void* kern = (const void*)mx4_gemm_k<DT, BN, SWAP>;
-  const int rc = ensure_smem_limit(kern, Plan<BN>::kSmem);
+// ------------------------------------------------------------- CTA pairs
+
+namespace pair {
+constexpr int S = 4;
+constexpr uint32_t kCodes = 128 * 128;                      // of P's or of half of Q's rows
+constexpr uint32_t kSP = 2 * kCodes, kSQ = kSP + 2 * kPiece;  // scale pieces: P's two, Q's [half][two]
+constexpr uint32_t kStage = kSQ + 4 * kPiece;
+constexpr uint32_t kOutPitch = 256 + 16;                    // bytes of a staged row of 128 outputs
+constexpr uint32_t kOutWarp = 32 * kOutPitch;
+constexpr uint32_t kRing = S * kStage;
+constexpr uint32_t kSmem = kRing + kEpiWarps * kOutWarp + 1024;
+constexpr uint32_t kSlotCols = 2 * 12;                      // a 128 columns: P's 4, Q's 8
+static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024 && 256 + S * kSlotCols <= 512, "");
+}  // namespace pair
+
+struct PairArgs {
+  CUtensorMap pmap, qmap;    // codes, boxes 128 bytes x 128 rows
+  CUtensorMap psmap, qsmap;  // scale pieces [pieces][128 words], boxes of two pieces
+  const void* bias;
+  void* out;
+  int prows, qrows, tiles;
+  int64_t ld;
+};
+
+// A TMA copy of one CTA of a pair whose bytes count on the barrier of the
+// pair's leader (`bar`: shared::cluster address).
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cbar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+}
+
+// The abort state of a pair: this CTA's flag and the peer's.
+struct PairAbort {
+  volatile int* mine;
+  uint32_t peer;
+  __device__ __forceinline__ bool raised() const { return *mine != 0; }
+};
+template <bool kCluster>
+__device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
+  if (mbar_try<kCluster>(bar, parity)) return true;
+  const uint64_t t0 = gtimer_ns();
+  while (!ab.raised()) {
+    if (mbar_try<kCluster>(bar, parity)) return true;
+    if (gtimer_ns() - t0 > kWaitNs) {
+      *ab.mine = 1;
+      st_cluster(ab.peer, 1);
+      atomicAdd(&g_mx4_timeouts, 1u);
+      return false;
+    }
+  }
+  return false;
+}
+
+// out[p, q]: P tokens, Q outputs.
+template <int DT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pair_k(const __grid_constant__ PairArgs g) {
+  using namespace pair;
+  using T = typename DType<DT>::T;
+  extern __shared__ __align__(1024) unsigned char dsm[];
+  // full[S] (leader's counts both CTAs' bytes), empty[S], acc (sums complete),
+  // taken (leader's: both CTAs' epilogues have read them)
+  __shared__ __align__(8) uint64_t bars[2 * S + 3];
+  __shared__ uint32_t tmem_sh;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = cluster_rank();
+  const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
+  unsigned char* sm = dsm + (sbase - sraw);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S, taken = accbar + 8,
+                 drainbar = taken + 8;
+  const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u)};
+  const int steps = (g.tiles + 1) / 2;
+  const int pt = (g.prows + 255) / 256, qt = (g.qrows + 255) / 256, ntile = pt * qt;
+  const int first = blockIdx.x / 2, stride = gridDim.x / 2;
+
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    mbar_init(accbar, 1);
+    mbar_init(taken, 2 * kEpiWarps);
+    mbar_init(drainbar, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_sh;
+  grid_begin();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t lead = mapa(full0, 0);
+      int i = 0;
+      bool ok = true;
+      for (int t = first; t < ntile && ok; t += stride) {
+        const int p0 = t % pt * 256 + (int)rank * 128, q0 = t / pt * 256, qh = q0 + (int)rank * 128;
+        for (int st = 0; st < steps; ++st, ++i) {
+          const int slot = i % S;
+          if (i >= S && !wait_pair<false>(empty0 + 8 * slot, ((i / S) - 1) & 1, ab)) {
+            ok = false;
+            break;
+          }
+          const uint32_t at = sbase + slot * kStage, bar = lead + 8 * slot;
+          if (rank == 0) mbar_expect_tx(full0 + 8 * slot, 2 * kStage);
+          tma_pair(at, &g.pmap, st * 128, p0, bar);
+          tma_pair(at + kCodes, &g.qmap, st * 128, qh, bar);
+          tma_pair(at + kSP, &g.psmap, 0, p0 / 128 * g.tiles + 2 * st, bar);
+          tma_pair(at + kSQ, &g.qsmap, 0, q0 / 128 * g.tiles + 2 * st, bar);
+          tma_pair(at + kSQ + 2 * kPiece, &g.qsmap, 0, (q0 / 128 + 1) * g.tiles + 2 * st, bar);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int i = 0, done = 0;
+      bool ok = true;
+      for (int t = first; t < ntile && ok; t += stride, ++done) {
+        if (done > 0 && !wait_pair<true>(taken, (done - 1) & 1, ab)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int st = 0; st < steps; ++st, ++i) {
+          const int slot = i % S;
+          if (!wait_pair<true>(full0 + 8 * slot, (i / S) & 1, ab)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t at = sbase + slot * kStage, tsc = tmem + 256 + slot * kSlotCols;
+          const int nt = min(2, g.tiles - 2 * st);
+          for (int k = 0; k < nt; ++k) {
+            const uint32_t tp = tsc + k * 12, tq = tp + 4;
+            copy_scales<2>(tp, at + kSP + k * kPiece);
+            copy_scales<2>(tq, at + kSQ + k * kPiece);
+            copy_scales<2>(tq + 4, at + kSQ + (2 + k) * kPiece);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              mma_mx4<2>(tmem, sw128_desc(at + (2 * k + h) * 32), sw128_desc(at + kCodes + (2 * k + h) * 32),
+                         idesc_mx4<256, 256>(h), tp, tq, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
+          }
+          mma_commit_both(empty0 + 8 * slot);
+        }
+        if (ok) mma_commit_both(accbar);
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* stage = sm + kRing + (warp - 2) * kOutWarp;
+    const uint32_t took = mapa(taken, 0);
+    T* out = static_cast<T*>(g.out);
+    const bool rows16 = (uintptr_t)out % 16 == 0 && g.ld % 8 == 0;
+    int done = 0;
+    for (int t = first; t < ntile; t += stride, ++done) {
+      const int p0 = t % pt * 256 + (int)rank * 128 + quad * 32, q0 = t / pt * 256 + half * 128;
+      bool ok = true;
+      if (lane == 0) ok = wait_pair<false>(accbar, done & 1, ab) && !ab.raised();
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        float acc[32];
+        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + half * 128 + c, acc);
+        if (g.bias) {
+          const int q = q0 + c + lane;
+          const float mine = q < g.qrows ? DType<DT>::to_f32(static_cast<const T*>(g.bias)[q]) : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j] += __shfl_sync(0xffffffffu, mine, j);
+        }
+        uint4* to = reinterpret_cast<uint4*>(stage + lane * kOutPitch + c * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          to[j] = make_uint4(pack_rn<DT>(acc[8 * j], acc[8 * j + 1]), pack_rn<DT>(acc[8 * j + 2], acc[8 * j + 3]),
+                             pack_rn<DT>(acc[8 * j + 4], acc[8 * j + 5]), pack_rn<DT>(acc[8 * j + 6], acc[8 * j + 7]));
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(took);  // the accumulator is free for the next tile
+      if (rows16) {
+        // 16 bytes a lane, two rows at a time
+        const int q = q0 + lane % 16 * 8;
+#pragma unroll 4
+        for (int r = lane / 16; r < 32; r += 2) {
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * kOutPitch + lane % 16 * 16);
+          if (p0 + r < g.prows && q < g.qrows) *reinterpret_cast<uint4*>(out + (int64_t)(p0 + r) * g.ld + q) = v;
+        }
+      } else {
+#pragma unroll 1
+        for (int r = 0; r < 32 && p0 + r < g.prows; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int q = q0 + j * 32 + lane;
+            const T v = *reinterpret_cast<const T*>(stage + r * kOutPitch + (j * 32 + lane) * 2);
+            if (q < g.qrows) out[(int64_t)(p0 + r) * g.ld + q] = v;
+          }
+      }
+      __syncwarp();  // the staged rows are read before the next tile's are written
+    }
+  }
+
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();  // no copy, commit or arrive can reach a CTA that has left
+  if (tid == 0 && ab.raised()) {
+    // after a wait that ran out: this pair's MMAs (bounded), and time for
+    // copies and arrives under way to land
+    if (rank == 0) {
+      mma_commit_both(drainbar);
+      drain(drainbar, 0);
+    }
+    const uint64_t t0 = gtimer_ns();
+    while (gtimer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ------------------------------------------------------------------- host
+
+int launch(const void* kern, uint32_t smem, dim3 grid, dim3 cluster, const void* args, cudaStream_t st) {
+  const int rc = ensure_smem_limit(kern, smem);
   if (rc != RQ_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((g.qrows + BN - 1) / BN), (unsigned)((g.prows + kP - 1) / kP), (unsigned)sk);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Plan<BN>::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = 1;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = (unsigned)sk;
+  at[1].val.clusterDim.x = cluster.x;
+  at[1].val.clusterDim.y = cluster.y;
+  at[1].val.clusterDim.z = cluster.z;
   cfg.attrs = at;
-  cfg.numAttrs = sk > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_k<DT, BN, SWAP>, g);
+  cfg.numAttrs = cluster.x * cluster.z > 1 ? 2 : 1;
+  void* params[] = {const_cast<void*>(args)};
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, kern, params);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return RQ_ERR_CUDA;
@@ -341,40 +583,66 @@ int code_map(const Mx4& x, int64_t pitch, uint32_t rows, CUtensorMap* map) {
   return tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 2, x.codes, d, s, b, map);
 }
 
-// How often the columns are split: until the grid fills the GPU, with at least
-// two stages a CTA.
-int split_for(int64_t tiles, int64_t steps) {
-  int sk = 1;
-  while (sk < 8 && tiles * sk * 2 <= num_sms() && steps >= 4 * sk) sk *= 2;
-  return sk;
+int scale_map(const Mx4& x, int64_t pitch, CUtensorMap* map) {
+  const uint64_t d[3] = {128, (uint64_t)((x.rows + 127) / 128 * (pitch / 128)), 1}, s[2] = {kPiece, 0};
+  const uint32_t b[3] = {128, 2, 1};
+  return tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, 2, x.scales, d, s, b, map);
+}
+
+template <int DT, int BN>
+int split_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int sk, cudaStream_t st) {
+  const int64_t pitch = mx4_pitch(K);
+  Args g;
+  int rc = code_map(b, pitch, kP, &g.pmap);
+  if (rc == RQ_OK) rc = code_map(a, pitch, BN, &g.qmap);
+  if (rc != RQ_OK) return rc;
+  g.pscales = b.scales;
+  g.qscales = a.scales;
+  g.bias = bias;
+  g.out = out;
+  g.prows = (int)b.rows;
+  g.qrows = (int)a.rows;
+  g.tiles = (int)(pitch / 128);
+  g.ld = b.rows;
+  const dim3 grid((unsigned)((a.rows + BN - 1) / BN), (unsigned)((b.rows + kP - 1) / kP), (unsigned)sk);
+  return launch((const void*)mx4_split_k<DT, BN>, Plan<BN>::kSmem, grid, dim3(1, 1, (unsigned)sk), &g, st);
+}
+
+template <int DT>
+int pair_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
+  const int64_t pitch = mx4_pitch(K);
+  PairArgs g;
+  int rc = code_map(a, pitch, 128, &g.pmap);
+  if (rc == RQ_OK) rc = code_map(b, pitch, 128, &g.qmap);
+  if (rc == RQ_OK) rc = scale_map(a, pitch, &g.psmap);
+  if (rc == RQ_OK) rc = scale_map(b, pitch, &g.qsmap);
+  if (rc != RQ_OK) return rc;
+  g.bias = bias;
+  g.out = out;
+  g.prows = (int)a.rows;
+  g.qrows = (int)b.rows;
+  g.tiles = (int)(pitch / 128);
+  g.ld = b.rows;
+  const int64_t ntile = ((a.rows + 255) / 256) * ((b.rows + 255) / 256), pairs = num_sms() / 2;
+  return launch((const void*)mx4_pair_k<DT>, pair::kSmem, dim3((unsigned)(2 * (ntile < pairs ? ntile : pairs))),
+                dim3(2, 1, 1), &g, st);
 }
 
 template <int DT>
 int matmul_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
-  const int64_t pitch = mx4_pitch(K), steps = (pitch / 128 + 1) / 2;
-  const bool swap = a.rows <= 256;
-  const Mx4 &p = swap ? b : a, &q = swap ? a : b;
-  const int bn = !swap ? 256 : a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : a.rows <= 128 ? 128 : 256;
-  Args g;
-  int rc = code_map(p, pitch, kP, &g.pmap);
-  if (rc == RQ_OK) rc = code_map(q, pitch, (uint32_t)bn, &g.qmap);
-  if (rc != RQ_OK) return rc;
-  g.pscales = p.scales;
-  g.qscales = q.scales;
-  g.bias = bias;
-  g.out = out;
-  g.prows = (int)p.rows;
-  g.qrows = (int)q.rows;
-  g.tiles = (int)(pitch / 128);
-  g.ld = b.rows;
-  const int sk = split_for(((p.rows + kP - 1) / kP) * ((q.rows + bn - 1) / bn), steps);
-  if (!swap) return run<DT, 256, false>(g, sk, st);
+  const int64_t steps = (mx4_pitch(K) / 128 + 1) / 2, sms = num_sms();
+  if (a.rows > 256 && ((a.rows + 255) / 256) * ((b.rows + 255) / 256) * 2 >= sms / 2) return pair_t<DT>(a, b, K, bias, out, st);
+  // the narrowest tile that holds the tokens, or 128 of them; then columns are
+  // split until the grid fills the GPU, with at least two stages a CTA
+  const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
+  const int64_t tiles = ((b.rows + kP - 1) / kP) * ((a.rows + bn - 1) / bn);
+  int sk = 1;
+  while (sk < 8 && tiles * sk * 2 <= sms && steps >= 4 * sk) sk *= 2;
   switch (bn) {
-    case 16: return run<DT, 16, true>(g, sk, st);
-    case 32: return run<DT, 32, true>(g, sk, st);
-    case 64: return run<DT, 64, true>(g, sk, st);
-    case 128: return run<DT, 128, true>(g, sk, st);
-    default: return run<DT, 256, true>(g, sk, st);
+    case 16: return split_t<DT, 16>(a, b, K, bias, out, sk, st);
+    case 32: return split_t<DT, 32>(a, b, K, bias, out, sk, st);
+    case 64: return split_t<DT, 64>(a, b, K, bias, out, sk, st);
+    default: return split_t<DT, 128>(a, b, K, bias, out, sk, st);
   }
 }
 

@@ -141,7 +141,8 @@ def sums(a, b, k):
 
 SIZES = [(1, 1, 1), (1, 128, 16), (1, 4096, 130), (3, 33, 257), (16, 1024, 384), (17, 500, 128), (33, 300, 100),
          (64, 2048, 1088), (100, 128, 64), (128, 640, 129), (129, 1093, 70), (200, 256, 512), (256, 1280, 96),
-         (257, 200, 300), (300, 1093, 1089), (513, 1024, 640), (1000, 64, 255)]
+         (257, 200, 300), (300, 1093, 1089), (513, 1024, 640), (1000, 64, 255),
+         (2500, 300, 1000), (1300, 640, 2049), (6000, 1093, 2600)]
 
 
 @pytest.mark.gpu
