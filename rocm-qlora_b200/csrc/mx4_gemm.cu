@@ -96,12 +96,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // 32 rows of 16 bytes (8-row groups 128 bytes apart, no swizzle) to 4 columns
-// of all four lane quarters (of a pair: each CTA's from its own shared memory).
-template <int CTAS>
+// of all four lane quarters.
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
   const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-  if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
 // e2m1 operands, power-of-two scales; `half`: which two of a word's
@@ -215,9 +213,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
         const int nt = min(2, g.tiles - 2 * st);
         for (int t = 0; t < nt; ++t) {
           const uint32_t tp = tsc + t * (PL::kSlotCols / 2), tq = tp + 4;
-          copy_scales<1>(tp, at + PL::kSP + t * kPiece);
+          copy_scales(tp, at + PL::kSP + t * kPiece);
 #pragma unroll
-          for (int j = 0; j < NB; ++j) copy_scales<1>(tq + 4 * j, at + PL::kSQ + (2 * j + t) * kPiece);
+          for (int j = 0; j < NB; ++j) copy_scales(tq + 4 * j, at + PL::kSQ + (2 * j + t) * kPiece);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             mma_mx4<1>(tmem, sw128_desc(at + (2 * t + h) * 32), sw128_desc(at + kPBytes + (2 * t + h) * 32),
@@ -314,21 +312,23 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
 // ------------------------------------------------------------- CTA pairs
 
 namespace pair {
-constexpr int S = 4;
+constexpr int S = 6;                                        // stages of codes in shared memory
 constexpr uint32_t kCodes = 128 * 128;                      // of P's or of half of Q's rows
-constexpr uint32_t kSP = 2 * kCodes, kSQ = kSP + 2 * kPiece;  // scale pieces: P's two, Q's [half][two]
-constexpr uint32_t kStage = kSQ + 4 * kPiece;
-constexpr uint32_t kOutPitch = 256 + 16;                    // bytes of a staged row of 128 outputs
-constexpr uint32_t kOutWarp = 32 * kOutPitch;
-constexpr uint32_t kRing = S * kStage;
-constexpr uint32_t kSmem = kRing + kEpiWarps * kOutWarp + 1024;
-constexpr uint32_t kSlotCols = 2 * 12;                      // a 128 columns: P's 4, Q's 8
-static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024 && 256 + S * kSlotCols <= 512, "");
+constexpr uint32_t kStage = 2 * kCodes;
+constexpr uint32_t kOutWarp = 32 * 128;                     // staged: 32 rows of 64 outputs
+constexpr uint32_t kSmem = S * kStage + kEpiWarps * kOutWarp + 1024;
+constexpr int SS = 5;                                       // groups of two stages' scales in tensor memory
+constexpr uint32_t kGroupCols = 4 * 12;                     // for each 128 columns P's 4 and Q's 8
+constexpr int kScaleWarps = 4, kEpi0 = 2 + kScaleWarps;     // first epilogue warp
+constexpr int kThreads = 32 * (kEpi0 + kEpiWarps);
+constexpr int kAhead = 2;                                   // groups of scales on their way in registers
+static_assert(kSmem <= 226 * 1024 && 256 + SS * kGroupCols <= 512, "");
 }  // namespace pair
 
 struct PairArgs {
   CUtensorMap pmap, qmap;    // codes, boxes 128 bytes x 128 rows
-  CUtensorMap psmap, qsmap;  // scale pieces [pieces][128 words], boxes of two pieces
+  const uint8_t* pscales;
+  const uint8_t* qscales;
   const void* bias;
   void* out;
   int prows, qrows, tiles;
@@ -351,7 +351,16 @@ __device__ __forceinline__ void mma_commit_both(uint32_t bar) {
       : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t cbar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+}
+
+// 12 columns of this thread's lane
+__device__ __forceinline__ void tmem_st12(uint32_t taddr, const uint4 (&v)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr + 4 * i), "r"(v[i].x),
+                 "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
+                 : "memory");
 }
 
 // The abort state of a pair: this CTA's flag and the peer's.
@@ -360,12 +369,11 @@ struct PairAbort {
   uint32_t peer;
   __device__ __forceinline__ bool raised() const { return *mine != 0; }
 };
-template <bool kCluster>
 __device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
-  if (mbar_try<kCluster>(bar, parity)) return true;
+  if (mbar_try<false>(bar, parity)) return true;
   const uint64_t t0 = gtimer_ns();
   while (!ab.raised()) {
-    if (mbar_try<kCluster>(bar, parity)) return true;
+    if (mbar_try<false>(bar, parity)) return true;
     if (gtimer_ns() - t0 > kWaitNs) {
       *ab.mine = 1;
       st_cluster(ab.peer, 1);
@@ -378,35 +386,43 @@ __device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const P
 
 // out[p, q]: P tokens, Q outputs.
 template <int DT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pair_k(const __grid_constant__ PairArgs g) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) mx4_pair_k(const __grid_constant__ PairArgs g) {
   using namespace pair;
   using T = typename DType<DT>::T;
   extern __shared__ __align__(1024) unsigned char dsm[];
-  // full[S] (leader's counts both CTAs' bytes), empty[S], acc (sums complete),
-  // taken (leader's: both CTAs' epilogues have read them)
-  __shared__ __align__(8) uint64_t bars[2 * S + 3];
+  // full[S] (leader's: both CTAs' codes have landed), empty[S], sready[SS]
+  // (scales are in tensor memory; leader's: in both CTAs'), sfree[SS], acc
+  // (sums complete), taken (leader's: both CTAs' epilogues have read them)
+  __shared__ __align__(8) uint64_t bars[2 * S + 2 * SS + 3];
+  __shared__ __align__(16) uint32_t sig_src[4], sig_dst[4];  // the 16-byte signal copies (contents unused)
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster_rank();
   const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
   unsigned char* sm = dsm + (sbase - sraw);
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S, taken = accbar + 8,
-                 drainbar = taken + 8;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, sready0 = empty0 + 8 * S, sfree0 = sready0 + 8 * SS,
+                 accbar = sfree0 + 8 * SS, taken = accbar + 8, drainbar = taken + 8;
   const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u)};
   const int steps = (g.tiles + 1) / 2;
   const int pt = (g.prows + 255) / 256, qt = (g.qrows + 255) / 256, ntile = pt * qt;
   const int first = blockIdx.x / 2, stride = gridDim.x / 2;
+  const int groups = (steps + 1) / 2, total = first < ntile ? ((ntile - 1 - first) / stride + 1) * groups : 0;
 
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
+    for (int i = 0; i < SS; ++i) {
+      mbar_init(sready0 + 8 * i, kScaleWarps);
+      mbar_init(sfree0 + 8 * i, 1);
+    }
     mbar_init(accbar, 1);
     mbar_init(taken, 2 * kEpiWarps);
     mbar_init(drainbar, 1);
     abort_flag = 0;
+    for (int i = 0; i < 4; ++i) sig_src[i] = sig_dst[i] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -427,10 +443,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
       int i = 0;
       bool ok = true;
       for (int t = first; t < ntile && ok; t += stride) {
-        const int p0 = t % pt * 256 + (int)rank * 128, q0 = t / pt * 256, qh = q0 + (int)rank * 128;
+        const int p0 = t % pt * 256 + (int)rank * 128, qh = t / pt * 256 + (int)rank * 128;
         for (int st = 0; st < steps; ++st, ++i) {
           const int slot = i % S;
-          if (i >= S && !wait_pair<false>(empty0 + 8 * slot, ((i / S) - 1) & 1, ab)) {
+          if (i >= S && !wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab)) {
             ok = false;
             break;
           }
@@ -438,46 +454,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
           if (rank == 0) mbar_expect_tx(full0 + 8 * slot, 2 * kStage);
           tma_pair(at, &g.pmap, st * 128, p0, bar);
           tma_pair(at + kCodes, &g.qmap, st * 128, qh, bar);
-          tma_pair(at + kSP, &g.psmap, 0, p0 / 128 * g.tiles + 2 * st, bar);
-          tma_pair(at + kSQ, &g.qsmap, 0, q0 / 128 * g.tiles + 2 * st, bar);
-          tma_pair(at + kSQ + 2 * kPiece, &g.qsmap, 0, (q0 / 128 + 1) * g.tiles + 2 * st, bar);
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int i = 0, done = 0;
+      int i = 0, gi = 0, done = 0;  // stages, groups, tiles
       bool ok = true;
       for (int t = first; t < ntile && ok; t += stride, ++done) {
-        if (done > 0 && !wait_pair<true>(taken, (done - 1) & 1, ab)) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (done > 0 && !wait_pair(taken, (done - 1) & 1, ab)) break;
         for (int st = 0; st < steps; ++st, ++i) {
-          const int slot = i % S;
-          if (!wait_pair<true>(full0 + 8 * slot, (i / S) & 1, ab)) {
+          const int slot = i % S, ss = gi % SS;
+          if (st % 2 == 0 && !wait_pair(sready0 + 8 * ss, (gi / SS) & 1, ab)) ok = false;
+          if (!ok || !wait_pair(full0 + 8 * slot, (i / S) & 1, ab)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t at = sbase + slot * kStage, tsc = tmem + 256 + slot * kSlotCols;
+          const uint32_t at = sbase + slot * kStage, tsc = tmem + 256 + ss * kGroupCols + (st & 1) * 24;
           const int nt = min(2, g.tiles - 2 * st);
-          for (int k = 0; k < nt; ++k) {
-            const uint32_t tp = tsc + k * 12, tq = tp + 4;
-            copy_scales<2>(tp, at + kSP + k * kPiece);
-            copy_scales<2>(tq, at + kSQ + k * kPiece);
-            copy_scales<2>(tq + 4, at + kSQ + (2 + k) * kPiece);
+          for (int k = 0; k < nt; ++k)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               mma_mx4<2>(tmem, sw128_desc(at + (2 * k + h) * 32), sw128_desc(at + kCodes + (2 * k + h) * 32),
-                         idesc_mx4<256, 256>(h), tp, tq, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
-          }
+                         idesc_mx4<256, 256>(h), tsc + k * 12, tsc + k * 12 + 4, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
           mma_commit_both(empty0 + 8 * slot);
+          if (st % 2 == 1 || st + 1 == steps) {
+            mma_commit_both(sfree0 + 8 * ss);
+            ++gi;
+          }
         }
         if (ok) mma_commit_both(accbar);
       }
+    } else if (lane == 0) {
+      // the peer's scales are in place: a signal that no fence holds up
+      bool ok = true;
+      for (int i = 0; i < total && ok; ++i) {
+        ok = wait_pair(sready0 + 8 * (i % SS), (i / SS) & 1, ab);
+        if (ok) bulk_signal(mapa(smem_u32(sig_dst), 0), smem_u32(sig_src), mapa(sready0 + 8 * (i % SS), 0));
+      }
+    }
+  } else if (warp < kEpi0) {
+    // ------------------------- scales to this warp's quarter of the lanes:
+    // lane l has 4 bytes of row l of each group of 32 rows.  Pieces past the
+    // last row or column are not read; what they would scale is 0 or not stored.
+    const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+    struct Group {
+      uint4 v[4][3];
+    };
+    int ft = first, fg = 0;  // tile and group of the next load
+    auto fetch = [&](Group& x) {
+      if (ft >= ntile) return;
+      const int p0 = ft % pt * 256 + (int)rank * 128, q0 = ft / pt * 256;
+      const int rows[3] = {p0, q0, q0 + 128}, most[3] = {g.prows, g.qrows, g.qrows};
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        const uint8_t* from = (j == 0 ? g.pscales : g.qscales) + ((int64_t)(rows[j] / 128) * g.tiles + 4 * fg) * kPiece +
+                              lane * 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x.v[k][j] = rows[j] < most[j] && 4 * fg + k < g.tiles ? __ldg(reinterpret_cast<const uint4*>(from + k * kPiece))
+                                                                 : make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (++fg == groups) fg = 0, ft += stride;
+    };
+    Group ring[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) fetch(ring[j]);
+    bool ok = true;
+    for (int i0 = 0; i0 < total && ok; i0 += kAhead) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j, ss = i % SS;
+        if (!ok || i >= total) break;
+        if (i >= SS) {
+          if (lane == 0) ok = wait_pair(sfree0 + 8 * ss, ((i / SS) - 1) & 1, ab);
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        const uint32_t to = tmem + quarter + 256 + ss * kGroupCols;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tmem_st12(to + 12 * k, ring[j].v[k]);
+        fetch(ring[j]);
+        asm volatile("tcgen05.wait::st.sync.aligned;\n\ttcgen05.fence::before_thread_sync;" ::: "memory");
+        if (lane == 0) {
+          if (rank == 0 && warp == 2) mbar_expect_tx(sready0 + 8 * ss, 16);  // the peer's signal
+          else mbar_arrive(sready0 + 8 * ss);
+        }
+      }
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    unsigned char* stage = sm + kRing + (warp - 2) * kOutWarp;
+    const int quad = warp & 3, half = (warp - kEpi0) >> 2;
+    unsigned char* stage = sm + S * kStage + (warp - kEpi0) * kOutWarp;
     const uint32_t took = mapa(taken, 0);
     T* out = static_cast<T*>(g.out);
     const bool rows16 = (uintptr_t)out % 16 == 0 && g.ld % 8 == 0;
@@ -485,47 +554,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     for (int t = first; t < ntile; t += stride, ++done) {
       const int p0 = t % pt * 256 + (int)rank * 128 + quad * 32, q0 = t / pt * 256 + half * 128;
       bool ok = true;
-      if (lane == 0) ok = wait_pair<false>(accbar, done & 1, ab) && !ab.raised();
+      if (lane == 0) ok = wait_pair(accbar, done & 1, ab) && !ab.raised();
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
+      uint4 w[16];  // this lane's row: 128 outputs, 8 a piece
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
         float acc[32];
-        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + half * 128 + c, acc);
+        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + half * 128 + c * 32, acc);
         if (g.bias) {
-          const int q = q0 + c + lane;
+          const int q = q0 + c * 32 + lane;
           const float mine = q < g.qrows ? DType<DT>::to_f32(static_cast<const T*>(g.bias)[q]) : 0.0f;
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[j] += __shfl_sync(0xffffffffu, mine, j);
         }
-        uint4* to = reinterpret_cast<uint4*>(stage + lane * kOutPitch + c * 2);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          to[j] = make_uint4(pack_rn<DT>(acc[8 * j], acc[8 * j + 1]), pack_rn<DT>(acc[8 * j + 2], acc[8 * j + 3]),
-                             pack_rn<DT>(acc[8 * j + 4], acc[8 * j + 5]), pack_rn<DT>(acc[8 * j + 6], acc[8 * j + 7]));
+          w[4 * c + j] =
+              make_uint4(pack_rn<DT>(acc[8 * j], acc[8 * j + 1]), pack_rn<DT>(acc[8 * j + 2], acc[8 * j + 3]),
+                         pack_rn<DT>(acc[8 * j + 4], acc[8 * j + 5]), pack_rn<DT>(acc[8 * j + 6], acc[8 * j + 7]));
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive_cluster(took);  // the accumulator is free for the next tile
-      if (rows16) {
-        // 16 bytes a lane, two rows at a time
-        const int q = q0 + lane % 16 * 8;
-#pragma unroll 4
-        for (int r = lane / 16; r < 32; r += 2) {
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * kOutPitch + lane % 16 * 16);
-          if (p0 + r < g.prows && q < g.qrows) *reinterpret_cast<uint4*>(out + (int64_t)(p0 + r) * g.ld + q) = v;
-        }
-      } else {
-#pragma unroll 1
-        for (int r = 0; r < 32 && p0 + r < g.prows; ++r)
+      // through shared memory, 64 outputs at a time, to stores of whole 128-byte
+      // row pieces; piece j of row r is at j ^ (r % 8)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int q = q0 + j * 32 + lane;
-            const T v = *reinterpret_cast<const T*>(stage + r * kOutPitch + (j * 32 + lane) * 2);
-            if (q < g.qrows) out[(int64_t)(p0 + r) * g.ld + q] = v;
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w[8 * h + j];
+        __syncwarp();
+        if (rows16) {
+          const int q = q0 + h * 64 + lane % 8 * 8;
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 4) {
+            const int r = r0 + lane / 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8 ^ (r & 7)) << 4));
+            if (p0 + r < g.prows && q < g.qrows) *reinterpret_cast<uint4*>(out + (int64_t)(p0 + r) * g.ld + q) = v;
           }
+        } else {
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int c = j * 32 + lane, q = q0 + h * 64 + c;
+              const T v = *reinterpret_cast<const T*>(stage + r * 128 + ((c / 8 ^ (r & 7)) << 4) + c % 8 * 2);
+              if (p0 + r < g.prows && q < g.qrows) out[(int64_t)(p0 + r) * g.ld + q] = v;
+            }
+        }
+        __syncwarp();  // the staged rows are read before the next ones are written
       }
-      __syncwarp();  // the staged rows are read before the next tile's are written
     }
   }
 
@@ -551,12 +630,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
 
 // ------------------------------------------------------------------- host
 
-int launch(const void* kern, uint32_t smem, dim3 grid, dim3 cluster, const void* args, cudaStream_t st) {
+int launch(const void* kern, uint32_t smem, dim3 grid, int threads, dim3 cluster, const void* args, cudaStream_t st) {
   const int rc = ensure_smem_limit(kern, smem);
   if (rc != RQ_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -583,12 +662,6 @@ int code_map(const Mx4& x, int64_t pitch, uint32_t rows, CUtensorMap* map) {
   return tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 2, x.codes, d, s, b, map);
 }
 
-int scale_map(const Mx4& x, int64_t pitch, CUtensorMap* map) {
-  const uint64_t d[3] = {128, (uint64_t)((x.rows + 127) / 128 * (pitch / 128)), 1}, s[2] = {kPiece, 0};
-  const uint32_t b[3] = {128, 2, 1};
-  return tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, 2, x.scales, d, s, b, map);
-}
-
 template <int DT, int BN>
 int split_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int sk, cudaStream_t st) {
   const int64_t pitch = mx4_pitch(K);
@@ -605,7 +678,7 @@ int split_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, 
   g.tiles = (int)(pitch / 128);
   g.ld = b.rows;
   const dim3 grid((unsigned)((a.rows + BN - 1) / BN), (unsigned)((b.rows + kP - 1) / kP), (unsigned)sk);
-  return launch((const void*)mx4_split_k<DT, BN>, Plan<BN>::kSmem, grid, dim3(1, 1, (unsigned)sk), &g, st);
+  return launch((const void*)mx4_split_k<DT, BN>, Plan<BN>::kSmem, grid, kThreads, dim3(1, 1, (unsigned)sk), &g, st);
 }
 
 template <int DT>
@@ -614,9 +687,9 @@ int pair_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, c
   PairArgs g;
   int rc = code_map(a, pitch, 128, &g.pmap);
   if (rc == RQ_OK) rc = code_map(b, pitch, 128, &g.qmap);
-  if (rc == RQ_OK) rc = scale_map(a, pitch, &g.psmap);
-  if (rc == RQ_OK) rc = scale_map(b, pitch, &g.qsmap);
   if (rc != RQ_OK) return rc;
+  g.pscales = a.scales;
+  g.qscales = b.scales;
   g.bias = bias;
   g.out = out;
   g.prows = (int)a.rows;
@@ -625,7 +698,7 @@ int pair_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, c
   g.ld = b.rows;
   const int64_t ntile = ((a.rows + 255) / 256) * ((b.rows + 255) / 256), pairs = num_sms() / 2;
   return launch((const void*)mx4_pair_k<DT>, pair::kSmem, dim3((unsigned)(2 * (ntile < pairs ? ntile : pairs))),
-                dim3(2, 1, 1), &g, st);
+                pair::kThreads, dim3(2, 1, 1), &g, st);
 }
 
 template <int DT>
