@@ -312,17 +312,18 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
 // ------------------------------------------------------------- CTA pairs
 
 namespace pair {
-constexpr int S = 6;                                        // stages of codes in shared memory
-constexpr uint32_t kCodes = 128 * 128;                      // of P's or of half of Q's rows
-constexpr uint32_t kStage = 2 * kCodes;
+// A stage holds 512 columns here: a wait or a commit costs the tensor pipe about
+// 100 cycles, next to the 1082 of a stage's 8 MMAs.
+constexpr int S = 3;
+constexpr uint32_t kCodes = 128 * 128;                      // 256 columns of P's or of half of Q's rows
+constexpr uint32_t kStage = 4 * kCodes;                     // P's two, Q's two
 constexpr uint32_t kOutWarp = 32 * 128;                     // staged: 32 rows of 64 outputs
 constexpr uint32_t kSmem = S * kStage + kEpiWarps * kOutWarp + 1024;
-constexpr int SS = 5;                                       // groups of two stages' scales in tensor memory
-constexpr uint32_t kGroupCols = 4 * 12;                     // for each 128 columns P's 4 and Q's 8
+constexpr uint32_t kSlotCols = 4 * 12;                      // scales: for each 128 columns P's 4 and Q's 8
 constexpr int kScaleWarps = 4, kEpi0 = 2 + kScaleWarps;     // first epilogue warp
 constexpr int kThreads = 32 * (kEpi0 + kEpiWarps);
-constexpr int kAhead = 2;                                   // groups of scales on their way in registers
-static_assert(kSmem <= 226 * 1024 && 256 + SS * kGroupCols <= 512, "");
+constexpr int kAhead = 2;                                   // stages of scales on their way in registers
+static_assert(kSmem <= 226 * 1024 && 256 + S * kSlotCols <= 512, "");
 }  // namespace pair
 
 struct PairArgs {
@@ -350,6 +351,7 @@ __device__ __forceinline__ void mma_commit_both(uint32_t bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// What the arrival tells of is in tensor memory, which its own fence orders.
 __device__ __forceinline__ void arrive_cluster(uint32_t cbar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
 }
@@ -390,39 +392,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
   using namespace pair;
   using T = typename DType<DT>::T;
   extern __shared__ __align__(1024) unsigned char dsm[];
-  // full[S] (leader's: both CTAs' codes have landed), empty[S], sready[SS]
-  // (scales are in tensor memory; leader's: in both CTAs'), sfree[SS], acc
-  // (sums complete), taken (leader's: both CTAs' epilogues have read them)
-  __shared__ __align__(8) uint64_t bars[2 * S + 2 * SS + 3];
-  __shared__ __align__(16) uint32_t sig_src[4], sig_dst[4];  // the 16-byte signal copies (contents unused)
+  // full[S] (leader's: both CTAs' codes have landed and scales are in both
+  // tensor memories), empty[S], acc (sums complete), taken (leader's: both
+  // CTAs' epilogues have read them)
+  __shared__ __align__(8) uint64_t bars[2 * S + 3];
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster_rank();
   const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
   unsigned char* sm = dsm + (sbase - sraw);
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, sready0 = empty0 + 8 * S, sfree0 = sready0 + 8 * SS,
-                 accbar = sfree0 + 8 * SS, taken = accbar + 8, drainbar = taken + 8;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S, taken = accbar + 8,
+                 drainbar = taken + 8, lead = mapa(full0, 0);
   const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u)};
-  const int steps = (g.tiles + 1) / 2;
+  const int steps = (g.tiles + 3) / 4;
   const int pt = (g.prows + 255) / 256, qt = (g.qrows + 255) / 256, ntile = pt * qt;
   const int first = blockIdx.x / 2, stride = gridDim.x / 2;
-  const int groups = (steps + 1) / 2, total = first < ntile ? ((ntile - 1 - first) / stride + 1) * groups : 0;
+  const int total = first < ntile ? ((ntile - 1 - first) / stride + 1) * steps : 0;  // stages
 
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(full0 + 8 * i, 1);
+      mbar_init(full0 + 8 * i, 1 + 2 * kScaleWarps);
       mbar_init(empty0 + 8 * i, 1);
-    }
-    for (int i = 0; i < SS; ++i) {
-      mbar_init(sready0 + 8 * i, kScaleWarps);
-      mbar_init(sfree0 + 8 * i, 1);
     }
     mbar_init(accbar, 1);
     mbar_init(taken, 2 * kEpiWarps);
     mbar_init(drainbar, 1);
     abort_flag = 0;
-    for (int i = 0; i < 4; ++i) sig_src[i] = sig_dst[i] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -439,7 +435,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t lead = mapa(full0, 0);
       int i = 0;
       bool ok = true;
       for (int t = first; t < ntile && ok; t += stride) {
@@ -452,46 +447,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
           }
           const uint32_t at = sbase + slot * kStage, bar = lead + 8 * slot;
           if (rank == 0) mbar_expect_tx(full0 + 8 * slot, 2 * kStage);
-          tma_pair(at, &g.pmap, st * 128, p0, bar);
-          tma_pair(at + kCodes, &g.qmap, st * 128, qh, bar);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            tma_pair(at + j * kCodes, &g.pmap, st * 256 + j * 128, p0, bar);
+            tma_pair(at + (2 + j) * kCodes, &g.qmap, st * 256 + j * 128, qh, bar);
+          }
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int i = 0, gi = 0, done = 0;  // stages, groups, tiles
+      int i = 0, done = 0;  // stages, tiles
       bool ok = true;
       for (int t = first; t < ntile && ok; t += stride, ++done) {
         if (done > 0 && !wait_pair(taken, (done - 1) & 1, ab)) break;
         for (int st = 0; st < steps; ++st, ++i) {
-          const int slot = i % S, ss = gi % SS;
-          if (st % 2 == 0 && !wait_pair(sready0 + 8 * ss, (gi / SS) & 1, ab)) ok = false;
-          if (!ok || !wait_pair(full0 + 8 * slot, (i / S) & 1, ab)) {
+          const int slot = i % S;
+          if (!wait_pair(full0 + 8 * slot, (i / S) & 1, ab)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t at = sbase + slot * kStage, tsc = tmem + 256 + ss * kGroupCols + (st & 1) * 24;
-          const int nt = min(2, g.tiles - 2 * st);
-          for (int k = 0; k < nt; ++k)
+          const uint32_t at = sbase + slot * kStage, tsc = tmem + 256 + slot * kSlotCols;
+          const int nt = min(4, g.tiles - 4 * st);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              mma_mx4<2>(tmem, sw128_desc(at + (2 * k + h) * 32), sw128_desc(at + kCodes + (2 * k + h) * 32),
-                         idesc_mx4<256, 256>(h), tsc + k * 12, tsc + k * 12 + 4, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k)
+            if (k < nt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t a = at + (k / 2) * kCodes + (k % 2 * 2 + h) * 32;
+                mma_mx4<2>(tmem, sw128_desc(a), sw128_desc(a + 2 * kCodes), idesc_mx4<256, 256>(h), tsc + k * 12,
+                           tsc + k * 12 + 4, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
+              }
           mma_commit_both(empty0 + 8 * slot);
-          if (st % 2 == 1 || st + 1 == steps) {
-            mma_commit_both(sfree0 + 8 * ss);
-            ++gi;
-          }
         }
         if (ok) mma_commit_both(accbar);
-      }
-    } else if (lane == 0) {
-      // the peer's scales are in place: a signal that no fence holds up
-      bool ok = true;
-      for (int i = 0; i < total && ok; ++i) {
-        ok = wait_pair(sready0 + 8 * (i % SS), (i / SS) & 1, ab);
-        if (ok) bulk_signal(mapa(smem_u32(sig_dst), 0), smem_u32(sig_src), mapa(sready0 + 8 * (i % SS), 0));
       }
     }
   } else if (warp < kEpi0) {
@@ -499,49 +489,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
     // lane l has 4 bytes of row l of each group of 32 rows.  Pieces past the
     // last row or column are not read; what they would scale is 0 or not stored.
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-    struct Group {
+    struct Scales {
       uint4 v[4][3];
     };
-    int ft = first, fg = 0;  // tile and group of the next load
-    auto fetch = [&](Group& x) {
+    int ft = first, fs = 0;  // tile and stage of the next load
+    auto fetch = [&](Scales& x) {
       if (ft >= ntile) return;
       const int p0 = ft % pt * 256 + (int)rank * 128, q0 = ft / pt * 256;
       const int rows[3] = {p0, q0, q0 + 128}, most[3] = {g.prows, g.qrows, g.qrows};
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
-        const uint8_t* from = (j == 0 ? g.pscales : g.qscales) + ((int64_t)(rows[j] / 128) * g.tiles + 4 * fg) * kPiece +
+        const uint8_t* from = (j == 0 ? g.pscales : g.qscales) + ((int64_t)(rows[j] / 128) * g.tiles + 4 * fs) * kPiece +
                               lane * 16;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          x.v[k][j] = rows[j] < most[j] && 4 * fg + k < g.tiles ? __ldg(reinterpret_cast<const uint4*>(from + k * kPiece))
+          x.v[k][j] = rows[j] < most[j] && 4 * fs + k < g.tiles ? __ldg(reinterpret_cast<const uint4*>(from + k * kPiece))
                                                                  : make_uint4(0u, 0u, 0u, 0u);
       }
-      if (++fg == groups) fg = 0, ft += stride;
+      if (++fs == steps) fs = 0, ft += stride;
     };
-    Group ring[kAhead];
+    Scales ring[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) fetch(ring[j]);
     bool ok = true;
     for (int i0 = 0; i0 < total && ok; i0 += kAhead) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const int i = i0 + j, ss = i % SS;
+        const int i = i0 + j, slot = i % S;
         if (!ok || i >= total) break;
-        if (i >= SS) {
-          if (lane == 0) ok = wait_pair(sfree0 + 8 * ss, ((i / SS) - 1) & 1, ab);
+        if (i >= S) {
+          if (lane == 0) ok = wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab);
           ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        const uint32_t to = tmem + quarter + 256 + ss * kGroupCols;
+        const uint32_t to = tmem + quarter + 256 + slot * kSlotCols;
 #pragma unroll
         for (int k = 0; k < 4; ++k) tmem_st12(to + 12 * k, ring[j].v[k]);
         fetch(ring[j]);
         asm volatile("tcgen05.wait::st.sync.aligned;\n\ttcgen05.fence::before_thread_sync;" ::: "memory");
-        if (lane == 0) {
-          if (rank == 0 && warp == 2) mbar_expect_tx(sready0 + 8 * ss, 16);  // the peer's signal
-          else mbar_arrive(sready0 + 8 * ss);
-        }
+        if (lane == 0) arrive_cluster(lead + 8 * slot);
       }
     }
   } else {
