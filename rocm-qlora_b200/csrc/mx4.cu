@@ -4,9 +4,10 @@
 // codes are those of the definition bit for bit.
 //
 // One pass over the data.  4 lanes hold a block and 16 a piece of 128 columns
-// (8 values a lane: one 16-byte load of a 16-bit type); the piece's four scale
-// bytes are written as one word.  Rows past M up to whole pieces of 128 are
-// warps of their own that write zero scales.
+// (8 values a lane: one 16-byte load of a 16-bit type).  To pack, 16 lanes take
+// rows r, r + 32, r + 64 and r + 96 of 128: four loads on their way at once, and
+// their 16 scale bytes lie side by side.  Rows past M up to whole pieces of 128
+// count as zeros.
 #include <cuda_runtime.h>
 
 #include "mx4_common.cuh"
@@ -68,13 +69,8 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float by) {
   return w;
 }
 
-// The scale byte of a block of which each of 4 neighbouring lanes has 8 values.
-__device__ __forceinline__ uint32_t m4_scale(const float (&v)[8]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+// The scale byte of a block whose largest magnitude has these bits.
+__device__ __forceinline__ uint32_t m4_scale(uint32_t top) {
   const uint32_t e = top >> 23;  // 127 + floor(log2 top), 0 below 2^-126
   return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
 }
@@ -82,30 +78,62 @@ __device__ __forceinline__ uint32_t m4_scale(const float (&v)[8]) {
 // 2^(127 - byte), the factor that takes values to codes.
 __device__ __forceinline__ float m4_factor(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
 
-template <int DT, bool VEC>
+// A warp has 256 columns of 4 rows.
+template <int DT, bool VEC, bool TOP>
 __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict__ x, int64_t ld, int64_t M, int K,
-                                                         uint32_t pieces, M4Divide nt, uint8_t* __restrict__ codes,
-                                                         uint8_t* __restrict__ scales, int32_t* __restrict__ top) {
+                                                         uint32_t warps, M4Divide np, int tiles,
+                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                         int32_t* __restrict__ most) {
   grid_begin();
   using T = typename DType<DT>::T;
-  const uint32_t p = blockIdx.x * kM4PerCta + threadIdx.x / kM4Lanes;
-  const int l = threadIdx.x % kM4Lanes;
-  const bool in = p < pieces;
-  const uint32_t row = in ? (uint32_t)(((uint64_t)p * nt.mul) >> nt.shift) : 0u, tile = in ? p - row * nt.by : 0u;
-  const bool any = in && row < M;
-  float v[8];
-  m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), (int)tile * 128 + l * 8, any ? K : 0, v);
-  const uint32_t byte = m4_scale(v);
-  const uint32_t w = e2m1x8(v, m4_factor(byte));
-  if (any) *reinterpret_cast<uint32_t*>(codes + ((int64_t)row * nt.by + tile) * 64 + l * 4) = w;
-  const uint32_t b0 = __shfl_sync(0xffffffffu, byte, 0, kM4Lanes), b1 = __shfl_sync(0xffffffffu, byte, 4, kM4Lanes),
-                 b2 = __shfl_sync(0xffffffffu, byte, 8, kM4Lanes), b3 = __shfl_sync(0xffffffffu, byte, 12, kM4Lanes);
-  if (in && l == 0)
-    *reinterpret_cast<uint32_t*>(scales + ((int64_t)(row / 128) * nt.by + tile) * 512 + row % 32 * 16 + row % 128 / 32 * 4) =
-        b0 | b1 << 8 | b2 << 16 | b3 << 24;
-  if (top) {
-    const int most = (int)__reduce_max_sync(0xffffffffu, any && byte != 255u ? byte : 0u);
-    if (threadIdx.x % 32 == 0 && most > *reinterpret_cast<volatile int32_t*>(top)) atomicMax(top, most);
+  const uint32_t p = blockIdx.x * (kM4Threads / 32) + threadIdx.x / 32;
+  const uint32_t q = (uint32_t)(((uint64_t)p * np.mul) >> np.shift);  // 32 groups of 4 rows to a tile of 128
+  const int l = threadIdx.x % kM4Lanes, tile = (int)(p - q * np.by) * 2 + threadIdx.x / kM4Lanes % 2;
+  const bool in = p < warps && tile < tiles;
+  const int64_t row0 = (int64_t)(q / 32) * 128 + q % 32;
+  const int col = tile * 128 + l * 8;
+  float v[4][8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = row0 + 32 * j;
+    const bool any = in && row < M;
+    m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), col, any ? K : 0, v[j]);
+  }
+  uint32_t bytes = 0, top = 0;  // row j's scale of this lane's block in byte j
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t byte = m4_scale(m);
+    bytes |= byte << (8 * j);
+    if (TOP && byte != 255u) top = max(top, byte);
+    const uint32_t w = e2m1x8(v[j], m4_factor(byte));
+    const int64_t row = row0 + 32 * j;
+    if (in && row < M) *reinterpret_cast<uint32_t*>(codes + (row * tiles + tile) * 64 + l * 4) = w;
+  }
+  uint32_t b[4];  // the four blocks' bytes, to be turned into the four rows'
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __shfl_sync(0xffffffffu, bytes, 4 * i, kM4Lanes);
+  if (in && l == 0) {
+    const uint32_t lo01 = __byte_perm(b[0], b[1], 0x5140), hi01 = __byte_perm(b[0], b[1], 0x7362),
+                   lo23 = __byte_perm(b[2], b[3], 0x5140), hi23 = __byte_perm(b[2], b[3], 0x7362);
+    *reinterpret_cast<uint4*>(scales + ((row0 / 128) * tiles + tile) * 512 + row0 % 32 * 16) =
+        make_uint4(__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410),
+                   __byte_perm(hi01, hi23, 0x7632));
+  }
+  if constexpr (TOP) {
+    __shared__ uint32_t part[kM4Threads / 32];
+    top = __reduce_max_sync(0xffffffffu, in ? top : 0u);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int i = 1; i < kM4Threads / 32; ++i) top = max(top, part[i]);
+      atomicMax(most, (int32_t)top);
+    }
   }
 }
 
@@ -152,23 +180,32 @@ static bool m4_rows(const void* p, int64_t ld, int64_t K, int dt) {
   return (uintptr_t)p % 16 == 0 && ld * (dt == RQ_F32 ? 4 : 2) % 16 == 0 && K % 8 == 0;
 }
 
+template <int DT, bool TOP>
+static int m4_pack_t(const void* x, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
+                     cudaStream_t st) {
+  const int tiles = (int)(mx4_pitch(K) / 128);
+  const M4Divide np = m4_divide((uint32_t)(tiles + 1) / 2);
+  const uint32_t warps = (uint32_t)((M + 127) / 128 * 32) * np.by;
+  auto* k = m4_rows(x, ld, K, DT) ? mx4_pack_k<DT, true, TOP> : mx4_pack_k<DT, false, TOP>;
+  return launch_dependent(k, (warps + kM4Threads / 32 - 1) / (kM4Threads / 32), kM4Threads, st, x, ld, M, (int)K, warps, np,
+                          tiles, codes, scales, top);
+}
+
 int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
              cudaStream_t st) {
-  const M4Divide nt = m4_divide((uint32_t)(mx4_pitch(K) / 128));
-  const uint32_t pieces = (uint32_t)((M + 127) / 128 * 128) * nt.by;
   if (top) {
     const cudaError_t e = cudaMemsetAsync(top, 0, 4, st);
     if (e != cudaSuccess) {
       set_cuda_error(e);
       return RQ_ERR_CUDA;
     }
+    return dt == RQ_F32    ? m4_pack_t<RQ_F32, true>(x, ld, M, K, codes, scales, top, st)
+           : dt == RQ_BF16 ? m4_pack_t<RQ_BF16, true>(x, ld, M, K, codes, scales, top, st)
+                           : m4_pack_t<RQ_F16, true>(x, ld, M, K, codes, scales, top, st);
   }
-  const bool vec = m4_rows(x, ld, K, dt);
-  auto* k = dt == RQ_F32 ? (vec ? mx4_pack_k<RQ_F32, true> : mx4_pack_k<RQ_F32, false>)
-            : dt == RQ_BF16 ? (vec ? mx4_pack_k<RQ_BF16, true> : mx4_pack_k<RQ_BF16, false>)
-                            : (vec ? mx4_pack_k<RQ_F16, true> : mx4_pack_k<RQ_F16, false>);
-  return launch_dependent(k, (pieces + kM4PerCta - 1) / kM4PerCta, kM4Threads, st, x, ld, M, (int)K, pieces, nt, codes,
-                          scales, top);
+  return dt == RQ_F32    ? m4_pack_t<RQ_F32, false>(x, ld, M, K, codes, scales, top, st)
+         : dt == RQ_BF16 ? m4_pack_t<RQ_BF16, false>(x, ld, M, K, codes, scales, top, st)
+                         : m4_pack_t<RQ_F16, false>(x, ld, M, K, codes, scales, top, st);
 }
 
 int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st) {
