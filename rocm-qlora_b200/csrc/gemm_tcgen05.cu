@@ -61,7 +61,6 @@
 #include <vector>
 
 #include "gemv_common.cuh"
-#include "mx4_common.cuh"
 #include "rq_internal.h"
 #include "tcgen05_common.cuh"
 
@@ -137,10 +136,6 @@ struct GemmArgs {
   void* y;            // Y [M][N] (dX: dX [M][K])
   int M, N, K, r;
   float s;            // LoRA scaling (dX: 1, gt already carries it)
-  // microscaled weights (dX): scale pieces, largest scale byte, padded columns
-  const uint8_t* mx_scales;
-  const int32_t* mx_top;
-  int pitch;
 };
 
 // The abort state of a CTA pair: this CTA's flag and the peer's (remote).
@@ -176,44 +171,6 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < kWaitLimit && !mbar_test<false>(bar, parity); ++i) __nanosleep(kPollNs);
 }
 
-// Shared-memory descriptor of an MN-major operand with 128-byte swizzle:
-// rows (K) of 128 bytes = 64 MN elements, 8-row groups 1024 bytes apart,
-// 64-element MN groups `lbo` bytes apart.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-// Instruction descriptor: 16-bit A/B of type DT, fp32 accumulate, A K-major,
-// B K-major (or MN-major), M = 256 (the CTA pair), N = BN.
-template <int DT, int BN>
-__device__ __forceinline__ uint32_t idesc_pair(bool b_mn = false) {
-  const uint32_t ab = DT == RQ_BF16 ? 1u : 0u;
-  return (1u << 4) | (ab << 7) | (ab << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
-         ((uint32_t)(256 >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accum)
-      : "memory");
-}
-// Arrive on the barrier at shared::cta offset `bar` of each CTA in `mask`
-// once every MMA this thread issued so far has completed.
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t mask) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"(mask)
-      : "memory");
-}
-
 // Two 32-column loads (base and LoRA accumulators of the same rows) under
 // one wait: one tensor-memory round trip instead of two.
 __device__ __forceinline__ void tmem_ld32x2(uint32_t ta, uint32_t tb, float (&a)[32], float (&b)[32]) {
@@ -246,11 +203,7 @@ __device__ __forceinline__ float ldg_pin_f32(const void* p) {
   return v;
 }
 
-// MX (dX only): codes are e2m1, with a power of two as the scale of 32 columns,
-// and N, which the reduction runs over, is any number (rows past it are zeros
-// by the TMA bounds).  In bf16 the weights are exact; in f16 they are taken
-// relative to the weight's largest scale, which the epilogue multiplies back.
-template <int DT, bool DX, int BN, bool I8, bool MX = false>
+template <int DT, bool DX, int BN, bool I8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(const __grid_constant__ GemmArgs g) {
   using TL = Tile<BN, I8>;
   using T = typename DType<DT>::T;
@@ -276,7 +229,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
 
   const int M = g.M, N = g.N, K = g.K;
   const int W_out = DX ? K : N;       // output columns
-  const int nkb = MX ? (N + BK - 1) / BK : (DX ? N : K) / BK;  // reduction steps
+  const int nkb = (DX ? N : K) / BK;  // reduction steps
   const int n0 = blockIdx.y * BN;     // the pair's first output column
   const int nh0 = n0 + (int)rank * BNH;  // this CTA's half: weight rows (forward) / output columns (dX)
   const int m0 = (blockIdx.z * 2 + (int)rank) * BM;  // this CTA's token rows
@@ -313,10 +266,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
   float* sclut = reinterpret_cast<float*>(sm + TL::kSmScl);
   for (int i = tid; i < 256 * kLutReps; i += kThreads) {
     const int v = i / kLutReps;
-    if constexpr (MX) lutp[i] = make_float2(e2m1_to_f32(v), e2m1_to_f32(v >> 4));
-    else lutp[i] = make_float2(kNF4[v & 15], kNF4[v >> 4]);
+    lutp[i] = make_float2(kNF4[v & 15], kNF4[v >> 4]);
   }
-  if (!MX && g.w.fmt != RQ_W_NF4)
+  if (g.w.fmt != RQ_W_NF4)
     for (int v = tid; v < 256; v += kThreads)
       sclut[v] = g.w.fmt == RQ_W_NF4_DQ_FP8 ? e4m3fnuz_to_f32(v) : ieee_div((float)(int8_t)v, 127.0f);
   // both CTAs' barriers initialised and the tensor memory allocated before
@@ -520,30 +472,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
       if (lane == 0) mbar_arrive(fullB0 + 8 * slot);
       return true;
     };
-    if constexpr (MX) {
-      // as below, with one scale byte for the thread's 32 or 16 columns
-      const int kt = g.pitch / 128, blk = (nh0 + dcol) / 32;
-      const int base = DT == RQ_F16 ? *g.mx_top : 127;
-      auto mfetch = [&](int kb) -> uint32_t {
-        const int n = kb * 64 + frow;
-        if (kb >= nkb || blk >= 4 * kt) return 0u;
-        return ldg_pin_u8(g.mx_scales + ((int64_t)(n / 128) * kt + blk / 4) * 512 + (n % 32) * 16 + (n % 128) / 32 * 4 +
-                          blk % 4);
-      };
-      uint32_t ring[kPrefetch];
-#pragma unroll
-      for (int i = 0; i < kPrefetch; ++i) ring[i] = mfetch(i);
-      bool go = true;
-      for (int kb = 0; kb < nkb && go; kb += kPrefetch) {
-#pragma unroll
-        for (int i = 0; i < kPrefetch; ++i) {
-          if (go && kb + i < nkb) {
-            go = convert(kb + i, pow2_scale((int)ring[i], base));
-            ring[i] = mfetch(kb + i + kPrefetch);
-          }
-        }
-      }
-    } else if constexpr (DX) {
+    if constexpr (DX) {
       // dX: the thread's block scale changes with the weight row, 64 rows a
       // stage; a register ring holds kPrefetch stages of raw scales (static
       // indices: fully unrolled)
@@ -636,7 +565,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
       const int c_lo = ((warp - 2) >> 2) * (BN / 2);  // warps w and w+4 split the columns
       const bool has_bias = !DX && g.bias != nullptr;
       T* y = static_cast<T*>(g.y);
-      const float back = MX && DT == RQ_F16 ? pow2_scale(*g.mx_top, 127) : 1.0f;
       for (int cb = c_lo; cb < c_lo + BN / 2; cb += 32) {
         float acc[32], u[32];
         if (has_lora)
@@ -652,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_k(
           for (int e = 0; e < 2; ++e) {
             const int n = n0 + cb + j + e;
             const float bv = (has_bias && n < W_out) ? load_scalar(g.bias, g.bdt, n) : 0.0f;
-            o[e] = lora_epilogue<DT>(MX && DT == RQ_F16 ? acc[j + e] * back : acc[j + e], has_bias, bv, has_lora ? u[j + e] : 0.0f, has_lora, g.s);
+            o[e] = lora_epilogue<DT>(acc[j + e], has_bias, bv, has_lora ? u[j + e] : 0.0f, has_lora, g.s);
           }
           pk[j / 2] = pack_rn<DT>(o[0], o[1]);
         }
@@ -902,10 +830,10 @@ bool gemm_supported(const LinearArgs& a, bool dx) {
   return a.w.N <= 0x7fffffff && a.w.K <= 0x7fffffff && a.M <= 0x7fffffff;
 }
 
-template <int DT, bool DX, int BN, bool I8, bool MX = false>
+template <int DT, bool DX, int BN, bool I8>
 static int gemm_run(const GemmArgs& g, uint64_t wout, uint64_t M, cudaStream_t st) {
   constexpr uint32_t smem = Tile<BN, I8>::kSmBytes;
-  const void* kern = (const void*)gemm_k<DT, DX, BN, I8, MX>;
+  const void* kern = (const void*)gemm_k<DT, DX, BN, I8>;
   const int rc = ensure_smem_limit(kern, smem);
   if (rc != RQ_OK) return rc;
   // CTA pairs along x, output tiles along y, 256-row token pairs along z
@@ -923,7 +851,7 @@ static int gemm_run(const GemmArgs& g, uint64_t wout, uint64_t M, cudaStream_t s
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_k<DT, DX, BN, I8, MX>, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_k<DT, DX, BN, I8>, g);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return RQ_ERR_CUDA;
@@ -1089,40 +1017,6 @@ int lora_down_tc(int dt, bool wt, const void* X, int64_t M, int64_t Kr, const vo
 int gemm_dx(const LinearArgs& a, const void* gt, cudaStream_t st) {
   if (a.r > 0 && ((uintptr_t)a.lora_a % 16 || (a.w.K * 2) % 16)) return RQ_ERR_ALIGN;
   return gemm_launch(a, true, a.x, gt, st);
-}
-
-// dX of a microscaled weight: dy [M][N] (row stride ld), w [N][pitch].
-int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
-           cudaStream_t st) {
-  GemmArgs g = {};
-  const uint64_t N = (uint64_t)w.rows, pitch = (uint64_t)mx4_pitch(K);
-  const int bn = pick_bn((uint64_t)K, (uint64_t)M);
-  {
-    const uint64_t d[3] = {N, (uint64_t)M, 1}, s[2] = {(uint64_t)ld * 2, 0};
-    const uint32_t b[3] = {BK, BM, 1};
-    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, 2, dy, d, s, b, &g.xmap);
-    if (rc != RQ_OK) return rc;
-  }
-  {
-    const uint64_t d[3] = {pitch / 2, N, 1}, s[2] = {pitch / 2, 0};
-    const uint32_t b[3] = {(uint32_t)bn / 4, 64, 1};
-    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, 2, w.codes, d, s, b, &g.cmap);
-    if (rc != RQ_OK) return rc;
-  }
-  g.tmap = g.bmap = g.xmap;
-  g.y = dx;
-  g.M = (int)M;
-  g.N = (int)N;
-  g.K = (int)K;
-  g.s = 1.0f;
-  g.mx_scales = w.scales;
-  g.mx_top = top;
-  g.pitch = (int)pitch;
-  if (dt == RQ_BF16)
-    return bn == 256 ? gemm_run<RQ_BF16, true, 256, false, true>(g, (uint64_t)K, (uint64_t)M, st)
-                     : gemm_run<RQ_BF16, true, 128, false, true>(g, (uint64_t)K, (uint64_t)M, st);
-  return bn == 256 ? gemm_run<RQ_F16, true, 256, false, true>(g, (uint64_t)K, (uint64_t)M, st)
-                   : gemm_run<RQ_F16, true, 128, false, true>(g, (uint64_t)K, (uint64_t)M, st);
 }
 
 }  // namespace rq

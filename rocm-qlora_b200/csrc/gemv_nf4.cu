@@ -1480,10 +1480,11 @@ int gemv_nf4_forward(const GemvArgs& g, bool beside, cudaStream_t st) {
 namespace rq {
 int gemm_take_timeouts(unsigned int* v);  // gemm_tcgen05.cu
 int mx4_take_timeouts(unsigned int* v);   // mx4_gemm.cu
+int mx4_dx_take_timeouts(unsigned int* v);  // mx4_dx.cu
 }
 
 extern "C" int rq_take_kernel_timeouts(unsigned int* count) {
-  unsigned int v = 0, w = 0, u = 0, zero = 0;
+  unsigned int v = 0, w = 0, u = 0, x = 0, zero = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, rq::g_kernel_timeouts, sizeof(v));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(rq::g_kernel_timeouts, &zero, sizeof(zero));
   if (e != cudaSuccess) {
@@ -1492,7 +1493,8 @@ extern "C" int rq_take_kernel_timeouts(unsigned int* count) {
   }
   int rc = rq::gemm_take_timeouts(&w);
   if (rc == RQ_OK) rc = rq::mx4_take_timeouts(&u);
+  if (rc == RQ_OK) rc = rq::mx4_dx_take_timeouts(&x);
   if (rc != RQ_OK) return rc;
-  if (count) *count = v + w + u;
+  if (count) *count = v + w + u + x;
   return RQ_OK;
 }

@@ -1,0 +1,404 @@
+// mx4_dx.cu -- the input gradient of a projection in microscaled 4 bits:
+//   dx[m, k] = sum_n dy[m, n] w[n, k],  dy in 16 bits, w [N, K] packed.
+//
+// The scales go along k, which the sum does not run over, so the block-scaled
+// tensor cores cannot take w; it is widened to dy's type in shared memory and
+// multiplied by tcgen05.mma kind::f16.  In bf16 every value of w is exact.  In
+// fp16 w is taken times 2^(127 - top) with the largest scale byte `top` (what
+// is then below 2^-24 rounds to a multiple of that), and the epilogue
+// multiplies that back.
+//
+// CTA pairs stay and take tiles of 256 tokens x BN columns in turn, as 2-SM
+// MMAs (M = 256): each CTA holds its 128 tokens of dy and widens half of the
+// columns.  A stage of the ring holds 128 rows of w (a wait or a commit costs
+// the tensor pipe about 100 cycles, next to the 1024 of a stage's 8 MMAs).
+//   warp 0      producer: dy [128 x 128] as two K-major tiles whose bytes count
+//               on the leader's barrier, and this CTA's codes of the stage
+//   warp 1      tensor memory; the leader's issues the MMAs, the peer's passes
+//               "widened" on to the leader with a 16-byte bulk copy (no fence
+//               holds that up)
+//   warps 2-9   widen: a thread has BN / 4 columns of a row, stores 16-byte units
+//               of an MN-major tile (w's own row layout, 128-byte swizzle)
+//   warps 10-13 epilogue, from one of two accumulators while the MMAs fill the
+//               other
+// Widening without a table: the 3 bits of a code's magnitude, put at the lowest
+// exponent bits and the highest mantissa bit of the 16-bit type, are the value
+// times 2^-126 (fp16: 2^-14), subnormals included, and one or two packed
+// multiplications take that and the scale in.  A word's 8 codes come out as
+// (0, 4), (1, 5), (2, 6), (3, 7); they are stored so, and the epilogue puts the
+// columns right.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "gemv_common.cuh"
+#include "mx4_common.cuh"
+#include "rq_internal.h"
+#include "tcgen05_common.cuh"
+
+namespace rq {
+
+__device__ unsigned int g_mx4_dx_timeouts;
+
+int mx4_dx_take_timeouts(unsigned int* v) {
+  unsigned int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(v, g_mx4_dx_timeouts, sizeof(*v));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_mx4_dx_timeouts, &zero, sizeof(zero));
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
+  }
+  return RQ_OK;
+}
+
+namespace {
+
+constexpr int kWiden = 8, kEpi = 4, kEpi0 = 2 + kWiden;  // warps
+constexpr int kThreads = 32 * (kEpi0 + kEpi);
+constexpr int kRows = 128;                               // rows of w (columns of dy) a stage
+constexpr uint32_t kA = 128 * 128;                       // 64 columns of dy of a CTA's 128 tokens
+constexpr int kAhead = 3;                                // stages of scales on their way in registers
+
+template <int BN>
+struct Plan {
+  static constexpr int BNH = BN / 2;                     // columns of a CTA
+  static constexpr uint32_t kChunk = kRows * 128;        // 64 widened columns of a stage
+  static constexpr uint32_t kB = 2 * kA, kC = kB + BNH / 64 * kChunk;
+  static constexpr uint32_t kCodes = kRows * BNH / 2;
+  static constexpr uint32_t kStage = kC + kCodes;
+  static constexpr int S = BN == 256 ? 3 : 4;
+  static constexpr uint32_t kOut = S * kStage;           // staged: a warp's 32 rows of 32 columns
+  static constexpr uint32_t kSmem = kOut + kEpi * 2048 + 1024;
+  static constexpr uint32_t kCols = 2 * BN;              // tensor memory: two accumulators
+  static_assert(kStage % 1024 == 0 && kSmem <= 226 * 1024, "");
+};
+
+struct Args {
+  CUtensorMap amap;   // dy [M][N], box 64 x 128, 128-byte swizzle
+  CUtensorMap cmap;   // codes [N][pitch / 2], box BN / 4 bytes x 128
+  const uint8_t* scales;
+  const int32_t* top;
+  void* out;          // [M][K]
+  int M, N, K, pieces;  // pieces of 128 columns
+};
+
+// Codes k and k + 4 of a word, at the low exponent bits.
+template <int DT, int K4>
+__device__ __forceinline__ uint32_t spread(uint32_t w) {
+  constexpr int up = DT == RQ_BF16 ? 6 : 9;
+  constexpr uint32_t magnitude = 0x00070007u << up;
+  const uint32_t a = up > 4 * K4 ? w << (up - 4 * K4) : w >> (4 * K4 - up), s = K4 < 3 ? w << (12 - 4 * K4) : w;
+  return (a & magnitude) | (s & 0x80008000u);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (DT == RQ_BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// What takes spread codes to values: in bf16 2^126 and then 2^(byte - 127)
+// (together they can leave the range), in fp16 2^(14 + byte - top).
+template <int DT>
+__device__ __forceinline__ uint32_t factor(uint32_t byte, int top) {
+  const uint32_t f = DT == RQ_BF16 ? pack_rn<DT>(pow2_scale((int)byte, 127), 0.0f)
+                                   : pack_rn<DT>(pow2_scale((int)byte, top) * 16384.0f, 0.0f);
+  return f << 16 | f;
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 widen8(uint32_t w, uint32_t by) {
+  uint4 v = make_uint4(spread<DT, 0>(w), spread<DT, 1>(w), spread<DT, 2>(w), spread<DT, 3>(w));
+  if constexpr (DT == RQ_BF16) {
+    const uint32_t up = 0x7e807e80u;  // 2^126
+    v = make_uint4(mul2<DT>(v.x, up), mul2<DT>(v.y, up), mul2<DT>(v.z, up), mul2<DT>(v.w, up));
+  }
+  return make_uint4(mul2<DT>(v.x, by), mul2<DT>(v.y, by), mul2<DT>(v.z, by), mul2<DT>(v.w, by));
+}
+
+template <int DT, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_k(const __grid_constant__ Args g) {
+  using PL = Plan<BN>;
+  using T = typename DType<DT>::T;
+  constexpr int S = PL::S;
+  extern __shared__ __align__(1024) unsigned char dsm[];
+  // dy[S] (leader's: both CTAs' dy), codes[S] (own), wide[S] (own 8 warps;
+  // leader's also the peer's signal), empty[S], acc[2], taken[2] (leader's)
+  __shared__ __align__(8) uint64_t bars[4 * S + 5];
+  __shared__ __align__(16) uint32_t sig_src[4], sig_dst[4];  // the 16-byte signal copies (contents unused)
+  __shared__ uint32_t tmem_sh;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = cluster_rank();
+  const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
+  unsigned char* sm = dsm + (sbase - sraw);
+  const uint32_t dy0 = smem_u32(bars), codes0 = dy0 + 8 * S, wide0 = codes0 + 8 * S, empty0 = wide0 + 8 * S,
+                 acc0 = empty0 + 8 * S, taken0 = acc0 + 16, drainbar = taken0 + 16;
+  const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u), &g_mx4_dx_timeouts};
+  const int steps = (g.N + kRows - 1) / kRows;
+  const int mt = (g.M + 255) / 256, ntile = mt * ((g.K + BN - 1) / BN);
+  const int first = blockIdx.x / 2, stride = gridDim.x / 2;
+  const int tiles = first < ntile ? (ntile - 1 - first) / stride + 1 : 0, total = tiles * steps;
+
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(dy0 + 8 * i, 1);
+      mbar_init(codes0 + 8 * i, 1);
+      mbar_init(wide0 + 8 * i, rank == 0 ? kWiden + 1 : kWiden);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc0 + 8 * i, 1);
+      mbar_init(taken0 + 8 * i, 2 * kEpi);
+    }
+    mbar_init(drainbar, 1);
+    abort_flag = 0;
+    for (int i = 0; i < 4; ++i) sig_src[i] = sig_dst[i] = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)),
+                 "r"(PL::kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_sh;
+  grid_begin();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t lead = mapa(dy0, 0);
+      for (int i = 0; i < total; ++i) {
+        const int t = first + i / steps * stride, st = i % steps, slot = i % S;
+        if (i >= S && !wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab)) break;
+        const uint32_t at = sbase + slot * PL::kStage;
+        const int m0 = t % mt * 256 + (int)rank * 128, c0 = t / mt * BN + (int)rank * PL::BNH;
+        mbar_expect_tx(codes0 + 8 * slot, PL::kCodes);
+        tma_2d(at + PL::kC, &g.cmap, c0 / 2, st * kRows, codes0 + 8 * slot);
+        if (rank == 0) {
+          mbar_expect_tx(wide0 + 8 * slot, 16);  // the peer's signal
+          mbar_expect_tx(dy0 + 8 * slot, 4 * kA);
+        }
+        tma_pair(at, &g.amap, st * kRows, m0, lead + 8 * slot);
+        tma_pair(at + kA, &g.amap, st * kRows + 64, m0, lead + 8 * slot);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_pair<DT, BN>(true);
+      bool ok = true;
+      for (int t = 0, i = 0; t < tiles && ok; ++t) {
+        const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
+        if (t >= 2 && !wait_pair(taken0 + 8 * (t & 1), ((t >> 1) - 1) & 1, ab)) break;
+        for (int st = 0; st < steps; ++st, ++i) {
+          const int slot = i % S;
+          ok = wait_pair(dy0 + 8 * slot, (i / S) & 1, ab) && wait_pair(wide0 + 8 * slot, (i / S) & 1, ab);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t a = sbase + slot * PL::kStage, b = a + PL::kB;
+#pragma unroll
+          for (int k = 0; k < kRows / 16; ++k)
+            mma_pair(d, sw128_desc(a + k / 4 * kA + k % 4 * 32), sw128_mn_desc(b + k * 2048, PL::kChunk), idesc,
+                     (st > 0 || k > 0) ? 1u : 0u);
+          mma_commit_pair(empty0 + 8 * slot, 3);
+        }
+        if (ok) mma_commit_pair(acc0 + 8 * (t & 1), 3);
+      }
+    } else if (lane == 0) {
+      const uint32_t dst = mapa(smem_u32(sig_dst), 0), lead = mapa(wide0, 0);
+      for (int i = 0; i < total; ++i) {
+        if (!wait_pair(wide0 + 8 * (i % S), (i / S) & 1, ab)) break;
+        bulk_signal(dst, smem_u32(sig_src), lead + 8 * (i % S));
+      }
+    }
+  } else if (warp < kEpi0) {
+    // row 32 (w % 4) + lane of the stage, columns BN / 4 (w / 4) .. of the CTA's
+    // half: the lanes of a store have 8 different units of the swizzle
+    constexpr int U = BN / 32;  // 16-byte units, of 8 codes each
+    const int w = warp - 2, row = (w & 3) * 32 + lane, col = (w >> 2) * (BN / 4);
+    const uint32_t store = PL::kB + col / 64 * PL::kChunk + row * 128;
+    const int unit = col % 64 / 8;
+    const int top = DT == RQ_F16 ? *g.top : 127;
+    // codes: 16-byte pieces of a row of BN / 4 bytes, in the swizzle of their TMA box
+    const uint32_t load = PL::kC + row * (BN / 4);
+    const int swz = BN == 256 ? (row >> 1) & 3 : (row >> 2) & 1, piece = col / 32;
+    auto fetch = [&](int i) -> uint32_t {  // the scale bytes of this thread's columns
+      if (i >= total) return 0u;
+      const int t = first + i / steps * stride, st = i % steps;
+      const int c = t / mt * BN + (int)rank * PL::BNH + col;
+      if (c >= g.pieces * 128) return 0u;
+      const uint8_t* p = g.scales + ((int64_t)st * g.pieces + c / 128) * 512 + (row % 32) * 16 + row / 32 * 4 + c % 128 / 32;
+      return BN == 256 ? __ldg(reinterpret_cast<const uint16_t*>(p)) : __ldg(p);
+    };
+    uint32_t ring[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) ring[j] = fetch(j);
+    bool ok = true;
+    for (int i0 = 0; i0 < total && ok; i0 += kAhead) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j, slot = i % S;
+        if (!ok || i >= total) break;
+        const uint32_t by[2] = {factor<DT>(ring[j] & 255u, top), BN == 256 ? factor<DT>(ring[j] >> 8, top) : 0u};
+        ring[j] = fetch(i + kAhead);
+        if (lane == 0) ok = wait_pair(codes0 + 8 * slot, (i / S) & 1, ab);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (!ok) break;
+        unsigned char* at = sm + slot * PL::kStage;
+#pragma unroll
+        for (int h = 0; h < U / 4; ++h) {  // 32 columns, one scale
+          const uint4 c = *reinterpret_cast<const uint4*>(at + load + (((piece + h) ^ swz) << 4));
+          const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(at + store + (((unit + 4 * h + u) ^ (row & 7)) << 4)) = widen8<DT>(cw[u], by[h]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wide0 + 8 * slot);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    unsigned char* stage = sm + PL::kOut + (warp - kEpi0) * 2048;
+    const uint32_t took = mapa(taken0, 0);
+    T* out = static_cast<T*>(g.out);
+    const float back = DT == RQ_F16 ? pow2_scale(*g.top, 127) : 1.0f;
+    const bool rows16 = (uintptr_t)out % 16 == 0 && g.K % 8 == 0;
+    for (int n = 0; n < tiles; ++n) {
+      const int t = first + n * stride, m0 = t % mt * 256 + (int)rank * 128 + quad * 32, c0 = t / mt * BN;
+      bool ok = true;
+      if (lane == 0) ok = wait_pair(acc0 + 8 * (n & 1), (n >> 1) & 1, ab) && !ab.raised();
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        float acc[32];
+        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(n & 1) * BN + c, acc);
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float* a = acc + 8 * u;  // columns 0, 4, 1, 5, 2, 6, 3, 7
+          if constexpr (DT == RQ_F16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[8 * u + j] *= back;
+          }
+          v[u] = make_uint4(pack_rn<DT>(a[0], a[2]), pack_rn<DT>(a[4], a[6]), pack_rn<DT>(a[1], a[3]), pack_rn<DT>(a[5], a[7]));
+        }
+        const int k = c0 + c;
+        if (rows16) {
+          if (m0 + lane < g.M) {
+            T* to = out + (int64_t)(m0 + lane) * g.K + k;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (k + 8 * u < g.K) reinterpret_cast<uint4*>(to)[u] = v[u];
+          }
+        } else {
+          // rows that are not 16-byte aligned: a row a time, one column a lane
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = v[u];
+          __syncwarp();
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r) {
+            const T x = *reinterpret_cast<const T*>(stage + r * 64 + ((lane / 8 ^ (r >> 1 & 3)) << 4) + lane % 8 * 2);
+            if (m0 + r < g.M && k + lane < g.K) out[(int64_t)(m0 + r) * g.K + k + lane] = x;
+          }
+          __syncwarp();
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(took + 8 * (n & 1));
+    }
+  }
+
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();  // no copy, commit or arrive can reach a CTA that has left
+  if (tid == 0 && ab.raised()) {
+    // after a wait that ran out: this pair's MMAs (bounded), and time for
+    // copies and arrives under way to land
+    if (rank == 0) {
+      mma_commit_pair(drainbar, 1);
+      drain(drainbar, 0);
+    }
+    const uint64_t t0 = gtimer_ns();
+    while (gtimer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PL::kCols) : "memory");
+}
+
+template <int DT, int BN>
+int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx, cudaStream_t st) {
+  Args g;
+  const int64_t pitch = mx4_pitch(K);
+  {
+    const uint64_t d[3] = {(uint64_t)w.rows, (uint64_t)M, 1}, s[2] = {(uint64_t)ld * 2, 0};
+    const uint32_t b[3] = {64, 128, 1};
+    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_128B, 2, dy, d, s, b, &g.amap);
+    if (rc != RQ_OK) return rc;
+  }
+  {
+    const uint64_t d[3] = {(uint64_t)pitch / 2, (uint64_t)w.rows, 1}, s[2] = {(uint64_t)pitch / 2, 0};
+    const uint32_t b[3] = {BN / 4, kRows, 1};
+    const int rc = tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                                     BN == 256 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, 2, w.codes, d, s,
+                                     b, &g.cmap);
+    if (rc != RQ_OK) return rc;
+  }
+  g.scales = w.scales;
+  g.top = top;
+  g.out = dx;
+  g.M = (int)M;
+  g.N = (int)w.rows;
+  g.K = (int)K;
+  g.pieces = (int)(pitch / 128);
+  const void* kern = (const void*)mx4_dx_k<DT, BN>;
+  const int rc = ensure_smem_limit(kern, Plan<BN>::kSmem);
+  if (rc != RQ_OK) return rc;
+  const int64_t ntile = ((M + 255) / 256) * ((K + BN - 1) / BN), pairs = num_sms() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (ntile < pairs ? ntile : pairs)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Plan<BN>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  void* params[] = {&g};
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, kern, params);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return RQ_ERR_CUDA;
+  }
+  return check_launch();
+}
+
+}  // namespace
+
+// 256 columns a tile unless that leaves SMs idle, then 128.
+int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
+           cudaStream_t st) {
+  const bool wide = 2 * ((M + 255) / 256) * ((K + 255) / 256) >= num_sms();
+  if (dt == RQ_BF16)
+    return wide ? run<RQ_BF16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_BF16, 128>(dy, ld, M, w, top, K, dx, st);
+  return wide ? run<RQ_F16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_F16, 128>(dy, ld, M, w, top, K, dx, st);
+}
+
+}  // namespace rq

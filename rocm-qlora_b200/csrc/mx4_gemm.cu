@@ -57,7 +57,6 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kP = 128;                  // rows of P a tile
 constexpr uint32_t kPBytes = kP * 128;        // codes of a stage: 256 columns
 constexpr uint32_t kPiece = 512;
-constexpr uint64_t kWaitNs = 2000000000ull;   // a bounded wait gives up after about 2 s
 
 constexpr int kPark = 132;                    // floats of a token's parked sums
 
@@ -130,7 +129,7 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   const uint64_t t0 = gtimer_ns();
   while (!*abort) {
     if (mbar_try<false>(bar, parity)) return true;
-    if (gtimer_ns() - t0 > kWaitNs) {
+    if (gtimer_ns() - t0 > kPairWaitNs) {
       *abort = 1;
       atomicAdd(&g_mx4_timeouts, 1u);
       return false;
@@ -138,11 +137,6 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   }
   return false;
 }
-__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = gtimer_ns();
-  while (!mbar_test<false>(bar, parity) && gtimer_ns() - t0 < kWaitNs) __nanosleep(100);
-}
-
 // out[q, p] (tokens Q, outputs P): sums of its share of the columns.
 template <int DT, int BN>
 __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant__ Args g) {
@@ -336,26 +330,6 @@ struct PairArgs {
   int64_t ld;
 };
 
-// A TMA copy of one CTA of a pair whose bytes count on the barrier of the
-// pair's leader (`bar`: shared::cluster address).
-__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
-      : "memory");
-}
-// What the arrival tells of is in tensor memory, which its own fence orders.
-__device__ __forceinline__ void arrive_cluster(uint32_t cbar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
-}
-
 // 12 columns of this thread's lane
 __device__ __forceinline__ void tmem_st12(uint32_t taddr, const uint4 (&v)[3]) {
 #pragma unroll
@@ -363,27 +337,6 @@ __device__ __forceinline__ void tmem_st12(uint32_t taddr, const uint4 (&v)[3]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr + 4 * i), "r"(v[i].x),
                  "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                  : "memory");
-}
-
-// The abort state of a pair: this CTA's flag and the peer's.
-struct PairAbort {
-  volatile int* mine;
-  uint32_t peer;
-  __device__ __forceinline__ bool raised() const { return *mine != 0; }
-};
-__device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
-  if (mbar_try<false>(bar, parity)) return true;
-  const uint64_t t0 = gtimer_ns();
-  while (!ab.raised()) {
-    if (mbar_try<false>(bar, parity)) return true;
-    if (gtimer_ns() - t0 > kWaitNs) {
-      *ab.mine = 1;
-      st_cluster(ab.peer, 1);
-      atomicAdd(&g_mx4_timeouts, 1u);
-      return false;
-    }
-  }
-  return false;
 }
 
 // out[p, q]: P tokens, Q outputs.
@@ -404,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
   unsigned char* sm = dsm + (sbase - sraw);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S, taken = accbar + 8,
                  drainbar = taken + 8, lead = mapa(full0, 0);
-  const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u)};
+  const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u), &g_mx4_timeouts};
   const int steps = (g.tiles + 3) / 4;
   const int pt = (g.prows + 255) / 256, qt = (g.qrows + 255) / 256, ntile = pt * qt;
   const int first = blockIdx.x / 2, stride = gridDim.x / 2;
@@ -479,9 +432,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
                 mma_mx4<2>(tmem, sw128_desc(a), sw128_desc(a + 2 * kCodes), idesc_mx4<256, 256>(h), tsc + k * 12,
                            tsc + k * 12 + 4, (st > 0 || k > 0 || h > 0) ? 1u : 0u);
               }
-          mma_commit_both(empty0 + 8 * slot);
+          mma_commit_pair(empty0 + 8 * slot, 3);
         }
-        if (ok) mma_commit_both(accbar);
+        if (ok) mma_commit_pair(accbar, 3);
       }
     }
   } else if (warp < kEpi0) {
@@ -602,7 +555,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
     // after a wait that ran out: this pair's MMAs (bounded), and time for
     // copies and arrives under way to land
     if (rank == 0) {
-      mma_commit_both(drainbar);
+      mma_commit_pair(drainbar, 1);
       drain(drainbar, 0);
     }
     const uint64_t t0 = gtimer_ns();

@@ -166,7 +166,7 @@ int token_logprobs_grad(const TokenRows& t, const float* stats, const float* slo
                         const float* upstream, void* dlogits, cudaStream_t st);
 
 // Microscaled 4-bit values (mx4.cu), their product (mx4_gemm.cu) and its
-// gradient (gemm_tcgen05.cu).
+// gradient (mx4_dx.cu).
 struct Mx4 {
   const uint8_t* codes;   // [rows, pitch / 2]
   const uint8_t* scales;  // [ceil(rows / 128), pitch / 128, 512]

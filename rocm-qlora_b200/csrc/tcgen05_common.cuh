@@ -120,6 +120,44 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
   return d;
 }
 
+// Shared-memory descriptor of an MN-major operand with 128-byte swizzle:
+// rows (K) of 128 bytes = 64 MN elements, 8-row groups 1024 bytes apart,
+// 64-element MN groups `lbo` bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// Instruction descriptor: 16-bit A/B of type DT, fp32 accumulate, A K-major,
+// B K-major (or MN-major), M = 256 (the CTA pair), N = BN.
+template <int DT, int BN>
+__device__ __forceinline__ uint32_t idesc_pair(bool b_mn = false) {
+  const uint32_t ab = DT == RQ_BF16 ? 1u : 0u;
+  return (1u << 4) | (ab << 7) | (ab << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+         ((uint32_t)(256 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accum)
+      : "memory");
+}
+// Arrive on the barrier at shared::cta offset `bar` of each CTA in `mask`
+// once every MMA this thread issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(mask)
+      : "memory");
+}
+
 // 32 consecutive fp32 columns of this thread's accumulator row
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -146,6 +184,49 @@ __device__ __forceinline__ uint32_t pack_rn(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+}
+
+// A TMA copy of one CTA of a pair whose bytes count on the barrier of the
+// pair's leader (`bar`: shared::cluster address).
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// What the arrival tells of is in tensor memory, which its own fence orders.
+__device__ __forceinline__ void arrive_cluster(uint32_t cbar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+}
+
+constexpr uint64_t kPairWaitNs = 2000000000ull;  // a bounded wait gives up after about 2 s
+
+// The abort state of a pair: this CTA's flag, the peer's, and the counter of
+// waits that ran out.
+struct PairAbort {
+  volatile int* mine;
+  uint32_t peer;  // shared::cluster address
+  unsigned int* count;
+  __device__ __forceinline__ bool raised() const { return *mine != 0; }
+};
+__device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
+  if (mbar_try<false>(bar, parity)) return true;
+  const uint64_t t0 = gtimer_ns();
+  while (!ab.raised()) {
+    if (mbar_try<false>(bar, parity)) return true;
+    if (gtimer_ns() - t0 > kPairWaitNs) {
+      *ab.mine = 1;
+      st_cluster(ab.peer, 1);
+      atomicAdd(ab.count, 1u);
+      return false;
+    }
+  }
+  return false;
+}
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = gtimer_ns();
+  while (!mbar_test<false>(bar, parity) && gtimer_ns() - t0 < kPairWaitNs) __nanosleep(100);
 }
 
 }  // namespace rq
