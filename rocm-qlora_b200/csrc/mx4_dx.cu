@@ -14,9 +14,7 @@
 // the tensor pipe about 100 cycles, next to the 1024 of a stage's 8 MMAs).
 //   warp 0      producer: dy [128 x 128] as two K-major tiles whose bytes count
 //               on the leader's barrier, and this CTA's codes of the stage
-//   warp 1      tensor memory; the leader's issues the MMAs, the peer's passes
-//               "widened" on to the leader with a 16-byte bulk copy (no fence
-//               holds that up)
+//   warp 1      tensor memory; the leader's issues the MMAs
 //   warps 2-9   widen: a thread has BN / 4 columns of a row, stores 16-byte units
 //               of an MN-major tile (w's own row layout, 128-byte swizzle)
 //   warps 10-13 epilogue, from one of two accumulators while the MMAs fill the
@@ -56,7 +54,6 @@ constexpr int kWiden = 8, kEpi = 4, kEpi0 = 2 + kWiden;  // warps
 constexpr int kThreads = 32 * (kEpi0 + kEpi);
 constexpr int kRows = 128;                               // rows of w (columns of dy) a stage
 constexpr uint32_t kA = 128 * 128;                       // 64 columns of dy of a CTA's 128 tokens
-constexpr int kAhead = 3;                                // stages of scales on their way in registers
 
 template <int BN>
 struct Plan {
@@ -98,23 +95,39 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// What takes spread codes to values: in bf16 2^126 and then 2^(byte - 127)
-// (together they can leave the range), in fp16 2^(14 + byte - top).
+// What takes spread codes to values: in bf16 2^(byte - 1), in two steps (2^126
+// first) where that leaves the range, in fp16 2^(14 + byte - top).
 template <int DT>
 __device__ __forceinline__ uint32_t factor(uint32_t byte, int top) {
-  const uint32_t f = DT == RQ_BF16 ? pack_rn<DT>(pow2_scale((int)byte, 127), 0.0f)
-                                   : pack_rn<DT>(pow2_scale((int)byte, top) * 16384.0f, 0.0f);
+  uint32_t f;
+  if constexpr (DT == RQ_BF16) f = pack_rn<DT>(pow2_scale((int)byte, byte > 128u ? 127 : 1), 0.0f);
+  else f = pack_rn<DT>(pow2_scale((int)byte, top) * 16384.0f, 0.0f);
   return f << 16 | f;
 }
 
-template <int DT>
+// Arrival on a barrier of the pair's leader, after this CTA's own writes to its
+// own shared memory: those need no more than CTA scope.  (A release at cluster
+// scope waits about a microsecond for everything remote.)
+__device__ __forceinline__ void arrive_leader(uint32_t cbar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+}
+
+template <int DT, bool FAR>
 __device__ __forceinline__ uint4 widen8(uint32_t w, uint32_t by) {
   uint4 v = make_uint4(spread<DT, 0>(w), spread<DT, 1>(w), spread<DT, 2>(w), spread<DT, 3>(w));
-  if constexpr (DT == RQ_BF16) {
+  if constexpr (FAR) {
     const uint32_t up = 0x7e807e80u;  // 2^126
     v = make_uint4(mul2<DT>(v.x, up), mul2<DT>(v.y, up), mul2<DT>(v.z, up), mul2<DT>(v.w, up));
   }
   return make_uint4(mul2<DT>(v.x, by), mul2<DT>(v.y, by), mul2<DT>(v.z, by), mul2<DT>(v.w, by));
+}
+
+// wait_pair by a warp: one try of all lanes where the phase is over already.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const PairAbort& ab, int lane) {
+  if (__all_sync(0xffffffffu, mbar_test<false>(bar, parity))) return true;
+  bool ok = true;
+  if (lane == 0) ok = wait_pair(bar, parity, ab);
+  return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
 }
 
 template <int DT, int BN>
@@ -123,18 +136,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
   using T = typename DType<DT>::T;
   constexpr int S = PL::S;
   extern __shared__ __align__(1024) unsigned char dsm[];
-  // dy[S] (leader's: both CTAs' dy), codes[S] (own), wide[S] (own 8 warps;
-  // leader's also the peer's signal), empty[S], acc[2], taken[2] (leader's)
-  __shared__ __align__(8) uint64_t bars[4 * S + 5];
-  __shared__ __align__(16) uint32_t sig_src[4], sig_dst[4];  // the 16-byte signal copies (contents unused)
+  // dy[S] (leader's: both CTAs' dy), codes[S] (own), read[S] (own codes are
+  // widened), wide[S] (leader's: both CTAs' widening warps), empty[S], acc[2],
+  // taken[2] (leader's)
+  __shared__ __align__(8) uint64_t bars[5 * S + 5];
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster_rank();
   const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
   unsigned char* sm = dsm + (sbase - sraw);
-  const uint32_t dy0 = smem_u32(bars), codes0 = dy0 + 8 * S, wide0 = codes0 + 8 * S, empty0 = wide0 + 8 * S,
-                 acc0 = empty0 + 8 * S, taken0 = acc0 + 16, drainbar = taken0 + 16;
+  const uint32_t dy0 = smem_u32(bars), codes0 = dy0 + 8 * S, read0 = codes0 + 8 * S, wide0 = read0 + 8 * S,
+                 empty0 = wide0 + 8 * S, acc0 = empty0 + 8 * S, taken0 = acc0 + 16, drainbar = taken0 + 16;
   const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u), &g_mx4_dx_timeouts};
   const int steps = (g.N + kRows - 1) / kRows;
   const int mt = (g.M + 255) / 256, ntile = mt * ((g.K + BN - 1) / BN);
@@ -145,7 +158,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
     for (int i = 0; i < S; ++i) {
       mbar_init(dy0 + 8 * i, 1);
       mbar_init(codes0 + 8 * i, 1);
-      mbar_init(wide0 + 8 * i, rank == 0 ? kWiden + 1 : kWiden);
+      mbar_init(read0 + 8 * i, kWiden);
+      mbar_init(wide0 + 8 * i, 2 * kWiden);
       mbar_init(empty0 + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -154,7 +168,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
     }
     mbar_init(drainbar, 1);
     abort_flag = 0;
-    for (int i = 0; i < 4; ++i) sig_src[i] = sig_dst[i] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -172,20 +185,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
 
   if (warp == 0) {
     if (lane == 0) {
+      // dy waits for the MMAs of its slot's stage before, the codes only for the
+      // widening: they are loaded ahead
       const uint32_t lead = mapa(dy0, 0);
-      for (int i = 0; i < total; ++i) {
-        const int t = first + i / steps * stride, st = i % steps, slot = i % S;
-        if (i >= S && !wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab)) break;
-        const uint32_t at = sbase + slot * PL::kStage;
-        const int m0 = t % mt * 256 + (int)rank * 128, c0 = t / mt * BN + (int)rank * PL::BNH;
+      int ahead = 0;
+      bool ok = true;
+      auto load_codes = [&](int i) {
+        const int t = first + i / steps * stride, slot = i % S;
         mbar_expect_tx(codes0 + 8 * slot, PL::kCodes);
-        tma_2d(at + PL::kC, &g.cmap, c0 / 2, st * kRows, codes0 + 8 * slot);
-        if (rank == 0) {
-          mbar_expect_tx(wide0 + 8 * slot, 16);  // the peer's signal
-          mbar_expect_tx(dy0 + 8 * slot, 4 * kA);
-        }
+        tma_2d(sbase + slot * PL::kStage + PL::kC, &g.cmap, (t / mt * BN + (int)rank * PL::BNH) / 2, i % steps * kRows,
+               codes0 + 8 * slot);
+      };
+      for (; ahead < S && ahead < total; ++ahead) load_codes(ahead);
+      for (int i = 0; i < total && ok; ++i) {
+        const int t = first + i / steps * stride, st = i % steps, slot = i % S;
+        if (i >= S) ok = wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab);
+        if (!ok) break;
+        const uint32_t at = sbase + slot * PL::kStage;
+        const int m0 = t % mt * 256 + (int)rank * 128;
+        if (rank == 0) mbar_expect_tx(dy0 + 8 * slot, 4 * kA);
         tma_pair(at, &g.amap, st * kRows, m0, lead + 8 * slot);
         tma_pair(at + kA, &g.amap, st * kRows + 64, m0, lead + 8 * slot);
+        // stage i's MMAs still run when stage ahead - S + 1 <= i + 1 is widened
+        if (ahead < total && ahead <= i + S) {
+          ok = wait_pair(read0 + 8 * (ahead % S), ((ahead / S) - 1) & 1, ab);
+          if (ok) load_codes(ahead++);
+        }
       }
     }
   } else if (warp == 1) {
@@ -209,12 +234,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
         }
         if (ok) mma_commit_pair(acc0 + 8 * (t & 1), 3);
       }
-    } else if (lane == 0) {
-      const uint32_t dst = mapa(smem_u32(sig_dst), 0), lead = mapa(wide0, 0);
-      for (int i = 0; i < total; ++i) {
-        if (!wait_pair(wide0 + 8 * (i % S), (i / S) & 1, ab)) break;
-        bulk_signal(dst, smem_u32(sig_src), lead + 8 * (i % S));
-      }
     }
   } else if (warp < kEpi0) {
     // row 32 (w % 4) + lane of the stage, columns BN / 4 (w / 4) .. of the CTA's
@@ -227,40 +246,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
     // codes: 16-byte pieces of a row of BN / 4 bytes, in the swizzle of their TMA box
     const uint32_t load = PL::kC + row * (BN / 4);
     const int swz = BN == 256 ? (row >> 1) & 3 : (row >> 2) & 1, piece = col / 32;
-    auto fetch = [&](int i) -> uint32_t {  // the scale bytes of this thread's columns
-      if (i >= total) return 0u;
-      const int t = first + i / steps * stride, st = i % steps;
-      const int c = t / mt * BN + (int)rank * PL::BNH + col;
-      if (c >= g.pieces * 128) return 0u;
-      const uint8_t* p = g.scales + ((int64_t)st * g.pieces + c / 128) * 512 + (row % 32) * 16 + row / 32 * 4 + c % 128 / 32;
-      return BN == 256 ? __ldg(reinterpret_cast<const uint16_t*>(p)) : __ldg(p);
-    };
-    uint32_t ring[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) ring[j] = fetch(j);
+    const uint32_t wide = mapa(wide0, 0);
+    int slot = 0;
+    uint32_t round = 0;  // how often the ring has gone round
     bool ok = true;
-    for (int i0 = 0; i0 < total && ok; i0 += kAhead) {
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int i = i0 + j, slot = i % S;
-        if (!ok || i >= total) break;
-        const uint32_t by[2] = {factor<DT>(ring[j] & 255u, top), BN == 256 ? factor<DT>(ring[j] >> 8, top) : 0u};
-        ring[j] = fetch(i + kAhead);
-        if (lane == 0) ok = wait_pair(codes0 + 8 * slot, (i / S) & 1, ab);
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    for (int n = 0; n < tiles && ok; ++n) {
+      const int c = (first + n * stride) / mt * BN + (int)rank * PL::BNH + col;
+      const bool any = c < g.pieces * 128;
+      const uint8_t* p = g.scales + (int64_t)(c / 128) * 512 + (row % 32) * 16 + row / 32 * 4 + c % 128 / 32;
+      auto scale = [&](int st) -> uint32_t {  // the scale bytes of this thread's columns
+        if (!any || st >= steps) return 0u;
+        const uint8_t* q = p + (int64_t)st * g.pieces * 512;
+        return BN == 256 ? __ldg(reinterpret_cast<const uint16_t*>(q)) : __ldg(q);
+      };
+      uint32_t s0 = scale(0), s1 = scale(1), s2 = scale(2);  // on their way
+      for (int st = 0; st < steps; ++st) {
+        const uint32_t by[2] = {factor<DT>(s0 & 255u, top), BN == 256 ? factor<DT>(s0 >> 8, top) : 0u};
+        // a scale above 2 in bf16 takes two steps
+        const bool far[2] = {DT == RQ_BF16 && (s0 & 255u) > 128u, DT == RQ_BF16 && BN == 256 && (s0 >> 8) > 128u};
+        s0 = s1;
+        s1 = s2;
+        s2 = scale(st + 3);
+        ok = wait_warp(codes0 + 8 * slot, round & 1, ab, lane);
         if (!ok) break;
         unsigned char* at = sm + slot * PL::kStage;
+        uint4 cw[U / 4];
+#pragma unroll
+        for (int h = 0; h < U / 4; ++h) cw[h] = *reinterpret_cast<const uint4*>(at + load + (((piece + h) ^ swz) << 4));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(read0 + 8 * slot);
+        if (round > 0) ok = wait_warp(empty0 + 8 * slot, (round - 1) & 1, ab, lane);
+        if (!ok) break;
 #pragma unroll
         for (int h = 0; h < U / 4; ++h) {  // 32 columns, one scale
-          const uint4 c = *reinterpret_cast<const uint4*>(at + load + (((piece + h) ^ swz) << 4));
-          const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+          const uint32_t word[4] = {cw[h].x, cw[h].y, cw[h].z, cw[h].w};
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<uint4*>(at + store + (((unit + 4 * h + u) ^ (row & 7)) << 4)) = widen8<DT>(cw[u], by[h]);
+            *reinterpret_cast<uint4*>(at + store + (((unit + 4 * h + u) ^ (row & 7)) << 4)) =
+                far[h] ? widen8<DT, true>(word[u], by[h]) : widen8<DT, false>(word[u], by[h]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
         __syncwarp();
-        if (lane == 0) mbar_arrive(wide0 + 8 * slot);
+        if (lane == 0) arrive_leader(wide + 8 * slot);
+        if (++slot == S) slot = 0, ++round;
       }
     }
   } else {
