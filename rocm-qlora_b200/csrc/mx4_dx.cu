@@ -15,9 +15,9 @@
 //   warp 0      producer: dy [128 x 128] as two K-major tiles whose bytes count
 //               on the leader's barrier, and this CTA's codes of the stage
 //   warp 1      tensor memory; the leader's issues the MMAs
-//   warps 2-9   widen: a thread has BN / 4 columns of a row, stores 16-byte units
-//               of an MN-major tile (w's own row layout, 128-byte swizzle)
-//   warps 10-13 epilogue, from one of two accumulators while the MMAs fill the
+//   8 or 16     widen: a thread has BN / 4 columns of a row, stores 16-byte units
+//   warps       of an MN-major tile (w's own row layout, 128-byte swizzle)
+//   4 warps     epilogue, from one of two accumulators while the MMAs fill the
 //               other
 // Widening without a table: the 3 bits of a code's magnitude, put at the lowest
 // exponent bits and the highest mantissa bit of the 16-bit type, are the value
@@ -50,13 +50,20 @@ int mx4_dx_take_timeouts(unsigned int* v) {
 
 namespace {
 
-constexpr int kWiden = 8, kEpi = 4, kEpi0 = 2 + kWiden;  // warps
-constexpr int kThreads = 32 * (kEpi0 + kEpi);
+constexpr int kWiden = 8, kEpi = 4;                      // warps
 constexpr int kRows = 128;                               // rows of w (columns of dy) a stage
 constexpr uint32_t kA = 128 * 128;                       // 64 columns of dy of a CTA's 128 tokens
 
-template <int BN>
+template <int DT, int BN>
 struct Plan {
+  // Teams of 8 widening warps that take the stages in turn.  Two hide the waits
+  // and fences between stages, but take issue slots and shared memory from each
+  // other: 8192 x 11008 -> 4096 in bf16 613 us with one and 583 with two, 2047 x
+  // 4096 -> 11008 in fp16 (whose multiplications are shorter) 145 and 162, 512 x
+  // 4096 -> 4096 (128 columns) 27 and 30.
+  static constexpr int kTeams = DT == RQ_BF16 && BN == 256 ? 2 : 1;
+  static constexpr int kEpi0 = 2 + kTeams * kWiden;      // first epilogue warp
+  static constexpr int kThreads = 32 * (kEpi0 + kEpi);
   static constexpr int BNH = BN / 2;                     // columns of a CTA
   static constexpr uint32_t kChunk = kRows * 128;        // 64 widened columns of a stage
   static constexpr uint32_t kB = 2 * kA, kC = kB + BNH / 64 * kChunk;
@@ -131,8 +138,8 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const P
 }
 
 template <int DT, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_k(const __grid_constant__ Args g) {
-  using PL = Plan<BN>;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThreads, 1) mx4_dx_k(const __grid_constant__ Args g) {
+  using PL = Plan<DT, BN>;
   using T = typename DType<DT>::T;
   constexpr int S = PL::S;
   extern __shared__ __align__(1024) unsigned char dsm[];
@@ -235,11 +242,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
         if (ok) mma_commit_pair(acc0 + 8 * (t & 1), 3);
       }
     }
-  } else if (warp < kEpi0) {
+  } else if (warp < PL::kEpi0) {
     // row 32 (w % 4) + lane of the stage, columns BN / 4 (w / 4) .. of the CTA's
     // half: the lanes of a store have 8 different units of the swizzle
     constexpr int U = BN / 32;  // 16-byte units, of 8 codes each
-    const int w = warp - 2, row = (w & 3) * 32 + lane, col = (w >> 2) * (BN / 4);
+    constexpr int TM = PL::kTeams;
+    const int w = (warp - 2) % kWiden, row = (w & 3) * 32 + lane, col = (w >> 2) * (BN / 4);
     const uint32_t store = PL::kB + col / 64 * PL::kChunk + row * 128;
     const int unit = col % 64 / 8;
     const int top = DT == RQ_F16 ? *g.top : 127;
@@ -247,8 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
     const uint32_t load = PL::kC + row * (BN / 4);
     const int swz = BN == 256 ? (row >> 1) & 3 : (row >> 2) & 1, piece = col / 32;
     const uint32_t wide = mapa(wide0, 0);
-    int slot = 0;
-    uint32_t round = 0;  // how often the ring has gone round
+    int i = (warp - 2) / kWiden;  // the team's next stage, of all
     bool ok = true;
     for (int n = 0; n < tiles && ok; ++n) {
       const int c = (first + n * stride) / mt * BN + (int)rank * PL::BNH + col;
@@ -259,14 +266,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
         const uint8_t* q = p + (int64_t)st * g.pieces * 512;
         return BN == 256 ? __ldg(reinterpret_cast<const uint16_t*>(q)) : __ldg(q);
       };
-      uint32_t s0 = scale(0), s1 = scale(1), s2 = scale(2);  // on their way
-      for (int st = 0; st < steps; ++st) {
+      int st = i - n * steps, slot = i % S;
+      uint32_t round = (uint32_t)(i / S);  // how often the ring has gone round
+      uint32_t s0 = scale(st), s1 = scale(st + TM), s2 = scale(st + 2 * TM);  // on their way
+      for (; st < steps; st += TM, i += TM) {
         const uint32_t by[2] = {factor<DT>(s0 & 255u, top), BN == 256 ? factor<DT>(s0 >> 8, top) : 0u};
         // a scale above 2 in bf16 takes two steps
         const bool far[2] = {DT == RQ_BF16 && (s0 & 255u) > 128u, DT == RQ_BF16 && BN == 256 && (s0 >> 8) > 128u};
         s0 = s1;
         s1 = s2;
-        s2 = scale(st + 3);
+        s2 = scale(st + 3 * TM);
         ok = wait_warp(codes0 + 8 * slot, round & 1, ab, lane);
         if (!ok) break;
         unsigned char* at = sm + slot * PL::kStage;
@@ -288,12 +297,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_dx_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
         __syncwarp();
         if (lane == 0) arrive_leader(wide + 8 * slot);
-        if (++slot == S) slot = 0, ++round;
+        slot += TM;
+        if (slot >= S) slot -= S, ++round;
       }
     }
   } else {
     const int quad = warp & 3;
-    unsigned char* stage = sm + PL::kOut + (warp - kEpi0) * 2048;
+    unsigned char* stage = sm + PL::kOut + (warp - PL::kEpi0) * 2048;
     const uint32_t took = mapa(taken0, 0);
     T* out = static_cast<T*>(g.out);
     const float back = DT == RQ_F16 ? pow2_scale(*g.top, 127) : 1.0f;
@@ -392,13 +402,13 @@ int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top,
   g.K = (int)K;
   g.pieces = (int)(pitch / 128);
   const void* kern = (const void*)mx4_dx_k<DT, BN>;
-  const int rc = ensure_smem_limit(kern, Plan<BN>::kSmem);
+  const int rc = ensure_smem_limit(kern, Plan<DT, BN>::kSmem);
   if (rc != RQ_OK) return rc;
   const int64_t ntile = ((M + 255) / 256) * ((K + BN - 1) / BN), pairs = num_sms() / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * (ntile < pairs ? ntile : pairs)));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Plan<BN>::kSmem;
+  cfg.blockDim = dim3(Plan<DT, BN>::kThreads);
+  cfg.dynamicSmemBytes = Plan<DT, BN>::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -420,10 +430,12 @@ int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top,
 
 }  // namespace
 
-// 256 columns a tile unless that leaves SMs idle, then 128.
+// 256 columns a tile, or 128 where twice the tiles still fit one round: an MMA of
+// 128 columns takes about as long (it reads as much of dy), so a second round of
+// them costs more than idle SMs.
 int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
            cudaStream_t st) {
-  const bool wide = 2 * ((M + 255) / 256) * ((K + 255) / 256) >= num_sms();
+  const bool wide = 2 * ((M + 255) / 256) * ((K + 255) / 256) > num_sms() / 2;
   if (dt == RQ_BF16)
     return wide ? run<RQ_BF16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_BF16, 128>(dy, ld, M, w, top, K, dx, st);
   return wide ? run<RQ_F16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_F16, 128>(dy, ld, M, w, top, K, dx, st);

@@ -190,14 +190,16 @@ def test_gradient_against_differences():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("scale", [2.0 ** -30, 2.0 ** -12, 2.0 ** 12])
-def test_half_precision_gradient_of_small_and_large_weights(scale):
+@pytest.mark.parametrize("dtype,scale", [(HF, 2.0 ** -30), (HF, 2.0 ** -12), (HF, 2.0 ** 12), (BF, 2.0 ** -118),
+                                         (BF, 2.0 ** -30), (BF, 2.0 ** 12), (BF, 2.0 ** 120)])
+def test_gradient_of_small_and_large_weights(dtype, scale):
     from rocm_qlora.mx4 import mx4_linear, pack_mx4
     g = torch.Generator(device="cuda").manual_seed(6)
-    w = torch.randn(96, 128, generator=g, device="cuda") * scale   # 2^-30: below what fp16 holds
+    w = torch.randn(96, 128, generator=g, device="cuda") * scale   # in fp16 2^-30 is below what the type holds
+    w[:, 32:64] *= 2.0 ** -4
     packed = pack_mx4(w)
-    x = torch.zeros(40, 128, device="cuda", dtype=HF, requires_grad=True)
-    dy = (torch.randn(40, 96, generator=g, device="cuda") * min(1.0, 0.1 / scale)).to(HF)
+    x = torch.zeros(40, 128, device="cuda", dtype=dtype, requires_grad=True)
+    dy = (torch.randn(40, 96, generator=g, device="cuda") * min(1.0, 0.1 / scale)).to(dtype)
     dx, = torch.autograd.grad(mx4_linear(x, packed), x, dy)
     wk = kept(w)
     close(dx, dy.to(F8) @ wk, sums(dy.to(F8), wk.t(), 96))
