@@ -114,16 +114,30 @@ __device__ __forceinline__ void store8f(void* p, int64_t at, int n, const float 
 
 // ------------------------------------------------------------------ norm
 
-// Sums of squares in 64 bits: any order of the sums gives the same 32-bit
-// norm but for ties of the last rounding, and no square leaves the range.
-template <int DT, bool VEC>
-__device__ __forceinline__ double squares8(const void* g, int64_t at, int n) {
-  float v[8];
-  load8f<DT, VEC>(g, at, n, v);
-  double s = 0.0;
+// The square of a value in 64 bits.  Widening takes a conversion, whose pipe
+// does 8 values a cycle; for 16-bit gradients the bits are moved instead: a
+// normal fp32 number's exponent grows by 896.  Zeros and subnormals (whose
+// 64-bit exponent is not the same for all) go through the conversion.
+__device__ __forceinline__ void add_squares(const float (&v)[8], double& s) {
+  uint32_t least = 0x7f800000u;
+  bool finite = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) s = fma((double)v[i], (double)v[i], s);
-  return s;
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t e = __float_as_uint(v[i]) & 0x7f800000u;
+    least = min(least, e);
+    finite &= e != 0x7f800000u;
+  }
+  if (least != 0u && finite) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+      const double d = __hiloint2double((int)((b >> 3) + (896u << 20)), (int)(b << 29));
+      s = fma(d, d, s);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fma((double)v[i], (double)v[i], s);
+  }
 }
 
 template <int DT, int MAX>
@@ -136,14 +150,29 @@ __global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_consta
   b += warp;
   double sum = 0.0;
   int i = b < end ? tensor_of(t, b) : 0;
-  for (; b < end; b += kAdWarps) {
+  while (b < end) {
     while (b >= t.first[i + 1]) ++i;
-    const uint32_t in = b - t.first[i];
+    const int64_t at = (int64_t)(b - t.first[i]) * kAdBlock + lane * 8;
+    const bool aligned = (uintptr_t)t.g[i] % 16 == 0;
+    // four blocks of one tensor at once, so that their loads are on the way together
+    constexpr int N = 4;
+    const uint32_t whole = min(end, t.first[i + 1] - 1);
+    if (aligned && b + (N - 1) * kAdWarps < whole) {
+      float v[N][8];
+#pragma unroll
+      for (int k = 0; k < N; ++k) load8f<DT, true>(t.g[i], at + k * kAdWarps * kAdBlock, 8, v[k]);
+#pragma unroll
+      for (int k = 0; k < N; ++k) add_squares(v[k], sum);
+      b += N * kAdWarps;
+      continue;
+    }
     const bool last = b + 1 == t.first[i + 1];
     const int n = (last ? t.tail[i] : kAdBlock) - lane * 8;
-    const int64_t at = (int64_t)in * kAdBlock + lane * 8;
-    const bool vec = (uintptr_t)t.g[i] % 16 == 0 && (!last || t.tail[i] == kAdBlock);
-    sum += vec ? squares8<DT, true>(t.g[i], at, n) : squares8<DT, false>(t.g[i], at, n);
+    float v[8];
+    if (aligned && (!last || t.tail[i] == kAdBlock)) load8f<DT, true>(t.g[i], at, 8, v);
+    else load8f<DT, false>(t.g[i], at, n, v);
+    add_squares(v, sum);
+    b += kAdWarps;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -219,37 +248,30 @@ __global__ void __launch_bounds__(kAdThreads) adam_begin_k(const __grid_constant
 
 // ------------------------------------------------------- moments in 8 bits
 
-// The root's code of a value t in [0, kRTop]: a float of 4 exponent and 4
-// mantissa bits, whose first 16 codes are the numbers 0 to 15.  Ties to even.
+// max that a NaN wins.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The root's code of a value t in [0, kRTop], in the low byte: a float of 4
+// exponent and 4 mantissa bits, whose first 16 codes are the numbers 0 to 15.
+// Ties to even, by integer rounding of the mantissa or, below 16, by adding
+// 1.5 2^23.
 __device__ __forceinline__ uint32_t root_code(float t) {
   const uint32_t bits = __float_as_uint(t);
-  const uint32_t high = ((bits + 0x3ffffu + ((bits >> 19) & 1u)) >> 19) - (130u << 4);
-  const uint32_t low = __float_as_uint(__fadd_rn(t, 12582912.0f)) & 0xffu;  // 1.5 2^23: rounds to a whole number
+  const uint32_t high = (bits + ((bits >> 19) & 1u) + (0x3ffffu - (130u << 23))) >> 19;
+  const uint32_t low = __float_as_uint(__fadd_rn(t, 12582912.0f));
   return t < 16.0f ? low : high;
 }
-__device__ __forceinline__ float root_value(uint32_t c) {
-  const bool low = c < 16u;
-  const float v = __uint_as_float(((low ? c + 16u : c) << 19) + (130u << 23));
-  return low ? v - 16.0f : v;
+// The value of byte i of w.  A code's bits above exponent 130 are v = (16 + M)
+// 2^(E - 1) from 16 on and v = 8 + c / 2 below, where the value is 2 v - 16:
+// it is the smaller of the two in either case.
+__device__ __forceinline__ float root_value(uint32_t w, int i) {
+  const float v = __uint_as_float(__byte_perm(w, 0u, 0x4440u | (uint32_t)i) * (1u << 19) + (130u << 23));
+  return fminf(v, fmaf(v, 2.0f, -16.0f));
 }
-
-// A block's scales: what its values are multiplied by on the way to codes
-// (0: all codes are 0) and on the way back.
-struct Scale8 {
-  float to, from;
-};
-__device__ __forceinline__ Scale8 scale8(uint32_t top_bits, float most) {
-  const float top = __uint_as_float(top_bits);
-  Scale8 s;
-  const bool live = top >= 0x1p-100f, bad = top_bits >= 0x7f800000u;
-  s.to = live && !bad ? ieee_div(most, top) : 0.0f;
-  s.from = bad ? __uint_as_float(0x7fc00000u) : live ? ieee_div(top, most) : 0.0f;
-  return s;
-}
-
-// Largest magnitude of the warp's values as a bit pattern, in which an
-// infinity or NaN is the largest.
-__device__ __forceinline__ uint32_t warp_top(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
 __device__ __forceinline__ void decode_moments(const uint8_t* codes_m, const uint8_t* codes_r, float2 scale,
                                                int64_t at, float (&m)[8], float (&v)[8]) {
@@ -264,35 +286,45 @@ __device__ __forceinline__ void decode_moments(const uint8_t* codes_m, const uin
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float r = __fmul_rn(root_value(((i < 4 ? cr.x : cr.y) >> (8 * (i & 3))) & 0xffu), scale.y);
+    const float r = __fmul_rn(root_value(i < 4 ? cr.x : cr.y, i & 3), scale.y);
     v[i] = __fmul_rn(r, r);
   }
 }
 
-// m and r = sqrt(v) of a whole warp's block to codes and scales.
+// m and r = sqrt(v) of a whole warp's block to codes and scales.  Of the four
+// quotients a block needs, lanes 0 to 3 have one each: most / max (what values
+// are multiplied by on the way to codes) and max / most, of m and of r.
 __device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&r)[8], int64_t block, int lane,
                                                uint8_t* codes_m, uint8_t* codes_r, float2* scales) {
-  uint32_t tm = 0, tr = 0;
+  float tm = fabsf(m[0]), tr = r[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    tm = max(tm, __float_as_uint(m[i]) & 0x7fffffffu);
-    tr = max(tr, __float_as_uint(r[i]) & 0x7fffffffu);
-  }
-  const Scale8 sm = scale8(warp_top(tm), kMTop), sr = scale8(warp_top(tr), kRTop);
-  if (lane == 0) scales[block] = make_float2(sm.from, sr.from);
-  uint32_t cm[4], cr[2] = {0, 0};
+  for (int i = 1; i < 8; ++i) tm = max_nan(tm, fabsf(m[i])), tr = max_nan(tr, r[i]);
+  // as bit patterns, in which an infinity or NaN is the largest
+  const uint32_t bm = __reduce_max_sync(0xffffffffu, __float_as_uint(tm) & 0x7fffffffu);
+  const uint32_t br = __reduce_max_sync(0xffffffffu, __float_as_uint(tr) & 0x7fffffffu);
+  const uint32_t bits = lane & 1 ? br : bm;
+  const float top = __uint_as_float(bits), most = lane & 1 ? kRTop : kMTop;
+  const bool bad = bits >= 0x7f800000u, live = top >= 0x1p-100f && !bad;
+  float q = ieee_div(lane & 2 ? top : most, lane & 2 ? most : live ? top : 1.0f);
+  q = live ? q : bad && (lane & 2) ? __uint_as_float(0x7fc00000u) : 0.0f;
+  const float to_m = __shfl_sync(0xffffffffu, q, 0), to_r = __shfl_sync(0xffffffffu, q, 1);
+  if (lane == 2 || lane == 3) reinterpret_cast<float*>(scales + block)[lane - 2] = q;
+  uint32_t cm[4], c[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    cm[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[2 * i], sm.to), __fmul_rn(m[2 * i + 1], sm.to)),
+    cm[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[2 * i], to_m), __fmul_rn(m[2 * i + 1], to_m)),
                                      __NV_SATFINITE, __NV_E4M3);
+  const float least = to_r > 0.0f ? 1.0f : 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t c = root_code(__fmul_rn(r[i], sr.to));
-    cr[i / 4] |= (r[i] > 0.0f && sr.to > 0.0f ? max(c, 1u) : 0u) << (8 * (i & 3));
+    const float t = __fmul_rn(r[i], to_r);
+    c[i] = root_code(r[i] > 0.0f ? fmaxf(t, least) : t);
   }
   const int64_t at = block * kAdBlock + lane * 8;
   *reinterpret_cast<uint2*>(codes_m + at) = make_uint2(cm[0] | cm[1] << 16, cm[2] | cm[3] << 16);
-  *reinterpret_cast<uint2*>(codes_r + at) = make_uint2(cr[0], cr[1]);
+  *reinterpret_cast<uint2*>(codes_r + at) =
+      make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                 __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
 
 // ------------------------------------------------------------------ update
@@ -330,12 +362,18 @@ __device__ __forceinline__ void update8(void* p, const void* g, int64_t at, int 
     const float x = __fmul_rn(gv[i], f.w);
     m[i] = __fadd_rn(__fmul_rn(m[i], a.beta1), __fmul_rn(x, a.rest1));
     v[i] = __fadd_rn(__fmul_rn(v[i], a.beta2), __fmul_rn(__fmul_rn(x, x), a.rest2));
-    r[i] = __fsqrt_rn(v[i]);
+    // in 8 bits the root is the state; elsewhere it only divides the step
+    if constexpr (EIGHT) r[i] = __fsqrt_rn(v[i]);
+    else asm("sqrt.approx.f32 %0, %1;" : "=f"(r[i]) : "f"(v[i]));
     if constexpr (LOW) {
       const int16_t l = (int16_t)(low[i / 2] >> (16 * (i & 1)));
       pv[i] = __uint_as_float(__float_as_uint(pv[i]) + (uint32_t)(int32_t)l);
     }
-    pv[i] = pv[i] * f.z - f.x * __fdividef(m[i], r[i] * f.y + a.eps);
+    // The divisor is at least eps or 2^-75, and an approximate reciprocal's error
+    // of 2^-23 is far below what the step's product with lr leaves of p.
+    float q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(r[i], f.y, a.eps)));
+    pv[i] = fmaf(pv[i], f.z, -(f.x * m[i]) * q);
   }
   if constexpr (LOW) {
     // The 32-bit value's upper half as bf16, rounded half away from zero so
