@@ -67,71 +67,111 @@ __device__ __forceinline__ void share(uint32_t blocks, uint32_t& b, uint32_t& en
   end = (uint32_t)((uint64_t)blocks * (blockIdx.x + 1) / gridDim.x);
 }
 
+// A lane's 8 values as they are in memory: 16-bit types packed in 4 words.
+template <int DT> struct Raw { uint32_t w[DT == RQ_F32 ? 8 : 4]; };
+
+template <int DT>
+__device__ __forceinline__ void put(Raw<DT>& r, int i, float x, float y);
+
 // 8 values at `at`, of which the first `n` exist (the others 0); VEC: all, and aligned.
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8f(const void* p, int64_t at, int n, float (&v)[8]) {
+__device__ __forceinline__ Raw<DT> load_raw(const void* p, int64_t at, int n) {
   using T = typename DType<DT>::T;
   const T* from = static_cast<const T*>(p) + at;
-  if constexpr (!VEC) {
+  Raw<DT> r;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int h = 0; h < (DT == RQ_F32 ? 2 : 1); ++h)
+      *reinterpret_cast<uint4*>(r.w + 4 * h) = reinterpret_cast<const uint4*>(from)[h];
+  } else {
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? DType<DT>::to_f32(from[i]) : 0.0f;
-  } else if constexpr (DT == RQ_F32) {
-    *reinterpret_cast<float4*>(v) = reinterpret_cast<const float4*>(from)[0];
-    *reinterpret_cast<float4*>(v + 4) = reinterpret_cast<const float4*>(from)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put(r, i, v[2 * i], v[2 * i + 1]);
+  }
+  return r;
+}
+
+// Values 2 i and 2 i + 1.
+template <int DT>
+__device__ __forceinline__ float2 pair_of(const Raw<DT>& r, int i) {
+  if constexpr (DT == RQ_F32) return make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+  else if constexpr (DT == RQ_BF16) return make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+}
+template <int DT>
+__device__ __forceinline__ void put(Raw<DT>& r, int i, float x, float y) {
+  if constexpr (DT == RQ_F32) r.w[2 * i] = __float_as_uint(x), r.w[2 * i + 1] = __float_as_uint(y);
+  else r.w[i] = pack2<DT>(x, y);
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store_raw(void* p, int64_t at, int n, const Raw<DT>& r) {
+  using T = typename DType<DT>::T;
+  T* to = static_cast<T*>(p) + at;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int h = 0; h < (DT == RQ_F32 ? 2 : 1); ++h)
+      reinterpret_cast<uint4*>(to)[h] = *reinterpret_cast<const uint4*>(r.w + 4 * h);
   } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(from);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == RQ_BF16) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
+      const float2 v = pair_of<DT>(r, i);
+      if (2 * i < n) to[2 * i] = DType<DT>::from_f32(v.x);
+      if (2 * i + 1 < n) to[2 * i + 1] = DType<DT>::from_f32(v.y);
     }
   }
 }
 
 template <int DT, bool VEC>
-__device__ __forceinline__ void store8f(void* p, int64_t at, int n, const float (&v)[8]) {
-  using T = typename DType<DT>::T;
-  T* to = static_cast<T*>(p) + at;
-  if constexpr (!VEC) {
+__device__ __forceinline__ void load8f(const void* p, int64_t at, int n, float (&v)[8]) {
+  const Raw<DT> r = load_raw<DT, VEC>(p, at, n);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) to[i] = DType<DT>::from_f32(v[i]);
-  } else if constexpr (DT == RQ_F32) {
-    reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
-    reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
-  } else {
-    *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
-                                               pack2<DT>(v[6], v[7]));
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = pair_of<DT>(r, i);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
   }
+}
+__device__ __forceinline__ void store8f(float* to, const float (&v)[8]) {
+  reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
+  reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
 }
 
 // ------------------------------------------------------------------ norm
 
-// The square of a value in 64 bits.  Widening takes a conversion, whose pipe
-// does 8 values a cycle; for 16-bit gradients the bits are moved instead: a
-// normal fp32 number's exponent grows by 896.  Zeros and subnormals (whose
-// 64-bit exponent is not the same for all) go through the conversion.
+// Adds the squares of a lane's 8 values in 64 bits.  Widening takes a
+// conversion, whose pipe does 8 values a cycle; for normal numbers the bits are
+// moved instead (the exponent grows by 896), in bf16 two values share the test
+// for others.
+template <int DT>
 __device__ __forceinline__ void add_squares(const float (&v)[8], double& s) {
-  uint32_t least = 0x7f800000u;
-  bool finite = true;
+  bool normal = true;
+  if constexpr (DT == RQ_BF16) {
+    uint32_t least = 0x7f807f80u, most = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t e = __float_as_uint(v[i]) & 0x7f800000u;
-    least = min(least, e);
-    finite &= e != 0x7f800000u;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t e = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632) & 0x7f807f80u;
+      least = __vminu2(least, e);
+      most = __vmaxu2(most, e);
+    }
+    normal = (least & 0xffffu) != 0u && least > 0xffffu && (most & 0xffffu) != 0x7f80u && most < 0x7f800000u;
+  } else {
+    uint32_t least = 0x7f800000u, most = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = __float_as_uint(v[i]) & 0x7f800000u;
+      least = min(least, e);
+      most = max(most, e);
+    }
+    normal = least != 0u && most != 0x7f800000u;
   }
-  if (least != 0u && finite) {
+  if (normal) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-      const double d = __hiloint2double((int)((b >> 3) + (896u << 20)), (int)(b << 29));
+      const double d = __hiloint2double((int)(__umulhi(b, 1u << 29) + (896u << 20)), DT == RQ_BF16 ? 0 : (int)(b << 29));
       s = fma(d, d, s);
     }
   } else {
@@ -162,7 +202,7 @@ __global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_consta
 #pragma unroll
       for (int k = 0; k < N; ++k) load8f<DT, true>(t.g[i], at + k * kAdWarps * kAdBlock, 8, v[k]);
 #pragma unroll
-      for (int k = 0; k < N; ++k) add_squares(v[k], sum);
+      for (int k = 0; k < N; ++k) add_squares<DT>(v[k], sum);
       b += N * kAdWarps;
       continue;
     }
@@ -171,7 +211,7 @@ __global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_consta
     float v[8];
     if (aligned && (!last || t.tail[i] == kAdBlock)) load8f<DT, true>(t.g[i], at, 8, v);
     else load8f<DT, false>(t.g[i], at, n, v);
-    add_squares(v, sum);
+    add_squares<DT>(v, sum);
     b += kAdWarps;
   }
 #pragma unroll
@@ -273,22 +313,14 @@ __device__ __forceinline__ float root_value(uint32_t w, int i) {
   return fminf(v, fmaf(v, 2.0f, -16.0f));
 }
 
-__device__ __forceinline__ void decode_moments(const uint8_t* codes_m, const uint8_t* codes_r, float2 scale,
-                                               int64_t at, float (&m)[8], float (&v)[8]) {
-  const uint2 cm = *reinterpret_cast<const uint2*>(codes_m + at), cr = *reinterpret_cast<const uint2*>(codes_r + at);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1));
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    m[2 * i] = __fmul_rn(f.x, scale.x);
-    m[2 * i + 1] = __fmul_rn(f.y, scale.x);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float r = __fmul_rn(root_value(i < 4 ? cr.x : cr.y, i & 3), scale.y);
-    v[i] = __fmul_rn(r, r);
-  }
+// Values 2 i and 2 i + 1 of m and v from a lane's code words.
+__device__ __forceinline__ void decode2(const uint2& cm, const uint2& cr, const float2& scale, int i, float2& m, float2& v) {
+  const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1)), c = i < 2 ? cr.x : cr.y;
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  m = make_float2(__fmul_rn(f.x, scale.x), __fmul_rn(f.y, scale.x));
+  const float a = __fmul_rn(root_value(c, 2 * i & 3), scale.y), b = __fmul_rn(root_value(c, (2 * i & 3) + 1), scale.y);
+  v = make_float2(__fmul_rn(a, a), __fmul_rn(b, b));
 }
 
 // m and r = sqrt(v) of a whole warp's block to codes and scales.  Of the four
@@ -338,88 +370,114 @@ struct AdState {
   float beta1, rest1, beta2, rest2, eps;
 };
 
+// What bf16 parameters leave: the 32-bit value of a bf16 and its 16 bits, and
+// back, rounded half away from zero so that what is left fits 16 bits with its
+// sign.
+__device__ __forceinline__ float join_low(float p, uint32_t low16) {
+  return __uint_as_float(__float_as_uint(p) + (uint32_t)(int32_t)(int16_t)low16);
+}
+__device__ __forceinline__ float split_low(float p, uint32_t& low16) {
+  const uint32_t bits = __float_as_uint(p);
+  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+  const uint32_t top = finite ? (bits + 0x8000u) & 0xffff0000u : (bits & 0x7fffffu) ? 0x7fc00000u : bits;
+  low16 = (finite ? bits - top : 0u) & 0xffffu;
+  return __uint_as_float(top);
+}
+
+// One value: m, v and p after the step, and r = sqrt(v).
+template <bool EIGHT>
+__device__ __forceinline__ float update(float g, float& m, float& v, float p, const float4& f, const AdState& a) {
+  const float x = __fmul_rn(g, f.w);
+  m = __fadd_rn(__fmul_rn(m, a.beta1), __fmul_rn(x, a.rest1));
+  v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(x, x), a.rest2));
+  // in 8 bits the root is the state (and takes v's place); elsewhere it only divides the step
+  float r, q;
+  if constexpr (EIGHT) v = r = __fsqrt_rn(v);
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  // The divisor is at least eps or 2^-75, and an approximate reciprocal's error
+  // of 2^-23 is far below what the step's product with lr leaves of p.
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(r, f.y, a.eps)));
+  return fmaf(p, f.z, -(f.x * m) * q);
+}
+
 template <int DT, bool VEC, bool EIGHT, bool LOW>
 __device__ __forceinline__ void update8(void* p, const void* g, int64_t at, int n, int64_t block, int lane,
                                         const float4& f, const AdState& a) {
   const int64_t sat = block * kAdBlock + lane * 8;
-  float gv[8], pv[8], m[8], v[8];
-  load8f<DT, VEC>(g, at, n, gv);
-  load8f<DT, VEC>(p, at, n, pv);
-  uint32_t low[4] = {};
-  if constexpr (LOW) {
-    const uint4 w = *reinterpret_cast<const uint4*>(a.low + sat);
-    low[0] = w.x, low[1] = w.y, low[2] = w.z, low[3] = w.w;
-  }
+  const Raw<DT> gr = load_raw<DT, VEC>(g, at, n);
+  Raw<DT> pr = load_raw<DT, VEC>(p, at, n);
+  Raw<RQ_BF16> low = {};
+  if constexpr (LOW) low = load_raw<RQ_BF16, true>(a.low, sat, 8);
+  float m[8], v[8];
+  uint2 cm, cr;
+  float2 scale;
   if constexpr (EIGHT) {
-    decode_moments(static_cast<const uint8_t*>(a.m), static_cast<const uint8_t*>(a.v), a.scales[block], sat, m, v);
+    cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + sat);
+    cr = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + sat);
+    scale = a.scales[block];
   } else {
     load8f<RQ_F32, true>(a.m, sat, 8, m);
     load8f<RQ_F32, true>(a.v, sat, 8, v);
   }
-  float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = __fmul_rn(gv[i], f.w);
-    m[i] = __fadd_rn(__fmul_rn(m[i], a.beta1), __fmul_rn(x, a.rest1));
-    v[i] = __fadd_rn(__fmul_rn(v[i], a.beta2), __fmul_rn(__fmul_rn(x, x), a.rest2));
-    // in 8 bits the root is the state; elsewhere it only divides the step
-    if constexpr (EIGHT) r[i] = __fsqrt_rn(v[i]);
-    else asm("sqrt.approx.f32 %0, %1;" : "=f"(r[i]) : "f"(v[i]));
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (EIGHT) {
+      float2 x, y;
+      decode2(cm, cr, scale, i, x, y);
+      m[2 * i] = x.x, m[2 * i + 1] = x.y;
+      v[2 * i] = y.x, v[2 * i + 1] = y.y;
+    }
+    const float2 gv = pair_of<DT>(gr, i);
+    float2 pv = pair_of<DT>(pr, i);
+    if constexpr (LOW) pv = make_float2(join_low(pv.x, low.w[i]), join_low(pv.y, low.w[i] >> 16));
+    pv.x = update<EIGHT>(gv.x, m[2 * i], v[2 * i], pv.x, f, a);
+    pv.y = update<EIGHT>(gv.y, m[2 * i + 1], v[2 * i + 1], pv.y, f, a);
     if constexpr (LOW) {
-      const int16_t l = (int16_t)(low[i / 2] >> (16 * (i & 1)));
-      pv[i] = __uint_as_float(__float_as_uint(pv[i]) + (uint32_t)(int32_t)l);
+      uint32_t x, y;
+      pv = make_float2(split_low(pv.x, x), split_low(pv.y, y));
+      low.w[i] = x | y << 16;
     }
-    // The divisor is at least eps or 2^-75, and an approximate reciprocal's error
-    // of 2^-23 is far below what the step's product with lr leaves of p.
-    float q;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(r[i], f.y, a.eps)));
-    pv[i] = fmaf(pv[i], f.z, -(f.x * m[i]) * q);
+    put<DT>(pr, i, pv.x, pv.y);
   }
-  if constexpr (LOW) {
-    // The 32-bit value's upper half as bf16, rounded half away from zero so
-    // that what is left fits 16 bits with its sign.
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t bits = __float_as_uint(pv[2 * i + h]);
-        const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-        const uint32_t top = finite ? (bits + 0x8000u) & 0xffff0000u : (bits & 0x7fffffu) ? 0x7fc00000u : bits;
-        w |= ((finite ? bits - top : 0u) & 0xffffu) << (16 * h);
-        pv[2 * i + h] = __uint_as_float(top);
-      }
-      low[i] = w;
-    }
-    *reinterpret_cast<uint4*>(a.low + sat) = make_uint4(low[0], low[1], low[2], low[3]);
-  }
-  store8f<DT, VEC>(p, at, n, pv);
+  store_raw<DT, VEC>(p, at, n, pr);
+  if constexpr (LOW) store_raw<RQ_BF16, true>(a.low, sat, 8, low);
   if constexpr (EIGHT) {
-    encode_moments(m, r, block, lane, static_cast<uint8_t*>(a.m), static_cast<uint8_t*>(a.v), a.scales);
+    encode_moments(m, v, block, lane, static_cast<uint8_t*>(a.m), static_cast<uint8_t*>(a.v), a.scales);
   } else {
-    store8f<RQ_F32, true>(a.m, sat, 8, m);
-    store8f<RQ_F32, true>(a.v, sat, 8, v);
+    store8f(static_cast<float*>(a.m) + sat, m);
+    store8f(static_cast<float*>(a.v) + sat, v);
   }
 }
 
 template <int DT, bool EIGHT, bool LOW, int MAX>
-__global__ void __launch_bounds__(kAdThreads) adam_update_k(const __grid_constant__ AdTensors<MAX> t, const AdState a) {
+__global__ void __launch_bounds__(kAdThreads, EIGHT ? 4 : 3) adam_update_k(const __grid_constant__ AdTensors<MAX> t, const AdState a) {
   grid_begin();
   const int lane = threadIdx.x % 32;
   uint32_t b, end;
   share(t.first[t.count], b, end);
   b += threadIdx.x / 32;
   int i = b < end ? tensor_of(t, b) : 0;
-  for (; b < end; b += kAdWarps) {
+  while (b < end) {
     while (b >= t.first[i + 1]) ++i;
-    const uint32_t in = b - t.first[i];
-    const bool last = b + 1 == t.first[i + 1];
-    const int n = (last ? t.tail[i] : kAdBlock) - lane * 8;
-    const int64_t at = (int64_t)in * kAdBlock + lane * 8, block = (int64_t)t.block[i] + in;
+    void* const p = t.p[i];
+    const void* const g = t.g[i];
     const float4 f = a.factors[t.slot[i]];
-    const bool vec = ((uintptr_t)t.g[i] | (uintptr_t)t.p[i]) % 16 == 0 && (!last || t.tail[i] == kAdBlock);
-    if (vec) update8<DT, true, EIGHT, LOW>(t.p[i], t.g[i], at, n, block, lane, f, a);
-    else update8<DT, false, EIGHT, LOW>(t.p[i], t.g[i], at, n, block, lane, f, a);
+    const uint32_t next = t.first[i + 1];
+    uint32_t in = b - t.first[i];
+    // whole blocks of an aligned tensor, then what is left one by one
+    if (((uintptr_t)g | (uintptr_t)p) % 16 == 0) {
+      const uint32_t whole = min(end, next - (t.tail[i] != kAdBlock));
+      int64_t at = (int64_t)in * kAdBlock + lane * 8, block = (int64_t)t.block[i] + in;
+#pragma unroll 1
+      for (; b < whole; b += kAdWarps, at += kAdWarps * kAdBlock, block += kAdWarps)
+        update8<DT, true, EIGHT, LOW>(p, g, at, 8, block, lane, f, a);
+      in = b - t.first[i];
+    }
+    if (b < end && b < next) {
+      const int n = (b + 1 == next ? t.tail[i] : kAdBlock) - lane * 8;
+      update8<DT, false, EIGHT, LOW>(p, g, (int64_t)in * kAdBlock + lane * 8, n, (int64_t)t.block[i] + in, lane, f, a);
+      b += kAdWarps;
+    }
   }
 }
 
@@ -430,10 +488,18 @@ __global__ void __launch_bounds__(kAdThreads) adam_unpack_k(const uint8_t* codes
   const uint32_t b = blockIdx.x * kAdWarps + threadIdx.x / 32;
   if (b >= blocks) return;
   const int64_t at = (int64_t)b * kAdBlock + threadIdx.x % 32 * 8;
+  const uint2 cm = *reinterpret_cast<const uint2*>(codes_m + at), cr = *reinterpret_cast<const uint2*>(codes_r + at);
+  const float2 scale = scales[b];
   float x[8], y[8];
-  decode_moments(codes_m, codes_r, scales[b], at, x, y);
-  store8f<RQ_F32, true>(m, at, 8, x);
-  store8f<RQ_F32, true>(v, at, 8, y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 s, t;
+    decode2(cm, cr, scale, i, s, t);
+    x[2 * i] = s.x, x[2 * i + 1] = s.y;
+    y[2 * i] = t.x, y[2 * i + 1] = t.y;
+  }
+  store8f(m + at, x);
+  store8f(v + at, y);
 }
 
 __global__ void __launch_bounds__(kAdThreads) adam_pack_k(const float* m, const float* v, uint32_t blocks,
