@@ -426,12 +426,11 @@ RQ_API int rq_token_logprobs_grad(const void* logits, int dtype, int64_t stride_
  *   scales [ceil(M / 128), Kp / 128, 512], 16-byte aligned, in the order that
  *          the tensor cores take: row r, block b is byte
  *          (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of its piece; rows past M
- *          and blocks past K are 0;
- *   top    the largest scale byte but 255 of all rows (or NULL). */
+ *          and blocks past K are 0. */
 #define RQ_MX4_BLOCK 32
 RQ_API int64_t rq_mx4_scale_bytes(int64_t M, int64_t K);
 RQ_API int rq_mx4_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K,
-                uint8_t* codes, uint8_t* scales, int32_t* top, void* stream);
+                uint8_t* codes, uint8_t* scales, void* stream);
 RQ_API int rq_mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K,
                   void* out, int dtype, void* stream);
 
@@ -443,7 +442,8 @@ RQ_API int rq_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_
                   const void* bias, void* out, int dtype, void* stream);
 
 /* The same for rows x [M, K] (bf16 or f16, row stride ld_x) that are packed on
- * the way.  workspace: rq_mx4_linear_workspace_bytes, 256-byte aligned. */
+ * the way.  workspace: rq_mx4_linear_workspace_bytes (0: none), 256-byte
+ * aligned. */
 RQ_API int64_t rq_mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 RQ_API int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M,
                   const uint8_t* w_codes, const uint8_t* w_scales, int64_t N, int64_t K,
@@ -452,16 +452,19 @@ RQ_API int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M,
 /* dx [M, K] (contiguous) = dy [M, N] . w, w the packed weight [N, K] and dy in
  * dtype (bf16 or f16) with row stride ld_dy, a multiple of 8 with dy 16-byte
  * aligned.  w enters in dy's dtype: exact in bf16; in f16 times 2^(127 - top),
- * which leaves out what is below 2^-24 of that.  top: as rq_mx4_pack wrote it. */
+ * top being its largest scale byte but 255, which leaves out what is below
+ * 2^-24 of that.  workspace: RQ_MX4_DX_WORKSPACE bytes, 16-byte aligned (f16
+ * only). */
+#define RQ_MX4_DX_WORKSPACE 1024
 RQ_API int rq_mx4_dx(const void* dy, int dtype, int64_t ld_dy, int64_t M,
-              const uint8_t* w_codes, const uint8_t* w_scales, const int32_t* top, int64_t N, int64_t K,
-              void* dx, void* stream);
+              const uint8_t* w_codes, const uint8_t* w_scales, int64_t N, int64_t K,
+              void* dx, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------- AdamW over many tensors */
 
 /* One tensor of a step: its values, its gradient (both of the call's dtype),
  * how many, its first block in the arenas of the moments, and its place among
- * steps and factors.  Blocks are of RQ_ADAM_BLOCK values, the last one short;
+ * the steps.  Blocks are of RQ_ADAM_BLOCK values, the last one short;
  * a call takes up to RQ_ADAM_TENSORS tensors. */
 typedef struct RqAdamTensor {
   void* param;
@@ -472,34 +475,38 @@ typedef struct RqAdamTensor {
 } RqAdamTensor;
 #define RQ_ADAM_BLOCK 256
 #define RQ_ADAM_TENSORS 1024
-#define RQ_NORM_PARTIALS 592
+#define RQ_NORM_PARTIALS 1184
 
 /* Sums of squares (64 bits) of the gradients of up to RQ_ADAM_TENSORS tensors
  * as RQ_NORM_PARTIALS values; rq_grad_norm_end makes *norm = sqrt(sum) of n. */
 RQ_API int rq_grad_norm_partial(const RqAdamTensor* tensors, int count, int dtype, double* partials, void* stream);
 RQ_API int rq_grad_norm_end(const double* partials, int n, float* norm, void* stream);
 
-/* Begins a step of the tensors: each one's steps[slot] + 1 = t, and
- *   factors[slot] = (lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), 1 - lr decay, c),
- * c = min(1, max_norm / (norm + 1e-6)) with the norm of n_partials values, 1 if
- * n_partials is 0.  lr_at: learning rate on the device (fp32) in lr's place, or NULL. */
-RQ_API int rq_adam_begin(const RqAdamTensor* tensors, int count, double lr, const float* lr_at, double beta1,
-                  double beta2, double decay, const double* partials, int n_partials, float max_norm, float* norm,
-                  int32_t* steps, float* factors, void* stream);
-
-/* The update with those factors:
+/* A step of the tensors, each one's t = steps[slot] + 1, which is counted up:
  *   g = c grad, m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g g,
- *   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ *   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * with c = min(1, max_norm / (norm + 1e-6)) of the norm of n_partials values,
+ * which is written to *norm; c is 1 if n_partials is 0.  lr_at: learning rate on
+ * the device (fp32) in lr's place, or NULL.
  * bits 32: m and v are fp32 arenas [blocks * 256].  bits 8: m holds e4m3 codes
  * of m (448 / max|m|) of a block, v codes of sqrt(v) (507904 / max sqrt(v)) with
  * 4 exponent and 4 mantissa bits (the whole numbers to 31, then 16 steps to a
  * power of two, to 31 2^14; not 0 for v > 0), scales [blocks, 2] what the codes
  * are multiplied by.  low (bf16 parameters, or NULL): int16 [blocks * 256], the
  * difference of a 32-bit value and its bf16 as bit patterns.  Arenas 16-byte
- * aligned. */
+ * aligned.  ticket: one zero, which the call leaves zero. */
+typedef struct RqAdamStep {
+  double lr, beta1, beta2, eps, decay;
+  const float* lr_at;
+  const double* partials;
+  int n_partials;
+  float max_norm;
+  float* norm;
+  int32_t* steps;
+  uint32_t* ticket;
+} RqAdamStep;
 RQ_API int rq_adam_update(const RqAdamTensor* tensors, int count, int dtype, int bits, void* m, void* v,
-                   float* scales, int16_t* low, const float* factors, double beta1, double beta2, double eps,
-                   void* stream);
+                   float* scales, int16_t* low, const RqAdamStep* step, void* stream);
 
 /* Moments of `blocks` blocks between their 8-bit form and fp32 (v, not its root). */
 RQ_API int rq_adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks,

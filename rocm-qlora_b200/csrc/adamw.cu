@@ -7,9 +7,9 @@
 //
 // A tensor's values are cut into blocks of 256 (the last one short); the
 // moments of all tensors lie in one arena of whole blocks.  A warp takes a
-// block, 8 values a lane.  Three launches, each the programmatic dependent of
-// the one before: the norm's partial sums (where it clips), one CTA that ends
-// the norm, counts the steps and forms each tensor's factors, and the update.
+// block, 8 values a lane.  One launch, and one before it, whose programmatic
+// dependent it is, for the norm's partial sums where it clips: every CTA adds
+// those up for itself, and the last one to end counts the tensors' steps.
 //
 // Moments in 8 bits, per block:
 //   m          e4m3 codes of m (448 / max|m|), scale max|m| / 448
@@ -24,6 +24,7 @@
 // multiply-add), so that a code is what the formula in 32 bits gives.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <math.h>
 
 #include "gemv_common.cuh"
 #include "linear_common.cuh"
@@ -41,7 +42,7 @@ struct AdTensors {
   const void* g[MAX];
   uint32_t first[MAX + 1];  // launch-wide number of a tensor's first block; [count]: blocks in all
   uint32_t block[MAX];      // its first block in the arena
-  uint16_t slot[MAX];       // its place among the steps and factors
+  uint16_t slot[MAX];       // its place among the steps
   uint16_t tail[MAX];       // values of its last block
   int count;
 };
@@ -250,42 +251,6 @@ __global__ void __launch_bounds__(kAdThreads) norm_end_k(const double* __restric
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// ---------------------------------------------------------------- factors
-
-struct AdSlots {
-  uint16_t slot[kAdLarge];
-  int count;
-};
-struct AdFactors {
-  double lr, decay, log_beta1, log_beta2;  // log 0 = -inf: the first moment is the gradient itself
-  const float* lr_at;                      // learning rate on the device, or null
-  float max_norm;
-};
-
-// One CTA: ends the norm, counts each tensor's step t and writes its factors
-//   x = lr / (1 - b1^t), y = 1 / sqrt(1 - b2^t), z = 1 - lr wd, w = c.
-// 1 - b^t is -expm1(t log b), in 64 bits.
-__global__ void __launch_bounds__(kAdThreads) adam_begin_k(const __grid_constant__ AdSlots s, AdFactors f,
-                                                           const double* __restrict__ partials, int n_partials,
-                                                           float* __restrict__ norm, int32_t* __restrict__ steps,
-                                                           float4* __restrict__ factors) {
-  grid_begin();
-  float c = 1.0f;
-  if (n_partials > 0) {
-    const float total = (float)sqrt(sum_partials(partials, n_partials));
-    if (threadIdx.x == 0) *norm = total;
-    const float quotient = __fmul_rn(ieee_div(1.0f, __fadd_rn(total, 1e-6f)), f.max_norm);
-    c = quotient > 1.0f ? 1.0f : quotient;  // a NaN stays one
-  }
-  const double lr = f.lr_at ? (double)*f.lr_at : f.lr;
-  for (int i = threadIdx.x; i < s.count; i += kAdThreads) {
-    const int t = steps[s.slot[i]] + 1;
-    steps[s.slot[i]] = t;
-    const double c1 = -expm1(t * f.log_beta1), c2 = -expm1(t * f.log_beta2);
-    factors[s.slot[i]] = make_float4((float)(lr / c1), (float)(1.0 / sqrt(c2)), (float)(1.0 - lr * f.decay), c);
-  }
-}
-
 // ------------------------------------------------------- moments in 8 bits
 
 // max that a NaN wins.
@@ -366,9 +331,26 @@ struct AdState {
   void* v;
   float2* scales;    // 8 bits: [blocks] (m, root)
   int16_t* low;      // what bf16 parameters leave of a 32-bit value, or null
-  const float4* factors;
   float beta1, rest1, beta2, rest2, eps;
+  // the step
+  double lr, decay, log_beta1, log_beta2;  // log 0 = -inf: the first moment is the gradient itself
+  const float* lr_at;                      // learning rate on the device, or null
+  const double* partials;
+  int n_partials;
+  float max_norm;
+  float* norm;
+  int32_t* steps;
+  uint32_t* ticket;
 };
+
+// What a step number t and the norm make of the formula:
+//   x = lr / (1 - b1^t), y = 1 / sqrt(1 - b2^t), z = 1 - lr wd, w = c.
+// 1 - b^t is -expm1(t log b), in 64 bits.
+__device__ __forceinline__ float4 factors_of(const AdState& a, int t, float c) {
+  const double lr = a.lr_at ? (double)*a.lr_at : a.lr;
+  const double c1 = -expm1(t * a.log_beta1), c2 = -expm1(t * a.log_beta2);
+  return make_float4((float)(lr / c1), (float)(1.0 / sqrt(c2)), (float)(1.0 - lr * a.decay), c);
+}
 
 // What bf16 parameters leave: the 32-bit value of a bf16 and its 16 bits, and
 // back, rounded half away from zero so that what is left fits 16 bits with its
@@ -453,15 +435,24 @@ template <int DT, bool EIGHT, bool LOW, int MAX>
 __global__ void __launch_bounds__(kAdThreads, EIGHT ? 4 : 3) adam_update_k(const __grid_constant__ AdTensors<MAX> t, const AdState a) {
   grid_begin();
   const int lane = threadIdx.x % 32;
+  float c = 1.0f;
+  if (a.n_partials > 0) {
+    const float total = (float)sqrt(sum_partials(a.partials, a.n_partials));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = total;
+    const float quotient = __fmul_rn(ieee_div(1.0f, __fadd_rn(total, 1e-6f)), a.max_norm);
+    c = quotient > 1.0f ? 1.0f : quotient;  // a NaN stays one
+  }
   uint32_t b, end;
   share(t.first[t.count], b, end);
   b += threadIdx.x / 32;
-  int i = b < end ? tensor_of(t, b) : 0;
+  int i = b < end ? tensor_of(t, b) : 0, step = 0;
+  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   while (b < end) {
     while (b >= t.first[i + 1]) ++i;
+    const int now = a.steps[t.slot[i]] + 1;
+    if (now != step) f = factors_of(a, step = now, c);
     void* const p = t.p[i];
     const void* const g = t.g[i];
-    const float4 f = a.factors[t.slot[i]];
     const uint32_t next = t.first[i + 1];
     uint32_t in = b - t.first[i];
     // whole blocks of an aligned tensor, then what is left one by one
@@ -478,6 +469,15 @@ __global__ void __launch_bounds__(kAdThreads, EIGHT ? 4 : 3) adam_update_k(const
       update8<DT, false, EIGHT, LOW>(p, g, (int64_t)in * kAdBlock + lane * 8, n, (int64_t)t.block[i] + in, lane, f, a);
       b += kAdWarps;
     }
+  }
+  // every CTA has read the steps before it takes a ticket; the last one counts
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) + 1 == gridDim.x;
+  __syncthreads();
+  if (last) {
+    for (int k = threadIdx.x; k < t.count; k += kAdThreads) ++a.steps[t.slot[k]];
+    if (threadIdx.x == 0) *a.ticket = 0u;
   }
 }
 
@@ -545,13 +545,13 @@ static int norm_t(const RqAdamTensor* list, int count, double* partials, cudaStr
   if (count <= kAdSmall) {
     AdTensors<kAdSmall> t;
     fill(t, list, count);
-    unsigned grid = grid_for(t.first[count], 4);
+    unsigned grid = grid_for(t.first[count], 8);
     if (grid > RQ_NORM_PARTIALS) grid = RQ_NORM_PARTIALS;
     return launch_dependent(norm_partial_k<DT, kAdSmall>, grid, kAdThreads, st, t, partials);
   }
   AdTensors<kAdLarge> t;
   fill(t, list, count);
-  unsigned grid = grid_for(t.first[count], 4);
+  unsigned grid = grid_for(t.first[count], 8);
   if (grid > RQ_NORM_PARTIALS) grid = RQ_NORM_PARTIALS;
   return launch_dependent(norm_partial_k<DT, kAdLarge>, grid, kAdThreads, st, t, partials);
 }
@@ -564,17 +564,6 @@ int grad_norm_partial(const RqAdamTensor* list, int count, int dt, double* parti
 
 int grad_norm_end(const double* partials, int n, float* norm, cudaStream_t st) {
   return launch_dependent(norm_end_k, 1, kAdThreads, st, partials, n, norm);
-}
-
-int adam_begin(const RqAdamTensor* list, int count, double lr, const float* lr_at, double beta1, double beta2,
-               double decay, const double* partials, int n_partials, float max_norm, float* norm, int32_t* steps,
-               float* factors, cudaStream_t st) {
-  AdSlots s;
-  s.count = count;
-  for (int i = 0; i < count; ++i) s.slot[i] = (uint16_t)list[i].slot;
-  const AdFactors f{lr, decay, log(beta1), log(beta2), lr_at, max_norm};
-  return launch_dependent(adam_begin_k, 1, kAdThreads, st, s, f, partials, n_partials, norm, steps,
-                          reinterpret_cast<float4*>(factors));
 }
 
 template <int DT, bool EIGHT, bool LOW, int MAX>
@@ -593,9 +582,28 @@ static int update_d(const RqAdamTensor* list, int count, int dt, const AdState& 
 }
 
 int adam_update(const RqAdamTensor* list, int count, int dt, int bits, void* m, void* v, float* scales, int16_t* low,
-                const float* factors, double beta1, double beta2, double eps, cudaStream_t st) {
-  const AdState a{m, v, reinterpret_cast<float2*>(scales), low, reinterpret_cast<const float4*>(factors), (float)beta1,
-                  (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
+                const RqAdamStep& step, cudaStream_t st) {
+  AdState a = {};
+  a.m = m;
+  a.v = v;
+  a.scales = reinterpret_cast<float2*>(scales);
+  a.low = low;
+  a.beta1 = (float)step.beta1;
+  a.rest1 = (float)(1.0 - step.beta1);
+  a.beta2 = (float)step.beta2;
+  a.rest2 = (float)(1.0 - step.beta2);
+  a.eps = (float)step.eps;
+  a.lr = step.lr;
+  a.decay = step.decay;
+  a.log_beta1 = log(step.beta1);
+  a.log_beta2 = log(step.beta2);
+  a.lr_at = step.lr_at;
+  a.partials = step.partials;
+  a.n_partials = step.n_partials;
+  a.max_norm = step.max_norm;
+  a.norm = step.norm;
+  a.steps = step.steps;
+  a.ticket = step.ticket;
   if (bits == 8)
     return count <= kAdSmall ? update_d<true, kAdSmall>(list, count, dt, a, st)
                              : update_d<true, kAdLarge>(list, count, dt, a, st);

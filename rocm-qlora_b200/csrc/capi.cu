@@ -514,7 +514,7 @@ int64_t rq_mx4_scale_bytes(int64_t M, int64_t K) {
 }
 
 int rq_mx4_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales,
-                int32_t* top, void* stream) {
+                void* stream) {
   RQ_PROLOGUE();
   if (!dtype_ok(dtype)) return RQ_ERR_DTYPE;
   if (!row_stride(M, ld_x, K)) return RQ_ERR_INVALID;
@@ -522,8 +522,8 @@ int rq_mx4_pack(const void* x, int dtype, int64_t ld_x, int64_t M, int64_t K, ui
   if (rc != RQ_OK) return rc;
   if (M * K == 0) return RQ_OK;
   if (!x) return RQ_ERR_INVALID;
-  if ((uintptr_t)x % dtype_size(dtype) || (uintptr_t)top % 4) return RQ_ERR_ALIGN;
-  return mx4_pack(x, dtype, ld_x, M, K, codes, scales, top, (cudaStream_t)stream);
+  if ((uintptr_t)x % dtype_size(dtype)) return RQ_ERR_ALIGN;
+  return mx4_pack(x, dtype, ld_x, M, K, codes, scales, (cudaStream_t)stream);
 }
 
 int rq_mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dtype,
@@ -566,21 +566,23 @@ int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M, const uint8
   if (!row_stride(M, ld_x, K) || !fits((M + 127) / 128 * 128 * (mx4_pitch(K) / 128))) return RQ_ERR_INVALID;
   if (M * N == 0) return RQ_OK;
   if (K < 1 || !x || !out) return RQ_ERR_INVALID;
-  if (!workspace || workspace_bytes < mx4_linear_workspace_bytes(M, N, K)) return RQ_ERR_WORKSPACE;
+  const int64_t need = mx4_linear_workspace_bytes(M, N, K);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return RQ_ERR_WORKSPACE;
   if ((uintptr_t)x % 2 || (uintptr_t)out % 2 || (uintptr_t)bias % 2 || (uintptr_t)workspace % 256) return RQ_ERR_ALIGN;
   return mx4_linear(x, dtype, ld_x, M, Mx4{w_codes, w_scales, N}, K, bias, out, workspace, (cudaStream_t)stream);
 }
 
 int rq_mx4_dx(const void* dy, int dtype, int64_t ld_dy, int64_t M, const uint8_t* w_codes, const uint8_t* w_scales,
-              const int32_t* top, int64_t N, int64_t K, void* dx, void* stream) {
+              int64_t N, int64_t K, void* dx, void* workspace, int64_t workspace_bytes, void* stream) {
   RQ_PROLOGUE();
   int rc = check_product(dtype, M, N, K);
   if (rc == RQ_OK) rc = check_mx4(w_codes, w_scales, N, K);
   if (rc != RQ_OK) return rc;
   if (M * K == 0) return RQ_OK;
-  if (N < 1 || !dy || !dx || !top || ld_dy < N || ld_dy % 8) return RQ_ERR_INVALID;
-  if ((uintptr_t)dy % 16 || (uintptr_t)dx % 2 || (uintptr_t)top % 4) return RQ_ERR_ALIGN;
-  return mx4_dx(dy, dtype, ld_dy, M, Mx4{w_codes, w_scales, N}, top, K, dx, (cudaStream_t)stream);
+  if (N < 1 || !dy || !dx || ld_dy < N || ld_dy % 8) return RQ_ERR_INVALID;
+  if (dtype == RQ_F16 && (!workspace || workspace_bytes < RQ_MX4_DX_WORKSPACE)) return RQ_ERR_WORKSPACE;
+  if ((uintptr_t)dy % 16 || (uintptr_t)dx % 2 || (uintptr_t)workspace % 16) return RQ_ERR_ALIGN;
+  return mx4_dx(dy, dtype, ld_dy, M, Mx4{w_codes, w_scales, N}, K, dx, workspace, (cudaStream_t)stream);
 }
 
 int rq_grad_norm_partial(const RqAdamTensor* tensors, int count, int dtype, double* partials, void* stream) {
@@ -601,35 +603,22 @@ int rq_grad_norm_end(const double* partials, int n, float* norm, void* stream) {
 
 static bool beta_ok(double b) { return b >= 0.0 && b < 1.0; }
 
-int rq_adam_begin(const RqAdamTensor* tensors, int count, double lr, const float* lr_at, double beta1, double beta2,
-                  double decay, const double* partials, int n_partials, float max_norm, float* norm, int32_t* steps,
-                  float* factors, void* stream) {
-  RQ_PROLOGUE();
-  const int rc = check_tensors(tensors, count, RQ_F32, false, true);
-  if (rc != RQ_OK && rc != RQ_ERR_ALIGN) return rc;  // the values' type is the update's to check
-  if (!beta_ok(beta1) || !beta_ok(beta2) || n_partials < 0 || (n_partials > 0 && (!partials || !norm)))
-    return RQ_ERR_INVALID;
-  if (count == 0) return RQ_OK;
-  if (!steps || !factors) return RQ_ERR_INVALID;
-  if ((uintptr_t)partials % 8 || (uintptr_t)norm % 4 || (uintptr_t)steps % 4 || (uintptr_t)factors % 16 ||
-      (uintptr_t)lr_at % 4)
-    return RQ_ERR_ALIGN;
-  return adam_begin(tensors, count, lr, lr_at, beta1, beta2, decay, partials, n_partials, max_norm, norm, steps,
-                    factors, (cudaStream_t)stream);
-}
-
 int rq_adam_update(const RqAdamTensor* tensors, int count, int dtype, int bits, void* m, void* v, float* scales,
-                   int16_t* low, const float* factors, double beta1, double beta2, double eps, void* stream) {
+                   int16_t* low, const RqAdamStep* step, void* stream) {
   RQ_PROLOGUE();
   const int rc = check_tensors(tensors, count, dtype, true, true);
   if (rc != RQ_OK) return rc;
-  if ((bits != 8 && bits != 32) || !beta_ok(beta1) || !beta_ok(beta2) || !(eps >= 0.0)) return RQ_ERR_INVALID;
+  if (!step || (bits != 8 && bits != 32) || !beta_ok(step->beta1) || !beta_ok(step->beta2) || !(step->eps >= 0.0))
+    return RQ_ERR_INVALID;
   if (low && dtype != RQ_BF16) return RQ_ERR_DTYPE;
   if (count == 0) return RQ_OK;
-  if (!m || !v || !factors || (bits == 8 && !scales)) return RQ_ERR_INVALID;
-  if ((uintptr_t)m % 16 || (uintptr_t)v % 16 || (uintptr_t)scales % 8 || (uintptr_t)low % 16 || (uintptr_t)factors % 16)
+  if (!m || !v || (bits == 8 && !scales) || !step->steps || !step->ticket) return RQ_ERR_INVALID;
+  if (step->n_partials < 0 || (step->n_partials > 0 && (!step->partials || !step->norm))) return RQ_ERR_INVALID;
+  if ((uintptr_t)m % 16 || (uintptr_t)v % 16 || (uintptr_t)scales % 8 || (uintptr_t)low % 16 ||
+      (uintptr_t)step->partials % 8 || (uintptr_t)step->norm % 4 || (uintptr_t)step->steps % 4 ||
+      (uintptr_t)step->ticket % 4 || (uintptr_t)step->lr_at % 4)
     return RQ_ERR_ALIGN;
-  return adam_update(tensors, count, dtype, bits, m, v, scales, low, factors, beta1, beta2, eps, (cudaStream_t)stream);
+  return adam_update(tensors, count, dtype, bits, m, v, scales, low, *step, (cudaStream_t)stream);
 }
 
 int rq_adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks, float* m, float* v,

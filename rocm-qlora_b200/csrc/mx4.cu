@@ -28,62 +28,11 @@ static M4Divide m4_divide(uint32_t d) {
   return M4Divide{(uint32_t)((1ull << (31 + s)) / d + 1), 31 + s, d};
 }
 
-// A lane's 8 values at columns col .. col + 7, 0 past K.  VEC: whole 16-byte
-// pieces, so all 8 exist or none does.
-template <int DT, bool VEC>
-__device__ __forceinline__ void m4_load(const typename DType<DT>::T* row, int col, int K, float (&v)[8]) {
-  if constexpr (!VEC) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < K ? DType<DT>::to_f32(row[col + i]) : 0.0f;
-  } else if constexpr (DT == RQ_F32) {
-    const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    *reinterpret_cast<float4*>(v) = col < K ? *reinterpret_cast<const float4*>(row + col) : z;
-    *reinterpret_cast<float4*>(v + 4) = col < K ? *reinterpret_cast<const float4*>(row + col + 4) : z;
-  } else {
-    const uint4 w = col < K ? *reinterpret_cast<const uint4*>(row + col) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == RQ_BF16) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
-    }
-  }
-}
-
-// Eight e2m1 codes (nearest, ties to even, saturating), the first in the low bits.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float by) {
-  uint32_t w;
-  asm("{\n .reg .b8 a, b, c, d;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
-      " mov.b32 %0, {a, b, c, d};\n}\n"
-      : "=r"(w)
-      : "f"(v[0] * by), "f"(v[1] * by), "f"(v[2] * by), "f"(v[3] * by), "f"(v[4] * by), "f"(v[5] * by), "f"(v[6] * by),
-        "f"(v[7] * by));
-  return w;
-}
-
-// The scale byte of a block whose largest magnitude has these bits.
-__device__ __forceinline__ uint32_t m4_scale(uint32_t top) {
-  const uint32_t e = top >> 23;  // 127 + floor(log2 top), 0 below 2^-126
-  return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
-}
-
-// 2^(127 - byte), the factor that takes values to codes.
-__device__ __forceinline__ float m4_factor(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
-
 // A warp has 256 columns of 4 rows.
-template <int DT, bool VEC, bool TOP>
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict__ x, int64_t ld, int64_t M, int K,
                                                          uint32_t warps, M4Divide np, int tiles,
-                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                         int32_t* __restrict__ most) {
+                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   grid_begin();
   using T = typename DType<DT>::T;
   const uint32_t p = blockIdx.x * (kM4Threads / 32) + threadIdx.x / 32;
@@ -99,7 +48,7 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
     const bool any = in && row < M;
     m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), col, any ? K : 0, v[j]);
   }
-  uint32_t bytes = 0, top = 0;  // row j's scale of this lane's block in byte j
+  uint32_t bytes = 0;  // row j's scale of this lane's block in byte j
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uint32_t m = 0;
@@ -109,7 +58,6 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const uint32_t byte = m4_scale(m);
     bytes |= byte << (8 * j);
-    if (TOP && byte != 255u) top = max(top, byte);
     const uint32_t w = e2m1x8(v[j], m4_factor(byte));
     const int64_t row = row0 + 32 * j;
     if (in && row < M) *reinterpret_cast<uint32_t*>(codes + (row * tiles + tile) * 64 + l * 4) = w;
@@ -123,17 +71,6 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
     *reinterpret_cast<uint4*>(scales + ((row0 / 128) * tiles + tile) * 512 + row0 % 32 * 16) =
         make_uint4(__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410),
                    __byte_perm(hi01, hi23, 0x7632));
-  }
-  if constexpr (TOP) {
-    __shared__ uint32_t part[kM4Threads / 32];
-    top = __reduce_max_sync(0xffffffffu, in ? top : 0u);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-#pragma unroll
-      for (int i = 1; i < kM4Threads / 32; ++i) top = max(top, part[i]);
-      atomicMax(most, (int32_t)top);
-    }
   }
 }
 
@@ -180,32 +117,16 @@ static bool m4_rows(const void* p, int64_t ld, int64_t K, int dt) {
   return (uintptr_t)p % 16 == 0 && ld * (dt == RQ_F32 ? 4 : 2) % 16 == 0 && K % 8 == 0;
 }
 
-template <int DT, bool TOP>
-static int m4_pack_t(const void* x, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
-                     cudaStream_t st) {
+int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, cudaStream_t st) {
   const int tiles = (int)(mx4_pitch(K) / 128);
   const M4Divide np = m4_divide((uint32_t)(tiles + 1) / 2);
   const uint32_t warps = (uint32_t)((M + 127) / 128 * 32) * np.by;
-  auto* k = m4_rows(x, ld, K, DT) ? mx4_pack_k<DT, true, TOP> : mx4_pack_k<DT, false, TOP>;
+  const bool vec = m4_rows(x, ld, K, dt);
+  auto* k = dt == RQ_F32 ? (vec ? mx4_pack_k<RQ_F32, true> : mx4_pack_k<RQ_F32, false>)
+            : dt == RQ_BF16 ? (vec ? mx4_pack_k<RQ_BF16, true> : mx4_pack_k<RQ_BF16, false>)
+                            : (vec ? mx4_pack_k<RQ_F16, true> : mx4_pack_k<RQ_F16, false>);
   return launch_dependent(k, (warps + kM4Threads / 32 - 1) / (kM4Threads / 32), kM4Threads, st, x, ld, M, (int)K, warps, np,
-                          tiles, codes, scales, top);
-}
-
-int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
-             cudaStream_t st) {
-  if (top) {
-    const cudaError_t e = cudaMemsetAsync(top, 0, 4, st);
-    if (e != cudaSuccess) {
-      set_cuda_error(e);
-      return RQ_ERR_CUDA;
-    }
-    return dt == RQ_F32    ? m4_pack_t<RQ_F32, true>(x, ld, M, K, codes, scales, top, st)
-           : dt == RQ_BF16 ? m4_pack_t<RQ_BF16, true>(x, ld, M, K, codes, scales, top, st)
-                           : m4_pack_t<RQ_F16, true>(x, ld, M, K, codes, scales, top, st);
-  }
-  return dt == RQ_F32    ? m4_pack_t<RQ_F32, false>(x, ld, M, K, codes, scales, top, st)
-         : dt == RQ_BF16 ? m4_pack_t<RQ_BF16, false>(x, ld, M, K, codes, scales, top, st)
-                         : m4_pack_t<RQ_F16, false>(x, ld, M, K, codes, scales, top, st);
+                          tiles, codes, scales);
 }
 
 int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st) {

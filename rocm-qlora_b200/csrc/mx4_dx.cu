@@ -4,9 +4,9 @@
 // The scales go along k, which the sum does not run over, so the block-scaled
 // tensor cores cannot take w; it is widened to dy's type in shared memory and
 // multiplied by tcgen05.mma kind::f16.  In bf16 every value of w is exact.  In
-// fp16 w is taken times 2^(127 - top) with the largest scale byte `top` (what
-// is then below 2^-24 rounds to a multiple of that), and the epilogue
-// multiplies that back.
+// fp16 w is taken times 2^(127 - top) with its largest scale byte `top`, which a
+// small kernel before finds (what is then below 2^-24 rounds to a multiple of
+// that), and the epilogue multiplies that back.
 //
 // CTA pairs stay and take tiles of 256 tokens x BN columns in turn, as 2-SM
 // MMAs (M = 256): each CTA holds its 128 tokens of dy and widens half of the
@@ -80,7 +80,7 @@ struct Args {
   CUtensorMap amap;   // dy [M][N], box 64 x 128, 128-byte swizzle
   CUtensorMap cmap;   // codes [N][pitch / 2], box BN / 4 bytes x 128
   const uint8_t* scales;
-  const int32_t* top;
+  const int32_t* tops;  // fp16: kTops maxima of scale bytes
   void* out;          // [M][K]
   int M, N, K, pieces;  // pieces of 128 columns
 };
@@ -135,6 +135,35 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const P
   bool ok = true;
   if (lane == 0) ok = wait_pair(bar, parity, ab);
   return __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+}
+
+// Largest scale byte but 255 of a CTA's share of n 16-byte pieces.
+constexpr int kTops = 148;
+static_assert(kTops * 4 <= RQ_MX4_DX_WORKSPACE, "");
+__global__ void __launch_bounds__(512) mx4_tops_k(const uint4* __restrict__ scales, int64_t n, int32_t* __restrict__ tops) {
+  grid_begin();
+  uint32_t top = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 512 + threadIdx.x; i < n; i += kTops * 512) {
+    const uint4 v = scales[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = __vmaxu4(top, w[j] & ~__vcmpeq4(w[j], 0xffffffffu));
+  }
+  top = max(max(top & 255u, top >> 8 & 255u), max(top >> 16 & 255u, top >> 24));
+  top = __reduce_max_sync(0xffffffffu, top);
+  __shared__ uint32_t part[16];
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) top = max(top, part[i]);
+    tops[blockIdx.x] = (int32_t)top;
+  }
+}
+// The largest of them, by a warp.
+__device__ __forceinline__ int top_of(const int32_t* tops, int lane) {
+  int top = 0;
+  for (int i = lane; i < kTops; i += 32) top = max(top, tops[i]);
+  return __reduce_max_sync(0xffffffffu, top);
 }
 
 template <int DT, int BN>
@@ -250,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     const int w = (warp - 2) % kWiden, row = (w & 3) * 32 + lane, col = (w >> 2) * (BN / 4);
     const uint32_t store = PL::kB + col / 64 * PL::kChunk + row * 128;
     const int unit = col % 64 / 8;
-    const int top = DT == RQ_F16 ? *g.top : 127;
+    const int top = DT == RQ_F16 ? top_of(g.tops, lane) : 127;
     // codes: 16-byte pieces of a row of BN / 4 bytes, in the swizzle of their TMA box
     const uint32_t load = PL::kC + row * (BN / 4);
     const int swz = BN == 256 ? (row >> 1) & 3 : (row >> 2) & 1, piece = col / 32;
@@ -306,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     unsigned char* stage = sm + PL::kOut + (warp - PL::kEpi0) * 2048;
     const uint32_t took = mapa(taken0, 0);
     T* out = static_cast<T*>(g.out);
-    const float back = DT == RQ_F16 ? pow2_scale(*g.top, 127) : 1.0f;
+    const float back = DT == RQ_F16 ? pow2_scale(top_of(g.tops, lane), 127) : 1.0f;
     const bool rows16 = (uintptr_t)out % 16 == 0 && g.K % 8 == 0;
     for (int n = 0; n < tiles; ++n) {
       const int t = first + n * stride, m0 = t % mt * 256 + (int)rank * 128 + quad * 32, c0 = t / mt * BN;
@@ -377,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
 }
 
 template <int DT, int BN>
-int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx, cudaStream_t st) {
+int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, int64_t K, void* dx, void* ws, cudaStream_t st) {
   Args g;
   const int64_t pitch = mx4_pitch(K);
   {
@@ -395,7 +424,7 @@ int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top,
     if (rc != RQ_OK) return rc;
   }
   g.scales = w.scales;
-  g.top = top;
+  g.tops = static_cast<const int32_t*>(ws);
   g.out = dx;
   g.M = (int)M;
   g.N = (int)w.rows;
@@ -433,12 +462,15 @@ int run(const void* dy, int64_t ld, int64_t M, const Mx4& w, const int32_t* top,
 // 256 columns a tile, or 128 where twice the tiles still fit one round: an MMA of
 // 128 columns takes about as long (it reads as much of dy), so a second round of
 // them costs more than idle SMs.
-int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
-           cudaStream_t st) {
+int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, void* dx, void* ws, cudaStream_t st) {
   const bool wide = 2 * ((M + 255) / 256) * ((K + 255) / 256) > num_sms() / 2;
   if (dt == RQ_BF16)
-    return wide ? run<RQ_BF16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_BF16, 128>(dy, ld, M, w, top, K, dx, st);
-  return wide ? run<RQ_F16, 256>(dy, ld, M, w, top, K, dx, st) : run<RQ_F16, 128>(dy, ld, M, w, top, K, dx, st);
+    return wide ? run<RQ_BF16, 256>(dy, ld, M, w, K, dx, ws, st) : run<RQ_BF16, 128>(dy, ld, M, w, K, dx, ws, st);
+  const int64_t pieces = (w.rows + 127) / 128 * (mx4_pitch(K) / 128) * 32;
+  const int rc = launch_dependent(mx4_tops_k, kTops, 512, st, reinterpret_cast<const uint4*>(w.scales), pieces,
+                                  static_cast<int32_t*>(ws));
+  if (rc != RQ_OK) return rc;
+  return wide ? run<RQ_F16, 256>(dy, ld, M, w, K, dx, ws, st) : run<RQ_F16, 128>(dy, ld, M, w, K, dx, ws, st);
 }
 
 }  // namespace rq

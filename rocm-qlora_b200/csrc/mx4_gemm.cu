@@ -60,22 +60,26 @@ constexpr uint32_t kPiece = 512;
 
 constexpr int kPark = 132;                    // floats of a token's parked sums
 
-template <int BN>
+// PACK: Q's rows come in 16 bits and are packed by the epilogue warps, for all of
+// the CTA's stages (beside the ring), while the first of P's are on their way.
+template <int BN, bool PACK>
 struct Plan {
   static constexpr int NB = (BN + 127) / 128;                       // scale pieces of Q a 128 columns
-  static constexpr uint32_t kQBytes = BN * 128;
-  static constexpr uint32_t kSP = kPBytes + kQBytes;                // P's scale pieces in a stage
-  static constexpr uint32_t kSQ = kSP + 2 * kPiece;                 // Q's: [piece][128 columns]
-  static constexpr uint32_t kStage = kSQ + 2 * NB * kPiece;
-  static constexpr int kStages = BN == 128 ? 5 : 6;
+  static constexpr uint32_t kQCodes = BN * 128, kQScales = 2 * NB * kPiece;  // [piece][128 columns]
+  static constexpr uint32_t kQStage = kQCodes + kQScales;
+  static constexpr uint32_t kSP = kPBytes;                          // P's scale pieces in a stage
+  static constexpr uint32_t kQ = kSP + 2 * kPiece;                  // Q's codes, then scales
+  static constexpr uint32_t kStage = kQ + (PACK ? 0 : kQStage);
+  // two CTAs an SM
+  static constexpr int kStages = BN == 128 ? 3 : 4;
   static constexpr uint32_t kRed = BN * kPark * 4;                  // parked sums, in the ring's place
   static constexpr uint32_t kRing = kStages * kStage;
   static constexpr uint32_t kSmem = (kRing > kRed ? kRing : kRed) + 1024;
   static constexpr uint32_t kAcc = BN < 32 ? 32 : BN;               // accumulator columns
   static constexpr uint32_t kSlotCols = 2 * (4 + 4 * NB);           // scale columns of a slot
   static constexpr uint32_t kNeed = kAcc + kStages * kSlotCols;
-  static constexpr uint32_t kCols = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
-  static_assert(kNeed <= 512 && kStage % 1024 == 0 && kSmem <= 226 * 1024, "");
+  static constexpr uint32_t kCols = kNeed <= 128 ? 128 : 256;
+  static_assert(kNeed <= 256 && kStage % 1024 == 0 && kQStage % 1024 == 0 && kRed <= kRing && kSmem <= 113 * 1024, "");
 };
 
 struct Args {
@@ -86,6 +90,10 @@ struct Args {
   void* out;
   int prows, qrows, tiles;  // tiles: pieces of 128 columns
   int64_t ld;
+  const void* x;            // PACK: Q's rows [qrows, K]
+  int64_t ldx;
+  int K, most;              // most: stages of a CTA
+  bool vec;
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -138,19 +146,19 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   return false;
 }
 // out[q, p] (tokens Q, outputs P): sums of its share of the columns.
-template <int DT, int BN>
-__global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant__ Args g) {
-  using PL = Plan<BN>;
+template <int DT, int BN, bool PACK>
+__global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant__ Args g) {
+  using PL = Plan<BN, PACK>;
   using T = typename DType<DT>::T;
   constexpr int S = PL::kStages, NB = PL::NB;
   extern __shared__ __align__(1024) unsigned char dsm[];
-  __shared__ __align__(8) uint64_t bars[2 * S + 1];
+  __shared__ __align__(8) uint64_t bars[2 * S + 2];
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag, issued, consumed;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
   unsigned char* sm = dsm + (sbase - sraw);
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S, accbar = empty0 + 8 * S, qbar = accbar + 8;
   volatile int* abort = &abort_flag;
   const int q0 = blockIdx.x * BN, p0 = blockIdx.y * (int)kP;
   const int sk = gridDim.z, rank = blockIdx.z;
@@ -163,6 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
       mbar_init(empty0 + 8 * i, 1);
     }
     mbar_init(accbar, 1);
+    mbar_init(qbar, kEpiWarps);
     abort_flag = issued = consumed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -188,31 +197,34 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
         if (i >= S && !wait(empty0 + 8 * slot, ((i / S) - 1) & 1, abort)) break;
         const uint32_t at = sbase + slot * PL::kStage, bar = full0 + 8 * slot;
         const uint32_t bytes = (uint32_t)min(2, g.tiles - 2 * st) * kPiece;
-        mbar_expect_tx(bar, kPBytes + PL::kQBytes + (1 + qpieces) * bytes);
+        mbar_expect_tx(bar, PACK ? kPBytes + bytes : kPBytes + PL::kQCodes + (1 + qpieces) * bytes);
         tma_2d(at, &g.pmap, st * 128, p0, bar);
-        tma_2d(at + kPBytes, &g.qmap, st * 128, q0, bar);
         bulk_load(at + PL::kSP, ps + (int64_t)st * 2 * kPiece, bytes, bar);
-        for (int j = 0; j < qpieces; ++j)
-          bulk_load(at + PL::kSQ + j * 2 * kPiece, qs + ((int64_t)j * g.tiles + st * 2) * kPiece, bytes, bar);
+        if constexpr (!PACK) {
+          tma_2d(at + PL::kQ, &g.qmap, st * 128, q0, bar);
+          for (int j = 0; j < qpieces; ++j)
+            bulk_load(at + PL::kQ + PL::kQCodes + j * 2 * kPiece, qs + ((int64_t)j * g.tiles + st * 2) * kPiece, bytes, bar);
+        }
         *reinterpret_cast<volatile int*>(&issued) = i + 1;
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      for (int st = s0; st < s1; ++st) {
+      const bool packed = !PACK || wait(qbar, 0, abort);
+      for (int st = s0; st < s1 && packed; ++st) {
         const int i = st - s0, slot = i % S;
         if (!wait(full0 + 8 * slot, (i / S) & 1, abort)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t at = sbase + slot * PL::kStage, tsc = tmem + PL::kAcc + slot * PL::kSlotCols;
+        const uint32_t at = sbase + slot * PL::kStage, q = PACK ? sbase + PL::kRing + i * PL::kQStage : at + PL::kQ, tsc = tmem + PL::kAcc + slot * PL::kSlotCols;
         const int nt = min(2, g.tiles - 2 * st);
         for (int t = 0; t < nt; ++t) {
           const uint32_t tp = tsc + t * (PL::kSlotCols / 2), tq = tp + 4;
           copy_scales(tp, at + PL::kSP + t * kPiece);
 #pragma unroll
-          for (int j = 0; j < NB; ++j) copy_scales(tq + 4 * j, at + PL::kSQ + (2 * j + t) * kPiece);
+          for (int j = 0; j < NB; ++j) copy_scales(tq + 4 * j, q + PL::kQCodes + (2 * j + t) * kPiece);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            mma_mx4<1>(tmem, sw128_desc(at + (2 * t + h) * 32), sw128_desc(at + kPBytes + (2 * t + h) * 32),
+            mma_mx4<1>(tmem, sw128_desc(at + (2 * t + h) * 32), sw128_desc(q + (2 * t + h) * 32),
                        idesc_mx4<128, BN>(h), tp, tq, (i > 0 || t > 0 || h > 0) ? 1u : 0u);
         }
         mma_commit(empty0 + 8 * slot);
@@ -220,6 +232,35 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_split_k(const __grid_constant
       }
       mma_commit(accbar);
     }
+  } else if constexpr (PACK) {
+    // a warp packs the 256 columns of a token's stage: 8 values a lane, a code
+    // row of 128 bytes in the swizzle of the TMA tiles
+    const T* x = static_cast<const T*>(g.x);
+    const int rows = min(BN, g.qrows - q0);
+    for (int e = warp - 2; e < (s1 - s0) * rows; e += kEpiWarps) {
+      const int i = e / rows, r = e % rows;
+      unsigned char* q = sm + PL::kRing + i * PL::kQStage;
+      const T* row = x + (int64_t)(q0 + r) * g.ldx;
+      const int col = (s0 + i) * 256 + lane * 8;
+      float v[8];
+      if (g.vec) m4_load<DT, true>(row, col, g.K, v);
+      else m4_load<DT, false>(row, col, g.K, v);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t byte = m4_scale(top);
+      *reinterpret_cast<uint32_t*>(q + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + lane % 4 * 4) = e2m1x8(v, m4_factor(byte));
+      uint32_t word = byte << (lane % 16 / 4 * 8);
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if (lane % 16 == 0)
+        *reinterpret_cast<uint32_t*>(q + PL::kQCodes + lane / 16 * kPiece + r / 128 * 2 * kPiece + r % 32 * 16 + r % 128 / 32 * 4) = word;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qbar);
   }
   __syncwarp();
 
@@ -602,12 +643,28 @@ int code_map(const Mx4& x, int64_t pitch, uint32_t rows, CUtensorMap* map) {
   return tensor_map_encode(CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 2, x.codes, d, s, b, map);
 }
 
-template <int DT, int BN>
-int split_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int sk, cudaStream_t st) {
-  const int64_t pitch = mx4_pitch(K);
+// Few tokens: the columns are split until two CTAs an SM have work, with at least
+// two stages each.
+int split_for(int64_t tiles, int64_t steps) {
+  const int64_t room = 2 * num_sms() / tiles, most = steps / 2;
+  const int64_t sk = room < most ? room : most;
+  return sk < 1 ? 1 : sk > 8 ? 8 : (int)sk;
+}
+
+struct Rows {  // tokens in 16 bits
+  const void* x;
+  int64_t ld;
+};
+
+template <int DT, int BN, bool PACK>
+int split_t(const Mx4& a, const Rows& x, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
+  using PL = Plan<BN, PACK>;
+  const int64_t pitch = mx4_pitch(K), steps = (pitch / 128 + 1) / 2;
   Args g;
   int rc = code_map(b, pitch, kP, &g.pmap);
-  if (rc == RQ_OK) rc = code_map(a, pitch, BN, &g.qmap);
+  if (rc != RQ_OK) return rc;
+  if constexpr (PACK) g.qmap = g.pmap;
+  else rc = code_map(a, pitch, BN, &g.qmap);
   if (rc != RQ_OK) return rc;
   g.pscales = b.scales;
   g.qscales = a.scales;
@@ -617,8 +674,16 @@ int split_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, 
   g.qrows = (int)a.rows;
   g.tiles = (int)(pitch / 128);
   g.ld = b.rows;
+  g.x = x.x;
+  g.ldx = x.ld;
+  g.K = (int)K;
+  g.vec = (uintptr_t)x.x % 16 == 0 && x.ld % 8 == 0 && K % 8 == 0;
+  const int64_t tiles = ((b.rows + kP - 1) / kP) * ((a.rows + BN - 1) / BN);
+  const int sk = split_for(tiles, steps);
+  const uint32_t smem = PL::kSmem + (PACK ? (uint32_t)((steps + sk - 1) / sk) * PL::kQStage : 0);
+  if (smem > 226 * 1024) return RQ_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((a.rows + BN - 1) / BN), (unsigned)((b.rows + kP - 1) / kP), (unsigned)sk);
-  return launch((const void*)mx4_split_k<DT, BN>, Plan<BN>::kSmem, grid, kThreads, dim3(1, 1, (unsigned)sk), &g, st);
+  return launch((const void*)mx4_split_k<DT, BN, PACK>, smem, grid, kThreads, dim3(1, 1, (unsigned)sk), &g, st);
 }
 
 template <int DT>
@@ -643,20 +708,13 @@ int pair_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, c
 
 template <int DT>
 int matmul_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
-  const int64_t steps = (mx4_pitch(K) / 128 + 1) / 2, sms = num_sms();
-  if (a.rows > 256 && ((a.rows + 255) / 256) * ((b.rows + 255) / 256) * 2 >= sms / 2) return pair_t<DT>(a, b, K, bias, out, st);
-  // the narrowest tile that holds the tokens, or 128 of them; then columns are
-  // split until the grid fills the GPU, with at least two stages a CTA
-  const int bn = a.rows <= 16 ? 16 : a.rows <= 32 ? 32 : a.rows <= 64 ? 64 : 128;
-  const int64_t tiles = ((b.rows + kP - 1) / kP) * ((a.rows + bn - 1) / bn);
-  int sk = 1;
-  while (sk < 8 && tiles * sk * 2 <= sms && steps >= 4 * sk) sk *= 2;
-  switch (bn) {
-    case 16: return split_t<DT, 16>(a, b, K, bias, out, sk, st);
-    case 32: return split_t<DT, 32>(a, b, K, bias, out, sk, st);
-    case 64: return split_t<DT, 64>(a, b, K, bias, out, sk, st);
-    default: return split_t<DT, 128>(a, b, K, bias, out, sk, st);
-  }
+  if (a.rows > 256 && ((a.rows + 255) / 256) * ((b.rows + 255) / 256) * 4 >= num_sms()) return pair_t<DT>(a, b, K, bias, out, st);
+  // the narrowest tile that holds the tokens, or 128 of them
+  const Rows x{nullptr, 0};
+  if (a.rows <= 16) return split_t<DT, 16, false>(a, x, b, K, bias, out, st);
+  if (a.rows <= 32) return split_t<DT, 32, false>(a, x, b, K, bias, out, st);
+  if (a.rows <= 64) return split_t<DT, 64, false>(a, x, b, K, bias, out, st);
+  return split_t<DT, 128, false>(a, x, b, K, bias, out, st);
 }
 
 }  // namespace
@@ -665,18 +723,29 @@ int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* ou
   return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, b, K, bias, out, st) : matmul_t<RQ_F16>(a, b, K, bias, out, st);
 }
 
+// Up to 16 tokens are packed by the product's own CTAs, unless a row is so long
+// that a CTA's share does not fit its shared memory.
+constexpr int64_t kPackRows = 16, kPackColumns = 12800;  // 50 stages
+static bool packs(int64_t M, int64_t K) { return M <= kPackRows && K <= kPackColumns; }
+
 // Codes of x, then their scales.
 static int64_t code_bytes(int64_t M, int64_t K) { return (M * mx4_pitch(K) / 2 + 255) / 256 * 256; }
 int64_t mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   (void)N;
-  return code_bytes(M, K) + (M + 127) / 128 * (mx4_pitch(K) / 128) * 512;
+  return packs(M, K) ? 0 : code_bytes(M, K) + (M + 127) / 128 * (mx4_pitch(K) / 128) * 512;
 }
 
 int mx4_linear(const void* x, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, const void* bias, void* out,
                void* ws, cudaStream_t st) {
+  if (packs(M, K)) {
+    const Mx4 a{nullptr, nullptr, M};
+    const Rows rows{x, ld};
+    return dt == RQ_BF16 ? split_t<RQ_BF16, 16, true>(a, rows, w, K, bias, out, st)
+                         : split_t<RQ_F16, 16, true>(a, rows, w, K, bias, out, st);
+  }
   uint8_t* codes = static_cast<uint8_t*>(ws);
   uint8_t* scales = codes + code_bytes(M, K);
-  const int rc = mx4_pack(x, dt, ld, M, K, codes, scales, nullptr, st);
+  const int rc = mx4_pack(x, dt, ld, M, K, codes, scales, st);
   if (rc != RQ_OK) return rc;
   return mx4_matmul(Mx4{codes, scales, M}, w, K, bias, out, dt, st);
 }

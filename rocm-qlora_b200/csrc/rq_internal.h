@@ -173,24 +173,19 @@ struct Mx4 {
   int64_t rows;
 };
 inline int64_t mx4_pitch(int64_t K) { return (K + 127) / 128 * 128; }
-int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, int32_t* top,
-             cudaStream_t st);
+int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* codes, uint8_t* scales, cudaStream_t st);
 int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st);
 int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int dt, cudaStream_t st);
 int64_t mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mx4_linear(const void* x, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, const void* bias, void* out,
                void* ws, cudaStream_t st);
-int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, const int32_t* top, int64_t K, void* dx,
-           cudaStream_t st);
+int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, void* dx, void* ws, cudaStream_t st);
 
 // AdamW over many tensors (adamw.cu).
 int grad_norm_partial(const RqAdamTensor* list, int count, int dt, double* partials, cudaStream_t st);
 int grad_norm_end(const double* partials, int n, float* norm, cudaStream_t st);
-int adam_begin(const RqAdamTensor* list, int count, double lr, const float* lr_at, double beta1, double beta2,
-               double decay, const double* partials, int n_partials, float max_norm, float* norm, int32_t* steps,
-               float* factors, cudaStream_t st);
 int adam_update(const RqAdamTensor* list, int count, int dt, int bits, void* m, void* v, float* scales, int16_t* low,
-                const float* factors, double beta1, double beta2, double eps, cudaStream_t st);
+                const RqAdamStep& step, cudaStream_t st);
 int adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks, float* m, float* v,
                 cudaStream_t st);
 int adam_pack(const float* m, const float* v, int64_t blocks, uint8_t* m8, uint8_t* r8, float* scales,

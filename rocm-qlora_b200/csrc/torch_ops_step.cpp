@@ -36,22 +36,17 @@ void check_packed(const Tensor& codes, const Tensor& scales, int64_t K) {
                     "not the packed 4-bit form of rows of ", K, " values");
 }
 
-std::tuple<Tensor, Tensor, Tensor> mx4_pack(const Tensor& x, bool with_top) {
+std::tuple<Tensor, Tensor> mx4_pack(const Tensor& x) {
   check_rows(x, "x");
   const int64_t M = x.size(0), K = x.size(1), pitch = pitch_of(K);
   const auto bytes = x.options().dtype(at::kByte);
   Tensor codes = at::empty({M, pitch / 2}, bytes), scales = at::empty({(M + 127) / 128, pitch / 128, 512}, bytes);
-  Tensor top = at::empty({with_top ? 1 : 0}, x.options().dtype(at::kInt));
-  if (x.is_meta()) return {codes, scales, top};
+  if (x.is_meta() || x.numel() == 0) return {codes, scales};
   const c10::cuda::CUDAGuard guard(x.device());
-  if (x.numel() == 0) {
-    top.zero_();
-  } else {
-    check(rq_mx4_pack(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), M, K, codes.data_ptr<uint8_t>(),
-                      scales.data_ptr<uint8_t>(), with_top ? top.data_ptr<int32_t>() : nullptr, stream_of(x)),
-          "rq_mx4_pack");
-  }
-  return {codes, scales, top};
+  check(rq_mx4_pack(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), M, K, codes.data_ptr<uint8_t>(),
+                    scales.data_ptr<uint8_t>(), stream_of(x)),
+        "rq_mx4_pack");
+  return {codes, scales};
 }
 
 Tensor mx4_unpack(const Tensor& codes, const Tensor& scales, int64_t K, at::ScalarType dtype) {
@@ -92,20 +87,20 @@ Tensor mx4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t need = rq_mx4_linear_workspace_bytes(M, N, K);
   TORCH_CHECK(need >= 0, "rocm_qlora: no product of [", M, ", ", K, "] and [", N, ", ", K, "]");
-  Tensor ws = at::empty({need}, codes.options());
+  Tensor ws;  // one token's rows need none
+  if (need > 0) ws = at::empty({need}, codes.options());
   const Tensor c = aligned(codes), s = aligned(scales);
   check(rq_mx4_linear(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), M, c.data_ptr<uint8_t>(),
-                      s.data_ptr<uint8_t>(), N, K, ptr(bias), out.data_ptr(), ws.data_ptr(), need, stream_of(x)),
+                      s.data_ptr<uint8_t>(), N, K, ptr(bias), out.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need, stream_of(x)),
         "rq_mx4_linear");
   return out;
 }
 
-Tensor mx4_dx(const Tensor& dy, const Tensor& codes, const Tensor& scales, const Tensor& top, int64_t K) {
+Tensor mx4_dx(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t K) {
   check_rows(dy, "dy");
   check_packed(codes, scales, K);
-  one_device(dy, codes, top);
-  TORCH_CHECK_VALUE(dy.size(1) == codes.size(0) && top.numel() == 1 && top.scalar_type() == at::kInt,
-                    "dy must have a column for each of the ", codes.size(0), " rows packed, and top be their largest scale");
+  one_device(dy, codes);
+  TORCH_CHECK_VALUE(dy.size(1) == codes.size(0), "dy must have a column for each of the ", codes.size(0), " rows packed");
   const int64_t M = dy.size(0), N = dy.size(1);
   if (N == 0) return at::zeros({M, K}, dy.options());
   Tensor dx = at::empty({M, K}, dy.options());
@@ -117,8 +112,11 @@ Tensor mx4_dx(const Tensor& dy, const Tensor& codes, const Tensor& scales, const
     d.copy_(dy);
   }
   const Tensor c = aligned(codes), s = aligned(scales);
+  Tensor ws;
+  if (dy.scalar_type() == at::kHalf) ws = at::empty({RQ_MX4_DX_WORKSPACE}, codes.options());
   check(rq_mx4_dx(d.data_ptr(), dtype_code(d.scalar_type()), d.stride(0), M, c.data_ptr<uint8_t>(),
-                  s.data_ptr<uint8_t>(), top.data_ptr<int32_t>(), N, K, dx.data_ptr(), stream_of(dy)),
+                  s.data_ptr<uint8_t>(), N, K, dx.data_ptr(), ws.defined() ? ws.data_ptr() : nullptr,
+                  RQ_MX4_DX_WORKSPACE, stream_of(dy)),
         "rq_mx4_dx");
   return dx;
 }
@@ -130,16 +128,15 @@ using torch::autograd::variable_list;
 // The rounding of x is passed through: dx = dy . w.
 struct Mx4Linear : Function<Mx4Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales,
-                        const Tensor& top, const optional<Tensor>& bias) {
-    ctx->save_for_backward({codes, scales, top});
+                        const optional<Tensor>& bias) {
+    ctx->save_for_backward({codes, scales});
     ctx->saved_data["K"] = x.size(1);
     return RQ_VIA(mx4_forward, x, codes, scales, bias);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("mx4_linear");
     const auto v = ctx->get_saved_variables();
-    return {RQ_VIA(mx4_dx, rows_of(grads[0]), v[0], v[1], v[2], ctx->saved_data["K"].toInt()), Tensor(), Tensor(),
-            Tensor(), Tensor()};
+    return {RQ_VIA(mx4_dx, rows_of(grads[0]), v[0], v[1], ctx->saved_data["K"].toInt()), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -155,11 +152,11 @@ void check_bias(const optional<Tensor>& bias, int64_t N, at::ScalarType dtype) {
 }
 
 // The public forms: any shape [..., K].
-std::tuple<Tensor, Tensor, Tensor> pack_mx4(const Tensor& x) {
+std::tuple<Tensor, Tensor> pack_mx4(const Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "pack_mx4 needs rows of at least one value, got ", x.sizes());
   check_float(x.scalar_type());
   check_gpu({&x});
-  return RQ_VIA(mx4_pack, rows_of(x.detach()), true);
+  return RQ_VIA(mx4_pack, rows_of(x.detach()));
 }
 
 Tensor unpack_mx4(const Tensor& codes, const Tensor& scales, at::IntArrayRef shape, at::ScalarType dtype) {
@@ -179,17 +176,16 @@ Tensor mx4_matmul(const Tensor& a_codes, const Tensor& a_scales, const Tensor& b
                 dtype);
 }
 
-Tensor mx4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tensor& top, int64_t K,
-                  const optional<Tensor>& bias) {
+Tensor mx4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t K, const optional<Tensor>& bias) {
   check_half(x.scalar_type(), "mx4_linear");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, "x ", x.sizes(), " does not fit a weight of rows of ", K, " values");
   check_bias(bias, codes.size(0), x.scalar_type());
-  check_gpu({&x, &codes, &scales, &top, bias ? &*bias : &x});
+  check_gpu({&x, &codes, &scales, bias ? &*bias : &x});
   const Tensor x2 = rows_of(x);
   const optional<Tensor> b = bias ? optional<Tensor>(bias->contiguous()) : bias;
   // a tangent of forward-mode differentiation goes to the autograd node too, which refuses it
   const bool grad = (at::GradMode::is_enabled() && x.requires_grad()) || x._fw_grad(/*level=*/0).defined();
-  const Tensor y = grad ? Mx4Linear::apply(x2, codes, scales, top, b) : RQ_VIA(mx4_forward, x2, codes, scales, b);
+  const Tensor y = grad ? Mx4Linear::apply(x2, codes, scales, b) : RQ_VIA(mx4_forward, x2, codes, scales, b);
   if (x.dim() == 2) return y;
   auto shape = x.sizes().vec();
   shape.back() = codes.size(0);
@@ -260,7 +256,7 @@ Tensor grad_norm(at::TensorList tensors) {
 struct AdamGroup {
   std::vector<Tensor> params;
   std::vector<int64_t> blocks;  // first block of each
-  Tensor m, v, scales, low, steps, factors;
+  Tensor m, v, scales, low, steps, ticket;
 };
 
 // Held by the optimizer, so that a step is one call whatever the number of
@@ -273,15 +269,15 @@ struct AdamW : torch::CustomClassHolder {
   }
 
   void add_group(std::vector<Tensor> params, Tensor m, Tensor v, optional<Tensor> scales, optional<Tensor> low,
-                 Tensor steps, Tensor factors) {
-    AdamGroup g{std::move(params), {}, m, v, scales.value_or(Tensor()), low.value_or(Tensor()), steps, factors};
+                 Tensor steps, Tensor ticket) {
+    AdamGroup g{std::move(params), {}, m, v, scales.value_or(Tensor()), low.value_or(Tensor()), steps, ticket};
     int64_t at = 0;
     for (const Tensor& p : g.params) {
       g.blocks.push_back(at);
       at += (p.numel() + RQ_ADAM_BLOCK - 1) / RQ_ADAM_BLOCK;
     }
     const auto of = bits == 8 ? at::kByte : at::kFloat;
-    one_device(m, v, scales, low, steps, factors);
+    one_device(m, v, scales, low, steps, ticket);
     TORCH_CHECK_VALUE(m.numel() == at * RQ_ADAM_BLOCK && v.numel() == m.numel() && m.is_contiguous() &&
                           v.is_contiguous() && m.scalar_type() == of && v.scalar_type() == of &&
                           (bits == 32 || (g.scales.defined() && g.scales.is_contiguous() && g.scales.numel() == 2 * at &&
@@ -289,8 +285,8 @@ struct AdamW : torch::CustomClassHolder {
                           (!g.low.defined() || (g.low.is_contiguous() && g.low.numel() == m.numel() &&
                                                 g.low.scalar_type() == at::kShort)) &&
                           steps.is_contiguous() && steps.scalar_type() == at::kInt &&
-                          steps.numel() == (int64_t)g.params.size() && factors.is_contiguous() &&
-                          factors.scalar_type() == at::kFloat && factors.numel() == 4 * steps.numel(),
+                          steps.numel() == (int64_t)g.params.size() && ticket.numel() == 1 &&
+                          ticket.scalar_type() == at::kInt,
                       "the arenas do not fit the parameters");
     groups.push_back(std::move(g));
   }
@@ -356,16 +352,23 @@ struct AdamW : torch::CustomClassHolder {
       if (lrs[i])
         TORCH_CHECK_VALUE(lrs[i]->numel() == 1 && lrs[i]->scalar_type() == at::kFloat && lrs[i]->device() == first.device(),
                           "a learning rate that is a tensor must be one float32 on the parameters' device");
+      RqAdamStep step = {};
+      step.lr = h[0];
+      step.beta1 = h[1];
+      step.beta2 = h[2];
+      step.eps = h[3];
+      step.decay = h[4];
+      step.lr_at = lrs[i] ? lrs[i]->data_ptr<float>() : nullptr;
+      step.partials = clip ? partials.data_ptr<double>() : nullptr;
+      step.n_partials = n;
+      step.max_norm = (float)max_norm;
+      step.norm = clip ? norm.data_ptr<float>() : nullptr;
+      step.steps = g.steps.data_ptr<int32_t>();
+      step.ticket = reinterpret_cast<uint32_t*>(g.ticket.data_ptr<int32_t>());
       in_launches(lists[i], [&](const RqAdamTensor* list, int count, int dt) {
-        check(rq_adam_begin(list, count, h[0], lrs[i] ? lrs[i]->data_ptr<float>() : nullptr, h[1], h[2], h[4],
-                            clip ? partials.data_ptr<double>() : nullptr, n, (float)max_norm,
-                            clip ? norm.data_ptr<float>() : nullptr, g.steps.data_ptr<int32_t>(),
-                            g.factors.data_ptr<float>(), st),
-              "rq_adam_begin");
         check(rq_adam_update(list, count, dt, bits, g.m.data_ptr(), g.v.data_ptr(),
                              bits == 8 ? g.scales.data_ptr<float>() : nullptr,
-                             g.low.defined() ? g.low.data_ptr<int16_t>() : nullptr, g.factors.data_ptr<float>(), h[1],
-                             h[2], h[3], st),
+                             g.low.defined() ? g.low.data_ptr<int16_t>() : nullptr, &step, st),
               "rq_adam_update");
       });
     }
@@ -409,23 +412,23 @@ void adam_pack_(const Tensor& m, const Tensor& v, Tensor m8, Tensor r8, Tensor s
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(rocm_qlora, m) {
-  m.def("mx4_pack(Tensor x, bool with_top) -> (Tensor, Tensor, Tensor)");
+  m.def("mx4_pack(Tensor x) -> (Tensor, Tensor)");
   m.def("mx4_unpack(Tensor codes, Tensor scales, int columns, ScalarType dtype) -> Tensor");
   m.def(
       "mx4_product(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, int columns, Tensor? bias, "
       "ScalarType dtype) -> Tensor");
   m.def("mx4_forward(Tensor x, Tensor codes, Tensor scales, Tensor? bias) -> Tensor");
-  m.def("mx4_dx(Tensor dy, Tensor codes, Tensor scales, Tensor top, int columns) -> Tensor");
+  m.def("mx4_dx(Tensor dy, Tensor codes, Tensor scales, int columns) -> Tensor");
   m.def("norm_of(Tensor[] tensors) -> Tensor");
   m.def("grad_norm(Tensor[] tensors) -> Tensor", &grad_norm);
   m.def("adam_unpack(Tensor m, Tensor r, Tensor scales) -> (Tensor, Tensor)");
   m.def("adam_pack_(Tensor m, Tensor v, Tensor(a!) m8, Tensor(b!) r8, Tensor(c!) scales) -> ()");
-  m.def("pack_mx4(Tensor x) -> (Tensor, Tensor, Tensor)", &pack_mx4);
+  m.def("pack_mx4(Tensor x) -> (Tensor, Tensor)", &pack_mx4);
   m.def("unpack_mx4(Tensor codes, Tensor scales, int[] shape, ScalarType dtype) -> Tensor", &unpack_mx4);
   m.def(
       "mx4_matmul(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, int columns, Tensor? bias, "
       "ScalarType dtype) -> Tensor", &mx4_matmul);
-  m.def("mx4_linear(Tensor x, Tensor codes, Tensor scales, Tensor top, int columns, Tensor? bias) -> Tensor", &mx4_linear);
+  m.def("mx4_linear(Tensor x, Tensor codes, Tensor scales, int columns, Tensor? bias) -> Tensor", &mx4_linear);
   m.class_<AdamW>("AdamW")
       .def(torch::init<int64_t>())
       .def("add_group", &AdamW::add_group)

@@ -53,7 +53,7 @@ _lib_lock = threading.Lock()
 
 
 def _bind(L: ctypes.CDLL) -> None:
-    P, I, I64, F, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
+    P, I, I64, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
     sig = {
         "rq_abi_version": ([], I),
         "rq_status_string": ([I], ctypes.c_char_p),
@@ -95,16 +95,15 @@ def _bind(L: ctypes.CDLL) -> None:
         "rq_preference_loss": ([I64, I64, P, I64, P, P, I, F, F, P, P, P, P, P], I),
         "rq_token_logprobs_grad": ([P, I, I64, I64, I64, I64, I64, P, I64, P, P, I, P, P, P], I),
         "rq_mx4_scale_bytes": ([I64, I64], I64),
-        "rq_mx4_pack": ([P, I, I64, I64, I64, P, P, P, P], I),
+        "rq_mx4_pack": ([P, I, I64, I64, I64, P, P, P], I),
         "rq_mx4_unpack": ([P, P, I64, I64, P, I, P], I),
         "rq_mx4_matmul": ([P, P, I64, P, P, I64, I64, P, P, I, P], I),
         "rq_mx4_linear_workspace_bytes": ([I64, I64, I64], I64),
         "rq_mx4_linear": ([P, I, I64, I64, P, P, I64, I64, P, P, P, I64, P], I),
-        "rq_mx4_dx": ([P, I, I64, I64, P, P, P, I64, I64, P, P], I),
+        "rq_mx4_dx": ([P, I, I64, I64, P, P, I64, I64, P, P, I64, P], I),
         "rq_grad_norm_partial": ([P, I, I, P, P], I),
         "rq_grad_norm_end": ([P, I, P, P], I),
-        "rq_adam_begin": ([P, I, D, P, D, D, D, P, I, F, P, P, P, P], I),
-        "rq_adam_update": ([P, I, I, I, P, P, P, P, P, D, D, D, P], I),
+        "rq_adam_update": ([P, I, I, I, P, P, P, P, P, P], I),
         "rq_adam_unpack": ([P, P, P, I64, P, P, P], I),
         "rq_adam_pack": ([P, P, I64, P, P, P, P], I),
         "launch_int4_dequant_matmul": ([P, P, P, P, P, I, I, I, I], None),
@@ -130,7 +129,7 @@ def exported_symbols() -> Tuple[str, ...]:
             "rq_act8_pack", "rq_act8_unpack", "rq_swiglu8_forward", "rq_swiglu8_backward",
             "rq_token_logprobs", "rq_preference_loss", "rq_token_logprobs_grad",
             "rq_mx4_scale_bytes", "rq_mx4_pack", "rq_mx4_unpack", "rq_mx4_matmul", "rq_mx4_linear_workspace_bytes",
-            "rq_mx4_linear", "rq_mx4_dx", "rq_grad_norm_partial", "rq_grad_norm_end", "rq_adam_begin",
+            "rq_mx4_linear", "rq_mx4_dx", "rq_grad_norm_partial", "rq_grad_norm_end",
             "rq_adam_update", "rq_adam_unpack", "rq_adam_pack",
             "launch_int4_dequant_matmul", "launch_int8_dequant_matmul")
 

@@ -33,7 +33,7 @@ def mx4_linear(x: torch.Tensor, weight: PackedMx4, bias: Optional[torch.Tensor] 
     if len(weight.shape) != 2:
         raise ValueError(f"the weight must be [N, K], got {weight.shape}")
     try:
-        return nat.loaded_ops().mx4_linear(x, weight.codes, weight.scales, weight.top, weight.shape[-1], bias)
+        return nat.loaded_ops().mx4_linear(x, weight.codes, weight.scales, weight.shape[-1], bias)
     except NotImplementedError as e:
         raise nat.NativeUnavailable(str(e)) from None
 
@@ -49,7 +49,6 @@ class Mx4Linear(nn.Module):
         byte = dict(dtype=torch.uint8, device=device)
         self.register_buffer("codes", torch.zeros(out_features, pitch // 2, **byte))
         self.register_buffer("scales", torch.zeros(tiles, pitch // 128, 512, **byte))
-        self.register_buffer("top", torch.zeros(1, dtype=torch.int32, device=device))
         self.register_buffer("bias", torch.zeros(out_features, dtype=dtype, device=device) if bias else None)
 
     @classmethod
@@ -58,14 +57,14 @@ class Mx4Linear(nn.Module):
         w = linear.weight.detach()
         m = cls(linear.in_features, linear.out_features, linear.bias is not None, w.dtype, "meta")
         packed = pack_mx4(nat.to_cuda(w))
-        m.codes, m.scales, m.top = packed.codes, packed.scales, packed.top
+        m.codes, m.scales = packed.codes, packed.scales
         if linear.bias is not None:
             m.bias = linear.bias.detach().to(packed.codes.device)
         return m
 
     @property
     def weight(self) -> PackedMx4:
-        return PackedMx4(self.codes, self.scales, self.top, (self.out_features, self.in_features), self.dtype)
+        return PackedMx4(self.codes, self.scales, (self.out_features, self.in_features), self.dtype)
 
     def dequantized(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return unpack_mx4(self.weight, dtype)

@@ -24,11 +24,9 @@ BLOCK = 32
 class PackedMx4:
     """``codes`` uint8 [rows, Kp / 2] (two a byte, the even column low) and
     ``scales`` uint8 [ceil(rows / 128), Kp / 128, 512] of a tensor of
-    ``shape`` [..., K], with Kp = K rounded up to 128; ``top`` int32 [1], the
-    largest scale byte."""
+    ``shape`` [..., K], with Kp = K rounded up to 128."""
     codes: torch.Tensor
     scales: torch.Tensor
-    top: torch.Tensor
     shape: Tuple[int, ...]
     dtype: torch.dtype
 
@@ -47,10 +45,10 @@ def pack_mx4(x: torch.Tensor) -> PackedMx4:
     """Pack x [..., K] (float32, bfloat16 or float16).  A block that holds an
     infinity or NaN unpacks to NaN."""
     try:
-        codes, scales, top = nat.loaded_ops().pack_mx4(x)
+        codes, scales = nat.loaded_ops().pack_mx4(x)
     except NotImplementedError as e:
         raise nat.NativeUnavailable(str(e)) from None
-    return PackedMx4(codes, scales, top, tuple(x.shape), x.dtype)
+    return PackedMx4(codes, scales, tuple(x.shape), x.dtype)
 
 
 def unpack_mx4(packed: PackedMx4, dtype: Optional[torch.dtype] = None) -> torch.Tensor:

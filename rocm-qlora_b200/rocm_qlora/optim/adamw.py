@@ -5,6 +5,8 @@ from typing import Any, Dict, Iterable, Optional, Tuple, Union
 
 import torch
 
+from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
+
 from rocm_qlora import _native as nat
 
 #: values of a tensor that share the scales of its 8-bit moments
@@ -27,8 +29,8 @@ class AdamW(torch.optim.Optimizer):
         p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
     Parameters are contiguous float32, bfloat16 or float16 tensors on one
-    CUDA device; a step is three launches at most for up to 1024 of a dtype,
-    without host synchronisation, and can be captured into a CUDA graph (steps
+    CUDA device; a step is one launch, or two with clipping, for up to 1024 of a
+    dtype, without host synchronisation, and can be captured into a CUDA graph (steps
     are counted on the device; make ``lr`` a float32 tensor there to change it
     between replays).
 
@@ -103,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
                  scales=torch.zeros(total, 2, device=device) if self.state_bits == 8 else None,
                  low=torch.zeros(total * BLOCK, dtype=torch.int16, device=device) if self.remainder else None,
                  steps=torch.zeros(len(params), dtype=torch.int32, device=device),
-                 factors=torch.zeros(len(params), 4, device=device))
+                 ticket=torch.zeros(1, dtype=torch.int32, device=device))
         self._arenas.append(a)
         at = 0
         for i, (p, n) in enumerate(zip(params, blocks)):
@@ -121,7 +123,7 @@ class AdamW(torch.optim.Optimizer):
         nat.loaded_ops()
         held = torch.classes.rocm_qlora.AdamW(self.state_bits)
         for group, a in zip(self.param_groups, self._arenas):
-            held.add_group(group["params"], a["m"], a["v"], a["scales"], a["low"], a["steps"], a["factors"])
+            held.add_group(group["params"], a["m"], a["v"], a["scales"], a["low"], a["steps"], a["ticket"])
         if self.max_grad_norm is not None:
             self.grad_norm = torch.zeros((), device=self._arenas[0]["m"].device)
         self._native = held
@@ -129,9 +131,18 @@ class AdamW(torch.optim.Optimizer):
 
     # --------------------------------------------------------------- step
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step of every parameter that has a gradient."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_optimizer_pre_hooks \
+                or _global_optimizer_post_hooks or torch.autograd._profiler_enabled():
+            return _step_with_hooks(self, closure)
+        return self._step(closure)
+
+    # the base class wraps step() in hooks and a profiler's range, at twice a
+    # small step's cost: they run where there are any
+    step.hooked = True
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -146,7 +157,7 @@ class AdamW(torch.optim.Optimizer):
             lrs.append(lr if on_device else None)
         clip = self.max_grad_norm is not None
         held.step(hyper, lrs, self.max_grad_norm if clip else -1.0,
-                  self.grad_norm if clip else self._arenas[0]["factors"])
+                  self.grad_norm if clip else self._arenas[0]["ticket"])
         return loss
 
     # ------------------------------------------------------------- states
@@ -196,3 +207,9 @@ class AdamW(torch.optim.Optimizer):
             for k, value in s.items():
                 if k != "params":
                     g[k] = tuple(value) if k == "betas" else value
+
+    def __getstate__(self):
+        raise TypeError("an AdamW is not copied or pickled: save its state_dict()")
+
+
+_step_with_hooks = torch.optim.Optimizer.profile_hook_step(AdamW._step)
