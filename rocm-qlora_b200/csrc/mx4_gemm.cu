@@ -92,8 +92,10 @@ struct Args {
   int64_t ld;
   const void* x;            // PACK: Q's rows [qrows, K]
   int64_t ldx;
-  int K, most;              // most: stages of a CTA
+  int K;
   bool vec;
+  bool early;               // the kernel before this one is the packing of Q's rows, which has itself waited for
+                            // all before it: P is there already
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -185,22 +187,34 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_sh;
-  grid_begin();
+  if (warp > 0 || !g.early) grid_begin();
 
   if (warp == 0) {
+    const uint8_t* ps = g.pscales + (int64_t)(p0 / 128) * g.tiles * kPiece;
+    const uint8_t* qs = g.qscales + (int64_t)(q0 / 128) * g.tiles * kPiece;
+    const int qpieces = min(NB, (g.qrows + 127) / 128 - q0 / 128);  // pieces past the last row do not exist
+    auto load_p = [&](int st, int slot) {
+      const uint32_t at = sbase + slot * PL::kStage, bar = full0 + 8 * slot;
+      const uint32_t bytes = (uint32_t)min(2, g.tiles - 2 * st) * kPiece;
+      mbar_expect_tx(bar, PACK ? kPBytes + bytes : kPBytes + PL::kQCodes + (1 + qpieces) * bytes);
+      tma_2d(at, &g.pmap, st * 128, p0, bar);
+      bulk_load(at + PL::kSP, ps + (int64_t)st * 2 * kPiece, bytes, bar);
+    };
+    const int early = g.early ? min(S, s1 - s0) : 0;
+    if (g.early) {
+      if (lane == 0)
+        for (int i = 0; i < early; ++i) load_p(s0 + i, i);
+      __syncwarp();
+      grid_begin();
+    }
     if (lane == 0) {
-      const uint8_t* ps = g.pscales + (int64_t)(p0 / 128) * g.tiles * kPiece;
-      const uint8_t* qs = g.qscales + (int64_t)(q0 / 128) * g.tiles * kPiece;
-      const int qpieces = min(NB, (g.qrows + 127) / 128 - q0 / 128);  // pieces past the last row do not exist
       for (int st = s0; st < s1; ++st) {
         const int i = st - s0, slot = i % S;
         if (i >= S && !wait(empty0 + 8 * slot, ((i / S) - 1) & 1, abort)) break;
-        const uint32_t at = sbase + slot * PL::kStage, bar = full0 + 8 * slot;
-        const uint32_t bytes = (uint32_t)min(2, g.tiles - 2 * st) * kPiece;
-        mbar_expect_tx(bar, PACK ? kPBytes + bytes : kPBytes + PL::kQCodes + (1 + qpieces) * bytes);
-        tma_2d(at, &g.pmap, st * 128, p0, bar);
-        bulk_load(at + PL::kSP, ps + (int64_t)st * 2 * kPiece, bytes, bar);
+        if (i >= early) load_p(st, slot);
         if constexpr (!PACK) {
+          const uint32_t at = sbase + slot * PL::kStage, bar = full0 + 8 * slot;
+          const uint32_t bytes = (uint32_t)min(2, g.tiles - 2 * st) * kPiece;
           tma_2d(at + PL::kQ, &g.qmap, st * 128, q0, bar);
           for (int j = 0; j < qpieces; ++j)
             bulk_load(at + PL::kQ + PL::kQCodes + j * 2 * kPiece, qs + ((int64_t)j * g.tiles + st * 2) * kPiece, bytes, bar);
@@ -644,9 +658,12 @@ int code_map(const Mx4& x, int64_t pitch, uint32_t rows, CUtensorMap* map) {
 }
 
 // Few tokens: the columns are split until two CTAs an SM have work, with at least
-// two stages each.
-int split_for(int64_t tiles, int64_t steps) {
-  const int64_t room = 2 * num_sms() / tiles, most = steps / 2;
+// two stages each of 16 or 32 tokens, four of 64, eight of 128: more sums to add
+// up cost more than they save (1111 x 1093 -> 1089, 5 stages of 128 tokens: 7.6
+// us whole and 9.3 in halves; 64 x 4096 -> 11008, 16 stages: 12.4 whole, 11.2 in
+// thirds; 16 tokens 11.5 and 9.3).
+int split_for(int64_t tiles, int64_t steps, int bn) {
+  const int64_t room = 2 * num_sms() / tiles, most = steps / (bn <= 32 ? 2 : bn / 16);
   const int64_t sk = room < most ? room : most;
   return sk < 1 ? 1 : sk > 8 ? 8 : (int)sk;
 }
@@ -657,7 +674,7 @@ struct Rows {  // tokens in 16 bits
 };
 
 template <int DT, int BN, bool PACK>
-int split_t(const Mx4& a, const Rows& x, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
+int split_t(const Mx4& a, const Rows& x, const Mx4& b, int64_t K, const void* bias, void* out, bool early, cudaStream_t st) {
   using PL = Plan<BN, PACK>;
   const int64_t pitch = mx4_pitch(K), steps = (pitch / 128 + 1) / 2;
   Args g;
@@ -677,9 +694,10 @@ int split_t(const Mx4& a, const Rows& x, const Mx4& b, int64_t K, const void* bi
   g.x = x.x;
   g.ldx = x.ld;
   g.K = (int)K;
+  g.early = early;
   g.vec = (uintptr_t)x.x % 16 == 0 && x.ld % 8 == 0 && K % 8 == 0;
   const int64_t tiles = ((b.rows + kP - 1) / kP) * ((a.rows + BN - 1) / BN);
-  const int sk = split_for(tiles, steps);
+  const int sk = split_for(tiles, steps, BN);
   const uint32_t smem = PL::kSmem + (PACK ? (uint32_t)((steps + sk - 1) / sk) * PL::kQStage : 0);
   if (smem > 226 * 1024) return RQ_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((a.rows + BN - 1) / BN), (unsigned)((b.rows + kP - 1) / kP), (unsigned)sk);
@@ -707,25 +725,27 @@ int pair_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, c
 }
 
 template <int DT>
-int matmul_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, cudaStream_t st) {
+int matmul_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, bool early, cudaStream_t st) {
   if (a.rows > 256 && ((a.rows + 255) / 256) * ((b.rows + 255) / 256) * 4 >= num_sms()) return pair_t<DT>(a, b, K, bias, out, st);
   // the narrowest tile that holds the tokens, or 128 of them
   const Rows x{nullptr, 0};
-  if (a.rows <= 16) return split_t<DT, 16, false>(a, x, b, K, bias, out, st);
-  if (a.rows <= 32) return split_t<DT, 32, false>(a, x, b, K, bias, out, st);
-  if (a.rows <= 64) return split_t<DT, 64, false>(a, x, b, K, bias, out, st);
-  return split_t<DT, 128, false>(a, x, b, K, bias, out, st);
+  if (a.rows <= 16) return split_t<DT, 16, false>(a, x, b, K, bias, out, early, st);
+  if (a.rows <= 32) return split_t<DT, 32, false>(a, x, b, K, bias, out, early, st);
+  if (a.rows <= 64) return split_t<DT, 64, false>(a, x, b, K, bias, out, early, st);
+  return split_t<DT, 128, false>(a, x, b, K, bias, out, early, st);
 }
 
 }  // namespace
 
 int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int dt, cudaStream_t st) {
-  return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, b, K, bias, out, st) : matmul_t<RQ_F16>(a, b, K, bias, out, st);
+  return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, b, K, bias, out, false, st) : matmul_t<RQ_F16>(a, b, K, bias, out, false, st);
 }
 
-// Up to 16 tokens are packed by the product's own CTAs, unless a row is so long
-// that a CTA's share does not fit its shared memory.
-constexpr int64_t kPackRows = 16, kPackColumns = 12800;  // 50 stages
+// Up to 8 tokens are packed by the product's own CTAs (4096 -> 11008: one token 9.3
+// us where the packing in a launch of its own makes 10.8, 8 tokens 11.7 and 11.2,
+// but a call takes 6.5 us of the host's time instead of 9.5), unless a row is so
+// long that a CTA's share does not fit its shared memory.
+constexpr int64_t kPackRows = 8, kPackColumns = 12800;  // 50 stages
 static bool packs(int64_t M, int64_t K) { return M <= kPackRows && K <= kPackColumns; }
 
 // Codes of x, then their scales.
@@ -740,14 +760,15 @@ int mx4_linear(const void* x, int dt, int64_t ld, int64_t M, const Mx4& w, int64
   if (packs(M, K)) {
     const Mx4 a{nullptr, nullptr, M};
     const Rows rows{x, ld};
-    return dt == RQ_BF16 ? split_t<RQ_BF16, 16, true>(a, rows, w, K, bias, out, st)
-                         : split_t<RQ_F16, 16, true>(a, rows, w, K, bias, out, st);
+    return dt == RQ_BF16 ? split_t<RQ_BF16, 16, true>(a, rows, w, K, bias, out, false, st)
+                         : split_t<RQ_F16, 16, true>(a, rows, w, K, bias, out, false, st);
   }
   uint8_t* codes = static_cast<uint8_t*>(ws);
   uint8_t* scales = codes + code_bytes(M, K);
   const int rc = mx4_pack(x, dt, ld, M, K, codes, scales, st);
   if (rc != RQ_OK) return rc;
-  return mx4_matmul(Mx4{codes, scales, M}, w, K, bias, out, dt, st);
+  const Mx4 a{codes, scales, M};
+  return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, w, K, bias, out, true, st) : matmul_t<RQ_F16>(a, w, K, bias, out, true, st);
 }
 
 }  // namespace rq
