@@ -74,6 +74,8 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
   }
 }
 
+// VEC: a lane has 8 values side by side; else every 16th, so that the lanes'
+// single values are side by side.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kM4Threads) mx4_unpack_k(const uint8_t* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales, uint32_t pieces, int K,
@@ -84,24 +86,31 @@ __global__ void __launch_bounds__(kM4Threads) mx4_unpack_k(const uint8_t* __rest
   if (p >= pieces) return;
   const int l = threadIdx.x % kM4Lanes;
   const uint32_t row = (uint32_t)(((uint64_t)p * nt.mul) >> nt.shift), tile = p - row * nt.by;
-  const float s = pow2_scale(scales[mx4_scale_at(row, (int)tile * 4 + l / 4, (int)nt.by)], 127);
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + ((int64_t)row * nt.by + tile) * 64 + l * 4);
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t h;
-    asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"((w >> (8 * i)) & 0xffu));
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    v[2 * i] = f.x * s;
-    v[2 * i + 1] = f.y * s;
-  }
-  const int col = (int)tile * 128 + l * 8;
-  T* to = static_cast<T*>(out) + (int64_t)row * K + col;
+  const uint32_t bytes = *reinterpret_cast<const uint32_t*>(scales + mx4_scale_at(row, (int)tile * 4, (int)nt.by));
+  const uint8_t* from = codes + ((int64_t)row * nt.by + tile) * 64;
+  T* to = static_cast<T*>(out) + (int64_t)row * K + (int)tile * 128;
+  const int left = K - (int)tile * 128;
   if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < K) to[i] = DType<DT>::from_f32(v[i]);
-  } else if (col < K) {
+    for (int i = 0; i < 8; ++i) {
+      const int at = i * kM4Lanes + l;
+      const float s = pow2_scale((int)(bytes >> (8 * (i / 2)) & 255u), 127);
+      const float v = e2m1_to_f32(from[at / 2] >> (4 * (at & 1))) * s;
+      if (at < left) to[at] = DType<DT>::from_f32(v);
+    }
+  } else if (l * 8 < left) {
+    const float s = pow2_scale((int)(bytes >> (8 * (l / 4)) & 255u), 127);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(from + l * 4);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h;
+      asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"((w >> (8 * i)) & 0xffu));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      v[2 * i] = f.x * s;
+      v[2 * i + 1] = f.y * s;
+    }
+    to += l * 8;
     if constexpr (DT == RQ_F32) {
       reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
       reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);

@@ -371,10 +371,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
           for (int u = 0; u < 4; ++u)
             *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = v[u];
           __syncwarp();
-#pragma unroll 4
-          for (int r = 0; r < 32; ++r) {
-            const T x = *reinterpret_cast<const T*>(stage + r * 64 + ((lane / 8 ^ (r >> 1 & 3)) << 4) + lane % 8 * 2);
-            if (m0 + r < g.M && k + lane < g.K) out[(int64_t)(m0 + r) * g.K + k + lane] = x;
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += 16) {
+            T x[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[r] = *reinterpret_cast<const T*>(stage + (r0 + r) * 64 + ((lane / 8 ^ (r >> 1 & 3)) << 4) + lane % 8 * 2);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (m0 + r0 + r < g.M && k + lane < g.K) out[(int64_t)(m0 + r0 + r) * g.K + k + lane] = x[r];
           }
           __syncwarp();
         }

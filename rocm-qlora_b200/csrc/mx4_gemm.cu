@@ -589,14 +589,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
             if (p0 + r < g.prows && q < g.qrows) *reinterpret_cast<uint4*>(out + (int64_t)(p0 + r) * g.ld + q) = v;
           }
         } else {
-#pragma unroll 4
-          for (int r = 0; r < 32; ++r)
+          // one output a lane, 8 rows' loads before their stores
+          const int q = q0 + h * 64 + lane;
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            T v[8][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int c = j * 32 + lane, q = q0 + h * 64 + c;
-              const T v = *reinterpret_cast<const T*>(stage + r * 128 + ((c / 8 ^ (r & 7)) << 4) + c % 8 * 2);
-              if (p0 + r < g.prows && q < g.qrows) out[(int64_t)(p0 + r) * g.ld + q] = v;
-            }
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                v[r][j] = *reinterpret_cast<const T*>(stage + (r0 + r) * 128 + ((j * 4 + lane / 8 ^ r) << 4) + lane % 8 * 2);
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (p0 + r0 + r < g.prows && q + 32 * j < g.qrows) out[(int64_t)(p0 + r0 + r) * g.ld + q + 32 * j] = v[r][j];
+          }
         }
         __syncwarp();  // the staged rows are read before the next ones are written
       }
