@@ -460,6 +460,11 @@ RQ_API int rq_mx4_dx(const void* dy, int dtype, int64_t ld_dy, int64_t M,
               const uint8_t* w_codes, const uint8_t* w_scales, int64_t N, int64_t K,
               void* dx, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Copies rows x [M, N] of 16-bit values (row stride ld_x, any alignment) to rows
+ * of stride ld_out, a multiple of 8 of at least N, out 16-byte aligned: what
+ * rq_mx4_dx takes.  Columns past N are left as they are or 0. */
+RQ_API int rq_align_rows(const void* x, int64_t ld_x, int64_t M, int64_t N, void* out, int64_t ld_out, void* stream);
+
 /* ---------------------------------------------- AdamW over many tensors */
 
 /* One tensor of a step: its values, its gradient (both of the call's dtype),

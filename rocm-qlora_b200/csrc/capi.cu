@@ -585,6 +585,16 @@ int rq_mx4_dx(const void* dy, int dtype, int64_t ld_dy, int64_t M, const uint8_t
   return mx4_dx(dy, dtype, ld_dy, M, Mx4{w_codes, w_scales, N}, K, dx, workspace, (cudaStream_t)stream);
 }
 
+int rq_align_rows(const void* x, int64_t ld_x, int64_t M, int64_t N, void* out, int64_t ld_out, void* stream) {
+  RQ_PROLOGUE();
+  if (!fits(M) || !fits(N) || !fits(M * (N / 1024 + 1)) || !row_stride(M, ld_x, N) || ld_out < N || ld_out % 8)
+    return RQ_ERR_INVALID;
+  if (M * N == 0) return RQ_OK;
+  if (!x || !out) return RQ_ERR_INVALID;
+  if ((uintptr_t)x % 2 || (uintptr_t)out % 16) return RQ_ERR_ALIGN;
+  return align_rows(x, ld_x, M, N, out, ld_out, (cudaStream_t)stream);
+}
+
 int rq_grad_norm_partial(const RqAdamTensor* tensors, int count, int dtype, double* partials, void* stream) {
   RQ_PROLOGUE();
   const int rc = check_tensors(tensors, count, dtype, false, false);

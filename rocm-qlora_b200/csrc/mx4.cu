@@ -148,4 +148,42 @@ int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K
   return launch_dependent(k, (pieces + kM4PerCta - 1) / kM4PerCta, kM4Threads, st, codes, scales, pieces, (int)K, nt, out);
 }
 
+// Rows of 16-bit values to rows that begin at 16 bytes: a thread writes 8 values.
+// Inside a row it reads the two aligned 16-byte pieces that hold them and shifts
+// (by as much for the whole row); at its ends value by value, so that nothing
+// outside the row is read.
+__global__ void __launch_bounds__(128) align_rows_k(const uint16_t* __restrict__ x, int64_t ld, int N, uint32_t per,
+                                                    uint16_t* __restrict__ out, int64_t ldo) {
+  grid_begin();
+  const uint32_t m = blockIdx.x / per;
+  const int c = (int)((blockIdx.x - m * per) * 128 + threadIdx.x) * 8;
+  if (c >= N) return;
+  const uint16_t* from = x + (int64_t)m * ld + c;
+  const uint32_t off = (uint32_t)((uintptr_t)from & 15);
+  uint32_t w[4];
+  if (c >= 8 && c + 16 <= N) {
+    const uint4* p = reinterpret_cast<const uint4*>((uintptr_t)from & ~(uintptr_t)15);
+    const uint4 a = __ldg(p), b = off ? __ldg(p + 1) : a;
+    const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const uint32_t k = off / 4, bits = off % 4 * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = k == 0 ? v[i] : k == 1 ? v[i + 1] : k == 2 ? v[i + 2] : v[i + 3];
+      const uint32_t hi = k == 0 ? v[i + 1] : k == 1 ? v[i + 2] : k == 2 ? v[i + 3] : v[i + 4 < 8 ? i + 4 : 7];
+      w[i] = __funnelshift_r(lo, hi, bits);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (c + 2 * i < N ? from[2 * i] : 0u) | (c + 2 * i + 1 < N ? from[2 * i + 1] : 0u) << 16;
+  }
+  *reinterpret_cast<uint4*>(out + (int64_t)m * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+int align_rows(const void* x, int64_t ld, int64_t M, int64_t N, void* out, int64_t ldo, cudaStream_t st) {
+  const uint32_t per = (uint32_t)((N + 1023) / 1024);
+  return launch_dependent(align_rows_k, (unsigned)(M * per), 128, st, static_cast<const uint16_t*>(x), ld, (int)N, per,
+                          static_cast<uint16_t*>(out), ldo);
+}
+
 }  // namespace rq

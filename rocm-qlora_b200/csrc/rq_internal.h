@@ -181,6 +181,8 @@ int mx4_linear(const void* x, int dt, int64_t ld, int64_t M, const Mx4& w, int64
                void* ws, cudaStream_t st);
 int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, void* dx, void* ws, cudaStream_t st);
 
+int align_rows(const void* x, int64_t ld, int64_t M, int64_t N, void* out, int64_t ldo, cudaStream_t st);
+
 // AdamW over many tensors (adamw.cu).
 int grad_norm_partial(const RqAdamTensor* list, int count, int dt, double* partials, cudaStream_t st);
 int grad_norm_end(const double* partials, int n, float* norm, cudaStream_t st);

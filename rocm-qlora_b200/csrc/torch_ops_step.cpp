@@ -109,7 +109,7 @@ Tensor mx4_dx(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64
   Tensor d = dy;
   if (d.stride(0) % 8 || d.stride(0) < N || (uintptr_t)d.data_ptr() % 16) {  // rows as the tensor maps take them
     d = at::empty({M, (N + 7) / 8 * 8}, dy.options()).narrow(1, 0, N);
-    d.copy_(dy);
+    check(rq_align_rows(dy.data_ptr(), dy.stride(0), M, N, d.data_ptr(), d.stride(0), stream_of(dy)), "rq_align_rows");
   }
   const Tensor c = aligned(codes), s = aligned(scales);
   Tensor ws;
