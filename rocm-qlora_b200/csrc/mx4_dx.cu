@@ -305,14 +305,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         s0 = s1;
         s1 = s2;
         s2 = scale(st + 3 * TM);
+        // The stage before in this slot was another team's: a test for its round's
+        // parity alone could take the round before that for this one.
+        if (TM > 1 && round > 0) ok = wait_warp(read0 + 8 * slot, (round - 1) & 1, ab, lane);
+        if (!ok) break;
         ok = wait_warp(codes0 + 8 * slot, round & 1, ab, lane);
         if (!ok) break;
         unsigned char* at = sm + slot * PL::kStage;
         uint4 cw[U / 4];
 #pragma unroll
         for (int h = 0; h < U / 4; ++h) cw[h] = *reinterpret_cast<const uint4*>(at + load + (((piece + h) ^ swz) << 4));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(read0 + 8 * slot);
         if (round > 0) ok = wait_warp(empty0 + 8 * slot, (round - 1) & 1, ab, lane);
         if (!ok) break;
 #pragma unroll
@@ -325,7 +327,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
         __syncwarp();
-        if (lane == 0) arrive_leader(wide + 8 * slot);
+        if (lane == 0) {
+          arrive_leader(wide + 8 * slot);
+          // Only now: the values have been used, so the loads of the codes are over.
+          // Said right after them, the next TMA copy overtook loads still in the
+          // queue (an arrival waits for neither those nor for the other proxy).
+          mbar_arrive(read0 + 8 * slot);
+        }
         slot += TM;
         if (slot >= S) slot -= S, ++round;
       }

@@ -7,7 +7,7 @@ batch, shared by all layers), and ``adapters_add`` computes
     y[m] = base[m] + scaling[a] * (x[m] @ A[a]) @ B[a].T,    a = ids[m]
 
 for all rows at once, in one launch, with its gradients (csrc/adapters.cu).
-``MultiLoRALinear`` is the layer: a QuantLinear and its bank.
+``MultiLoRALinear`` is the layer: a QuantLinear or Mx4Linear and its bank.
 """
 from typing import Optional, Sequence
 
@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from rocm_qlora import _native as nat
 from rocm_qlora.activation8.packed import BLOCK, PackedActivation, rows_of
+from rocm_qlora.mx4.linear import Mx4Linear
 from rocm_qlora.quantization import layer_ops
 
 MAX_RANK = 128
@@ -243,7 +244,8 @@ class AdapterBank(nn.Module):
 
 
 class MultiLoRALinear(nn.Module):
-    """A frozen QuantLinear shared by the rows of all requests, and its bank."""
+    """A frozen QuantLinear (or Mx4Linear) shared by the rows of all requests,
+    and its bank."""
 
     def __init__(self, quant_linear: nn.Module, bank: AdapterBank):
         super().__init__()
@@ -257,7 +259,7 @@ class MultiLoRALinear(nn.Module):
     def forward(self, x: torch.Tensor, plan: Optional[AdapterPlan] = None,
                 packed_x: Optional[PackedActivation] = None) -> torch.Tensor:
         b = self.base_layer
-        if b.merged_mode and b.merged_fp16_weight is not None:
+        if isinstance(b, Mx4Linear) or (b.merged_mode and b.merged_fp16_weight is not None):
             return self.bank(b(x), x, plan, packed_x)
         return bank_linear(x, b.weight_view(), b.bias, self.bank.lora_A, self.bank.lora_B, self.bank.scaling, plan,
                            packed_x)

@@ -169,6 +169,30 @@ def test_product_and_its_gradient(rows, k, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,k,n", [(4096, 4096, 4096), (2047, 11008, 4096), (300, 4096, 11008), (4096, 1024, 8200)])
+def test_long_runs_of_tiles_and_stages(rows, k, n, dtype):
+    """Many tiles a CTA and many rounds of its rings, several times over: every
+    call gives the same values, near the product in 32 bits (whose own sums are
+    off by less than 2^-20 of the terms' root sum of squares)."""
+    from rocm_qlora import _native as nat
+    from rocm_qlora.mx4 import mx4_matmul, pack_mx4, unpack_mx4
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    w = pack_mx4((torch.randn(n, k, generator=g, device="cuda") * 0.02).to(dtype))
+    x = pack_mx4(torch.randn(rows, k, generator=g, device="cuda").to(dtype))
+    dy = torch.randn(rows, n, generator=g, device="cuda").to(dtype)
+    wide = unpack_mx4(w, torch.float32)
+    for f, a, b in ((lambda: mx4_matmul(x, w, dtype=dtype), unpack_mx4(x, torch.float32), wide.t()),
+                    (lambda: nat.loaded_ops().mx4_dx(dy, w.codes, w.scales, k), dy.float(), wide)):
+        want = a @ b
+        bound = HALF[dtype] * want.abs() + 2.0 ** -16 * (a.square() @ b.square()).sqrt() + TINY[dtype]
+        first = f()
+        assert bool(((first.float() - want).abs() <= bound).all())
+        for _ in range(6):
+            assert torch.equal(f(), first)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """On inputs that the 4-bit form holds exactly the product is linear in x."""
     from rocm_qlora.mx4 import mx4_linear, pack_mx4
@@ -369,3 +393,39 @@ def test_differentiable_once_and_no_forward_derivatives():
     import torch.autograd.forward_ad as fw
     with fw.dual_level(), pytest.raises(Exception):
         operators().mx4_linear(fw.make_dual(x.detach(), torch.empty_like(x)), *meta(72), 160, None)
+
+
+def traced(device, grad):
+    from rocm_qlora.mx4 import mx4_linear, mx4_matmul, pack_mx4, unpack_mx4
+    x = torch.empty(2, 3, 200, device=device, dtype=BF, requires_grad=grad)
+    packed = pack_mx4(torch.empty(72, 200, device=device, dtype=BF))
+    y = mx4_linear(x, packed)
+    found = [(y, (2, 3, 72), BF), (mx4_matmul(pack_mx4(x), packed, dtype=HF), (2, 3, 72), HF),
+             (unpack_mx4(packed), (72, 200), BF), (packed.codes, (72, 128), torch.uint8)]
+    if grad:
+        found.append((torch.autograd.grad(y.float().sum(), x)[0], (2, 3, 200), BF))
+    return found
+
+
+# without a GPU autograd itself has no streams for fake CUDA tensors
+@pytest.mark.parametrize("grad,device", [(False, "cuda"), (True, "meta"),
+                                         pytest.param(True, "cuda", marks=pytest.mark.gpu)])
+def test_fake_tensors(grad, device):
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=False):
+        for value, shape, dtype in traced(device, grad):
+            assert isinstance(value, FakeTensor) and value.shape == tuple(shape) and value.dtype == dtype
+            assert value.device.type == device
+
+
+@pytest.mark.gpu
+def test_traced_graph_runs():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from rocm_qlora.mx4 import mx4_linear, pack_mx4, unpack_mx4
+    packed = pack_mx4(torch.randn(72, 200, device="cuda", dtype=BF))
+    f = lambda x: unpack_mx4(pack_mx4(mx4_linear(x, packed)))  # noqa: E731
+    x = torch.randn(20, 200, device="cuda", dtype=BF)
+    graph = make_fx(f)(x)
+    names = {str(n.target) for n in graph.graph.nodes if n.op == "call_function"}
+    assert any("rocm_qlora.mx4_forward" in n for n in names), names
+    assert torch.equal(graph(x), f(x))
