@@ -305,9 +305,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         s0 = s1;
         s1 = s2;
         s2 = scale(st + 3 * TM);
-        // The stage before in this slot was another team's: a test for its round's
-        // parity alone could take the round before that for this one.
-        if (TM > 1 && round > 0) ok = wait_warp(read0 + 8 * slot, (round - 1) & 1, ab, lane);
+        // In this order: the stage before in this slot may have been another team's,
+        // and a test of the codes' parity could take the round before that for this
+        // one while its codes are still on their way.  Its MMAs are over, so they
+        // are not.
+        if (round > 0) ok = wait_warp(empty0 + 8 * slot, (round - 1) & 1, ab, lane);
         if (!ok) break;
         ok = wait_warp(codes0 + 8 * slot, round & 1, ab, lane);
         if (!ok) break;
@@ -315,8 +317,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         uint4 cw[U / 4];
 #pragma unroll
         for (int h = 0; h < U / 4; ++h) cw[h] = *reinterpret_cast<const uint4*>(at + load + (((piece + h) ^ swz) << 4));
-        if (round > 0) ok = wait_warp(empty0 + 8 * slot, (round - 1) & 1, ab, lane);
-        if (!ok) break;
 #pragma unroll
         for (int h = 0; h < U / 4; ++h) {  // 32 columns, one scale
           const uint32_t word[4] = {cw[h].x, cw[h].y, cw[h].z, cw[h].w};
