@@ -74,12 +74,60 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
   }
 }
 
-// VEC: a lane has 8 values side by side; else every 16th, so that the lanes'
-// single values are side by side.
-template <int DT, bool VEC>
+// As packing: 16 lanes take four rows of a piece, 8 values a lane.
+template <int DT>
 __global__ void __launch_bounds__(kM4Threads) mx4_unpack_k(const uint8_t* __restrict__ codes,
-                                                           const uint8_t* __restrict__ scales, uint32_t pieces, int K,
-                                                           M4Divide nt, void* __restrict__ out) {
+                                                           const uint8_t* __restrict__ scales, int64_t M, int K,
+                                                           uint32_t warps, M4Divide np, int tiles,
+                                                           void* __restrict__ out) {
+  grid_begin();
+  using T = typename DType<DT>::T;
+  const uint32_t p = blockIdx.x * (kM4Threads / 32) + threadIdx.x / 32;
+  const uint32_t q = (uint32_t)(((uint64_t)p * np.mul) >> np.shift);
+  const int l = threadIdx.x % kM4Lanes, tile = (int)(p - q * np.by) * 2 + threadIdx.x / kM4Lanes % 2;
+  const int64_t row0 = (int64_t)(q / 32) * 128 + q % 32;
+  const int col = tile * 128 + l * 8;
+  if (p >= warps || col >= K) return;
+  // byte l / 4 of word j: row j's scale of this lane's block
+  const uint4 s4 = *reinterpret_cast<const uint4*>(scales + ((row0 / 128) * tiles + tile) * 512 + row0 % 32 * 16);
+  const uint32_t s[4] = {s4.x, s4.y, s4.z, s4.w};
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = row0 + 32 * j;
+    w[j] = row < M ? *reinterpret_cast<const uint32_t*>(codes + (row * tiles + tile) * 64 + l * 4) : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = row0 + 32 * j;
+    if (row >= M) break;
+    const float f = pow2_scale((int)(s[j] >> (8 * (l / 4)) & 255u), 127);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h;
+      asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"((w[j] >> (8 * i)) & 0xffu));
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      v[2 * i] = x.x * f;
+      v[2 * i + 1] = x.y * f;
+    }
+    T* to = static_cast<T*>(out) + row * K + col;
+    if constexpr (DT == RQ_F32) {
+      reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
+      reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
+    } else {
+      *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
+                                                 pack2<DT>(v[6], v[7]));
+    }
+  }
+}
+
+// Rows that are not 16-byte aligned: a lane has every 16th value of a piece, so
+// that the lanes' single values are side by side.
+template <int DT>
+__global__ void __launch_bounds__(kM4Threads) mx4_unpack_odd_k(const uint8_t* __restrict__ codes,
+                                                               const uint8_t* __restrict__ scales, uint32_t pieces,
+                                                               int K, M4Divide nt, void* __restrict__ out) {
   grid_begin();
   using T = typename DType<DT>::T;
   const uint32_t p = blockIdx.x * kM4PerCta + threadIdx.x / kM4Lanes;
@@ -90,34 +138,12 @@ __global__ void __launch_bounds__(kM4Threads) mx4_unpack_k(const uint8_t* __rest
   const uint8_t* from = codes + ((int64_t)row * nt.by + tile) * 64;
   T* to = static_cast<T*>(out) + (int64_t)row * K + (int)tile * 128;
   const int left = K - (int)tile * 128;
-  if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = i * kM4Lanes + l;
-      const float s = pow2_scale((int)(bytes >> (8 * (i / 2)) & 255u), 127);
-      const float v = e2m1_to_f32(from[at / 2] >> (4 * (at & 1))) * s;
-      if (at < left) to[at] = DType<DT>::from_f32(v);
-    }
-  } else if (l * 8 < left) {
-    const float s = pow2_scale((int)(bytes >> (8 * (l / 4)) & 255u), 127);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(from + l * 4);
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t h;
-      asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"((w >> (8 * i)) & 0xffu));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
-    }
-    to += l * 8;
-    if constexpr (DT == RQ_F32) {
-      reinterpret_cast<float4*>(to)[0] = *reinterpret_cast<const float4*>(v);
-      reinterpret_cast<float4*>(to)[1] = *reinterpret_cast<const float4*>(v + 4);
-    } else {
-      *reinterpret_cast<uint4*>(to) = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]),
-                                                 pack2<DT>(v[6], v[7]));
-    }
+  for (int i = 0; i < 8; ++i) {
+    const int at = i * kM4Lanes + l;
+    const float s = pow2_scale((int)(bytes >> (8 * (i / 2)) & 255u), 127);
+    const float v = e2m1_to_f32(from[at / 2] >> (4 * (at & 1))) * s;
+    if (at < left) to[at] = DType<DT>::from_f32(v);
   }
 }
 
@@ -139,12 +165,19 @@ int mx4_pack(const void* x, int dt, int64_t ld, int64_t M, int64_t K, uint8_t* c
 }
 
 int mx4_unpack(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, void* out, int dt, cudaStream_t st) {
-  const M4Divide nt = m4_divide((uint32_t)(mx4_pitch(K) / 128));
+  const int tiles = (int)(mx4_pitch(K) / 128);
+  if (m4_rows(out, K, K, dt)) {
+    const M4Divide np = m4_divide((uint32_t)(tiles + 1) / 2);
+    const uint32_t warps = (uint32_t)((M + 127) / 128 * 32) * np.by;
+    auto* k = dt == RQ_F32 ? mx4_unpack_k<RQ_F32> : dt == RQ_BF16 ? mx4_unpack_k<RQ_BF16> : mx4_unpack_k<RQ_F16>;
+    return launch_dependent(k, (warps + kM4Threads / 32 - 1) / (kM4Threads / 32), kM4Threads, st, codes, scales, M, (int)K,
+                            warps, np, tiles, out);
+  }
+  const M4Divide nt = m4_divide((uint32_t)tiles);
   const uint32_t pieces = (uint32_t)M * nt.by;
-  const bool vec = m4_rows(out, K, K, dt);
-  auto* k = dt == RQ_F32 ? (vec ? mx4_unpack_k<RQ_F32, true> : mx4_unpack_k<RQ_F32, false>)
-            : dt == RQ_BF16 ? (vec ? mx4_unpack_k<RQ_BF16, true> : mx4_unpack_k<RQ_BF16, false>)
-                            : (vec ? mx4_unpack_k<RQ_F16, true> : mx4_unpack_k<RQ_F16, false>);
+  auto* k = dt == RQ_F32    ? mx4_unpack_odd_k<RQ_F32>
+            : dt == RQ_BF16 ? mx4_unpack_odd_k<RQ_BF16>
+                            : mx4_unpack_odd_k<RQ_F16>;
   return launch_dependent(k, (pieces + kM4PerCta - 1) / kM4PerCta, kM4Threads, st, codes, scales, pieces, (int)K, nt, out);
 }
 

@@ -58,9 +58,9 @@ template <int DT, int BN>
 struct Plan {
   // Teams of 8 widening warps that take the stages in turn.  Two hide the waits
   // and fences between stages, but take issue slots and shared memory from each
-  // other: 8192 x 11008 -> 4096 in bf16 613 us with one and 583 with two, 2047 x
-  // 4096 -> 11008 in fp16 (whose multiplications are shorter) 145 and 162, 512 x
-  // 4096 -> 4096 (128 columns) 27 and 30.
+  // other: 8192 x 11008 -> 4096 in bf16 630 us with one and 600 with two, 4096 x
+  // 4096 -> 4096 135 and 116; 2047 x 4096 -> 11008 in fp16 (whose widening is
+  // shorter) 147 and 155, 512 x 4096 -> 4096 (128 columns) 26 and 29.
   static constexpr int kTeams = DT == RQ_BF16 && BN == 256 ? 2 : 1;
   static constexpr int kEpi0 = 2 + kTeams * kWiden;      // first epilogue warp
   static constexpr int kThreads = 32 * (kEpi0 + kEpi);
