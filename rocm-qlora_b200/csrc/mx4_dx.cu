@@ -186,7 +186,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
                  empty0 = wide0 + 8 * S, acc0 = empty0 + 8 * S, taken0 = acc0 + 16, drainbar = taken0 + 16;
   const PairAbort ab{&abort_flag, mapa(smem_u32(&abort_flag), rank ^ 1u), &g_mx4_dx_timeouts};
   const int steps = (g.N + kRows - 1) / kRows;
-  const int mt = (g.M + 255) / 256, ntile = mt * ((g.K + BN - 1) / BN);
+  // tiles of the same tokens follow one another: dy, the larger operand, is read
+  // from HBM once
+  const int ct = (g.K + BN - 1) / BN, ntile = (g.M + 255) / 256 * ct;
   const int first = blockIdx.x / 2, stride = gridDim.x / 2;
   const int tiles = first < ntile ? (ntile - 1 - first) / stride + 1 : 0, total = tiles * steps;
 
@@ -229,7 +231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
       auto load_codes = [&](int i) {
         const int t = first + i / steps * stride, slot = i % S;
         mbar_expect_tx(codes0 + 8 * slot, PL::kCodes);
-        tma_2d(sbase + slot * PL::kStage + PL::kC, &g.cmap, (t / mt * BN + (int)rank * PL::BNH) / 2, i % steps * kRows,
+        tma_2d(sbase + slot * PL::kStage + PL::kC, &g.cmap, (t % ct * BN + (int)rank * PL::BNH) / 2, i % steps * kRows,
                codes0 + 8 * slot);
       };
       for (; ahead < S && ahead < total; ++ahead) load_codes(ahead);
@@ -238,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         if (i >= S) ok = wait_pair(empty0 + 8 * slot, ((i / S) - 1) & 1, ab);
         if (!ok) break;
         const uint32_t at = sbase + slot * PL::kStage;
-        const int m0 = t % mt * 256 + (int)rank * 128;
+        const int m0 = t / ct * 256 + (int)rank * 128;
         if (rank == 0) mbar_expect_tx(dy0 + 8 * slot, 4 * kA);
         tma_pair(at, &g.amap, st * kRows, m0, lead + 8 * slot);
         tma_pair(at + kA, &g.amap, st * kRows + 64, m0, lead + 8 * slot);
@@ -287,7 +289,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     int i = (warp - 2) / kWiden;  // the team's next stage, of all
     bool ok = true;
     for (int n = 0; n < tiles && ok; ++n) {
-      const int c = (first + n * stride) / mt * BN + (int)rank * PL::BNH + col;
+      const int c = (first + n * stride) % ct * BN + (int)rank * PL::BNH + col;
       const bool any = c < g.pieces * 128;
       const uint8_t* p = g.scales + (int64_t)(c / 128) * 512 + (row % 32) * 16 + row / 32 * 4 + c % 128 / 32;
       auto scale = [&](int st) -> uint32_t {  // the scale bytes of this thread's columns
@@ -346,7 +348,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     const float back = DT == RQ_F16 ? pow2_scale(top_of(g.tops, lane), 127) : 1.0f;
     const bool rows16 = (uintptr_t)out % 16 == 0 && g.K % 8 == 0;
     for (int n = 0; n < tiles; ++n) {
-      const int t = first + n * stride, m0 = t % mt * 256 + (int)rank * 128 + quad * 32, c0 = t / mt * BN;
+      const int t = first + n * stride, m0 = t / ct * 256 + (int)rank * 128 + quad * 32, c0 = t % ct * BN;
       bool ok = true;
       if (lane == 0) ok = wait_pair(acc0 + 8 * (n & 1), (n >> 1) & 1, ab) && !ab.raised();
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
