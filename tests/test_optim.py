@@ -380,6 +380,46 @@ def test_refused_parameters():
         opt.step()
 
 
+@pytest.mark.gpu
+def test_hooks_schedulers_and_profiler_ranges():
+    from rocm_qlora.optim import AdamW
+    (p,) = made([(300,)], F4, seed=10)
+    opt = AdamW([p], lr=1, weight_decay=0)
+    called = []
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda t: 0.5 ** t)
+    opt.step()
+    schedule.step()
+    assert opt.param_groups[0]["lr"] == 0.5
+    before = opt.register_step_pre_hook(lambda *a: called.append("before"))
+    after = opt.register_step_post_hook(lambda *a: called.append("after"))
+    opt.step()
+    before.remove(), after.remove()
+    opt.step()
+    assert called == ["before", "after"] and int(opt.state[p]["step"]) == 3
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as seen:
+        opt.step()
+    assert any(e.key.startswith("Optimizer.step#AdamW") for e in seen.key_averages())
+    with pytest.raises(TypeError, match="state_dict"):
+        import copy
+        copy.deepcopy(opt)
+
+
+@pytest.mark.gpu
+def test_half_precision_with_a_gradient_scaler():
+    """GradScaler skips a step whose gradients overflow and takes the others."""
+    from rocm_qlora.optim import AdamW
+    (p,) = made([(600,)], F4, seed=11)
+    opt = AdamW([p], lr=1e-2, state_bits=8, max_grad_norm=1.0)
+    scaler = torch.amp.GradScaler("cuda", init_scale=4.0)
+    start = p.detach().clone()
+    for scale, steps in ((float("inf"), 0), (4.0, 1)):
+        scaler.scale(torch.zeros((), device="cuda", requires_grad=True))  # the scale's own lazy start
+        p.grad = torch.ones_like(p) * scale
+        scaler.step(opt)
+        scaler.update()
+        assert int(opt.state[p]["step"]) == steps and bool((p == start).all()) == (steps == 0)
+
+
 # ------------------------------------------------------------- refused, CPU
 
 def test_refused_numbers():
