@@ -41,24 +41,23 @@ __global__ void __launch_bounds__(kM4Threads) mx4_pack_k(const void* __restrict_
   const bool in = p < warps && tile < tiles;
   const int64_t row0 = (int64_t)(q / 32) * 128 + q % 32;
   const int col = tile * 128 + l * 8;
-  float v[4][8];
+  M4Raw<DT> r[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int64_t row = row0 + 32 * j;
     const bool any = in && row < M;
-    m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), col, any ? K : 0, v[j]);
+    r[j] = m4_load<DT, VEC>(static_cast<const T*>(x) + (any ? row * ld : 0), col, any ? K : 0);
   }
+  uint32_t top[4];
+  m4_top<DT, 4>(r, top);
   uint32_t bytes = 0;  // row j's scale of this lane's block in byte j
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[j][i]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t byte = m4_scale(m);
+    const uint32_t byte = m4_scale(top[j]);
     bytes |= byte << (8 * j);
-    const uint32_t w = e2m1x8(v[j], m4_factor(byte));
+    float v[8];
+    m4_values<DT>(r[j], v);
+    const uint32_t w = e2m1x8(v, m4_factor(byte));
     const int64_t row = row0 + 32 * j;
     if (in && row < M) *reinterpret_cast<uint32_t*>(codes + (row * tiles + tile) * 64 + l * 4) = w;
   }

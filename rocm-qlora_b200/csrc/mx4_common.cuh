@@ -27,29 +27,81 @@ __device__ __forceinline__ int64_t mx4_scale_at(int64_t r, int b, int tiles) {
   return ((r / 128) * tiles + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4;
 }
 
-// A lane's 8 values at columns col .. col + 7, 0 past K.  VEC: whole 16-byte
-// pieces, so all 8 exist or none does.
+// A lane's 8 values as they are in memory (16-bit types packed in 4 words), at
+// columns col .. col + 7, 0 past K.  VEC: whole 16-byte pieces, so all 8 exist or
+// none does.
+template <int DT> struct M4Raw { uint32_t w[DT == RQ_F32 ? 8 : 4]; };
+
 template <int DT, bool VEC>
-__device__ __forceinline__ void m4_load(const typename DType<DT>::T* row, int col, int K, float (&v)[8]) {
-  if constexpr (!VEC) {
+__device__ __forceinline__ M4Raw<DT> m4_load(const typename DType<DT>::T* row, int col, int K) {
+  M4Raw<DT> r = {};
+  if constexpr (VEC) {
+    if (col < K) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < K ? DType<DT>::to_f32(row[col + i]) : 0.0f;
-  } else if constexpr (DT == RQ_F32) {
-    const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    *reinterpret_cast<float4*>(v) = col < K ? *reinterpret_cast<const float4*>(row + col) : z;
-    *reinterpret_cast<float4*>(v + 4) = col < K ? *reinterpret_cast<const float4*>(row + col + 4) : z;
+      for (int h = 0; h < (DT == RQ_F32 ? 2 : 1); ++h)
+        *reinterpret_cast<uint4*>(r.w + 4 * h) = *reinterpret_cast<const uint4*>(row + col + 4 * h);
+    }
   } else {
-    const uint4 w = col < K ? *reinterpret_cast<const uint4*>(row + col) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == RQ_BF16) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (DT == RQ_F32) {
+        r.w[i] = col + i < K ? __float_as_uint(row[col + i]) : 0u;
       } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        const uint32_t v = col + i < K ? reinterpret_cast<const uint16_t*>(row)[col + i] : 0u;
+        r.w[i / 2] |= v << (16 * (i & 1));
+      }
+    }
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void m4_values(const M4Raw<DT>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < (DT == RQ_F32 ? 8 : 4); ++i) {
+    if constexpr (DT == RQ_F32) {
+      v[i] = __uint_as_float(r.w[i]);
+    } else if constexpr (DT == RQ_BF16) {
+      v[2 * i] = __uint_as_float(r.w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// Largest magnitudes of blocks of which each of 4 neighbouring lanes has 8 values,
+// as fp32 bits, in which an infinity or NaN is the largest.  16-bit magnitudes are
+// compared two at a time, and two blocks share a word on their way.
+template <int DT, int N>
+__device__ __forceinline__ void m4_top(const M4Raw<DT> (&r)[N], uint32_t (&top)[N]) {
+  if constexpr (DT == RQ_F32) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, r[n].w[i] & 0x7fffffffu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      top[n] = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    }
+  } else {
+    uint32_t m[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      m[n] = __vmaxs2(__vmaxs2(r[n].w[0] & 0x7fff7fffu, r[n].w[1] & 0x7fff7fffu),
+                      __vmaxs2(r[n].w[2] & 0x7fff7fffu, r[n].w[3] & 0x7fff7fffu));
+#pragma unroll
+    for (int n = 0; n < N; n += 2) {
+      const uint32_t other = n + 1 < N ? m[n + 1 < N ? n + 1 : n] : 0u;
+      uint32_t both = __vmaxs2(__byte_perm(m[n], other, 0x5410), __byte_perm(m[n], other, 0x7632));
+      both = __vmaxs2(both, __shfl_xor_sync(0xffffffffu, both, 1));
+      both = __vmaxs2(both, __shfl_xor_sync(0xffffffffu, both, 2));
+#pragma unroll
+      for (int h = 0; h < 2 && n + h < N; ++h) {
+        const uint16_t bits = (uint16_t)(h ? both >> 16 : both);
+        top[n + h] = __float_as_uint(DType<DT>::to_f32(*reinterpret_cast<const typename DType<DT>::T*>(&bits)));
       }
     }
   }

@@ -256,15 +256,12 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
       unsigned char* q = sm + PL::kRing + i * PL::kQStage;
       const T* row = x + (int64_t)(q0 + r) * g.ldx;
       const int col = (s0 + i) * 256 + lane * 8;
+      const M4Raw<DT> raw[1] = {g.vec ? m4_load<DT, true>(row, col, g.K) : m4_load<DT, false>(row, col, g.K)};
+      uint32_t top[1];
+      m4_top<DT, 1>(raw, top);
+      const uint32_t byte = m4_scale(top[0]);
       float v[8];
-      if (g.vec) m4_load<DT, true>(row, col, g.K, v);
-      else m4_load<DT, false>(row, col, g.K, v);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t byte = m4_scale(top);
+      m4_values<DT>(raw[0], v);
       *reinterpret_cast<uint32_t*>(q + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + lane % 4 * 4) = e2m1x8(v, m4_factor(byte));
       uint32_t word = byte << (lane % 16 / 4 * 8);
       word |= __shfl_xor_sync(0xffffffffu, word, 4);
