@@ -262,13 +262,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // The root's code of a value t in [0, kRTop], in the low byte: a float of 4
 // exponent and 4 mantissa bits, whose first 16 codes are the numbers 0 to 15.
-// Ties to even, by integer rounding of the mantissa or, below 16, by adding
-// 1.5 2^23.
+// Adding 1.5 2^(23 + e) rounds t to q 2^e, ties to even, with e = 0 below 32 and
+// 16 <= q <= 32 from there; the code is q + 16 e, and the sum holds q in its low
+// bits and e in its exponent.
 __device__ __forceinline__ uint32_t root_code(float t) {
-  const uint32_t bits = __float_as_uint(t);
-  const uint32_t high = (bits + ((bits >> 19) & 1u) + (0x3ffffu - (130u << 23))) >> 19;
-  const uint32_t low = __float_as_uint(__fadd_rn(t, 12582912.0f));
-  return t < 16.0f ? low : high;
+  const uint32_t e = max(__float_as_uint(t) & 0x7f800000u, 131u << 23);  // 2^(4 + e)
+  const uint32_t sum = __float_as_uint(__fadd_rn(t, __uint_as_float(e + (19u << 23 | 0x400000u))));
+  return sum + (sum >> 19) - ((150u << 4) + 8u);
 }
 // The value of byte i of w.  A code's bits above exponent 130 are v = (16 + M)
 // 2^(E - 1) from 16 on and v = 8 + c / 2 below, where the value is 2 v - 16:
