@@ -325,6 +325,10 @@ struct AdamW : torch::CustomClassHolder {
     const Tensor& first = groups[0].m;
     std::vector<Lists> lists;
     int64_t launches = 0;
+    // all is checked before the first launch: a refused step changes nothing
+    for (const optional<Tensor>& lr : lrs)
+      TORCH_CHECK_VALUE(!lr || (lr->numel() == 1 && lr->scalar_type() == at::kFloat && lr->device() == first.device()),
+                        "a learning rate that is a tensor must be one float32 on the parameters' device");
     for (const AdamGroup& g : groups) {
       one_device(first, g.m);
       lists.push_back(gather(g));
@@ -349,9 +353,6 @@ struct AdamW : torch::CustomClassHolder {
     for (size_t i = 0; i < groups.size(); ++i) {
       const AdamGroup& g = groups[i];
       const double* h = hyper.data() + 5 * i;
-      if (lrs[i])
-        TORCH_CHECK_VALUE(lrs[i]->numel() == 1 && lrs[i]->scalar_type() == at::kFloat && lrs[i]->device() == first.device(),
-                          "a learning rate that is a tensor must be one float32 on the parameters' device");
       RqAdamStep step = {};
       step.lr = h[0];
       step.beta1 = h[1];

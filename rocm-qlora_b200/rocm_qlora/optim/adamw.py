@@ -83,6 +83,11 @@ class AdamW(torch.optim.Optimizer):
         device = self.param_groups[0]["params"][0].device
         if len(params) > 65536:
             raise ValueError(f"a parameter group holds at most 65536 tensors, got {len(params)}")
+        # one launch updates them side by side
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for p in params if p.numel() and p.is_contiguous() and not p.is_meta)
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("a parameter group holds a parameter twice, or two that share memory")
         for p in params:
             if not p.is_cuda:
                 raise nat.NativeUnavailable(
@@ -124,8 +129,6 @@ class AdamW(torch.optim.Optimizer):
         held = torch.classes.rocm_qlora.AdamW(self.state_bits)
         for group, a in zip(self.param_groups, self._arenas):
             held.add_group(group["params"], a["m"], a["v"], a["scales"], a["low"], a["steps"], a["ticket"])
-        if self.max_grad_norm is not None:
-            self.grad_norm = torch.zeros((), device=self._arenas[0]["m"].device)
         self._native = held
         return held
 
@@ -156,6 +159,11 @@ class AdamW(torch.optim.Optimizer):
             hyper += (0.0 if on_device else lr, b1, b2, group["eps"], group["weight_decay"])
             lrs.append(lr if on_device else None)
         clip = self.max_grad_norm is not None
+        if clip:
+            if not self.max_grad_norm > 0.0:
+                raise ValueError(f"max_grad_norm must be positive, got {self.max_grad_norm}")
+            if self.grad_norm is None:
+                self.grad_norm = torch.zeros((), device=self._arenas[0]["m"].device)
         held.step(hyper, lrs, self.max_grad_norm if clip else -1.0,
                   self.grad_norm if clip else self._arenas[0]["ticket"])
         return loss

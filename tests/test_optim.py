@@ -381,6 +381,25 @@ def test_refused_parameters():
 
 
 @pytest.mark.gpu
+def test_a_refused_step_changes_nothing_and_clipping_may_come_later():
+    from rocm_qlora.optim import AdamW
+    a, b = made([(300,), (20, 20)], F4, seed=12)
+    opt = AdamW([dict(params=[a]), dict(params=[b], lr=torch.zeros(()))], lr=1e-2, weight_decay=0)
+    before = a.detach().clone()
+    with pytest.raises(ValueError):
+        opt.step()  # the second group's learning rate is on the CPU
+    assert torch.equal(a.detach(), before) and int(opt.state[a]["step"]) == 0
+    opt.param_groups[1]["lr"] = 1e-2
+    opt.max_grad_norm = -1.0
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.max_grad_norm = 0.5
+    opt.step()
+    norm = math.sqrt(sum(float(p.grad.to(F8).square().sum()) for p in (a, b)))
+    assert abs(float(opt.grad_norm) - norm) <= 2.0 ** -23 * norm and int(opt.state[a]["step"]) == 1
+
+
+@pytest.mark.gpu
 def test_hooks_schedulers_and_profiler_ranges():
     from rocm_qlora.optim import AdamW
     (p,) = made([(300,)], F4, seed=10)
@@ -431,6 +450,16 @@ def test_refused_numbers():
             AdamW([p], **kw)
     with pytest.raises(ValueError):
         AdamW([])
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate")
+def test_refused_parameters_that_share_memory():
+    """One launch updates a group's tensors side by side."""
+    from rocm_qlora.optim import AdamW
+    p, whole = torch.nn.Parameter(torch.zeros(8)), torch.zeros(40)
+    for params in ([p, p], [torch.nn.Parameter(whole[:21]), torch.nn.Parameter(whole[20:])]):
+        with pytest.raises(ValueError, match="share memory"):
+            AdamW(params)
 
 
 def test_refused_devices():
