@@ -6,25 +6,26 @@
 // memory, and sums in fp32 in tensor memory: 4 times the rate of 16-bit
 // operands, and no value is ever unpacked.
 //
-// A stage of a CTA's ring holds 256 columns: the codes of 128 rows of operand P
-// and of some of operand Q (128 bytes a row, by TMA with 128-byte swizzle), and
-// both scales' pieces of 512 bytes (128 rows x 128 columns, stored in the order
-// that tensor memory takes).  tcgen05.cp spreads a piece over 4 columns of
-// tensor memory; every slot has columns of its own, so a copy never overwrites
-// scales in use.
-//   warp 0     producer (one thread)
-//   warp 1     tensor memory; one thread copies scales and issues the MMAs
-//   warps 2-9  epilogue: warps w and w + 4 share the 32 rows of lane quarter w % 4
+// Codes come to a ring of stages by TMA, 128 bytes (256 columns) of a row with
+// 128-byte swizzle; scales are pieces of 512 bytes (128 rows x 128 columns,
+// stored in the order that tensor memory takes), 4 columns of tensor memory each.
+// Every slot of the ring has scale columns of its own, so none is overwritten in
+// use.  Warp 0 loads (one thread), warp 1 has the tensor memory and issues the
+// MMAs (one thread), 8 epilogue warps share the 32 rows of a lane quarter by twos.
 // Two kernels:
 //   mx4_pair_k   many tiles.  CTA pairs stay and take tiles of 256 tokens x 256
 //                outputs in turn (2-SM MMAs; a CTA loads its 128 tokens and half
-//                of the outputs, so a stage's 35 KB feed 512 cycles of MMA, where
-//                a CTA alone needs 51 KB: the L2 gave 45 bytes a cycle and SM);
-//                the epilogue empties the accumulator into shared memory, and
-//                the next tile's MMAs run while it stores.
-//   mx4_split_k  few tiles.  P are outputs, Q up to 256 tokens, and a cluster
+//                of the outputs).  The epilogue empties the accumulator into
+//                registers, and the next tile's MMAs run while it stores.  Bound
+//                by the tensor cores: 8192 x 4096 -> 11008 in bf16 takes 143 us,
+//                5.1 PFLOP/s (MMA pipe 67 % active; 4096 x 4096 -> 4096, whose
+//                3.5 rounds of tiles take four, 32 us).
+//   mx4_split_k  few tiles.  P are outputs, Q up to 128 tokens, and a cluster
 //                splits the columns: each CTA parks its sums in shared memory,
 //                and all add up a share in rank order (fixed order: deterministic).
+//                Bound by latency: 64 x 4096 -> 11008 takes 11.4 us, 3.4 of
+//                them the weight's bytes at the copy bandwidth; one token x
+//                4096 -> 4096 6.2.
 // Waits are bounded: one that runs out counts a kernel timeout, the CTAs drain
 // their copies and store nothing.
 #include <cuda.h>
@@ -359,7 +360,11 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
 
 namespace pair {
 // A stage holds 512 columns here: a wait or a commit costs the tensor pipe about
-// 100 cycles, next to the 1082 of a stage's 8 MMAs.
+// 100 cycles, next to the 1082 of a stage's 8 MMAs.  Four warps store the scales
+// to tensor memory, from registers: as copies (tcgen05.cp) between the MMAs a
+// stage's 12 pieces cost the pipe about 960 cycles more, since one copy at a time
+// overlaps an MMA (8192 x 4096 -> 11008: 214 us with copies, 188 with stores,
+// both with stages of 256 columns; 146 with stages of 512).
 constexpr int S = 3;
 constexpr uint32_t kCodes = 128 * 128;                      // 256 columns of P's or of half of Q's rows
 constexpr uint32_t kStage = 4 * kCodes;                     // P's two, Q's two
