@@ -9,6 +9,19 @@ namespace rq {
 
 constexpr int kDQBlock2 = 256;  // second-level block of QuantLinear.enable_double_quant
 
+// 32 bytes at once, from and to an address that is a multiple of that.
+__device__ __forceinline__ void load32(const void* from, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void store32(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // First statement of a kernel that is launched as the programmatic dependent
 // of the one before it: it reads and writes nothing before every grid before
 // it has finished, and lets its own dependent come up only then, so that a

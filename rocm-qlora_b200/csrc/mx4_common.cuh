@@ -27,21 +27,25 @@ __device__ __forceinline__ int64_t mx4_scale_at(int64_t r, int b, int tiles) {
   return ((r / 128) * tiles + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4;
 }
 
-// A lane's 8 values as they are in memory (16-bit types packed in 4 words), at
-// columns col .. col + 7, 0 past K.  VEC: whole 16-byte pieces, so all 8 exist or
-// none does.
-template <int DT> struct M4Raw { uint32_t w[DT == RQ_F32 ? 8 : 4]; };
+// A lane's values as they are in memory (16-bit types two to a word), at columns
+// col .. col + W - 1, 0 past K.  ALIGN: bytes at which all pieces of a row lie, of
+// which all values exist or none does; 0: none.
+template <int DT, int W = 8> struct M4Raw { uint32_t w[DT == RQ_F32 ? W : W / 2]; };
 
-template <int DT, bool VEC>
-__device__ __forceinline__ M4Raw<DT> m4_load(const typename DType<DT>::T* row, int col, int K) {
-  M4Raw<DT> r = {};
-  if constexpr (VEC) {
+template <int DT, int ALIGN, int W = 8>
+__device__ __forceinline__ M4Raw<DT, W> m4_load(const typename DType<DT>::T* row, int col, int K) {
+  M4Raw<DT, W> r = {};
+  constexpr int words = DT == RQ_F32 ? W : W / 2;
+  if constexpr (ALIGN == 32 && words == 8) {
+    if (col < K) load32(row + col, r.w);
+  } else if constexpr (ALIGN) {
     if (col < K) {
 #pragma unroll
-      for (int h = 0; h < (DT == RQ_F32 ? 2 : 1); ++h)
-        *reinterpret_cast<uint4*>(r.w + 4 * h) = *reinterpret_cast<const uint4*>(row + col + 4 * h);
+      for (int h = 0; h < words / 4; ++h)
+        *reinterpret_cast<uint4*>(r.w + 4 * h) = reinterpret_cast<const uint4*>(row + col)[h];
     }
   } else {
+    static_assert(W == 8, "");
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (DT == RQ_F32) {
@@ -55,10 +59,10 @@ __device__ __forceinline__ M4Raw<DT> m4_load(const typename DType<DT>::T* row, i
   return r;
 }
 
-template <int DT>
-__device__ __forceinline__ void m4_values(const M4Raw<DT>& r, float (&v)[8]) {
+template <int DT, int W>
+__device__ __forceinline__ void m4_values(const M4Raw<DT, W>& r, float (&v)[W]) {
 #pragma unroll
-  for (int i = 0; i < (DT == RQ_F32 ? 8 : 4); ++i) {
+  for (int i = 0; i < (DT == RQ_F32 ? W : W / 2); ++i) {
     if constexpr (DT == RQ_F32) {
       v[i] = __uint_as_float(r.w[i]);
     } else if constexpr (DT == RQ_BF16) {
@@ -72,12 +76,13 @@ __device__ __forceinline__ void m4_values(const M4Raw<DT>& r, float (&v)[8]) {
   }
 }
 
-// Largest magnitudes of blocks of which each of 4 neighbouring lanes has 8 values,
-// as fp32 bits, in which an infinity or NaN is the largest.  16-bit magnitudes are
+// Largest magnitudes of blocks, of which each of 32 / W neighbouring lanes has W
+// values, as fp32 bits, in which an infinity or NaN is the largest.  16-bit magnitudes are
 // compared two at a time, and two blocks share a word on their way.
-template <int DT, int N>
-__device__ __forceinline__ void m4_top(const M4Raw<DT> (&r)[N], uint32_t (&top)[N]) {
+template <int DT, int W, int N>
+__device__ __forceinline__ void m4_top(const M4Raw<DT, W> (&r)[N], uint32_t (&top)[N]) {
   if constexpr (DT == RQ_F32) {
+    static_assert(DT != RQ_F32 || W == 8, "");
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       uint32_t m = 0;
@@ -89,15 +94,17 @@ __device__ __forceinline__ void m4_top(const M4Raw<DT> (&r)[N], uint32_t (&top)[
   } else {
     uint32_t m[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      m[n] = __vmaxs2(__vmaxs2(r[n].w[0] & 0x7fff7fffu, r[n].w[1] & 0x7fff7fffu),
-                      __vmaxs2(r[n].w[2] & 0x7fff7fffu, r[n].w[3] & 0x7fff7fffu));
+    for (int n = 0; n < N; ++n) {
+      m[n] = 0;
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) m[n] = __vmaxs2(m[n], r[n].w[i] & 0x7fff7fffu);
+    }
 #pragma unroll
     for (int n = 0; n < N; n += 2) {
       const uint32_t other = n + 1 < N ? m[n + 1 < N ? n + 1 : n] : 0u;
       uint32_t both = __vmaxs2(__byte_perm(m[n], other, 0x5410), __byte_perm(m[n], other, 0x7632));
       both = __vmaxs2(both, __shfl_xor_sync(0xffffffffu, both, 1));
-      both = __vmaxs2(both, __shfl_xor_sync(0xffffffffu, both, 2));
+      if constexpr (W == 8) both = __vmaxs2(both, __shfl_xor_sync(0xffffffffu, both, 2));
 #pragma unroll
       for (int h = 0; h < 2 && n + h < N; ++h) {
         const uint16_t bits = (uint16_t)(h ? both >> 16 : both);
@@ -108,7 +115,7 @@ __device__ __forceinline__ void m4_top(const M4Raw<DT> (&r)[N], uint32_t (&top)[
 }
 
 // Eight e2m1 codes (nearest, ties to even, saturating), the first in the low bits.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float by) {
+__device__ __forceinline__ uint32_t e2m1x8(const float* v, float by) {
   uint32_t w;
   asm("{\n .reg .b8 a, b, c, d;\n"
       " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"

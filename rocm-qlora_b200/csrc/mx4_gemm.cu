@@ -257,12 +257,12 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
       unsigned char* q = sm + PL::kRing + i * PL::kQStage;
       const T* row = x + (int64_t)(q0 + r) * g.ldx;
       const int col = (s0 + i) * 256 + lane * 8;
-      const M4Raw<DT> raw[1] = {g.vec ? m4_load<DT, true>(row, col, g.K) : m4_load<DT, false>(row, col, g.K)};
+      const M4Raw<DT> raw[1] = {g.vec ? m4_load<DT, 16>(row, col, g.K) : m4_load<DT, 0>(row, col, g.K)};
       uint32_t top[1];
-      m4_top<DT, 1>(raw, top);
+      m4_top<DT, 8, 1>(raw, top);
       const uint32_t byte = m4_scale(top[0]);
       float v[8];
-      m4_values<DT>(raw[0], v);
+      m4_values<DT, 8>(raw[0], v);
       *reinterpret_cast<uint32_t*>(q + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + lane % 4 * 4) = e2m1x8(v, m4_factor(byte));
       uint32_t word = byte << (lane % 16 / 4 * 8);
       word |= __shfl_xor_sync(0xffffffffu, word, 4);
