@@ -498,7 +498,7 @@ RQ_API int rq_grad_norm_end(const double* partials, int n, float* norm, void* st
  * 4 exponent and 4 mantissa bits (the whole numbers to 31, then 16 steps to a
  * power of two, to 31 2^14; not 0 for v > 0), scales [blocks, 2] what the codes
  * are multiplied by.  low (bf16 parameters, or NULL): int16 [blocks * 256], the
- * difference of a 32-bit value and its bf16 as bit patterns.  Arenas 16-byte
+ * difference of a 32-bit value and its bf16 as bit patterns.  Arenas 32-byte
  * aligned.  ticket: one zero, which the call leaves zero. */
 typedef struct RqAdamStep {
   double lr, beta1, beta2, eps, decay;
@@ -513,7 +513,8 @@ typedef struct RqAdamStep {
 RQ_API int rq_adam_update(const RqAdamTensor* tensors, int count, int dtype, int bits, void* m, void* v,
                    float* scales, int16_t* low, const RqAdamStep* step, void* stream);
 
-/* Moments of `blocks` blocks between their 8-bit form and fp32 (v, not its root). */
+/* Moments of `blocks` blocks between their 8-bit form and fp32 (v, not its root;
+ * 32-byte aligned). */
 RQ_API int rq_adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, int64_t blocks,
                    float* m, float* v, void* stream);
 RQ_API int rq_adam_pack(const float* m, const float* v, int64_t blocks, uint8_t* m8, uint8_t* r8, float* scales,

@@ -624,7 +624,7 @@ int rq_adam_update(const RqAdamTensor* tensors, int count, int dtype, int bits, 
   if (count == 0) return RQ_OK;
   if (!m || !v || (bits == 8 && !scales) || !step->steps || !step->ticket) return RQ_ERR_INVALID;
   if (step->n_partials < 0 || (step->n_partials > 0 && (!step->partials || !step->norm))) return RQ_ERR_INVALID;
-  if ((uintptr_t)m % 16 || (uintptr_t)v % 16 || (uintptr_t)scales % 8 || (uintptr_t)low % 16 ||
+  if ((uintptr_t)m % 32 || (uintptr_t)v % 32 || (uintptr_t)scales % 8 || (uintptr_t)low % 16 ||
       (uintptr_t)step->partials % 8 || (uintptr_t)step->norm % 4 || (uintptr_t)step->steps % 4 ||
       (uintptr_t)step->ticket % 4 || (uintptr_t)step->lr_at % 4)
     return RQ_ERR_ALIGN;
@@ -637,7 +637,7 @@ int rq_adam_unpack(const uint8_t* m8, const uint8_t* r8, const float* scales, in
   if (!fits(blocks)) return RQ_ERR_INVALID;
   if (blocks == 0) return RQ_OK;
   if (!m8 || !r8 || !scales || !m || !v) return RQ_ERR_INVALID;
-  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 16 || (uintptr_t)v % 16)
+  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 32 || (uintptr_t)v % 32)
     return RQ_ERR_ALIGN;
   return adam_unpack(m8, r8, scales, blocks, m, v, (cudaStream_t)stream);
 }
@@ -648,7 +648,7 @@ int rq_adam_pack(const float* m, const float* v, int64_t blocks, uint8_t* m8, ui
   if (!fits(blocks)) return RQ_ERR_INVALID;
   if (blocks == 0) return RQ_OK;
   if (!m8 || !r8 || !scales || !m || !v) return RQ_ERR_INVALID;
-  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 16 || (uintptr_t)v % 16)
+  if ((uintptr_t)m8 % 8 || (uintptr_t)r8 % 8 || (uintptr_t)scales % 8 || (uintptr_t)m % 32 || (uintptr_t)v % 32)
     return RQ_ERR_ALIGN;
   return adam_pack(m, v, blocks, m8, r8, scales, (cudaStream_t)stream);
 }

@@ -404,7 +404,8 @@ void adam_pack_(const Tensor& m, const Tensor& v, Tensor m8, Tensor r8, Tensor s
               "rocm_qlora: not moments and their 8-bit form");
   if (m.is_meta()) return;
   const c10::cuda::CUDAGuard guard(m.device());
-  const Tensor m4 = aligned(m), v4 = aligned(v);
+  const auto whole = [](const Tensor& t) { return (uintptr_t)t.data_ptr() % 32 ? t.clone() : t; };
+  const Tensor m4 = whole(m), v4 = whole(v);
   check(rq_adam_pack(m4.data_ptr<float>(), v4.data_ptr<float>(), m8.numel() / RQ_ADAM_BLOCK, m8.data_ptr<uint8_t>(),
                      r8.data_ptr<uint8_t>(), scales.data_ptr<float>(), stream_of(m)),
         "rq_adam_pack");
