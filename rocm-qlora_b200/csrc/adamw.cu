@@ -130,16 +130,6 @@ __device__ __forceinline__ void store_raw(void* p, int64_t at, int n, const Raw<
   }
 }
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8f(const void* p, int64_t at, int n, float (&v)[8]) {
-  const Raw<DT> r = load_raw<DT, VEC>(p, at, n);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = pair_of<DT>(r, i);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
 // 8 fp32 moments of a lane, in one access: with two of 16 bytes a warp's accesses
 // leave every second 16 bytes out (reading 202 M moments back 365 us, now 301).
 __device__ __forceinline__ void load_moments(const float* from, float (&v)[8]) {
@@ -159,35 +149,51 @@ __device__ __forceinline__ void store_moments(float* to, const float (&v)[8]) {
 
 // Adds the squares of a lane's 8 values in 64 bits.  Widening takes a
 // conversion, whose pipe does 8 values a cycle; for normal numbers the bits are
-// moved instead (the exponent grows by 896), in bf16 two values share the test
-// for others.
+// moved instead (the exponent grows by 896), in bf16 from the packed words, where
+// two values share the test for others.
 template <int DT>
-__device__ __forceinline__ void add_squares(const float (&v)[8], double& s) {
-  bool normal = true;
+__device__ __forceinline__ void add_squares(const Raw<DT>& r, double& s) {
+  constexpr uint32_t up = 896u << 20;
   if constexpr (DT == RQ_BF16) {
     uint32_t least = 0x7f807f80u, most = 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t e = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632) & 0x7f807f80u;
+      const uint32_t e = r.w[i] & 0x7f807f80u;
       least = __vminu2(least, e);
       most = __vmaxu2(most, e);
     }
-    normal = (least & 0xffffu) != 0u && least > 0xffffu && (most & 0xffffu) != 0x7f80u && most < 0x7f800000u;
-  } else {
-    uint32_t least = 0x7f800000u, most = 0u;
+    if ((least & 0xffffu) != 0u && least > 0xffffu && (most & 0xffffu) != 0x7f80u && most < 0x7f800000u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double x = __hiloint2double((int)((r.w[i] & 0x7fffu) * 8192u + up), 0);
+        const double y = __hiloint2double((int)(((r.w[i] & 0x7fff0000u) >> 3) + up), 0);
+        s = fma(x, x, s);
+        s = fma(y, y, s);
+      }
+      return;
+    }
+  }
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = pair_of<DT>(r, i);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+  uint32_t least = 0x7f800000u, most = 0u;
+  if constexpr (DT != RQ_BF16) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t e = __float_as_uint(v[i]) & 0x7f800000u;
       least = min(least, e);
       most = max(most, e);
     }
-    normal = least != 0u && most != 0x7f800000u;
   }
-  if (normal) {
+  if (DT != RQ_BF16 && least != 0u && most != 0x7f800000u) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-      const double d = __hiloint2double((int)(__umulhi(b, 1u << 29) + (896u << 20)), DT == RQ_BF16 ? 0 : (int)(b << 29));
+      const double d = __hiloint2double((int)(__umulhi(b, 1u << 29) + up), (int)(b << 29));
       s = fma(d, d, s);
     }
   } else {
@@ -214,9 +220,9 @@ __global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_consta
     constexpr int N = 4;
     const uint32_t whole = min(end, t.first[i + 1] - 1);
     if (aligned && b + (N - 1) * kAdWarps < whole) {
-      float v[N][8];
+      Raw<DT> v[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) load8f<DT, true>(t.g[i], at + k * kAdWarps * kAdBlock, 8, v[k]);
+      for (int k = 0; k < N; ++k) v[k] = load_raw<DT, true>(t.g[i], at + k * kAdWarps * kAdBlock, 8);
 #pragma unroll
       for (int k = 0; k < N; ++k) add_squares<DT>(v[k], sum);
       b += N * kAdWarps;
@@ -224,10 +230,8 @@ __global__ void __launch_bounds__(kAdThreads) norm_partial_k(const __grid_consta
     }
     const bool last = b + 1 == t.first[i + 1];
     const int n = (last ? t.tail[i] : kAdBlock) - lane * 8;
-    float v[8];
-    if (aligned && (!last || t.tail[i] == kAdBlock)) load8f<DT, true>(t.g[i], at, 8, v);
-    else load8f<DT, false>(t.g[i], at, n, v);
-    add_squares<DT>(v, sum);
+    if (aligned && (!last || t.tail[i] == kAdBlock)) add_squares<DT>(load_raw<DT, true>(t.g[i], at, 8), sum);
+    else add_squares<DT>(load_raw<DT, false>(t.g[i], at, n), sum);
     b += kAdWarps;
   }
 #pragma unroll
@@ -268,10 +272,15 @@ __global__ void __launch_bounds__(kAdThreads) norm_end_k(const double* __restric
 
 // ------------------------------------------------------- moments in 8 bits
 
-// max that a NaN wins.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// Largest magnitude, which a NaN wins; smallest value.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -281,25 +290,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // 16 <= q <= 32 from there; the code is q + 16 e, and the sum holds q in its low
 // bits and e in its exponent.
 __device__ __forceinline__ uint32_t root_code(float t) {
-  const uint32_t e = max(__float_as_uint(t) & 0x7f800000u, 131u << 23);  // 2^(4 + e)
-  const uint32_t sum = __float_as_uint(__fadd_rn(t, __uint_as_float(e + (19u << 23 | 0x400000u))));
+  // 2^(4 + e) is the power of two in t, at least 2^4
+  const uint32_t at = __viaddmax_u32(__float_as_uint(t) & 0x7f800000u, 19u << 23 | 0x400000u, 150u << 23 | 0x400000u);
+  const uint32_t sum = __float_as_uint(__fadd_rn(t, __uint_as_float(at)));
   return sum + (sum >> 19) - ((150u << 4) + 8u);
 }
-// The value of byte i of w.  A code's bits above exponent 130 are v = (16 + M)
-// 2^(E - 1) from 16 on and v = 8 + c / 2 below, where the value is 2 v - 16:
-// it is the smaller of the two in either case.
-__device__ __forceinline__ float root_value(uint32_t w, int i) {
-  const float v = __uint_as_float(__byte_perm(w, 0u, 0x4440u | (uint32_t)i) * (1u << 19) + (130u << 23));
-  return fminf(v, fmaf(v, 2.0f, -16.0f));
-}
-
-// Values 2 i and 2 i + 1 of m and v from a lane's code words.
+// Values 2 i and 2 i + 1 of m and v from a lane's code words.  A root's code at the
+// lowest exponent and highest mantissa bits of a half is the value times 2^-18,
+// subnormals included.
 __device__ __forceinline__ void decode2(const uint2& cm, const uint2& cr, const float2& scale, int i, float2& m, float2& v) {
-  const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1)), c = i < 2 ? cr.x : cr.y;
+  const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1));
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   m = make_float2(__fmul_rn(f.x, scale.x), __fmul_rn(f.y, scale.x));
-  const float a = __fmul_rn(root_value(c, 2 * i & 3), scale.y), b = __fmul_rn(root_value(c, (2 * i & 3) + 1), scale.y);
+  const uint32_t c = __byte_perm(i < 2 ? cr.x : cr.y, 0u, i & 1 ? 0x3424u : 0x1404u) >> 2;
+  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&c));
+  const float by = scale.y * 0x1p18f, a = __fmul_rn(r.x, by), b = __fmul_rn(r.y, by);
   v = make_float2(__fmul_rn(a, a), __fmul_rn(b, b));
 }
 
@@ -308,9 +314,8 @@ __device__ __forceinline__ void decode2(const uint2& cm, const uint2& cr, const 
 // are multiplied by on the way to codes) and max / most, of m and of r.
 __device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&r)[8], int64_t block, int lane,
                                                uint8_t* codes_m, uint8_t* codes_r, float2* scales) {
-  float tm = fabsf(m[0]), tr = r[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) tm = max_nan(tm, fabsf(m[i])), tr = max_nan(tr, r[i]);
+  const float tm = max_nan(max_nan(m[0], m[1], m[2]), max_nan(m[3], m[4], m[5]), max_nan(m[6], m[7], 0.0f));
+  const float tr = max_nan(max_nan(r[0], r[1], r[2]), max_nan(r[3], r[4], r[5]), max_nan(r[6], r[7], 0.0f));
   // as bit patterns, in which an infinity or NaN is the largest
   const uint32_t bm = __reduce_max_sync(0xffffffffu, __float_as_uint(tm) & 0x7fffffffu);
   const uint32_t br = __reduce_max_sync(0xffffffffu, __float_as_uint(tr) & 0x7fffffffu);
@@ -326,12 +331,16 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
   for (int i = 0; i < 4; ++i)
     cm[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[2 * i], to_m), __fmul_rn(m[2 * i + 1], to_m)),
                                      __NV_SATFINITE, __NV_E4M3);
-  const float least = to_r > 0.0f ? 1.0f : 0.0f;
+  float t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = __fmul_rn(r[i], to_r);
-    c[i] = root_code(r[i] > 0.0f ? fmaxf(t, least) : t);
+  for (int i = 0; i < 8; ++i) t[i] = __fmul_rn(r[i], to_r);
+  // what is not 0 is at least 1: seldom less before
+  if (min3(min3(t[0], t[1], t[2]), min3(t[3], t[4], t[5]), fminf(t[6], t[7])) < 1.0f && to_r > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = r[i] > 0.0f ? fmaxf(t[i], 1.0f) : t[i];
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = root_code(t[i]);
   const int64_t at = block * kAdBlock + lane * 8;
   *reinterpret_cast<uint2*>(codes_m + at) = make_uint2(cm[0] | cm[1] << 16, cm[2] | cm[3] << 16);
   *reinterpret_cast<uint2*>(codes_r + at) =
