@@ -24,9 +24,9 @@
 // multiply-add), so that a code is what the formula in 32 bits gives.
 //
 // With 32-bit moments a step is bound by memory (40 M values in fp32, 448 tensors,
-// clipped, 32 bytes a value: 208 us, 6.1 TB/s), with 8-bit ones by issue slots,
-// 73 % busy (160 M values in bf16, 448 tensors, clipped, 12 bytes a value: 448 us,
-// 4.3 TB/s).
+// clipped, 32 bytes a value: 208 us, 6.1 TB/s), with 8-bit ones by issue slots
+// and memory (160 M values in bf16, 448 tensors, clipped, 12 bytes a value: 380 us,
+// 5.0 TB/s; 202 M with remainders, 14 bytes: 496 us, 5.7 TB/s).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -272,6 +272,31 @@ __global__ void __launch_bounds__(kAdThreads) norm_end_k(const double* __restric
 
 // ------------------------------------------------------- moments in 8 bits
 
+// Two values in one instruction, each rounded as by itself.
+__device__ __forceinline__ uint64_t pair64(float2 a) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a.x), "f"(a.y));
+  return d;
+}
+__device__ __forceinline__ float2 float2_of(uint64_t a) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair64(a)), "l"(pair64(b)));
+  return float2_of(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) { return mul2(a, make_float2(b, b)); }
+// One by one: the compiler makes a product of pairs and their addition one rounding.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 fma2(float2 a, float b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair64(a)), "l"(pair64(make_float2(b, b))), "l"(pair64(c)));
+  return float2_of(d);
+}
+
 // Largest magnitude, which a NaN wins; smallest value.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float d;
@@ -302,11 +327,11 @@ __device__ __forceinline__ void decode2(const uint2& cm, const uint2& cr, const 
   const uint32_t w = (i < 2 ? cm.x : cm.y) >> (16 * (i & 1));
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  m = make_float2(__fmul_rn(f.x, scale.x), __fmul_rn(f.y, scale.x));
+  m = mul2(f, scale.x);
   const uint32_t c = __byte_perm(i < 2 ? cr.x : cr.y, 0u, i & 1 ? 0x3424u : 0x1404u) >> 2;
   const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&c));
-  const float by = scale.y * 0x1p18f, a = __fmul_rn(r.x, by), b = __fmul_rn(r.y, by);
-  v = make_float2(__fmul_rn(a, a), __fmul_rn(b, b));
+  const float2 a = mul2(r, scale.y * 0x1p18f);
+  v = mul2(a, a);
 }
 
 // m and r = sqrt(v) of a whole warp's block to codes and scales.  Of the four
@@ -329,11 +354,14 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
   uint32_t cm[4], c[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    cm[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[2 * i], to_m), __fmul_rn(m[2 * i + 1], to_m)),
-                                     __NV_SATFINITE, __NV_E4M3);
+    cm[i] = __nv_cvt_float2_to_fp8x2(mul2(make_float2(m[2 * i], m[2 * i + 1]), to_m), __NV_SATFINITE, __NV_E4M3);
   float t[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = __fmul_rn(r[i], to_r);
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = mul2(make_float2(r[2 * i], r[2 * i + 1]), to_r);
+    t[2 * i] = x.x;
+    t[2 * i + 1] = x.y;
+  }
   // what is not 0 is at least 1: seldom less before
   if (min3(min3(t[0], t[1], t[2]), min3(t[3], t[4], t[5]), fminf(t[6], t[7])) < 1.0f && to_r > 0.0f) {
 #pragma unroll
@@ -390,54 +418,77 @@ __device__ __forceinline__ float split_low(float p, uint32_t& low16) {
   return __uint_as_float(top);
 }
 
-// One value: m, v and p after the step, and r = sqrt(v).
+// Two values: m, v and p after the step, and r = sqrt(v).
 template <bool EIGHT>
-__device__ __forceinline__ float update(float g, float& m, float& v, float p, const float4& f, const AdState& a) {
-  const float x = __fmul_rn(g, f.w);
-  m = __fadd_rn(__fmul_rn(m, a.beta1), __fmul_rn(x, a.rest1));
-  v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(x, x), a.rest2));
+__device__ __forceinline__ float2 update(float2 g, float2& m, float2& v, float2 p, const float4& f, const AdState& a) {
+  const float2 x = mul2(g, f.w);
+  m = add2(mul2(m, a.beta1), mul2(x, a.rest1));
+  v = add2(mul2(v, a.beta2), mul2(mul2(x, x), a.rest2));
   // in 8 bits the root is the state (and takes v's place); elsewhere it only divides the step
-  float r, q;
-  if constexpr (EIGHT) v = r = __fsqrt_rn(v);
-  else asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  float2 r, q;
+  if constexpr (EIGHT) {
+    v = r = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
+  } else {
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  }
   // The divisor is at least eps or 2^-75, and an approximate reciprocal's error
   // of 2^-23 is far below what the step's product with lr leaves of p.
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(r, f.y, a.eps)));
-  return fmaf(p, f.z, -(f.x * m) * q);
+  const float2 d = fma2(r, f.y, make_float2(a.eps, a.eps));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(d.y));
+  return fma2(p, f.z, mul2(mul2(m, -f.x), q));
+}
+
+// What a lane reads of a block.
+template <int DT, bool EIGHT, bool LOW>
+struct In {
+  Raw<DT> g, p;
+  Raw<RQ_BF16> low;
+  uint2 cm, cr;  // 8 bits
+  float2 scale;
+  float m[8], v[8];  // 32 bits
+};
+
+template <int DT, bool VEC, bool EIGHT, bool LOW>
+__device__ __forceinline__ void fetch(In<DT, EIGHT, LOW>& d, const void* p, const void* g, int64_t at, int n,
+                                      int64_t block, int lane, const AdState& a) {
+  const int64_t sat = block * kAdBlock + lane * 8;
+  d.g = load_raw<DT, VEC>(g, at, n);
+  d.p = load_raw<DT, VEC>(p, at, n);
+  if constexpr (LOW) d.low = load_raw<RQ_BF16, true>(a.low, sat, 8);
+  if constexpr (EIGHT) {
+    d.cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + sat);
+    d.cr = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + sat);
+    d.scale = a.scales[block];
+  } else {
+    load_moments(static_cast<const float*>(a.m) + sat, d.m);
+    load_moments(static_cast<const float*>(a.v) + sat, d.v);
+  }
 }
 
 template <int DT, bool VEC, bool EIGHT, bool LOW>
-__device__ __forceinline__ void update8(void* p, const void* g, int64_t at, int n, int64_t block, int lane,
-                                        const float4& f, const AdState& a) {
+__device__ __forceinline__ void update8(const In<DT, EIGHT, LOW>& d, void* p, int64_t at, int n, int64_t block,
+                                        int lane, const float4& f, const AdState& a) {
   const int64_t sat = block * kAdBlock + lane * 8;
-  const Raw<DT> gr = load_raw<DT, VEC>(g, at, n);
-  Raw<DT> pr = load_raw<DT, VEC>(p, at, n);
-  Raw<RQ_BF16> low = {};
-  if constexpr (LOW) low = load_raw<RQ_BF16, true>(a.low, sat, 8);
+  Raw<DT> pr;
+  Raw<RQ_BF16> low;
   float m[8], v[8];
-  uint2 cm, cr;
-  float2 scale;
-  if constexpr (EIGHT) {
-    cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + sat);
-    cr = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + sat);
-    scale = a.scales[block];
-  } else {
-    load_moments(static_cast<const float*>(a.m) + sat, m);
-    load_moments(static_cast<const float*>(a.v) + sat, v);
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    float2 mv, vv;
     if constexpr (EIGHT) {
-      float2 x, y;
-      decode2(cm, cr, scale, i, x, y);
-      m[2 * i] = x.x, m[2 * i + 1] = x.y;
-      v[2 * i] = y.x, v[2 * i + 1] = y.y;
+      decode2(d.cm, d.cr, d.scale, i, mv, vv);
+    } else {
+      mv = make_float2(d.m[2 * i], d.m[2 * i + 1]);
+      vv = make_float2(d.v[2 * i], d.v[2 * i + 1]);
     }
-    const float2 gv = pair_of<DT>(gr, i);
-    float2 pv = pair_of<DT>(pr, i);
-    if constexpr (LOW) pv = make_float2(join_low(pv.x, low.w[i]), join_low(pv.y, low.w[i] >> 16));
-    pv.x = update<EIGHT>(gv.x, m[2 * i], v[2 * i], pv.x, f, a);
-    pv.y = update<EIGHT>(gv.y, m[2 * i + 1], v[2 * i + 1], pv.y, f, a);
+    const float2 gv = pair_of<DT>(d.g, i);
+    float2 pv = pair_of<DT>(d.p, i);
+    if constexpr (LOW) pv = make_float2(join_low(pv.x, d.low.w[i]), join_low(pv.y, d.low.w[i] >> 16));
+    pv = update<EIGHT>(gv, mv, vv, pv, f, a);
+    m[2 * i] = mv.x, m[2 * i + 1] = mv.y;
+    v[2 * i] = vv.x, v[2 * i + 1] = vv.y;
     if constexpr (LOW) {
       uint32_t x, y;
       pv = make_float2(split_low(pv.x, x), split_low(pv.y, y));
@@ -455,8 +506,13 @@ __device__ __forceinline__ void update8(void* p, const void* g, int64_t at, int 
   }
 }
 
+// CTAs an SM.  Four would leave 64 registers a thread, too few for the next block's
+// inputs (8 bits, 202 M values with remainders: 496 us with three, 541 with four).
+constexpr int kAdResident = 3;
+
 template <int DT, bool EIGHT, bool LOW, int MAX>
-__global__ void __launch_bounds__(kAdThreads, EIGHT ? 4 : 3) adam_update_k(const __grid_constant__ AdTensors<MAX> t, const AdState a) {
+__global__ void __launch_bounds__(kAdThreads, kAdResident) adam_update_k(const __grid_constant__ AdTensors<MAX> t,
+                                                                        const AdState a) {
   grid_begin();
   const int lane = threadIdx.x % 32;
   float c = 1.0f;
@@ -483,14 +539,25 @@ __global__ void __launch_bounds__(kAdThreads, EIGHT ? 4 : 3) adam_update_k(const
     if (((uintptr_t)g | (uintptr_t)p) % 16 == 0) {
       const uint32_t whole = min(end, next - (t.tail[i] != kAdBlock));
       int64_t at = (int64_t)in * kAdBlock + lane * 8, block = (int64_t)t.block[i] + in;
+      // with 8-bit moments the next block is on its way while this one is computed
+      // (160 M values in bf16 419 us without, 380 with)
+      In<DT, EIGHT, LOW> d;
+      if (EIGHT && b < whole) fetch<DT, true, EIGHT, LOW>(d, p, g, at, 8, block, lane, a);
 #pragma unroll 1
-      for (; b < whole; b += kAdWarps, at += kAdWarps * kAdBlock, block += kAdWarps)
-        update8<DT, true, EIGHT, LOW>(p, g, at, 8, block, lane, f, a);
+      for (; b < whole; b += kAdWarps, at += kAdWarps * kAdBlock, block += kAdWarps) {
+        if constexpr (!EIGHT) fetch<DT, true, EIGHT, LOW>(d, p, g, at, 8, block, lane, a);
+        const In<DT, EIGHT, LOW> now_in = d;
+        if (EIGHT && b + kAdWarps < whole)
+          fetch<DT, true, EIGHT, LOW>(d, p, g, at + kAdWarps * kAdBlock, 8, block + kAdWarps, lane, a);
+        update8<DT, true, EIGHT, LOW>(now_in, p, at, 8, block, lane, f, a);
+      }
       in = b - t.first[i];
     }
     if (b < end && b < next) {
       const int n = (b + 1 == next ? t.tail[i] : kAdBlock) - lane * 8;
-      update8<DT, false, EIGHT, LOW>(p, g, (int64_t)in * kAdBlock + lane * 8, n, (int64_t)t.block[i] + in, lane, f, a);
+      In<DT, EIGHT, LOW> d;
+      fetch<DT, false, EIGHT, LOW>(d, p, g, (int64_t)in * kAdBlock + lane * 8, n, (int64_t)t.block[i] + in, lane, a);
+      update8<DT, false, EIGHT, LOW>(d, p, (int64_t)in * kAdBlock + lane * 8, n, (int64_t)t.block[i] + in, lane, f, a);
       b += kAdWarps;
     }
   }
@@ -594,7 +661,10 @@ template <int DT, bool EIGHT, bool LOW, int MAX>
 static int update_t(const RqAdamTensor* list, int count, const AdState& a, cudaStream_t st) {
   AdTensors<MAX> t;
   fill(t, list, count);
-  return launch_dependent(adam_update_k<DT, EIGHT, LOW, MAX>, grid_for(t.first[count], 8), kAdThreads, st, t, a);
+  // 32 bits: more than are resident, or the last to end are waited for (208 us with
+  // 8 an SM, 222 with 3)
+  const unsigned grid = grid_for(t.first[count], EIGHT ? kAdResident : 8);
+  return launch_dependent(adam_update_k<DT, EIGHT, LOW, MAX>, grid, kAdThreads, st, t, a);
 }
 
 template <bool EIGHT, int MAX>
