@@ -126,12 +126,13 @@ def test_pack_strides_and_shapes():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, BF, HF])
 @pytest.mark.parametrize("first", [0, 4, 8, 16])
-def test_pack_rows_at_every_alignment(first, dtype):
+@pytest.mark.parametrize("rows,widths", [(131, (16, 144, 400, 1040, 1048)), (999, (1040, 1048, 2064))])
+def test_pack_rows_at_every_alignment(rows, widths, first, dtype):
     """Rows that lie at multiples of 32, 16 and 8 bytes, in widths of whole and of part pieces."""
     from rocm_qlora.mx4 import pack_mx4, unpack_mx4
     g = torch.Generator().manual_seed(first)
-    x = torch.randn(131, 1072, generator=g).to(dtype)
-    for k in (16, 144, 400, 1040, 1048):
+    x = torch.randn(rows, 2080, generator=g).to(dtype)
+    for k in widths:
         part = x.cuda()[:, first:first + k]
         p = pack_mx4(part)
         check_form(x[:, first:first + k], p)
