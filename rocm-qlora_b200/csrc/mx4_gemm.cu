@@ -387,23 +387,6 @@ struct PairArgs {
   int64_t ld;
 };
 
-// 16 columns of this thread's lane, and the wait for them (which changes nothing,
-// but what follows depends on it).
-__device__ __forceinline__ void tmem_issue16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ready16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-
 // 12 columns of this thread's lane
 __device__ __forceinline__ void tmem_st12(uint32_t taddr, const uint4 (&v)[3]) {
 #pragma unroll
@@ -567,7 +550,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
     int done = 0;
     for (int t = first; t < ntile; t += stride, ++done) {
       const int p0 = t % pt * 256 + (int)rank * 128 + quad * 32, q0 = t / pt * 256 + half * 128;
-      if (g.bias) {  // 128 outputs' bias, in this warp's staging
+      // 128 outputs' bias in this warp's staging, while it waits: as shuffles of a lane's
+      // values they held up the next tile's MMAs (8192 x 4096 -> 11008 with bias 164 us,
+      // now 152; without 147)
+      if (g.bias) {
 #pragma unroll
         for (int j = 0; j < 128; j += 32) {
           const int q = q0 + j + lane;
@@ -581,28 +567,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint4 w[16];  // this lane's row: 128 outputs, 8 a piece
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
-      // 16 columns are rounded while the next ones are on their way: the next tile's
-      // MMAs wait for this (8192 x 4096 -> 11008 142.7 us; 144.9 with 32 at a time)
-      uint32_t raw[2][16];
-      tmem_issue16(from, raw[0]);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        tmem_ready16(raw[c & 1]);
-        if (c < 7) tmem_issue16(from + (c + 1) * 16, raw[(c + 1) & 1]);
-        float acc[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[j] = __uint_as_float(raw[c & 1][j]);
+      for (int c = 0; c < 4; ++c) {
+        float acc[32];
+        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + half * 128 + c * 32, acc);
         if (g.bias) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 b = reinterpret_cast<const float4*>(stage)[c * 4 + j];
+          for (int j = 0; j < 8; ++j) {
+            const float4 b = reinterpret_cast<const float4*>(stage)[c * 8 + j];
             acc[4 * j] += b.x, acc[4 * j + 1] += b.y, acc[4 * j + 2] += b.z, acc[4 * j + 3] += b.w;
           }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          w[2 * c + j] =
+        for (int j = 0; j < 4; ++j)
+          w[4 * c + j] =
               make_uint4(pack_rn<DT>(acc[8 * j], acc[8 * j + 1]), pack_rn<DT>(acc[8 * j + 2], acc[8 * j + 3]),
                          pack_rn<DT>(acc[8 * j + 4], acc[8 * j + 5]), pack_rn<DT>(acc[8 * j + 6], acc[8 * j + 7]));
       }
