@@ -176,7 +176,7 @@ def prepare(case, seed):
     s["case"] = case
     if case["op"] == "adam":
         s["step"] = STEPS
-        if case["bits"] == 8 and not own:
+        if case["bits"] == 8:
             s["m"], s["v"] = _kept_m(s["m"]), _kept_r(s["v"].sqrt()).square()
     elif case["op"] != "pack":
         # a frozen weight is packed once, when the model is loaded
