@@ -407,8 +407,15 @@ __device__ __forceinline__ float4 factors_of(const AdState& a, int t, float c) {
 // What bf16 parameters leave: the 32-bit value of a bf16 and its 16 bits, and
 // back, rounded half away from zero so that what is left fits 16 bits with its
 // sign.
+// A parameter that was written from outside comes with the remainder of the
+// value before, which is less than a unit in its last place.  Two kinds of pair do
+// not count, since rounding leaves none: a negative remainder at 0, where one
+// step down in the bits is a NaN, and any at an infinity (a value above the
+// largest bf16 becomes one for good).
 __device__ __forceinline__ float join_low(float p, uint32_t low16) {
-  return __uint_as_float(__float_as_uint(p) + (uint32_t)(int32_t)(int16_t)low16);
+  const uint32_t sum = __float_as_uint(p) + (uint32_t)(int32_t)(int16_t)low16;
+  const bool other_sign = (int32_t)(sum ^ __float_as_uint(p)) < 0;  // only a step down from 0
+  return other_sign || !(fabsf(p) < __uint_as_float(0x7f800000u)) ? p : __uint_as_float(sum);
 }
 __device__ __forceinline__ float split_low(float p, uint32_t& low16) {
   const uint32_t bits = __float_as_uint(p);

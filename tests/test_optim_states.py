@@ -1,0 +1,103 @@
+"""What happens to the states of rocm_qlora.optim.AdamW from outside a step:
+parameters that are written over, states and learning rates that are loaded,
+groups without parameters, gradients that are views or not finite."""
+import pytest
+import torch
+
+from tests.test_optim import BF, F8, HALF, NUMBERS, TINY, formula
+
+
+def stepped(values, bits, steps=3, seed=20):
+    """A bf16 parameter with a remainder, after some steps."""
+    from rocm_qlora.optim import AdamW
+    g = torch.Generator().manual_seed(seed)
+    p = torch.nn.Parameter(torch.randn(values, generator=g).to(BF).cuda())
+    opt = AdamW([p], **NUMBERS, state_bits=bits, remainder=True)
+    for _ in range(steps):
+        p.grad = (torch.randn(values, generator=g) * 0.1).to(BF).cuda()
+        opt.step()
+    return p, opt
+
+
+def check_from(p, opt, start, t):
+    """One step of p from the values `start`, to which a remainder of less than
+    a unit in their last place may belong (2^-7 of them; nothing of it at 0 but
+    2^-134): p is the formula's, rounded to bf16 once."""
+    m, v = (x[:p.numel()].clone() for x in opt.moments())
+    opt.step()
+    want, _, _, _, step = formula(start, p.grad, m, v, t)
+    slack = (2.0 ** -7 + 2.0 ** -22) * start.to(F8).abs() + 2.0 ** -18 * step + 2.0 ** -133
+    bound = HALF[BF] * (want.abs() + slack) + slack + TINY[BF]
+    off = (p.detach().to(F8) - want).abs()
+    assert bool((off <= bound).all()), (int((~(off <= bound)).sum()), float(off.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("write", ["zero", "negative zero", "negated", "half", "some zero"])
+def test_a_parameter_written_over_goes_on_from_what_was_written(write, bits):
+    p, opt = stepped(1000, bits)
+    low = opt.state[p]["remainder"]
+    assert bool((low < 0).any()) and bool((low > 0).any())
+    with torch.no_grad():
+        if write == "zero":
+            p.zero_()
+        elif write == "negative zero":
+            p.fill_(-0.0)
+        elif write == "negated":
+            p.neg_()
+        elif write == "half":
+            p.fill_(0.5)
+        else:
+            p[::3] = 0.0
+    check_from(p, opt, p.detach().clone(), 4)
+    check_from(p, opt, p.detach().clone(), 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_infinities_written_into_a_parameter_stay(bits):
+    p, opt = stepped(600, bits)
+    start = p.detach().clone()
+    start[:200], start[200:400] = float("inf"), float("-inf")
+    with torch.no_grad():
+        p.copy_(start)
+    opt.step()
+    assert torch.equal(p.detach()[:400], start[:400]) and bool(torch.isfinite(p.detach()[400:]).all())
+
+
+@pytest.mark.gpu
+def test_merged_and_reset_adapters_go_on():
+    """merge_lora zeroes an adapter's matrices, set_adapter writes another one."""
+    from rocm_qlora import LoRALinear, QuantLinear
+    from rocm_qlora.lora import AdapterBank
+    from rocm_qlora.optim import AdamW
+    torch.manual_seed(21)
+    layer = LoRALinear(QuantLinear.from_linear(torch.nn.Linear(128, 64, bias=False, dtype=BF, device="cuda"), bits=4),
+                       r=8).cuda()
+    layer.lora_A.data, layer.lora_B.data = layer.lora_A.data.to(BF), layer.lora_B.data.to(BF)
+    bank = AdapterBank(128, 64, 2, 16, BF, torch.device("cuda"))
+    torch.nn.init.normal_(bank.lora_A)
+    torch.nn.init.normal_(bank.lora_B)
+    params = [layer.lora_A, layer.lora_B, bank.lora_A, bank.lora_B]
+    opts = [AdamW([p], **NUMBERS, remainder=True) for p in params]
+
+    def gradients():
+        for p in params:
+            p.grad = torch.randn_like(p) * 0.1
+
+    for _ in range(3):
+        gradients()
+        for o in opts:
+            o.step()
+    layer.merge_lora()
+    layer.unmerge_lora()
+    bank.set_adapter(1, torch.randn(8, 128, device="cuda"), torch.zeros(64, 8, device="cuda"), 1.0)
+    gradients()
+    for p, o in zip(params, opts):
+        start = p.detach().clone()
+        m, v = (x[:p.numel()].view(p.shape).clone() for x in o.moments())
+        o.step()
+        want, _, _, _, step = formula(start, p.grad, m, v, 4)
+        slack = (2.0 ** -7 + 2.0 ** -22) * start.to(F8).abs() + 2.0 ** -18 * step + 2.0 ** -133
+        assert bool(((p.detach().to(F8) - want).abs() <= HALF[BF] * (want.abs() + slack) + slack + TINY[BF]).all())
