@@ -114,13 +114,6 @@ __device__ __forceinline__ uint32_t factor(uint32_t byte, int top) {
   return f << 16 | f;
 }
 
-// Arrival on a barrier of the pair's leader, after this CTA's own writes to its
-// own shared memory: those need no more than CTA scope.  (A release at cluster
-// scope waits about a microsecond for everything remote.)
-__device__ __forceinline__ void arrive_leader(uint32_t cbar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
-}
-
 template <int DT, bool FAR>
 __device__ __forceinline__ uint4 widen8(uint32_t w, uint32_t by) {
   uint4 v = make_uint4(spread<DT, 0>(w), spread<DT, 1>(w), spread<DT, 2>(w), spread<DT, 3>(w));
@@ -175,11 +168,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
   constexpr int S = PL::S;
   extern __shared__ __align__(1024) unsigned char dsm[];
   // dy[S] (leader's: both CTAs' dy), codes[S] (own), read[S] (own codes are
-  // widened), wide[S] (leader's: both CTAs' widening warps), empty[S], acc[2],
-  // taken[2] (leader's)
+  // widened), wide[S] (leader's: its widening warps, and a signal of the peer's
+  // for each), empty[S], acc[2], taken[2] (leader's)
   __shared__ __align__(8) uint64_t bars[5 * S + 5];
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_flag;
+  __shared__ __align__(16) uint32_t sig_src[4], sig_dst[4];  // of the 16-byte signals (contents unused)
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = cluster_rank();
   const uint32_t sraw = smem_u32(dsm), sbase = (sraw + 1023u) & ~1023u;
@@ -199,7 +193,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
       mbar_init(dy0 + 8 * i, 1);
       mbar_init(codes0 + 8 * i, 1);
       mbar_init(read0 + 8 * i, kWiden);
-      mbar_init(wide0 + 8 * i, 2 * kWiden);
+      mbar_init(wide0 + 8 * i, kWiden);
       mbar_init(empty0 + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -208,6 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     }
     mbar_init(drainbar, 1);
     abort_flag = 0;
+    for (int i = 0; i < 4; ++i) sig_src[i] = sig_dst[i] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -263,7 +258,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         if (t >= 2 && !wait_pair(taken0 + 8 * (t & 1), ((t >> 1) - 1) & 1, ab)) break;
         for (int st = 0; st < steps; ++st, ++i) {
           const int slot = i % S;
-          ok = wait_pair(dy0 + 8 * slot, (i / S) & 1, ab) && wait_pair(wide0 + 8 * slot, (i / S) & 1, ab);
+          ok = wait_pair(dy0 + 8 * slot, (i / S) & 1, ab) && wait_pair<true>(wide0 + 8 * slot, (i / S) & 1, ab);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t a = sbase + slot * PL::kStage, b = a + PL::kB;
@@ -288,7 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
     // codes: 16-byte pieces of a row of BN / 4 bytes, in the swizzle of their TMA box
     const uint32_t load = PL::kC + row * (BN / 4);
     const int swz = BN == 256 ? (row >> 1) & 3 : (row >> 2) & 1, piece = col / 32;
-    const uint32_t wide = mapa(wide0, 0);
+    const uint32_t wide = mapa(wide0, 0), sig_lead = mapa(smem_u32(sig_dst), 0);
     int i = (warp - 2) / kWiden;  // the team's next stage, of all
     bool ok = true;
     for (int n = 0; n < tiles && ok; ++n) {
@@ -333,7 +328,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // visible to the tensor cores
         __syncwarp();
         if (lane == 0) {
-          arrive_leader(wide + 8 * slot);
+          // The leader's warps arrive and each expect the 16 bytes of a signal from one
+          // of the peer's, whose values its MMAs read too.  A signal is a copy in the
+          // proxy that the values were just made visible to, and its completion is
+          // ordered for the cluster.  An arrival from the other CTA would need a release
+          // at cluster scope, which waits for everything remote (8192 x 4096 ->
+          // 11008 641 us with that, 534 with signals; 4096 -> 4096 of one token 43 and 25).
+          if (rank == 0) mbar_expect_tx(wide0 + 8 * slot, 16);
+          else bulk_signal(sig_lead, smem_u32(sig_src), wide + 8 * slot);
           // Only now: the values have been used, so the loads of the codes are over.
           // Said right after them, the next TMA copy overtook loads still in the
           // queue (an arrival waits for neither those nor for the other proxy).

@@ -210,11 +210,12 @@ struct PairAbort {
   unsigned int* count;
   __device__ __forceinline__ bool raised() const { return *mine != 0; }
 };
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
-  if (mbar_try<false>(bar, parity)) return true;
+  if (mbar_try<kCluster>(bar, parity)) return true;
   const uint64_t t0 = gtimer_ns();
   while (!ab.raised()) {
-    if (mbar_try<false>(bar, parity)) return true;
+    if (mbar_try<kCluster>(bar, parity)) return true;
     if (gtimer_ns() - t0 > kPairWaitNs) {
       *ab.mine = 1;
       st_cluster(ab.peer, 1);
