@@ -449,6 +449,12 @@ RQ_API int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M,
                   const uint8_t* w_codes, const uint8_t* w_scales, int64_t N, int64_t K,
                   const void* bias, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* How long a product of few tokens (rq_mx4_matmul, rq_mx4_linear) waits for its
+ * own copies and sums before it gives up, in ns: 2 s unless set; 0: every wait has
+ * run out before it begins; below 0: 2 s again.  Outputs whose sums a wait ran out
+ * for are NaN, and rq_take_kernel_timeouts counts it. */
+RQ_API int rq_mx4_set_wait(int64_t ns);
+
 /* dx [M, K] (contiguous) = dy [M, N] . w, w the packed weight [N, K] and dy in
  * dtype (bf16 or f16) with row stride ld_dy, a multiple of 8 with dy 16-byte
  * aligned.  w enters in dy's dtype: exact in bf16; in f16 times 2^(127 - top),

@@ -552,6 +552,11 @@ int rq_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, co
   return mx4_matmul(Mx4{a_codes, a_scales, M}, Mx4{b_codes, b_scales, N}, K, bias, out, dtype, (cudaStream_t)stream);
 }
 
+int rq_mx4_set_wait(int64_t ns) {
+  mx4_set_wait(ns);
+  return RQ_OK;
+}
+
 int64_t rq_mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   return !fits(M) || !fits(N) || !fits(K) ? -1 : mx4_linear_workspace_bytes(M, N, K);
 }

@@ -27,9 +27,12 @@
 //                them the weight's bytes at the copy bandwidth; one token x
 //                4096 -> 4096 6.2.
 // Waits are bounded: one that runs out counts a kernel timeout, the CTAs drain
-// their copies and store nothing.
+// their copies, and mx4_pair_k stores nothing more, mx4_split_k NaNs (other CTAs
+// of the cluster add up what this one should have had).
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "gemv_common.cuh"
 #include "mx4_common.cuh"
@@ -94,6 +97,7 @@ struct Args {
   const void* x;            // PACK: Q's rows [qrows, K]
   int64_t ldx;
   int K;
+  uint64_t limit;           // of a wait, in ns; 0: has run out before it begins
   bool vec;
   bool early;               // the kernel before this one is the packing of Q's rows, which has itself waited for
                             // all before it: P is there already
@@ -135,12 +139,12 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t limit) {
   if (mbar_try<false>(bar, parity)) return true;
   const uint64_t t0 = gtimer_ns();
   while (!*abort) {
     if (mbar_try<false>(bar, parity)) return true;
-    if (gtimer_ns() - t0 > kPairWaitNs) {
+    if (gtimer_ns() - t0 > limit) {
       *abort = 1;
       atomicAdd(&g_mx4_timeouts, 1u);
       return false;
@@ -173,9 +177,11 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
-    mbar_init(accbar, 1);
+    mbar_init(accbar, 2);
     mbar_init(qbar, kEpiWarps);
-    abort_flag = issued = consumed = 0;
+    issued = consumed = 0;
+    abort_flag = g.limit == 0;
+    if (g.limit == 0) atomicAdd(&g_mx4_timeouts, 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
     if (lane == 0) {
       for (int st = s0; st < s1; ++st) {
         const int i = st - s0, slot = i % S;
-        if (i >= S && !wait(empty0 + 8 * slot, ((i / S) - 1) & 1, abort)) break;
+        if (i >= S && !wait(empty0 + 8 * slot, ((i / S) - 1) & 1, abort, g.limit)) break;
         if (i >= early) load_p(st, slot);
         if constexpr (!PACK) {
           const uint32_t at = sbase + slot * PL::kStage, bar = full0 + 8 * slot;
@@ -225,10 +231,10 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const bool packed = !PACK || wait(qbar, 0, abort);
+      const bool packed = !PACK || wait(qbar, 0, abort, g.limit);
       for (int st = s0; st < s1 && packed; ++st) {
         const int i = st - s0, slot = i % S;
-        if (!wait(full0 + 8 * slot, (i / S) & 1, abort)) break;
+        if (!wait(full0 + 8 * slot, (i / S) & 1, abort, g.limit)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t at = sbase + slot * PL::kStage, q = PACK ? sbase + PL::kRing + i * PL::kQStage : at + PL::kQ, tsc = tmem + PL::kAcc + slot * PL::kSlotCols;
         const int nt = min(2, g.tiles - 2 * st);
@@ -246,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
         *reinterpret_cast<volatile int*>(&consumed) = i + 1;
       }
       mma_commit(accbar);
+      mbar_arrive(accbar);  // whoever sees the barrier sees an abort before it too
     }
   } else if constexpr (PACK) {
     // a warp packs the 256 columns of a token's stage: 8 values a lane, a code
@@ -282,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
   T* out = static_cast<T*>(g.out);
   bool ok = false;
   if (warp >= 2) {
-    if (lane == 0) ok = wait(accbar, 0, abort) && !*abort;
+    if (lane == 0) ok = wait(accbar, 0, abort, g.limit) && !*abort;
     ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   }
@@ -296,12 +303,12 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
       if (sk > 1) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (c + j < BN) red[(c + j) * kPark + row] = ok && s1 > s0 ? acc[j] : 0.0f;
-      } else if (ok) {
+          if (c + j < BN && ok) red[(c + j) * kPark + row] = acc[j];
+      } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (c + j < BN && q0 + c + j < g.qrows && n < g.prows)
-            out[(int64_t)(q0 + c + j) * g.ld + n] = DType<DT>::from_f32(acc[j] + bv);
+            out[(int64_t)(q0 + c + j) * g.ld + n] = DType<DT>::from_f32(ok ? acc[j] + bv : __uint_as_float(0x7fc00000u));
       }
     }
   }
@@ -318,6 +325,10 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_split_k(const __grid_constant
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PL::kCols) : "memory");
   }
   if (sk > 1) {
+    if (*abort) {  // the same for all threads since their last barrier
+      __syncthreads();  // copies under way have been drained
+      for (int i = tid; i < BN * kPark; i += kThreads) reinterpret_cast<uint32_t*>(sm)[i] = 0x7fc00000u;
+    }
     __syncwarp();
     cluster_sync();  // all sums are parked
     // this CTA's share: groups of 4 outputs of a token, the loads of all ranks at once
@@ -691,6 +702,8 @@ int split_for(int64_t tiles, int64_t steps, int bn) {
   return sk < 1 ? 1 : sk > 8 ? 8 : (int)sk;
 }
 
+std::atomic<uint64_t> g_limit{kPairWaitNs};
+
 struct Rows {  // tokens in 16 bits
   const void* x;
   int64_t ld;
@@ -718,6 +731,7 @@ int split_t(const Mx4& a, const Rows& x, const Mx4& b, int64_t K, const void* bi
   g.ldx = x.ld;
   g.K = (int)K;
   g.early = early;
+  g.limit = g_limit.load(std::memory_order_relaxed);
   g.vec = (uintptr_t)x.x % 16 == 0 && x.ld % 8 == 0 && K % 8 == 0;
   const int64_t tiles = ((b.rows + kP - 1) / kP) * ((a.rows + BN - 1) / BN);
   const int sk = split_for(tiles, steps, BN);
@@ -759,6 +773,8 @@ int matmul_t(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out,
 }
 
 }  // namespace
+
+void mx4_set_wait(int64_t ns) { g_limit.store(ns < 0 ? kPairWaitNs : (uint64_t)ns, std::memory_order_relaxed); }
 
 int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* out, int dt, cudaStream_t st) {
   return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, b, K, bias, out, false, st) : matmul_t<RQ_F16>(a, b, K, bias, out, false, st);

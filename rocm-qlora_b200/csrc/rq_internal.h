@@ -179,6 +179,7 @@ int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* ou
 int64_t mx4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mx4_linear(const void* x, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, const void* bias, void* out,
                void* ws, cudaStream_t st);
+void mx4_set_wait(int64_t ns);
 int mx4_dx(const void* dy, int dt, int64_t ld, int64_t M, const Mx4& w, int64_t K, void* dx, void* ws, cudaStream_t st);
 
 int align_rows(const void* x, int64_t ld, int64_t M, int64_t N, void* out, int64_t ldo, cudaStream_t st);

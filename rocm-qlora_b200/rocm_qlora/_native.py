@@ -98,6 +98,7 @@ def _bind(L: ctypes.CDLL) -> None:
         "rq_mx4_pack": ([P, I, I64, I64, I64, P, P, P], I),
         "rq_mx4_unpack": ([P, P, I64, I64, P, I, P], I),
         "rq_mx4_matmul": ([P, P, I64, P, P, I64, I64, P, P, I, P], I),
+        "rq_mx4_set_wait": ([I64], I),
         "rq_mx4_linear_workspace_bytes": ([I64, I64, I64], I64),
         "rq_mx4_linear": ([P, I, I64, I64, P, P, I64, I64, P, P, P, I64, P], I),
         "rq_mx4_dx": ([P, I, I64, I64, P, P, I64, I64, P, P, I64, P], I),
@@ -129,7 +130,8 @@ def exported_symbols() -> Tuple[str, ...]:
             "rq_adapter_plan_words", "rq_adapter_plan", "rq_adapters_apply", "rq_adapters_grad",
             "rq_act8_pack", "rq_act8_unpack", "rq_swiglu8_forward", "rq_swiglu8_backward",
             "rq_token_logprobs", "rq_preference_loss", "rq_token_logprobs_grad",
-            "rq_mx4_scale_bytes", "rq_mx4_pack", "rq_mx4_unpack", "rq_mx4_matmul", "rq_mx4_linear_workspace_bytes",
+            "rq_mx4_scale_bytes", "rq_mx4_pack", "rq_mx4_unpack", "rq_mx4_matmul", "rq_mx4_set_wait",
+            "rq_mx4_linear_workspace_bytes",
             "rq_mx4_linear", "rq_mx4_dx", "rq_align_rows", "rq_grad_norm_partial", "rq_grad_norm_end",
             "rq_adam_update", "rq_adam_unpack", "rq_adam_pack",
             "launch_int4_dequant_matmul", "launch_int8_dequant_matmul")

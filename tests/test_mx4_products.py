@@ -21,3 +21,45 @@ def test_gradient_is_the_same_every_time(rows, k, n, dtype):
     got = [nat.loaded_ops().mx4_dx(dy, packed.codes, packed.scales, k) for _ in range(50)]
     close(got[0], dy.to(F8) @ wk, sums(dy.to(F8), wk.t(), n))
     assert all(torch.equal(x, got[0]) for x in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 4096, 4096), (8, 1024, 130), (16, 4096, 2048), (33, 2048, 1000),
+                                      (64, 4096, 2048), (200, 4096, 512), (20, 200, 100)])
+def test_a_wait_that_runs_out_leaves_no_partial_sums(rows, k, n):
+    """Without time for a wait no product has its sums, whether one CTA or a
+    cluster makes them: outputs are NaN, the timeouts are counted, and the next
+    call is as ever."""
+    import ctypes
+    from rocm_qlora import _native as nat
+    from rocm_qlora.mx4 import mx4_linear, pack_mx4
+    L = nat.load_library()
+    x, bias = torch.randn(rows, k, device="cuda", dtype=BF), torch.randn(n, device="cuda", dtype=BF)
+    w = pack_mx4(torch.randn(n, k, device="cuda", dtype=BF))
+    want = mx4_linear(x, w, bias)
+    out = torch.full((rows, n), 7.0, device="cuda", dtype=BF)
+    need = L.rq_mx4_linear_workspace_bytes(rows, n, k)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    count = ctypes.c_uint(0)
+
+    def call():
+        torch.cuda.synchronize()
+        rc = L.rq_mx4_linear(x.data_ptr(), 1, k, rows, w.codes.data_ptr(), w.scales.data_ptr(), n, k, bias.data_ptr(),
+                             out.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and L.rq_take_kernel_timeouts(ctypes.byref(count)) == 0
+        return count.value
+
+    assert L.rq_take_kernel_timeouts(ctypes.byref(count)) == 0
+    try:
+        assert L.rq_mx4_set_wait(0) == 0
+        assert call() > 0 and bool(torch.isnan(out).all())
+    finally:
+        assert L.rq_mx4_set_wait(-1) == 0
+    assert call() == 0 and torch.equal(out, want)
+
+
+def test_the_limit_of_a_wait_takes_any_number():
+    from rocm_qlora import _native as nat
+    L = nat.load_library()
+    for ns in (0, 1, 2 ** 62, -2 ** 63, -1):
+        assert L.rq_mx4_set_wait(ns) == 0
