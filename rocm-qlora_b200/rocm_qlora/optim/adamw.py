@@ -1,7 +1,8 @@
 """AdamW over many tensors in one launch, its moments in 32 or in 8 bits
 (csrc/adamw.cu), and the norm of many gradients.
 """
-from typing import Any, Dict, Iterable, Optional, Tuple, Union
+import copy
+from typing import Any, Dict, Iterable, List, Optional, Tuple, Union
 
 import torch
 
@@ -197,8 +198,10 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
-        """Copies the saved values into the states, whose places stay (captured
-        graphs see them)."""
+        """Copies the saved values into the states, and saved learning rates into
+        the tensors that hold them here: both stay where they are, so that
+        captured graphs see the loaded values, and nothing is shared with
+        ``state_dict``."""
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("the saved state is of other parameter groups")
@@ -211,10 +214,26 @@ class AdamW(torch.optim.Optimizer):
                 pairs += [(own[k], new[k]) for k in own]
         for own, new in pairs:
             own.copy_(new)
+        taken: List[torch.Tensor] = []
         for g, s in zip(groups, saved):
             for k, value in s.items():
-                if k != "params":
-                    g[k] = tuple(value) if k == "betas" else value
+                if k == "lr":
+                    self._load_rate(g, value, taken)
+                elif k != "params":
+                    g[k] = tuple(value) if k == "betas" else copy.deepcopy(value)
+
+    def _load_rate(self, group: Dict[str, Any], value: Union[float, torch.Tensor], taken: List[torch.Tensor]) -> None:
+        """taken: the tensors that have taken a group's rate so far."""
+        own = group["lr"]
+        if not isinstance(own, torch.Tensor):
+            if isinstance(value, torch.Tensor):
+                value = value.detach().to(self._arenas[0]["m"].device, torch.float32, copy=True)
+            group["lr"] = value
+            return
+        if any(own is t for t in taken) and float(own) != float(value):
+            own = group["lr"] = own.clone()  # groups that had one rate and now have two
+        own.copy_(value.reshape(own.shape) if isinstance(value, torch.Tensor) else torch.full_like(own, value))
+        taken.append(own)
 
     def __getstate__(self):
         raise TypeError("an AdamW is not copied or pickled: save its state_dict()")

@@ -4,7 +4,7 @@ groups without parameters, gradients that are views or not finite."""
 import pytest
 import torch
 
-from tests.test_optim import BF, F8, HALF, NUMBERS, TINY, formula
+from tests.test_optim import BF, F4, F8, HALF, NUMBERS, TINY, formula, made
 
 
 def stepped(values, bits, steps=3, seed=20):
@@ -101,3 +101,70 @@ def test_merged_and_reset_adapters_go_on():
         want, _, _, _, step = formula(start, p.grad, m, v, 4)
         slack = (2.0 ** -7 + 2.0 ** -22) * start.to(F8).abs() + 2.0 ** -18 * step + 2.0 ** -133
         assert bool(((p.detach().to(F8) - want).abs() <= HALF[BF] * (want.abs() + slack) + slack + TINY[BF]).all())
+
+
+# ------------------------------------------------------ loaded learning rates
+
+def with_rate(lr, seed=25, **kw):
+    from rocm_qlora.optim import AdamW
+    (p,) = made([(300,)], F4, seed=seed)
+    return p, AdamW([p], lr=lr, **kw)
+
+
+def rate(value):
+    return torch.full((), value, device="cuda")
+
+
+@pytest.mark.gpu
+def test_a_loaded_rate_is_seen_by_a_captured_step():
+    own = rate(1e-2)
+    p, opt = with_rate(own)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    q, other = with_rate(rate(0.25))
+    other.load_state_dict(opt.state_dict())
+    other.param_groups[0]["lr"].fill_(0.25)
+    assert float(own) == float(torch.tensor(1e-2))      # each has a rate of its own
+    q.data.copy_(p.data)
+    opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] is own and float(own) == 0.25
+    graph.replay()
+    other.step()
+    assert torch.equal(p, q) and int(opt.state[p]["step"]) == 2
+
+
+@pytest.mark.gpu
+def test_rates_loaded_from_the_cpu_and_from_numbers():
+    p, opt = with_rate(rate(0.5))
+    saved = torch.utils._pytree.tree_map(lambda x: x.cpu() if isinstance(x, torch.Tensor) else x, opt.state_dict())
+    own = rate(1e-3)
+    _, other = with_rate(own)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["lr"] is own and float(own) == 0.5
+    other.step()
+    q, number = with_rate(1e-3)
+    number.load_state_dict(saved)                        # takes a tensor of its own, on its device
+    lr = number.param_groups[0]["lr"]
+    assert lr.is_cuda and lr is not saved["param_groups"][0]["lr"] and float(lr) == 0.5
+    number.step()
+    _, third = with_rate(0.125)
+    other.load_state_dict(third.state_dict())            # a number into the tensor that is there
+    assert other.param_groups[0]["lr"] is own and float(own) == 0.125
+    other.step()
+
+
+@pytest.mark.gpu
+def test_groups_that_shared_a_rate_take_their_own():
+    from rocm_qlora.optim import AdamW
+    own = rate(1e-2)
+    a, b = made([(300,), (40, 20)], F4, seed=26)
+    opt = AdamW([dict(params=[a]), dict(params=[b])], lr=own)
+    saved = opt.state_dict()
+    opt.load_state_dict(saved)
+    assert all(g["lr"] is own for g in opt.param_groups)
+    saved["param_groups"][0]["lr"], saved["param_groups"][1]["lr"] = rate(0.5), rate(0.25)
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] is own and [float(g["lr"]) for g in opt.param_groups] == [0.5, 0.25]
+    opt.step()
