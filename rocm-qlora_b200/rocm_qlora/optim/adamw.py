@@ -74,14 +74,19 @@ class AdamW(torch.optim.Optimizer):
         try:
             self._check_numbers(group)
             self._check_params(group["params"])
+            self._arenas.append(self._make_state(group["params"]))
         except Exception:
             self.param_groups.pop()
             raise
-        self._make_state(group["params"])
         self._native = None
 
+    @property
+    def _device(self) -> torch.device:
+        """The first parameter's; a group may have none."""
+        return next((p.device for g in self.param_groups for p in g["params"]), torch.device("cpu"))
+
     def _check_params(self, params) -> None:
-        device = self.param_groups[0]["params"][0].device
+        device = self._device
         if len(params) > 65536:
             raise ValueError(f"a parameter group holds at most 65536 tensors, got {len(params)}")
         # one launch updates them side by side
@@ -101,8 +106,8 @@ class AdamW(torch.optim.Optimizer):
             if self.remainder and p.dtype != torch.bfloat16:
                 raise TypeError(f"remainder keeps what bfloat16 parameters leave, got a parameter of {p.dtype}")
 
-    def _make_state(self, params) -> None:
-        device = params[0].device
+    def _make_state(self, params) -> Dict[str, Any]:
+        device = self._device
         blocks = [-(-p.numel() // BLOCK) for p in params]
         total = sum(blocks)
         of = torch.uint8 if self.state_bits == 8 else torch.float32
@@ -112,7 +117,6 @@ class AdamW(torch.optim.Optimizer):
                  low=torch.zeros(total * BLOCK, dtype=torch.int16, device=device) if self.remainder else None,
                  steps=torch.zeros(len(params), dtype=torch.int32, device=device),
                  ticket=torch.zeros(1, dtype=torch.int32, device=device))
-        self._arenas.append(a)
         at = 0
         for i, (p, n) in enumerate(zip(params, blocks)):
             part = slice(at * BLOCK, at * BLOCK + p.numel())
@@ -124,12 +128,16 @@ class AdamW(torch.optim.Optimizer):
             if a["low"] is not None:
                 s["remainder"] = a["low"][part].view(p.shape)
             at += n
+        return a
 
     def _held(self):
         nat.loaded_ops()
         held = torch.classes.rocm_qlora.AdamW(self.state_bits)
         for group, a in zip(self.param_groups, self._arenas):
-            held.add_group(group["params"], a["m"], a["v"], a["scales"], a["low"], a["steps"], a["ticket"])
+            if group["params"]:
+                held.add_group(group["params"], a["m"], a["v"], a["scales"], a["low"], a["steps"], a["ticket"])
+        if self.grad_norm is not None and self.grad_norm.device != self._device:
+            self.grad_norm = None  # made before the first parameter came
         self._native = held
         return held
 
@@ -155,6 +163,8 @@ class AdamW(torch.optim.Optimizer):
         hyper, lrs = [], []
         for group in self.param_groups:
             self._check_numbers(group)
+            if not group["params"]:
+                continue
             lr, (b1, b2) = group["lr"], group["betas"]
             on_device = isinstance(lr, torch.Tensor)
             hyper += (0.0 if on_device else lr, b1, b2, group["eps"], group["weight_decay"])
@@ -164,7 +174,7 @@ class AdamW(torch.optim.Optimizer):
             if not self.max_grad_norm > 0.0:
                 raise ValueError(f"max_grad_norm must be positive, got {self.max_grad_norm}")
             if self.grad_norm is None:
-                self.grad_norm = torch.zeros((), device=self._arenas[0]["m"].device)
+                self.grad_norm = torch.zeros((), device=self._device)
         held.step(hyper, lrs, self.max_grad_norm if clip else -1.0,
                   self.grad_norm if clip else self._arenas[0]["ticket"])
         return loss
@@ -178,6 +188,8 @@ class AdamW(torch.optim.Optimizer):
         a = self._arenas[group]
         if self.state_bits == 32:
             return a["m"], a["v"]
+        if not a["m"].numel():  # a group without parameters
+            return a["m"].float(), a["v"].float()
         return nat.loaded_ops().adam_unpack(a["m"], a["v"], a["scales"])
 
     @torch.no_grad()
@@ -192,7 +204,7 @@ class AdamW(torch.optim.Optimizer):
         if self.state_bits == 32:
             a["m"].copy_(m)
             a["v"].copy_(v)
-        else:
+        elif m.numel():
             nat.loaded_ops().adam_pack_(m.contiguous(), v.contiguous(), a["m"], a["v"], a["scales"])
         a["steps"].fill_(int(step))
 
@@ -227,7 +239,7 @@ class AdamW(torch.optim.Optimizer):
         own = group["lr"]
         if not isinstance(own, torch.Tensor):
             if isinstance(value, torch.Tensor):
-                value = value.detach().to(self._arenas[0]["m"].device, torch.float32, copy=True)
+                value = value.detach().to(self._device, torch.float32, copy=True)
             group["lr"] = value
             return
         if any(own is t for t in taken) and float(own) != float(value):

@@ -1,6 +1,8 @@
 """What happens to the states of rocm_qlora.optim.AdamW from outside a step:
 parameters that are written over, states and learning rates that are loaded,
 groups without parameters, gradients that are views or not finite."""
+import math
+
 import pytest
 import torch
 
@@ -168,3 +170,69 @@ def test_groups_that_shared_a_rate_take_their_own():
     opt.load_state_dict(saved)
     assert opt.param_groups[0]["lr"] is own and [float(g["lr"]) for g in opt.param_groups] == [0.5, 0.25]
     opt.step()
+
+
+# ------------------------------------------------------------- empty groups
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("clip", [None, 0.05])
+@pytest.mark.parametrize("place", ["first", "last", "added"])
+def test_a_group_without_parameters(place, clip, bits):
+    """A split into decayed and other parameters may leave one side empty."""
+    from rocm_qlora.optim import AdamW
+    (p,), (q,) = made([(300,)], F4, seed=27), made([(300,)], F4, seed=27)
+    groups = [dict(params=[p]), dict(params=[], weight_decay=0.0)]
+    opt = AdamW(groups[::-1] if place == "first" else groups if place == "last" else groups[:1], **NUMBERS,
+                state_bits=bits, max_grad_norm=clip)
+    if place == "added":
+        opt.add_param_group(groups[1])
+    plain = AdamW([q], **NUMBERS, state_bits=bits, max_grad_norm=clip)
+    for _ in range(2):
+        opt.step()
+        plain.step()
+    assert torch.equal(p, q) and len(opt.param_groups) == 2
+    if clip:
+        assert torch.equal(opt.grad_norm, plain.grad_norm)
+    empty = 0 if place == "first" else 1
+    assert all(x.shape == (0,) and x.dtype == F4 for x in opt.moments(empty))
+    opt.set_moments(*opt.moments(empty), 2, empty)
+    opt.load_state_dict(opt.state_dict())
+    opt.step()
+    plain.step()
+    assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
+def test_only_empty_groups_and_a_first_parameter_later():
+    from rocm_qlora.optim import AdamW
+    opt = AdamW([dict(params=[])], **NUMBERS, max_grad_norm=0.5)
+    opt.step()
+    (p,), (q,) = made([(300,)], F4, seed=28), made([(300,)], F4, seed=28)
+    opt.add_param_group(dict(params=[p]))
+    opt.step()
+    plain = AdamW([q], **NUMBERS, max_grad_norm=0.5)
+    plain.step()
+    assert torch.equal(p, q) and torch.equal(opt.grad_norm, plain.grad_norm)
+
+
+@pytest.mark.gpu
+def test_a_refused_group_leaves_the_others():
+    from rocm_qlora.optim import AdamW
+    (p,) = made([(300,)], F4, seed=29)
+    opt = AdamW([p], **NUMBERS)
+    for group, error in ((dict(params=[torch.nn.Parameter(torch.zeros(8, device="cuda", dtype=F8))]), TypeError),
+                         (dict(params=[torch.nn.Parameter(torch.zeros(8, device="cuda"))], lr=-1.0), ValueError)):
+        with pytest.raises(error):
+            opt.add_param_group(group)
+        assert len(opt.param_groups) == 1
+        opt.step()
+    assert int(opt.state[p]["step"]) == 2 and math.isfinite(float(p.detach().sum()))
+
+
+def test_empty_groups_need_no_gpu():
+    from rocm_qlora.optim import AdamW
+    for bits in (8, 32):
+        opt = AdamW([dict(params=[]), dict(params=[], lr=0.5)], state_bits=bits, max_grad_norm=1.0)
+        assert opt.step() is None and opt.step(lambda: 2.5) == 2.5
+        assert len(opt.param_groups) == 2 and opt.moments(1)[0].shape == (0,)
