@@ -309,8 +309,10 @@ struct AdamW : torch::CustomClassHolder {
                        grad.scalar_type());
       TORCH_CHECK_TYPE(!g.low.defined() || p.scalar_type() == at::kBFloat16,
                        "remainder keeps what bfloat16 parameters leave: a parameter is ", p.scalar_type());
-      const Tensor flat = grad.is_contiguous() ? grad : grad.contiguous();
-      if (!grad.is_contiguous()) lists.keep.push_back(flat);
+      // a lazily negated view is stored with the other sign, whatever its strides
+      const bool as_is = grad.is_contiguous() && !grad.is_neg();
+      const Tensor flat = as_is ? grad : grad.resolve_neg().contiguous();
+      if (!as_is) lists.keep.push_back(flat);
       lists.by[dtype_code(p.scalar_type())].push_back(
           RqAdamTensor{p.data_ptr(), flat.data_ptr(), p.numel(), g.blocks[i], (int32_t)i});
     }

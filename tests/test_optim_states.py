@@ -105,6 +105,22 @@ def test_merged_and_reset_adapters_go_on():
         assert bool(((p.detach().to(F8) - want).abs() <= HALF[BF] * (want.abs() + slack) + slack + TINY[BF]).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_gradient_with_a_lazy_sign(bits):
+    """The imaginary part of a conjugate is a view whose values are stored with
+    the other sign."""
+    from rocm_qlora.optim import AdamW
+    (p, q), g = made([(300,), (300,)], F4, seed=24), torch.Generator().manual_seed(24)
+    q.data.copy_(p.data)
+    p.grad = torch._neg_view(torch.randn(300, generator=g).cuda())
+    assert p.grad.is_neg()
+    q.grad = p.grad.clone()
+    AdamW([p], state_bits=bits).step()
+    AdamW([q], state_bits=bits).step()
+    assert not q.grad.is_neg() and torch.equal(p, q)
+
+
 # ------------------------------------------------------ loaded learning rates
 
 def with_rate(lr, seed=25, **kw):
