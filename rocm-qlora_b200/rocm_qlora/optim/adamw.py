@@ -213,7 +213,11 @@ class AdamW(torch.optim.Optimizer):
         """Copies the saved values into the states, and saved learning rates into
         the tensors that hold them here: both stay where they are, so that
         captured graphs see the loaded values, and nothing is shared with
-        ``state_dict``."""
+        ``state_dict``.  Hooks that are registered for loading run."""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("the saved state is of other parameter groups")
@@ -233,6 +237,8 @@ class AdamW(torch.optim.Optimizer):
                     self._load_rate(g, value, taken)
                 elif k != "params":
                     g[k] = tuple(value) if k == "betas" else copy.deepcopy(value)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def _load_rate(self, group: Dict[str, Any], value: Union[float, torch.Tensor], taken: List[torch.Tensor]) -> None:
         """taken: the tensors that have taken a group's rate so far."""

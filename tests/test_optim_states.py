@@ -188,6 +188,22 @@ def test_groups_that_shared_a_rate_take_their_own():
     opt.step()
 
 
+@pytest.mark.gpu
+def test_load_state_dict_runs_its_hooks():
+    _, opt = with_rate(1e-2)
+    _, other = with_rate(1.0)
+    called = []
+
+    def before(o, state):
+        called.append("before")
+        return dict(state, param_groups=[dict(g, lr=0.5) for g in state["param_groups"]])
+
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(lambda o: called.append("after"))
+    other.load_state_dict(opt.state_dict())
+    assert called == ["before", "after"] and other.param_groups[0]["lr"] == 0.5
+
+
 # ------------------------------------------------------------- empty groups
 
 @pytest.mark.gpu
