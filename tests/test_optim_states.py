@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.test_optim import BF, F4, F8, HALF, NUMBERS, TINY, formula, made
+from tests.test_optim import BF, F4, F8, HALF, NUMBERS, TINY, formula, kept8, made
 
 
 def stepped(values, bits, steps=3, seed=20):
@@ -103,6 +103,36 @@ def test_merged_and_reset_adapters_go_on():
         want, _, _, _, step = formula(start, p.grad, m, v, 4)
         slack = (2.0 ** -7 + 2.0 ** -22) * start.to(F8).abs() + 2.0 ** -18 * step + 2.0 ** -133
         assert bool(((p.detach().to(F8) - want).abs() <= HALF[BF] * (want.abs() + slack) + slack + TINY[BF]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_gradients_that_are_not_finite_reach_no_other_value(bits):
+    """In 32 bits a NaN or an infinity stays where it is; in 8 bits it takes the
+    moments of its block, whose other parameters' step is the formula's."""
+    from rocm_qlora.optim import AdamW
+    g = torch.Generator().manual_seed(23)
+    p = torch.nn.Parameter(torch.ones(1024, device="cuda"))
+    p.grad = (torch.randn(1024, generator=g) * 0.1).cuda()
+    p.grad[300], p.grad[600] = float("nan"), float("inf")
+    opt = AdamW([p], **NUMBERS, state_bits=bits)
+    opt.step()
+    bad = torch.zeros(1024, dtype=torch.bool, device="cuda")
+    bad[[300, 600]] = True
+    want = formula(torch.ones_like(p), p.grad, torch.zeros_like(p), torch.zeros_like(p), 1)[0]
+    off = (p.detach().to(F8) - want).abs()
+    assert bool((off[~bad] <= 2.0 ** -22).all()) and not bool(torch.isfinite(p.detach()[bad]).any())
+    m, v = opt.moments()
+    if bits == 32:
+        assert torch.equal(torch.isfinite(m), ~bad) and torch.equal(torch.isfinite(v), ~bad)
+        return
+    assert bool(torch.isnan(m[256:768]).all()) and bool(torch.isnan(v[256:768]).all())
+    f = torch.tensor(1 - 0.9), torch.tensor(1 - 0.999)
+    x = p.grad.cpu()
+    want = kept8((x * f[0]).numpy(), (x * x * f[1]).numpy())
+    for got, w in zip((m, v), want):
+        for part in (slice(0, 256), slice(768, 1024)):
+            assert torch.equal(got[part].cpu(), torch.from_numpy(w[part]))
 
 
 @pytest.mark.gpu
