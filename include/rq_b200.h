@@ -497,7 +497,8 @@ RQ_API int rq_grad_norm_end(const double* partials, int n, float* norm, void* st
  *   g = c grad, m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g g,
  *   p = p (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * with c = min(1, max_norm / (norm + 1e-6)) of the norm of n_partials values,
- * which is written to *norm; c is 1 if n_partials is 0.  lr_at: learning rate on
+ * which is written to *norm; c is 1 if n_partials is 0.  An eps above 0 counts as
+ * 2^-126 at least.  lr_at: learning rate on
  * the device (fp32) in lr's place, or NULL.
  * bits 32: m and v are fp32 arenas [blocks * 256].  bits 8: m holds e4m3 codes
  * of m (448 / max|m|) of a block, v codes of sqrt(v) (507904 / max sqrt(v)) with

@@ -29,6 +29,7 @@
 // 5.0 TB/s; 202 M with remainders, 14 bytes: 496 us, 5.7 TB/s).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 
 #include "gemv_common.cuh"
@@ -693,7 +694,8 @@ int adam_update(const RqAdamTensor* list, int count, int dt, int bits, void* m, 
   a.rest1 = (float)(1.0 - step.beta1);
   a.beta2 = (float)step.beta2;
   a.rest2 = (float)(1.0 - step.beta2);
-  a.eps = (float)step.eps;
+  // the quotient takes subnormal divisors as 0
+  a.eps = step.eps > 0.0 && step.eps < FLT_MIN ? FLT_MIN : (float)step.eps;
   a.lr = step.lr;
   a.decay = step.decay;
   a.log_beta1 = log(step.beta1);

@@ -298,3 +298,16 @@ def test_empty_groups_need_no_gpu():
         opt = AdamW([dict(params=[]), dict(params=[], lr=0.5)], state_bits=bits, max_grad_norm=1.0)
         assert opt.step() is None and opt.step(lambda: 2.5) == 2.5
         assert len(opt.param_groups) == 2 and opt.moments(1)[0].shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_eps_below_the_normal_range_keeps_untouched_values(bits):
+    """A value that never had a gradient has a step of 0 / eps."""
+    from rocm_qlora.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.zeros_like(p)
+    p.grad[5] = 0.1
+    AdamW([p], lr=1e-2, eps=1e-40, weight_decay=0.0, state_bits=bits).step()
+    assert bool((p.detach()[torch.arange(300, device="cuda") != 5] == 1.0).all())
+    assert abs(float(p.detach()[5]) - 0.99) <= 2.0 ** -22
