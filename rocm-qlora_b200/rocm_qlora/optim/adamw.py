@@ -29,6 +29,9 @@ class AdamW(torch.optim.Optimizer):
         m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
         p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
+    in 32 bits (root and quotient by the approximate instructions: a step is off
+    by at most 14 x 2^-24 of what it adds up) and rounded once to the type.
+
     Parameters are contiguous float32, bfloat16 or float16 tensors on one
     CUDA device; a step is one launch, or two with clipping, for up to 1024 of a
     dtype, without host synchronisation, and can be captured into a CUDA graph (steps

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.test_optim import BF, F4, F8, HALF, NUMBERS, TINY, formula, kept8, made
+from tests.test_optim import BF, F4, F8, HF, HALF, NUMBERS, TINY, formula, kept8, made
 
 
 def stepped(values, bits, steps=3, seed=20):
@@ -103,6 +103,27 @@ def test_merged_and_reset_adapters_go_on():
         want, _, _, _, step = formula(start, p.grad, m, v, 4)
         slack = (2.0 ** -7 + 2.0 ** -22) * start.to(F8).abs() + 2.0 ** -18 * step + 2.0 ** -133
         assert bool(((p.detach().to(F8) - want).abs() <= HALF[BF] * (want.abs() + slack) + slack + TINY[BF]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F4, BF, HF])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_first_step_from_zero_is_the_step_itself(bits, dtype):
+    """lora_B begins at 0, where the step is all of the parameter.  From empty
+    moments it is lr' m q with m = rest1 g, q = 1 / (sqrt(rest2 g g) y + eps):
+    roundings of 2^-24 are two in m, one and a half in the root of three in v,
+    one each in the root, y, the divisor, the quotient, lr', the two products and
+    the sum; an approximate root and quotient are off by 2^-23 each.  14 of
+    2^-24, and then the type's."""
+    from rocm_qlora.optim import AdamW
+    g = torch.Generator().manual_seed(22)
+    p = torch.nn.Parameter(torch.zeros(5000, dtype=dtype, device="cuda"))
+    p.grad = (torch.randn(5000, generator=g) * 10.0 ** (-3 * torch.rand(5000, generator=g))).to(dtype).cuda()
+    AdamW([p], **NUMBERS, state_bits=bits).step()
+    zero = torch.zeros(5000, device="cuda")
+    want, _, _, _, step = formula(zero, p.grad, zero, zero, 1)
+    slack = 14 * 2.0 ** -24 * step
+    assert bool(((p.detach().to(F8) - want).abs() <= HALF[dtype] * (want.abs() + slack) + slack + TINY[dtype]).all())
 
 
 @pytest.mark.gpu
