@@ -13,6 +13,7 @@ import torch.nn as nn
 
 from rocm_qlora.activation8 import pack_activation
 from rocm_qlora.lora import adapter_bank
+from rocm_qlora.mx4.packed import PackedMx4
 from rocm_qlora.quantization.quant_linear import QuantLinear
 from rocm_qlora.quantization import layer_ops
 
@@ -74,9 +75,11 @@ class LoRALinear(nn.Module):
                 return layer_ops.LoRAQuantFunction.apply(x, self.lora_A, self.lora_B, xd, b.weight_view(), b.bias,
                                                          self.scaling)
             return layer_ops.lora_forward(x, self.lora_A, self.lora_B, xd, b.weight_view(), b.bias, self.scaling)
-        # any other base module: the reference's composition, unchanged
-        if hasattr(self.base_layer, 'weight'):
-            base_out = self.base_layer(x.to(self.base_layer.weight.dtype))
+        # any other base module: the reference's composition (4-bit values that were
+        # packed from 32 bits are multiplied with 16-bit activations of either type)
+        weight = getattr(self.base_layer, 'weight', None)
+        if weight is not None and not (isinstance(weight, PackedMx4) and weight.dtype == torch.float32):
+            base_out = self.base_layer(x.to(weight.dtype))
         else:
             base_out = self.base_layer(x)
         lora_out = self.lora_dropout(x) @ self.lora_A.to(x.dtype).T @ self.lora_B.to(x.dtype).T * self.scaling
@@ -89,6 +92,8 @@ class LoRALinear(nn.Module):
         if self.merged:
             raise RuntimeError("LoRA already merged")
         b = self.base_layer
+        if not hasattr(b, "dequantized_weight"):
+            raise TypeError(f"merge_lora needs a QuantLinear base, got {type(b).__name__}")
         if isinstance(b, QuantLinear) and b.weight_quant.is_cuda:
             # dequantize, B @ A * scaling and the fp32 add in one pass over the codes
             merged_weight = layer_ops.merge_weight(b.weight_view(), self.lora_A, self.lora_B, self.scaling,
