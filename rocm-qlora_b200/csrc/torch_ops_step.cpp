@@ -163,6 +163,8 @@ Tensor unpack_mx4(const Tensor& codes, const Tensor& scales, at::IntArrayRef sha
   check_float(dtype);
   check_gpu({&codes, &scales});
   TORCH_CHECK_VALUE(!shape.empty(), "unpack_mx4 needs at least one dimension");
+  TORCH_CHECK_VALUE(codes.dim() == 2 && c10::multiply_integers(shape.slice(0, shape.size() - 1)) == codes.size(0),
+                    "shape ", shape, " does not have the rows of codes ", codes.sizes());
   Tensor out = RQ_VIA(mx4_unpack, codes, scales, shape.back(), dtype);
   return shape.size() == 2 ? out : out.view(shape);
 }

@@ -63,3 +63,15 @@ def test_the_limit_of_a_wait_takes_any_number():
     L = nat.load_library()
     for ns in (0, 1, 2 ** 62, -2 ** 63, -1):
         assert L.rq_mx4_set_wait(ns) == 0
+
+
+def test_unpacking_into_another_number_of_rows_is_refused():
+    from rocm_qlora import _native as nat
+    from tests.test_mx4 import meta
+    ops, (codes, scales) = nat.loaded_ops(), meta(6, 160)
+    assert ops.unpack_mx4(codes, scales, [2, 3, 160], BF).shape == (2, 3, 160)
+    for shape in ([5, 160], [7, 160], [2, 2, 160], [160]):
+        with pytest.raises(ValueError, match="rows"):
+            ops.unpack_mx4(codes, scales, shape, BF)
+    one = meta(1, 160)
+    assert ops.unpack_mx4(*one, [160], BF).shape == (160,)
