@@ -452,7 +452,8 @@ RQ_API int rq_mx4_linear(const void* x, int dtype, int64_t ld_x, int64_t M,
 /* How long a product of few tokens (rq_mx4_matmul, rq_mx4_linear) waits for its
  * own copies and sums before it gives up, in ns: 2 s unless set; 0: every wait has
  * run out before it begins; below 0: 2 s again.  Outputs whose sums a wait ran out
- * for are NaN, and rq_take_kernel_timeouts counts it. */
+ * for are NaN, and rq_take_kernel_timeouts counts it.  A captured call keeps the
+ * limit of its capture. */
 RQ_API int rq_mx4_set_wait(int64_t ns);
 
 /* dx [M, K] (contiguous) = dy [M, N] . w, w the packed weight [N, K] and dy in

@@ -25,8 +25,8 @@
 //
 // With 32-bit moments a step is bound by memory (40 M values in fp32, 448 tensors,
 // clipped, 32 bytes a value: 208 us, 6.1 TB/s), with 8-bit ones by issue slots
-// and memory (160 M values in bf16, 448 tensors, clipped, 12 bytes a value: 380 us,
-// 5.0 TB/s; 202 M with remainders, 14 bytes: 496 us, 5.7 TB/s).
+// and memory (160 M values in bf16, 448 tensors, clipped, 12 bytes a value: 379 us,
+// 5.1 TB/s; 202 M with remainders, 14 bytes: 498 us, 5.7 TB/s).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -444,7 +444,7 @@ __device__ __forceinline__ float2 update(float2 g, float2& m, float2& v, float2 
   // rounding leaves: next to the step's ten roundings that makes 14 of 2^-24 at worst,
   // for a parameter that begins at 0 too.  Correctly rounded ones make a small step 30 %
   // longer (one projection's adapters 5.2 us and 6.7) and one with 8-bit moments 11 %
-  // (160 M values in bf16 380 us and 421).  The divisor is at least eps or 2^-75.
+  // (160 M values in bf16 379 us and 421).  The divisor is at least eps or 2^-75.
   const float2 d = fma2(r, f.y, make_float2(a.eps, a.eps));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(d.y));
@@ -518,7 +518,7 @@ __device__ __forceinline__ void update8(const In<DT, EIGHT, LOW>& d, void* p, in
 }
 
 // CTAs an SM.  Four would leave 64 registers a thread, too few for the next block's
-// inputs (8 bits, 202 M values with remainders: 496 us with three, 541 with four).
+// inputs (8 bits, 202 M values with remainders: 498 us with three, 541 with four).
 constexpr int kAdResident = 3;
 
 template <int DT, bool EIGHT, bool LOW, int MAX>
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kAdThreads, kAdResident) adam_update_k(const _
       const uint32_t whole = min(end, next - (t.tail[i] != kAdBlock));
       int64_t at = (int64_t)in * kAdBlock + lane * 8, block = (int64_t)t.block[i] + in;
       // with 8-bit moments the next block is on its way while this one is computed
-      // (160 M values in bf16 419 us without, 380 with)
+      // (160 M values in bf16 419 us without, 379 with)
       In<DT, EIGHT, LOW> d;
       if (EIGHT && b < whole) fetch<DT, true, EIGHT, LOW>(d, p, g, at, 8, block, lane, a);
 #pragma unroll 1

@@ -25,8 +25,9 @@
 // multiplications take that and the scale in.  A word's 8 codes come out as
 // (0, 4), (1, 5), (2, 6), (3, 7); they are stored so, and the epilogue puts the
 // columns right.
-// Bound by the tensor cores, whose pipe is 68 % active: 8192 x 11008 -> 4096 in
-// bf16 takes 522 us, 1415 TFLOP/s, and reads 231 MB (operands 204).
+// Bound by the tensor cores, whose pipe is 67 % active: dy 8192 x 11008 to dx 8192 x
+// 4096 in bf16 takes 533 us, 1386 TFLOP/s, and reads 235 MB (operands 204); once the
+// power limit is reached 580 to 600.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -60,9 +61,9 @@ template <int DT, int BN>
 struct Plan {
   // Teams of 8 widening warps that take the stages in turn.  Two hide the waits
   // and fences between stages, but take issue slots and shared memory from each
-  // other: 8192 x 11008 -> 4096 in bf16 630 us with one and 600 with two (tiles
-  // in another order than now), 4096 x 4096 -> 4096 135 and 116; 2047 x 4096 -> 11008 in fp16 (whose widening is
-  // shorter) 147 and 155, 512 x 4096 -> 4096 (128 columns) 26 and 29.
+  // other: dy 8192 x 11008 to 4096 columns in bf16 613 us with one and 531 with two,
+  // 4096 x 4096 to 4096 140 and 119; 2047 x 4096 to 11008 in fp16 (whose widening is
+  // shorter) 149 and 157, 512 x 4096 to 4096 (tiles of 128 columns) 26.7 and 28.7.
   static constexpr int kTeams = DT == RQ_BF16 && BN == 256 ? 2 : 1;
   static constexpr int kEpi0 = 2 + kTeams * kWiden;      // first epilogue warp
   static constexpr int kThreads = 32 * (kEpi0 + kEpi);
@@ -332,8 +333,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
           // of the peer's, whose values its MMAs read too.  A signal is a copy in the
           // proxy that the values were just made visible to, and its completion is
           // ordered for the cluster.  An arrival from the other CTA would need a release
-          // at cluster scope, which waits for everything remote (8192 x 4096 ->
-          // 11008 641 us with that, 534 with signals; 4096 -> 4096 of one token 43 and 25).
+          // at cluster scope, which waits for everything remote (dy 8192 x 11008 641
+          // us with that, 533 with signals; one token's 4096 to 4096 43 and 25).
           if (rank == 0) mbar_expect_tx(wide0 + 8 * slot, 16);
           else bulk_signal(sig_lead, smem_u32(sig_src), wide + 8 * slot);
           // Only now: the values have been used, so the loads of the codes are over.

@@ -17,15 +17,15 @@
 //                outputs in turn (2-SM MMAs; a CTA loads its 128 tokens and half
 //                of the outputs).  The epilogue empties the accumulator into
 //                registers, and the next tile's MMAs run while it stores.  Bound
-//                by the tensor cores: 8192 x 4096 -> 11008 in bf16 takes 143 us,
-//                5.1 PFLOP/s (MMA pipe 67 % active; 4096 x 4096 -> 4096, whose
+//                by the tensor cores: 8192 x 4096 -> 11008 in bf16 takes 145 us,
+//                5.1 PFLOP/s (MMA pipe 66 % active; 4096 x 4096 -> 4096, whose
 //                3.5 rounds of tiles take four, 32 us).
 //   mx4_split_k  few tiles.  P are outputs, Q up to 128 tokens, and a cluster
 //                splits the columns: each CTA parks its sums in shared memory,
 //                and all add up a share in rank order (fixed order: deterministic).
-//                Bound by latency: 64 x 4096 -> 11008 takes 11.4 us, 3.4 of
+//                Bound by latency: 64 x 4096 -> 11008 takes 11.0 us, 3.4 of
 //                them the weight's bytes at the copy bandwidth; one token x
-//                4096 -> 4096 6.2.
+//                4096 -> 4096 6.3.
 // Waits are bounded: one that runs out counts a kernel timeout, the CTAs drain
 // their copies, and mx4_pair_k stores nothing more, mx4_split_k NaNs (other CTAs
 // of the cluster add up what this one should have had).
@@ -375,7 +375,7 @@ namespace pair {
 // to tensor memory, from registers: as copies (tcgen05.cp) between the MMAs a
 // stage's 12 pieces cost the pipe about 960 cycles more, since one copy at a time
 // overlaps an MMA (8192 x 4096 -> 11008: 214 us with copies, 188 with stores,
-// both with stages of 256 columns; 146 with stages of 512).
+// both with stages of 256 columns; 145 with stages of 512).
 constexpr int S = 3;
 constexpr uint32_t kCodes = 128 * 128;                      // 256 columns of P's or of half of Q's rows
 constexpr uint32_t kStage = 4 * kCodes;                     // P's two, Q's two
@@ -563,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
       const int p0 = t % pt * 256 + (int)rank * 128 + quad * 32, q0 = t / pt * 256 + half * 128;
       // 128 outputs' bias in this warp's staging, while it waits: as shuffles of a lane's
       // values they held up the next tile's MMAs (8192 x 4096 -> 11008 with bias 164 us,
-      // now 152; without 147)
+      // now 150; without 145)
       if (g.bias) {
 #pragma unroll
         for (int j = 0; j < 128; j += 32) {
@@ -693,9 +693,9 @@ int code_map(const Mx4& x, int64_t pitch, uint32_t rows, CUtensorMap* map) {
 
 // Few tokens: the columns are split until two CTAs an SM have work, with at least
 // two stages each of 16 or 32 tokens, four of 64, eight of 128: more sums to add
-// up cost more than they save (1111 x 1093 -> 1089, 5 stages of 128 tokens: 7.6
-// us whole and 9.3 in halves; 64 x 4096 -> 11008, 16 stages: 12.4 whole, 11.2 in
-// thirds; 16 tokens 11.5 and 9.3).
+// up cost more than they save (1111 x 1093 -> 1089, 5 stages of 128 tokens: 7.8
+// us whole and 8.7 in halves; 64 x 4096 -> 11008, 16 stages: 12.6 whole, 11.0 in
+// thirds; 16 tokens 11.7 and 9.5).
 int split_for(int64_t tiles, int64_t steps, int bn) {
   const int64_t room = 2 * num_sms() / tiles, most = steps / (bn <= 32 ? 2 : bn / 16);
   const int64_t sk = room < most ? room : most;
@@ -780,10 +780,11 @@ int mx4_matmul(const Mx4& a, const Mx4& b, int64_t K, const void* bias, void* ou
   return dt == RQ_BF16 ? matmul_t<RQ_BF16>(a, b, K, bias, out, false, st) : matmul_t<RQ_F16>(a, b, K, bias, out, false, st);
 }
 
-// Up to 8 tokens are packed by the product's own CTAs (4096 -> 11008: one token 9.3
-// us where the packing in a launch of its own makes 10.8, 8 tokens 11.7 and 11.2,
-// but a call takes 6.5 us of the host's time instead of 9.5), unless a row is so
-// long that a CTA's share does not fit its shared memory.
+// Up to 8 tokens are packed by the product's own CTAs, unless a row is so long that
+// a CTA's share does not fit its shared memory.  4096 -> 11008: one token 9.4 us where
+// the packing in a launch of its own makes 10.9; 8 tokens 11.7 and 11.1, but a call
+// takes 6.7 us of the host's time instead of 10.4, which is what an eager step of few
+// tokens waits for (captured, 8 tokens are 0.6 us better off with two launches).
 constexpr int64_t kPackRows = 8, kPackColumns = 12800;  // 50 stages
 static bool packs(int64_t M, int64_t K) { return M <= kPackRows && K <= kPackColumns; }
 
