@@ -256,7 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Plan<DT, BN>::kThrea
       bool ok = true;
       for (int t = 0, i = 0; t < tiles && ok; ++t) {
         const uint32_t d = tmem + (uint32_t)(t & 1) * BN;
-        if (t >= 2 && !wait_pair(taken0 + 8 * (t & 1), ((t >> 1) - 1) & 1, ab)) break;
+        if (t >= 2 && !wait_pair<true>(taken0 + 8 * (t & 1), ((t >> 1) - 1) & 1, ab)) break;
         for (int st = 0; st < steps; ++st, ++i) {
           const int slot = i % S;
           ok = wait_pair(dy0 + 8 * slot, (i / S) & 1, ab) && wait_pair<true>(wide0 + 8 * slot, (i / S) & 1, ab);

@@ -481,10 +481,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1) m
       int i = 0, done = 0;  // stages, tiles
       bool ok = true;
       for (int t = first; t < ntile && ok; t += stride, ++done) {
-        if (done > 0 && !wait_pair(taken, (done - 1) & 1, ab)) break;
+        if (done > 0 && !wait_pair<true>(taken, (done - 1) & 1, ab)) break;
         for (int st = 0; st < steps; ++st, ++i) {
           const int slot = i % S;
-          if (!wait_pair(full0 + 8 * slot, (i / S) & 1, ab)) {
+          if (!wait_pair<true>(full0 + 8 * slot, (i / S) & 1, ab)) {
             ok = false;
             break;
           }

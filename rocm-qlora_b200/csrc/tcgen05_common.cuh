@@ -210,6 +210,8 @@ struct PairAbort {
   unsigned int* count;
   __device__ __forceinline__ bool raised() const { return *mine != 0; }
 };
+// kCluster: for arrivals of the other CTA's threads (as fast: 8192 x 4096 -> 11008 in 4
+// bits 148 us both ways).
 template <bool kCluster = false>
 __device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, const PairAbort& ab) {
   if (mbar_try<kCluster>(bar, parity)) return true;
